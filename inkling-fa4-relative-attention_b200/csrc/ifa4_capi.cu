@@ -129,20 +129,41 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+template <class Fn>
+cudaError_t driver_fn(const char* name, Fn* fn) {
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  cudaError_t err = cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q);
+  if (err == cudaSuccess && q != cudaDriverEntryPointSuccess) err = cudaErrorNotSupported;
+  *fn = reinterpret_cast<Fn>(p);
+  return err;
+}
+
+// cuTensorMapEncodeTiled, with a context current on the calling thread.  Runtime calls bind one
+// when they need it, the encoder does not: on a thread that has made no such call yet (a worker of
+// torch's autograd engine, a fresh host thread) it fails with "invalid context", so the device's
+// primary context is bound first.  A context the caller has made current stays.
 int get_encode_fn(EncodeTiledFn* fn) {
+  typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
   static EncodeTiledFn cached = nullptr;
+  static CtxGetCurrentFn get_current = nullptr;
   static std::once_flag once;
   static cudaError_t err = cudaSuccess;
   std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-    if (err == cudaSuccess && q != cudaDriverEntryPointSuccess) err = cudaErrorNotSupported;
-    cached = reinterpret_cast<EncodeTiledFn>(p);
+    err = driver_fn("cuTensorMapEncodeTiled", &cached);
+    if (err == cudaSuccess) err = driver_fn("cuCtxGetCurrent", &get_current);
   });
-  if (err != cudaSuccess || cached == nullptr)
+  if (err != cudaSuccess || cached == nullptr || get_current == nullptr)
     return cuda_fail(err == cudaSuccess ? cudaErrorNotSupported : err,
                      "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
+  CUcontext ctx = nullptr;
+  if (get_current(&ctx) != CUDA_SUCCESS || ctx == nullptr) {
+    int dev;
+    int rc = current_device(&dev);
+    if (rc) return rc;
+    cudaError_t e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaSetDevice");
+  }
   *fn = cached;
   return IFA4_OK;
 }
