@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define IFA4_ABI_VERSION 7
+#define IFA4_ABI_VERSION 8
 
 enum {
   IFA4_OK = 0,
@@ -322,6 +322,207 @@ typedef struct IFA4RelLogitsParams {
 } IFA4RelLogitsParams;
 
 int ifa4_rel_logits_launch(const IFA4RelLogitsParams* params, void* stream);
+
+/* Decode for a batch whose sequences share their first keys (ABI version 8; not in the reference,
+ * whose decode reads every sequence's keys).  Same result as ifa4_decode_launch with
+ * IFA4_ALIGN_BOTTOM_RIGHT on the same parameters, but the K/V of the first shared_prefix_len
+ * keys are read once for the batch instead of once per sequence.
+ * decode.block_table is required (a paged cache), causal_align must be IFA4_ALIGN_BOTTOM_RIGHT,
+ * row b of q / rel / out belongs to sequence b (total_q = batch, cu_seqlens_q = 0..batch), and
+ * n_heads / kv_heads <= 128.  All sequences of at least shared_prefix_len keys must hold the same
+ * keys and values there (normally the same pages; the pages are taken from the table row of one
+ * of them); shorter ones are attended whole through their own table rows.
+ * decode.num_splits / chunk_len plan the keys behind the prefix; decode.max_seqlen_k is the
+ * longest whole sequence, prefix included.  Deterministic: no atomics on results. */
+typedef struct IFA4SharedPrefixParams {
+  IFA4DecodeParams decode;
+  int32_t shared_prefix_len;  /* >= 0; 0 is a plain decode                                 */
+  int32_t prefix_splits;      /* CTAs that share a row tile's prefix keys; 0 = automatic   */
+} IFA4SharedPrefixParams;
+
+int ifa4_decode_shared_prefix_workspace_size(const IFA4SharedPrefixParams* params,
+                                             size_t* bytes_out);
+int ifa4_decode_shared_prefix_launch(const IFA4SharedPrefixParams* params, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+enum { IFA4_WEIGHT_BF16 = 0, IFA4_WEIGHT_F32 = 1 };
+
+/* Norm and rotation of the query and key heads in front of the attention (ABI version 8; the
+ * reference repository has these steps only in its diagram, outputs/architecture.md:18-64):
+ *   y   = x * rsqrt(mean_i x_i^2 + eps) * w        per token and head, when normalize is set
+ *   out = y with the pairs of its first rotary_dim dims turned by pos * inv_freq_i
+ * in fp32 with one rounding to bf16.  The pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * interleaved.  pos is the token's position in its sequence as in IFA4RelLogitsParams (queries
+ * and keys are the last len_q of len_k positions; cu_seqlens_q NULL: one sequence from 0); the
+ * angle is exact for any position.
+ * q, k [total_q, heads, 128] (slices of a merged projection qualify), q_out, k_out alike; in
+ * place (the same address and strides) is allowed.  Rows behind the last sequence are zeroed
+ * with zero_padding, else left as they were.  All rows 16-byte aligned with strides that are
+ * multiples of 8 elements; n_heads or kv_heads may be 0. */
+typedef struct IFA4QkNormRopeParams {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* q_weight;         /* [128], weight_dtype; NULL: ones                        */
+  const void* k_weight;
+  const void* inv_freq;         /* [rotary_dim / 2] fp64, or fp32 with inv_freq_f32       */
+  const int32_t* cu_seqlens_q;  /* optional, int32 [batch + 1] on the device              */
+  const int32_t* cu_seqlens_k;  /* optional, needs cu_seqlens_q                           */
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_t, k_stride_h;
+  int64_t q_out_stride_t, q_out_stride_h;
+  int64_t k_out_stride_t, k_out_stride_h;
+  int64_t total_q;
+  int32_t batch;
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t head_dim;             /* 128                                                    */
+  int32_t rotary_dim;           /* 0 (no rotation) or a multiple of 16 up to 128          */
+  int32_t interleaved;
+  int32_t normalize;
+  int32_t weight_dtype;         /* IFA4_WEIGHT_*                                          */
+  int32_t inv_freq_f32;
+  int32_t zero_padding;
+  int32_t dtype;
+  float eps;                    /* >= 0                                                   */
+} IFA4QkNormRopeParams;
+
+int ifa4_qk_norm_rope_launch(const IFA4QkNormRopeParams* params, void* stream);
+
+/* Gradients of ifa4_qk_norm_rope_launch: with g = R^T dout, r = rsqrt(mean x^2 + eps) and
+ * xhat = x r, dx = r (g w - xhat mean(g w xhat)) and dw = sum over tokens and heads of g xhat
+ * (fp32 sums in a fixed order).  dq_out / dk_out are the gradients of q_out / k_out; dq / dk are
+ * written in full (rows behind the last sequence get 0, and count in no sum).  dq_weight /
+ * dk_weight [128] of weight_dtype, or NULL when not wanted; they need normalize and the workspace. */
+typedef struct IFA4QkNormRopeBackwardParams {
+  const void* dq_out;
+  const void* dk_out;
+  const void* q;
+  const void* k;
+  void* dq;
+  void* dk;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq_weight;
+  void* dk_weight;
+  const void* inv_freq;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_k;
+  int64_t dq_out_stride_t, dq_out_stride_h;
+  int64_t dk_out_stride_t, dk_out_stride_h;
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_t, k_stride_h;
+  int64_t dq_stride_t, dq_stride_h;
+  int64_t dk_stride_t, dk_stride_h;
+  int64_t total_q;
+  int32_t batch;
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t normalize;
+  int32_t weight_dtype;
+  int32_t inv_freq_f32;
+  int32_t dtype;
+  float eps;
+} IFA4QkNormRopeBackwardParams;
+
+int ifa4_qk_norm_rope_backward_workspace_size(const IFA4QkNormRopeBackwardParams* params,
+                                              size_t* bytes_out);
+int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* params, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Append of new tokens to the paged cache the attention reads (ABI version 8; the reference's
+ * diagram has the cache update, outputs/architecture.md:117-120, and no code).  The tokens of
+ * sequence b, rows cu_seqlens_q[b] .. of k and v, are its last len_q keys (positions as above, the
+ * key counts cu_seqlens_k include them): position p goes to page block_table[b, p / page_size],
+ * slot p % page_size.  k rows are normalised and rotated as in IFA4QkNormRopeParams, v rows are
+ * copied, and q rows (optional, n_heads = 0 without) are normalised and rotated into q_out in
+ * the same launch.  A position below 0 or past the table, and a table entry outside
+ * [0, num_pages), writes nothing.  Nothing else in the caches is touched. */
+typedef struct IFA4KvAppendParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_cache;                /* [num_pages, page_size, kv_heads, 128]                  */
+  void* v_cache;
+  const void* q_weight;
+  const void* k_weight;
+  const void* inv_freq;
+  const int32_t* cu_seqlens_q;
+  const int32_t* cu_seqlens_k;
+  const int32_t* block_table;
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+  int64_t q_out_stride_t, q_out_stride_h;
+  int64_t k_stride_page, k_cache_stride_t, k_cache_stride_h;
+  int64_t v_stride_page, v_cache_stride_t, v_cache_stride_h;
+  int64_t block_table_stride;
+  int64_t total_q;
+  int32_t batch;
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t interleaved;
+  int32_t normalize;
+  int32_t weight_dtype;
+  int32_t inv_freq_f32;
+  int32_t zero_padding;
+  int32_t dtype;
+  int32_t page_size;            /* a power of two >= 16                                   */
+  int32_t num_pages;
+  int32_t table_width;          /* entries of a table row                                 */
+  float eps;
+} IFA4KvAppendParams;
+
+int ifa4_kv_append_launch(const IFA4KvAppendParams* params, void* stream);
+
+/* Learned relative position bias by distance buckets (ABI version 8; not in the reference, whose
+ * bias comes from a projection): rel[h, d] = table[bucket(d), h] for 0 <= d < rel_extent, where
+ * bucket(d) is the last b with starts[b] <= d (ascending starts; bucket 0 if there is none).  The
+ * attention reads the result as rel_logits with token stride 0.
+ * The gradient adds drel [total_q, n_heads, >= rel_extent] bf16 (token stride 0 allowed) over the
+ * tokens before cu_seqlens_q[batch] (all of them when it is NULL) and each bucket's distances:
+ * fp32 sums in a fixed order, written in full. */
+typedef struct IFA4BucketBiasParams {
+  const void* table;            /* [buckets, n_heads] of weight_dtype                     */
+  const int32_t* starts;        /* [buckets] on the device                                */
+  void* rel;                    /* [n_heads, rel_extent] bf16                             */
+  int64_t table_stride_b, table_stride_h;
+  int64_t rel_stride_h;
+  int32_t n_heads;
+  int32_t rel_extent;
+  int32_t buckets;              /* 1 .. IFA4_MAX_BUCKETS                                  */
+  int32_t weight_dtype;
+} IFA4BucketBiasParams;
+
+typedef struct IFA4BucketBiasBackwardParams {
+  const void* drel;
+  const int32_t* starts;
+  const int32_t* cu_seqlens_q;  /* optional                                               */
+  void* dtable;                 /* [buckets, n_heads] of weight_dtype                     */
+  int64_t drel_stride_t, drel_stride_h;
+  int64_t dtable_stride_b, dtable_stride_h;
+  int64_t total_q;
+  int32_t batch;
+  int32_t n_heads;
+  int32_t rel_extent;
+  int32_t buckets;
+  int32_t weight_dtype;
+} IFA4BucketBiasBackwardParams;
+
+#define IFA4_MAX_BUCKETS 1024
+
+int ifa4_bucket_bias_launch(const IFA4BucketBiasParams* params, void* stream);
+int ifa4_bucket_bias_backward_workspace_size(const IFA4BucketBiasBackwardParams* params,
+                                             size_t* bytes_out);
+int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* params, void* workspace,
+                                     size_t workspace_bytes, void* stream);
 
 /* Self-test of the failure detection (test hook; the reference has no counterpart): launches
  * on `stream` a kernel whose barrier wait can never complete, so the kernels' bounded-wait path

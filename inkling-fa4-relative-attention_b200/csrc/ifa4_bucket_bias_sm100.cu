@@ -1,0 +1,244 @@
+// Learned relative position bias by distance buckets for sm_100a, and its gradient.
+//   rel[h, d]    = table[bucket(d), h]                               0 <= d < rel_extent
+//   grad[b, h]   = sum over tokens t and distances d of bucket b of drel[t, h, d]
+// bucket(d) is the last bucket whose start is <= d (ascending starts; bucket 0 also takes what
+// lies before its start).
+//
+// The forward writes one [n_heads, rel_extent] table, which the attention reads with token
+// stride 0.  The gradient is one read of drel (HBM bound): a thread owns V neighbouring columns
+// of one head and adds its tokens in registers (fp32, eight loads in flight), a block adds its
+// token lanes and then its columns by bucket in a fixed order and writes one partial per head and
+// bucket; a second kernel adds the blocks' partials in a fixed order (no atomics).  With a single
+// token chunk the first kernel writes the result itself.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ifa4_internal.h"
+#include "ifa4_ptx.cuh"
+
+namespace ifa4 {
+namespace bucket {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ void store_as(void* dst, long long i, float v, int f32) {
+  if (f32) {
+    static_cast<float*>(dst)[i] = v;
+  } else {
+    __nv_bfloat16 b = __float2bfloat16_rn(v);
+    static_cast<uint16_t*>(dst)[i] = *reinterpret_cast<uint16_t*>(&b);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) bucket_bias_kernel(const __grid_constant__
+                                                                   BucketBiasKernelArgs a) {
+  __shared__ int starts[kMaxBuckets];
+  for (int i = threadIdx.x; i < a.buckets; i += kThreads) starts[i] = __ldg(a.starts + i);
+  __syncthreads();
+  const int d = blockIdx.x * kThreads + threadIdx.x;
+  const int h = blockIdx.y;
+  if (d >= a.rel_extent) return;
+  int lo = 0, hi = a.buckets - 1;  // last bucket with starts[b] <= d, bucket 0 if none
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (starts[mid] <= d) lo = mid; else hi = mid - 1;
+  }
+  const long long i = lo * a.table_sb + h * a.table_sh;
+  const float v = a.table_f32 ? __ldg(static_cast<const float*>(a.table) + i)
+                              : bf16_bits_to_float(__ldg(static_cast<const uint16_t*>(a.table) + i));
+  __nv_bfloat16 b = __float2bfloat16_rn(v);
+  a.rel[h * a.rel_sh + d] = *reinterpret_cast<uint16_t*>(&b);
+}
+
+template <int V>
+struct Vec;
+template <>
+struct Vec<8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const uint16_t* p) { v = ldg_nc_v4(p); }
+  __device__ __forceinline__ void add(float (&s)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[2 * i] += __uint_as_float(w[i] << 16);
+      s[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <>
+struct Vec<2> {
+  uint32_t v;
+  __device__ __forceinline__ void load(const uint16_t* p) {
+    v = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+  __device__ __forceinline__ void add(float (&s)[2]) const {
+    s[0] += __uint_as_float(v << 16);
+    s[1] += __uint_as_float(v & 0xffff0000u);
+  }
+};
+template <>
+struct Vec<1> {
+  uint16_t v;
+  __device__ __forceinline__ void load(const uint16_t* p) { v = __ldg(p); }
+  __device__ __forceinline__ void add(float (&s)[1]) const { s[0] += bf16_bits_to_float(v); }
+};
+
+// Block (x, y): column block x = (head block, column part), token chunk y.  A block covers
+// a.heads heads x a.cols columns (columns of one head from a.cols * part on), a.lanes token lanes.
+template <int V>
+__global__ void __launch_bounds__(kThreads) bucket_grad_kernel(const __grid_constant__
+                                                                   BucketGradKernelArgs a) {
+  __shared__ float sums[kThreads * V];      // [lane][head][column]
+  __shared__ int starts[kMaxBuckets + 1];
+  for (int i = threadIdx.x; i <= a.buckets; i += kThreads)
+    starts[i] = i == 0 ? 0 : (i == a.buckets ? a.rel_extent
+                                              : min(max(__ldg(a.starts + i), 0), a.rel_extent));
+  const int part = blockIdx.x % a.col_parts;
+  const int h0 = (blockIdx.x / a.col_parts) * a.heads;
+  const int e0 = part * a.cols;
+  const int n_cols = min(a.cols, a.rel_extent - e0);
+  const int vecs = a.cols / V;                 // threads of a head (the last part may use fewer)
+  const int per_lane = a.heads * vecs;         // threads of a token lane
+  const int lane = threadIdx.x / per_lane;
+  const int in_lane = threadIdx.x - lane * per_lane;
+  const int hl = in_lane / vecs;
+  const int c = (in_lane - hl * vecs) * V;
+  long long tokens = a.total_q;
+  if (a.cu_q != nullptr) tokens = min(tokens, static_cast<long long>(max(__ldg(a.cu_q + a.batch), 0)));
+  const long long t0 = blockIdx.y * a.chunk;
+  const long long t1 = min(tokens, t0 + a.chunk);
+  const bool on = lane < a.lanes && h0 + hl < a.n_heads && c < n_cols;
+  float s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = 0.f;
+  if (on) {
+    const long long step = static_cast<long long>(a.lanes) * a.drel_st;
+    long long t = t0 + lane;
+    const uint16_t* p = a.drel + t * a.drel_st + (h0 + hl) * a.drel_sh + e0 + c;
+    for (; t + 7 * a.lanes < t1; t += 8 * a.lanes) {
+      Vec<V> x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i].load(p + i * step);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i].add(s);
+      p += 8 * step;
+    }
+    for (; t < t1; t += a.lanes) {
+      Vec<V> x;
+      x.load(p);
+      x.add(s);
+      p += step;
+    }
+  }
+  if (lane < a.lanes) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[(lane * a.heads + hl) * a.cols + c + i] = s[i];
+  }
+  __syncthreads();
+  // columns: add the token lanes
+  const int width = a.heads * a.cols;
+  if (a.lanes > 1) {
+    for (int i = threadIdx.x; i < width; i += kThreads) {
+      float v = sums[i];
+      for (int k = 1; k < a.lanes; ++k) v += sums[k * width + i];
+      sums[i] = v;
+    }
+    __syncthreads();
+  }
+  // buckets: eight lanes per head and bucket
+  const int sub = threadIdx.x & 7;
+  const int tasks = a.heads * a.buckets;
+  for (int task0 = 0; task0 < tasks; task0 += kThreads / 8) {
+    const int task = task0 + (threadIdx.x >> 3);
+    const int th = task < tasks ? task / a.buckets : 0;
+    const int b = task - th * a.buckets;
+    float v = 0.f;
+    if (task < tasks) {
+      const int lo = max(starts[b] - e0, 0), hi = min(starts[b + 1] - e0, n_cols);
+      for (int i = lo + sub; i < hi; i += 8) v += sums[th * a.cols + i];
+    }
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 2);
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    if (sub == 0 && task < tasks && h0 + th < a.n_heads) {
+      if (a.slots == 1)
+        store_as(a.grad, b * a.grad_sb + (h0 + th) * a.grad_sh, v, a.grad_f32);
+      else
+        a.partial[((static_cast<long long>(blockIdx.y) * a.col_parts + part) * a.n_heads + h0 + th) *
+                      a.buckets + b] = v;
+    }
+  }
+}
+
+// grad[b, h] = sum over slots of partial[slot][h][b]; a block adds 32 neighbouring (h, b).
+__global__ void __launch_bounds__(1024) bucket_grad_sum_kernel(const __grid_constant__
+                                                                   BucketGradKernelArgs a) {
+  __shared__ float s[32][33];
+  const int n = a.n_heads * a.buckets;
+  const int i = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  float acc = 0.f;
+  if (i < n)
+    for (int k = row; k < a.slots; k += 32) acc += a.partial[static_cast<long long>(k) * n + i];
+  s[row][threadIdx.x & 31] = acc;
+  __syncthreads();
+  if (row == 0 && i < n) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v += s[k][threadIdx.x];
+    store_as(a.grad, (i % a.buckets) * a.grad_sb + (i / a.buckets) * a.grad_sh, v, a.grad_f32);
+  }
+}
+
+}  // namespace bucket
+
+cudaError_t launch_bucket_bias_sm100(const BucketBiasKernelArgs& args, cudaStream_t stream) {
+  const dim3 grid((args.rel_extent + bucket::kThreads - 1) / bucket::kThreads, args.n_heads);
+  bucket::bucket_bias_kernel<<<grid, bucket::kThreads, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+// Column blocks and token chunks of the gradient (fills heads, cols, col_parts, lanes, chunk,
+// slots of `a` from its sizes).  vec: columns a thread loads at once (8, 2 or 1).
+void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms) {
+  const int vecs = (a->rel_extent + vec - 1) / vec;  // vec divides rel_extent
+  const int head_vecs = vecs < bucket::kThreads ? vecs : bucket::kThreads;
+  a->cols = head_vecs * vec;
+  a->col_parts = (vecs + head_vecs - 1) / head_vecs;
+  int heads = bucket::kThreads / head_vecs;
+  if (heads > a->n_heads) heads = a->n_heads;
+  a->heads = heads;
+  a->lanes = bucket::kThreads / (heads * head_vecs);
+  const long long col_blocks =
+      static_cast<long long>((a->n_heads + heads - 1) / heads) * a->col_parts;
+  // enough chunks for eight blocks per SM, at least 16 tokens per lane
+  long long chunks = (8ll * sms + col_blocks - 1) / col_blocks;
+  const long long most = (a->total_q + 16ll * a->lanes - 1) / (16ll * a->lanes);
+  if (chunks > most) chunks = most;
+  if (chunks < 1) chunks = 1;
+  if (chunks > 65535) chunks = 65535;
+  a->chunk = (a->total_q + chunks - 1) / chunks;
+  if (a->chunk < 1) a->chunk = 1;  // no token: one block column writes the zeros
+  a->chunks = static_cast<int>((a->total_q + a->chunk - 1) / a->chunk);
+  if (a->chunks < 1) a->chunks = 1;
+  a->slots = a->chunks * a->col_parts;
+}
+
+cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
+                                     cudaStream_t stream) {
+  const dim3 grid((args.n_heads + args.heads - 1) / args.heads * args.col_parts, args.chunks);
+  if (vec == 8)
+    bucket::bucket_grad_kernel<8><<<grid, bucket::kThreads, 0, stream>>>(args);
+  else if (vec == 2)
+    bucket::bucket_grad_kernel<2><<<grid, bucket::kThreads, 0, stream>>>(args);
+  else
+    bucket::bucket_grad_kernel<1><<<grid, bucket::kThreads, 0, stream>>>(args);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || args.slots == 1) return e;
+  const int n = args.n_heads * args.buckets;
+  bucket::bucket_grad_sum_kernel<<<(n + 31) / 32, 1024, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+}  // namespace ifa4

@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/inkling_fa4.h"
@@ -168,16 +169,17 @@ int get_encode_fn(EncodeTiledFn* fn) {
   return IFA4_OK;
 }
 
-// [rows, heads, 128] bf16 with element strides (st, sh), boxes of 64 dims x 1 head x box_rows,
+// [rows, heads, 128] bf16 with element strides (st, sh), boxes of 64 dims x box_heads x box_rows,
 // 128-byte swizzle; out-of-range rows read as zero.
 int encode_rows_heads_dims(CUtensorMap* map, const void* base, int64_t rows, int64_t heads,
-                           int64_t st, int64_t sh, uint32_t box_rows, const char* name) {
+                           int64_t st, int64_t sh, uint32_t box_rows, const char* name,
+                           uint32_t box_heads = 1) {
   EncodeTiledFn fn;
   int rc = get_encode_fn(&fn);
   if (rc) return rc;
   cuuint64_t dims[3] = {128, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2};
-  cuuint32_t box[3] = {64, 1, box_rows};
+  cuuint32_t box[3] = {64, box_heads, box_rows};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -571,6 +573,39 @@ static int decode_plan(const IFA4DecodeParams* p, int* num_splits, int* chunk_le
   return IFA4_OK;
 }
 
+// Kernel arguments of a decode (without workspace and status).
+static ifa4::DecodeKernelArgs decode_args(const IFA4DecodeParams* p, int splits, int chunk) {
+  ifa4::DecodeKernelArgs a{};
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.rel = static_cast<const uint16_t*>(p->rel);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.cu_q = p->cu_seqlens_q;
+  a.cu_k = p->cu_seqlens_k;
+  a.q_st = p->q_stride_t;
+  a.q_sh = p->q_stride_h;
+  a.rel_st = p->rel_stride_t;
+  a.rel_sh = p->rel_stride_h;
+  a.out_st = p->out_stride_t;
+  a.out_sh = p->out_stride_h;
+  a.batch = p->batch;
+  a.n_heads = p->n_heads;
+  a.kv_heads = p->kv_heads;
+  a.rel_extent = p->rel_extent;
+  a.causal = p->causal ? 1 : 0;
+  a.window_left = p->window_left < 0 ? -1 : p->window_left;
+  a.align_bottom_right = p->causal_align == IFA4_ALIGN_BOTTOM_RIGHT;
+  a.group = p->n_heads / p->kv_heads;
+  a.heads_per_cta = a.group < 16 ? a.group : 16;
+  a.num_splits = splits;
+  a.chunk_len = chunk;
+  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  a.lse = p->lse;
+  a.lse_sh = p->lse_stride_h;
+  a.lse_st = p->lse_stride_t;
+  fill_paged(p, 64, &a);
+  return a;
+}
+
 int ifa4_decode_workspace_size(const IFA4DecodeParams* p, size_t* bytes_out,
                                int32_t* num_splits_out, int32_t* chunk_len_out) {
   g_last_error[0] = '\0';
@@ -609,39 +644,12 @@ int ifa4_decode_launch(const IFA4DecodeParams* p, void* workspace, size_t worksp
   int* status = nullptr;
   if ((rc = device_status_ptr(&status))) return rc;
 
-  ifa4::DecodeKernelArgs a{};
-  a.q = static_cast<const uint16_t*>(p->q);
-  a.rel = static_cast<const uint16_t*>(p->rel);
-  a.out = static_cast<uint16_t*>(p->out);
-  a.cu_q = p->cu_seqlens_q;
-  a.cu_k = p->cu_seqlens_k;
-  a.q_st = p->q_stride_t;
-  a.q_sh = p->q_stride_h;
-  a.rel_st = p->rel_stride_t;
-  a.rel_sh = p->rel_stride_h;
-  a.out_st = p->out_stride_t;
-  a.out_sh = p->out_stride_h;
-  a.batch = p->batch;
-  a.n_heads = p->n_heads;
-  a.kv_heads = p->kv_heads;
-  a.rel_extent = p->rel_extent;
-  a.causal = p->causal ? 1 : 0;
-  a.window_left = p->window_left < 0 ? -1 : p->window_left;
-  a.align_bottom_right = p->causal_align == IFA4_ALIGN_BOTTOM_RIGHT;
-  a.group = p->n_heads / p->kv_heads;
-  a.heads_per_cta = a.group < 16 ? a.group : 16;
-  a.num_splits = splits;
-  a.chunk_len = chunk;
-  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  ifa4::DecodeKernelArgs a = decode_args(p, splits, chunk);
   if (ws > 0) {
     const size_t parts = static_cast<size_t>(p->batch) * p->n_heads * splits;
     a.ws_o = static_cast<float*>(workspace);
     a.ws_lse = a.ws_o + parts * 128;
   }
-  a.lse = p->lse;
-  a.lse_sh = p->lse_stride_h;
-  a.lse_st = p->lse_stride_t;
-  fill_paged(p, 64, &a);
   a.status = status;
   CUtensorMap tk, tv;
   if ((rc = encode_kv(p, 64, &tk, &tv))) return rc;
@@ -877,6 +885,603 @@ int ifa4_backward_launch(const IFA4BackwardParams* p, void* workspace, size_t wo
                                               static_cast<int>(ks),
                                               static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "backward launch");
+  return IFA4_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------
+// Decode behind a shared prefix
+// ---------------------------------------------------------------------------------------
+namespace {
+struct SharedPrefixPlan {
+  IFA4DecodeParams own;   // the decode of the keys behind the prefix
+  int own_splits, chunk;
+  int seqs_per_tile, key_pair, splits, parts;
+  size_t bytes;           // workspace
+};
+
+int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) {
+  const char* what = "decode_shared_prefix";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  const IFA4DecodeParams* d = &p->decode;
+  int rc = validate_common(d, what);
+  if (rc) return rc;
+  if (p->shared_prefix_len < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: shared_prefix_len must be >= 0", what);
+  if (p->prefix_splits < 0 || p->prefix_splits > 1024)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: prefix_splits %d outside [0, 1024]", what,
+                p->prefix_splits);
+  if (d->block_table == nullptr && d->batch > 0 && d->total_q > 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: needs a paged cache (block_table is NULL)", what);
+  if (d->causal_align != IFA4_ALIGN_BOTTOM_RIGHT)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: causal_align must be bottom-right", what);
+  const int group = d->n_heads / d->kv_heads;
+  if (group > 128)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: more than 128 query heads per KV head", what);
+  *plan = SharedPrefixPlan{};
+  if (d->batch == 0 || d->total_q == 0) return IFA4_OK;
+  if (d->total_q != d->batch)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: expects exactly one query per sequence (total_q %lld != batch %d)", what,
+                static_cast<long long>(d->total_q), d->batch);
+  plan->own = *d;
+  if (p->shared_prefix_len > 0 && d->max_seqlen_k > 0)
+    plan->own.max_seqlen_k = d->max_seqlen_k > p->shared_prefix_len
+                                 ? d->max_seqlen_k - p->shared_prefix_len : 1;
+  size_t own_bytes = 0;
+  if ((rc = decode_plan(&plan->own, &plan->own_splits, &plan->chunk, &own_bytes))) return rc;
+  if (p->shared_prefix_len == 0) {
+    plan->bytes = own_bytes;
+    return IFA4_OK;
+  }
+  plan->seqs_per_tile = 128 / group;
+  const int tiles = (d->batch + plan->seqs_per_tile - 1) / plan->seqs_per_tile;
+  plan->key_pair = tiles == 1;
+  int sms = 148;
+  if ((rc = sm_count(&sms))) return rc;
+  const int64_t ctas = static_cast<int64_t>(d->kv_heads) * ((tiles + 1) / 2);
+  int64_t span = p->shared_prefix_len;
+  if (d->window_left >= 0 && d->window_left + 128LL < span) span = d->window_left + 128LL;
+  const int64_t key_tiles = (span + 127) / 128;
+  int splits = p->prefix_splits;
+  if (splits == 0) {
+    // the split count with the least work on the busiest SM: waves of CTAs x (key tiles of a
+    // CTA + about three tiles' worth of start and epilogue)
+    int64_t best = INT64_MAX;
+    const int64_t most = key_tiles < 64 ? key_tiles : 64;
+    for (int64_t s = 1; s <= most; ++s) {
+      const int64_t waves = (ctas * s + sms - 1) / sms;
+      const int64_t cost = waves * ((key_tiles + s - 1) / s + 3);
+      if (cost < best) {
+        best = cost;
+        splits = static_cast<int>(s);
+      }
+    }
+  }
+  plan->splits = splits;
+  plan->parts = plan->key_pair ? 2 * splits : splits;
+  plan->bytes = static_cast<size_t>(d->batch) * d->n_heads * (plan->parts + plan->own_splits) *
+                (128 + 1) * sizeof(float);
+  return IFA4_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int ifa4_decode_shared_prefix_workspace_size(const IFA4SharedPrefixParams* p, size_t* bytes_out) {
+  g_last_error[0] = '\0';
+  if (bytes_out == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "decode_shared_prefix: bytes_out is NULL");
+  SharedPrefixPlan plan;
+  int rc = shared_prefix_plan(p, &plan);
+  if (rc) return rc;
+  *bytes_out = plan.bytes;
+  return IFA4_OK;
+}
+
+int ifa4_decode_shared_prefix_launch(const IFA4SharedPrefixParams* p, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  g_last_error[0] = '\0';
+  SharedPrefixPlan plan;
+  int rc = shared_prefix_plan(p, &plan);
+  if (rc) return rc;
+  const IFA4DecodeParams* d = &p->decode;
+  if (d->batch == 0 || d->total_q == 0) return IFA4_OK;
+  if (p->shared_prefix_len == 0)
+    return ifa4_decode_launch(d, workspace, workspace_bytes, stream);
+  if (workspace == nullptr || workspace_bytes < plan.bytes)
+    return fail(IFA4_ERR_WORKSPACE, "decode_shared_prefix: workspace of %zu bytes required, got %zu",
+                plan.bytes, workspace_bytes);
+  if (!aligned16(workspace))
+    return fail(IFA4_ERR_WORKSPACE, "decode_shared_prefix: workspace must be 16-byte aligned");
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
+  const size_t rows = static_cast<size_t>(d->batch) * d->n_heads;
+
+  ifa4::SharedPrefixKernelArgs a{};
+  a.rel = static_cast<const uint16_t*>(d->rel);
+  a.rel_st = d->rel_stride_t;
+  a.rel_sh = d->rel_stride_h;
+  a.cu_k = d->cu_seqlens_k;
+  a.batch = d->batch;
+  a.n_heads = d->n_heads;
+  a.kv_heads = d->kv_heads;
+  a.rel_extent = d->rel_extent;
+  a.group = d->n_heads / d->kv_heads;
+  a.seqs_per_tile = plan.seqs_per_tile;
+  a.prefix_len = p->shared_prefix_len;
+  a.window_left = d->window_left < 0 ? -1 : d->window_left;
+  a.key_pair = plan.key_pair;
+  a.splits = plan.splits;
+  a.parts = plan.parts;
+  a.bias_vec = aligned16(d->rel) && d->rel_stride_t % 8 == 0 && d->rel_stride_h % 8 == 0 &&
+               d->rel_extent % 8 == 0;
+  a.scale_log2 = d->softmax_scale * 1.4426950408889634f;
+  fill_paged(d, 128, &a);
+  a.v = static_cast<const uint16_t*>(d->v);
+  a.v_st = d->v_stride_t;
+  a.v_sh = d->v_stride_h;
+  a.v_sp = d->v_stride_page;
+  float* ws = static_cast<float*>(workspace);
+  a.ws_o = ws;
+  float* own_o = ws + rows * plan.parts * 128;
+  a.ws_lse = own_o + rows * plan.own_splits * 128;
+  float* own_lse = a.ws_lse + rows * plan.parts;
+  a.own_o = own_o;
+  a.own_lse = own_lse;
+  a.own_parts = plan.own_splits;
+  a.out = static_cast<uint16_t*>(d->out);
+  a.out_st = d->out_stride_t;
+  a.out_sh = d->out_stride_h;
+  a.lse = d->lse;
+  a.lse_sh = d->lse_stride_h;
+  a.lse_st = d->lse_stride_t;
+  a.status = status;
+
+  ifa4::DecodeKernelArgs o = decode_args(&plan.own, plan.own_splits, plan.chunk);
+  o.prefix_len = p->shared_prefix_len;
+  o.ws_o = own_o;
+  o.ws_lse = own_lse;
+  o.status = status;
+
+  CUtensorMap tq, tk, tv, tk64, tv64;
+  if ((rc = encode_rows_heads_dims(&tq, d->q, d->total_q, d->n_heads, d->q_stride_t,
+                                   d->q_stride_h, plan.seqs_per_tile, "q", a.group)))
+    return rc;
+  if ((rc = encode_kv(d, 128, &tk, &tv))) return rc;
+  if ((rc = encode_kv(d, 64, &tk64, &tv64))) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = ifa4::launch_shared_prefix_sm100(a, tq, tk, tv, s);
+  if (e != cudaSuccess) return cuda_fail(e, "decode_shared_prefix launch");
+  e = ifa4::launch_decode_sm100(o, tk64, tv64, s);
+  if (e != cudaSuccess) return cuda_fail(e, "decode_shared_prefix own keys launch");
+  e = ifa4::launch_shared_prefix_combine_sm100(a, s);
+  if (e != cudaSuccess) return cuda_fail(e, "decode_shared_prefix combine launch");
+  return IFA4_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------
+// Norm and rotation of q and k; append to the paged cache
+// ---------------------------------------------------------------------------------------
+namespace {
+// Row tensors [tokens, heads, 128]: 16-byte aligned, strides multiples of 8 elements.
+int check_rows(const char* what, const char* name, const void* p, int64_t st, int64_t sh,
+               bool written) {
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: %s is NULL", what, name);
+  if (!aligned16(p))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: %s must be 16-byte aligned", what, name);
+  if (st % 8 != 0 || sh % 8 != 0 || st < 0 || sh < 0 || (written && (st == 0 || sh == 0)))
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: %s token and head strides must be %s multiples of 8 elements", what, name,
+                written ? "positive" : "non-negative");
+  return IFA4_OK;
+}
+
+template <class P>
+int validate_norm_rope(const P* p, const char* what) {
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  if (p->dtype != IFA4_DTYPE_BF16)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: dtype %d unsupported (bf16 only)", what, p->dtype);
+  if (p->head_dim != ifa4::kHeadDim)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (128 only)", what, p->head_dim);
+  if (p->total_q < 0 || p->n_heads < 0 || p->kv_heads < 0 || p->n_heads > 65535 ||
+      p->kv_heads > 65535)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: bad total_q or head counts", what);
+  if (p->rotary_dim < 0 || p->rotary_dim > 128 || p->rotary_dim % 16 != 0)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: rotary_dim %d is not a multiple of 16 in [0, 128]",
+                what, p->rotary_dim);
+  if (p->rotary_dim > 0 &&
+      (p->inv_freq == nullptr ||
+       (reinterpret_cast<uintptr_t>(p->inv_freq) & (p->inv_freq_f32 ? 3u : 7u)) != 0))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: rotary_dim needs an aligned inv_freq", what);
+  if (p->weight_dtype != IFA4_WEIGHT_BF16 && p->weight_dtype != IFA4_WEIGHT_F32)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: weight_dtype %d unsupported", what, p->weight_dtype);
+  const unsigned wmask = p->weight_dtype == IFA4_WEIGHT_F32 ? 3u : 1u;
+  if (((reinterpret_cast<uintptr_t>(p->q_weight) | reinterpret_cast<uintptr_t>(p->k_weight)) &
+       wmask) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned weights", what);
+  if (!p->normalize && (p->q_weight != nullptr || p->k_weight != nullptr))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: weights without the norm", what);
+  if (p->normalize && !(p->eps >= 0.f && p->eps < 3.0e38f))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", what);
+  if (p->cu_seqlens_k != nullptr && p->cu_seqlens_q == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: cu_seqlens_k given without cu_seqlens_q", what);
+  if (p->cu_seqlens_q != nullptr && p->batch <= 0 && p->total_q > 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: batch must be > 0 with cu_seqlens_q", what);
+  if (p->total_q > (1LL << 40)) return fail(IFA4_ERR_UNSUPPORTED, "%s: total_q beyond 2^40", what);
+  return IFA4_OK;
+}
+
+// A token's rows are shared by several warps when there are few tokens: about 32 warps per SM in
+// all, two rows (a half-warp each) at least.
+int token_parts(int64_t tokens, int rows, int sms) {
+  const int64_t want = (32LL * sms + tokens - 1) / tokens;
+  const int most = (rows + 1) / 2;
+  return static_cast<int>(want < 1 ? 1 : (want > most ? most : want));
+}
+
+template <class P>
+void fill_qkv(const P* p, ifa4::QkvKernelArgs* a) {
+  a->q = static_cast<const uint16_t*>(p->q);
+  a->k = static_cast<const uint16_t*>(p->k);
+  a->q_out = static_cast<uint16_t*>(p->q_out);
+  a->q_weight = p->q_weight;
+  a->k_weight = p->k_weight;
+  a->inv_freq = p->inv_freq;
+  a->cu_q = p->cu_seqlens_q;
+  a->cu_k = p->cu_seqlens_k;
+  a->q_st = p->q_stride_t;
+  a->q_sh = p->q_stride_h;
+  a->k_st = p->k_stride_t;
+  a->k_sh = p->k_stride_h;
+  a->qo_st = p->q_out_stride_t;
+  a->qo_sh = p->q_out_stride_h;
+  a->batch = p->batch;
+  a->n_heads = p->n_heads;
+  a->kv_heads = p->kv_heads;
+  a->rotary_dim = p->rotary_dim;
+  a->interleaved = p->interleaved ? 1 : 0;
+  a->normalize = p->normalize ? 1 : 0;
+  a->weight_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
+  a->inv_freq_f32 = p->inv_freq_f32 ? 1 : 0;
+  a->zero_padding = p->zero_padding ? 1 : 0;
+  a->eps = p->eps;
+}
+
+int launch_qkv(const char* what, ifa4::QkvKernelArgs* a, int64_t tokens, int rows, void* stream) {
+  if (rows == 0) return IFA4_OK;
+  int sms = 148;
+  int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int parts = token_parts(tokens, rows, sms);
+  a->rows_per_part = (rows + parts - 1) / parts;
+  a->parts = (rows + a->rows_per_part - 1) / a->rows_per_part;
+  a->units = tokens * a->parts;
+  cudaError_t e = ifa4::launch_qkv_rows_sm100(*a, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return IFA4_OK;
+}
+
+int validate_qk_norm_rope_backward(const IFA4QkNormRopeBackwardParams* p) {
+  const char* what = "qk_norm_rope_backward";
+  int rc = validate_norm_rope(p, what);
+  if (rc) return rc;
+  if (!p->normalize && (p->dq_weight != nullptr || p->dk_weight != nullptr))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: weight gradients without the norm", what);
+  const unsigned wmask = p->weight_dtype == IFA4_WEIGHT_F32 ? 3u : 1u;
+  if (((reinterpret_cast<uintptr_t>(p->dq_weight) | reinterpret_cast<uintptr_t>(p->dk_weight)) &
+       wmask) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned weight gradients", what);
+  if (p->total_q == 0) return IFA4_OK;
+  if (p->n_heads > 0 &&
+      ((rc = check_rows(what, "dq_out", p->dq_out, p->dq_out_stride_t, p->dq_out_stride_h, false)) ||
+       (rc = check_rows(what, "q", p->q, p->q_stride_t, p->q_stride_h, false)) ||
+       (rc = check_rows(what, "dq", p->dq, p->dq_stride_t, p->dq_stride_h, true))))
+    return rc;
+  if (p->kv_heads > 0 &&
+      ((rc = check_rows(what, "dk_out", p->dk_out, p->dk_out_stride_t, p->dk_out_stride_h, false)) ||
+       (rc = check_rows(what, "k", p->k, p->k_stride_t, p->k_stride_h, false)) ||
+       (rc = check_rows(what, "dk", p->dk, p->dk_stride_t, p->dk_stride_h, true))))
+    return rc;
+  return IFA4_OK;
+}
+
+// Units, blocks and workspace of the backward.
+int plan_qk_backward(const IFA4QkNormRopeBackwardParams* p, int* parts, int* blocks,
+                     size_t* bytes) {
+  int sms = 148;
+  int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int rows = p->n_heads > p->kv_heads ? p->n_heads : p->kv_heads;
+  *parts = p->total_q > 0 && rows > 0 ? token_parts(p->total_q, rows, sms) : 1;
+  const int64_t want = (p->total_q * *parts + ifa4::kQkvBackwardWarps - 1) / ifa4::kQkvBackwardWarps;
+  const int64_t cap = static_cast<int64_t>(sms) * 6;  // one resident wave
+  *blocks = static_cast<int>(want < 1 ? 1 : (want < cap ? want : cap));
+  *bytes = p->dq_weight != nullptr || p->dk_weight != nullptr
+               ? static_cast<size_t>(*blocks) * 256 * sizeof(float) : 0;
+  return IFA4_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int ifa4_qk_norm_rope_launch(const IFA4QkNormRopeParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "qk_norm_rope";
+  int rc = validate_norm_rope(p, what);
+  if (rc) return rc;
+  if (p->total_q == 0) return IFA4_OK;
+  if (p->n_heads > 0 &&
+      ((rc = check_rows(what, "q", p->q, p->q_stride_t, p->q_stride_h, false)) ||
+       (rc = check_rows(what, "q_out", p->q_out, p->q_out_stride_t, p->q_out_stride_h, true))))
+    return rc;
+  if (p->kv_heads > 0 &&
+      ((rc = check_rows(what, "k", p->k, p->k_stride_t, p->k_stride_h, false)) ||
+       (rc = check_rows(what, "k_out", p->k_out, p->k_out_stride_t, p->k_out_stride_h, true))))
+    return rc;
+  ifa4::QkvKernelArgs a{};
+  fill_qkv(p, &a);
+  a.k_out = static_cast<uint16_t*>(p->k_out);
+  a.ko_st = p->k_out_stride_t;
+  a.ko_sh = p->k_out_stride_h;
+  return launch_qkv("qk_norm_rope launch", &a, p->total_q, p->n_heads + p->kv_heads, stream);
+}
+
+int ifa4_qk_norm_rope_backward_workspace_size(const IFA4QkNormRopeBackwardParams* p,
+                                              size_t* bytes_out) {
+  g_last_error[0] = '\0';
+  if (bytes_out == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "qk_norm_rope_backward: bytes_out is NULL");
+  int rc = validate_qk_norm_rope_backward(p);
+  if (rc) return rc;
+  int parts, blocks;
+  return plan_qk_backward(p, &parts, &blocks, bytes_out);
+}
+
+int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  g_last_error[0] = '\0';
+  int rc = validate_qk_norm_rope_backward(p);
+  if (rc) return rc;
+  int parts, blocks;
+  size_t bytes;
+  if ((rc = plan_qk_backward(p, &parts, &blocks, &bytes))) return rc;
+  if (p->total_q == 0 && bytes == 0) return IFA4_OK;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(IFA4_ERR_WORKSPACE, "qk_norm_rope_backward: workspace of %zu bytes required, got %zu",
+                bytes, workspace_bytes);
+  if (bytes > 0 && !aligned16(workspace))
+    return fail(IFA4_ERR_WORKSPACE, "qk_norm_rope_backward: workspace must be 16-byte aligned");
+  ifa4::QkvBackwardKernelArgs a{};
+  a.dq_out = static_cast<const uint16_t*>(p->dq_out);
+  a.dk_out = static_cast<const uint16_t*>(p->dk_out);
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.dq = static_cast<uint16_t*>(p->dq);
+  a.dk = static_cast<uint16_t*>(p->dk);
+  a.q_weight = p->q_weight;
+  a.k_weight = p->k_weight;
+  a.dq_weight = p->dq_weight;
+  a.dk_weight = p->dk_weight;
+  a.inv_freq = p->inv_freq;
+  a.cu_q = p->cu_seqlens_q;
+  a.cu_k = p->cu_seqlens_k;
+  a.partial = bytes > 0 ? static_cast<float*>(workspace) : nullptr;
+  a.dqo_st = p->dq_out_stride_t;
+  a.dqo_sh = p->dq_out_stride_h;
+  a.dko_st = p->dk_out_stride_t;
+  a.dko_sh = p->dk_out_stride_h;
+  a.q_st = p->q_stride_t;
+  a.q_sh = p->q_stride_h;
+  a.k_st = p->k_stride_t;
+  a.k_sh = p->k_stride_h;
+  a.dq_st = p->dq_stride_t;
+  a.dq_sh = p->dq_stride_h;
+  a.dk_st = p->dk_stride_t;
+  a.dk_sh = p->dk_stride_h;
+  a.units = p->total_q * parts;
+  a.batch = p->batch;
+  a.n_heads = p->n_heads;
+  a.kv_heads = p->kv_heads;
+  a.rotary_dim = p->rotary_dim;
+  a.interleaved = p->interleaved ? 1 : 0;
+  a.normalize = p->normalize ? 1 : 0;
+  a.weight_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
+  a.inv_freq_f32 = p->inv_freq_f32 ? 1 : 0;
+  a.parts = parts;
+  a.q_per_part = (p->n_heads + parts - 1) / parts;
+  a.k_per_part = (p->kv_heads + parts - 1) / parts;
+  a.eps = p->eps;
+  cudaError_t e = ifa4::launch_qkv_backward_sm100(a, blocks, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_backward launch");
+  return IFA4_OK;
+}
+
+int ifa4_kv_append_launch(const IFA4KvAppendParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "kv_append";
+  int rc = validate_norm_rope(p, what);
+  if (rc) return rc;
+  if (p->page_size < 16 || p->page_size > (1 << 20) || (p->page_size & (p->page_size - 1)) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: page_size %d must be a power of two in [16, 2^20]",
+                what, p->page_size);
+  if (p->num_pages < 0 || p->table_width < 0 || p->block_table_stride < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative num_pages, table_width or table stride",
+                what);
+  if (p->total_q == 0) return IFA4_OK;
+  if (p->kv_heads == 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: kv_heads must be > 0", what);
+  if (p->cu_seqlens_q == nullptr || p->cu_seqlens_k == nullptr || p->block_table == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: needs cu_seqlens_q, cu_seqlens_k and block_table",
+                what);
+  if (p->n_heads > 0 &&
+      ((rc = check_rows(what, "q", p->q, p->q_stride_t, p->q_stride_h, false)) ||
+       (rc = check_rows(what, "q_out", p->q_out, p->q_out_stride_t, p->q_out_stride_h, true))))
+    return rc;
+  if ((rc = check_rows(what, "k", p->k, p->k_stride_t, p->k_stride_h, false)) ||
+      (rc = check_rows(what, "v", p->v, p->v_stride_t, p->v_stride_h, false)) ||
+      (rc = check_rows(what, "k_cache", p->k_cache, p->k_cache_stride_t, p->k_cache_stride_h,
+                       true)) ||
+      (rc = check_rows(what, "v_cache", p->v_cache, p->v_cache_stride_t, p->v_cache_stride_h,
+                       true)))
+    return rc;
+  if (p->k_stride_page <= 0 || p->k_stride_page % 8 != 0 || p->v_stride_page <= 0 ||
+      p->v_stride_page % 8 != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: k/v page strides must be positive multiples of 8 elements", what);
+  ifa4::QkvKernelArgs a{};
+  fill_qkv(p, &a);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.v_st = p->v_stride_t;
+  a.v_sh = p->v_stride_h;
+  a.k_cache = static_cast<uint16_t*>(p->k_cache);
+  a.v_cache = static_cast<uint16_t*>(p->v_cache);
+  a.kc_sp = p->k_stride_page;
+  a.kc_st = p->k_cache_stride_t;
+  a.kc_sh = p->k_cache_stride_h;
+  a.vc_sp = p->v_stride_page;
+  a.vc_st = p->v_cache_stride_t;
+  a.vc_sh = p->v_cache_stride_h;
+  a.block_table = p->block_table;
+  a.bt_stride = p->block_table_stride;
+  a.page_shift = log2_exact(p->page_size);
+  a.table_width = p->table_width;
+  a.num_pages = p->num_pages;
+  return launch_qkv("kv_append launch", &a, p->total_q, p->n_heads + 2 * p->kv_heads, stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------
+// Bias by distance buckets
+// ---------------------------------------------------------------------------------------
+namespace {
+static_assert(ifa4::kMaxBuckets == IFA4_MAX_BUCKETS, "bucket limit");
+
+template <class P>
+int validate_buckets(const P* p, const char* what) {
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  if (p->n_heads <= 0 || p->n_heads > 65535 || p->rel_extent <= 0 || p->rel_extent > (1 << 24))
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: n_heads must be in [1, 65535], rel_extent in [1, 2^24]", what);
+  if (p->buckets <= 0 || p->buckets > IFA4_MAX_BUCKETS)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: buckets %d outside [1, %d]", what, p->buckets,
+                IFA4_MAX_BUCKETS);
+  if (p->weight_dtype != IFA4_WEIGHT_BF16 && p->weight_dtype != IFA4_WEIGHT_F32)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: weight_dtype %d unsupported", what, p->weight_dtype);
+  if (p->starts == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: starts is NULL", what);
+  return IFA4_OK;
+}
+
+int plan_bucket_backward(const IFA4BucketBiasBackwardParams* p, ifa4::BucketGradKernelArgs* a,
+                         int* vec, size_t* bytes) {
+  const char* what = "bucket_bias_backward";
+  int rc = validate_buckets(p, what);
+  if (rc) return rc;
+  if (p->total_q < 0 || p->total_q > (1LL << 40))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: total_q outside [0, 2^40]", what);
+  if (p->drel == nullptr && p->total_q > 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: drel is NULL", what);
+  if (p->dtable == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: dtable is NULL", what);
+  const unsigned wmask = p->weight_dtype == IFA4_WEIGHT_F32 ? 3u : 1u;
+  if ((reinterpret_cast<uintptr_t>(p->dtable) & wmask) != 0 ||
+      (reinterpret_cast<uintptr_t>(p->drel) & 1u) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned drel or dtable", what);
+  if (p->drel_stride_t < 0 || p->drel_stride_h < 0 || p->dtable_stride_b < 0 ||
+      p->dtable_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative strides", what);
+  if (p->cu_seqlens_q != nullptr && p->batch < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative batch", what);
+  a->drel = static_cast<const uint16_t*>(p->drel);
+  a->starts = p->starts;
+  a->cu_q = p->cu_seqlens_q;
+  a->grad = p->dtable;
+  a->drel_st = p->drel_stride_t;
+  a->drel_sh = p->drel_stride_h;
+  a->grad_sb = p->dtable_stride_b;
+  a->grad_sh = p->dtable_stride_h;
+  a->total_q = p->total_q;
+  a->batch = p->batch;
+  a->n_heads = p->n_heads;
+  a->rel_extent = p->rel_extent;
+  a->buckets = p->buckets;
+  a->grad_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
+  // widest loads the layout allows
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p->drel);
+  *vec = 1;
+  for (int v : {8, 2})
+    if (at % (2 * v) == 0 && p->drel_stride_t % v == 0 && p->drel_stride_h % v == 0 &&
+        p->rel_extent % v == 0) {
+      *vec = v;
+      break;
+    }
+  int sms = 148;
+  if ((rc = sm_count(&sms))) return rc;
+  ifa4::plan_bucket_grad(a, *vec, sms);
+  *bytes = a->slots > 1 ? static_cast<size_t>(a->slots) * p->n_heads * p->buckets * sizeof(float) : 0;
+  return IFA4_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int ifa4_bucket_bias_launch(const IFA4BucketBiasParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "bucket_bias";
+  int rc = validate_buckets(p, what);
+  if (rc) return rc;
+  const unsigned wmask = p->weight_dtype == IFA4_WEIGHT_F32 ? 3u : 1u;
+  if (p->table == nullptr || p->rel == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if ((reinterpret_cast<uintptr_t>(p->table) & wmask) != 0 ||
+      (reinterpret_cast<uintptr_t>(p->rel) & 1u) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned table or rel", what);
+  if (p->table_stride_b < 0 || p->table_stride_h < 0 || p->rel_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative strides", what);
+  ifa4::BucketBiasKernelArgs a{};
+  a.table = p->table;
+  a.starts = p->starts;
+  a.rel = static_cast<uint16_t*>(p->rel);
+  a.table_sb = p->table_stride_b;
+  a.table_sh = p->table_stride_h;
+  a.rel_sh = p->rel_stride_h;
+  a.n_heads = p->n_heads;
+  a.rel_extent = p->rel_extent;
+  a.buckets = p->buckets;
+  a.table_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
+  cudaError_t e = ifa4::launch_bucket_bias_sm100(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "bucket_bias launch");
+  return IFA4_OK;
+}
+
+int ifa4_bucket_bias_backward_workspace_size(const IFA4BucketBiasBackwardParams* p,
+                                             size_t* bytes_out) {
+  g_last_error[0] = '\0';
+  if (bytes_out == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "bucket_bias_backward: bytes_out is NULL");
+  ifa4::BucketGradKernelArgs a{};
+  int vec;
+  return plan_bucket_backward(p, &a, &vec, bytes_out);
+}
+
+int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* p, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  g_last_error[0] = '\0';
+  ifa4::BucketGradKernelArgs a{};
+  int vec;
+  size_t bytes;
+  int rc = plan_bucket_backward(p, &a, &vec, &bytes);
+  if (rc) return rc;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(IFA4_ERR_WORKSPACE, "bucket_bias_backward: workspace of %zu bytes required, got %zu",
+                bytes, workspace_bytes);
+  if (bytes > 0 && !aligned16(workspace))
+    return fail(IFA4_ERR_WORKSPACE, "bucket_bias_backward: workspace must be 16-byte aligned");
+  a.partial = static_cast<float*>(workspace);
+  cudaError_t e = ifa4::launch_bucket_grad_sm100(a, vec, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "bucket_bias_backward launch");
   return IFA4_OK;
 }
 

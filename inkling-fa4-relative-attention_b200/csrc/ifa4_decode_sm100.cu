@@ -12,7 +12,8 @@
 //               with the fused relative-bias gather.
 // The four warps' (max, sum, O) states are merged in shared memory; with one split the CTA
 // writes the bf16 output, otherwise a normalised fp32 partial and its log2-sum-exp, which
-// rel_attn_decode_combine_kernel merges.
+// rel_attn_decode_combine_kernel merges (or, with prefix_len > 0, when only the keys behind the
+// batch's shared prefix are read here, shared_prefix_combine_kernel).
 //
 // Paged KV cache (kPaged): the whole producer warp runs, fetching the next tile's page numbers
 // from the block table while the current tile is issued; a 64-key tile is loaded as 64 / box
@@ -97,6 +98,7 @@ __device__ __forceinline__ SeqInfo seq_info(const DecodeKernelArgs& a, int b) {
   s.hi = s.sk;
   if (a.causal) s.hi = min(s.hi, ms + 1);
   s.lo = a.window_left >= 0 ? max(0, ms - a.window_left) : 0;
+  if (s.sk >= a.prefix_len) s.lo = max(s.lo, a.prefix_len);  // the prefix is read elsewhere
   s.base = kPaged ? s.lo & ~((1 << a.box_shift) - 1) : s.lo;
   s.nchunks = s.hi > s.lo ? (s.hi - s.base + a.chunk_len - 1) / a.chunk_len : 0;
   return s;
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const float val = L > 0.f ? acc / L : 0.f;
       if (!IFA4_DBG_CHECK(a.status, si.q_row >= 0 && si.q_row < a.batch && h < a.n_heads)) {
         // a bad query row or head: nothing is stored
-      } else if (gridDim.x == 1) {
+      } else if (a.ws_o == nullptr) {
         uint16_t* dst = a.out + static_cast<long long>(si.q_row) * a.out_st +
                         static_cast<long long>(h) * a.out_sh + d;
         __nv_bfloat16 bv = __float2bfloat16_rn(val);
@@ -484,7 +486,7 @@ cudaError_t launch_decode_sm100(const DecodeKernelArgs& args, const CUtensorMap&
     decode::rel_attn_decode_kernel<false><<<grid, decode::kThreads, decode::kSmemAlloc, stream>>>(
         args, tm_k, tm_v);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || args.num_splits == 1) return e;
+  if (e != cudaSuccess || args.ws_o == nullptr || args.prefix_len > 0) return e;
   dim3 cgrid(args.n_heads, args.batch);
   decode::rel_attn_decode_combine_kernel<<<cgrid, 128, 0, stream>>>(args);
   return cudaGetLastError();

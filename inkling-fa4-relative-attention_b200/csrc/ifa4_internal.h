@@ -138,11 +138,131 @@ struct DecodeKernelArgs {
   const int32_t* block_table;  // paged KV cache, as in PrefillKernelArgs
   long long bt_stride;
   int page_shift, box_shift, num_pages;
+  // shared prefix (0: none): sequences of at least this many keys start at key prefix_len, and the
+  // partials (always written then, whatever num_splits) go to shared_prefix_combine_kernel
+  int prefix_len;
   int* status;
 };
 
 cudaError_t launch_decode_sm100(const DecodeKernelArgs& args, const CUtensorMap& tm_k,
                                 const CUtensorMap& tm_v, cudaStream_t stream);
+
+// Prefix part of a decode batch that shares its first prefix_len keys, and the merge with the
+// sequences' own keys (decode partials own_o / own_lse).
+struct SharedPrefixKernelArgs {
+  const uint16_t* rel;
+  long long rel_st, rel_sh;
+  const int32_t* cu_k;
+  int batch, n_heads, kv_heads, rel_extent;
+  int group;                 // n_heads / kv_heads
+  int seqs_per_tile;         // 128 / group: sequences in a 128-row tile
+  int prefix_len, window_left;
+  int key_pair;              // one row tile per KV head: halves alternate over key tiles
+  int splits;                // key splits (CTAs per row tile pair and KV head)
+  int parts;                 // prefix partials per row: splits, or 2 * splits with key_pair
+  int bias_vec;              // as in PrefillKernelArgs
+  float scale_log2;
+  const int32_t* block_table;
+  long long bt_stride;
+  int page_shift, box_shift, num_pages;
+  const uint16_t* v;         // V cache base (the unit in which the prefix ends)
+  long long v_st, v_sh, v_sp;
+  float* ws_o;               // [parts, batch, n_heads, 128]
+  float* ws_lse;             // [parts, batch, n_heads], log2 units, -inf: no visible key
+  const float* own_o;        // [batch, n_heads, own_parts, 128]
+  const float* own_lse;      // [batch, n_heads, own_parts]
+  int own_parts;
+  uint16_t* out;
+  long long out_st, out_sh;
+  float* lse;                // optional natural-log LSE
+  long long lse_sh, lse_st;
+  int* status;
+};
+
+cudaError_t launch_shared_prefix_sm100(const SharedPrefixKernelArgs& args, const CUtensorMap& tm_q,
+                                       const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                       cudaStream_t stream);
+cudaError_t launch_shared_prefix_combine_sm100(const SharedPrefixKernelArgs& args,
+                                               cudaStream_t stream);
+
+// Norm and rotation of q and k rows; with k_cache set, k and v rows go to the paged caches.
+struct QkvKernelArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* q_out;
+  uint16_t* k_out;
+  uint16_t* k_cache;
+  uint16_t* v_cache;
+  const void* q_weight;      // [128] bf16 or fp32, null: ones
+  const void* k_weight;
+  const void* inv_freq;      // [rotary_dim / 2] fp64 or fp32
+  const int32_t* cu_q;       // optional (null: one sequence)
+  const int32_t* cu_k;       // optional
+  const int32_t* block_table;
+  long long q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh, ko_st, ko_sh;
+  long long kc_sp, kc_st, kc_sh, vc_sp, vc_st, vc_sh;
+  long long bt_stride;
+  long long units;           // total_q * parts
+  int batch, n_heads, kv_heads;
+  int rotary_dim, interleaved, normalize, weight_f32, inv_freq_f32, zero_padding;
+  int parts, rows_per_part;  // a token's rows are shared by `parts` warps
+  int page_shift, table_width, num_pages;
+  float eps;
+};
+
+struct QkvBackwardKernelArgs {
+  const uint16_t* dq_out;
+  const uint16_t* dk_out;
+  const uint16_t* q;
+  const uint16_t* k;
+  uint16_t* dq;
+  uint16_t* dk;
+  const void* q_weight;
+  const void* k_weight;
+  void* dq_weight;           // optional, like the weights
+  void* dk_weight;
+  const void* inv_freq;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  float* partial;            // [blocks, 2, 128] (null: no weight gradients)
+  long long dqo_st, dqo_sh, dko_st, dko_sh, q_st, q_sh, k_st, k_sh, dq_st, dq_sh, dk_st, dk_sh;
+  long long units;
+  int batch, n_heads, kv_heads;
+  int rotary_dim, interleaved, normalize, weight_f32, inv_freq_f32;
+  int parts, q_per_part, k_per_part;
+  float eps;
+};
+
+cudaError_t launch_qkv_rows_sm100(const QkvKernelArgs& args, int sms, cudaStream_t stream);
+cudaError_t launch_qkv_backward_sm100(const QkvBackwardKernelArgs& args, int blocks,
+                                      cudaStream_t stream);
+constexpr int kQkvBackwardWarps = 4;  // warps of a block of the backward kernel
+
+// Bias by distance buckets and its gradient.
+constexpr int kMaxBuckets = 1024;
+struct BucketBiasKernelArgs {
+  const void* table;         // table[b * table_sb + h * table_sh], bf16 or fp32
+  const int32_t* starts;     // [buckets]
+  uint16_t* rel;             // rel[h * rel_sh + d]
+  long long table_sb, table_sh, rel_sh;
+  int n_heads, rel_extent, buckets, table_f32;
+};
+struct BucketGradKernelArgs {
+  const uint16_t* drel;
+  const int32_t* starts;
+  const int32_t* cu_q;       // optional: tokens from cu_q[batch] on are not counted
+  void* grad;                // grad[b * grad_sb + h * grad_sh], bf16 or fp32
+  float* partial;            // [slots, n_heads, buckets]
+  long long drel_st, drel_sh, grad_sb, grad_sh;
+  long long total_q, chunk;  // tokens, tokens per chunk
+  int batch, n_heads, rel_extent, buckets, grad_f32;
+  int heads, cols, col_parts, lanes, chunks, slots;  // plan_bucket_grad
+};
+cudaError_t launch_bucket_bias_sm100(const BucketBiasKernelArgs& args, cudaStream_t stream);
+void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms);
+cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
+                                     cudaStream_t stream);
 
 struct BackwardKernelArgs {
   const uint16_t* rel;       // bf16 bits

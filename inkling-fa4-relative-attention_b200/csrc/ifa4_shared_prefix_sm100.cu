@@ -1,0 +1,672 @@
+// Decode attention over a prefix that a batch of sequences shares, for sm_100a: the prefix part
+// of ifa4_decode_shared_prefix_launch, and the merge of its partials with those of the
+// sequences' own keys (rel_attn_decode_kernel restricted to keys past the prefix).
+//
+// With G query heads per KV head and B sequences, B * G query rows read the same prefix keys:
+// the prefix is a matrix product of up to 128 rows a tile against 128-key tiles, so its K and V
+// are read once per 128 (or 256) rows instead of once per sequence, and S = Q K^T and O += P V
+// run on tcgen05.  Row r of a tile is head r mod G of sequence r div G; a tile's rows are one TMA
+// box of Q ({64 dims, G heads, 128 / G sequences}).
+//
+// Per row (one softmax thread each): distance d = (len - 1) - key, bias rel[h, d] where
+// 0 <= d < R, window d <= W, online softmax in the exp2 domain with P written back to TMEM as
+// bf16, exactly as in the prefill kernel (whose roles and TMEM plan this kernel has).
+// Sequences with fewer keys than the prefix take no part (their rows have weight 0 here; the
+// decode kernel then covers all of their keys).
+//
+// The grid is (row tiles, KV heads, key splits); every CTA writes its rows' normalised fp32
+// partial outputs and log2-sum-exps, and shared_prefix_combine_kernel merges all partials of a
+// row.  The CTA's two softmax groups (and TMEM halves) work on
+//   kKeyPair = false: two row tiles at the same keys (batches of more than one tile per KV head:
+//                     K and V are shared by 256 rows);
+//   kKeyPair = true:  one row tile at alternating key tiles (small batches: one group's softmax
+//                     overlaps the other's products; each group writes its own partial).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ifa4_internal.h"
+#include "ifa4_ptx.cuh"
+
+namespace ifa4 {
+namespace prefix {
+
+constexpr int kBM = 128;
+constexpr int kBN = 128;
+constexpr int kThreads = 384;
+// as in the prefill kernel: warps 0-3 give registers to the eight softmax warps
+constexpr int kRegsControl = 56, kRegsSoftmax = 224;
+static_assert(4 * 32 * kRegsControl + 8 * 32 * kRegsSoftmax <= 384 * 168, "register split");
+constexpr uint32_t kHalf = 128u * 128u;  // 128 rows x 128 B (64 dims)
+constexpr uint32_t kTile = 2u * kHalf;
+constexpr uint32_t kSmemQ = 0;           // 2 row tiles (the second one is staging with kKeyPair)
+constexpr uint32_t kSmemK = 2 * kTile;   // 2 stages
+constexpr uint32_t kSmemV = 4 * kTile;   // 2 stages
+constexpr uint32_t kSmemBar = 6 * kTile;
+constexpr uint32_t kSmemBytes = kSmemBar + 256;
+constexpr uint32_t kSmemAlloc = kSmemBytes + 1024;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleThreshold = 8.0f;
+
+constexpr uint32_t kIdescQK = idesc_bf16_f32(128, 128, /*b_mn_major=*/false);
+constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, /*b_mn_major=*/true);
+
+struct Bars {
+  uint64_t q_full;
+  uint64_t k_full[2], k_empty[2];
+  uint64_t v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2];
+  uint64_t o_full[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+  int lo;   // first visible key over the CTA's rows (past the prefix: no row takes part)
+  int ref;  // first of the CTA's sequences that take part: its table row names the prefix pages
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+__device__ __forceinline__ void issue_qk(uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr) {
+  const uint64_t qd = sdesc_sw128(q_addr, 16, 1024);
+  const uint64_t kd = sdesc_sw128(k_addr, 16, 1024);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    const uint32_t off = (kk >> 2) * kHalf + (kk & 3) * 32;
+    umma_ss(tmem_s, sdesc_advance(qd, off), sdesc_advance(kd, off), kIdescQK, kk > 0 ? 1u : 0u);
+  }
+}
+
+__device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr,
+                                         bool accumulate) {
+  const uint64_t vd = sdesc_sw128(v_addr, kHalf, 1024);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_ts(tmem_o, tmem_p + kk * 8, sdesc_advance(vd, kk * 2048), kIdescPV,
+            (kk > 0 || accumulate) ? 1u : 0u);
+}
+
+// Row r of row tile `tile`: its sequence and head, and whether it takes part.
+struct Row {
+  int b, h, len;
+  bool on;
+};
+__device__ __forceinline__ Row row_of(const SharedPrefixKernelArgs& a, int tile, int r, int kvh) {
+  Row w;
+  const int bl = r / a.group;
+  w.b = tile * a.seqs_per_tile + bl;
+  w.h = kvh * a.group + (r - bl * a.group);
+  w.on = bl < a.seqs_per_tile && w.b < a.batch;
+  w.len = w.on ? __ldg(a.cu_k + w.b + 1) - __ldg(a.cu_k + w.b) : 0;
+  w.on = w.on && w.len >= a.prefix_len;
+  return w;
+}
+
+template <bool kKeyPair>
+__global__ void __launch_bounds__(kThreads, 1)
+    shared_prefix_kernel(const __grid_constant__ SharedPrefixKernelArgs a,
+                         const __grid_constant__ CUtensorMap tm_q,
+                         const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + kSmemBar);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int tile0 = kKeyPair ? blockIdx.x : 2 * blockIdx.x;
+  const int kvh = blockIdx.y;
+  const int split = blockIdx.z;
+  constexpr int kTiles = kKeyPair ? 1 : 2;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bars->q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->k_full[i], 1);
+      mbar_init(&bars->k_empty[i], 1);
+      mbar_init(&bars->v_full[i], 1);
+      mbar_init(&bars->v_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 4);
+      mbar_init(&bars->o_full[i], 1);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    bars->lo = 0x7fffffff;
+    bars->ref = 0x7fffffff;
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(&bars->tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  // rows of the Q tiles that no TMA box covers (group does not divide 128) are zeros
+  const int box_rows = a.seqs_per_tile * a.group;
+  for (int i = threadIdx.x; i < kTiles * 2 * (kBM - box_rows) * 8; i += kThreads) {
+    const int c = i & 7, rest = i >> 3;
+    const int hf = rest / (kBM - box_rows);
+    const int row = box_rows + rest - hf * (kBM - box_rows);
+    *reinterpret_cast<uint4*>(smem + kSmemQ + hf * kHalf + row * 128 + c * 16) =
+        make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  // this thread's row (softmax warps)
+  const int s = warp >= 4 ? (warp - 4) >> 2 : 0;
+  const int row = (warp & 3) * 32 + lane;
+  Row me{0, 0, 0, false};
+  int key_lo = 0;
+  if (warp >= 4) {
+    me = row_of(a, tile0 + (kKeyPair ? 0 : s), row, kvh);
+    if (a.window_left >= 0) key_lo = max(0, me.len - 1 - a.window_left);
+    if (key_lo >= a.prefix_len) me.on = false;
+    const int lo = __reduce_min_sync(0xffffffffu, me.on ? key_lo : 0x7fffffff);
+    const int ref = __reduce_min_sync(0xffffffffu, me.on ? me.b : 0x7fffffff);
+    if (lane == 0 && lo != 0x7fffffff) {
+      atomicMin(&bars->lo, lo);
+      atomicMin(&bars->ref, ref);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  // this CTA's share of the key tiles
+  int j_lo = 0, n_kv = 0;
+  if (bars->ref != 0x7fffffff) {
+    const int first = bars->lo / kBN, all = (a.prefix_len + kBN - 1) / kBN - first;
+    const int per = (all + a.splits - 1) / a.splits;
+    j_lo = first + split * per;
+    n_kv = max(0, min(per, all - split * per));
+  }
+  const AbortCtx ab{&bars->abort_flag, a.status, kStatusDecodeTimeout};
+  if (warp < 4) setmaxnreg_dec<kRegsControl>();
+  else setmaxnreg_inc<kRegsSoftmax>();
+  if (warp < 4) {
+    if (warp == 0 && n_kv > 0) {
+      // ---------------------------------------------------------------- TMA producer (warp)
+      const uint64_t pol_kv = l2_policy_evict_last();
+      const uint64_t pol_q = l2_policy_evict_first();
+      const int box = 1 << a.box_shift;
+      const int units = kBN >> a.box_shift;
+      const int page_mask = (1 << a.page_shift) - 1;
+      const int32_t* bt = a.block_table + static_cast<long long>(bars->ref) * a.bt_stride;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars->q_full, kTiles * 2 * box_rows * 128);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_3d_hint(smem + kSmemQ + i * kTile + hf * kHalf, &tm_q, &bars->q_full,
+                             hf * 64, kvh * a.group, (tile0 + i) * a.seqs_per_tile, pol_q);
+      }
+      // page of unit `lane` of key tile j; -1 past the prefix or for an entry outside
+      // [0, num_pages)
+      auto unit_block = [&](int j) {
+        const int key = (j_lo + j) * kBN + lane * box;
+        int blk = -1;
+        if (lane < units && key < a.prefix_len) {
+          blk = __ldg(bt + (key >> a.page_shift));
+          if (blk < 0 || blk >= a.num_pages) blk = -1;
+        }
+        return blk;
+      };
+      bool ok = true;
+      int blk = unit_block(0);
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const int key0 = (j_lo + j) * kBN;
+        const int blk_next = j + 1 < n_kv ? unit_block(j + 1) : -1;
+        const int in_page = (key0 + lane * box) & page_mask;
+        const int page = blk >= 0 ? blk : a.num_pages;  // out of range: TMA writes zeros
+        const uint32_t st = j & 1, ph = ((j >> 1) & 1) ^ 1;
+        if (!(ok = mbar_wait_warp(&bars->k_empty[st], ph, ab))) break;
+        if (lane == 0) mbar_arrive_expect_tx(&bars->k_full[st], kTile);
+        __syncwarp();
+        if (lane < units) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_4d_hint(smem + kSmemK + st * kTile + hf * kHalf + lane * box * 128, &tm_k,
+                             &bars->k_full[st], hf * 64, kvh, in_page, page, pol_kv);
+        }
+        if (!(ok = mbar_wait_warp(&bars->v_empty[st], ph, ab))) break;
+        // the unit in which the prefix ends: its later slots may hold anything, so its V rows are
+        // copied here with zeros behind the prefix (P is 0 there, but 0 * NaN is not)
+        const int pu = (a.prefix_len < key0 + kBN && (a.prefix_len & (box - 1)) != 0)
+                           ? (a.prefix_len - key0) >> a.box_shift : -1;
+        uint32_t v_bytes = kTile;
+        if (pu >= 0) {
+          const int pblk = __shfl_sync(0xffffffffu, blk, pu);
+          const int pkey = key0 + pu * box;
+          const int nvalid = a.prefix_len - pkey;
+          const uint16_t* src = a.v + static_cast<long long>(pblk < 0 ? 0 : pblk) * a.v_sp +
+                                static_cast<long long>(pkey & page_mask) * a.v_st +
+                                static_cast<long long>(kvh) * a.v_sh;
+          uint8_t* dst = smem + kSmemV + st * kTile;
+#pragma unroll 4
+          for (int i = lane; i < box * 16; i += 32) {
+            const int r = i >> 4, ch = i & 15;
+            uint4 val = make_uint4(0u, 0u, 0u, 0u);
+            if (r < nvalid && pblk >= 0) val = ldg_nc_v4(src + static_cast<long long>(r) * a.v_st + ch * 8);
+            const int rw = pu * box + r;
+            *reinterpret_cast<uint4*>(dst + (ch >> 3) * kHalf + rw * 128 +
+                                      (((ch & 7) ^ (rw & 7)) << 4)) = val;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          v_bytes -= static_cast<uint32_t>(box) * 256u;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&bars->v_full[st], v_bytes);
+        __syncwarp();
+        if (lane < units && lane != pu) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_4d_hint(smem + kSmemV + st * kTile + hf * kHalf + lane * box * 128, &tm_v,
+                             &bars->v_full[st], hf * 64, kvh, in_page, page, pol_kv);
+        }
+        blk = blk_next;
+      }
+      if (lane == 0) {  // every issued load has landed before the CTA may exit
+        mbar_wait(&bars->q_full, 0, ab);
+        for (int i = 0; i < 2 && i < n_kv; ++i) {
+          const int last = n_kv - 1 - i;
+          mbar_wait(&bars->k_full[last & 1], (last >> 1) & 1, ab);
+          mbar_wait(&bars->v_full[last & 1], (last >> 1) & 1, ab);
+        }
+      }
+    } else if (warp == 1 && n_kv > 0) {
+      // ---------------------------------------------------------------- UMMA issuer
+      if (lane == 0) {
+        const uint32_t q_addr = smem_u32(smem + kSmemQ);
+        const uint32_t k_addr = smem_u32(smem + kSmemK);
+        const uint32_t v_addr = smem_u32(smem + kSmemV);
+        bool ok = mbar_wait(&bars->q_full, 0, ab);
+        if (kKeyPair) {
+          // key tile j on half s = j mod 2: S(j + 1) is issued before P(j) is waited for
+          auto qk = [&](int j) {
+            const int st = j & 1;
+            if (!(ok = ok && mbar_wait(&bars->k_full[st], (j >> 1) & 1, ab))) return;
+            tc_fence_after();
+            issue_qk(tbase + st * 128, q_addr, k_addr + st * kTile);
+            umma_commit(&bars->s_full[st]);
+            umma_commit(&bars->k_empty[st]);
+          };
+          if (ok) qk(0);
+          if (ok && n_kv > 1) qk(1);
+          for (int j = 0; j < n_kv && ok; ++j) {
+            const int st = j & 1;
+            if (!(ok = mbar_wait(&bars->p_full[st], (j >> 1) & 1, ab))) break;
+            if (!(ok = mbar_wait(&bars->v_full[st], (j >> 1) & 1, ab))) break;
+            tc_fence_after();
+            issue_pv(tbase + 256 + st * 128, tbase + st * 128, v_addr + st * kTile, j > 1);
+            umma_commit(&bars->v_empty[st]);
+            if (j + 2 < n_kv) qk(j + 2);  // overwrites P(j) in order after its product
+            else umma_commit(&bars->o_full[st]);
+          }
+        } else {
+          for (int j = 0; j <= n_kv && ok; ++j) {
+            const int st = j & 1, pst = (j - 1) & 1;
+            if (j < n_kv && !(ok = mbar_wait(&bars->k_full[st], (j >> 1) & 1, ab))) break;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (j > 0) {  // O_i += P_i V of tile j - 1
+                if (!(ok = mbar_wait(&bars->p_full[i], (j - 1) & 1, ab))) break;
+                if (i == 0 && !(ok = mbar_wait(&bars->v_full[pst], ((j - 1) >> 1) & 1, ab))) break;
+                tc_fence_after();
+                issue_pv(tbase + 256 + i * 128, tbase + i * 128, v_addr + pst * kTile, j > 1);
+              } else {
+                tc_fence_after();
+              }
+              if (j < n_kv) {  // S_i = Q_i K^T of tile j
+                issue_qk(tbase + i * 128, q_addr + i * kTile, k_addr + st * kTile);
+                umma_commit(&bars->s_full[i]);
+              } else {
+                umma_commit(&bars->o_full[i]);
+              }
+            }
+            if (!ok) break;
+            if (j < n_kv) umma_commit(&bars->k_empty[st]);
+            if (j > 0) umma_commit(&bars->v_empty[pst]);
+          }
+        }
+        umma_commit(&bars->drain);  // every issued MMA completes before TMEM is released
+        mbar_wait(&bars->drain, 0, ab);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tbase + lane_off + s * 128;
+    const uint32_t t_o = tbase + lane_off + 256 + s * 128;
+    const int key_hi = a.prefix_len;
+    const int dmax = me.len - 1;  // bias distance at key 0
+    const uint16_t* rel_row = a.rel + static_cast<long long>(me.b) * a.rel_st +
+                              static_cast<long long>(me.h) * a.rel_sh;
+    constexpr int kStep = kKeyPair ? 2 : 1;
+    const int j0 = kKeyPair ? s : 0;
+    const int part = kKeyPair ? 2 * split + s : split;  // partial this half writes
+    float m_run = -INFINITY, l_run = 0.f;
+    uint32_t pc = 0;
+    bool ok = true;
+    for (int j = j0; j < n_kv && ok; j += kStep) {
+      const int k0 = (j_lo + j) * kBN;
+      const int bl = dmax - a.rel_extent + 1 - k0;  // first column with bias
+      const int bh = dmax - k0;                     // last column with bias (>= 0)
+      const int cl = key_lo - k0, ch = key_hi - k0;  // visible columns [cl, ch)
+      const bool has_bias = me.on && bl <= 127;
+      // rows that take no part are never read back: they need no mask
+      const bool has_mask = me.on && (cl > 0 || ch < kBN);
+      const bool warp_bias = __any_sync(0xffffffffu, has_bias);
+      uint32_t bwin[2][20];
+      if (a.bias_vec && warp_bias) {
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc)
+          load_bias_window(rel_row, bh, cc, a.rel_extent,
+                           has_bias && cc * 32 + 31 >= bl && cc * 32 <= bh, bwin[cc]);
+      }
+      if (!(ok = mbar_wait_warp(&bars->s_full[s], pc & 1, ab))) break;
+      ++pc;
+      tc_fence_after();
+      bool done = false;
+      // Interior tiles after the first: exponentials against the running max, redone below when
+      // a score outgrew it (see the prefill kernel).
+      if (j > j0 && !__any_sync(0xffffffffu, has_bias || has_mask)) {
+        const uint64_t mul2 = f2_pack(a.scale_log2, a.scale_log2);
+        const uint64_t neg2 = f2_pack(-m_run, -m_run);
+        uint64_t acc[4] = {0, 0, 0, 0};
+        uint32_t pk[2][32];
+        uint32_t rq[2][16];
+        tmem_ld16(t_s, rq[0]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c < 7) tmem_ld16(t_s + (c + 1) * 16, rq[(c + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int col = c * 16 + 2 * i;
+            float y0, y1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(rq[c & 1][2 * i]),
+                                     __uint_as_float(rq[c & 1][2 * i + 1])),
+                             mul2, neg2),
+                      y0, y1);
+            float p0, p1;
+            if ((col & 15) < 2) {  // 2 of 16 on the FMA pipe, as in the prefill
+              exp2_poly_pair_capped(y0, y1, p0, p1);
+            } else {
+              p0 = fast_exp2(y0);
+              p1 = fast_exp2(y1);
+            }
+            acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
+            pk[c >> 2][(c & 3) * 8 + i] = pack_bf16x2(p0, p1);
+          }
+          if (c < 7) tmem_wait_ld();
+        }
+        const uint64_t a01 = f2_add(acc[0], acc[1]), a23 = f2_add(acc[2], acc[3]);
+        float u0, u1;
+        f2_unpack(f2_add(a01, a23), u0, u1);
+        const float l_tile = u0 + u1;
+        if (__all_sync(0xffffffffu, l_tile <= 4294967296.0f)) {  // false for inf and NaN
+          tmem_st32(t_s, pk[0]);
+          tmem_st32(t_s + 32, pk[1]);
+          l_run += l_tile;
+          done = true;
+        }
+      }
+      if (!done) {
+        // Pass 1: the logits (scaled, biased, masked) replace S in TMEM; their row max.
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_s + c * 32, r);
+          tmem_wait_ld();
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * a.scale_log2;
+          const bool chunk_bias = has_bias && c * 32 + 31 >= bl && c * 32 <= bh;
+          if (a.bias_vec) {
+            if (__any_sync(0xffffffffu, chunk_bias)) add_bias_window(bwin[c & 1], bh, c, x);
+            if (c < 2 && warp_bias)
+              load_bias_window(rel_row, bh, c + 2, a.rel_extent,
+                               has_bias && (c + 2) * 32 + 31 >= bl && (c + 2) * 32 <= bh,
+                               bwin[c & 1]);
+          } else if (chunk_bias) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int d = bh - c * 32 - i;
+              if (d >= 0 && d < a.rel_extent)
+                x[i] += bf16_bits_to_float(__ldg(rel_row + d)) * kLog2e;
+            }
+          }
+          if (has_mask) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int col = c * 32 + i;
+              if (col < cl || col >= ch) x[i] = -INFINITY;
+            }
+          }
+          float m0 = x[0], m1 = x[1];
+#pragma unroll
+          for (int i = 2; i < 30; i += 4) {
+            m0 = fmax3(m0, x[i], x[i + 1]);
+            m1 = fmax3(m1, x[i + 2], x[i + 3]);
+          }
+          m0 = fmax3(m0, x[30], x[31]);
+          mx = fmax3(mx, m0, m1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(x[i]);
+          __syncwarp();  // reconverge after the per-row branches: tcgen05.st is .aligned
+          tmem_st32(t_s + c * 32, r);
+        }
+        tmem_wait_st();
+        const float m_new = fmaxf(m_run, mx);
+        float alpha = 1.f;
+        bool need_rescale = false;
+        if (j == j0) {
+          m_run = m_new;
+        } else if (m_new > m_run + kRescaleThreshold) {
+          alpha = fast_exp2(m_run - m_new);
+          need_rescale = true;
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
+        __syncwarp();
+        // Pass 2: p = 2^(x - m), P (bf16) over the first 64 columns of S.
+        uint32_t rr[2][32];
+        tmem_ld32(t_s, rr[0]);
+        tmem_wait_ld();
+        uint64_t acc[4] = {0, 0, 0, 0};
+        const uint64_t neg2 = f2_pack(-m_use, -m_use);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < 3) tmem_ld32(t_s + (c + 1) * 32, rr[(c + 1) & 1]);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float y0, y1;
+            f2_unpack(f2_add(f2_pack(__uint_as_float(rr[c & 1][2 * i]),
+                                     __uint_as_float(rr[c & 1][2 * i + 1])),
+                             neg2),
+                      y0, y1);
+            const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
+            acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
+            pk[i] = pack_bf16x2(p0, p1);
+          }
+          tmem_st16(t_s + c * 16, pk);
+          if (c < 3) tmem_wait_ld();
+        }
+        const uint64_t a01 = f2_add(acc[0], acc[1]), a23 = f2_add(acc[2], acc[3]);
+        float u0, u1;
+        f2_unpack(f2_add(a01, a23), u0, u1);
+        l_run += u0 + u1;
+        // The previous product of this half is complete (its commit preceded this S's).
+        if (__any_sync(0xffffffffu, need_rescale)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(t_o + c * 32, o);
+          }
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->p_full[s]);
+    }
+    // Epilogue: normalised fp32 partial and its log2-sum-exp; a half without a key tile, or a row
+    // that takes no part, writes the log2-sum-exp -inf only.
+    const bool any = n_kv > j0;  // warpgroup-uniform
+    const bool seen = ok && any && me.on && !(l_run == 0.f);  // a NaN sum stays one
+    const int tile = tile0 + (kKeyPair ? 0 : s);
+    const int bl = row / a.group;
+    const int b = tile * a.seqs_per_tile + bl;
+    const bool stored = bl < a.seqs_per_tile && b < a.batch;
+    const int h = kvh * a.group + (row - bl * a.group);
+    if (stored && IFA4_DBG_CHECK(a.status, part < a.parts && h < a.n_heads))
+      a.ws_lse[(static_cast<long long>(part) * a.batch + b) * a.n_heads + h] =
+          seen ? m_run + __log2f(l_run) : -INFINITY;
+    if (any && ok && mbar_wait_warp(&bars->o_full[s], 0, ab)) {
+      tc_fence_after();
+      const float inv_l = seen ? 1.f / l_run : 0.f;
+      // every MMA that reads Q precedes the product o_full[s] waits for: its tile is free
+      uint8_t* stage = smem + kSmemQ + s * kTile;
+#pragma unroll
+      for (int hp = 0; hp < 2; ++hp) {
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t o[32];
+          tmem_ld32(t_o + hp * 64 + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const int g = c * 8 + v;  // 16-byte granule (4 floats) of the 256-byte segment
+            uint4* dst = reinterpret_cast<uint4*>(stage + (g >> 3) * kHalf + row * 128 +
+                                                  (((g & 7) ^ (row & 7)) << 4));
+            *dst = make_uint4(__float_as_uint(__uint_as_float(o[4 * v]) * inv_l),
+                              __float_as_uint(__uint_as_float(o[4 * v + 1]) * inv_l),
+                              __float_as_uint(__uint_as_float(o[4 * v + 2]) * inv_l),
+                              __float_as_uint(__uint_as_float(o[4 * v + 3]) * inv_l));
+          }
+        }
+        __syncwarp();
+        const int wrow0 = (warp & 3) * 32;
+        const int g = lane & 15;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int r = wrow0 + 2 * i + (lane >> 4);
+          const int rb = r / a.group;
+          const int ob = tile * a.seqs_per_tile + rb;
+          if (rb < a.seqs_per_tile && ob < a.batch) {
+            const uint4 val = *reinterpret_cast<const uint4*>(
+                stage + (g >> 3) * kHalf + r * 128 + (((g & 7) ^ (r & 7)) << 4));
+            const int oh = kvh * a.group + (r - rb * a.group);
+            if (IFA4_DBG_CHECK(a.status, part < a.parts && oh < a.n_heads))
+              *reinterpret_cast<uint4*>(
+                  a.ws_o + ((static_cast<long long>(part) * a.batch + ob) * a.n_heads + oh) * 128 +
+                  hp * 64 + g * 4) = val;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tbase, kTmemCols);
+  }
+}
+
+// Merge of a row's partials (a.parts of the prefix, a.own_parts of its own keys), one warp per
+// (sequence, head): weights 2^(lse_i - max lse); lanes own 4 of the 128 dims.
+__global__ void __launch_bounds__(128)
+    shared_prefix_combine_kernel(const __grid_constant__ SharedPrefixKernelArgs a) {
+  const long long w = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const long long rows = static_cast<long long>(a.batch) * a.n_heads;
+  if (w >= rows) return;
+  const int b = static_cast<int>(w / a.n_heads);
+  const int h = static_cast<int>(w - static_cast<long long>(b) * a.n_heads);
+  const int n = a.parts + a.own_parts;
+  // partial i: the prefix's first, then the own keys'
+  auto lse_of = [&](int i) {
+    return i < a.parts ? a.ws_lse[i * rows + w] : a.own_lse[w * a.own_parts + (i - a.parts)];
+  };
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 32) m = fmaxf(m, lse_of(i));
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  float wsum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (m != -INFINITY) {
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float mine = i0 + lane < n ? fast_exp2(lse_of(i0 + lane) - m) : 0.f;
+      const int cnt = min(32, n - i0);
+#pragma unroll 4
+      for (int i = 0; i < cnt; ++i) {
+        const float wt = __shfl_sync(0xffffffffu, mine, i);
+        if (wt == 0.f) continue;  // no weight: its output may never have been written
+        const int p = i0 + i;
+        const float* src = p < a.parts ? a.ws_o + (p * rows + w) * 128
+                                       : a.own_o + (w * a.own_parts + (p - a.parts)) * 128;
+        const float4 o = reinterpret_cast<const float4*>(src)[lane];
+        wsum += wt;
+        acc.x += wt * o.x;
+        acc.y += wt * o.y;
+        acc.z += wt * o.z;
+        acc.w += wt * o.w;
+      }
+    }
+  }
+  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  uint2 packed;
+  packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+  packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(a.out + b * a.out_st + h * a.out_sh + lane * 4) = packed;
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[h * a.lse_sh + b * a.lse_st] =
+        wsum > 0.f ? (m + __log2f(wsum)) * 0.6931471805599453f : -INFINITY;
+}
+
+}  // namespace prefix
+
+cudaError_t launch_shared_prefix_sm100(const SharedPrefixKernelArgs& args, const CUtensorMap& tm_q,
+                                       const CUtensorMap& tm_k, const CUtensorMap& tm_v,
+                                       cudaStream_t stream) {
+  static std::atomic<bool> attr_rows[64], attr_keys[64];
+  cudaError_t e = set_smem_limit_once(prefix::shared_prefix_kernel<false>, prefix::kSmemAlloc,
+                                      attr_rows);
+  if (e == cudaSuccess)
+    e = set_smem_limit_once(prefix::shared_prefix_kernel<true>, prefix::kSmemAlloc, attr_keys);
+  if (e != cudaSuccess) return e;
+  const int tiles = (args.batch + args.seqs_per_tile - 1) / args.seqs_per_tile;
+  const dim3 grid(args.key_pair ? tiles : (tiles + 1) / 2, args.kv_heads, args.splits);
+  if (args.key_pair)
+    prefix::shared_prefix_kernel<true>
+        <<<grid, prefix::kThreads, prefix::kSmemAlloc, stream>>>(args, tm_q, tm_k, tm_v);
+  else
+    prefix::shared_prefix_kernel<false>
+        <<<grid, prefix::kThreads, prefix::kSmemAlloc, stream>>>(args, tm_q, tm_k, tm_v);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_shared_prefix_combine_sm100(const SharedPrefixKernelArgs& args,
+                                               cudaStream_t stream) {
+  const long long rows = static_cast<long long>(args.batch) * args.n_heads;
+  prefix::shared_prefix_combine_kernel<<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
+      args);
+  return cudaGetLastError();
+}
+
+}  // namespace ifa4

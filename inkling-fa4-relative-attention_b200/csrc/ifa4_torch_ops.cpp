@@ -1,4 +1,5 @@
-// torch operators over the C ABI: inkling_fa4::prefill_ and inkling_fa4::decode_.
+// torch operators over the C ABI: inkling_fa4::prefill_, decode_, decode_shared_prefix_,
+// qk_norm_rope_, qk_norm_rope_backward_, kv_append_, bucket_bias_ and bucket_bias_backward_.
 //
 // The Python package checks its arguments (the reference's call surface and error messages) and
 // then calls one of these operators, which fills the IFA4 parameter block from the tensors'
@@ -99,14 +100,14 @@ int64_t prefill_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   return ifa4_prefill_launch_ws(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream);
 }
 
-int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                  const at::Tensor& rel, const at::Tensor& out, const at::Tensor& cu_q,
-                  const at::Tensor& cu_k, const c10::optional<at::Tensor>& lse,
-                  const c10::optional<at::Tensor>& block_table,
-                  const c10::optional<at::Tensor>& workspace, int64_t rel_extent, bool causal,
-                  int64_t window_left, int64_t causal_align, int64_t max_seqlen_k,
-                  double softmax_scale, int64_t num_splits, int64_t chunk_len) {
-  const c10::cuda::CUDAGuard guard(q.device());
+IFA4DecodeParams decode_params(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& rel, const at::Tensor& out,
+                               const at::Tensor& cu_q, const at::Tensor& cu_k,
+                               const c10::optional<at::Tensor>& lse,
+                               const c10::optional<at::Tensor>& block_table, int64_t rel_extent,
+                               bool causal, int64_t window_left, int64_t causal_align,
+                               int64_t max_seqlen_k, double softmax_scale, int64_t num_splits,
+                               int64_t chunk_len) {
   // the decode parameter block starts with the same fields as the prefill one
   IFA4PrefillParams common{};
   fill_common(&common, q, k, v, rel, out, cu_q, cu_k, block_table, rel_extent, causal,
@@ -155,6 +156,20 @@ int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   p.softmax_scale = static_cast<float>(softmax_scale);
   p.num_splits = static_cast<int32_t>(num_splits);
   p.chunk_len = static_cast<int32_t>(chunk_len);
+  return p;
+}
+
+int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                  const at::Tensor& rel, const at::Tensor& out, const at::Tensor& cu_q,
+                  const at::Tensor& cu_k, const c10::optional<at::Tensor>& lse,
+                  const c10::optional<at::Tensor>& block_table,
+                  const c10::optional<at::Tensor>& workspace, int64_t rel_extent, bool causal,
+                  int64_t window_left, int64_t causal_align, int64_t max_seqlen_k,
+                  double softmax_scale, int64_t num_splits, int64_t chunk_len) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const IFA4DecodeParams p = decode_params(q, k, v, rel, out, cu_q, cu_k, lse, block_table,
+                                           rel_extent, causal, window_left, causal_align,
+                                           max_seqlen_k, softmax_scale, num_splits, chunk_len);
   void* stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
   size_t need = 0;
   int rc = ifa4_decode_workspace_size(&p, &need, nullptr, nullptr);
@@ -170,6 +185,229 @@ int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             need > 0 ? static_cast<size_t>(ws.nbytes()) : 0, stream);
 }
 
+int64_t decode_shared_prefix_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                const at::Tensor& rel, const at::Tensor& out,
+                                const at::Tensor& cu_q, const at::Tensor& cu_k,
+                                const c10::optional<at::Tensor>& lse,
+                                const at::Tensor& block_table,
+                                const c10::optional<at::Tensor>& workspace, int64_t rel_extent,
+                                int64_t window_left, int64_t max_seqlen_k, double softmax_scale,
+                                int64_t num_splits, int64_t chunk_len, int64_t shared_prefix_len,
+                                int64_t prefix_splits) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  IFA4SharedPrefixParams p{};
+  p.decode = decode_params(q, k, v, rel, out, cu_q, cu_k, lse, block_table, rel_extent, true,
+                           window_left, IFA4_ALIGN_BOTTOM_RIGHT, max_seqlen_k, softmax_scale,
+                           num_splits, chunk_len);
+  p.shared_prefix_len = static_cast<int32_t>(shared_prefix_len);
+  p.prefix_splits = static_cast<int32_t>(prefix_splits);
+  void* stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  size_t need = 0;
+  int rc = ifa4_decode_shared_prefix_workspace_size(&p, &need);
+  if (rc) return rc;
+  at::Tensor ws;
+  if (need > 0) {
+    if (workspace.has_value() && static_cast<size_t>(workspace->nbytes()) >= need)
+      ws = *workspace;
+    else
+      ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+  }
+  return ifa4_decode_shared_prefix_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream);
+}
+
+const void* ptr_or_null(const c10::optional<at::Tensor>& t) {
+  return t.has_value() ? t->data_ptr() : nullptr;
+}
+
+// The fields the norm-and-rotation parameter blocks share.  eps < 0: no norm.
+template <class P>
+void fill_norm_rope(P* p, const c10::optional<at::Tensor>& q_weight,
+                    const c10::optional<at::Tensor>& k_weight,
+                    const c10::optional<at::Tensor>& inv_freq,
+                    const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
+                    int64_t total_q, int64_t heads, int64_t kv_heads, bool interleaved,
+                    double eps) {
+  p->q_weight = ptr_or_null(q_weight);
+  p->k_weight = ptr_or_null(k_weight);
+  p->inv_freq = ptr_or_null(inv_freq);
+  p->cu_seqlens_q = static_cast<const int32_t*>(ptr_or_null(cu_q));
+  p->cu_seqlens_k = static_cast<const int32_t*>(ptr_or_null(cu_k));
+  p->total_q = total_q;
+  p->batch = cu_q.has_value() ? static_cast<int32_t>(cu_q->numel() - 1) : 1;
+  p->n_heads = static_cast<int32_t>(heads);
+  p->kv_heads = static_cast<int32_t>(kv_heads);
+  p->head_dim = 128;
+  p->rotary_dim = inv_freq.has_value() ? static_cast<int32_t>(2 * inv_freq->numel()) : 0;
+  p->interleaved = interleaved;
+  p->normalize = eps >= 0;
+  const c10::optional<at::Tensor>& w = q_weight.has_value() ? q_weight : k_weight;
+  p->weight_dtype = w.has_value() && w->scalar_type() == at::kFloat ? IFA4_WEIGHT_F32
+                                                                    : IFA4_WEIGHT_BF16;
+  p->inv_freq_f32 = inv_freq.has_value() && inv_freq->scalar_type() == at::kFloat;
+  p->dtype = IFA4_DTYPE_BF16;
+  p->eps = eps >= 0 ? static_cast<float>(eps) : 0.f;
+}
+
+int64_t qk_norm_rope_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_out,
+                        const at::Tensor& k_out, const c10::optional<at::Tensor>& q_weight,
+                        const c10::optional<at::Tensor>& k_weight,
+                        const c10::optional<at::Tensor>& inv_freq,
+                        const c10::optional<at::Tensor>& cu_q,
+                        const c10::optional<at::Tensor>& cu_k, bool interleaved, double eps) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  IFA4QkNormRopeParams p{};
+  fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, q.size(0), q.size(1), k.size(1),
+                 interleaved, eps);
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.q_out = q_out.data_ptr();
+  p.k_out = k_out.data_ptr();
+  p.q_stride_t = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.k_stride_t = k.stride(0);
+  p.k_stride_h = k.stride(1);
+  p.q_out_stride_t = q_out.stride(0);
+  p.q_out_stride_h = q_out.stride(1);
+  p.k_out_stride_t = k_out.stride(0);
+  p.k_out_stride_h = k_out.stride(1);
+  p.zero_padding = 1;
+  return ifa4_qk_norm_rope_launch(&p,
+                                  c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+}
+
+int64_t qk_norm_rope_backward_op(
+    const at::Tensor& dq_out, const at::Tensor& dk_out, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& dq, const at::Tensor& dk, const c10::optional<at::Tensor>& q_weight,
+    const c10::optional<at::Tensor>& k_weight, const c10::optional<at::Tensor>& dq_weight,
+    const c10::optional<at::Tensor>& dk_weight, const c10::optional<at::Tensor>& inv_freq,
+    const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
+    bool interleaved, double eps) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  IFA4QkNormRopeBackwardParams p{};
+  fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, q.size(0), q.size(1), k.size(1),
+                 interleaved, eps);
+  p.dq_out = dq_out.data_ptr();
+  p.dk_out = dk_out.data_ptr();
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.dq = dq.data_ptr();
+  p.dk = dk.data_ptr();
+  p.dq_weight = dq_weight.has_value() ? dq_weight->data_ptr() : nullptr;
+  p.dk_weight = dk_weight.has_value() ? dk_weight->data_ptr() : nullptr;
+  p.dq_out_stride_t = dq_out.stride(0);
+  p.dq_out_stride_h = dq_out.stride(1);
+  p.dk_out_stride_t = dk_out.stride(0);
+  p.dk_out_stride_h = dk_out.stride(1);
+  p.q_stride_t = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.k_stride_t = k.stride(0);
+  p.k_stride_h = k.stride(1);
+  p.dq_stride_t = dq.stride(0);
+  p.dq_stride_h = dq.stride(1);
+  p.dk_stride_t = dk.stride(0);
+  p.dk_stride_h = dk.stride(1);
+  size_t need = 0;
+  const int rc = ifa4_qk_norm_rope_backward_workspace_size(&p, &need);
+  if (rc) return rc;
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+  return ifa4_qk_norm_rope_backward_launch(
+      &p, need > 0 ? ws.data_ptr() : nullptr, need,
+      c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+}
+
+int64_t kv_append_op(const c10::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
+                     const c10::optional<at::Tensor>& q_out, const at::Tensor& k_cache,
+                     const at::Tensor& v_cache, const c10::optional<at::Tensor>& q_weight,
+                     const c10::optional<at::Tensor>& k_weight,
+                     const c10::optional<at::Tensor>& inv_freq, const at::Tensor& cu_q,
+                     const at::Tensor& cu_k, const at::Tensor& block_table, bool interleaved,
+                     double eps, bool zero_padding) {
+  const c10::cuda::CUDAGuard guard(k.device());
+  IFA4KvAppendParams p{};
+  fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, k.size(0),
+                 q.has_value() ? q->size(1) : 0, k.size(1), interleaved, eps);
+  if (q.has_value()) {
+    p.q = q->data_ptr();
+    p.q_out = q_out->data_ptr();
+    p.q_stride_t = q->stride(0);
+    p.q_stride_h = q->stride(1);
+    p.q_out_stride_t = q_out->stride(0);
+    p.q_out_stride_h = q_out->stride(1);
+  }
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_cache = k_cache.data_ptr();
+  p.v_cache = v_cache.data_ptr();
+  p.k_stride_t = k.stride(0);
+  p.k_stride_h = k.stride(1);
+  p.v_stride_t = v.stride(0);
+  p.v_stride_h = v.stride(1);
+  p.k_stride_page = k_cache.stride(0);
+  p.k_cache_stride_t = k_cache.stride(1);
+  p.k_cache_stride_h = k_cache.stride(2);
+  p.v_stride_page = v_cache.stride(0);
+  p.v_cache_stride_t = v_cache.stride(1);
+  p.v_cache_stride_h = v_cache.stride(2);
+  p.block_table = static_cast<const int32_t*>(block_table.data_ptr());
+  p.block_table_stride = block_table.stride(0);
+  p.zero_padding = zero_padding;
+  p.page_size = static_cast<int32_t>(k_cache.size(1));
+  p.num_pages = static_cast<int32_t>(k_cache.size(0));
+  p.table_width = static_cast<int32_t>(block_table.size(1));
+  return ifa4_kv_append_launch(&p, c10::cuda::getCurrentCUDAStream(k.device().index()).stream());
+}
+
+int32_t weight_dtype(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat ? IFA4_WEIGHT_F32 : IFA4_WEIGHT_BF16;
+}
+
+int64_t bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, const at::Tensor& rel) {
+  const c10::cuda::CUDAGuard guard(table.device());
+  IFA4BucketBiasParams p{};
+  p.table = table.data_ptr();
+  p.starts = static_cast<const int32_t*>(starts.data_ptr());
+  p.rel = rel.data_ptr();
+  p.table_stride_b = table.stride(0);
+  p.table_stride_h = table.stride(1);
+  p.rel_stride_h = rel.stride(0);
+  p.n_heads = static_cast<int32_t>(table.size(1));
+  p.rel_extent = static_cast<int32_t>(rel.size(1));
+  p.buckets = static_cast<int32_t>(starts.numel());
+  p.weight_dtype = weight_dtype(table);
+  return ifa4_bucket_bias_launch(
+      &p, c10::cuda::getCurrentCUDAStream(table.device().index()).stream());
+}
+
+int64_t bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts,
+                                const at::Tensor& dtable,
+                                const c10::optional<at::Tensor>& cu_q) {
+  const c10::cuda::CUDAGuard guard(drel.device());
+  IFA4BucketBiasBackwardParams p{};
+  p.drel = drel.data_ptr();
+  p.starts = static_cast<const int32_t*>(starts.data_ptr());
+  p.cu_seqlens_q = static_cast<const int32_t*>(ptr_or_null(cu_q));
+  p.dtable = dtable.data_ptr();
+  p.drel_stride_t = drel.stride(0);
+  p.drel_stride_h = drel.stride(1);
+  p.dtable_stride_b = dtable.stride(0);
+  p.dtable_stride_h = dtable.stride(1);
+  p.total_q = drel.size(0);
+  p.batch = cu_q.has_value() ? static_cast<int32_t>(cu_q->numel() - 1) : 0;
+  p.n_heads = static_cast<int32_t>(drel.size(1));
+  p.rel_extent = static_cast<int32_t>(drel.size(2));
+  p.buckets = static_cast<int32_t>(starts.numel());
+  p.weight_dtype = weight_dtype(dtable);
+  size_t need = 0;
+  const int rc = ifa4_bucket_bias_backward_workspace_size(&p, &need);
+  if (rc) return rc;
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, drel.options().dtype(at::kByte));
+  return ifa4_bucket_bias_backward_launch(
+      &p, need > 0 ? ws.data_ptr() : nullptr, need,
+      c10::cuda::getCurrentCUDAStream(drel.device().index()).stream());
+}
+
 }  // namespace
 
 TORCH_LIBRARY(inkling_fa4, m) {
@@ -181,9 +419,32 @@ TORCH_LIBRARY(inkling_fa4, m) {
         "Tensor cu_k, Tensor(b!)? lse, Tensor? block_table, Tensor? workspace, int rel_extent, "
         "bool causal, int window_left, int causal_align, int max_seqlen_k, float softmax_scale, "
         "int num_splits, int chunk_len) -> int");
+  m.def("decode_shared_prefix_(Tensor q, Tensor k, Tensor v, Tensor rel, Tensor(a!) out, "
+        "Tensor cu_q, Tensor cu_k, Tensor(b!)? lse, Tensor block_table, Tensor? workspace, "
+        "int rel_extent, int window_left, int max_seqlen_k, float softmax_scale, int num_splits, "
+        "int chunk_len, int shared_prefix_len, int prefix_splits) -> int");
+  m.def("qk_norm_rope_(Tensor q, Tensor k, Tensor(a!) q_out, Tensor(b!) k_out, Tensor? q_weight, "
+        "Tensor? k_weight, Tensor? inv_freq, Tensor? cu_q, Tensor? cu_k, bool interleaved, "
+        "float eps) -> int");
+  m.def("qk_norm_rope_backward_(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor(a!) dq, "
+        "Tensor(b!) dk, Tensor? q_weight, Tensor? k_weight, Tensor(c!)? dq_weight, "
+        "Tensor(d!)? dk_weight, Tensor? inv_freq, Tensor? cu_q, Tensor? cu_k, bool interleaved, "
+        "float eps) -> int");
+  m.def("kv_append_(Tensor? q, Tensor k, Tensor v, Tensor(a!)? q_out, Tensor(b!) k_cache, "
+        "Tensor(c!) v_cache, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor cu_q, "
+        "Tensor cu_k, Tensor block_table, bool interleaved, float eps, bool zero_padding) -> int");
+  m.def("bucket_bias_(Tensor table, Tensor starts, Tensor(a!) rel) -> int");
+  m.def("bucket_bias_backward_(Tensor drel, Tensor starts, Tensor(a!) dtable, Tensor? cu_q) "
+        "-> int");
 }
 
 TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("prefill_", &prefill_op);
   m.impl("decode_", &decode_op);
+  m.impl("decode_shared_prefix_", &decode_shared_prefix_op);
+  m.impl("qk_norm_rope_", &qk_norm_rope_op);
+  m.impl("qk_norm_rope_backward_", &qk_norm_rope_backward_op);
+  m.impl("kv_append_", &kv_append_op);
+  m.impl("bucket_bias_", &bucket_bias_op);
+  m.impl("bucket_bias_backward_", &bucket_bias_backward_op);
 }

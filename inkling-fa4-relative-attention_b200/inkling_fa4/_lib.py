@@ -23,7 +23,10 @@ STATUS_DEBUG_BOUNDS = 64
 IFA4_ALIGN_REFERENCE = 0
 IFA4_ALIGN_BOTTOM_RIGHT = 1
 IFA4_DTYPE_BF16 = 0
-ABI_VERSION = 7
+IFA4_WEIGHT_BF16 = 0
+IFA4_WEIGHT_F32 = 1
+MAX_BUCKETS = 1024
+ABI_VERSION = 8
 MAX_OUT_PEERS = 7
 MAX_KV_SPLITS = 16
 NOALLOC_DECODE_SCRATCH_BYTES = 16 * 1024 * 1024
@@ -38,6 +41,15 @@ EXPORTED_SYMBOLS = (
     "ifa4_backward_launch",
     "ifa4_backward_workspace_size",
     "ifa4_rel_logits_launch",
+    "ifa4_decode_shared_prefix_launch",
+    "ifa4_decode_shared_prefix_workspace_size",
+    "ifa4_qk_norm_rope_launch",
+    "ifa4_qk_norm_rope_backward_launch",
+    "ifa4_qk_norm_rope_backward_workspace_size",
+    "ifa4_kv_append_launch",
+    "ifa4_bucket_bias_launch",
+    "ifa4_bucket_bias_backward_launch",
+    "ifa4_bucket_bias_backward_workspace_size",
     "ifa4_read_device_status",
     "ifa4_selftest_bounded_wait",
     "ifa4_measure_read_stream",
@@ -120,6 +132,64 @@ class RelLogitsParams(ctypes.Structure):
         [("alpha", ctypes.c_float), ("nf", ctypes.c_float)]
 
 
+class SharedPrefixParams(ctypes.Structure):
+    """Mirror of ``IFA4SharedPrefixParams``."""
+    _fields_ = [("decode", DecodeParams), ("shared_prefix_len", ctypes.c_int32),
+                ("prefix_splits", ctypes.c_int32)]
+
+
+_NORM_ROPE_SIZES = ("batch", "n_heads", "kv_heads", "head_dim", "rotary_dim", "interleaved",
+                    "normalize", "weight_dtype", "inv_freq_f32")
+
+
+class QkNormRopeParams(ctypes.Structure):
+    """Mirror of ``IFA4QkNormRopeParams``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight",
+                                               "inv_freq", "cu_seqlens_q", "cu_seqlens_k")] + \
+        _pairs("q", "k", "q_out", "k_out") + [("total_q", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in _NORM_ROPE_SIZES + ("zero_padding", "dtype")] + \
+        [("eps", ctypes.c_float)]
+
+
+class QkNormRopeBackwardParams(ctypes.Structure):
+    """Mirror of ``IFA4QkNormRopeBackwardParams``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dq_out", "dk_out", "q", "k", "dq", "dk",
+                                               "q_weight", "k_weight", "dq_weight", "dk_weight",
+                                               "inv_freq", "cu_seqlens_q", "cu_seqlens_k")] + \
+        _pairs("dq_out", "dk_out", "q", "k", "dq", "dk") + [("total_q", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in _NORM_ROPE_SIZES + ("dtype",)] + [("eps", ctypes.c_float)]
+
+
+class KvAppendParams(ctypes.Structure):
+    """Mirror of ``IFA4KvAppendParams``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache",
+                                               "q_weight", "k_weight", "inv_freq",
+                                               "cu_seqlens_q", "cu_seqlens_k", "block_table")] + \
+        _pairs("q", "k", "v", "q_out") + \
+        [(n, ctypes.c_int64) for n in ("k_stride_page", "k_cache_stride_t", "k_cache_stride_h",
+                                       "v_stride_page", "v_cache_stride_t", "v_cache_stride_h",
+                                       "block_table_stride", "total_q")] + \
+        [(n, ctypes.c_int32) for n in _NORM_ROPE_SIZES + ("zero_padding", "dtype", "page_size",
+                                                          "num_pages", "table_width")] + \
+        [("eps", ctypes.c_float)]
+
+
+class BucketBiasParams(ctypes.Structure):
+    """Mirror of ``IFA4BucketBiasParams``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "starts", "rel")] + \
+        [(n, ctypes.c_int64) for n in ("table_stride_b", "table_stride_h", "rel_stride_h")] + \
+        [(n, ctypes.c_int32) for n in ("n_heads", "rel_extent", "buckets", "weight_dtype")]
+
+
+class BucketBiasBackwardParams(ctypes.Structure):
+    """Mirror of ``IFA4BucketBiasBackwardParams``."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("drel", "starts", "cu_seqlens_q", "dtable")] + \
+        [(n, ctypes.c_int64) for n in ("drel_stride_t", "drel_stride_h", "dtable_stride_b",
+                                       "dtable_stride_h", "total_q")] + \
+        [(n, ctypes.c_int32) for n in ("batch", "n_heads", "rel_extent", "buckets",
+                                       "weight_dtype")]
+
+
 class Ifa4Error(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"inkling_fa4 error {code}: {message}")
@@ -180,6 +250,16 @@ def lib() -> ctypes.CDLL:
     L.ifa4_backward_workspace_size.restype = ctypes.c_int
     L.ifa4_rel_logits_launch.argtypes = [ctypes.POINTER(RelLogitsParams), vp]
     L.ifa4_rel_logits_launch.restype = ctypes.c_int
+    for name, params in (("decode_shared_prefix", SharedPrefixParams),
+                         ("qk_norm_rope_backward", QkNormRopeBackwardParams),
+                         ("bucket_bias_backward", BucketBiasBackwardParams)):
+        launch, size = getattr(L, f"ifa4_{name}_launch"), getattr(L, f"ifa4_{name}_workspace_size")
+        launch.argtypes, launch.restype = [ctypes.POINTER(params), vp, sz, vp], ctypes.c_int
+        size.argtypes, size.restype = [ctypes.POINTER(params), ctypes.POINTER(sz)], ctypes.c_int
+    for name, params in (("qk_norm_rope", QkNormRopeParams), ("kv_append", KvAppendParams),
+                         ("bucket_bias", BucketBiasParams)):
+        launch = getattr(L, f"ifa4_{name}_launch")
+        launch.argtypes, launch.restype = [ctypes.POINTER(params), vp], ctypes.c_int
     L.ifa4_selftest_bounded_wait.argtypes = [ctypes.c_int64, vp]
     L.ifa4_selftest_bounded_wait.restype = ctypes.c_int
     L.ifa4_measure_read_stream.argtypes = [vp, sz, vp, vp]

@@ -28,7 +28,8 @@ OUT = os.path.join(PKG_DIR, "_lib", "libinkling_fa4.so")
 OUT_DEBUG = os.path.join(PKG_DIR, "_lib", "libinkling_fa4_debug.so")
 OUT_TORCH_OPS = os.path.join(PKG_DIR, "_lib", "libifa4_torch_ops.so")
 SOURCES = ["ifa4_capi.cu", "ifa4_prefill_sm100.cu", "ifa4_decode_sm100.cu", "ifa4_backward_sm100.cu",
-           "ifa4_rel_logits_sm100.cu"]
+           "ifa4_rel_logits_sm100.cu", "ifa4_qkv_sm100.cu", "ifa4_shared_prefix_sm100.cu",
+           "ifa4_bucket_bias_sm100.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -70,8 +71,8 @@ def build(verbose: bool = False, force: bool = False, debug: bool = False) -> st
 
 
 def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
-    """Compile ``csrc/ifa4_torch_ops.cpp`` (the torch operators inkling_fa4::prefill_ and
-    inkling_fa4::decode_ over the C ABI) with g++ against torch's headers and libraries, linked
+    """Compile ``csrc/ifa4_torch_ops.cpp`` (the torch operators inkling_fa4::prefill_,
+    inkling_fa4::decode_ and so on over the C ABI) with g++ against torch's headers and libraries, linked
     to the in-tree ``libinkling_fa4.so`` (found next to it at run time)."""
     import torch
     from torch.utils import cpp_extension
