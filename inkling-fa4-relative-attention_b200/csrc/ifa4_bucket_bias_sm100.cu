@@ -125,12 +125,13 @@ __global__ void __launch_bounds__(kThreads) bucket_grad_kernel(const __grid_cons
       for (int i = 0; i < 8; ++i) x[i].add(s);
       p += 8 * step;
     }
-    for (; t < t1; t += a.lanes) {
-      Vec<V> x;
-      x.load(p);
-      x.add(s);
-      p += step;
-    }
+    Vec<V> x[7];  // the last tokens, all loads in flight as well
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (t + i * a.lanes < t1) x[i].load(p + i * step);
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (t + i * a.lanes < t1) x[i].add(s);
   }
   if (lane < a.lanes) {
 #pragma unroll

@@ -1115,13 +1115,15 @@ int validate_norm_rope(const P* p, const char* what) {
   return IFA4_OK;
 }
 
-// A token's rows are shared by several warps when there are few tokens: about 32 warps per SM in
-// all, two rows (a half-warp each) at least.
+// A token's rows are shared by several warps when there are few tokens: about 64 units per SM in
+// all (four rounds of the resident warps), four rows (what a warp does at once) at least.
 int token_parts(int64_t tokens, int rows, int sms) {
-  const int64_t want = (32LL * sms + tokens - 1) / tokens;
-  const int most = (rows + 1) / 2;
+  const int64_t want = (64LL * sms + tokens - 1) / tokens;
+  const int most = (rows + 3) / 4;
   return static_cast<int>(want < 1 ? 1 : (want > most ? most : want));
 }
+
+int round4(int n) { return (n + 3) / 4 * 4; }
 
 template <class P>
 void fill_qkv(const P* p, ifa4::QkvKernelArgs* a) {
@@ -1157,7 +1159,7 @@ int launch_qkv(const char* what, ifa4::QkvKernelArgs* a, int64_t tokens, int row
   int rc = sm_count(&sms);
   if (rc) return rc;
   const int parts = token_parts(tokens, rows, sms);
-  a->rows_per_part = (rows + parts - 1) / parts;
+  a->rows_per_part = round4((rows + parts - 1) / parts);
   a->parts = (rows + a->rows_per_part - 1) / a->rows_per_part;
   a->units = tokens * a->parts;
   cudaError_t e = ifa4::launch_qkv_rows_sm100(*a, sms, static_cast<cudaStream_t>(stream));
@@ -1198,7 +1200,7 @@ int plan_qk_backward(const IFA4QkNormRopeBackwardParams* p, int* parts, int* blo
   const int rows = p->n_heads > p->kv_heads ? p->n_heads : p->kv_heads;
   *parts = p->total_q > 0 && rows > 0 ? token_parts(p->total_q, rows, sms) : 1;
   const int64_t want = (p->total_q * *parts + ifa4::kQkvBackwardWarps - 1) / ifa4::kQkvBackwardWarps;
-  const int64_t cap = static_cast<int64_t>(sms) * 6;  // one resident wave
+  const int64_t cap = static_cast<int64_t>(sms) * ifa4::kQkvBackwardBlocksPerSm;
   *blocks = static_cast<int>(want < 1 ? 1 : (want < cap ? want : cap));
   *bytes = p->dq_weight != nullptr || p->dk_weight != nullptr
                ? static_cast<size_t>(*blocks) * 256 * sizeof(float) : 0;
@@ -1292,8 +1294,8 @@ int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, voi
   a.weight_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
   a.inv_freq_f32 = p->inv_freq_f32 ? 1 : 0;
   a.parts = parts;
-  a.q_per_part = (p->n_heads + parts - 1) / parts;
-  a.k_per_part = (p->kv_heads + parts - 1) / parts;
+  a.q_per_part = round4((p->n_heads + parts - 1) / parts);
+  a.k_per_part = round4((p->kv_heads + parts - 1) / parts);
   a.eps = p->eps;
   cudaError_t e = ifa4::launch_qkv_backward_sm100(a, blocks, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_backward launch");

@@ -10,9 +10,12 @@
 // where the angle does) and no position, however far, loses accuracy to range reduction; its top
 // 32 bits go to sincospif (error below 2e-7 rad).
 //
-// Work split: a unit is one token and a part of its heads; one warp per unit, a half-warp per
-// head row (16 lanes x 8 dims, 16-byte loads and stores), four row pairs in flight.  The lane's
-// angles depend on the token only, so they are computed once per unit and stay in registers.
+// Work split: a unit is one token and a part of its heads; one warp per unit, eight lanes per head
+// row (16 dims each, so four rows run at once and a row's sum takes three shuffles), loaded and
+// stored in 16-byte pieces.  A lane's dims are chosen so that both elements of its eight pairs are
+// its own: 8l.. and rotary_dim / 2 + 8l.. for the two halves, 16l.. interleaved.  The angles
+// depend on the token only: 64 lanes' worth are computed once per unit (two a lane), handed round
+// through shared memory and kept in registers for all rows.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -27,6 +30,7 @@ namespace qkv {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr unsigned kFull = 0xffffffffu;
+static_assert(kWarps == kQkvBackwardWarps, "unit planning in the C ABI layer");
 
 enum { kRotNone = 0, kRotHalf = 1, kRotPairs = 2 };
 
@@ -40,24 +44,28 @@ __device__ __forceinline__ uint4 ldg_v4(const void* p) {
   return r;
 }
 
-__device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
+// Eight bf16 <-> four packed fp32 pairs.
+__device__ __forceinline__ void unpack8(const uint4& v, uint64_t* x) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i)
+    x[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                    pack_bf16x2(x[6], x[7]));
+__device__ __forceinline__ uint32_t pack2(uint64_t x) {
+  float lo, hi;
+  f2_unpack(x, lo, hi);
+  return pack_bf16x2(lo, hi);
 }
 
-// Sum over the 16 lanes of a half-warp.
-__device__ __forceinline__ float half_sum(float v) {
+__device__ __forceinline__ uint4 pack8(const uint64_t* x) {
+  return make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
+}
+
+// Sum over the eight lanes of a row.
+__device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
-  for (int m = 8; m > 0; m >>= 1) v += __shfl_xor_sync(kFull, v, m);
+  for (int m = 4; m > 0; m >>= 1) v += __shfl_xor_sync(kFull, v, m);
   return v;
 }
 
@@ -77,6 +85,10 @@ __device__ __forceinline__ Where locate(const int32_t* cu_q, const int32_t* cu_k
   w.inside = true;
   if (cu_q == nullptr) return w;
   int lo = 0, n = batch;
+  if (t < batch && __ldg(cu_q + t) <= t && t < __ldg(cu_q + t + 1)) {
+    lo = static_cast<int>(t);  // one token a sequence up to here (decode): no search
+    n = 1;
+  }
   while (n > 1) {
     const int step = (n + 31) >> 5;
     const int i = lane * step;
@@ -111,71 +123,88 @@ __device__ __forceinline__ void angle_cos_sin(unsigned long long f, long long po
   sincospif(static_cast<float>(hi) * (1.0f / 2147483648.0f), &s, &c);
 }
 
-// The lane's part of a rotation: lane l (of 16) holds dims 8l .. 8l + 7.
-//   kRotHalf:  with n = rotary_dim / 16, lanes [0, n) hold the first elements of the pairs and
-//              lanes [n, 2n) the second ones; out = own * cos + partner * sin with the sign of
-//              the sine folded in; other lanes pass through.
-//   kRotPairs: both elements of four pairs are the lane's own.
+// The lane's part of a rotation.  Lane l (of 8) of a row holds 16 dims: 8 from a_off on and 8 from
+// b_off on, as packed pairs x[0..3] and x[4..7].  Lanes below rotary_dim / 16 are turned, with the
+// pairs 8l .. 8l + 7; the others hold the dims behind rotary_dim and pass them through.
 template <int kRot>
 struct Rotation {
-  static constexpr int kPairs = kRot == kRotHalf ? 8 : (kRot == kRotPairs ? 4 : 1);
-  unsigned long long f[kPairs];
-  float c[kPairs], s[kPairs];
-  int partner;
-  bool turned;   // the lane holds rotated dims
-  bool first;    // ... first elements (kRotHalf)
+  unsigned long long f[2];  // frequencies of pairs lane and lane + 32 (the ones this lane computes)
+  uint64_t c[4], s[4], ns[4];  // cosines, sines and their negatives of the lane's own pairs
+  int a_off, b_off;
+  bool turned;
 
-  __device__ __forceinline__ void init(const void* inv_freq, int f32, int rotary_dim, int l) {
-    if (kRot == kRotNone) return;
-    const int n = kRot == kRotHalf ? rotary_dim / 16 : rotary_dim / 8;
-    first = l < n;
-    turned = kRot == kRotHalf ? l < 2 * n : l < n;
-    partner = kRot == kRotHalf && turned ? (first ? l + n : l - n) : l;
-    const int i0 = kRot == kRotHalf ? 8 * (first ? l : l - n) : 4 * l;
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) f[i] = turned ? turn_fraction(inv_freq, f32, i0 + i) : 0ull;
-  }
-
-  // dir = 1: forward; -1: the transposed rotation (gradients).
-  __device__ __forceinline__ void at(long long pos, float dir) {
-    if (kRot == kRotNone) return;
-#pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      c[i] = 1.f;
-      s[i] = 0.f;
-    }
-    if (turned) {
-      const float sign = kRot == kRotHalf && first ? -dir : dir;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        angle_cos_sin(f[i], pos, c[i], s[i]);
-        s[i] *= sign;
-      }
-    }
-  }
-
-  // Whole warp.
-  __device__ __forceinline__ void apply(float (&y)[8]) const {
+  __device__ __forceinline__ void init(const void* inv_freq, int f32, int rotary_dim, int lane) {
+    const int l = lane & 7;
+    turned = kRot != kRotNone && l < rotary_dim / 16;
+    a_off = 16 * l;
+    b_off = 16 * l + 8;
     if (kRot == kRotHalf) {
-      float p[8];
+      a_off = turned ? 8 * l : rotary_dim + 16 * (l - rotary_dim / 16);
+      b_off = turned ? rotary_dim / 2 + 8 * l : a_off + 8;
+    }
+    if (kRot != kRotNone) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = __shfl_sync(kFull, y[i], partner, 16);
-      if (turned) {
+      for (int i = 0; i < 2; ++i)
+        f[i] = lane + 32 * i < rotary_dim / 2 ? turn_fraction(inv_freq, f32, lane + 32 * i) : 0ull;
+    }
+  }
+
+  // Whole warp; `table` is the warp's own shared memory.
+  __device__ __forceinline__ void at(long long pos, int lane, float2* table) {
+    if (kRot == kRotNone) return;
+    __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * c[i] + p[i] * s[i];
+    for (int i = 0; i < 2; ++i) {
+      float2 cs;
+      angle_cos_sin(f[i], pos, cs.x, cs.y);
+      table[lane + 32 * i] = cs;
+    }
+    __syncwarp();
+    const float4* mine = reinterpret_cast<const float4*>(table + 8 * (lane & 7));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = mine[i];  // cos, sin, cos, sin
+      c[i] = f2_pack(v.x, v.z);
+      s[i] = f2_pack(v.y, v.w);
+      ns[i] = f2_pack(-v.y, -v.w);
+    }
+  }
+
+  // Forward, or (kBack) the transposed rotation.
+  template <bool kBack>
+  __device__ __forceinline__ void apply(uint64_t (&x)[8]) const {
+    if (kRot == kRotNone || !turned) return;
+    if (kRot == kRotHalf) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t a = x[i], b = x[4 + i];
+        x[i] = f2_fma(a, c[i], f2_mul(b, kBack ? s[i] : ns[i]));
+        x[4 + i] = f2_fma(b, c[i], f2_mul(a, kBack ? ns[i] : s[i]));
       }
-    } else if (kRot == kRotPairs) {
-      if (turned) {
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = y[2 * i], b = y[2 * i + 1];
-          y[2 * i] = a * c[i] - b * s[i];
-          y[2 * i + 1] = b * c[i] + a * s[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        float a, b, c0, c1, s0, s1;
+        f2_unpack(x[i], a, b);
+        f2_unpack(c[i >> 1], c0, c1);
+        f2_unpack(s[i >> 1], s0, s1);
+        const float ci = (i & 1) ? c1 : c0;
+        const float si = kBack ? -((i & 1) ? s1 : s0) : ((i & 1) ? s1 : s0);
+        x[i] = f2_pack(a * ci - b * si, b * ci + a * si);
       }
     }
   }
 };
+
+// The lane's 16 weights as packed pairs.
+__device__ __forceinline__ void lane_weights(const float* w, int a_off, int b_off, uint64_t (&o)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 v = *reinterpret_cast<const float4*>(w + (i < 2 ? a_off + 4 * i : b_off + 4 * (i - 2)));
+    o[2 * i] = f2_pack(v.x, v.y);
+    o[2 * i + 1] = f2_pack(v.z, v.w);
+  }
+}
 
 // Weight vectors of q and k as fp32 in shared memory (ones when absent).
 __device__ __forceinline__ float load_weight(const void* w, int f32, int i) {
@@ -188,88 +217,108 @@ template <int kRot, bool kAppend>
 __global__ void __launch_bounds__(kThreads) qkv_rows_kernel(const __grid_constant__
                                                                 QkvKernelArgs a) {
   __shared__ __align__(16) float ws[2][128];
+  __shared__ __align__(16) float2 angles[kWarps][64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int l = lane & 15, hw = lane >> 4;
+  const int oct = lane >> 3;
+  Rotation<kRot> rot;
+  rot.init(a.inv_freq, a.inv_freq_f32, a.rotary_dim, lane);
   if (a.normalize) {
     ws[0][threadIdx.x] = load_weight(a.q_weight, a.weight_f32, threadIdx.x);
     ws[1][threadIdx.x] = load_weight(a.k_weight, a.weight_f32, threadIdx.x);
   }
-  Rotation<kRot> rot;
-  rot.init(a.inv_freq, a.inv_freq_f32, a.rotary_dim, l);
   __syncthreads();
 
   const int rows = a.n_heads + a.kv_heads + (kAppend ? a.kv_heads : 0);
+  const int v_rows = a.n_heads + a.kv_heads;  // first V row
   const long long step = static_cast<long long>(gridDim.x) * kWarps;
   for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp; u < a.units; u += step) {
     const long long t = a.parts == 1 ? u : u / a.parts;
     const int r0 = static_cast<int>(u - t * a.parts) * a.rows_per_part;
     const int r1 = min(rows, r0 + a.rows_per_part);
-    auto source = [&](int r) -> const uint16_t* {
-      if (r < a.n_heads) return a.q + t * a.q_st + r * a.q_sh;
-      r -= a.n_heads;
-      if (!kAppend || r < a.kv_heads) return a.k + t * a.k_st + r * a.k_sh;
-      return a.v + t * a.v_st + (r - a.kv_heads) * a.v_sh;
-    };
-    uint4 x[4];
-    auto load4 = [&](int r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ri = r + 2 * i + hw;
-        x[i] = ri < r1 ? ldg_v4(source(ri) + 8 * l) : make_uint4(0u, 0u, 0u, 0u);
+    const uint16_t* const qt = a.q + t * a.q_st;
+    const uint16_t* const kt = a.k + t * a.k_st;
+    const uint16_t* const vt = kAppend ? a.v + t * a.v_st : nullptr;
+    uint4 xa[2], xb[2];  // two steps of four rows in flight
+    auto load = [&](int r, uint4& va, uint4& vb) {
+      const int ri = r + oct;
+      va = vb = make_uint4(0u, 0u, 0u, 0u);
+      if (ri < r1) {
+        const uint16_t* p = ri < a.n_heads ? qt + ri * a.q_sh : kt + (ri - a.n_heads) * a.k_sh;
+        if (kAppend && ri >= v_rows) p = vt + (ri - v_rows) * a.v_sh;
+        va = ldg_v4(p + rot.a_off);
+        vb = ldg_v4(p + rot.b_off);
       }
     };
-    load4(r0);
+    load(r0, xa[0], xb[0]);
+    load(r0 + 4, xa[1], xb[1]);
     const Where w = locate(a.cu_q, a.cu_k, a.batch, t, lane);
-    rot.at(w.pos, 1.f);
-    long long k_slot = -1, v_slot = -1;  // element offset of the token's slot in the caches
-    if (kAppend && w.inside && w.pos >= 0 && (w.pos >> a.page_shift) < a.table_width) {
-      const int page = __ldg(a.block_table + static_cast<long long>(w.b) * a.bt_stride +
-                             (w.pos >> a.page_shift));
-      if (page >= 0 && page < a.num_pages) {
-        const long long in_page = w.pos & ((1ll << a.page_shift) - 1);
-        k_slot = page * a.kc_sp + in_page * a.kc_st;
-        v_slot = page * a.vc_sp + in_page * a.vc_st;
-      }
+    int page = -1;
+    if (kAppend && w.inside && w.pos >= 0 && (w.pos >> a.page_shift) < a.table_width)
+      page = __ldg(a.block_table + static_cast<long long>(w.b) * a.bt_stride +
+                   (w.pos >> a.page_shift));
+    rot.at(w.pos, lane, angles[warp]);
+    uint16_t* kc = nullptr;  // the token's slots in the caches
+    uint16_t* vc = nullptr;
+    if (kAppend && page >= 0 && page < a.num_pages) {
+      const long long in_page = w.pos & ((1ll << a.page_shift) - 1);
+      kc = a.k_cache + page * a.kc_sp + in_page * a.kc_st;
+      vc = a.v_cache + page * a.vc_sp + in_page * a.vc_st;
     }
-    for (int r = r0; r < r1; r += 8) {
-      if (r > r0) load4(r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ri = r + 2 * i + hw;
-        const bool is_q = ri < a.n_heads;
-        const bool is_v = kAppend && ri >= a.n_heads + a.kv_heads;
-        float y[8];
-        unpack8(x[i], y);
+    uint16_t* const qo = w.inside || a.zero_padding ? a.q_out + t * a.qo_st : nullptr;
+    uint16_t* const ko = kAppend ? kc
+                                 : (w.inside || a.zero_padding ? a.k_out + t * a.ko_st : nullptr);
+    const long long ko_sh = kAppend ? a.kc_sh : a.ko_sh;
+
+    auto finish = [&](int r, uint4 va, uint4 vb) {
+      const int ri = r + oct;
+      const bool is_q = ri < a.n_heads;
+      if (!kAppend || r < v_rows) {  // (warp-uniform) not V rows only
+        uint64_t x[8];
+        unpack8(va, x);
+        unpack8(vb, x + 4);
         if (a.normalize) {
-          float ss = 0.f;
+          uint64_t s2 = f2_mul(x[0], x[0]), s3 = f2_mul(x[1], x[1]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss += y[e] * y[e];
-          const float rn = rsqrtf(half_sum(ss) * (1.f / 128.f) + a.eps);
-          const float4* wv = reinterpret_cast<const float4*>(ws[is_q ? 0 : 1] + 8 * l);
-          const float4 wa = wv[0], wb = wv[1];
-          const float wf[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+          for (int i = 2; i < 8; i += 2) {
+            s2 = f2_fma(x[i], x[i], s2);
+            s3 = f2_fma(x[i + 1], x[i + 1], s3);
+          }
+          float lo, hi;
+          f2_unpack(f2_add(s2, s3), lo, hi);
+          const float rn = rsqrtf(row_sum(lo + hi) * (1.f / 128.f) + a.eps);
+          const uint64_t rn2 = f2_pack(rn, rn);
+          uint64_t wt[8];
+          lane_weights(ws[is_q ? 0 : 1], rot.a_off, rot.b_off, wt);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= rn * wf[e];
+          for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], f2_mul(wt[i], rn2));
         }
-        rot.apply(y);
-        uint4 out = is_v ? x[i] : pack8(y);
-        uint16_t* dst = nullptr;
-        if (ri < r1) {
-          if (is_q) {
-            dst = a.q_out + t * a.qo_st + ri * a.qo_sh;
-          } else if (!kAppend) {
-            dst = a.k_out + t * a.ko_st + (ri - a.n_heads) * a.ko_sh;
-          } else if (is_v) {
-            dst = v_slot >= 0 ? a.v_cache + v_slot + (ri - a.n_heads - a.kv_heads) * a.vc_sh : nullptr;
-          } else {
-            dst = k_slot >= 0 ? a.k_cache + k_slot + (ri - a.n_heads) * a.kc_sh : nullptr;
-          }
-          if (!w.inside) {  // behind the last sequence: zeros, or left as it was
-            out = make_uint4(0u, 0u, 0u, 0u);
-            if (!a.zero_padding) dst = nullptr;
-          }
+        rot.template apply<false>(x);
+        if (!kAppend || ri < v_rows) {
+          va = pack8(x);
+          vb = pack8(x + 4);
         }
-        if (dst != nullptr) *reinterpret_cast<uint4*>(dst + 8 * l) = out;
+      }
+      if (!w.inside) va = vb = make_uint4(0u, 0u, 0u, 0u);
+      uint16_t* dst = is_q ? qo : ko;
+      long long off = is_q ? ri * a.qo_sh : (ri - a.n_heads) * ko_sh;
+      if (kAppend && ri >= v_rows) {
+        dst = vc;
+        off = (ri - v_rows) * a.vc_sh;
+      }
+      if (ri < r1 && dst != nullptr) {
+        *reinterpret_cast<uint4*>(dst + off + rot.a_off) = va;
+        *reinterpret_cast<uint4*>(dst + off + rot.b_off) = vb;
+      }
+    };
+    for (int r = r0; r < r1; r += 8) {
+      uint4 va = xa[0], vb = xb[0];
+      if (r + 8 < r1) load(r + 8, xa[0], xb[0]);
+      finish(r, va, vb);
+      if (r + 4 < r1) {
+        va = xa[1];
+        vb = xb[1];
+        if (r + 12 < r1) load(r + 12, xa[1], xb[1]);
+        finish(r + 4, va, vb);
       }
     }
   }
@@ -278,97 +327,109 @@ __global__ void __launch_bounds__(kThreads) qkv_rows_kernel(const __grid_constan
 // Gradients.  With g = R^T dout, xhat = x * r, r = rsqrt(mean x^2 + eps):
 //   dw = sum over tokens and heads of g * xhat
 //   dx = r * (g w - xhat * mean(g w xhat)) = r * g w - x * r^3 * mean(g w x)
-// r is recomputed from x (nothing is saved by the forward).  Each half-warp keeps the sums of dw
-// of its rows in registers; a block adds its half-warps in a fixed order and writes one partial
-// per weight vector, and qkv_weight_grad_kernel adds the blocks' partials, again in a fixed
-// order: no atomics, the same result every time.
+// r is recomputed from x (nothing is saved by the forward).  Each lane keeps the sums of dw of
+// its dims and rows in registers; a block adds its rows' lanes in a fixed order and writes one
+// partial per weight vector, and qkv_weight_grad_kernel adds the blocks' partials, again in a
+// fixed order: no atomics, the same result every time.
 template <int kRot>
-__global__ void __launch_bounds__(kThreads) qkv_backward_kernel(const __grid_constant__
+__global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm) qkv_backward_kernel(const __grid_constant__
                                                                     QkvBackwardKernelArgs a) {
   __shared__ __align__(16) float ws[2][128];
-  __shared__ float part[2][2 * kWarps][128];
+  __shared__ __align__(16) float2 angles[kWarps][64];
+  __shared__ __align__(16) float part[4 * kWarps][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int l = lane & 15, hw = lane >> 4;
+  const int oct = lane >> 3;
+  Rotation<kRot> rot;
+  rot.init(a.inv_freq, a.inv_freq_f32, a.rotary_dim, lane);
   ws[0][threadIdx.x] = load_weight(a.q_weight, a.weight_f32, threadIdx.x);
   ws[1][threadIdx.x] = load_weight(a.k_weight, a.weight_f32, threadIdx.x);
-  Rotation<kRot> rot;
-  rot.init(a.inv_freq, a.inv_freq_f32, a.rotary_dim, l);
   __syncthreads();
-  float acc[2][8];
+  uint64_t acc[2][8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[0][e] = acc[1][e] = 0.f;
+  for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0ull;
 
   const long long step = static_cast<long long>(gridDim.x) * kWarps;
   for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp; u < a.units; u += step) {
     const long long t = a.parts == 1 ? u : u / a.parts;
     const int part_i = static_cast<int>(u - t * a.parts);
     const Where w = locate(a.cu_q, a.cu_k, a.batch, t, lane);
-    rot.at(w.pos, -1.f);
+    rot.at(w.pos, lane, angles[warp]);
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
       const int heads = kind == 0 ? a.n_heads : a.kv_heads;
       const int per = kind == 0 ? a.q_per_part : a.k_per_part;
       const int r0 = part_i * per, r1 = min(heads, r0 + per);
-      const uint16_t* xb = kind == 0 ? a.q + t * a.q_st : a.k + t * a.k_st;
-      const uint16_t* gb = kind == 0 ? a.dq_out + t * a.dqo_st : a.dk_out + t * a.dko_st;
-      uint16_t* ob = kind == 0 ? a.dq + t * a.dq_st : a.dk + t * a.dk_st;
+      const uint16_t* const xt = kind == 0 ? a.q + t * a.q_st : a.k + t * a.k_st;
+      const uint16_t* const gt = kind == 0 ? a.dq_out + t * a.dqo_st : a.dk_out + t * a.dko_st;
+      uint16_t* const ot = kind == 0 ? a.dq + t * a.dq_st : a.dk + t * a.dk_st;
       const long long x_sh = kind == 0 ? a.q_sh : a.k_sh, g_sh = kind == 0 ? a.dqo_sh : a.dko_sh;
       const long long o_sh = kind == 0 ? a.dq_sh : a.dk_sh;
-      const float4* wv = reinterpret_cast<const float4*>(ws[kind] + 8 * l);
-      const float4 wa = wv[0], wb = wv[1];
-      const float wf[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-      for (int r = r0; r < r1; r += 4) {
-        uint4 xr[2], gr[2];
+      uint4 raw[4];  // x, dout of the next four rows
+      auto load = [&](int r) {
+        const int ri = r + oct;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int ri = r + 2 * i + hw;
-          const bool on = ri < r1 && w.inside;
-          xr[i] = on ? ldg_v4(xb + ri * x_sh + 8 * l) : make_uint4(0u, 0u, 0u, 0u);
-          gr[i] = on ? ldg_v4(gb + ri * g_sh + 8 * l) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 4; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (ri < r1 && w.inside) {
+          raw[0] = ldg_v4(xt + ri * x_sh + rot.a_off);
+          raw[1] = ldg_v4(xt + ri * x_sh + rot.b_off);
+          raw[2] = ldg_v4(gt + ri * g_sh + rot.a_off);
+          raw[3] = ldg_v4(gt + ri * g_sh + rot.b_off);
         }
+      };
+      if (r0 < r1) load(r0);
+      for (int r = r0; r < r1; r += 4) {
+        const int ri = r + oct;
+        const bool on = ri < r1 && w.inside;  // a row that is none has r = rsqrt(eps), maybe inf
+        uint64_t x[8], g[8];
+        unpack8(raw[0], x);
+        unpack8(raw[1], x + 4);
+        unpack8(raw[2], g);
+        unpack8(raw[3], g + 4);
+        if (r + 4 < r1) load(r + 4);
+        rot.template apply<true>(g);
+        if (a.normalize) {
+          uint64_t wt[8], gw[8];
+          lane_weights(ws[kind], rot.a_off, rot.b_off, wt);
+          uint64_t ss = 0ull, dot = 0ull;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int ri = r + 2 * i + hw;
-          const bool on = ri < r1 && w.inside;  // a row that is none has r = rsqrt(eps), maybe inf
-          float x[8], g[8];
-          unpack8(xr[i], x);
-          unpack8(gr[i], g);
-          rot.apply(g);
-          if (a.normalize) {
-            float ss = 0.f, dot = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              ss += x[e] * x[e];
-              dot += g[e] * wf[e] * x[e];
-            }
-            ss = half_sum(ss);
-            dot = half_sum(dot);
-            const float rn = rsqrtf(ss * (1.f / 128.f) + a.eps);
-            const float back = dot * (1.f / 128.f) * rn * rn;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (on) acc[kind][e] += g[e] * (x[e] * rn);
-              g[e] = rn * (g[e] * wf[e] - x[e] * back);
-            }
+          for (int i = 0; i < 8; ++i) {
+            gw[i] = f2_mul(g[i], wt[i]);
+            ss = f2_fma(x[i], x[i], ss);
+            dot = f2_fma(gw[i], x[i], dot);
           }
-          if (ri < r1)
-            *reinterpret_cast<uint4*>(ob + ri * o_sh + 8 * l) =
-                on ? pack8(g) : make_uint4(0u, 0u, 0u, 0u);
+          float lo, hi, dlo, dhi;
+          f2_unpack(ss, lo, hi);
+          f2_unpack(dot, dlo, dhi);
+          const float rn = rsqrtf(row_sum(lo + hi) * (1.f / 128.f) + a.eps);
+          const float back = -(row_sum(dlo + dhi) * (1.f / 128.f)) * rn * rn * rn;
+          const uint64_t rn2 = f2_pack(rn, rn), back2 = f2_pack(back, back);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (on) acc[kind][i] = f2_fma(g[i], f2_mul(x[i], rn2), acc[kind][i]);
+            g[i] = f2_fma(x[i], back2, f2_mul(gw[i], rn2));
+          }
+        }
+        if (ri < r1) {
+          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.a_off) = on ? pack8(g) : z;
+          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.b_off) = on ? pack8(g + 4) : z;
         }
       }
     }
   }
   if (a.partial == nullptr) return;
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) part[kind][2 * warp + hw][8 * l + e] = acc[kind][e];
-  __syncthreads();
-#pragma unroll
   for (int kind = 0; kind < 2; ++kind) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int dim = (i < 4 ? rot.a_off + 2 * i : rot.b_off + 2 * (i - 4));
+      *reinterpret_cast<uint64_t*>(&part[4 * warp + oct][dim]) = acc[kind][i];
+    }
+    __syncthreads();
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2 * kWarps; ++i) s += part[kind][i][threadIdx.x];
+    for (int i = 0; i < 4 * kWarps; ++i) s += part[i][threadIdx.x];
     a.partial[(static_cast<long long>(blockIdx.x) * 2 + kind) * 128 + threadIdx.x] = s;
   }
 }
@@ -400,25 +461,46 @@ __global__ void __launch_bounds__(1024) qkv_weight_grad_kernel(const float* part
 
 }  // namespace qkv
 
-cudaError_t launch_qkv_rows_sm100(const QkvKernelArgs& args, int sms, cudaStream_t stream) {
-  const long long want = (args.units + qkv::kWarps - 1) / qkv::kWarps;
-  const long long cap = static_cast<long long>(sms) * 16;
-  const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
-  const int rot = args.rotary_dim == 0 ? qkv::kRotNone
-                                       : (args.interleaved ? qkv::kRotPairs : qkv::kRotHalf);
-#define IFA4_QKV(R, A)                                                     \
-  if (rot == R && (args.k_cache != nullptr) == A) {                        \
-    qkv::qkv_rows_kernel<R, A><<<grid, qkv::kThreads, 0, stream>>>(args);  \
-    return cudaGetLastError();                                             \
+// Blocks of one kernel that are resident on the current device at a time.
+template <typename K>
+static cudaError_t resident_blocks(K kernel, int sms, std::atomic<int> (&cache)[64], int* out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  int n = cache[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, qkv::kThreads, 0);
+    if (e != cudaSuccess) return e;
+    if (n < 1) n = 1;
+    cache[dev].store(n, std::memory_order_release);
   }
-  IFA4_QKV(qkv::kRotNone, false)
-  IFA4_QKV(qkv::kRotNone, true)
-  IFA4_QKV(qkv::kRotHalf, false)
-  IFA4_QKV(qkv::kRotHalf, true)
-  IFA4_QKV(qkv::kRotPairs, false)
-  IFA4_QKV(qkv::kRotPairs, true)
-#undef IFA4_QKV
-  return cudaErrorInvalidValue;
+  *out = n * sms;
+  return cudaSuccess;
+}
+
+template <int kRot, bool kAppend>
+static cudaError_t launch_rows(const QkvKernelArgs& args, int sms, cudaStream_t stream) {
+  static std::atomic<int> cache[64];
+  int cap = 0;
+  cudaError_t e = resident_blocks(qkv::qkv_rows_kernel<kRot, kAppend>, sms, cache, &cap);
+  if (e != cudaSuccess) return e;
+  const long long want = (args.units + qkv::kWarps - 1) / qkv::kWarps;
+  const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
+  qkv::qkv_rows_kernel<kRot, kAppend><<<grid, qkv::kThreads, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_qkv_rows_sm100(const QkvKernelArgs& args, int sms, cudaStream_t stream) {
+  const bool append = args.k_cache != nullptr;
+  if (args.rotary_dim == 0)
+    return append ? launch_rows<qkv::kRotNone, true>(args, sms, stream)
+                  : launch_rows<qkv::kRotNone, false>(args, sms, stream);
+  if (args.interleaved)
+    return append ? launch_rows<qkv::kRotPairs, true>(args, sms, stream)
+                  : launch_rows<qkv::kRotPairs, false>(args, sms, stream);
+  return append ? launch_rows<qkv::kRotHalf, true>(args, sms, stream)
+                : launch_rows<qkv::kRotHalf, false>(args, sms, stream);
 }
 
 cudaError_t launch_qkv_backward_sm100(const QkvBackwardKernelArgs& args, int blocks,
