@@ -238,7 +238,7 @@ cudaError_t launch_qkv_rows_sm100(const QkvKernelArgs& args, int sms, cudaStream
 cudaError_t launch_qkv_backward_sm100(const QkvBackwardKernelArgs& args, int blocks,
                                       cudaStream_t stream);
 constexpr int kQkvBackwardWarps = 4;        // warps of a block of the backward kernel
-constexpr int kQkvBackwardBlocksPerSm = 3;  // resident ones
+constexpr int kQkvBackwardBlocksPerSm = 4;  // resident ones
 
 // Bias by distance buckets and its gradient.
 constexpr int kMaxBuckets = 1024;

@@ -14,8 +14,16 @@
 // row (16 dims each, so four rows run at once and a row's sum takes three shuffles), loaded and
 // stored in 16-byte pieces.  A lane's dims are chosen so that both elements of its eight pairs are
 // its own: 8l.. and rotary_dim / 2 + 8l.. for the two halves, 16l.. interleaved.  The angles
-// depend on the token only: 64 lanes' worth are computed once per unit (two a lane), handed round
+// depend on the token only: they are computed once per unit (two pairs a lane), handed round
 // through shared memory and kept in registers for all rows.
+//
+// HBM bound in bytes, but close to the issue rate: a quad of rows takes about 270 instructions, 68 %
+// of the issue slots at 32k tokens x 40 heads (671 MB in 123 us, 5.4 TB/s; backward 1007 MB in
+// 197 us, 5.1 TB/s).  Measured and slower there: half a warp per row with the pairs exchanged by
+// shuffles 187 us (backward 293); equal runs of quads per warp over token borders 130; whole tokens
+// in turn with an evenly cut rest 157 (its cursors cost more than the balance gives); one loop per
+// kind of row (spills) 174; the next token streamed by cp.async into shared memory, 8 warps per SM,
+// 126 (interleaved pairs 191 instead of 133, append 114 instead of 83, backward 215).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -214,8 +222,8 @@ __device__ __forceinline__ float load_weight(const void* w, int f32, int i) {
 }
 
 template <int kRot, bool kAppend>
-__global__ void __launch_bounds__(kThreads) qkv_rows_kernel(const __grid_constant__
-                                                                QkvKernelArgs a) {
+__global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
+    qkv_rows_kernel(const __grid_constant__ QkvKernelArgs a) {
   __shared__ __align__(16) float ws[2][128];
   __shared__ __align__(16) float2 angles[kWarps][64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -332,8 +340,8 @@ __global__ void __launch_bounds__(kThreads) qkv_rows_kernel(const __grid_constan
 // partial per weight vector, and qkv_weight_grad_kernel adds the blocks' partials, again in a
 // fixed order: no atomics, the same result every time.
 template <int kRot>
-__global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm) qkv_backward_kernel(const __grid_constant__
-                                                                    QkvBackwardKernelArgs a) {
+__global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
+    qkv_backward_kernel(const __grid_constant__ QkvBackwardKernelArgs a) {
   __shared__ __align__(16) float ws[2][128];
   __shared__ __align__(16) float2 angles[kWarps][64];
   __shared__ __align__(16) float part[4 * kWarps][128];

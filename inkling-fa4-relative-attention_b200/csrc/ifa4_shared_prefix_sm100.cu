@@ -360,14 +360,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool has_bias = me.on && bl <= 127;
       // rows that take no part are never read back: they need no mask
       const bool has_mask = me.on && (cl > 0 || ch < kBN);
-      const bool warp_bias = __any_sync(0xffffffffu, has_bias);
-      uint32_t bwin[2][20];
-      if (a.bias_vec && warp_bias) {
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc)
-          load_bias_window(rel_row, bh, cc, a.rel_extent,
-                           has_bias && cc * 32 + 31 >= bl && cc * 32 <= bh, bwin[cc]);
-      }
       if (!(ok = mbar_wait_warp(&bars->s_full[s], pc & 1, ab))) break;
       ++pc;
       tc_fence_after();
@@ -417,52 +409,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!done) {
-        // Pass 1: the logits (scaled, biased, masked) replace S in TMEM; their row max.
+        // The row's 128 logits (scaled, biased, masked) in registers, their max, P.
+        uint32_t x[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
+        tmem_wait_ld();
         float mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(t_s + c * 32, r);
-          tmem_wait_ld();
-          float x[32];
+          float y[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * a.scale_log2;
+          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(x[c][i]) * a.scale_log2;
           const bool chunk_bias = has_bias && c * 32 + 31 >= bl && c * 32 <= bh;
           if (a.bias_vec) {
-            if (__any_sync(0xffffffffu, chunk_bias)) add_bias_window(bwin[c & 1], bh, c, x);
-            if (c < 2 && warp_bias)
-              load_bias_window(rel_row, bh, c + 2, a.rel_extent,
-                               has_bias && (c + 2) * 32 + 31 >= bl && (c + 2) * 32 <= bh,
-                               bwin[c & 1]);
+            if (__any_sync(0xffffffffu, chunk_bias)) {
+              uint32_t win[20];
+              load_bias_window(rel_row, bh, c, a.rel_extent, chunk_bias, win);
+              add_bias_window(win, bh, c, y);
+            }
           } else if (chunk_bias) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int d = bh - c * 32 - i;
               if (d >= 0 && d < a.rel_extent)
-                x[i] += bf16_bits_to_float(__ldg(rel_row + d)) * kLog2e;
+                y[i] += bf16_bits_to_float(__ldg(rel_row + d)) * kLog2e;
             }
           }
           if (has_mask) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int col = c * 32 + i;
-              if (col < cl || col >= ch) x[i] = -INFINITY;
+              if (col < cl || col >= ch) y[i] = -INFINITY;
             }
           }
-          float m0 = x[0], m1 = x[1];
+          float m0 = y[0], m1 = y[1];
 #pragma unroll
           for (int i = 2; i < 30; i += 4) {
-            m0 = fmax3(m0, x[i], x[i + 1]);
-            m1 = fmax3(m1, x[i + 2], x[i + 3]);
+            m0 = fmax3(m0, y[i], y[i + 1]);
+            m1 = fmax3(m1, y[i + 2], y[i + 3]);
           }
-          m0 = fmax3(m0, x[30], x[31]);
+          m0 = fmax3(m0, y[30], y[31]);
           mx = fmax3(mx, m0, m1);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(x[i]);
-          __syncwarp();  // reconverge after the per-row branches: tcgen05.st is .aligned
-          tmem_st32(t_s + c * 32, r);
+          for (int i = 0; i < 32; ++i) x[c][i] = __float_as_uint(y[i]);
         }
-        tmem_wait_st();
         const float m_new = fmaxf(m_run, mx);
         float alpha = 1.f;
         bool need_rescale = false;
@@ -475,30 +465,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_run = m_new;
         }
         const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
-        __syncwarp();
-        // Pass 2: p = 2^(x - m), P (bf16) over the first 64 columns of S.
-        uint32_t rr[2][32];
-        tmem_ld32(t_s, rr[0]);
-        tmem_wait_ld();
+        __syncwarp();  // reconverge after the per-row branches: tcgen05.st is .aligned
         uint64_t acc[4] = {0, 0, 0, 0};
         const uint64_t neg2 = f2_pack(-m_use, -m_use);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (c < 3) tmem_ld32(t_s + (c + 1) * 32, rr[(c + 1) & 1]);
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float y0, y1;
-            f2_unpack(f2_add(f2_pack(__uint_as_float(rr[c & 1][2 * i]),
-                                     __uint_as_float(rr[c & 1][2 * i + 1])),
+            f2_unpack(f2_add(f2_pack(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])),
                              neg2),
                       y0, y1);
             const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
             acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
             pk[i] = pack_bf16x2(p0, p1);
           }
-          tmem_st16(t_s + c * 16, pk);
-          if (c < 3) tmem_wait_ld();
+          tmem_st16(t_s + c * 16, pk);  // P (bf16) over the first 64 columns of S
         }
         const uint64_t a01 = f2_add(acc[0], acc[1]), a23 = f2_add(acc[2], acc[3]);
         float u0, u1;
@@ -588,20 +571,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Merge of a row's partials (a.parts of the prefix, a.own_parts of its own keys), one warp per
-// (sequence, head): weights 2^(lse_i - max lse); lanes own 4 of the 128 dims.
-__global__ void __launch_bounds__(128)
+// Merge of a row's partials (a.parts of the prefix, a.own_parts of its own keys): weights
+// 2^(lse_i - max lse).  A block per (sequence, head); its warps share the partials, lanes own 4 of
+// the 128 dims, and the warps' sums meet in shared memory.  One warp walking all partials of a row
+// took 20 us for 75 of them (33 sequences x 12 heads), this form TIME.
+constexpr int kCombineWarps = 4;
+__global__ void __launch_bounds__(32 * kCombineWarps)
     shared_prefix_combine_kernel(const __grid_constant__ SharedPrefixKernelArgs a) {
-  const long long w = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  __shared__ __align__(16) float4 sums[kCombineWarps][32];
+  __shared__ float weights[kCombineWarps];
+  const long long row = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long rows = static_cast<long long>(a.batch) * a.n_heads;
-  if (w >= rows) return;
-  const int b = static_cast<int>(w / a.n_heads);
-  const int h = static_cast<int>(w - static_cast<long long>(b) * a.n_heads);
+  const int b = static_cast<int>(row / a.n_heads);
+  const int h = static_cast<int>(row - static_cast<long long>(b) * a.n_heads);
   const int n = a.parts + a.own_parts;
   // partial i: the prefix's first, then the own keys'
   auto lse_of = [&](int i) {
-    return i < a.parts ? a.ws_lse[i * rows + w] : a.own_lse[w * a.own_parts + (i - a.parts)];
+    return i < a.parts ? a.ws_lse[i * rows + row] : a.own_lse[row * a.own_parts + (i - a.parts)];
   };
   float m = -INFINITY;
   for (int i = lane; i < n; i += 32) m = fmaxf(m, lse_of(i));
@@ -610,33 +597,51 @@ __global__ void __launch_bounds__(128)
   float wsum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (m != -INFINITY) {
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const float mine = i0 + lane < n ? fast_exp2(lse_of(i0 + lane) - m) : 0.f;
-      const int cnt = min(32, n - i0);
-#pragma unroll 4
-      for (int i = 0; i < cnt; ++i) {
-        const float wt = __shfl_sync(0xffffffffu, mine, i);
-        if (wt == 0.f) continue;  // no weight: its output may never have been written
-        const int p = i0 + i;
-        const float* src = p < a.parts ? a.ws_o + (p * rows + w) * 128
-                                       : a.own_o + (w * a.own_parts + (p - a.parts)) * 128;
-        const float4 o = reinterpret_cast<const float4*>(src)[lane];
-        wsum += wt;
-        acc.x += wt * o.x;
-        acc.y += wt * o.y;
-        acc.z += wt * o.z;
-        acc.w += wt * o.w;
+    for (int i0 = warp; i0 < n; i0 += 4 * kCombineWarps) {
+      float wt[4];
+      float4 o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int p = i0 + k * kCombineWarps;
+        wt[k] = p < n ? fast_exp2(lse_of(p) - m) : 0.f;
+        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (wt[k] != 0.f) {  // no weight: its output may never have been written
+          const float* src = p < a.parts ? a.ws_o + (p * rows + row) * 128
+                                         : a.own_o + (row * a.own_parts + (p - a.parts)) * 128;
+          o[k] = reinterpret_cast<const float4*>(src)[lane];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        wsum += wt[k];
+        acc.x += wt[k] * o[k].x;
+        acc.y += wt[k] * o[k].y;
+        acc.z += wt[k] * o[k].z;
+        acc.w += wt[k] * o[k].w;
       }
     }
   }
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  sums[warp][lane] = acc;
+  if (lane == 0) weights[warp] = wsum;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int k = 1; k < kCombineWarps; ++k) {
+    const float4 o = sums[k][lane];
+    acc.x += o.x;
+    acc.y += o.y;
+    acc.z += o.z;
+    acc.w += o.w;
+    wsum += weights[k];
+  }
+  const float inv = wsum > 0.f ? 1.f / wsum : (wsum == 0.f ? 0.f : wsum);  // NaN stays
   uint2 packed;
   packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
   packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
   *reinterpret_cast<uint2*>(a.out + b * a.out_st + h * a.out_sh + lane * 4) = packed;
   if (lane == 0 && a.lse != nullptr)
     a.lse[h * a.lse_sh + b * a.lse_st] =
-        wsum > 0.f ? (m + __log2f(wsum)) * 0.6931471805599453f : -INFINITY;
+        wsum == 0.f ? -INFINITY : (m + __log2f(wsum)) * 0.6931471805599453f;
 }
 
 }  // namespace prefix
@@ -664,8 +669,8 @@ cudaError_t launch_shared_prefix_sm100(const SharedPrefixKernelArgs& args, const
 cudaError_t launch_shared_prefix_combine_sm100(const SharedPrefixKernelArgs& args,
                                                cudaStream_t stream) {
   const long long rows = static_cast<long long>(args.batch) * args.n_heads;
-  prefix::shared_prefix_combine_kernel<<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(
-      args);
+  prefix::shared_prefix_combine_kernel<<<static_cast<unsigned>(rows), 32 * prefix::kCombineWarps, 0,
+                                         stream>>>(args);
   return cudaGetLastError();
 }
 
