@@ -409,50 +409,54 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!done) {
-        // The row's 128 logits (scaled, biased, masked) in registers, their max, P.
-        uint32_t x[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
-        tmem_wait_ld();
+        // Pass 1: the logits (scaled, biased, masked) replace S in TMEM; their row max.  The
+        // chunk loops stay rolled: a short launch runs them once or twice per CTA, and fetching
+        // unrolled code costs it more than the TMEM round trips.
         float mx = -INFINITY;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          float y[32];
+          uint32_t r[32];
+          tmem_ld32(t_s + c * 32, r);
+          tmem_wait_ld();
+          float x[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = __uint_as_float(x[c][i]) * a.scale_log2;
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]) * a.scale_log2;
           const bool chunk_bias = has_bias && c * 32 + 31 >= bl && c * 32 <= bh;
           if (a.bias_vec) {
             if (__any_sync(0xffffffffu, chunk_bias)) {
               uint32_t win[20];
               load_bias_window(rel_row, bh, c, a.rel_extent, chunk_bias, win);
-              add_bias_window(win, bh, c, y);
+              add_bias_window(win, bh, c, x);
             }
           } else if (chunk_bias) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int d = bh - c * 32 - i;
               if (d >= 0 && d < a.rel_extent)
-                y[i] += bf16_bits_to_float(__ldg(rel_row + d)) * kLog2e;
+                x[i] += bf16_bits_to_float(__ldg(rel_row + d)) * kLog2e;
             }
           }
           if (has_mask) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const int col = c * 32 + i;
-              if (col < cl || col >= ch) y[i] = -INFINITY;
+              if (col < cl || col >= ch) x[i] = -INFINITY;
             }
           }
-          float m0 = y[0], m1 = y[1];
+          float m0 = x[0], m1 = x[1];
 #pragma unroll
           for (int i = 2; i < 30; i += 4) {
-            m0 = fmax3(m0, y[i], y[i + 1]);
-            m1 = fmax3(m1, y[i + 2], y[i + 3]);
+            m0 = fmax3(m0, x[i], x[i + 1]);
+            m1 = fmax3(m1, x[i + 2], x[i + 3]);
           }
-          m0 = fmax3(m0, y[30], y[31]);
+          m0 = fmax3(m0, x[30], x[31]);
           mx = fmax3(mx, m0, m1);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[c][i] = __float_as_uint(y[i]);
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(x[i]);
+          __syncwarp();  // reconverge after the per-row branches: tcgen05.st is .aligned
+          tmem_st32(t_s + c * 32, r);
         }
+        tmem_wait_st();
         const float m_new = fmaxf(m_run, mx);
         float alpha = 1.f;
         bool need_rescale = false;
@@ -465,23 +469,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           m_run = m_new;
         }
         const float m_use = (m_run == -INFINITY) ? 0.f : m_run;
-        __syncwarp();  // reconverge after the per-row branches: tcgen05.st is .aligned
+        __syncwarp();
+        // Pass 2: p = 2^(x - m), P (bf16) over the first 64 columns of S.
         uint64_t acc[4] = {0, 0, 0, 0};
         const uint64_t neg2 = f2_pack(-m_use, -m_use);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tmem_ld32(t_s + c * 32, r);
+          tmem_wait_ld();
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float y0, y1;
-            f2_unpack(f2_add(f2_pack(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])),
-                             neg2),
+            f2_unpack(f2_add(f2_pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), neg2),
                       y0, y1);
             const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
             acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
             pk[i] = pack_bf16x2(p0, p1);
           }
-          tmem_st16(t_s + c * 16, pk);  // P (bf16) over the first 64 columns of S
+          tmem_st16(t_s + c * 16, pk);
         }
         const uint64_t a01 = f2_add(acc[0], acc[1]), a23 = f2_add(acc[2], acc[3]);
         float u0, u1;
@@ -489,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l_run += u0 + u1;
         // The previous product of this half is complete (its commit preceded this S's).
         if (__any_sync(0xffffffffu, need_rescale)) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[32];
             tmem_ld32(t_o + c * 32, o);
@@ -522,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv_l = seen ? 1.f / l_run : 0.f;
       // every MMA that reads Q precedes the product o_full[s] waits for: its tile is free
       uint8_t* stage = smem + kSmemQ + s * kTile;
-#pragma unroll
+#pragma unroll 1
       for (int hp = 0; hp < 2; ++hp) {
         __syncwarp();
 #pragma unroll
@@ -572,17 +579,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merge of a row's partials (a.parts of the prefix, a.own_parts of its own keys): weights
-// 2^(lse_i - max lse).  A block per (sequence, head); its warps share the partials, lanes own 4 of
-// the 128 dims, and the warps' sums meet in shared memory.  One warp walking all partials of a row
-// took 20 us for 75 of them (33 sequences x 12 heads), this form TIME.
-constexpr int kCombineWarps = 4;
-__global__ void __launch_bounds__(32 * kCombineWarps)
+// 2^(lse_i - max lse).  kWarps warps share a row's partials, four in flight each; lanes own 4 of the
+// 128 dims, and the warps' sums meet in shared memory.  One warp walking all partials of a row
+// took 20 us for 75 of them (33 sequences x 12 heads), four 5.8 us; with 10 of them (128 x 32
+// rows) one warp takes 6.4 us and four 8.2 us.
+constexpr int kCombineThreads = 128;
+template <int kWarps>
+__global__ void __launch_bounds__(kCombineThreads)
     shared_prefix_combine_kernel(const __grid_constant__ SharedPrefixKernelArgs a) {
-  __shared__ __align__(16) float4 sums[kCombineWarps][32];
-  __shared__ float weights[kCombineWarps];
-  const long long row = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ __align__(16) float4 sums[kCombineThreads / 32][32];
+  __shared__ float weights[kCombineThreads / 32];
+  const int warp = (threadIdx.x >> 5) % kWarps, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * (kCombineThreads / 32 / kWarps) +
+                        (threadIdx.x >> 5) / kWarps;
   const long long rows = static_cast<long long>(a.batch) * a.n_heads;
+  if (row >= rows) return;  // only with one warp per row
   const int b = static_cast<int>(row / a.n_heads);
   const int h = static_cast<int>(row - static_cast<long long>(b) * a.n_heads);
   const int n = a.parts + a.own_parts;
@@ -597,12 +608,12 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
   float wsum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (m != -INFINITY) {
-    for (int i0 = warp; i0 < n; i0 += 4 * kCombineWarps) {
+    for (int i0 = warp; i0 < n; i0 += 4 * kWarps) {
       float wt[4];
       float4 o[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int p = i0 + k * kCombineWarps;
+        const int p = i0 + k * kWarps;
         wt[k] = p < n ? fast_exp2(lse_of(p) - m) : 0.f;
         o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (wt[k] != 0.f) {  // no weight: its output may never have been written
@@ -621,18 +632,20 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
       }
     }
   }
-  sums[warp][lane] = acc;
-  if (lane == 0) weights[warp] = wsum;
-  __syncthreads();
-  if (warp != 0) return;
+  if (kWarps > 1) {
+    sums[warp][lane] = acc;
+    if (lane == 0) weights[warp] = wsum;
+    __syncthreads();
+    if (warp != 0) return;
 #pragma unroll
-  for (int k = 1; k < kCombineWarps; ++k) {
-    const float4 o = sums[k][lane];
-    acc.x += o.x;
-    acc.y += o.y;
-    acc.z += o.z;
-    acc.w += o.w;
-    wsum += weights[k];
+    for (int k = 1; k < kWarps; ++k) {
+      const float4 o = sums[k][lane];
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+      wsum += weights[k];
+    }
   }
   const float inv = wsum > 0.f ? 1.f / wsum : (wsum == 0.f ? 0.f : wsum);  // NaN stays
   uint2 packed;
@@ -669,8 +682,13 @@ cudaError_t launch_shared_prefix_sm100(const SharedPrefixKernelArgs& args, const
 cudaError_t launch_shared_prefix_combine_sm100(const SharedPrefixKernelArgs& args,
                                                cudaStream_t stream) {
   const long long rows = static_cast<long long>(args.batch) * args.n_heads;
-  prefix::shared_prefix_combine_kernel<<<static_cast<unsigned>(rows), 32 * prefix::kCombineWarps, 0,
-                                         stream>>>(args);
+  constexpr int kT = prefix::kCombineThreads;
+  static_assert(kT == 128, "four warps");
+  if (args.parts + args.own_parts <= 16)
+    prefix::shared_prefix_combine_kernel<1>
+        <<<static_cast<unsigned>((rows + 3) / 4), kT, 0, stream>>>(args);
+  else
+    prefix::shared_prefix_combine_kernel<4><<<static_cast<unsigned>(rows), kT, 0, stream>>>(args);
   return cudaGetLastError();
 }
 
