@@ -40,12 +40,19 @@ constexpr int kRegsControl = 56, kRegsSoftmax = 224;
 static_assert(4 * 32 * kRegsControl + 8 * 32 * kRegsSoftmax <= 384 * 168, "register split");
 constexpr uint32_t kHalf = 128u * 128u;  // 128 rows x 128 B (64 dims)
 constexpr uint32_t kTile = 2u * kHalf;
-constexpr uint32_t kSmemQ = 0;           // 2 row tiles (the second one is staging with kKeyPair)
-constexpr uint32_t kSmemK = 2 * kTile;   // 2 stages
-constexpr uint32_t kSmemV = 4 * kTile;   // 2 stages
-constexpr uint32_t kSmemBar = 6 * kTile;
-constexpr uint32_t kSmemBytes = kSmemBar + 256;
-constexpr uint32_t kSmemAlloc = kSmemBytes + 1024;
+// Q tiles, then the K and V stages: two row tiles and two stages, or one and three.
+template <bool kKeyPair>
+struct Layout {
+  static constexpr int kTiles = kKeyPair ? 1 : 2;
+  static constexpr int kStages = kKeyPair ? 3 : 2;
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kK = kTiles * kTile;
+  static constexpr uint32_t kV = kK + kStages * kTile;
+  static constexpr uint32_t kBar = kV + kStages * kTile;
+  static constexpr uint32_t kAlloc = kBar + 256 + 1024;  // + slack for 1024-byte alignment
+};
+static_assert(Layout<true>::kAlloc <= 227u * 1024u && Layout<false>::kAlloc <= 227u * 1024u,
+              "shared memory");
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleThreshold = 8.0f;
@@ -55,8 +62,8 @@ constexpr uint32_t kIdescPV = idesc_bf16_f32(128, 128, /*b_mn_major=*/true);
 
 struct Bars {
   uint64_t q_full;
-  uint64_t k_full[2], k_empty[2];
-  uint64_t v_full[2], v_empty[2];
+  uint64_t k_full[3], k_empty[3];
+  uint64_t v_full[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
   uint64_t o_full[2];
   uint64_t drain;
@@ -66,6 +73,18 @@ struct Bars {
   int ref;  // first of the CTA's sequences that take part: its table row names the prefix pages
 };
 static_assert(sizeof(Bars) <= 256, "barrier block");
+
+// Position in a ring of kStages stages.
+template <int kStages>
+struct Ring {
+  uint32_t stage = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 __device__ __forceinline__ void issue_qk(uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr) {
   const uint64_t qd = sdesc_sw128(q_addr, 16, 1024);
@@ -111,21 +130,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Bars* bars = reinterpret_cast<Bars*>(smem + kSmemBar);
+  using L = Layout<kKeyPair>;
+  Bars* bars = reinterpret_cast<Bars*>(smem + L::kBar);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int tile0 = kKeyPair ? blockIdx.x : 2 * blockIdx.x;
   const int kvh = blockIdx.y;
   const int split = blockIdx.z;
-  constexpr int kTiles = kKeyPair ? 1 : 2;
 
+  const int box_rows = a.seqs_per_tile * a.group;
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&bars->k_full[i], 1);
       mbar_init(&bars->k_empty[i], 1);
       mbar_init(&bars->v_full[i], 1);
       mbar_init(&bars->v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], 4);
       mbar_init(&bars->o_full[i], 1);
@@ -135,23 +157,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     bars->lo = 0x7fffffff;
     bars->ref = 0x7fffffff;
     fence_mbar_init();
+    // Q right away: it depends on nothing
+    const uint64_t pol_q = l2_policy_evict_first();
+    mbar_arrive_expect_tx(&bars->q_full, L::kTiles * 2 * box_rows * 128);
+#pragma unroll
+    for (int i = 0; i < L::kTiles; ++i)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        tma_load_3d_hint(smem + L::kQ + i * kTile + hf * kHalf, &tm_q, &bars->q_full, hf * 64,
+                         kvh * a.group, (tile0 + i) * a.seqs_per_tile, pol_q);
   }
   if (warp == 2) {
     tmem_alloc(&bars->tmem_base, kTmemCols);
     tmem_relinquish();
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tm_q);
+  if (warp == 3 && lane == 0) {
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
   // rows of the Q tiles that no TMA box covers (group does not divide 128) are zeros
-  const int box_rows = a.seqs_per_tile * a.group;
-  for (int i = threadIdx.x; i < kTiles * 2 * (kBM - box_rows) * 8; i += kThreads) {
+  for (int i = threadIdx.x; i < L::kTiles * 2 * (kBM - box_rows) * 8; i += kThreads) {
     const int c = i & 7, rest = i >> 3;
     const int hf = rest / (kBM - box_rows);
     const int row = box_rows + rest - hf * (kBM - box_rows);
-    *reinterpret_cast<uint4*>(smem + kSmemQ + hf * kHalf + row * 128 + c * 16) =
+    *reinterpret_cast<uint4*>(smem + L::kQ + hf * kHalf + row * 128 + c * 16) =
         make_uint4(0u, 0u, 0u, 0u);
   }
   fence_proxy_async_smem();
@@ -188,23 +217,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp < 4) setmaxnreg_dec<kRegsControl>();
   else setmaxnreg_inc<kRegsSoftmax>();
   if (warp < 4) {
-    if (warp == 0 && n_kv > 0) {
+    if (warp == 0 && n_kv == 0) {
+      if (lane == 0) mbar_wait(&bars->q_full, 0, ab);  // Q has landed before the CTA may exit
+    } else if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer (warp)
       const uint64_t pol_kv = l2_policy_evict_last();
-      const uint64_t pol_q = l2_policy_evict_first();
       const int box = 1 << a.box_shift;
       const int units = kBN >> a.box_shift;
       const int page_mask = (1 << a.page_shift) - 1;
       const int32_t* bt = a.block_table + static_cast<long long>(bars->ref) * a.bt_stride;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&bars->q_full, kTiles * 2 * box_rows * 128);
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf)
-            tma_load_3d_hint(smem + kSmemQ + i * kTile + hf * kHalf, &tm_q, &bars->q_full,
-                             hf * 64, kvh * a.group, (tile0 + i) * a.seqs_per_tile, pol_q);
-      }
       // page of unit `lane` of key tile j; -1 past the prefix or for an entry outside
       // [0, num_pages)
       auto unit_block = [&](int j) {
@@ -218,19 +239,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       bool ok = true;
       int blk = unit_block(0);
-      for (int j = 0; j < n_kv && ok; ++j) {
+      Ring<L::kStages> ring;
+      for (int j = 0; j < n_kv && ok; ++j, ring.next()) {
         const int key0 = (j_lo + j) * kBN;
         const int blk_next = j + 1 < n_kv ? unit_block(j + 1) : -1;
         const int in_page = (key0 + lane * box) & page_mask;
         const int page = blk >= 0 ? blk : a.num_pages;  // out of range: TMA writes zeros
-        const uint32_t st = j & 1, ph = ((j >> 1) & 1) ^ 1;
+        const uint32_t st = ring.stage, ph = ring.phase ^ 1u;
         if (!(ok = mbar_wait_warp(&bars->k_empty[st], ph, ab))) break;
         if (lane == 0) mbar_arrive_expect_tx(&bars->k_full[st], kTile);
         __syncwarp();
         if (lane < units) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf)
-            tma_load_4d_hint(smem + kSmemK + st * kTile + hf * kHalf + lane * box * 128, &tm_k,
+            tma_load_4d_hint(smem + L::kK + st * kTile + hf * kHalf + lane * box * 128, &tm_k,
                              &bars->k_full[st], hf * 64, kvh, in_page, page, pol_kv);
         }
         if (!(ok = mbar_wait_warp(&bars->v_empty[st], ph, ab))) break;
@@ -246,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint16_t* src = a.v + static_cast<long long>(pblk < 0 ? 0 : pblk) * a.v_sp +
                                 static_cast<long long>(pkey & page_mask) * a.v_st +
                                 static_cast<long long>(kvh) * a.v_sh;
-          uint8_t* dst = smem + kSmemV + st * kTile;
+          uint8_t* dst = smem + L::kV + st * kTile;
 #pragma unroll 4
           for (int i = lane; i < box * 16; i += 32) {
             const int r = i >> 4, ch = i & 15;
@@ -265,47 +287,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < units && lane != pu) {
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf)
-            tma_load_4d_hint(smem + kSmemV + st * kTile + hf * kHalf + lane * box * 128, &tm_v,
+            tma_load_4d_hint(smem + L::kV + st * kTile + hf * kHalf + lane * box * 128, &tm_v,
                              &bars->v_full[st], hf * 64, kvh, in_page, page, pol_kv);
         }
         blk = blk_next;
       }
       if (lane == 0) {  // every issued load has landed before the CTA may exit
         mbar_wait(&bars->q_full, 0, ab);
-        for (int i = 0; i < 2 && i < n_kv; ++i) {
+        for (int i = 0; i < L::kStages && i < n_kv; ++i) {
           const int last = n_kv - 1 - i;
-          mbar_wait(&bars->k_full[last & 1], (last >> 1) & 1, ab);
-          mbar_wait(&bars->v_full[last & 1], (last >> 1) & 1, ab);
+          mbar_wait(&bars->k_full[last % L::kStages], (last / L::kStages) & 1, ab);
+          mbar_wait(&bars->v_full[last % L::kStages], (last / L::kStages) & 1, ab);
         }
       }
     } else if (warp == 1 && n_kv > 0) {
       // ---------------------------------------------------------------- UMMA issuer
       if (lane == 0) {
-        const uint32_t q_addr = smem_u32(smem + kSmemQ);
-        const uint32_t k_addr = smem_u32(smem + kSmemK);
-        const uint32_t v_addr = smem_u32(smem + kSmemV);
+        const uint32_t q_addr = smem_u32(smem + L::kQ);
+        const uint32_t k_addr = smem_u32(smem + L::kK);
+        const uint32_t v_addr = smem_u32(smem + L::kV);
         bool ok = mbar_wait(&bars->q_full, 0, ab);
         if (kKeyPair) {
           // key tile j on half s = j mod 2: S(j + 1) is issued before P(j) is waited for
+          Ring<L::kStages> kr, vr;
           auto qk = [&](int j) {
-            const int st = j & 1;
-            if (!(ok = ok && mbar_wait(&bars->k_full[st], (j >> 1) & 1, ab))) return;
+            if (!(ok = ok && mbar_wait(&bars->k_full[kr.stage], kr.phase, ab))) return;
             tc_fence_after();
-            issue_qk(tbase + st * 128, q_addr, k_addr + st * kTile);
-            umma_commit(&bars->s_full[st]);
-            umma_commit(&bars->k_empty[st]);
+            issue_qk(tbase + (j & 1) * 128, q_addr, k_addr + kr.stage * kTile);
+            umma_commit(&bars->s_full[j & 1]);
+            umma_commit(&bars->k_empty[kr.stage]);
+            kr.next();
           };
           if (ok) qk(0);
           if (ok && n_kv > 1) qk(1);
-          for (int j = 0; j < n_kv && ok; ++j) {
-            const int st = j & 1;
-            if (!(ok = mbar_wait(&bars->p_full[st], (j >> 1) & 1, ab))) break;
-            if (!(ok = mbar_wait(&bars->v_full[st], (j >> 1) & 1, ab))) break;
+          for (int j = 0; j < n_kv && ok; ++j, vr.next()) {
+            const int half = j & 1;
+            if (!(ok = mbar_wait(&bars->p_full[half], (j >> 1) & 1, ab))) break;
+            if (!(ok = mbar_wait(&bars->v_full[vr.stage], vr.phase, ab))) break;
             tc_fence_after();
-            issue_pv(tbase + 256 + st * 128, tbase + st * 128, v_addr + st * kTile, j > 1);
-            umma_commit(&bars->v_empty[st]);
+            issue_pv(tbase + 256 + half * 128, tbase + half * 128, v_addr + vr.stage * kTile, j > 1);
+            umma_commit(&bars->v_empty[vr.stage]);
             if (j + 2 < n_kv) qk(j + 2);  // overwrites P(j) in order after its product
-            else umma_commit(&bars->o_full[st]);
+            else umma_commit(&bars->o_full[half]);
           }
         } else {
           for (int j = 0; j <= n_kv && ok; ++j) {
@@ -527,44 +550,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (any && ok && mbar_wait_warp(&bars->o_full[s], 0, ab)) {
       tc_fence_after();
       const float inv_l = seen ? 1.f / l_run : 0.f;
-      // every MMA that reads Q precedes the product o_full[s] waits for: its tile is free
-      uint8_t* stage = smem + kSmemQ + s * kTile;
+      if (__any_sync(0xffffffffu, stored)) {
+        // each lane writes its own row, a 32-byte sector at a time
+        float* dst = a.ws_o + ((static_cast<long long>(part) * a.batch + b) * a.n_heads + h) * 128;
 #pragma unroll 1
-      for (int hp = 0; hp < 2; ++hp) {
-        __syncwarp();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          tmem_ld32(t_o + hp * 64 + c * 32, o);
+          tmem_ld32(t_o + c * 32, o);
           tmem_wait_ld();
+          if (stored && IFA4_DBG_CHECK(a.status, part < a.parts && h < a.n_heads)) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const int g = c * 8 + v;  // 16-byte granule (4 floats) of the 256-byte segment
-            uint4* dst = reinterpret_cast<uint4*>(stage + (g >> 3) * kHalf + row * 128 +
-                                                  (((g & 7) ^ (row & 7)) << 4));
-            *dst = make_uint4(__float_as_uint(__uint_as_float(o[4 * v]) * inv_l),
-                              __float_as_uint(__uint_as_float(o[4 * v + 1]) * inv_l),
-                              __float_as_uint(__uint_as_float(o[4 * v + 2]) * inv_l),
-                              __float_as_uint(__uint_as_float(o[4 * v + 3]) * inv_l));
-          }
-        }
-        __syncwarp();
-        const int wrow0 = (warp & 3) * 32;
-        const int g = lane & 15;
+            for (int v = 0; v < 4; ++v) {
+              float f[8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = wrow0 + 2 * i + (lane >> 4);
-          const int rb = r / a.group;
-          const int ob = tile * a.seqs_per_tile + rb;
-          if (rb < a.seqs_per_tile && ob < a.batch) {
-            const uint4 val = *reinterpret_cast<const uint4*>(
-                stage + (g >> 3) * kHalf + r * 128 + (((g & 7) ^ (r & 7)) << 4));
-            const int oh = kvh * a.group + (r - rb * a.group);
-            if (IFA4_DBG_CHECK(a.status, part < a.parts && oh < a.n_heads))
-              *reinterpret_cast<uint4*>(
-                  a.ws_o + ((static_cast<long long>(part) * a.batch + ob) * a.n_heads + oh) * 128 +
-                  hp * 64 + g * 4) = val;
+              for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[8 * v + i]) * inv_l;
+              asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * 32 + 8 * v),
+                           "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),
+                           "f"(f[6]), "f"(f[7])
+                           : "memory");
+            }
           }
+          __syncwarp();
         }
       }
     }
@@ -663,19 +669,20 @@ cudaError_t launch_shared_prefix_sm100(const SharedPrefixKernelArgs& args, const
                                        const CUtensorMap& tm_k, const CUtensorMap& tm_v,
                                        cudaStream_t stream) {
   static std::atomic<bool> attr_rows[64], attr_keys[64];
-  cudaError_t e = set_smem_limit_once(prefix::shared_prefix_kernel<false>, prefix::kSmemAlloc,
-                                      attr_rows);
+  cudaError_t e = set_smem_limit_once(prefix::shared_prefix_kernel<false>,
+                                      prefix::Layout<false>::kAlloc, attr_rows);
   if (e == cudaSuccess)
-    e = set_smem_limit_once(prefix::shared_prefix_kernel<true>, prefix::kSmemAlloc, attr_keys);
+    e = set_smem_limit_once(prefix::shared_prefix_kernel<true>, prefix::Layout<true>::kAlloc,
+                            attr_keys);
   if (e != cudaSuccess) return e;
   const int tiles = (args.batch + args.seqs_per_tile - 1) / args.seqs_per_tile;
   const dim3 grid(args.key_pair ? tiles : (tiles + 1) / 2, args.kv_heads, args.splits);
   if (args.key_pair)
     prefix::shared_prefix_kernel<true>
-        <<<grid, prefix::kThreads, prefix::kSmemAlloc, stream>>>(args, tm_q, tm_k, tm_v);
+        <<<grid, prefix::kThreads, prefix::Layout<true>::kAlloc, stream>>>(args, tm_q, tm_k, tm_v);
   else
     prefix::shared_prefix_kernel<false>
-        <<<grid, prefix::kThreads, prefix::kSmemAlloc, stream>>>(args, tm_q, tm_k, tm_v);
+        <<<grid, prefix::kThreads, prefix::Layout<false>::kAlloc, stream>>>(args, tm_q, tm_k, tm_v);
   return cudaGetLastError();
 }
 
