@@ -946,12 +946,20 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
   const int64_t key_tiles = (span + 127) / 128;
   int splits = p->prefix_splits;
   if (splits == 0) {
-    // the split count with the least work on the busiest SM: waves of CTAs x (key tiles of a
-    // CTA + about three tiles' worth of start and epilogue)
+    // The split count with the least work on the busiest SM: waves of CTAs x (key tiles of a CTA
+    // + about three tiles' worth of start and epilogue).  The own keys' kernel runs beside this
+    // one on the SMs it leaves: when its CTAs (two per SM) fit half of the GPU, that many SMs are
+    // left (33 sequences, 10k prefix: 27 us with 80 of these CTAs and 132 of those, 34 us with
+    // 108; 8 sequences, 2k: 16.4 us with 88, 17.3 us with 128); a larger one comes after it
+    // (128 sequences, 32k: 126 us with 144 CTAs, 138 us with 112).
+    const int64_t hpc = group < 16 ? group : 16;
+    const int64_t own_ctas = static_cast<int64_t>(d->batch) * d->kv_heads *
+                             ((group + hpc - 1) / hpc) * plan->own_splits;
+    const int64_t room = own_ctas <= sms ? sms - (own_ctas + 1) / 2 : sms;
     int64_t best = INT64_MAX;
     const int64_t most = key_tiles < 64 ? key_tiles : 64;
     for (int64_t s = 1; s <= most; ++s) {
-      const int64_t waves = (ctas * s + sms - 1) / sms;
+      const int64_t waves = (ctas * s + room - 1) / room;
       const int64_t cost = waves * ((key_tiles + s - 1) / s + 3);
       if (cost < best) {
         best = cost;

@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const SeqInfo si = seq_info<kPaged>(a, b);
   const int bs = a.align_bottom_right ? si.sk - 1 : 1 - si.sk;  // bias distance at key 0
 
+  if (a.prefix_len > 0) launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -438,6 +439,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   }
+  // behind a shared prefix this kernel runs beside the prefix kernel and ends after it, so the
+  // merge that follows waits for both
+  if (a.prefix_len > 0) wait_previous_kernel();
 }
 
 // Merge num_splits normalised partials per (sequence, head): weights 2^(lse_s - max lse).
@@ -479,6 +483,11 @@ cudaError_t launch_decode_sm100(const DecodeKernelArgs& args, const CUtensorMap&
   if (se != cudaSuccess) return se;
   const int head_blocks = (args.group + args.heads_per_cta - 1) / args.heads_per_cta;
   dim3 grid(args.num_splits, args.kv_heads * head_blocks, args.batch);
+  if (args.prefix_len > 0) {
+    if (args.block_table == nullptr) return cudaErrorInvalidValue;
+    return launch_early(decode::rel_attn_decode_kernel<true>, grid, decode::kThreads,
+                        decode::kSmemAlloc, stream, args, tm_k, tm_v);
+  }
   if (args.block_table != nullptr)
     decode::rel_attn_decode_kernel<true><<<grid, decode::kThreads, decode::kSmemAlloc, stream>>>(
         args, tm_k, tm_v);
@@ -486,7 +495,7 @@ cudaError_t launch_decode_sm100(const DecodeKernelArgs& args, const CUtensorMap&
     decode::rel_attn_decode_kernel<false><<<grid, decode::kThreads, decode::kSmemAlloc, stream>>>(
         args, tm_k, tm_v);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || args.ws_o == nullptr || args.prefix_len > 0) return e;
+  if (e != cudaSuccess || args.ws_o == nullptr) return e;
   dim3 cgrid(args.n_heads, args.batch);
   decode::rel_attn_decode_combine_kernel<<<cgrid, 128, 0, stream>>>(args);
   return cudaGetLastError();

@@ -30,6 +30,24 @@ cudaError_t set_smem_limit_once(K kernel, uint32_t bytes, std::atomic<bool> (&do
   return cudaSuccess;
 }
 
+// Launch that may start before the previous kernel of the stream has finished, as soon as all of its
+// blocks have called launch_dependents() (see ifa4_ptx.cuh) or ended.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, uint32_t smem,
+                         cudaStream_t stream, const A&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Status bits written by kernels that abandoned a bounded wait.
 constexpr int kStatusPrefillTimeout = 1;
 constexpr int kStatusDecodeTimeout = 2;

@@ -535,6 +535,16 @@ __device__ __forceinline__ void add_bias_window(const uint32_t (&w)[20], int dto
   for (int i = 0; i < 32; ++i) x[i] += b[i] * 1.4426950408889634f;
 }
 
+// Programmatic dependent launch: lets the next kernel of the stream start (when it was launched to
+// start early) once every block has said so; waits until the previous kernel has completed and its
+// writes are visible (at once when this kernel was not launched early).
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Warpgroup-wide register re-split (every warp of the warpgroup executes it; the sum over the
 // CTA's warps must fit in the registers the CTA was launched with).
 template <uint32_t kRegs>

@@ -14,6 +14,10 @@
 // Sequences with fewer keys than the prefix take no part (their rows have weight 0 here; the
 // decode kernel then covers all of their keys).
 //
+// The three kernels (prefix, own keys, merge) are launched to overlap: the own keys' kernel starts
+// as soon as the prefix kernel's CTAs have and fills the SMs they leave, and ends after it; the
+// merge's blocks wait for that.
+//
 // The grid is (row tiles, KV heads, key splits); every CTA writes its rows' normalised fp32
 // partial outputs and log2-sum-exps, and shared_prefix_combine_kernel merges all partials of a
 // row.  The CTA's two softmax groups (and TMEM halves) work on
@@ -138,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kvh = blockIdx.y;
   const int split = blockIdx.z;
 
+  launch_dependents();  // the own keys' kernel needs nothing from this one
   const int box_rows = a.seqs_per_tile * a.group;
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -603,6 +608,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   const int b = static_cast<int>(row / a.n_heads);
   const int h = static_cast<int>(row - static_cast<long long>(b) * a.n_heads);
   const int n = a.parts + a.own_parts;
+  wait_previous_kernel();  // both kernels' partials (the own keys' ends after the prefix's)
   // partial i: the prefix's first, then the own keys'
   auto lse_of = [&](int i) {
     return i < a.parts ? a.ws_lse[i * rows + row] : a.own_lse[row * a.own_parts + (i - a.parts)];
@@ -692,11 +698,10 @@ cudaError_t launch_shared_prefix_combine_sm100(const SharedPrefixKernelArgs& arg
   constexpr int kT = prefix::kCombineThreads;
   static_assert(kT == 128, "four warps");
   if (args.parts + args.own_parts <= 16)
-    prefix::shared_prefix_combine_kernel<1>
-        <<<static_cast<unsigned>((rows + 3) / 4), kT, 0, stream>>>(args);
-  else
-    prefix::shared_prefix_combine_kernel<4><<<static_cast<unsigned>(rows), kT, 0, stream>>>(args);
-  return cudaGetLastError();
+    return launch_early(prefix::shared_prefix_combine_kernel<1>,
+                        dim3(static_cast<unsigned>((rows + 3) / 4)), kT, 0, stream, args);
+  return launch_early(prefix::shared_prefix_combine_kernel<4>, dim3(static_cast<unsigned>(rows)), kT,
+                      0, stream, args);
 }
 
 }  // namespace ifa4
