@@ -1058,7 +1058,12 @@ int ifa4_decode_shared_prefix_launch(const IFA4SharedPrefixParams* p, void* work
                                    d->q_stride_h, plan.seqs_per_tile, "q", a.group)))
     return rc;
   if ((rc = encode_kv(d, 128, &tk, &tv))) return rc;
-  if ((rc = encode_kv(d, 64, &tk64, &tv64))) return rc;
+  if (d->page_size <= 64) {  // pages no longer than a tile of either kernel: the same boxes
+    tk64 = tk;
+    tv64 = tv;
+  } else if ((rc = encode_kv(d, 64, &tk64, &tv64))) {
+    return rc;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = ifa4::launch_shared_prefix_sm100(a, tq, tk, tv, s);
   if (e != cudaSuccess) return cuda_fail(e, "decode_shared_prefix launch");

@@ -198,11 +198,12 @@ class Ifa4Error(RuntimeError):
 
 _lib = None
 _torch_ops = None
+_overloads = {}
 TORCH_OPS_PATH = os.path.join(_LIB_DIR, "libifa4_torch_ops.so")
 
 
 def torch_ops():
-    """The torch operators ``torch.ops.inkling_fa4`` over the C ABI (``prefill_``, ``decode_``),
+    """The torch operators ``torch.ops.inkling_fa4`` over the C ABI (``prefill_``, ``decode_``, ..),
     or None when they are not built or the debug library is selected (they link the release
     library).  The package then calls the C ABI through ctypes instead: the same entry points,
     with more host work per call."""
@@ -218,6 +219,17 @@ def torch_ops():
     torch.ops.load_library(TORCH_OPS_PATH)
     _torch_ops = torch.ops.inkling_fa4
     return _torch_ops
+
+
+def torch_op(name: str):
+    """The operator ``inkling_fa4::name`` ready to call (looked up once), or None as ``torch_ops``."""
+    op = _overloads.get(name)
+    if op is None:
+        ops = torch_ops()
+        if ops is None:
+            return None
+        op = _overloads[name] = getattr(ops, name).default
+    return op
 
 
 def lib() -> ctypes.CDLL:

@@ -20,13 +20,55 @@ USE_TORCH_OPS = True
 def _tma_ready(t: torch.Tensor) -> torch.Tensor:
     """q/k/v go through TMA: last stride 1, other strides multiples of 8 elements (16 bytes),
     16-byte aligned base.  Anything else is copied to a contiguous tensor."""
-    ok = (t.stride(-1) == 1 and all(s > 0 and s % 8 == 0 for s in t.stride()[:-1])
-          and t.data_ptr() % 16 == 0)
-    return t if ok else t.contiguous()
+    *outer, last = t.stride()
+    if last == 1 and t.data_ptr() % 16 == 0:
+        for s in outer:
+            if s <= 0 or s % 8:
+                break
+        else:
+            return t
+    return t.contiguous()
+
+
+def _inputs_ok(q, k, v, rel_logits, cu_q, cu_k, rel_extent, n_heads, kv_heads, head_dim,
+               causal_align, block_table):
+    """Whether ``_check_inputs`` would accept these arguments, decided in one cheap pass (the usual
+    case; anything doubtful goes through the full checks for its error)."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    dev = q.get_device()
+    if (dev < 0 or k.get_device() != dev or v.get_device() != dev or rel_logits.get_device() != dev
+            or cu_q.get_device() != dev or cu_k.get_device() != dev or q.dtype is not bf16
+            or k.dtype is not bf16 or v.dtype is not bf16 or rel_logits.dtype is not bf16
+            or cu_q.dtype is not i32 or cu_k.dtype is not i32 or head_dim != HEAD_DIM):
+        return False
+    qs, ks, rs, cs = q.shape, k.shape, rel_logits.shape, cu_q.shape
+    if (len(qs) != 3 or qs[2] != HEAD_DIM or len(rs) != 3 or rs[0] != qs[0] or rs[1] != qs[1]
+            or len(cs) != 1 or cs[0] < 1 or cu_k.shape != cs or v.shape != ks
+            or ks[-1] != HEAD_DIM or not 0 < rel_extent <= rs[2] or causal_align not in ALIGN):
+        return False
+    if block_table is None:
+        if len(ks) != 3:
+            return False
+    elif (len(ks) != 4 or ks[1] < 16 or ks[1] & (ks[1] - 1) or block_table.get_device() != dev
+          or block_table.dtype is not i32 or block_table.dim() != 2
+          or block_table.shape[0] != cs[0] - 1
+          or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        return False
+    heads, kv = qs[1], ks[-2]
+    return (kv > 0 and heads % kv == 0 and (n_heads is None or n_heads == heads)
+            and (kv_heads is None or kv_heads == kv))
 
 
 def _check_inputs(name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, n_heads, kv_heads,
                   head_dim, window_size, causal_align, block_table=None):
+    try:
+        if type(rel_extent) is int and _inputs_ok(q, k, v, rel_logits, cu_q, cu_k, rel_extent,
+                                                  n_heads, kv_heads, head_dim, causal_align,
+                                                  block_table):
+            window_left = int(window_size[0]) if window_size is not None else -1
+            return q.shape[1], k.shape[-2], rel_extent, window_left
+    except (AttributeError, TypeError, IndexError):
+        pass  # not tensors: the checks below say which
     paged = block_table is not None
     tensors = [("q", q), ("k", k), ("v", v), ("rel_logits", rel_logits),
                ("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)]
@@ -147,7 +189,7 @@ def _prepare(name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, causal, window_s
         q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
     rel = rel_logits if rel_logits.stride(-1) == 1 else rel_logits.contiguous()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
             raise ValueError(f"{name}: out must match q in shape, dtype and device")

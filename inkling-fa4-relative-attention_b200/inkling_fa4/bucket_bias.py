@@ -76,9 +76,9 @@ def _forward(table, starts, total_q, rel_extent):
         raise ValueError(f"{name}: total_q must be >= 0, rel_extent in [1, 2^24]")
     heads = table.shape[1]
     rel = torch.empty((heads, rel_extent), dtype=torch.bfloat16, device=table.device)
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.bucket_bias_.default(table, starts, rel)
+    op = _lib.torch_op("bucket_bias_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(table, starts, rel)
         if rc:
             _lib.check(rc)
     else:
@@ -117,9 +117,9 @@ def _backward(drel, starts, dtype, cu_seqlens_q):
         drel = drel.contiguous()
     heads, buckets = drel.shape[1], starts.numel()
     dtable = torch.empty((buckets, heads), dtype=dtype, device=drel.device)
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.bucket_bias_backward_.default(drel, starts, dtable, cu_seqlens_q)
+    op = _lib.torch_op("bucket_bias_backward_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(drel, starts, dtable, cu_seqlens_q)
         if rc:
             _lib.check(rc)
         return dtable

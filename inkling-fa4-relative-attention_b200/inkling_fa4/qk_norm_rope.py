@@ -34,6 +34,10 @@ def _rows_ready(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _empty_like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _check_rows(name, nm, t, like, heads=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: {nm} must be a torch.Tensor")
@@ -148,12 +152,11 @@ def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
     if eps < 0 and inv_freq is None:
         raise ValueError(f"{name}: neither a norm (eps) nor a rotation (inv_freq)")
     q, k = _rows_ready(q), _rows_ready(k)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.qk_norm_rope_.default(q, k, q_out, k_out, q_weight, k_weight, inv_freq, cu_q,
-                                       cu_k, bool(interleaved), eps)
+    q_out, k_out = _empty_like(q), _empty_like(k)
+    op = _lib.torch_op("qk_norm_rope_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(q, k, q_out, k_out, q_weight, k_weight, inv_freq, cu_q, cu_k, bool(interleaved),
+                eps)
         if rc:
             _lib.check(rc)
         return q_out, k_out
@@ -178,15 +181,13 @@ def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_fre
     q_weight, k_weight, eps, inv_freq = _check_step(name, q.device, q_weight, k_weight, eps,
                                                     inv_freq)
     q, k, dq_out, dk_out = (_rows_ready(t) for t in (q, k, dq_out, dk_out))
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dq, dk = _empty_like(q), _empty_like(k)
     dqw = torch.empty_like(q_weight) if q_weight is not None and weight_grads[0] else None
     dkw = torch.empty_like(k_weight) if k_weight is not None and weight_grads[1] else None
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.qk_norm_rope_backward_.default(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight,
-                                                dqw, dkw, inv_freq, cu_q, cu_k,
-                                                bool(interleaved), eps)
+    op = _lib.torch_op("qk_norm_rope_backward_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, dqw, dkw, inv_freq, cu_q, cu_k,
+                bool(interleaved), eps)
         if rc:
             _lib.check(rc)
         return dq, dk, dqw, dkw
@@ -318,7 +319,7 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
         _check_rows(name, "q", q, k)
         if q_out is None:
             q = _rows_ready(q)
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            q_out = _empty_like(q)
         else:
             _check_rows(name, "q_out", q_out, k, q.shape[1])
             _check_written(name, "q_out", q_out)
@@ -327,11 +328,10 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
             if not same and any(t.untyped_storage().data_ptr() == store for t in (q, k, v)):
                 raise ValueError(f"{name}: q_out must be q itself or share no storage with q, k, v")
             q = _rows_ready(q)
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.kv_append_.default(q, k, v, q_out, k_cache, v_cache, q_weight, k_weight, inv_freq,
-                                    cu_seqlens_q, cu_seqlens_k, block_table, bool(interleaved),
-                                    eps, zero_padding)
+    op = _lib.torch_op("kv_append_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(q, k, v, q_out, k_cache, v_cache, q_weight, k_weight, inv_freq, cu_seqlens_q,
+                cu_seqlens_k, block_table, bool(interleaved), eps, zero_padding)
         if rc:
             _lib.check(rc)
         return q_out

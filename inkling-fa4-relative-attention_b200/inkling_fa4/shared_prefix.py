@@ -52,12 +52,11 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
         raise ValueError(f"{name}: shared_prefix_len {shared_prefix_len} is beyond the table's "
                          f"{block_table.shape[1]} pages of {k.shape[1]}")
     max_seqlen_k = int(max_seqlen_k) if max_seqlen_k else 0
-    ops = _lib.torch_ops() if _ops.USE_TORCH_OPS else None
-    if ops is not None:
-        rc = ops.decode_shared_prefix_.default(
-            q, k, v, rel, out, cu_seqlens_q, cu_seqlens_k, lse, block_table, workspace, rel_extent,
-            window_left, max_seqlen_k, scale, int(num_splits), int(chunk_len), shared_prefix_len,
-            int(prefix_splits))
+    op = _lib.torch_op("decode_shared_prefix_") if _ops.USE_TORCH_OPS else None
+    if op is not None:
+        rc = op(q, k, v, rel, out, cu_seqlens_q, cu_seqlens_k, lse, block_table, workspace,
+                rel_extent, window_left, max_seqlen_k, scale, int(num_splits), int(chunk_len),
+                shared_prefix_len, int(prefix_splits))
         if rc:
             _lib.check(rc)
         return (out, lse) if lse is not None else out
