@@ -13,7 +13,8 @@
 // Work split: a unit is one token and a part of its heads; one warp per unit, eight lanes per head
 // row (16 dims each, so four rows run at once and a row's sum takes three shuffles), loaded and
 // stored in 16-byte pieces.  A lane's dims are chosen so that both elements of its eight pairs are
-// its own: 8l.. and rotary_dim / 2 + 8l.. for the two halves, 16l.. interleaved.  The angles
+// its own (8l.. and rotary_dim / 2 + 8l.. for the two halves, 8l.. and 64 + 8l.. interleaved) and so
+// that eight lanes' 16 bytes are neighbours: whole sectors in every access.  The angles
 // depend on the token only: they are computed once per unit (two pairs a lane), handed round
 // through shared memory and kept in registers for all rows.
 //
@@ -132,23 +133,29 @@ __device__ __forceinline__ void angle_cos_sin(unsigned long long f, long long po
 }
 
 // The lane's part of a rotation.  Lane l (of 8) of a row holds 16 dims: 8 from a_off on and 8 from
-// b_off on, as packed pairs x[0..3] and x[4..7].  Lanes below rotary_dim / 16 are turned, with the
-// pairs 8l .. 8l + 7; the others hold the dims behind rotary_dim and pass them through.
+// b_off on, as packed pairs x[0..3] and x[4..7].
+//   kRotHalf:  lanes below n = rotary_dim / 16 hold both halves of the pairs 8l .. 8l + 7; the
+//              others share the dims behind rotary_dim, which pass through.
+//   kRotPairs: the pairs 4l .. 4l + 3 and 32 + 4l .. 32 + 4l + 3, turned where their dims lie
+//              below rotary_dim.
 template <int kRot>
 struct Rotation {
   unsigned long long f[2];  // frequencies of pairs lane and lane + 32 (the ones this lane computes)
   uint64_t c[4], s[4], ns[4];  // cosines, sines and their negatives of the lane's own pairs
   int a_off, b_off;
-  bool turned;
+  bool a_turned, b_turned;
 
   __device__ __forceinline__ void init(const void* inv_freq, int f32, int rotary_dim, int lane) {
     const int l = lane & 7;
-    turned = kRot != kRotNone && l < rotary_dim / 16;
-    a_off = 16 * l;
-    b_off = 16 * l + 8;
+    a_off = 8 * l;
+    b_off = 64 + 8 * l;
+    a_turned = a_off < rotary_dim;
+    b_turned = b_off < rotary_dim;
     if (kRot == kRotHalf) {
-      a_off = turned ? 8 * l : rotary_dim + 16 * (l - rotary_dim / 16);
-      b_off = turned ? rotary_dim / 2 + 8 * l : a_off + 8;
+      const int n = rotary_dim / 16;
+      a_turned = b_turned = l < n;
+      a_off = a_turned ? 8 * l : rotary_dim + 8 * (l - n);
+      b_off = a_turned ? rotary_dim / 2 + 8 * l : rotary_dim + 8 * (8 - n) + 8 * (l - n);
     }
     if (kRot != kRotNone) {
 #pragma unroll
@@ -168,10 +175,11 @@ struct Rotation {
       table[lane + 32 * i] = cs;
     }
     __syncwarp();
-    const float4* mine = reinterpret_cast<const float4*>(table + 8 * (lane & 7));
+    const int l = lane & 7;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 v = mine[i];  // cos, sin, cos, sin
+      const int pair = kRot == kRotHalf ? 8 * l + 2 * i : 4 * l + (i < 2 ? 2 * i : 28 + 2 * i);
+      const float4 v = *reinterpret_cast<const float4*>(table + pair);  // cos, sin, cos, sin
       c[i] = f2_pack(v.x, v.z);
       s[i] = f2_pack(v.y, v.w);
       ns[i] = f2_pack(-v.y, -v.w);
@@ -181,8 +189,9 @@ struct Rotation {
   // Forward, or (kBack) the transposed rotation.
   template <bool kBack>
   __device__ __forceinline__ void apply(uint64_t (&x)[8]) const {
-    if (kRot == kRotNone || !turned) return;
+    if (kRot == kRotNone) return;
     if (kRot == kRotHalf) {
+      if (!a_turned) return;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t a = x[i], b = x[4 + i];
@@ -192,6 +201,7 @@ struct Rotation {
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        if (i < 4 ? !a_turned : !b_turned) continue;
         float a, b, c0, c1, s0, s1;
         f2_unpack(x[i], a, b);
         f2_unpack(c[i >> 1], c0, c1);
