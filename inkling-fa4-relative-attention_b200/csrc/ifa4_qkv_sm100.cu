@@ -53,22 +53,20 @@ __device__ __forceinline__ uint4 ldg_v4(const void* p) {
   return r;
 }
 
-// Eight bf16 <-> four packed fp32 pairs.
-__device__ __forceinline__ void unpack8(const uint4& v, uint64_t* x) {
+// Eight bf16 <-> eight fp32.  (The rotation in packed fp32 pairs, two values an instruction, was
+// slower, 128 us instead of 118 at 32k tokens x 40 heads: it needs the sines' negatives as well.)
+__device__ __forceinline__ void unpack8(const uint4& v, float* x) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    x[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
 }
 
-__device__ __forceinline__ uint32_t pack2(uint64_t x) {
-  float lo, hi;
-  f2_unpack(x, lo, hi);
-  return pack_bf16x2(lo, hi);
-}
-
-__device__ __forceinline__ uint4 pack8(const uint64_t* x) {
-  return make_uint4(pack2(x[0]), pack2(x[1]), pack2(x[2]), pack2(x[3]));
+__device__ __forceinline__ uint4 pack8(const float* x) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                    pack_bf16x2(x[6], x[7]));
 }
 
 // Sum over the eight lanes of a row.
@@ -133,7 +131,7 @@ __device__ __forceinline__ void angle_cos_sin(unsigned long long f, long long po
 }
 
 // The lane's part of a rotation.  Lane l (of 8) of a row holds 16 dims: 8 from a_off on and 8 from
-// b_off on, as packed pairs x[0..3] and x[4..7].
+// b_off on, as x[0..7] and x[8..15].
 //   kRotHalf:  lanes below n = rotary_dim / 16 hold both halves of the pairs 8l .. 8l + 7; the
 //              others share the dims behind rotary_dim, which pass through.
 //   kRotPairs: the pairs 4l .. 4l + 3 and 32 + 4l .. 32 + 4l + 3, turned where their dims lie
@@ -141,7 +139,7 @@ __device__ __forceinline__ void angle_cos_sin(unsigned long long f, long long po
 template <int kRot>
 struct Rotation {
   unsigned long long f[2];  // frequencies of pairs lane and lane + 32 (the ones this lane computes)
-  uint64_t c[4], s[4], ns[4];  // cosines, sines and their negatives of the lane's own pairs
+  float c[8], s[8];         // cosines and sines of the lane's own pairs
   int a_off, b_off;
   bool a_turned, b_turned;
 
@@ -180,47 +178,39 @@ struct Rotation {
     for (int i = 0; i < 4; ++i) {
       const int pair = kRot == kRotHalf ? 8 * l + 2 * i : 4 * l + (i < 2 ? 2 * i : 28 + 2 * i);
       const float4 v = *reinterpret_cast<const float4*>(table + pair);  // cos, sin, cos, sin
-      c[i] = f2_pack(v.x, v.z);
-      s[i] = f2_pack(v.y, v.w);
-      ns[i] = f2_pack(-v.y, -v.w);
+      c[2 * i] = v.x;
+      s[2 * i] = v.y;
+      c[2 * i + 1] = v.z;
+      s[2 * i + 1] = v.w;
     }
   }
 
   // Forward, or (kBack) the transposed rotation.
   template <bool kBack>
-  __device__ __forceinline__ void apply(uint64_t (&x)[8]) const {
-    if (kRot == kRotNone) return;
-    if (kRot == kRotHalf) {
-      if (!a_turned) return;
+  __device__ __forceinline__ void apply(float (&x)[16]) const {
+    if (kRot == kRotNone || (kRot == kRotHalf && !a_turned)) return;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint64_t a = x[i], b = x[4 + i];
-        x[i] = f2_fma(a, c[i], f2_mul(b, kBack ? s[i] : ns[i]));
-        x[4 + i] = f2_fma(b, c[i], f2_mul(a, kBack ? ns[i] : s[i]));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < 4 ? !a_turned : !b_turned) continue;
-        float a, b, c0, c1, s0, s1;
-        f2_unpack(x[i], a, b);
-        f2_unpack(c[i >> 1], c0, c1);
-        f2_unpack(s[i >> 1], s0, s1);
-        const float ci = (i & 1) ? c1 : c0;
-        const float si = kBack ? -((i & 1) ? s1 : s0) : ((i & 1) ? s1 : s0);
-        x[i] = f2_pack(a * ci - b * si, b * ci + a * si);
-      }
+    for (int i = 0; i < 8; ++i) {
+      if (kRot == kRotPairs && (i < 4 ? !a_turned : !b_turned)) continue;
+      float& a = kRot == kRotHalf ? x[i] : x[2 * i];
+      float& b = kRot == kRotHalf ? x[8 + i] : x[2 * i + 1];
+      const float si = kBack ? -s[i] : s[i];
+      const float ta = a * c[i] - b * si;
+      b = b * c[i] + a * si;
+      a = ta;
     }
   }
 };
 
-// The lane's 16 weights as packed pairs.
-__device__ __forceinline__ void lane_weights(const float* w, int a_off, int b_off, uint64_t (&o)[8]) {
+// The lane's 16 weights.
+__device__ __forceinline__ void lane_weights(const float* w, int a_off, int b_off, float (&o)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float4 v = *reinterpret_cast<const float4*>(w + (i < 2 ? a_off + 4 * i : b_off + 4 * (i - 2)));
-    o[2 * i] = f2_pack(v.x, v.y);
-    o[2 * i + 1] = f2_pack(v.z, v.w);
+    o[4 * i] = v.x;
+    o[4 * i + 1] = v.y;
+    o[4 * i + 2] = v.z;
+    o[4 * i + 3] = v.w;
   }
 }
 
@@ -291,29 +281,26 @@ __global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
       const int ri = r + oct;
       const bool is_q = ri < a.n_heads;
       if (!kAppend || r < v_rows) {  // (warp-uniform) not V rows only
-        uint64_t x[8];
+        float x[16];
         unpack8(va, x);
-        unpack8(vb, x + 4);
+        unpack8(vb, x + 8);
         if (a.normalize) {
-          uint64_t s2 = f2_mul(x[0], x[0]), s3 = f2_mul(x[1], x[1]);
+          float s0 = x[0] * x[0], s1 = x[1] * x[1];
 #pragma unroll
-          for (int i = 2; i < 8; i += 2) {
-            s2 = f2_fma(x[i], x[i], s2);
-            s3 = f2_fma(x[i + 1], x[i + 1], s3);
+          for (int i = 2; i < 16; i += 2) {
+            s0 += x[i] * x[i];
+            s1 += x[i + 1] * x[i + 1];
           }
-          float lo, hi;
-          f2_unpack(f2_add(s2, s3), lo, hi);
-          const float rn = rsqrtf(row_sum(lo + hi) * (1.f / 128.f) + a.eps);
-          const uint64_t rn2 = f2_pack(rn, rn);
-          uint64_t wt[8];
+          const float rn = rsqrtf(row_sum(s0 + s1) * (1.f / 128.f) + a.eps);
+          float wt[16];
           lane_weights(ws[is_q ? 0 : 1], rot.a_off, rot.b_off, wt);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = f2_mul(x[i], f2_mul(wt[i], rn2));
+          for (int i = 0; i < 16; ++i) x[i] *= wt[i] * rn;
         }
         rot.template apply<false>(x);
         if (!kAppend || ri < v_rows) {
           va = pack8(x);
-          vb = pack8(x + 4);
+          vb = pack8(x + 8);
         }
       }
       if (!w.inside) va = vb = make_uint4(0u, 0u, 0u, 0u);
@@ -362,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
   ws[0][threadIdx.x] = load_weight(a.q_weight, a.weight_f32, threadIdx.x);
   ws[1][threadIdx.x] = load_weight(a.k_weight, a.weight_f32, threadIdx.x);
   __syncthreads();
-  uint64_t acc[2][8];
+  float acc[2][16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[0][i] = acc[1][i] = 0ull;
+  for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0.f;
 
   const long long step = static_cast<long long>(gridDim.x) * kWarps;
   for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp; u < a.units; u += step) {
@@ -398,39 +385,34 @@ __global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
       for (int r = r0; r < r1; r += 4) {
         const int ri = r + oct;
         const bool on = ri < r1 && w.inside;  // a row that is none has r = rsqrt(eps), maybe inf
-        uint64_t x[8], g[8];
+        float x[16], g[16];
         unpack8(raw[0], x);
-        unpack8(raw[1], x + 4);
+        unpack8(raw[1], x + 8);
         unpack8(raw[2], g);
-        unpack8(raw[3], g + 4);
+        unpack8(raw[3], g + 8);
         if (r + 4 < r1) load(r + 4);
         rot.template apply<true>(g);
         if (a.normalize) {
-          uint64_t wt[8], gw[8];
+          float wt[16];
           lane_weights(ws[kind], rot.a_off, rot.b_off, wt);
-          uint64_t ss = 0ull, dot = 0ull;
+          float ss = 0.f, dot = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            gw[i] = f2_mul(g[i], wt[i]);
-            ss = f2_fma(x[i], x[i], ss);
-            dot = f2_fma(gw[i], x[i], dot);
+          for (int i = 0; i < 16; ++i) {
+            ss += x[i] * x[i];
+            dot += g[i] * wt[i] * x[i];
           }
-          float lo, hi, dlo, dhi;
-          f2_unpack(ss, lo, hi);
-          f2_unpack(dot, dlo, dhi);
-          const float rn = rsqrtf(row_sum(lo + hi) * (1.f / 128.f) + a.eps);
-          const float back = -(row_sum(dlo + dhi) * (1.f / 128.f)) * rn * rn * rn;
-          const uint64_t rn2 = f2_pack(rn, rn), back2 = f2_pack(back, back);
+          const float rn = rsqrtf(row_sum(ss) * (1.f / 128.f) + a.eps);
+          const float back = row_sum(dot) * (1.f / 128.f) * rn * rn;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (on) acc[kind][i] = f2_fma(g[i], f2_mul(x[i], rn2), acc[kind][i]);
-            g[i] = f2_fma(x[i], back2, f2_mul(gw[i], rn2));
+          for (int i = 0; i < 16; ++i) {
+            if (on) acc[kind][i] += g[i] * (x[i] * rn);
+            g[i] = rn * (g[i] * wt[i] - x[i] * back);
           }
         }
         if (ri < r1) {
           const uint4 z = make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.a_off) = on ? pack8(g) : z;
-          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.b_off) = on ? pack8(g + 4) : z;
+          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.b_off) = on ? pack8(g + 8) : z;
         }
       }
     }
@@ -440,10 +422,8 @@ __global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
   for (int kind = 0; kind < 2; ++kind) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int dim = (i < 4 ? rot.a_off + 2 * i : rot.b_off + 2 * (i - 4));
-      *reinterpret_cast<uint64_t*>(&part[4 * warp + oct][dim]) = acc[kind][i];
-    }
+    for (int i = 0; i < 16; ++i)
+      part[4 * warp + oct][i < 8 ? rot.a_off + i : rot.b_off + i - 8] = acc[kind][i];
     __syncthreads();
     float s = 0.f;
 #pragma unroll
