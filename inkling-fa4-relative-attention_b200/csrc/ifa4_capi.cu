@@ -1205,18 +1205,43 @@ int validate_qk_norm_rope_backward(const IFA4QkNormRopeBackwardParams* p) {
 }
 
 // Units, blocks and workspace of the backward.
-int plan_qk_backward(const IFA4QkNormRopeBackwardParams* p, int* parts, int* blocks,
-                     size_t* bytes) {
+struct QkBackwardPlan {
+  int unit_quads, q_parts, k_parts;
+  int q_blocks, blocks;
+  size_t bytes;
+};
+int plan_qk_backward(const IFA4QkNormRopeBackwardParams* p, QkBackwardPlan* plan) {
   int sms = 148;
   int rc = sm_count(&sms);
   if (rc) return rc;
-  const int rows = p->n_heads > p->kv_heads ? p->n_heads : p->kv_heads;
-  *parts = p->total_q > 0 && rows > 0 ? token_parts(p->total_q, rows, sms) : 1;
-  const int64_t want = (p->total_q * *parts + ifa4::kQkvBackwardWarps - 1) / ifa4::kQkvBackwardWarps;
+  const int q_quads = (p->n_heads + 3) / 4, k_quads = (p->kv_heads + 3) / 4;
+  const int64_t quads = p->total_q * (q_quads + k_quads);
+  *plan = QkBackwardPlan{};
+  // units of up to eight quads, fewer where that leaves warps (about 16 per SM) without any
+  const int64_t per = quads / (16LL * sms);
+  plan->unit_quads = static_cast<int>(per < 1 ? 1 : (per > 8 ? 8 : per));
+  plan->q_parts = (q_quads + plan->unit_quads - 1) / plan->unit_quads;
+  plan->k_parts = (k_quads + plan->unit_quads - 1) / plan->unit_quads;
+  // blocks in proportion to the work: a unit's start (place, angles) costs about half a quad
   const int64_t cap = static_cast<int64_t>(sms) * ifa4::kQkvBackwardBlocksPerSm;
-  *blocks = static_cast<int>(want < 1 ? 1 : (want < cap ? want : cap));
-  *bytes = p->dq_weight != nullptr || p->dk_weight != nullptr
-               ? static_cast<size_t>(*blocks) * 256 * sizeof(float) : 0;
+  auto blocks_for = [](int64_t units) {
+    return (units + ifa4::kQkvBackwardWarps - 1) / ifa4::kQkvBackwardWarps;
+  };
+  int64_t q_blocks = blocks_for(p->total_q * plan->q_parts);
+  int64_t k_blocks = blocks_for(p->total_q * plan->k_parts);
+  if (q_blocks + k_blocks > cap) {
+    const int64_t q_work = 2 * q_quads + plan->q_parts, k_work = 2 * k_quads + plan->k_parts;
+    int64_t q = (cap * q_work + (q_work + k_work) / 2) / (q_work + k_work);
+    if (k_blocks > 0 && q > cap - 1) q = cap - 1;
+    if (q_blocks > 0 && q < 1) q = 1;
+    if (q < q_blocks) q_blocks = q;
+    if (cap - q < k_blocks) k_blocks = cap - q;
+  }
+  plan->q_blocks = static_cast<int>(q_blocks);
+  plan->blocks = static_cast<int>(q_blocks + k_blocks);
+  if (plan->blocks < 1) plan->blocks = 1;  // nothing to do: one block writes the zeros
+  if (p->dq_weight != nullptr || p->dk_weight != nullptr)
+    plan->bytes = static_cast<size_t>(plan->blocks) * 128 * sizeof(float);
   return IFA4_OK;
 }
 }  // namespace
@@ -1252,8 +1277,10 @@ int ifa4_qk_norm_rope_backward_workspace_size(const IFA4QkNormRopeBackwardParams
     return fail(IFA4_ERR_INVALID_ARGUMENT, "qk_norm_rope_backward: bytes_out is NULL");
   int rc = validate_qk_norm_rope_backward(p);
   if (rc) return rc;
-  int parts, blocks;
-  return plan_qk_backward(p, &parts, &blocks, bytes_out);
+  QkBackwardPlan plan;
+  if ((rc = plan_qk_backward(p, &plan))) return rc;
+  *bytes_out = plan.bytes;
+  return IFA4_OK;
 }
 
 int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, void* workspace,
@@ -1261,10 +1288,10 @@ int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, voi
   g_last_error[0] = '\0';
   int rc = validate_qk_norm_rope_backward(p);
   if (rc) return rc;
-  int parts, blocks;
-  size_t bytes;
-  if ((rc = plan_qk_backward(p, &parts, &blocks, &bytes))) return rc;
-  if (p->total_q == 0 && bytes == 0) return IFA4_OK;
+  QkBackwardPlan plan;
+  if ((rc = plan_qk_backward(p, &plan))) return rc;
+  const size_t bytes = plan.bytes;
+  if (bytes == 0 && (p->total_q == 0 || p->n_heads + p->kv_heads == 0)) return IFA4_OK;
   if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
     return fail(IFA4_ERR_WORKSPACE, "qk_norm_rope_backward: workspace of %zu bytes required, got %zu",
                 bytes, workspace_bytes);
@@ -1297,7 +1324,7 @@ int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, voi
   a.dq_sh = p->dq_stride_h;
   a.dk_st = p->dk_stride_t;
   a.dk_sh = p->dk_stride_h;
-  a.units = p->total_q * parts;
+  a.total_q = p->total_q;
   a.batch = p->batch;
   a.n_heads = p->n_heads;
   a.kv_heads = p->kv_heads;
@@ -1306,11 +1333,12 @@ int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* p, voi
   a.normalize = p->normalize ? 1 : 0;
   a.weight_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
   a.inv_freq_f32 = p->inv_freq_f32 ? 1 : 0;
-  a.parts = parts;
-  a.q_per_part = round4((p->n_heads + parts - 1) / parts);
-  a.k_per_part = round4((p->kv_heads + parts - 1) / parts);
+  a.q_blocks = plan.q_blocks;
+  a.unit_quads = plan.unit_quads;
+  a.q_parts = plan.q_parts;
+  a.k_parts = plan.k_parts;
   a.eps = p->eps;
-  cudaError_t e = ifa4::launch_qkv_backward_sm100(a, blocks, static_cast<cudaStream_t>(stream));
+  cudaError_t e = ifa4::launch_qkv_backward_sm100(a, plan.blocks, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_backward launch");
   return IFA4_OK;
 }

@@ -243,12 +243,14 @@ struct QkvBackwardKernelArgs {
   const void* inv_freq;
   const int32_t* cu_q;
   const int32_t* cu_k;
-  float* partial;            // [blocks, 2, 128] (null: no weight gradients)
+  float* partial;            // [blocks, 128], q's first (null: no weight gradients)
   long long dqo_st, dqo_sh, dko_st, dko_sh, q_st, q_sh, k_st, k_sh, dq_st, dq_sh, dk_st, dk_sh;
-  long long units;
+  long long total_q;
   int batch, n_heads, kv_heads;
   int rotary_dim, interleaved, normalize, weight_f32, inv_freq_f32;
-  int parts, q_per_part, k_per_part;
+  int q_blocks;              // the first blocks work on q, the others on k
+  int unit_quads;            // most quads (four rows) of a unit
+  int q_parts, k_parts;      // units of a token's q, and of its k
   float eps;
 };
 

@@ -18,13 +18,17 @@
 // depend on the token only: they are computed once per unit (two pairs a lane), handed round
 // through shared memory and kept in registers for all rows.
 //
-// HBM bound in bytes, but close to the issue rate: a quad of rows takes about 270 instructions, 68 %
-// of the issue slots at 32k tokens x 40 heads (671 MB in 123 us, 5.4 TB/s; backward 1007 MB in
-// 197 us, 5.1 TB/s).  Measured and slower there: half a warp per row with the pairs exchanged by
-// shuffles 187 us (backward 293); equal runs of quads per warp over token borders 130; whole tokens
-// in turn with an evenly cut rest 157 (its cursors cost more than the balance gives); one loop per
-// kind of row (spills) 174; the next token streamed by cp.async into shared memory, 8 warps per SM,
-// 126 (interleaved pairs 191 instead of 133, append 114 instead of 83, backward 215).
+// HBM bound in bytes (671 MB at 32k tokens x 40 heads in 118 us, 5.7 TB/s, where the rotation alone
+// runs at 6.1 and a device copy at 6.55), held back by the work per row: 20 warps per SM keep some
+// 40 KB of loads in flight, and a quad takes over 200 instructions and a chain of three shuffles
+// and a reciprocal root.  The append writes its rows to pages (402 MB in 81 us, 5.0 TB/s; 5.9 for
+// the copies alone), the backward (1007 MB) takes 184 us, 5.5 TB/s.  Measured and slower at those
+// sizes: half a warp per row with the pairs exchanged by shuffles 187 us (backward 293); 16
+// neighbouring dims a lane, whose accesses cover half sectors, for interleaved pairs 129 instead of
+// 105 (30011 tokens); equal runs of quads per warp over token borders 130; whole tokens in turn with
+// an evenly cut rest 157; one loop per kind of row (spills) 174; units of one kind, all q first,
+// 121-125; the next token streamed by cp.async into shared memory, 8 warps per SM, 126 (append
+// 114); backward warps that do q and k rows, with two sets of sums, 194.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -332,127 +336,135 @@ __global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
 // Gradients.  With g = R^T dout, xhat = x * r, r = rsqrt(mean x^2 + eps):
 //   dw = sum over tokens and heads of g * xhat
 //   dx = r * (g w - xhat * mean(g w xhat)) = r * g w - x * r^3 * mean(g w x)
-// r is recomputed from x (nothing is saved by the forward).  Each lane keeps the sums of dw of
-// its dims and rows in registers; a block adds its rows' lanes in a fixed order and writes one
-// partial per weight vector, and qkv_weight_grad_kernel adds the blocks' partials, again in a
-// fixed order: no atomics, the same result every time.
+// r is recomputed from x (nothing is saved by the forward).  A block works on q rows or on k rows
+// only (the blocks are shared out by the work of the two), so a lane keeps one set of 16 sums of dw
+// in registers; a block adds its lanes in a fixed order and writes one partial, and
+// qkv_weight_grad_kernel adds the blocks' partials, again in a fixed order: no atomics, the same
+// result every time.
 template <int kRot>
 __global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
     qkv_backward_kernel(const __grid_constant__ QkvBackwardKernelArgs a) {
-  __shared__ __align__(16) float ws[2][128];
+  __shared__ __align__(16) float ws[128];
   __shared__ __align__(16) float2 angles[kWarps][64];
   __shared__ __align__(16) float part[4 * kWarps][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int oct = lane >> 3;
+  const bool is_q = blockIdx.x < a.q_blocks;
+  const int block = is_q ? blockIdx.x : blockIdx.x - a.q_blocks;
+  const int blocks = is_q ? a.q_blocks : gridDim.x - a.q_blocks;
   Rotation<kRot> rot;
   rot.init(a.inv_freq, a.inv_freq_f32, a.rotary_dim, lane);
-  ws[0][threadIdx.x] = load_weight(a.q_weight, a.weight_f32, threadIdx.x);
-  ws[1][threadIdx.x] = load_weight(a.k_weight, a.weight_f32, threadIdx.x);
+  ws[threadIdx.x] = load_weight(is_q ? a.q_weight : a.k_weight, a.weight_f32, threadIdx.x);
   __syncthreads();
-  float acc[2][16];
+  const int heads = is_q ? a.n_heads : a.kv_heads;
+  const int quads = (heads + 3) / 4;
+  const int parts = is_q ? a.q_parts : a.k_parts;
+  const uint16_t* const xb = is_q ? a.q : a.k;
+  const uint16_t* const gb = is_q ? a.dq_out : a.dk_out;
+  uint16_t* const ob = is_q ? a.dq : a.dk;
+  const long long x_st = is_q ? a.q_st : a.k_st, x_sh = is_q ? a.q_sh : a.k_sh;
+  const long long g_st = is_q ? a.dqo_st : a.dko_st, g_sh = is_q ? a.dqo_sh : a.dko_sh;
+  const long long o_st = is_q ? a.dq_st : a.dk_st, o_sh = is_q ? a.dq_sh : a.dk_sh;
+  float acc[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = 0.f;
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
 
-  const long long step = static_cast<long long>(gridDim.x) * kWarps;
-  for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp; u < a.units; u += step) {
-    const long long t = a.parts == 1 ? u : u / a.parts;
-    const int part_i = static_cast<int>(u - t * a.parts);
+  const long long units = a.total_q * parts;
+  const long long step = static_cast<long long>(blocks) * kWarps;
+  for (long long u = static_cast<long long>(block) * kWarps + warp; u < units; u += step) {
+    const long long t = parts == 1 ? u : u / parts;
+    const int j0 = static_cast<int>(u - t * parts) * a.unit_quads;
+    const int r1 = min(heads, 4 * min(j0 + a.unit_quads, quads));
+    int ri = 4 * j0 + oct;
+    const uint16_t* x_p = xb + t * x_st + ri * x_sh;
+    const uint16_t* g_p = gb + t * g_st + ri * g_sh;
+    uint16_t* o_p = ob + t * o_st + ri * o_sh;
+    uint4 raw[4];  // x, dout of the next four rows
+    auto load = [&](int row) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < r1) {
+        raw[0] = ldg_v4(x_p + rot.a_off);
+        raw[1] = ldg_v4(x_p + rot.b_off);
+        raw[2] = ldg_v4(g_p + rot.a_off);
+        raw[3] = ldg_v4(g_p + rot.b_off);
+      }
+      x_p += 4 * x_sh;
+      g_p += 4 * g_sh;
+    };
+    load(ri);
     const Where w = locate(a.cu_q, a.cu_k, a.batch, t, lane);
     rot.at(w.pos, lane, angles[warp]);
+    for (int r = 4 * j0; r < r1; r += 4, ri += 4) {
+      const bool on = ri < r1 && w.inside;  // a row that is none has r = rsqrt(eps), maybe inf
+      float x[16], g[16];
+      unpack8(raw[0], x);
+      unpack8(raw[1], x + 8);
+      unpack8(raw[2], g);
+      unpack8(raw[3], g + 8);
+      if (r + 4 < r1) load(ri + 4);
+      rot.template apply<true>(g);
+      if (a.normalize) {
+        float wt[16];
+        lane_weights(ws, rot.a_off, rot.b_off, wt);
+        float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-      const int heads = kind == 0 ? a.n_heads : a.kv_heads;
-      const int per = kind == 0 ? a.q_per_part : a.k_per_part;
-      const int r0 = part_i * per, r1 = min(heads, r0 + per);
-      const uint16_t* const xt = kind == 0 ? a.q + t * a.q_st : a.k + t * a.k_st;
-      const uint16_t* const gt = kind == 0 ? a.dq_out + t * a.dqo_st : a.dk_out + t * a.dko_st;
-      uint16_t* const ot = kind == 0 ? a.dq + t * a.dq_st : a.dk + t * a.dk_st;
-      const long long x_sh = kind == 0 ? a.q_sh : a.k_sh, g_sh = kind == 0 ? a.dqo_sh : a.dko_sh;
-      const long long o_sh = kind == 0 ? a.dq_sh : a.dk_sh;
-      uint4 raw[4];  // x, dout of the next four rows
-      auto load = [&](int r) {
-        const int ri = r + oct;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (ri < r1 && w.inside) {
-          raw[0] = ldg_v4(xt + ri * x_sh + rot.a_off);
-          raw[1] = ldg_v4(xt + ri * x_sh + rot.b_off);
-          raw[2] = ldg_v4(gt + ri * g_sh + rot.a_off);
-          raw[3] = ldg_v4(gt + ri * g_sh + rot.b_off);
+        for (int i = 0; i < 16; ++i) {
+          ss += x[i] * x[i];
+          dot += g[i] * wt[i] * x[i];
         }
-      };
-      if (r0 < r1) load(r0);
-      for (int r = r0; r < r1; r += 4) {
-        const int ri = r + oct;
-        const bool on = ri < r1 && w.inside;  // a row that is none has r = rsqrt(eps), maybe inf
-        float x[16], g[16];
-        unpack8(raw[0], x);
-        unpack8(raw[1], x + 8);
-        unpack8(raw[2], g);
-        unpack8(raw[3], g + 8);
-        if (r + 4 < r1) load(r + 4);
-        rot.template apply<true>(g);
-        if (a.normalize) {
-          float wt[16];
-          lane_weights(ws[kind], rot.a_off, rot.b_off, wt);
-          float ss = 0.f, dot = 0.f;
+        const float rn = rsqrtf(row_sum(ss) * (1.f / 128.f) + a.eps);
+        const float back = row_sum(dot) * (1.f / 128.f) * rn * rn;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            ss += x[i] * x[i];
-            dot += g[i] * wt[i] * x[i];
-          }
-          const float rn = rsqrtf(row_sum(ss) * (1.f / 128.f) + a.eps);
-          const float back = row_sum(dot) * (1.f / 128.f) * rn * rn;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (on) acc[kind][i] += g[i] * (x[i] * rn);
-            g[i] = rn * (g[i] * wt[i] - x[i] * back);
-          }
-        }
-        if (ri < r1) {
-          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.a_off) = on ? pack8(g) : z;
-          *reinterpret_cast<uint4*>(ot + ri * o_sh + rot.b_off) = on ? pack8(g + 8) : z;
+        for (int i = 0; i < 16; ++i) {
+          if (on) acc[i] += g[i] * (x[i] * rn);
+          g[i] = rn * (g[i] * wt[i] - x[i] * back);
         }
       }
+      if (ri < r1) {
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(o_p + rot.a_off) = on ? pack8(g) : z;
+        *reinterpret_cast<uint4*>(o_p + rot.b_off) = on ? pack8(g + 8) : z;
+      }
+      o_p += 4 * o_sh;
     }
   }
   if (a.partial == nullptr) return;
 #pragma unroll
-  for (int kind = 0; kind < 2; ++kind) {
-    __syncthreads();
+  for (int i = 0; i < 16; ++i)
+    part[4 * warp + oct][i < 8 ? rot.a_off + i : rot.b_off + i - 8] = acc[i];
+  __syncthreads();
+  float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      part[4 * warp + oct][i < 8 ? rot.a_off + i : rot.b_off + i - 8] = acc[kind][i];
-    __syncthreads();
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4 * kWarps; ++i) s += part[i][threadIdx.x];
-    a.partial[(static_cast<long long>(blockIdx.x) * 2 + kind) * 128 + threadIdx.x] = s;
-  }
+  for (int i = 0; i < 4 * kWarps; ++i) sum += part[i][threadIdx.x];
+  a.partial[static_cast<long long>(blockIdx.x) * 128 + threadIdx.x] = sum;
 }
 
-// Sum of the blocks' partials: block c adds columns 32 c .. 32 c + 31 of the 256 (q, then k).
-__global__ void __launch_bounds__(1024) qkv_weight_grad_kernel(const float* partial, int blocks,
-                                                               void* dq_weight, void* dk_weight,
-                                                               int f32) {
+// Sum of the blocks' partials ([q_blocks][128], then those of k): block c adds 32 columns of q
+// (c < 4) or of k.
+__global__ void __launch_bounds__(1024) qkv_weight_grad_kernel(const float* partial, int q_blocks,
+                                                               int blocks, void* dq_weight,
+                                                               void* dk_weight, int f32) {
   __shared__ float s[32][33];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), lane_row = threadIdx.x >> 5;
+  const bool is_q = blockIdx.x < 4;
+  const int col = (blockIdx.x & 3) * 32 + (threadIdx.x & 31), lane_row = threadIdx.x >> 5;
+  const int first = is_q ? 0 : q_blocks, last = is_q ? q_blocks : blocks;
   float acc = 0.f;
-  for (int i = lane_row; i < blocks; i += 32) acc += partial[static_cast<long long>(i) * 256 + col];
+  for (int i = first + lane_row; i < last; i += 32)
+    acc += partial[static_cast<long long>(i) * 128 + col];
   s[lane_row][threadIdx.x & 31] = acc;
   __syncthreads();
   if (lane_row == 0) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) sum += s[i][threadIdx.x];
-    void* dst = col < 128 ? dq_weight : dk_weight;
+    void* dst = is_q ? dq_weight : dk_weight;
     if (dst == nullptr) return;
     if (f32) {
-      static_cast<float*>(dst)[col & 127] = sum;
+      static_cast<float*>(dst)[col] = sum;
     } else {
       __nv_bfloat16 v = __float2bfloat16_rn(sum);
-      static_cast<uint16_t*>(dst)[col & 127] = *reinterpret_cast<uint16_t*>(&v);
+      static_cast<uint16_t*>(dst)[col] = *reinterpret_cast<uint16_t*>(&v);
     }
   }
 }
@@ -513,8 +525,8 @@ cudaError_t launch_qkv_backward_sm100(const QkvBackwardKernelArgs& args, int blo
     qkv::qkv_backward_kernel<qkv::kRotPairs><<<blocks, qkv::kThreads, 0, stream>>>(args);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || args.partial == nullptr) return e;
-  qkv::qkv_weight_grad_kernel<<<8, 1024, 0, stream>>>(args.partial, blocks, args.dq_weight,
-                                                      args.dk_weight, args.weight_f32);
+  qkv::qkv_weight_grad_kernel<<<8, 1024, 0, stream>>>(
+      args.partial, args.q_blocks, blocks, args.dq_weight, args.dk_weight, args.weight_f32);
   return cudaGetLastError();
 }
 
