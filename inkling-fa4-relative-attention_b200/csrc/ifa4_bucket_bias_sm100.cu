@@ -214,9 +214,9 @@ void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms) {
   const long long col_blocks =
       static_cast<long long>((a->n_heads + heads - 1) / heads) * a->col_parts;
   // one resident wave of blocks (four per SM; 32k tokens x 32 heads x 128: 52 us, 62 us with two
-  // waves of half the tokens), at least 16 tokens per lane
+  // waves of half the tokens), at least 32 tokens per lane (one chunk needs no second kernel)
   long long chunks = 4ll * sms / col_blocks;
-  const long long most = (a->total_q + 16ll * a->lanes - 1) / (16ll * a->lanes);
+  const long long most = (a->total_q + 32ll * a->lanes - 1) / (32ll * a->lanes);
   if (chunks > most) chunks = most;
   if (chunks < 1) chunks = 1;
   if (chunks > 65535) chunks = 65535;

@@ -1,5 +1,5 @@
-// torch operators over the C ABI: inkling_fa4::prefill_, decode_, decode_shared_prefix_,
-// qk_norm_rope_, qk_norm_rope_backward_, kv_append_, bucket_bias_ and bucket_bias_backward_.
+// torch operators over the C ABI: inkling_fa4::prefill_ and decode_, and (at the end of the file) the
+// operators next to the attention.
 //
 // The Python package checks its arguments (the reference's call surface and error messages) and
 // then calls one of these operators, which fills the IFA4 parameter block from the tensors'
@@ -13,6 +13,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
+
+#include <vector>
 
 #include "../../include/inkling_fa4.h"
 
@@ -185,46 +187,66 @@ int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             need > 0 ? static_cast<size_t>(ws.nbytes()) : 0, stream);
 }
 
-int64_t decode_shared_prefix_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                const at::Tensor& rel, const at::Tensor& out,
-                                const at::Tensor& cu_q, const at::Tensor& cu_k,
-                                const c10::optional<at::Tensor>& lse,
-                                const at::Tensor& block_table,
-                                const c10::optional<at::Tensor>& workspace, int64_t rel_extent,
-                                int64_t window_left, int64_t max_seqlen_k, double softmax_scale,
-                                int64_t num_splits, int64_t chunk_len, int64_t shared_prefix_len,
-                                int64_t prefix_splits) {
-  const c10::cuda::CUDAGuard guard(q.device());
-  IFA4SharedPrefixParams p{};
-  p.decode = decode_params(q, k, v, rel, out, cu_q, cu_k, lse, block_table, rel_extent, true,
-                           window_left, IFA4_ALIGN_BOTTOM_RIGHT, max_seqlen_k, softmax_scale,
-                           num_splits, chunk_len);
-  p.shared_prefix_len = static_cast<int32_t>(shared_prefix_len);
-  p.prefix_splits = static_cast<int32_t>(prefix_splits);
-  void* stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
-  size_t need = 0;
-  int rc = ifa4_decode_shared_prefix_workspace_size(&p, &need);
-  if (rc) return rc;
-  at::Tensor ws;
-  if (need > 0) {
-    if (workspace.has_value() && static_cast<size_t>(workspace->nbytes()) >= need)
-      ws = *workspace;
-    else
-      ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
-  }
-  return ifa4_decode_shared_prefix_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream);
+// ---------------------------------------------------------------------------------------------
+// Operators next to the attention.  Each takes the arguments of its Python entry point as they are,
+// decides whether they are the plain case (types, shapes, one device, layouts the kernels read in
+// place), allocates the outputs, launches and returns them; anything else, failed launches among it,
+// returns an empty list, and the entry point then goes through its own checks and the C ABI, which
+// copy what has to be copied and say what is wrong.  So the usual call costs one dispatcher call.
+// ---------------------------------------------------------------------------------------------
+typedef std::vector<at::Tensor> Tensors;
+typedef c10::optional<at::Tensor> MaybeTensor;
+
+const void* ptr_or_null(const MaybeTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+void* stream_of(const at::Tensor& t) {
+  return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
+}
+at::Tensor bytes_like(const at::Tensor& t, size_t n) {
+  return at::empty({static_cast<int64_t>(n)}, t.options().dtype(at::kByte));
+}
+at::Tensor rows_like(const at::Tensor& t) {  // contiguous, same sizes
+  return at::empty(t.sizes(), t.options());
 }
 
-const void* ptr_or_null(const c10::optional<at::Tensor>& t) {
-  return t.has_value() ? t->data_ptr() : nullptr;
+// [tokens, heads, 128] bf16 rows the kernels read in place.
+bool plain_rows(const at::Tensor& t, const at::Tensor& like) {
+  return t.dim() == 3 && t.size(2) == 128 && t.scalar_type() == at::kBFloat16 &&
+         t.device() == like.device() && t.size(0) == like.size(0) && t.stride(2) == 1 &&
+         t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned16(t);
+}
+bool plain_cu(const MaybeTensor& t, const at::Tensor& like) {
+  return !t.has_value() || (t->dim() == 1 && t->numel() >= 2 && t->scalar_type() == at::kInt &&
+                            t->device() == like.device() && t->stride(0) == 1);
+}
+bool plain_weight(const MaybeTensor& t, const at::Tensor& like) {
+  return !t.has_value() ||
+         (t->dim() == 1 && t->numel() == 128 && t->stride(0) == 1 && t->device() == like.device() &&
+          (t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat));
+}
+// The step's other arguments.  eps < 0: no norm.
+bool plain_step(const at::Tensor& like, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
+                const MaybeTensor& inv_freq, const MaybeTensor& cu_q, const MaybeTensor& cu_k,
+                double eps) {
+  if (!plain_cu(cu_q, like) || !plain_cu(cu_k, like) || !plain_weight(q_weight, like) ||
+      !plain_weight(k_weight, like))
+    return false;
+  if (cu_k.has_value() && (!cu_q.has_value() || cu_k->numel() != cu_q->numel())) return false;
+  if (q_weight.has_value() && k_weight.has_value() &&
+      q_weight->scalar_type() != k_weight->scalar_type())
+    return false;
+  if (!(eps >= 0) && (q_weight.has_value() || k_weight.has_value())) return false;
+  if (!inv_freq.has_value()) return true;
+  return inv_freq->dim() == 1 && inv_freq->numel() > 0 && inv_freq->numel() <= 64 &&
+         inv_freq->numel() % 8 == 0 && inv_freq->stride(0) == 1 &&
+         inv_freq->device() == like.device() &&
+         (inv_freq->scalar_type() == at::kDouble || inv_freq->scalar_type() == at::kFloat);
 }
 
-// The fields the norm-and-rotation parameter blocks share.  eps < 0: no norm.
+// The fields the norm-and-rotation parameter blocks share.
 template <class P>
-void fill_norm_rope(P* p, const c10::optional<at::Tensor>& q_weight,
-                    const c10::optional<at::Tensor>& k_weight,
-                    const c10::optional<at::Tensor>& inv_freq,
-                    const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
+void fill_norm_rope(P* p, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
+                    const MaybeTensor& inv_freq, const MaybeTensor& cu_q, const MaybeTensor& cu_k,
                     int64_t total_q, int64_t heads, int64_t kv_heads, bool interleaved,
                     double eps) {
   p->q_weight = ptr_or_null(q_weight);
@@ -240,7 +262,7 @@ void fill_norm_rope(P* p, const c10::optional<at::Tensor>& q_weight,
   p->rotary_dim = inv_freq.has_value() ? static_cast<int32_t>(2 * inv_freq->numel()) : 0;
   p->interleaved = interleaved;
   p->normalize = eps >= 0;
-  const c10::optional<at::Tensor>& w = q_weight.has_value() ? q_weight : k_weight;
+  const MaybeTensor& w = q_weight.has_value() ? q_weight : k_weight;
   p->weight_dtype = w.has_value() && w->scalar_type() == at::kFloat ? IFA4_WEIGHT_F32
                                                                     : IFA4_WEIGHT_BF16;
   p->inv_freq_f32 = inv_freq.has_value() && inv_freq->scalar_type() == at::kFloat;
@@ -248,13 +270,15 @@ void fill_norm_rope(P* p, const c10::optional<at::Tensor>& q_weight,
   p->eps = eps >= 0 ? static_cast<float>(eps) : 0.f;
 }
 
-int64_t qk_norm_rope_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_out,
-                        const at::Tensor& k_out, const c10::optional<at::Tensor>& q_weight,
-                        const c10::optional<at::Tensor>& k_weight,
-                        const c10::optional<at::Tensor>& inv_freq,
-                        const c10::optional<at::Tensor>& cu_q,
-                        const c10::optional<at::Tensor>& cu_k, bool interleaved, double eps) {
+Tensors qk_norm_rope_op(const at::Tensor& q, const at::Tensor& k, const MaybeTensor& q_weight,
+                        const MaybeTensor& k_weight, const MaybeTensor& inv_freq,
+                        const MaybeTensor& cu_q, const MaybeTensor& cu_k, bool interleaved,
+                        double eps) {
+  if (!plain_rows(q, q) || !plain_rows(k, q) || !(eps >= 0 || inv_freq.has_value()) ||
+      !plain_step(q, q_weight, k_weight, inv_freq, cu_q, cu_k, eps))
+    return {};
   const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor q_out = rows_like(q), k_out = rows_like(k);
   IFA4QkNormRopeParams p{};
   fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, q.size(0), q.size(1), k.size(1),
                  interleaved, eps);
@@ -271,29 +295,40 @@ int64_t qk_norm_rope_op(const at::Tensor& q, const at::Tensor& k, const at::Tens
   p.k_out_stride_t = k_out.stride(0);
   p.k_out_stride_h = k_out.stride(1);
   p.zero_padding = 1;
-  return ifa4_qk_norm_rope_launch(&p,
-                                  c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+  if (ifa4_qk_norm_rope_launch(&p, stream_of(q))) return {};
+  return {q_out, k_out};
 }
 
-int64_t qk_norm_rope_backward_op(
-    const at::Tensor& dq_out, const at::Tensor& dk_out, const at::Tensor& q, const at::Tensor& k,
-    const at::Tensor& dq, const at::Tensor& dk, const c10::optional<at::Tensor>& q_weight,
-    const c10::optional<at::Tensor>& k_weight, const c10::optional<at::Tensor>& dq_weight,
-    const c10::optional<at::Tensor>& dk_weight, const c10::optional<at::Tensor>& inv_freq,
-    const c10::optional<at::Tensor>& cu_q, const c10::optional<at::Tensor>& cu_k,
-    bool interleaved, double eps) {
+// Returns dq, dk and the gradients of the weights that are there and wanted.
+Tensors qk_norm_rope_backward_op(const at::Tensor& dq_out, const at::Tensor& dk_out,
+                                 const at::Tensor& q, const at::Tensor& k,
+                                 const MaybeTensor& q_weight, const MaybeTensor& k_weight,
+                                 const MaybeTensor& inv_freq, const MaybeTensor& cu_q,
+                                 const MaybeTensor& cu_k, bool interleaved, double eps,
+                                 bool want_q_weight, bool want_k_weight) {
+  if (!plain_rows(q, q) || !plain_rows(k, q) || !plain_rows(dq_out, q) || !plain_rows(dk_out, q) ||
+      dq_out.size(1) != q.size(1) || dk_out.size(1) != k.size(1) ||
+      !plain_step(q, q_weight, k_weight, inv_freq, cu_q, cu_k, eps))
+    return {};
   const c10::cuda::CUDAGuard guard(q.device());
+  Tensors out{rows_like(q), rows_like(k)};
   IFA4QkNormRopeBackwardParams p{};
   fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, q.size(0), q.size(1), k.size(1),
                  interleaved, eps);
+  if (q_weight.has_value() && want_q_weight) {
+    out.push_back(at::empty_like(*q_weight));
+    p.dq_weight = out.back().data_ptr();
+  }
+  if (k_weight.has_value() && want_k_weight) {
+    out.push_back(at::empty_like(*k_weight));
+    p.dk_weight = out.back().data_ptr();
+  }
   p.dq_out = dq_out.data_ptr();
   p.dk_out = dk_out.data_ptr();
   p.q = q.data_ptr();
   p.k = k.data_ptr();
-  p.dq = dq.data_ptr();
-  p.dk = dk.data_ptr();
-  p.dq_weight = dq_weight.has_value() ? dq_weight->data_ptr() : nullptr;
-  p.dk_weight = dk_weight.has_value() ? dk_weight->data_ptr() : nullptr;
+  p.dq = out[0].data_ptr();
+  p.dk = out[1].data_ptr();
   p.dq_out_stride_t = dq_out.stride(0);
   p.dq_out_stride_h = dq_out.stride(1);
   p.dk_out_stride_t = dk_out.stride(0);
@@ -302,39 +337,54 @@ int64_t qk_norm_rope_backward_op(
   p.q_stride_h = q.stride(1);
   p.k_stride_t = k.stride(0);
   p.k_stride_h = k.stride(1);
-  p.dq_stride_t = dq.stride(0);
-  p.dq_stride_h = dq.stride(1);
-  p.dk_stride_t = dk.stride(0);
-  p.dk_stride_h = dk.stride(1);
+  p.dq_stride_t = out[0].stride(0);
+  p.dq_stride_h = out[0].stride(1);
+  p.dk_stride_t = out[1].stride(0);
+  p.dk_stride_h = out[1].stride(1);
   size_t need = 0;
-  const int rc = ifa4_qk_norm_rope_backward_workspace_size(&p, &need);
-  if (rc) return rc;
+  if (ifa4_qk_norm_rope_backward_workspace_size(&p, &need)) return {};
   at::Tensor ws;
-  if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
-  return ifa4_qk_norm_rope_backward_launch(
-      &p, need > 0 ? ws.data_ptr() : nullptr, need,
-      c10::cuda::getCurrentCUDAStream(q.device().index()).stream());
+  if (need > 0) ws = bytes_like(q, need);
+  if (ifa4_qk_norm_rope_backward_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(q)))
+    return {};
+  return out;
 }
 
-int64_t kv_append_op(const c10::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
-                     const c10::optional<at::Tensor>& q_out, const at::Tensor& k_cache,
-                     const at::Tensor& v_cache, const c10::optional<at::Tensor>& q_weight,
-                     const c10::optional<at::Tensor>& k_weight,
-                     const c10::optional<at::Tensor>& inv_freq, const at::Tensor& cu_q,
-                     const at::Tensor& cu_k, const at::Tensor& block_table, bool interleaved,
-                     double eps, bool zero_padding) {
+// The append with its queries; returns q_out.
+Tensors kv_append_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                     const at::Tensor& k_cache, const at::Tensor& v_cache,
+                     const MaybeTensor& q_weight, const MaybeTensor& k_weight,
+                     const MaybeTensor& inv_freq, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                     const at::Tensor& block_table, bool interleaved, double eps) {
+  if (!plain_rows(k, k) || !plain_rows(v, k) || !plain_rows(q, k) || v.size(1) != k.size(1) ||
+      !plain_step(k, q_weight, k_weight, inv_freq, cu_q, cu_k, eps))
+    return {};
+  for (const at::Tensor* c : {&k_cache, &v_cache})
+    if (c->dim() != 4 || c->scalar_type() != at::kBFloat16 || c->device() != k.device() ||
+        c->size(2) != k.size(1) || c->size(3) != 128 || c->stride(3) != 1 || !aligned16(*c))
+      return {};
+  for (int i = 0; i < 3; ++i)
+    if (k_cache.stride(i) <= 0 || k_cache.stride(i) % 8 != 0 || v_cache.stride(i) <= 0 ||
+        v_cache.stride(i) % 8 != 0)
+      return {};
+  const int64_t page_size = k_cache.size(1);
+  if (v_cache.sizes() != k_cache.sizes() || k_cache.data_ptr() == v_cache.data_ptr() ||
+      page_size < 16 || (page_size & (page_size - 1)) != 0 || block_table.dim() != 2 ||
+      block_table.scalar_type() != at::kInt || block_table.device() != k.device() ||
+      block_table.size(0) != cu_q.numel() - 1 || block_table.numel() == 0 ||
+      block_table.stride(1) != 1)
+    return {};
   const c10::cuda::CUDAGuard guard(k.device());
+  const at::Tensor q_out = rows_like(q);
   IFA4KvAppendParams p{};
-  fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, k.size(0),
-                 q.has_value() ? q->size(1) : 0, k.size(1), interleaved, eps);
-  if (q.has_value()) {
-    p.q = q->data_ptr();
-    p.q_out = q_out->data_ptr();
-    p.q_stride_t = q->stride(0);
-    p.q_stride_h = q->stride(1);
-    p.q_out_stride_t = q_out->stride(0);
-    p.q_out_stride_h = q_out->stride(1);
-  }
+  fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, k.size(0), q.size(1), k.size(1),
+                 interleaved, eps);
+  p.q = q.data_ptr();
+  p.q_out = q_out.data_ptr();
+  p.q_stride_t = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.q_out_stride_t = q_out.stride(0);
+  p.q_out_stride_h = q_out.stride(1);
   p.k = k.data_ptr();
   p.v = v.data_ptr();
   p.k_cache = k_cache.data_ptr();
@@ -351,19 +401,86 @@ int64_t kv_append_op(const c10::optional<at::Tensor>& q, const at::Tensor& k, co
   p.v_cache_stride_h = v_cache.stride(2);
   p.block_table = static_cast<const int32_t*>(block_table.data_ptr());
   p.block_table_stride = block_table.stride(0);
-  p.zero_padding = zero_padding;
-  p.page_size = static_cast<int32_t>(k_cache.size(1));
+  p.zero_padding = 1;
+  p.page_size = static_cast<int32_t>(page_size);
   p.num_pages = static_cast<int32_t>(k_cache.size(0));
   p.table_width = static_cast<int32_t>(block_table.size(1));
-  return ifa4_kv_append_launch(&p, c10::cuda::getCurrentCUDAStream(k.device().index()).stream());
+  if (ifa4_kv_append_launch(&p, stream_of(k))) return {};
+  return {q_out};
+}
+
+// Returns out.
+Tensors decode_shared_prefix_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                const at::Tensor& rel, const at::Tensor& cu_q,
+                                const at::Tensor& cu_k, const at::Tensor& block_table,
+                                const MaybeTensor& workspace, int64_t rel_extent,
+                                int64_t window_left, int64_t max_seqlen_k, double softmax_scale,
+                                int64_t num_splits, int64_t chunk_len, int64_t shared_prefix_len,
+                                int64_t prefix_splits) {
+  auto outer_ok = [](const at::Tensor& t) {
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+      if (t.stride(i) <= 0 || t.stride(i) % 8 != 0) return false;
+    return t.stride(t.dim() - 1) == 1 && aligned16(t);
+  };
+  if (!plain_rows(q, q) || !outer_ok(q) || k.dim() != 4 || v.sizes() != k.sizes() ||
+      k.size(3) != 128 || k.scalar_type() != at::kBFloat16 || v.scalar_type() != at::kBFloat16 ||
+      k.device() != q.device() || v.device() != q.device() || !outer_ok(k) || !outer_ok(v) ||
+      !plain_cu(cu_q, q) || !plain_cu(cu_k, q) || cu_k.numel() != cu_q.numel() ||
+      q.size(0) != cu_q.numel() - 1 || rel.dim() != 3 || rel.scalar_type() != at::kBFloat16 ||
+      rel.device() != q.device() || rel.size(0) != q.size(0) || rel.size(1) != q.size(1) ||
+      rel.stride(2) != 1 || rel_extent < 1 || rel_extent > rel.size(2) || k.size(2) < 1 ||
+      q.size(1) % k.size(2) != 0)
+    return {};
+  const int64_t page_size = k.size(1);
+  if (page_size < 16 || (page_size & (page_size - 1)) != 0 || block_table.dim() != 2 ||
+      block_table.scalar_type() != at::kInt || block_table.device() != q.device() ||
+      block_table.size(0) != q.size(0) || block_table.numel() == 0 || block_table.stride(1) != 1 ||
+      shared_prefix_len < 0 || shared_prefix_len > block_table.size(1) * page_size ||
+      shared_prefix_len > 0x7fffffff || !(softmax_scale > 0))
+    return {};
+  for (int64_t x : {window_left, max_seqlen_k, num_splits, chunk_len, prefix_splits})
+    if (x < -1 || x > 0x7fffffff) return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor out = rows_like(q);
+  IFA4SharedPrefixParams p{};
+  p.decode = decode_params(q, k, v, rel, out, cu_q, cu_k, c10::nullopt, block_table, rel_extent,
+                           true, window_left, IFA4_ALIGN_BOTTOM_RIGHT, max_seqlen_k, softmax_scale,
+                           num_splits, chunk_len);
+  p.shared_prefix_len = static_cast<int32_t>(shared_prefix_len);
+  p.prefix_splits = static_cast<int32_t>(prefix_splits);
+  size_t need = 0;
+  if (ifa4_decode_shared_prefix_workspace_size(&p, &need)) return {};
+  at::Tensor ws;
+  if (need > 0) {
+    if (workspace.has_value() && workspace->device() == q.device() && workspace->is_contiguous() &&
+        aligned16(*workspace) && static_cast<size_t>(workspace->nbytes()) >= need)
+      ws = *workspace;
+    else
+      ws = bytes_like(q, need);
+  }
+  if (ifa4_decode_shared_prefix_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(q)))
+    return {};
+  return {out};
 }
 
 int32_t weight_dtype(const at::Tensor& t) {
   return t.scalar_type() == at::kFloat ? IFA4_WEIGHT_F32 : IFA4_WEIGHT_BF16;
 }
+bool plain_starts(const at::Tensor& starts, const at::Tensor& like) {
+  return starts.dim() == 1 && starts.scalar_type() == at::kInt && starts.numel() >= 1 &&
+         starts.numel() <= IFA4_MAX_BUCKETS && starts.device() == like.device() &&
+         starts.stride(0) == 1;
+}
 
-int64_t bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, const at::Tensor& rel) {
+Tensors bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, int64_t total_q,
+                       int64_t rel_extent) {
+  if (table.dim() != 2 || (table.scalar_type() != at::kFloat && table.scalar_type() != at::kBFloat16) ||
+      !plain_starts(starts, table) || table.size(0) != starts.numel() || table.size(1) < 1 ||
+      total_q < 0 || rel_extent < 1 || rel_extent > (1 << 24))
+    return {};
   const c10::cuda::CUDAGuard guard(table.device());
+  const int64_t heads = table.size(1);
+  const at::Tensor rel = at::empty({heads, rel_extent}, table.options().dtype(at::kBFloat16));
   IFA4BucketBiasParams p{};
   p.table = table.data_ptr();
   p.starts = static_cast<const int32_t*>(starts.data_ptr());
@@ -371,18 +488,26 @@ int64_t bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, const 
   p.table_stride_b = table.stride(0);
   p.table_stride_h = table.stride(1);
   p.rel_stride_h = rel.stride(0);
-  p.n_heads = static_cast<int32_t>(table.size(1));
-  p.rel_extent = static_cast<int32_t>(rel.size(1));
+  p.n_heads = static_cast<int32_t>(heads);
+  p.rel_extent = static_cast<int32_t>(rel_extent);
   p.buckets = static_cast<int32_t>(starts.numel());
   p.weight_dtype = weight_dtype(table);
-  return ifa4_bucket_bias_launch(
-      &p, c10::cuda::getCurrentCUDAStream(table.device().index()).stream());
+  if (ifa4_bucket_bias_launch(&p, stream_of(table))) return {};
+  return {rel.unsqueeze(0).expand({total_q, heads, rel_extent})};
 }
 
-int64_t bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts,
-                                const at::Tensor& dtable,
-                                const c10::optional<at::Tensor>& cu_q) {
+Tensors bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts, bool f32,
+                                const MaybeTensor& cu_q) {
+  if (drel.dim() != 3 || drel.scalar_type() != at::kBFloat16 || drel.size(1) < 1 ||
+      drel.size(2) < 1 || drel.size(2) > (1 << 24) || (drel.size(2) > 1 && drel.stride(2) != 1) ||
+      !plain_starts(starts, drel))
+    return {};
+  if (cu_q.has_value() && (cu_q->dim() != 1 || cu_q->numel() < 1 || cu_q->scalar_type() != at::kInt ||
+                           cu_q->device() != drel.device() || cu_q->stride(0) != 1))
+    return {};
   const c10::cuda::CUDAGuard guard(drel.device());
+  const at::Tensor dtable = at::empty({starts.numel(), drel.size(1)},
+                                      drel.options().dtype(f32 ? at::kFloat : at::kBFloat16));
   IFA4BucketBiasBackwardParams p{};
   p.drel = drel.data_ptr();
   p.starts = static_cast<const int32_t*>(starts.data_ptr());
@@ -397,15 +522,15 @@ int64_t bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts
   p.n_heads = static_cast<int32_t>(drel.size(1));
   p.rel_extent = static_cast<int32_t>(drel.size(2));
   p.buckets = static_cast<int32_t>(starts.numel());
-  p.weight_dtype = weight_dtype(dtable);
+  p.weight_dtype = f32 ? IFA4_WEIGHT_F32 : IFA4_WEIGHT_BF16;
   size_t need = 0;
-  const int rc = ifa4_bucket_bias_backward_workspace_size(&p, &need);
-  if (rc) return rc;
+  if (ifa4_bucket_bias_backward_workspace_size(&p, &need)) return {};
   at::Tensor ws;
-  if (need > 0) ws = at::empty({static_cast<int64_t>(need)}, drel.options().dtype(at::kByte));
-  return ifa4_bucket_bias_backward_launch(
-      &p, need > 0 ? ws.data_ptr() : nullptr, need,
-      c10::cuda::getCurrentCUDAStream(drel.device().index()).stream());
+  if (need > 0) ws = bytes_like(drel, need);
+  if (ifa4_bucket_bias_backward_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need,
+                                       stream_of(drel)))
+    return {};
+  return {dtable};
 }
 
 }  // namespace
@@ -419,32 +544,29 @@ TORCH_LIBRARY(inkling_fa4, m) {
         "Tensor cu_k, Tensor(b!)? lse, Tensor? block_table, Tensor? workspace, int rel_extent, "
         "bool causal, int window_left, int causal_align, int max_seqlen_k, float softmax_scale, "
         "int num_splits, int chunk_len) -> int");
-  m.def("decode_shared_prefix_(Tensor q, Tensor k, Tensor v, Tensor rel, Tensor(a!) out, "
-        "Tensor cu_q, Tensor cu_k, Tensor(b!)? lse, Tensor block_table, Tensor? workspace, "
-        "int rel_extent, int window_left, int max_seqlen_k, float softmax_scale, int num_splits, "
-        "int chunk_len, int shared_prefix_len, int prefix_splits) -> int");
-  m.def("qk_norm_rope_(Tensor q, Tensor k, Tensor(a!) q_out, Tensor(b!) k_out, Tensor? q_weight, "
+  m.def("decode_shared_prefix(Tensor q, Tensor k, Tensor v, Tensor rel, Tensor cu_q, Tensor cu_k, "
+        "Tensor block_table, Tensor(a!)? workspace, int rel_extent, int window_left, "
+        "int max_seqlen_k, float softmax_scale, int num_splits, int chunk_len, "
+        "int shared_prefix_len, int prefix_splits) -> Tensor[]");
+  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, "
+        "Tensor? cu_q, Tensor? cu_k, bool interleaved, float eps) -> Tensor[]");
+  m.def("qk_norm_rope_backward(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor? q_weight, "
         "Tensor? k_weight, Tensor? inv_freq, Tensor? cu_q, Tensor? cu_k, bool interleaved, "
-        "float eps) -> int");
-  m.def("qk_norm_rope_backward_(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor(a!) dq, "
-        "Tensor(b!) dk, Tensor? q_weight, Tensor? k_weight, Tensor(c!)? dq_weight, "
-        "Tensor(d!)? dk_weight, Tensor? inv_freq, Tensor? cu_q, Tensor? cu_k, bool interleaved, "
-        "float eps) -> int");
-  m.def("kv_append_(Tensor? q, Tensor k, Tensor v, Tensor(a!)? q_out, Tensor(b!) k_cache, "
-        "Tensor(c!) v_cache, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor cu_q, "
-        "Tensor cu_k, Tensor block_table, bool interleaved, float eps, bool zero_padding) -> int");
-  m.def("bucket_bias_(Tensor table, Tensor starts, Tensor(a!) rel) -> int");
-  m.def("bucket_bias_backward_(Tensor drel, Tensor starts, Tensor(a!) dtable, Tensor? cu_q) "
-        "-> int");
+        "float eps, bool want_q_weight, bool want_k_weight) -> Tensor[]");
+  m.def("kv_append_(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+        "Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor cu_q, Tensor cu_k, "
+        "Tensor block_table, bool interleaved, float eps) -> Tensor[]");
+  m.def("bucket_bias(Tensor table, Tensor starts, int total_q, int rel_extent) -> Tensor[]");
+  m.def("bucket_bias_backward(Tensor drel, Tensor starts, bool f32, Tensor? cu_q) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("prefill_", &prefill_op);
   m.impl("decode_", &decode_op);
-  m.impl("decode_shared_prefix_", &decode_shared_prefix_op);
-  m.impl("qk_norm_rope_", &qk_norm_rope_op);
-  m.impl("qk_norm_rope_backward_", &qk_norm_rope_backward_op);
+  m.impl("decode_shared_prefix", &decode_shared_prefix_op);
+  m.impl("qk_norm_rope", &qk_norm_rope_op);
+  m.impl("qk_norm_rope_backward", &qk_norm_rope_backward_op);
   m.impl("kv_append_", &kv_append_op);
-  m.impl("bucket_bias_", &bucket_bias_op);
-  m.impl("bucket_bias_backward_", &bucket_bias_backward_op);
+  m.impl("bucket_bias", &bucket_bias_op);
+  m.impl("bucket_bias_backward", &bucket_bias_backward_op);
 }

@@ -232,6 +232,19 @@ def torch_op(name: str):
     return op
 
 
+def try_op(name: str, *args):
+    """The outputs of the operator ``inkling_fa4::name`` for a plain call, or None: the arguments
+    are not its plain case (or not tensors at all, or on the CPU), its launch failed, or there is no
+    operator library; the caller then goes through its own checks and the C ABI."""
+    op = _overloads.get(name) or torch_op(name)
+    if op is None:
+        return None
+    try:
+        return op(*args) or None
+    except (RuntimeError, TypeError):
+        return None
+
+
 def lib() -> ctypes.CDLL:
     """Load the CUDA library (once).  Raises if it is absent: no CPU fallback exists."""
     global _lib

@@ -62,6 +62,10 @@ def _weight_dtype(name, dtype):
 
 def _forward(table, starts, total_q, rel_extent):
     name = "bucket_bias"
+    if _ops.USE_TORCH_OPS:
+        outs = _lib.try_op("bucket_bias", table, starts, total_q, rel_extent)
+        if outs is not None:
+            return outs[0]
     if not isinstance(table, torch.Tensor):
         raise TypeError(f"{name}: table must be a torch.Tensor")
     if not table.is_cuda:
@@ -76,25 +80,24 @@ def _forward(table, starts, total_q, rel_extent):
         raise ValueError(f"{name}: total_q must be >= 0, rel_extent in [1, 2^24]")
     heads = table.shape[1]
     rel = torch.empty((heads, rel_extent), dtype=torch.bfloat16, device=table.device)
-    op = _lib.torch_op("bucket_bias_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(table, starts, rel)
-        if rc:
-            _lib.check(rc)
-    else:
-        p = _lib.BucketBiasParams()
-        p.table, p.starts, p.rel = table.data_ptr(), starts.data_ptr(), rel.data_ptr()
-        p.table_stride_b, p.table_stride_h = table.stride()
-        p.rel_stride_h = rel_extent
-        p.n_heads, p.rel_extent, p.buckets, p.weight_dtype = heads, rel_extent, starts.numel(), wt
-        with torch.cuda.device(table.device):
-            stream = torch.cuda.current_stream(table.device).cuda_stream
-            _lib.check(_lib.lib().ifa4_bucket_bias_launch(ctypes.byref(p), ctypes.c_void_p(stream)))
+    p = _lib.BucketBiasParams()
+    p.table, p.starts, p.rel = table.data_ptr(), starts.data_ptr(), rel.data_ptr()
+    p.table_stride_b, p.table_stride_h = table.stride()
+    p.rel_stride_h = rel_extent
+    p.n_heads, p.rel_extent, p.buckets, p.weight_dtype = heads, rel_extent, starts.numel(), wt
+    with torch.cuda.device(table.device):
+        stream = torch.cuda.current_stream(table.device).cuda_stream
+        _lib.check(_lib.lib().ifa4_bucket_bias_launch(ctypes.byref(p), ctypes.c_void_p(stream)))
     return rel.unsqueeze(0).expand(total_q, heads, rel_extent)
 
 
 def _backward(drel, starts, dtype, cu_seqlens_q):
     name = "bucket_bias_backward"
+    if _ops.USE_TORCH_OPS and (dtype is torch.float32 or dtype is torch.bfloat16):
+        outs = _lib.try_op("bucket_bias_backward", drel, starts, dtype is torch.float32,
+                           cu_seqlens_q)
+        if outs is not None:
+            return outs[0]
     if not isinstance(drel, torch.Tensor):
         raise TypeError(f"{name}: drel must be a torch.Tensor")
     if not drel.is_cuda:
@@ -117,12 +120,6 @@ def _backward(drel, starts, dtype, cu_seqlens_q):
         drel = drel.contiguous()
     heads, buckets = drel.shape[1], starts.numel()
     dtable = torch.empty((buckets, heads), dtype=dtype, device=drel.device)
-    op = _lib.torch_op("bucket_bias_backward_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(drel, starts, dtable, cu_seqlens_q)
-        if rc:
-            _lib.check(rc)
-        return dtable
     p = _lib.BucketBiasBackwardParams()
     p.drel, p.starts, p.dtable = drel.data_ptr(), starts.data_ptr(), dtable.data_ptr()
     p.cu_seqlens_q = None if cu_seqlens_q is None else cu_seqlens_q.data_ptr()

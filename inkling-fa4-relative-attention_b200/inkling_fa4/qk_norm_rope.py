@@ -34,6 +34,14 @@ def _rows_ready(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _eps(eps):
+    """eps as the operators take it: negative for no norm, NaN (never the plain case) for a value
+    that the checks will refuse."""
+    if eps is None:
+        return _NO_NORM
+    return eps if isinstance(eps, float) and 0 <= eps < math.inf else math.nan
+
+
 def _empty_like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
@@ -144,6 +152,11 @@ def _stream(device):
 
 def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
     name = "qk_norm_rope"
+    if _ops.USE_TORCH_OPS:
+        outs = _lib.try_op("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, cu_q, cu_k,
+                           interleaved, _eps(eps))
+        if outs is not None:
+            return outs[0], outs[1]
     _check_rows(name, "q", q, None)
     _check_rows(name, "k", k, q)
     cu_q, cu_k = _check_cu(name, q.device, cu_q, cu_k)
@@ -153,13 +166,6 @@ def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
         raise ValueError(f"{name}: neither a norm (eps) nor a rotation (inv_freq)")
     q, k = _rows_ready(q), _rows_ready(k)
     q_out, k_out = _empty_like(q), _empty_like(k)
-    op = _lib.torch_op("qk_norm_rope_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(q, k, q_out, k_out, q_weight, k_weight, inv_freq, cu_q, cu_k, bool(interleaved),
-                eps)
-        if rc:
-            _lib.check(rc)
-        return q_out, k_out
     p = _lib.QkNormRopeParams()
     _fill_rows(p, q=q, k=k, q_out=q_out, k_out=k_out)
     _fill_step(p, q.shape[1], k.shape[1], q_weight, k_weight, cu_q, cu_k, eps, inv_freq,
@@ -173,6 +179,13 @@ def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
 def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved,
               weight_grads):
     name = "qk_norm_rope_backward"
+    if _ops.USE_TORCH_OPS:
+        outs = _lib.try_op("qk_norm_rope_backward", dq_out, dk_out, q, k, q_weight, k_weight,
+                           inv_freq, cu_q, cu_k, interleaved, _eps(eps), *weight_grads)
+        if outs is not None:
+            dq, dk, *dw = outs
+            dqw = dw.pop(0) if q_weight is not None and weight_grads[0] else None
+            return dq, dk, dqw, dw.pop(0) if dw else None
     _check_rows(name, "q", q, None)
     _check_rows(name, "k", k, q)
     _check_rows(name, "dq_out", dq_out, q, q.shape[1])
@@ -184,13 +197,6 @@ def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_fre
     dq, dk = _empty_like(q), _empty_like(k)
     dqw = torch.empty_like(q_weight) if q_weight is not None and weight_grads[0] else None
     dkw = torch.empty_like(k_weight) if k_weight is not None and weight_grads[1] else None
-    op = _lib.torch_op("qk_norm_rope_backward_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(dq_out, dk_out, q, k, dq, dk, q_weight, k_weight, dqw, dkw, inv_freq, cu_q, cu_k,
-                bool(interleaved), eps)
-        if rc:
-            _lib.check(rc)
-        return dq, dk, dqw, dkw
     p = _lib.QkNormRopeBackwardParams()
     _fill_rows(p, dq_out=dq_out, dk_out=dk_out, q=q, k=k, dq=dq, dk=dk)
     _fill_step(p, q.shape[1], k.shape[1], q_weight, k_weight, cu_q, cu_k, eps, inv_freq,
@@ -206,6 +212,10 @@ def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_fre
             ctypes.byref(p), ctypes.c_void_p(0 if ws is None else ws.data_ptr()), need,
             _stream(q.device)))
     return dq, dk, dqw, dkw
+
+
+def _wants_grad(t):
+    return t is not None and getattr(t, "requires_grad", False)
 
 
 class QkNormRopeFunction(torch.autograd.Function):
@@ -239,8 +249,8 @@ def inkling_qk_norm_rope(q, k, q_weight=None, k_weight=None, cu_seqlens_q=None, 
     neighbouring dims instead of the two halves.  Rows behind the last sequence
     (``cu_seqlens_q[batch]``) come out as zeros, and so do their gradients, which count in no
     weight gradient."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (_wants_grad(q) or _wants_grad(k) or _wants_grad(q_weight)
+                                    or _wants_grad(k_weight)):
         return QkNormRopeFunction.apply(q, k, q_weight, k_weight, cu_seqlens_q, cu_seqlens_k, eps,
                                         inv_freq, interleaved)
     return _forward(q, k, q_weight, k_weight, cu_seqlens_q, cu_seqlens_k, eps, inv_freq,
@@ -279,6 +289,11 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
     Returns the queries (``q_out`` if given, which may be ``q`` itself: rows behind the last
     sequence are then left as they were; a new tensor has zeros there), or None without ``q``."""
     name = "kv_append"
+    if q is not None and q_out is None and _ops.USE_TORCH_OPS:
+        outs = _lib.try_op("kv_append_", q, k, v, k_cache, v_cache, q_weight, k_weight, inv_freq,
+                           cu_seqlens_q, cu_seqlens_k, block_table, interleaved, _eps(eps))
+        if outs is not None:
+            return outs[0]
     _check_rows(name, "k", k, None)
     _check_rows(name, "v", v, k, k.shape[1])
     device = k.device
@@ -328,13 +343,6 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
             if not same and any(t.untyped_storage().data_ptr() == store for t in (q, k, v)):
                 raise ValueError(f"{name}: q_out must be q itself or share no storage with q, k, v")
             q = _rows_ready(q)
-    op = _lib.torch_op("kv_append_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(q, k, v, q_out, k_cache, v_cache, q_weight, k_weight, inv_freq, cu_seqlens_q,
-                cu_seqlens_k, block_table, bool(interleaved), eps, zero_padding)
-        if rc:
-            _lib.check(rc)
-        return q_out
     p = _lib.KvAppendParams()
     _fill_rows(p, k=k, v=v)
     if q is not None:

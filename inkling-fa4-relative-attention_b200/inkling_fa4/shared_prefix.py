@@ -36,6 +36,15 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
     CUDA tensor (allocated per call when absent or too small); calls that may run at the same
     time need one each."""
     name = "decode_shared_prefix"
+    if (out is None and lse is None and not return_lse and n_heads is None and kv_heads is None
+            and head_dim == _ops.HEAD_DIM and _ops.USE_TORCH_OPS):
+        outs = _lib.try_op("decode_shared_prefix", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k,
+                           block_table, workspace, rel_extent,
+                           -1 if window_size is None else window_size[0], max_seqlen_k or 0,
+                           1.0 / _ops.HEAD_DIM if softmax_scale is None else softmax_scale,
+                           num_splits, chunk_len, shared_prefix_len, prefix_splits)
+        if outs is not None:
+            return outs[0]
     if block_table is None:
         raise ValueError(f"{name}: needs a paged cache (block_table)")
     block_table = _ops._table(block_table)
@@ -52,14 +61,6 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
         raise ValueError(f"{name}: shared_prefix_len {shared_prefix_len} is beyond the table's "
                          f"{block_table.shape[1]} pages of {k.shape[1]}")
     max_seqlen_k = int(max_seqlen_k) if max_seqlen_k else 0
-    op = _lib.torch_op("decode_shared_prefix_") if _ops.USE_TORCH_OPS else None
-    if op is not None:
-        rc = op(q, k, v, rel, out, cu_seqlens_q, cu_seqlens_k, lse, block_table, workspace,
-                rel_extent, window_left, max_seqlen_k, scale, int(num_splits), int(chunk_len),
-                shared_prefix_len, int(prefix_splits))
-        if rc:
-            _lib.check(rc)
-        return (out, lse) if lse is not None else out
     p = _lib.SharedPrefixParams()
     p.decode = _ops._decode_params(q, k, v, rel, out, cu_seqlens_q, cu_seqlens_k, n_heads,
                                    kv_heads, rel_extent, True, window_left, "bottom_right",

@@ -285,6 +285,6 @@ def test_oracle_gradient_against_differences(rot, interleaved, eps):
 def test_operator_schemas():
     ops = _lib.torch_ops()
     assert ops is not None, "libifa4_torch_ops.so not built"
-    for name in ("decode_shared_prefix_", "qk_norm_rope_", "qk_norm_rope_backward_", "kv_append_",
-                 "bucket_bias_", "bucket_bias_backward_"):
+    for name in ("decode_shared_prefix", "qk_norm_rope", "qk_norm_rope_backward", "kv_append_",
+                 "bucket_bias", "bucket_bias_backward"):
         assert str(getattr(ops, name).default._schema).startswith(f"inkling_fa4::{name}(")
