@@ -613,10 +613,11 @@ __global__ void __launch_bounds__(kCombineThreads)
   auto lse_of = [&](int i) {
     return i < a.parts ? a.ws_lse[i * rows + row] : a.own_lse[row * a.own_parts + (i - a.parts)];
   };
+  auto larger = [](float x, float y) { return y > x || y != y ? y : x; };  // a NaN wins
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) m = fmaxf(m, lse_of(i));
+  for (int i = lane; i < n; i += 32) m = larger(m, lse_of(i));
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  for (int k = 16; k > 0; k >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, k));
   float wsum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (m != -INFINITY) {
