@@ -13,7 +13,8 @@
 // The four warps' (max, sum, O) states are merged in shared memory; with one split the CTA
 // writes the bf16 output, otherwise a normalised fp32 partial and its log2-sum-exp, which
 // rel_attn_decode_combine_kernel merges (or, with prefix_len > 0, when only the keys behind the
-// batch's shared prefix are read here, shared_prefix_combine_kernel).
+// batch's shared prefix are read here, merges the prefix's partials in or leaves both to
+// shared_prefix_combine_kernel).
 //
 // Paged KV cache (kPaged): the whole producer warp runs, fetching the next tile's page numbers
 // from the block table while the current tile is issued; a 64-key tile is loaded as 64 / box
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const SeqInfo si = seq_info<kPaged>(a, b);
   const int bs = a.align_bottom_right ? si.sk - 1 : 1 - si.sk;  // bias distance at key 0
 
-  if (a.prefix_len > 0) launch_dependents();
+  if (a.prefix_len > 0 && a.px_parts == 0) launch_dependents();  // the merge
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -405,6 +406,77 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   __syncthreads();
+  if (a.px_parts > 0) {
+    // One warp per row, lanes own 4 of the 128 dims: the four warps' states, then the prefix's
+    // partials (weights 2^(lse_i - max)), then the output.
+    wait_previous_kernel();  // the prefix kernel
+    const long long rows = static_cast<long long>(a.batch) * a.n_heads;
+    for (int row = warp; row < nh; row += kConsumerWarps + 1) {
+      const long long at = static_cast<long long>(b) * a.n_heads + h0 + row;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kConsumerWarps; ++w) M = fmaxf(M, mm[w * 16 + row]);
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (M != -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < kConsumerWarps; ++w) {
+          const float f = fast_exp2(mm[w * 16 + row] - M);
+          const float4 o4 = reinterpret_cast<const float4*>(mo + (w * 16 + row) * 128)[lane];
+          L += ml[w * 16 + row] * f;
+          acc.x += o4.x * f;
+          acc.y += o4.y * f;
+          acc.z += o4.z * f;
+          acc.w += o4.w * f;
+        }
+      }
+      auto larger = [](float x, float y) { return y > x || y != y ? y : x; };  // a NaN wins
+      float m = M;
+      for (int i = lane; i < a.px_parts; i += 32) m = larger(m, a.px_lse[i * rows + at]);
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, k));
+      if (m != -INFINITY) {
+        const float own = M == -INFINITY ? 0.f : fast_exp2(M - m);
+        L *= own;
+        acc.x *= own;
+        acc.y *= own;
+        acc.z *= own;
+        acc.w *= own;
+        for (int i0 = 0; i0 < a.px_parts; i0 += 8) {
+          float wt[8];
+          float4 o4[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            wt[k] = i0 + k < a.px_parts ? fast_exp2(a.px_lse[(i0 + k) * rows + at] - m) : 0.f;
+            o4[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (wt[k] != 0.f)  // no weight: its output may never have been written
+              o4[k] = reinterpret_cast<const float4*>(a.px_o + ((i0 + k) * rows + at) * 128)[lane];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            L += wt[k];
+            acc.x += wt[k] * o4[k].x;
+            acc.y += wt[k] * o4[k].y;
+            acc.z += wt[k] * o4[k].z;
+            acc.w += wt[k] * o4[k].w;
+          }
+        }
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;  // NaN stays
+      if (IFA4_DBG_CHECK(a.status, si.q_row >= 0 && si.q_row < a.batch && h0 + row < a.n_heads)) {
+        uint2 packed;
+        packed.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+        packed.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(a.out + static_cast<long long>(si.q_row) * a.out_st +
+                                  static_cast<long long>(h0 + row) * a.out_sh + lane * 4) = packed;
+        if (lane == 0 && a.lse != nullptr)
+          a.lse[static_cast<long long>(h0 + row) * a.lse_sh +
+                static_cast<long long>(si.q_row) * a.lse_st] =
+              L == 0.f ? -INFINITY : (m + __log2f(L)) * 0.6931471805599453f;
+      }
+    }
+    return;
+  }
   if (threadIdx.x < 128) {
     const int d = threadIdx.x;
     for (int row = 0; row < nh; ++row) {

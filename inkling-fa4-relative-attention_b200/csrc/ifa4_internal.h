@@ -156,9 +156,13 @@ struct DecodeKernelArgs {
   const int32_t* block_table;  // paged KV cache, as in PrefillKernelArgs
   long long bt_stride;
   int page_shift, box_shift, num_pages;
-  // shared prefix (0: none): sequences of at least this many keys start at key prefix_len, and the
-  // partials (always written then, whatever num_splits) go to shared_prefix_combine_kernel
+  // shared prefix (0: none): sequences of at least this many keys start at key prefix_len.  With one
+  // split the CTA merges the prefix's partials itself (px_*, as SharedPrefixKernelArgs has them);
+  // otherwise its own go to shared_prefix_combine_kernel
   int prefix_len;
+  const float* px_o;
+  const float* px_lse;
+  int px_parts;
   int* status;
 };
 

@@ -14,13 +14,13 @@
 // Sequences with fewer keys than the prefix take no part (their rows have weight 0 here; the
 // decode kernel then covers all of their keys).
 //
-// The three kernels (prefix, own keys, merge) are launched to overlap: the own keys' kernel starts
-// as soon as the prefix kernel's CTAs have and fills the SMs they leave, and ends after it; the
-// merge's blocks wait for that.
+// The kernels are launched to overlap: the own keys' kernel starts as soon as the prefix kernel's
+// CTAs have, fills the SMs they leave, and merges the prefix's partials into its rows once that
+// kernel has completed.  Only when the own keys themselves are split does a third kernel merge all
+// partials (its blocks wait for both).
 //
 // The grid is (row tiles, KV heads, key splits); every CTA writes its rows' normalised fp32
-// partial outputs and log2-sum-exps, and shared_prefix_combine_kernel merges all partials of a
-// row.  The CTA's two softmax groups (and TMEM halves) work on
+// partial outputs and log2-sum-exps.  The CTA's two softmax groups (and TMEM halves) work on
 //   kKeyPair = false: two row tiles at the same keys (batches of more than one tile per KV head:
 //                     K and V are shared by 256 rows);
 //   kKeyPair = true:  one row tile at alternating key tiles (small batches: one group's softmax
