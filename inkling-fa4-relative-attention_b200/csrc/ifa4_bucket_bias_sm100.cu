@@ -5,7 +5,9 @@
 // lies before its start).
 //
 // The forward writes one [n_heads, rel_extent] table, which the attention reads with token
-// stride 0.  The gradient is one read of drel (HBM bound): a thread owns V neighbouring columns
+// stride 0 (2 us, its launch).  The gradient is one read of drel, HBM bound: 268 MB (32k tokens x 32
+// heads x 128) in 43 us, 6.2 TB/s, and 2.15 GB (x 1024) in 297 us, 7.2 TB/s, what a read-only stream
+// reaches; the shorter one pays its start and its bucket sums.  A thread owns V neighbouring columns
 // of one head and adds its tokens in registers (fp32, eight loads in flight), a block adds its
 // token lanes and then its columns by bucket in a fixed order and writes one partial per head and
 // bucket; a second kernel adds the blocks' partials in a fixed order (no atomics).  With a single
@@ -148,21 +150,25 @@ __global__ void __launch_bounds__(kThreads) bucket_grad_kernel(const __grid_cons
     }
     __syncthreads();
   }
-  // buckets: eight lanes per head and bucket
-  const int sub = threadIdx.x & 7;
+  launch_dependents();  // the sum over slots
+  // buckets: a thread per head and bucket, eight where buckets hold 16 columns and more on average
+  const int per = a.rel_extent >= 16 * a.buckets ? 8 : 1;
+  const int sub = threadIdx.x & (per - 1);
   const int tasks = a.heads * a.buckets;
-  for (int task0 = 0; task0 < tasks; task0 += kThreads / 8) {
-    const int task = task0 + (threadIdx.x >> 3);
+  for (int task0 = 0; task0 < tasks; task0 += kThreads / per) {
+    const int task = task0 + threadIdx.x / per;
     const int th = task < tasks ? task / a.buckets : 0;
     const int b = task - th * a.buckets;
     float v = 0.f;
     if (task < tasks) {
       const int lo = max(starts[b] - e0, 0), hi = min(starts[b + 1] - e0, n_cols);
-      for (int i = lo + sub; i < hi; i += 8) v += sums[th * a.cols + i];
+      for (int i = lo + sub; i < hi; i += per) v += sums[th * a.cols + i];
     }
-    v += __shfl_xor_sync(0xffffffffu, v, 4);
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    if (per == 8) {
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+    }
     if (sub == 0 && task < tasks && h0 + th < a.n_heads) {
       if (a.slots == 1)
         store_as(a.grad, b * a.grad_sb + (h0 + th) * a.grad_sh, v, a.grad_f32);
@@ -179,6 +185,7 @@ __global__ void __launch_bounds__(1024) bucket_grad_sum_kernel(const __grid_cons
   __shared__ float s[32][33];
   const int n = a.n_heads * a.buckets;
   const int i = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  wait_previous_kernel();
   float acc = 0.f;
   if (i < n)
     for (int k = row; k < a.slots; k += 32) acc += a.partial[static_cast<long long>(k) * n + i];
@@ -213,8 +220,9 @@ void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms) {
   a->lanes = bucket::kThreads / (heads * head_vecs);
   const long long col_blocks =
       static_cast<long long>((a->n_heads + heads - 1) / heads) * a->col_parts;
-  // one resident wave of blocks (four per SM; 32k tokens x 32 heads x 128: 52 us, 62 us with two
-  // waves of half the tokens), at least 32 tokens per lane (one chunk needs no second kernel)
+  // one resident wave of blocks (four per SM; 32k tokens x 32 heads x 128: 43 us, 46 us with two
+  // waves of half the tokens, 44 us with three blocks), at least 32 tokens per lane (one chunk needs
+  // no second kernel)
   long long chunks = 4ll * sms / col_blocks;
   const long long most = (a->total_q + 32ll * a->lanes - 1) / (32ll * a->lanes);
   if (chunks > most) chunks = most;
@@ -239,8 +247,7 @@ cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || args.slots == 1) return e;
   const int n = args.n_heads * args.buckets;
-  bucket::bucket_grad_sum_kernel<<<(n + 31) / 32, 1024, 0, stream>>>(args);
-  return cudaGetLastError();
+  return launch_early(bucket::bucket_grad_sum_kernel, dim3((n + 31) / 32), 1024, 0, stream, args);
 }
 
 }  // namespace ifa4

@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, kQkvBackwardBlocksPerSm)
     }
   }
   if (a.partial == nullptr) return;
+  launch_dependents();  // the sum over blocks
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     part[4 * warp + oct][i < 8 ? rot.a_off + i : rot.b_off + i - 8] = acc[i];
@@ -449,6 +450,7 @@ __global__ void __launch_bounds__(1024) qkv_weight_grad_kernel(const float* part
   const bool is_q = blockIdx.x < 4;
   const int col = (blockIdx.x & 3) * 32 + (threadIdx.x & 31), lane_row = threadIdx.x >> 5;
   const int first = is_q ? 0 : q_blocks, last = is_q ? q_blocks : blocks;
+  wait_previous_kernel();
   float acc = 0.f;
   for (int i = first + lane_row; i < last; i += 32)
     acc += partial[static_cast<long long>(i) * 128 + col];
@@ -525,9 +527,9 @@ cudaError_t launch_qkv_backward_sm100(const QkvBackwardKernelArgs& args, int blo
     qkv::qkv_backward_kernel<qkv::kRotPairs><<<blocks, qkv::kThreads, 0, stream>>>(args);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || args.partial == nullptr) return e;
-  qkv::qkv_weight_grad_kernel<<<8, 1024, 0, stream>>>(
-      args.partial, args.q_blocks, blocks, args.dq_weight, args.dk_weight, args.weight_f32);
-  return cudaGetLastError();
+  return launch_early(qkv::qkv_weight_grad_kernel, dim3(8), 1024, 0, stream,
+                      const_cast<const float*>(args.partial), args.q_blocks, blocks, args.dq_weight,
+                      args.dk_weight, args.weight_f32);
 }
 
 }  // namespace ifa4
