@@ -17,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "ifa4_internal.h"
 #include "ifa4_ptx.cuh"
 
@@ -70,6 +72,19 @@ struct Vec<8> {
   }
 };
 template <>
+struct Vec<4> {
+  uint2 v;
+  __device__ __forceinline__ void load(const uint16_t* p) {
+    v = __ldg(reinterpret_cast<const uint2*>(p));
+  }
+  __device__ __forceinline__ void add(float (&s)[4]) const {
+    s[0] += __uint_as_float(v.x << 16);
+    s[1] += __uint_as_float(v.x & 0xffff0000u);
+    s[2] += __uint_as_float(v.y << 16);
+    s[3] += __uint_as_float(v.y & 0xffff0000u);
+  }
+};
+template <>
 struct Vec<2> {
   uint32_t v;
   __device__ __forceinline__ void load(const uint16_t* p) {
@@ -89,6 +104,8 @@ struct Vec<1> {
 
 // Block (x, y): column block x = (head block, column part), token chunk y.  A block covers
 // a.heads heads x a.cols columns (columns of one head from a.cols * part on), a.lanes token lanes.
+// With a.flat the heads lie one behind the other and a thread's columns may cross from one to the
+// next (rel_extent is then not a multiple of V, the columns of a block are).
 template <int V>
 __global__ void __launch_bounds__(kThreads) bucket_grad_kernel(const __grid_constant__
                                                                    BucketGradKernelArgs a) {
@@ -101,17 +118,18 @@ __global__ void __launch_bounds__(kThreads) bucket_grad_kernel(const __grid_cons
   const int h0 = (blockIdx.x / a.col_parts) * a.heads;
   const int e0 = part * a.cols;
   const int n_cols = min(a.cols, a.rel_extent - e0);
-  const int vecs = a.cols / V;                 // threads of a head (the last part may use fewer)
-  const int per_lane = a.heads * vecs;         // threads of a token lane
+  const int vecs = a.flat ? a.heads * a.cols / V : a.cols / V;  // threads of a head, or of a lane
+  const int per_lane = a.flat ? vecs : a.heads * vecs;          // threads of a token lane
   const int lane = threadIdx.x / per_lane;
   const int in_lane = threadIdx.x - lane * per_lane;
-  const int hl = in_lane / vecs;
+  const int hl = a.flat ? 0 : in_lane / vecs;
   const int c = (in_lane - hl * vecs) * V;
+  const int c_end = a.flat ? min(a.heads, a.n_heads - h0) * a.rel_extent : n_cols;
   long long tokens = a.total_q;
   if (a.cu_q != nullptr) tokens = min(tokens, static_cast<long long>(max(__ldg(a.cu_q + a.batch), 0)));
   const long long t0 = blockIdx.y * a.chunk;
   const long long t1 = min(tokens, t0 + a.chunk);
-  const bool on = lane < a.lanes && h0 + hl < a.n_heads && c < n_cols;
+  const bool on = lane < a.lanes && h0 + hl < a.n_heads && c < c_end;
   float s[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = 0.f;
@@ -207,19 +225,60 @@ cudaError_t launch_bucket_bias_sm100(const BucketBiasKernelArgs& args, cudaStrea
   return cudaGetLastError();
 }
 
-// Column blocks and token chunks of the gradient (fills heads, cols, col_parts, lanes, chunk,
-// slots of `a` from its sizes).  vec: columns a thread loads at once (8, 2 or 1).
-void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms) {
-  const int vecs = (a->rel_extent + vec - 1) / vec;  // vec divides rel_extent
-  const int head_vecs = vecs < bucket::kThreads ? vecs : bucket::kThreads;
-  a->cols = head_vecs * vec;
-  a->col_parts = (vecs + head_vecs - 1) / head_vecs;
-  int heads = bucket::kThreads / head_vecs;
-  if (heads > a->n_heads) heads = a->n_heads;
-  a->heads = heads;
-  a->lanes = bucket::kThreads / (heads * head_vecs);
+// Column blocks and token chunks of the gradient (fills flat, heads, cols, col_parts, lanes, chunk,
+// slots of `a` from its sizes).  Returns the columns a thread loads at once: the most the layout
+// allows.  Where rel_extent is not a multiple of eight but the heads lie one behind the other, a
+// block takes whole heads as one row of columns (32k x 32 x 100: 76 us in pairs of columns,
+// 39 us).
+int plan_bucket_grad(BucketGradKernelArgs* a, int sms) {
+  auto loads = [&](int v) {  // rows of columns in pieces of v
+    return reinterpret_cast<uintptr_t>(a->drel) % (2 * v) == 0 && a->drel_st % v == 0;
+  };
+  int vec = 1, together = 1;  // together: heads whose columns make whole pieces
+  a->flat = 0;
+  for (int v : {8, 4, 2})
+    if (loads(v) && a->drel_sh % v == 0 && a->rel_extent % v == 0) {
+      vec = v;
+      break;
+    }
+  if (vec < 8 && loads(8) && a->drel_sh == a->rel_extent &&
+      static_cast<long long>(a->n_heads) * a->rel_extent % 8 == 0) {
+    while (static_cast<long long>(together) * a->rel_extent % 8 != 0) together *= 2;
+    if (together * static_cast<long long>(a->rel_extent) <= bucket::kThreads * 8) {
+      a->flat = 1;
+      vec = 8;
+    }
+  }
+  if (a->flat) {
+    a->cols = a->rel_extent;
+    a->col_parts = 1;
+    int heads = bucket::kThreads * 8 / a->rel_extent / together * together;
+    const int all = (a->n_heads + together - 1) / together * together;
+    a->heads = heads < all ? heads : all;
+    a->lanes = bucket::kThreads / (a->heads * a->rel_extent / 8);
+  } else {
+    const int vecs = a->rel_extent / vec;
+    const int head_vecs = vecs < bucket::kThreads ? vecs : bucket::kThreads;
+    a->cols = head_vecs * vec;
+    a->col_parts = (vecs + head_vecs - 1) / head_vecs;
+    // heads of a block: the count that leaves the fewest threads without columns, the larger one
+    // of equals
+    int most_heads = bucket::kThreads / head_vecs;
+    if (most_heads > a->n_heads) most_heads = a->n_heads;
+    double best = 0;
+    for (int heads = most_heads; heads >= 1; --heads) {
+      const int lanes = bucket::kThreads / (heads * head_vecs);
+      const int blocks = (a->n_heads + heads - 1) / heads;
+      const double used = static_cast<double>(a->n_heads) / (blocks * heads) * heads * head_vecs * lanes;
+      if (used > best * 1.001) {
+        best = used;
+        a->heads = heads;
+        a->lanes = lanes;
+      }
+    }
+  }
   const long long col_blocks =
-      static_cast<long long>((a->n_heads + heads - 1) / heads) * a->col_parts;
+      static_cast<long long>((a->n_heads + a->heads - 1) / a->heads) * a->col_parts;
   // one resident wave of blocks (four per SM; 32k tokens x 32 heads x 128: 43 us, 46 us with two
   // waves of half the tokens, 44 us with three blocks), at least 32 tokens per lane (one chunk needs
   // no second kernel)
@@ -233,6 +292,7 @@ void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms) {
   a->chunks = static_cast<int>((a->total_q + a->chunk - 1) / a->chunk);
   if (a->chunks < 1) a->chunks = 1;
   a->slots = a->chunks * a->col_parts;
+  return vec;
 }
 
 cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
@@ -240,6 +300,8 @@ cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
   const dim3 grid((args.n_heads + args.heads - 1) / args.heads * args.col_parts, args.chunks);
   if (vec == 8)
     bucket::bucket_grad_kernel<8><<<grid, bucket::kThreads, 0, stream>>>(args);
+  else if (vec == 4)
+    bucket::bucket_grad_kernel<4><<<grid, bucket::kThreads, 0, stream>>>(args);
   else if (vec == 2)
     bucket::bucket_grad_kernel<2><<<grid, bucket::kThreads, 0, stream>>>(args);
   else

@@ -7,7 +7,6 @@
 #include <stdio.h>
 #include <string.h>
 
-#include <initializer_list>
 #include <mutex>
 
 #include "../../include/inkling_fa4.h"
@@ -1468,18 +1467,9 @@ int plan_bucket_backward(const IFA4BucketBiasBackwardParams* p, ifa4::BucketGrad
   a->rel_extent = p->rel_extent;
   a->buckets = p->buckets;
   a->grad_f32 = p->weight_dtype == IFA4_WEIGHT_F32;
-  // widest loads the layout allows
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p->drel);
-  *vec = 1;
-  for (int v : {8, 2})
-    if (at % (2 * v) == 0 && p->drel_stride_t % v == 0 && p->drel_stride_h % v == 0 &&
-        p->rel_extent % v == 0) {
-      *vec = v;
-      break;
-    }
   int sms = 148;
   if ((rc = sm_count(&sms))) return rc;
-  ifa4::plan_bucket_grad(a, *vec, sms);
+  *vec = ifa4::plan_bucket_grad(a, sms);
   *bytes = a->slots > 1 ? static_cast<size_t>(a->slots) * p->n_heads * p->buckets * sizeof(float) : 0;
   return IFA4_OK;
 }

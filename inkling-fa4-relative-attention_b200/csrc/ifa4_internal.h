@@ -282,10 +282,10 @@ struct BucketGradKernelArgs {
   long long drel_st, drel_sh, grad_sb, grad_sh;
   long long total_q, chunk;  // tokens, tokens per chunk
   int batch, n_heads, rel_extent, buckets, grad_f32;
-  int heads, cols, col_parts, lanes, chunks, slots;  // plan_bucket_grad
+  int flat, heads, cols, col_parts, lanes, chunks, slots;  // plan_bucket_grad
 };
 cudaError_t launch_bucket_bias_sm100(const BucketBiasKernelArgs& args, cudaStream_t stream);
-void plan_bucket_grad(BucketGradKernelArgs* a, int vec, int sms);
+int plan_bucket_grad(BucketGradKernelArgs* a, int sms);
 cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
                                      cudaStream_t stream);
 

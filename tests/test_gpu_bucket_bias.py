@@ -59,6 +59,10 @@ CASES = [  # tokens, heads, rel_extent, starts
     (300, 2, 64, [3, 10, 10, 500]),                 # late first start, an empty bucket, one beyond
     (64, 40, 8, [0, 4]),
     (20, 1, 9000, [0, 8999]),
+    (600, 32, 100, relative_bucket_starts(20, 100)),   # heads one behind the other, read across
+    (513, 40, 129, relative_bucket_starts(32, 128)),
+    (100, 9, 24, relative_bucket_starts(8, 24)),
+    (70, 6, 20, relative_bucket_starts(8, 24)),
 ]
 
 
