@@ -1144,10 +1144,12 @@ int validate_norm_rope(const P* p, const char* what) {
   return IFA4_OK;
 }
 
-// A token's rows are shared by several warps when there are few tokens: about 64 units per SM in
-// all (four rounds of the resident warps), four rows (what a warp does at once) at least.
+// A token's rows are shared by several warps when there are fewer tokens than resident warps (20 per
+// SM), four rows (what a warp does at once) at least.  2048 tokens x 40 heads: 10.4 us; with twice
+// to three times as many units 11.7-12.1, with eight times 15 (every unit locates its token and
+// computes its angles).
 int token_parts(int64_t tokens, int rows, int sms) {
-  const int64_t want = (64LL * sms + tokens - 1) / tokens;
+  const int64_t want = 20LL * sms / tokens;
   const int most = (rows + 3) / 4;
   return static_cast<int>(want < 1 ? 1 : (want > most ? most : want));
 }
@@ -1191,6 +1193,8 @@ int launch_qkv(const char* what, ifa4::QkvKernelArgs* a, int64_t tokens, int row
   a->rows_per_part = round4((rows + parts - 1) / parts);
   a->parts = (rows + a->rows_per_part - 1) / a->rows_per_part;
   a->units = tokens * a->parts;
+  a->v_parts = (a->kv_heads + 7) / 8;
+  a->v_units = a->k_cache != nullptr ? tokens * a->v_parts : 0;
   cudaError_t e = ifa4::launch_qkv_rows_sm100(*a, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, what);
   return IFA4_OK;
@@ -1408,7 +1412,7 @@ int ifa4_kv_append_launch(const IFA4KvAppendParams* p, void* stream) {
   a.page_shift = log2_exact(p->page_size);
   a.table_width = p->table_width;
   a.num_pages = p->num_pages;
-  return launch_qkv("kv_append launch", &a, p->total_q, p->n_heads + 2 * p->kv_heads, stream);
+  return launch_qkv("kv_append launch", &a, p->total_q, p->n_heads + p->kv_heads, stream);
 }
 
 }  // extern "C"

@@ -228,7 +228,9 @@ struct QkvKernelArgs {
   long long units;           // total_q * parts
   int batch, n_heads, kv_heads;
   int rotary_dim, interleaved, normalize, weight_f32, inv_freq_f32, zero_padding;
-  int parts, rows_per_part;  // a token's rows are shared by `parts` warps
+  long long v_units;         // append: total_q * v_parts units of V rows behind them
+  int v_parts;               // ceil(kv_heads / 8)
+  int parts, rows_per_part;  // a token's q and k rows are shared by `parts` warps
   int page_shift, table_width, num_pages;
   float eps;
 };

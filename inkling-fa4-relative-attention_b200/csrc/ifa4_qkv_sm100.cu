@@ -21,8 +21,9 @@
 // HBM bound in bytes (671 MB at 32k tokens x 40 heads in 118 us, 5.7 TB/s, where the rotation alone
 // runs at 6.1 and a device copy at 6.55), held back by the work per row: 20 warps per SM keep some
 // 40 KB of loads in flight, and a quad takes over 200 instructions and a chain of three shuffles
-// and a reciprocal root.  The append writes its rows to pages (402 MB in 81 us, 5.0 TB/s; 5.9 for
-// the copies alone), the backward (1007 MB) takes 184 us, 5.5 TB/s.  Measured and slower at those
+// and a reciprocal root.  The append writes its rows to pages (402 MB in 75 us, 5.4 TB/s; 5.9 for
+// the copies alone; V rows have units of their own, 81 us when they were rows of the same units at
+// 122 registers), the backward (1007 MB) takes 184 us, 5.5 TB/s.  Measured and slower at those
 // sizes: half a warp per row with the pairs exchanged by shuffles 187 us (backward 293); 16
 // neighbouring dims a lane, whose accesses cover half sectors, for interleaved pairs 129 instead of
 // 105 (30011 tokens); equal runs of quads per warp over token borders 130; whole tokens in turn with
@@ -226,7 +227,7 @@ __device__ __forceinline__ float load_weight(const void* w, int f32, int i) {
 }
 
 template <int kRot, bool kAppend>
-__global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
+__global__ void __launch_bounds__(kThreads, 5)
     qkv_rows_kernel(const __grid_constant__ QkvKernelArgs a) {
   __shared__ __align__(16) float ws[2][128];
   __shared__ __align__(16) float2 angles[kWarps][64];
@@ -240,23 +241,29 @@ __global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
   }
   __syncthreads();
 
-  const int rows = a.n_heads + a.kv_heads + (kAppend ? a.kv_heads : 0);
-  const int v_rows = a.n_heads + a.kv_heads;  // first V row
+  const int rows = a.n_heads + a.kv_heads;
+  // place of a token's rows in a cache (append); null: none
+  auto slot = [&](const Where& w, uint16_t* cache, long long sp, long long st) -> uint16_t* {
+    if (!w.inside || w.pos < 0 || (w.pos >> a.page_shift) >= a.table_width) return nullptr;
+    const int page = __ldg(a.block_table + static_cast<long long>(w.b) * a.bt_stride +
+                           (w.pos >> a.page_shift));
+    if (page < 0 || page >= a.num_pages) return nullptr;
+    return cache + page * sp + (w.pos & ((1ll << a.page_shift) - 1)) * st;
+  };
   const long long step = static_cast<long long>(gridDim.x) * kWarps;
-  for (long long u = static_cast<long long>(blockIdx.x) * kWarps + warp; u < a.units; u += step) {
+  long long u = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  for (; u < a.units; u += step) {
     const long long t = a.parts == 1 ? u : u / a.parts;
     const int r0 = static_cast<int>(u - t * a.parts) * a.rows_per_part;
     const int r1 = min(rows, r0 + a.rows_per_part);
     const uint16_t* const qt = a.q + t * a.q_st;
     const uint16_t* const kt = a.k + t * a.k_st;
-    const uint16_t* const vt = kAppend ? a.v + t * a.v_st : nullptr;
     uint4 xa[2], xb[2];  // two steps of four rows in flight
     auto load = [&](int r, uint4& va, uint4& vb) {
       const int ri = r + oct;
       va = vb = make_uint4(0u, 0u, 0u, 0u);
       if (ri < r1) {
         const uint16_t* p = ri < a.n_heads ? qt + ri * a.q_sh : kt + (ri - a.n_heads) * a.k_sh;
-        if (kAppend && ri >= v_rows) p = vt + (ri - v_rows) * a.v_sh;
         va = ldg_v4(p + rot.a_off);
         vb = ldg_v4(p + rot.b_off);
       }
@@ -264,56 +271,38 @@ __global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
     load(r0, xa[0], xb[0]);
     load(r0 + 4, xa[1], xb[1]);
     const Where w = locate(a.cu_q, a.cu_k, a.batch, t, lane);
-    int page = -1;
-    if (kAppend && w.inside && w.pos >= 0 && (w.pos >> a.page_shift) < a.table_width)
-      page = __ldg(a.block_table + static_cast<long long>(w.b) * a.bt_stride +
-                   (w.pos >> a.page_shift));
-    rot.at(w.pos, lane, angles[warp]);
-    uint16_t* kc = nullptr;  // the token's slots in the caches
-    uint16_t* vc = nullptr;
-    if (kAppend && page >= 0 && page < a.num_pages) {
-      const long long in_page = w.pos & ((1ll << a.page_shift) - 1);
-      kc = a.k_cache + page * a.kc_sp + in_page * a.kc_st;
-      vc = a.v_cache + page * a.vc_sp + in_page * a.vc_st;
-    }
+    uint16_t* ko;  // the token's rows of k_out, or its slot in the K cache
+    if (kAppend) ko = slot(w, a.k_cache, a.kc_sp, a.kc_st);
+    else ko = w.inside || a.zero_padding ? a.k_out + t * a.ko_st : nullptr;
     uint16_t* const qo = w.inside || a.zero_padding ? a.q_out + t * a.qo_st : nullptr;
-    uint16_t* const ko = kAppend ? kc
-                                 : (w.inside || a.zero_padding ? a.k_out + t * a.ko_st : nullptr);
     const long long ko_sh = kAppend ? a.kc_sh : a.ko_sh;
+    rot.at(w.pos, lane, angles[warp]);
 
     auto finish = [&](int r, uint4 va, uint4 vb) {
       const int ri = r + oct;
       const bool is_q = ri < a.n_heads;
-      if (!kAppend || r < v_rows) {  // (warp-uniform) not V rows only
-        float x[16];
-        unpack8(va, x);
-        unpack8(vb, x + 8);
-        if (a.normalize) {
-          float s0 = x[0] * x[0], s1 = x[1] * x[1];
+      float x[16];
+      unpack8(va, x);
+      unpack8(vb, x + 8);
+      if (a.normalize) {
+        float s0 = x[0] * x[0], s1 = x[1] * x[1];
 #pragma unroll
-          for (int i = 2; i < 16; i += 2) {
-            s0 += x[i] * x[i];
-            s1 += x[i + 1] * x[i + 1];
-          }
-          const float rn = rsqrtf(row_sum(s0 + s1) * (1.f / 128.f) + a.eps);
-          float wt[16];
-          lane_weights(ws[is_q ? 0 : 1], rot.a_off, rot.b_off, wt);
+        for (int i = 2; i < 16; i += 2) {
+          s0 += x[i] * x[i];
+          s1 += x[i + 1] * x[i + 1];
+        }
+        const float rn = rsqrtf(row_sum(s0 + s1) * (1.f / 128.f) + a.eps);
+        float wt[16];
+        lane_weights(ws[is_q ? 0 : 1], rot.a_off, rot.b_off, wt);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] *= wt[i] * rn;
-        }
-        rot.template apply<false>(x);
-        if (!kAppend || ri < v_rows) {
-          va = pack8(x);
-          vb = pack8(x + 8);
-        }
+        for (int i = 0; i < 16; ++i) x[i] *= wt[i] * rn;
       }
+      rot.template apply<false>(x);
+      va = pack8(x);
+      vb = pack8(x + 8);
       if (!w.inside) va = vb = make_uint4(0u, 0u, 0u, 0u);
-      uint16_t* dst = is_q ? qo : ko;
-      long long off = is_q ? ri * a.qo_sh : (ri - a.n_heads) * ko_sh;
-      if (kAppend && ri >= v_rows) {
-        dst = vc;
-        off = (ri - v_rows) * a.vc_sh;
-      }
+      uint16_t* const dst = is_q ? qo : ko;
+      const long long off = is_q ? ri * a.qo_sh : (ri - a.n_heads) * ko_sh;
       if (ri < r1 && dst != nullptr) {
         *reinterpret_cast<uint4*>(dst + off + rot.a_off) = va;
         *reinterpret_cast<uint4*>(dst + off + rot.b_off) = vb;
@@ -329,6 +318,26 @@ __global__ void __launch_bounds__(kThreads, kAppend ? 4 : 5)
         if (r + 12 < r1) load(r + 12, xa[1], xb[1]);
         finish(r + 4, va, vb);
       }
+    }
+  }
+  if (kAppend) {
+    // V rows are copied: a unit is up to eight rows of a token, 16 lanes a row
+    const int hw = lane >> 4, l16 = lane & 15;
+    for (u -= a.units; u < a.v_units; u += step) {
+      const long long t = a.v_parts == 1 ? u : u / a.v_parts;
+      const int r0 = static_cast<int>(u - t * a.v_parts) * 8 + hw;
+      const uint16_t* const vt = a.v + t * a.v_st + 8 * l16;
+      uint4 x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + 2 * i < a.kv_heads) x[i] = ldg_v4(vt + (r0 + 2 * i) * a.v_sh);
+      const Where w = locate(a.cu_q, a.cu_k, a.batch, t, lane);
+      uint16_t* const vo = slot(w, a.v_cache, a.vc_sp, a.vc_st);
+      if (vo == nullptr) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (r0 + 2 * i < a.kv_heads)
+          *reinterpret_cast<uint4*>(vo + (r0 + 2 * i) * a.vc_sh + 8 * l16) = x[i];
     }
   }
 }
@@ -497,7 +506,7 @@ static cudaError_t launch_rows(const QkvKernelArgs& args, int sms, cudaStream_t 
   int cap = 0;
   cudaError_t e = resident_blocks(qkv::qkv_rows_kernel<kRot, kAppend>, sms, cache, &cap);
   if (e != cudaSuccess) return e;
-  const long long want = (args.units + qkv::kWarps - 1) / qkv::kWarps;
+  const long long want = (args.units + args.v_units + qkv::kWarps - 1) / qkv::kWarps;
   const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
   qkv::qkv_rows_kernel<kRot, kAppend><<<grid, qkv::kThreads, 0, stream>>>(args);
   return cudaGetLastError();
