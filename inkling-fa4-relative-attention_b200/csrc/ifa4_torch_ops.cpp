@@ -224,10 +224,12 @@ bool plain_weight(const MaybeTensor& t, const at::Tensor& like) {
          (t->dim() == 1 && t->numel() == 128 && t->stride(0) == 1 && t->device() == like.device() &&
           (t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat));
 }
-// The step's other arguments.  eps < 0: no norm.
+// The step's other arguments.  eps -1: no norm; any other value that is not >= 0 (NaN stands for
+// what the Python checks have to look at) is not the plain case.
 bool plain_step(const at::Tensor& like, const MaybeTensor& q_weight, const MaybeTensor& k_weight,
                 const MaybeTensor& inv_freq, const MaybeTensor& cu_q, const MaybeTensor& cu_k,
                 double eps) {
+  if (!(eps >= 0) && eps != -1.0) return false;
   if (!plain_cu(cu_q, like) || !plain_cu(cu_k, like) || !plain_weight(q_weight, like) ||
       !plain_weight(k_weight, like))
     return false;

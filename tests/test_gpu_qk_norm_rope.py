@@ -226,6 +226,22 @@ def test_empty_and_no_weight_gradients():
     assert dq.shape == e.shape and bool((dwq == 0).all()) and bool((dwk == 0).all())
 
 
+def test_eps_of_any_kind(both_paths):
+    """A whole number is an eps like any other; what is none is refused, rotation or not."""
+    x = _randn(5, 2, 128, seed=7).cuda()
+    inv = _inv_freq(64).cuda()
+    for eps in (0, 1):
+        got = inkling_qk_norm_rope(x, x, eps=eps, inv_freq=inv)[0]
+        assert torch.equal(got, inkling_qk_norm_rope(x, x, eps=float(eps), inv_freq=inv)[0])
+        want = oracle.norm_rope(_np(x), None, np.arange(5), eps, _np(inv), False)
+        _check_rows(got, want, _np(inv), False)
+    for eps in (-1.0, -1, -1e-6, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="eps"):
+            inkling_qk_norm_rope(x, x, eps=eps, inv_freq=inv)
+        with pytest.raises(ValueError, match="eps"):
+            inkling_qk_norm_rope_backward(x, x, x, x, eps=eps, inv_freq=inv)
+
+
 def test_refusals():
     x = torch.zeros(4, 2, 128, dtype=torch.bfloat16, device="cuda")
     cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
