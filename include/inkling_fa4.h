@@ -330,13 +330,15 @@ int ifa4_rel_logits_launch(const IFA4RelLogitsParams* params, void* stream);
  * decode.block_table is required (a paged cache), causal_align must be IFA4_ALIGN_BOTTOM_RIGHT,
  * row b of q / rel / out belongs to sequence b (total_q = batch, cu_seqlens_q = 0..batch), and
  * n_heads / kv_heads <= 128.  All sequences of at least shared_prefix_len keys must hold the same
- * keys and values there (normally the same pages; the pages are taken from the table row of one
- * of them); shorter ones are attended whole through their own table rows.
+ * keys and values there, as far as their windows reach (normally the same pages; the pages are
+ * taken from the table row of the one whose window reaches furthest back among those that are
+ * worked on together); shorter ones are attended whole through their own table rows.  A value that
+ * is no number reaches every sequence that is worked on with one that sees it.
  * decode.num_splits / chunk_len plan the keys behind the prefix; decode.max_seqlen_k is the
  * longest whole sequence, prefix included.  Deterministic: no atomics on results. */
 typedef struct IFA4SharedPrefixParams {
   IFA4DecodeParams decode;
-  int32_t shared_prefix_len;  /* >= 0; 0 is a plain decode                                 */
+  int32_t shared_prefix_len;  /* 0 to 2^30; 0 is a plain decode                            */
   int32_t prefix_splits;      /* CTAs that share a row tile's prefix keys; 0 = automatic   */
 } IFA4SharedPrefixParams;
 

@@ -906,8 +906,9 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
   const IFA4DecodeParams* d = &p->decode;
   int rc = validate_common(d, what);
   if (rc) return rc;
-  if (p->shared_prefix_len < 0)
-    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: shared_prefix_len must be >= 0", what);
+  if (p->shared_prefix_len < 0 || p->shared_prefix_len > (1 << 30))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: shared_prefix_len %d outside [0, 2^30]", what,
+                p->shared_prefix_len);
   if (p->prefix_splits < 0 || p->prefix_splits > 1024)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: prefix_splits %d outside [0, 1024]", what,
                 p->prefix_splits);

@@ -73,9 +73,12 @@ struct Bars {
   uint64_t drain;
   uint32_t tmem_base;
   int abort_flag;
-  int lo;   // first visible key over the CTA's rows (past the prefix: no row takes part)
-  int ref;  // first of the CTA's sequences that take part: its table row names the prefix pages
+  // Over the CTA's rows that take part: the first visible key (upper half) and, of the sequences
+  // that see it, the first (lower half), whose table row names the prefix pages: with a window no
+  // other row needs to name all of them still.  All ones: no row takes part.
+  unsigned long long first;
 };
+constexpr unsigned long long kNoRow = ~0ull;
 static_assert(sizeof(Bars) <= 256, "barrier block");
 
 // Position in a ring of kStages stages.
@@ -159,8 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
-    bars->lo = 0x7fffffff;
-    bars->ref = 0x7fffffff;
+    bars->first = kNoRow;
     fence_mbar_init();
     // Q right away: it depends on nothing
     const uint64_t pol_q = l2_policy_evict_first();
@@ -200,11 +202,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (a.window_left >= 0) key_lo = max(0, me.len - 1 - a.window_left);
     if (key_lo >= a.prefix_len) me.on = false;
     const int lo = __reduce_min_sync(0xffffffffu, me.on ? key_lo : 0x7fffffff);
-    const int ref = __reduce_min_sync(0xffffffffu, me.on ? me.b : 0x7fffffff);
-    if (lane == 0 && lo != 0x7fffffff) {
-      atomicMin(&bars->lo, lo);
-      atomicMin(&bars->ref, ref);
-    }
+    const int ref = __reduce_min_sync(0xffffffffu, me.on && key_lo == lo ? me.b : 0x7fffffff);
+    if (lane == 0 && lo != 0x7fffffff)
+      atomicMin(&bars->first, static_cast<unsigned long long>(lo) << 32 | static_cast<unsigned>(ref));
   }
   tc_fence_before();
   __syncthreads();
@@ -212,8 +212,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tbase = bars->tmem_base;
   // this CTA's share of the key tiles
   int j_lo = 0, n_kv = 0;
-  if (bars->ref != 0x7fffffff) {
-    const int first = bars->lo / kBN, all = (a.prefix_len + kBN - 1) / kBN - first;
+  if (bars->first != kNoRow) {
+    const int first = static_cast<int>(bars->first >> 32) / kBN;
+    const int all = (a.prefix_len + kBN - 1) / kBN - first;
     const int per = (all + a.splits - 1) / a.splits;
     j_lo = first + split * per;
     n_kv = max(0, min(per, all - split * per));
@@ -230,13 +231,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int box = 1 << a.box_shift;
       const int units = kBN >> a.box_shift;
       const int page_mask = (1 << a.page_shift) - 1;
-      const int32_t* bt = a.block_table + static_cast<long long>(bars->ref) * a.bt_stride;
-      // page of unit `lane` of key tile j; -1 past the prefix or for an entry outside
-      // [0, num_pages)
+      const int first_key = static_cast<int>(bars->first >> 32);
+      const int32_t* bt =
+          a.block_table + static_cast<long long>(bars->first & 0xffffffffu) * a.bt_stride;
+      // page of unit `lane` of key tile j; -1 past the prefix, before the first visible key (a page
+      // that has left every window may hold anything by now) or for an entry outside [0, num_pages)
       auto unit_block = [&](int j) {
         const int key = (j_lo + j) * kBN + lane * box;
         int blk = -1;
-        if (lane < units && key < a.prefix_len) {
+        if (lane < units && key < a.prefix_len && key + box > first_key) {
           blk = __ldg(bt + (key >> a.page_shift));
           if (blk < 0 || blk >= a.num_pages) blk = -1;
         }

@@ -438,7 +438,7 @@ Tensors decode_shared_prefix_op(const at::Tensor& q, const at::Tensor& k, const 
       block_table.scalar_type() != at::kInt || block_table.device() != q.device() ||
       block_table.size(0) != q.size(0) || block_table.numel() == 0 || block_table.stride(1) != 1 ||
       shared_prefix_len < 0 || shared_prefix_len > block_table.size(1) * page_size ||
-      shared_prefix_len > 0x7fffffff || !(softmax_scale > 0))
+      shared_prefix_len > (1 << 30) || !(softmax_scale > 0))
     return {};
   for (int64_t x : {window_left, max_seqlen_k, num_splits, chunk_len, prefix_splits})
     if (x < -1 || x > 0x7fffffff) return {};
@@ -453,13 +453,11 @@ Tensors decode_shared_prefix_op(const at::Tensor& q, const at::Tensor& k, const 
   size_t need = 0;
   if (ifa4_decode_shared_prefix_workspace_size(&p, &need)) return {};
   at::Tensor ws;
-  if (need > 0) {
-    if (workspace.has_value() && workspace->device() == q.device() && workspace->is_contiguous() &&
-        aligned16(*workspace) && static_cast<size_t>(workspace->nbytes()) >= need)
-      ws = *workspace;
-    else
-      ws = bytes_like(q, need);
-  }
+  if (workspace.has_value() && (workspace->device() != q.device() || !workspace->is_contiguous()))
+    return {};
+  if (need > 0)
+    ws = workspace.has_value() && static_cast<size_t>(workspace->nbytes()) >= need
+             ? *workspace : bytes_like(q, need);
   if (ifa4_decode_shared_prefix_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(q)))
     return {};
   return {out};

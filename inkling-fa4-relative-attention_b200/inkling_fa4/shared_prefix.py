@@ -25,10 +25,12 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
 
     ``cu_seqlens_k`` counts all keys of a sequence, prefix included, and ``block_table`` rows
     list all its pages.  Every sequence of at least ``shared_prefix_len`` keys must hold the same
-    keys and values there; normally the table rows begin with the same pages, and the pages of
-    one of these sequences are the ones that are read.  Sequences with fewer keys share nothing
+    keys and values there, as far as its window reaches; normally the table rows begin with the
+    same pages, and the pages of one of these sequences, of those that are worked on together the
+    one whose window reaches furthest back, are the ones that are read.  (A value among them that
+    is no number reaches every sequence that is worked on with one that sees it.)  Sequences with fewer keys share nothing
     and are attended through their own pages.  ``shared_prefix_len`` is a host integer (it sizes
-    the grid) and need not be a multiple of the page size; 0 is a plain decode.
+    the grid, at most 2^30) and need not be a multiple of the page size; 0 is a plain decode.
 
     One query per sequence (``cu_seqlens_q`` = 0..batch), at most 128 query heads per KV head.
     ``prefix_splits``: CTAs that share a row tile's prefix keys (0: automatic); ``num_splits`` /
@@ -55,11 +57,15 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
     if q.shape[0] != cu_seqlens_q.numel() - 1:
         raise ValueError(f"{name}: expects exactly one query token per sequence")
     shared_prefix_len = int(shared_prefix_len)
-    if not 0 <= shared_prefix_len < 1 << 31:
-        raise ValueError(f"{name}: shared_prefix_len must be in [0, 2^31)")
+    if not 0 <= shared_prefix_len <= 1 << 30:
+        raise ValueError(f"{name}: shared_prefix_len must be in [0, 2^30]")
     if shared_prefix_len > block_table.shape[1] * k.shape[1]:
         raise ValueError(f"{name}: shared_prefix_len {shared_prefix_len} is beyond the table's "
                          f"{block_table.shape[1]} pages of {k.shape[1]}")
+    if workspace is not None and not (isinstance(workspace, torch.Tensor)
+                                      and workspace.device == q.device
+                                      and workspace.is_contiguous()):
+        raise ValueError(f"{name}: workspace must be a contiguous tensor on q's device")
     max_seqlen_k = int(max_seqlen_k) if max_seqlen_k else 0
     p = _lib.SharedPrefixParams()
     p.decode = _ops._decode_params(q, k, v, rel, out, cu_seqlens_q, cu_seqlens_k, n_heads,

@@ -165,6 +165,25 @@ def test_prefix_of_zero_is_the_plain_decode():
     assert torch.equal(b.run(prefix=0), b.plain())
 
 
+@pytest.mark.parametrize("own", [[700, 650, 610], [610] * 20 + [700] * 60])
+@pytest.mark.parametrize("page", [16, 64])
+def test_pages_behind_every_window(own, page):
+    """Pages that have left a sequence's window may be gone from its table row, and from the cache:
+    those no window reaches hold NaN by now.  The windows of the sequences behind the first ones
+    reach further back than theirs, or less far (20 + 60 sequences, three row tiles)."""
+    prefix, window = 1000, 1000
+    b = Batch(prefix, own, 8, 2, 128, page, seed=12)
+    live = torch.zeros(b.kc.shape[0], dtype=torch.bool)
+    for i, n in enumerate(b.lens):
+        first = (n - 1 - window) // page  # the page of the first visible key
+        live[b.table[i, first:-(-n // page)].long()] = True
+        b.table[i, :first] = -1
+    assert not live.all()
+    b.kc[~live] = float("nan")
+    b.vc[~live] = float("nan")
+    b.cuda().check(window)
+
+
 def test_large_scores_and_masked_values():
     """Scores of several hundred: the running maximum moves between tiles.  The lowest bf16 value
     and -inf as bias hide keys; a row whose bias hides every key it sees gives 0."""
@@ -213,6 +232,12 @@ def test_refusals():
         b.run(prefix=-1)
     with pytest.raises(ValueError, match="beyond the table"):
         b.run(prefix=10000)
+    for ws in (torch.zeros(8 << 20, dtype=torch.uint8),  # on the CPU
+               torch.zeros(2 << 20, 8, dtype=torch.uint8, device="cuda")[:, ::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            b.run(workspace=ws)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        b.run(workspace=torch.zeros((8 << 20) + 8, dtype=torch.uint8, device="cuda")[8:])
     with pytest.raises(ValueError, match="one query"):
         inkling_fa4_rel_attention_decode_shared_prefix(
             b.q.repeat(2, 1, 1), b.kc, b.vc, b.rel.repeat(2, 1, 1), b.cu_q, b.cu_k, 1, 67, 16, 64,

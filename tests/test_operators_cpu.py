@@ -159,6 +159,7 @@ def _shared(**kw):
 
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(shared_prefix_len=-1), INVALID, b"shared_prefix_len"),
+    (dict(shared_prefix_len=(1 << 30) + 1), INVALID, b"shared_prefix_len"),
     (dict(prefix_splits=-1), INVALID, b"prefix_splits"),
     (dict(block_table=None), INVALID, b"block_table"),
     (dict(causal_align=_lib.IFA4_ALIGN_REFERENCE), UNSUPPORTED, b"bottom-right"),
