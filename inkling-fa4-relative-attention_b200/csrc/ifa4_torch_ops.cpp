@@ -1,5 +1,5 @@
-// torch operators over the C ABI: inkling_fa4::prefill_ and decode_, and (at the end of the file) the
-// operators next to the attention.
+// torch operators over the C ABI: inkling_fa4::prefill_ and decode_; and (at the end of the file) the
+// Python calls of the operators next to the attention.
 //
 // The Python package checks its arguments (the reference's call surface and error messages) and
 // then calls one of these operators, which fills the IFA4 parameter block from the tensors'
@@ -9,9 +9,14 @@
 // assignments and two foreign calls per attention call with one dispatcher call (the host cost
 // that bounds small launches).  The operators return the C ABI's status code; the caller turns a
 // nonzero code into an exception with ifa4_last_error_string().
+#include <Python.h>
+
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <ATen/record_function.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <vector>
@@ -191,8 +196,12 @@ int64_t decode_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
 // Operators next to the attention.  Each takes the arguments of its Python entry point as they are,
 // decides whether they are the plain case (types, shapes, one device, layouts the kernels read in
 // place), allocates the outputs, launches and returns them; anything else, failed launches among it,
-// returns an empty list, and the entry point then goes through its own checks and the C ABI, which
-// copy what has to be copied and say what is wrong.  So the usual call costs one dispatcher call.
+// returns nothing, and the entry point then goes through its own checks and the C ABI, which copy
+// what has to be copied and say what is wrong.  They are plain Python functions (the table at the end
+// of the file), not dispatcher operators: they have one implementation and no autograd formula, and
+// a small call costs the host more than the device.  Norm and rotation of 128 tokens: 5.4 us of host
+// time a call, 8.2 as a dispatcher operator (whose argument matching and boxing took 2 us); the append
+// of one token 6.0 us with its Python part, 11 before.
 // ---------------------------------------------------------------------------------------------
 typedef std::vector<at::Tensor> Tensors;
 typedef c10::optional<at::Tensor> MaybeTensor;
@@ -202,16 +211,19 @@ bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_
 void* stream_of(const at::Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
 at::Tensor bytes_like(const at::Tensor& t, size_t n) {
-  return at::empty({static_cast<int64_t>(n)}, t.options().dtype(at::kByte));
+  return new_tensor({static_cast<int64_t>(n)}, at::kByte, t);
 }
 at::Tensor rows_like(const at::Tensor& t) {  // contiguous, same sizes
-  return at::empty(t.sizes(), t.options());
+  return new_tensor(t.sizes(), at::kBFloat16, t);
 }
 
 // [tokens, heads, 128] bf16 rows the kernels read in place.
 bool plain_rows(const at::Tensor& t, const at::Tensor& like) {
-  return t.dim() == 3 && t.size(2) == 128 && t.scalar_type() == at::kBFloat16 &&
+  return t.is_cuda() && t.dim() == 3 && t.size(2) == 128 && t.scalar_type() == at::kBFloat16 &&
          t.device() == like.device() && t.size(0) == like.size(0) && t.stride(2) == 1 &&
          t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned16(t);
 }
@@ -318,11 +330,11 @@ Tensors qk_norm_rope_backward_op(const at::Tensor& dq_out, const at::Tensor& dk_
   fill_norm_rope(&p, q_weight, k_weight, inv_freq, cu_q, cu_k, q.size(0), q.size(1), k.size(1),
                  interleaved, eps);
   if (q_weight.has_value() && want_q_weight) {
-    out.push_back(at::empty_like(*q_weight));
+    out.push_back(new_tensor({128}, q_weight->scalar_type(), q));
     p.dq_weight = out.back().data_ptr();
   }
   if (k_weight.has_value() && want_k_weight) {
-    out.push_back(at::empty_like(*k_weight));
+    out.push_back(new_tensor({128}, k_weight->scalar_type(), q));
     p.dk_weight = out.back().data_ptr();
   }
   p.dq_out = dq_out.data_ptr();
@@ -474,13 +486,13 @@ bool plain_starts(const at::Tensor& starts, const at::Tensor& like) {
 
 Tensors bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, int64_t total_q,
                        int64_t rel_extent) {
-  if (table.dim() != 2 || (table.scalar_type() != at::kFloat && table.scalar_type() != at::kBFloat16) ||
+  if (!table.is_cuda() || table.dim() != 2 || (table.scalar_type() != at::kFloat && table.scalar_type() != at::kBFloat16) ||
       !plain_starts(starts, table) || table.size(0) != starts.numel() || table.size(1) < 1 ||
       total_q < 0 || rel_extent < 1 || rel_extent > (1 << 24))
     return {};
   const c10::cuda::CUDAGuard guard(table.device());
   const int64_t heads = table.size(1);
-  const at::Tensor rel = at::empty({heads, rel_extent}, table.options().dtype(at::kBFloat16));
+  const at::Tensor rel = new_tensor({heads, rel_extent}, at::kBFloat16, table);
   IFA4BucketBiasParams p{};
   p.table = table.data_ptr();
   p.starts = static_cast<const int32_t*>(starts.data_ptr());
@@ -493,12 +505,15 @@ Tensors bucket_bias_op(const at::Tensor& table, const at::Tensor& starts, int64_
   p.buckets = static_cast<int32_t>(starts.numel());
   p.weight_dtype = weight_dtype(table);
   if (ifa4_bucket_bias_launch(&p, stream_of(table))) return {};
-  return {rel.unsqueeze(0).expand({total_q, heads, rel_extent})};
+  // the tokens of rel_logits are the same memory
+  const int64_t sizes[] = {total_q, heads, rel_extent}, strides[] = {0, rel_extent, 1};
+  rel.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes), at::IntArrayRef(strides));
+  return {rel};
 }
 
 Tensors bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts, bool f32,
                                 const MaybeTensor& cu_q) {
-  if (drel.dim() != 3 || drel.scalar_type() != at::kBFloat16 || drel.size(1) < 1 ||
+  if (!drel.is_cuda() || drel.dim() != 3 || drel.scalar_type() != at::kBFloat16 || drel.size(1) < 1 ||
       drel.size(2) < 1 || drel.size(2) > (1 << 24) || (drel.size(2) > 1 && drel.stride(2) != 1) ||
       !plain_starts(starts, drel))
     return {};
@@ -506,8 +521,8 @@ Tensors bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts
                            cu_q->device() != drel.device() || cu_q->stride(0) != 1))
     return {};
   const c10::cuda::CUDAGuard guard(drel.device());
-  const at::Tensor dtable = at::empty({starts.numel(), drel.size(1)},
-                                      drel.options().dtype(f32 ? at::kFloat : at::kBFloat16));
+  const at::Tensor dtable = new_tensor({starts.numel(), drel.size(1)},
+                                       f32 ? at::kFloat : at::kBFloat16, drel);
   IFA4BucketBiasBackwardParams p{};
   p.drel = drel.data_ptr();
   p.starts = static_cast<const int32_t*>(starts.data_ptr());
@@ -533,7 +548,193 @@ Tensors bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts
   return {dtable};
 }
 
+// ---------------------------------------------------------------------------------------------
+// The same as Python functions: positional arguments; a tuple of tensors, or None.
+// ---------------------------------------------------------------------------------------------
+struct Arguments {
+  PyObject* const* objects;
+  Py_ssize_t count;
+  Py_ssize_t next = 0;
+  bool ok = true;  // false: a type that is not the plain case
+
+  PyObject* take() {
+    if (next < count) return objects[next++];
+    ok = false;
+    return Py_None;
+  }
+  at::Tensor tensor_of(PyObject* o) {
+    if (THPVariable_Check(o)) return THPVariable_Unpack(o);
+    ok = false;
+    return at::Tensor();
+  }
+  at::Tensor tensor() { return tensor_of(take()); }
+  MaybeTensor maybe() {
+    PyObject* o = take();
+    if (o == Py_None) return c10::nullopt;
+    return tensor_of(o);
+  }
+  bool flag() {
+    PyObject* o = take();
+    ok = ok && PyBool_Check(o);
+    return o == Py_True;
+  }
+  int64_t integer() {
+    PyObject* o = take();
+    int overflow = 0;
+    if (!PyLong_Check(o)) {
+      ok = false;
+      return 0;
+    }
+    const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+    ok = ok && overflow == 0;
+    return v;
+  }
+  double real() {
+    PyObject* o = take();
+    ok = ok && PyFloat_Check(o);
+    return ok ? PyFloat_AS_DOUBLE(o) : 0.0;
+  }
+  bool complete() const { return ok && next == count; }
+};
+
+// Other Python threads run while this one allocates and launches.
+struct WithoutGil {
+  PyThreadState* state = PyEval_SaveThread();
+  ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
+// Reads the arguments (`read`, which returns the work) and does the work.
+template <class Read>
+PyObject* call(const char* name, PyObject* const* objects, Py_ssize_t count, Read read) {
+  Tensors out;
+  try {
+    RECORD_FUNCTION(name, c10::ArrayRef<const c10::IValue>{});
+    Arguments a{objects, count};
+    auto work = read(a);
+    if (a.complete()) {
+      WithoutGil no_gil;
+      out = work();
+    }
+  } catch (const std::exception&) {  // an allocation, a tensor without memory: the checks say it
+    out.clear();
+  }
+  if (out.empty()) Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(static_cast<Py_ssize_t>(out.size()));
+  if (result == nullptr) return nullptr;
+  for (size_t i = 0; i < out.size(); ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(out[i]));
+    if (o == nullptr) {
+      Py_DECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, static_cast<Py_ssize_t>(i), o);
+  }
+  return result;
+}
+
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::qk_norm_rope", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), k = a.tensor();
+    auto wq = a.maybe(), wk = a.maybe(), inv_freq = a.maybe(), cu_q = a.maybe(), cu_k = a.maybe();
+    const bool interleaved = a.flag();
+    const double eps = a.real();
+    return [=] { return qk_norm_rope_op(q, k, wq, wk, inv_freq, cu_q, cu_k, interleaved, eps); };
+  });
+}
+
+PyObject* py_qk_norm_rope_backward(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::qk_norm_rope_backward", objects, count, [](Arguments& a) {
+    auto dq_out = a.tensor(), dk_out = a.tensor(), q = a.tensor(), k = a.tensor();
+    auto wq = a.maybe(), wk = a.maybe(), inv_freq = a.maybe(), cu_q = a.maybe(), cu_k = a.maybe();
+    const bool interleaved = a.flag();
+    const double eps = a.real();
+    const bool want_q = a.flag(), want_k = a.flag();
+    return [=] {
+      return qk_norm_rope_backward_op(dq_out, dk_out, q, k, wq, wk, inv_freq, cu_q, cu_k,
+                                      interleaved, eps, want_q, want_k);
+    };
+  });
+}
+
+PyObject* py_kv_append(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::kv_append", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), k = a.tensor(), v = a.tensor();
+    auto k_cache = a.tensor(), v_cache = a.tensor();
+    auto wq = a.maybe(), wk = a.maybe(), inv_freq = a.maybe();
+    auto cu_q = a.tensor(), cu_k = a.tensor(), block_table = a.tensor();
+    const bool interleaved = a.flag();
+    const double eps = a.real();
+    return [=] {
+      return kv_append_op(q, k, v, k_cache, v_cache, wq, wk, inv_freq, cu_q, cu_k, block_table,
+                          interleaved, eps);
+    };
+  });
+}
+
+PyObject* py_decode_shared_prefix(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::decode_shared_prefix", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), k = a.tensor(), v = a.tensor(), rel = a.tensor();
+    auto cu_q = a.tensor(), cu_k = a.tensor(), block_table = a.tensor();
+    auto workspace = a.maybe();
+    const int64_t rel_extent = a.integer(), window_left = a.integer(), max_seqlen_k = a.integer();
+    const double softmax_scale = a.real();
+    const int64_t num_splits = a.integer(), chunk_len = a.integer();
+    const int64_t shared_prefix_len = a.integer(), prefix_splits = a.integer();
+    return [=] {
+      return decode_shared_prefix_op(q, k, v, rel, cu_q, cu_k, block_table, workspace, rel_extent,
+                                     window_left, max_seqlen_k, softmax_scale, num_splits,
+                                     chunk_len, shared_prefix_len, prefix_splits);
+    };
+  });
+}
+
+PyObject* py_bucket_bias(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::bucket_bias", objects, count, [](Arguments& a) {
+    auto table = a.tensor(), starts = a.tensor();
+    const int64_t total_q = a.integer(), rel_extent = a.integer();
+    return [=] { return bucket_bias_op(table, starts, total_q, rel_extent); };
+  });
+}
+
+PyObject* py_bucket_bias_backward(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::bucket_bias_backward", objects, count, [](Arguments& a) {
+    auto drel = a.tensor(), starts = a.tensor();
+    const bool f32 = a.flag();
+    auto cu_q = a.maybe();
+    return [=] { return bucket_bias_backward_op(drel, starts, f32, cu_q); };
+  });
+}
+
+template <class F>
+PyMethodDef method(const char* name, F* f) {
+  return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL,
+          nullptr};
+}
+PyMethodDef kMethods[] = {
+    method("qk_norm_rope", py_qk_norm_rope),
+    method("qk_norm_rope_backward", py_qk_norm_rope_backward),
+    method("kv_append", py_kv_append),
+    method("decode_shared_prefix", py_decode_shared_prefix),
+    method("bucket_bias", py_bucket_bias),
+    method("bucket_bias_backward", py_bucket_bias_backward),
+};
 }  // namespace
+
+// A dict of the functions above by name (called once, with the GIL held).
+extern "C" PyObject* ifa4_python_calls(void) {
+  PyObject* calls = PyDict_New();
+  if (calls == nullptr) return nullptr;
+  for (PyMethodDef& m : kMethods) {
+    PyObject* f = PyCFunction_New(&m, nullptr);
+    const int rc = f == nullptr ? -1 : PyDict_SetItemString(calls, m.ml_name, f);
+    Py_XDECREF(f);
+    if (rc != 0) {
+      Py_DECREF(calls);
+      return nullptr;
+    }
+  }
+  return calls;
+}
 
 TORCH_LIBRARY(inkling_fa4, m) {
   m.def("prefill_(Tensor q, Tensor k, Tensor v, Tensor rel, Tensor(a!) out, Tensor cu_q, "
@@ -544,29 +745,9 @@ TORCH_LIBRARY(inkling_fa4, m) {
         "Tensor cu_k, Tensor(b!)? lse, Tensor? block_table, Tensor? workspace, int rel_extent, "
         "bool causal, int window_left, int causal_align, int max_seqlen_k, float softmax_scale, "
         "int num_splits, int chunk_len) -> int");
-  m.def("decode_shared_prefix(Tensor q, Tensor k, Tensor v, Tensor rel, Tensor cu_q, Tensor cu_k, "
-        "Tensor block_table, Tensor(a!)? workspace, int rel_extent, int window_left, "
-        "int max_seqlen_k, float softmax_scale, int num_splits, int chunk_len, "
-        "int shared_prefix_len, int prefix_splits) -> Tensor[]");
-  m.def("qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, "
-        "Tensor? cu_q, Tensor? cu_k, bool interleaved, float eps) -> Tensor[]");
-  m.def("qk_norm_rope_backward(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor? q_weight, "
-        "Tensor? k_weight, Tensor? inv_freq, Tensor? cu_q, Tensor? cu_k, bool interleaved, "
-        "float eps, bool want_q_weight, bool want_k_weight) -> Tensor[]");
-  m.def("kv_append_(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, "
-        "Tensor? q_weight, Tensor? k_weight, Tensor? inv_freq, Tensor cu_q, Tensor cu_k, "
-        "Tensor block_table, bool interleaved, float eps) -> Tensor[]");
-  m.def("bucket_bias(Tensor table, Tensor starts, int total_q, int rel_extent) -> Tensor[]");
-  m.def("bucket_bias_backward(Tensor drel, Tensor starts, bool f32, Tensor? cu_q) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("prefill_", &prefill_op);
   m.impl("decode_", &decode_op);
-  m.impl("decode_shared_prefix", &decode_shared_prefix_op);
-  m.impl("qk_norm_rope", &qk_norm_rope_op);
-  m.impl("qk_norm_rope_backward", &qk_norm_rope_backward_op);
-  m.impl("kv_append_", &kv_append_op);
-  m.impl("bucket_bias", &bucket_bias_op);
-  m.impl("bucket_bias_backward", &bucket_bias_backward_op);
 }

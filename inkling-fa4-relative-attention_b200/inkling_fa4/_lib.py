@@ -198,7 +198,7 @@ class Ifa4Error(RuntimeError):
 
 _lib = None
 _torch_ops = None
-_overloads = {}
+_calls = {}  # Python calls of the operator library by name
 TORCH_OPS_PATH = os.path.join(_LIB_DIR, "libifa4_torch_ops.so")
 
 
@@ -217,32 +217,24 @@ def torch_ops():
 
     lib()  # load the C ABI first (one shared instance: status word, last-error message)
     torch.ops.load_library(TORCH_OPS_PATH)
+    make = ctypes.PyDLL(TORCH_OPS_PATH).ifa4_python_calls
+    make.restype, make.argtypes = ctypes.py_object, []
+    _calls.update(make())
     _torch_ops = torch.ops.inkling_fa4
     return _torch_ops
 
 
-def torch_op(name: str):
-    """The operator ``inkling_fa4::name`` ready to call (looked up once), or None as ``torch_ops``."""
-    op = _overloads.get(name)
-    if op is None:
-        ops = torch_ops()
-        if ops is None:
+def plain_call(name: str, *args):
+    """What the Python call ``name`` of the operator library (csrc/ifa4_torch_ops.cpp) returns for a
+    plain call, or None: the arguments are not its plain case (or not tensors at all, or on the
+    CPU), its launch failed, or there is no operator library; the caller then goes through its own
+    checks and the C ABI."""
+    call = _calls.get(name)
+    if call is None:
+        if torch_ops() is None:
             return None
-        op = _overloads[name] = getattr(ops, name).default
-    return op
-
-
-def try_op(name: str, *args):
-    """The outputs of the operator ``inkling_fa4::name`` for a plain call, or None: the arguments
-    are not its plain case (or not tensors at all, or on the CPU), its launch failed, or there is no
-    operator library; the caller then goes through its own checks and the C ABI."""
-    op = _overloads.get(name) or torch_op(name)
-    if op is None:
-        return None
-    try:
-        return op(*args) or None
-    except (RuntimeError, TypeError):
-        return None
+        call = _calls[name]
+    return call(*args)
 
 
 def lib() -> ctypes.CDLL:

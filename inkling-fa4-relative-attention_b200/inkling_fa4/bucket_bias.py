@@ -63,7 +63,7 @@ def _weight_dtype(name, dtype):
 def _forward(table, starts, total_q, rel_extent):
     name = "bucket_bias"
     if _ops.USE_TORCH_OPS:
-        outs = _lib.try_op("bucket_bias", table, starts, total_q, rel_extent)
+        outs = _lib.plain_call("bucket_bias", table, starts, total_q, rel_extent)
         if outs is not None:
             return outs[0]
     if not isinstance(table, torch.Tensor):
@@ -92,12 +92,17 @@ def _forward(table, starts, total_q, rel_extent):
 
 
 def _backward(drel, starts, dtype, cu_seqlens_q):
-    name = "bucket_bias_backward"
     if _ops.USE_TORCH_OPS and (dtype is torch.float32 or dtype is torch.bfloat16):
-        outs = _lib.try_op("bucket_bias_backward", drel, starts, dtype is torch.float32,
-                           cu_seqlens_q)
+        outs = _lib.plain_call("bucket_bias_backward", drel, starts, dtype is torch.float32,
+                               cu_seqlens_q)
         if outs is not None:
             return outs[0]
+    return _checked_backward(drel, starts, dtype, cu_seqlens_q)
+
+
+@torch.no_grad()
+def _checked_backward(drel, starts, dtype, cu_seqlens_q):
+    name = "bucket_bias_backward"
     if not isinstance(drel, torch.Tensor):
         raise TypeError(f"{name}: drel must be a torch.Tensor")
     if not drel.is_cuda:
@@ -166,7 +171,6 @@ def inkling_bucket_bias(table, starts, total_q, rel_extent, cu_seqlens_q=None):
     return _forward(table, starts, total_q, rel_extent)
 
 
-@torch.no_grad()
 def inkling_bucket_bias_backward(drel, starts, num_buckets, *, dtype=torch.float32,
                                  cu_seqlens_q=None):
     """Gradient ``[num_buckets, n_heads]`` (``dtype`` float32 or bfloat16) of the table given the

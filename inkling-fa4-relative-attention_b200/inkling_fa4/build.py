@@ -20,6 +20,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -71,9 +72,10 @@ def build(verbose: bool = False, force: bool = False, debug: bool = False) -> st
 
 
 def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
-    """Compile ``csrc/ifa4_torch_ops.cpp`` (the torch operators inkling_fa4::prefill_,
-    inkling_fa4::decode_ and so on over the C ABI) with g++ against torch's headers and libraries, linked
-    to the in-tree ``libinkling_fa4.so`` (found next to it at run time)."""
+    """Compile ``csrc/ifa4_torch_ops.cpp`` (the torch operators inkling_fa4::prefill_ and
+    inkling_fa4::decode_ and the Python calls of the other operators, over the C ABI) with g++
+    against torch's and Python's headers and libraries, linked to the in-tree
+    ``libinkling_fa4.so`` (found next to it at run time)."""
     import torch
     from torch.utils import cpp_extension
 
@@ -84,13 +86,15 @@ def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
         if os.path.getmtime(OUT_TORCH_OPS) >= newest:
             return OUT_TORCH_OPS
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
-    incs = cpp_extension.include_paths() + [os.path.join(cuda_home, "include")]
+    incs = cpp_extension.include_paths() + [os.path.join(cuda_home, "include"),
+                                            sysconfig.get_paths()["include"]]
     libdir = cpp_extension.library_paths()[0]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     tmp = OUT_TORCH_OPS + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *[f"-I{i}" for i in incs], src, "-o", tmp, f"-L{libdir}", f"-L{os.path.dirname(OUT)}",
-           "-linkling_fa4", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+           "-linkling_fa4", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+           "-ltorch",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libdir}"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -23,7 +23,7 @@ import torch
 from . import _lib, _ops
 
 HEAD_DIM = _ops.HEAD_DIM
-_NO_NORM = -1.0  # eps the operators take for "no norm"
+_NO_NORM = -1.0  # eps that the plain calls take for "no norm"
 
 
 def _rows_ready(t: torch.Tensor) -> torch.Tensor:
@@ -35,7 +35,7 @@ def _rows_ready(t: torch.Tensor) -> torch.Tensor:
 
 
 def _eps(eps):
-    """eps as the operators take it: negative for no norm, NaN (never the plain case) for a value
+    """eps as the plain calls take it: -1 for no norm, NaN (never the plain case) for a value
     that the checks will refuse."""
     if eps is None:
         return _NO_NORM
@@ -153,8 +153,8 @@ def _stream(device):
 def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
     name = "qk_norm_rope"
     if _ops.USE_TORCH_OPS:
-        outs = _lib.try_op("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, cu_q, cu_k,
-                           interleaved, _eps(eps))
+        outs = _lib.plain_call("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, cu_q, cu_k,
+                               interleaved, _eps(eps))
         if outs is not None:
             return outs[0], outs[1]
     _check_rows(name, "q", q, None)
@@ -180,12 +180,19 @@ def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_fre
               weight_grads):
     name = "qk_norm_rope_backward"
     if _ops.USE_TORCH_OPS:
-        outs = _lib.try_op("qk_norm_rope_backward", dq_out, dk_out, q, k, q_weight, k_weight,
-                           inv_freq, cu_q, cu_k, interleaved, _eps(eps), *weight_grads)
+        outs = _lib.plain_call("qk_norm_rope_backward", dq_out, dk_out, q, k, q_weight, k_weight,
+                               inv_freq, cu_q, cu_k, interleaved, _eps(eps), *weight_grads)
         if outs is not None:
             dq, dk, *dw = outs
             dqw = dw.pop(0) if q_weight is not None and weight_grads[0] else None
             return dq, dk, dqw, dw.pop(0) if dw else None
+    return _checked_backward(name, dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps,
+                             inv_freq, interleaved, weight_grads)
+
+
+@torch.no_grad()
+def _checked_backward(name, dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq,
+                      interleaved, weight_grads):
     _check_rows(name, "q", q, None)
     _check_rows(name, "k", k, q)
     _check_rows(name, "dq_out", dq_out, q, q.shape[1])
@@ -257,7 +264,6 @@ def inkling_qk_norm_rope(q, k, q_weight=None, k_weight=None, cu_seqlens_q=None, 
                     interleaved)
 
 
-@torch.no_grad()
 def inkling_qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight=None, k_weight=None,
                                   cu_seqlens_q=None, cu_seqlens_k=None, *, eps=1e-6,
                                   inv_freq=None, interleaved=False):
@@ -268,7 +274,6 @@ def inkling_qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight=None, k_weight=
                      inv_freq, interleaved, (True, True))
 
 
-@torch.no_grad()
 def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlens_k, *, q=None,
                       q_weight=None, k_weight=None, eps=1e-6, inv_freq=None, interleaved=False,
                       q_out=None):
@@ -288,12 +293,20 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
 
     Returns the queries (``q_out`` if given, which may be ``q`` itself: rows behind the last
     sequence are then left as they were; a new tensor has zeros there), or None without ``q``."""
-    name = "kv_append"
     if q is not None and q_out is None and _ops.USE_TORCH_OPS:
-        outs = _lib.try_op("kv_append_", q, k, v, k_cache, v_cache, q_weight, k_weight, inv_freq,
-                           cu_seqlens_q, cu_seqlens_k, block_table, interleaved, _eps(eps))
+        outs = _lib.plain_call("kv_append", q, k, v, k_cache, v_cache, q_weight, k_weight,
+                               inv_freq, cu_seqlens_q, cu_seqlens_k, block_table, interleaved,
+                               _eps(eps))
         if outs is not None:
             return outs[0]
+    return _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlens_k, q,
+                           q_weight, k_weight, eps, inv_freq, interleaved, q_out)
+
+
+@torch.no_grad()
+def _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlens_k, q, q_weight,
+                    k_weight, eps, inv_freq, interleaved, q_out):
+    name = "kv_append"
     _check_rows(name, "k", k, None)
     _check_rows(name, "v", v, k, k.shape[1])
     device = k.device

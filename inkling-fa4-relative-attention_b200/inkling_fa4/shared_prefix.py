@@ -9,7 +9,6 @@ import torch
 from . import _lib, _ops
 
 
-@torch.no_grad()
 def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k,
                                                    max_seqlen_q, max_seqlen_k, rel_extent,
                                                    shared_prefix_len, window_size=(-1, -1),
@@ -37,16 +36,26 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
     ``chunk_len``: the plan of the own keys, as in the decode.  ``workspace``: a reusable uint8
     CUDA tensor (allocated per call when absent or too small); calls that may run at the same
     time need one each."""
-    name = "decode_shared_prefix"
     if (out is None and lse is None and not return_lse and n_heads is None and kv_heads is None
             and head_dim == _ops.HEAD_DIM and _ops.USE_TORCH_OPS):
-        outs = _lib.try_op("decode_shared_prefix", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k,
-                           block_table, workspace, rel_extent,
-                           -1 if window_size is None else window_size[0], max_seqlen_k or 0,
-                           1.0 / _ops.HEAD_DIM if softmax_scale is None else softmax_scale,
-                           num_splits, chunk_len, shared_prefix_len, prefix_splits)
+        outs = _lib.plain_call("decode_shared_prefix", q, k, v, rel_logits, cu_seqlens_q,
+                               cu_seqlens_k, block_table, workspace, rel_extent,
+                               -1 if window_size is None else window_size[0], max_seqlen_k or 0,
+                               1.0 / _ops.HEAD_DIM if softmax_scale is None else softmax_scale,
+                               num_splits, chunk_len, shared_prefix_len, prefix_splits)
         if outs is not None:
             return outs[0]
+    return _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_extent,
+                    shared_prefix_len, window_size, n_heads, kv_heads, head_dim, block_table,
+                    softmax_scale, out, prefix_splits, num_splits, chunk_len, workspace,
+                    return_lse, lse)
+
+
+@torch.no_grad()
+def _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_extent,
+             shared_prefix_len, window_size, n_heads, kv_heads, head_dim, block_table,
+             softmax_scale, out, prefix_splits, num_splits, chunk_len, workspace, return_lse, lse):
+    name = "decode_shared_prefix"
     if block_table is None:
         raise ValueError(f"{name}: needs a paged cache (block_table)")
     block_table = _ops._table(block_table)

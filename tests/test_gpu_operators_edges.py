@@ -3,6 +3,7 @@ keys, several calls at once, the debug build, autograd with leaves that an eager
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -164,6 +165,40 @@ def test_gradients_in_a_graph_beside_an_eager_graph_of_the_same_leaves():
     torch.cuda.synchronize()
     assert torch.equal(captured[0], dq) and torch.equal(captured[1], dk)
     assert torch.equal(captured[2] + captured[3], dw) and torch.equal(captured[4], dt)
+
+
+def test_plain_calls_hold_nothing_and_make_no_autograd_nodes():
+    """The calls that skip the Python checks: outputs need no gradient whatever the inputs do, no
+    reference or memory is left behind, and threads may call at the same time."""
+    q, k = _randn(40, 4, 128, seed=1).requires_grad_(), _randn(40, 2, 128, seed=2)
+    w = torch.nn.Parameter(torch.ones(128, device="cuda"))
+    table, starts = _randn(8, 4, seed=3), torch.arange(8, dtype=torch.int32, device="cuda")
+    inv = _inv()
+
+    def calls():
+        return (*_lib.plain_call("qk_norm_rope", q, k, w, w, inv, None, None, False, 1e-6),
+                *_lib.plain_call("bucket_bias", table, starts, 40, 16))
+
+    first = calls()
+    assert not any(t.requires_grad or t.grad_fn is not None for t in first)
+    assert first[2].shape == (40, 4, 16) and first[2].stride() == (0, 16, 1)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(first, calls()))
+    counts = [sys.getrefcount(t) for t in (q, k, w, inv, table, starts, None)]
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+
+    def many(_):
+        for _ in range(200):
+            got = calls()
+        return all(torch.equal(a, b) for a, b in zip(first, got))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(many, range(4)))
+    del pool
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == held
+    assert [sys.getrefcount(t) for t in (q, k, w, inv, table, starts, None)] == counts
 
 
 def run_debug_cases():

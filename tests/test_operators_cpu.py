@@ -283,9 +283,18 @@ def test_oracle_gradient_against_differences(rot, interleaved, eps):
             assert abs((loss(x, w + step) - loss(x, w - step)) / (2 * h) - dw[j]) < 1e-7
 
 
-def test_operator_schemas():
-    ops = _lib.torch_ops()
-    assert ops is not None, "libifa4_torch_ops.so not built"
-    for name in ("decode_shared_prefix", "qk_norm_rope", "qk_norm_rope_backward", "kv_append_",
-                 "bucket_bias", "bucket_bias_backward"):
-        assert str(getattr(ops, name).default._schema).startswith(f"inkling_fa4::{name}(")
+def test_plain_calls():
+    """Every Python call of the operator library is there; what is not its plain case (the wrong
+    number or types of arguments, tensors on the CPU) gives None, not an error."""
+    assert _lib.torch_ops() is not None, "libifa4_torch_ops.so not built"
+    x = torch.zeros(2, 2, 128, dtype=torch.bfloat16)
+    norm = (x, x, None, None, None, None, None, False, 1e-6)
+    calls = {"decode_shared_prefix": (), "qk_norm_rope": norm, "kv_append": (x,) * 15,
+             "qk_norm_rope_backward": (x, x, *norm, True, True),
+             "bucket_bias": (x[0], torch.zeros(2, dtype=torch.int32), 4, 16),
+             "bucket_bias_backward": (x, torch.zeros(2, dtype=torch.int32), True, None)}
+    for name, args in calls.items():
+        assert name in _lib._calls
+        for a in (args, (), args + (None,), args[:-1] + (object(),), (None,) * len(args),
+                  (1 << 70,) * len(args)):
+            assert _lib.plain_call(name, *a) is None, (name, a)
