@@ -956,9 +956,9 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
     // The split count with the least work on the busiest SM: waves of CTAs x (key tiles of a CTA
     // + about three tiles' worth of start and epilogue).  The own keys' kernel runs beside this
     // one on the SMs it leaves: when its CTAs (two per SM) fit half of the GPU, that many SMs are
-    // left (33 sequences, 10k prefix: 27 us with 80 of these CTAs and 132 of those, 34 us with
-    // 108; 8 sequences, 2k: 16.4 us with 88, 17.3 us with 128); a larger one comes after it
-    // (128 sequences, 32k: 126 us with 144 CTAs, 138 us with 112).
+    // left (33 sequences, 10k prefix: 26.6 us with 80 of these CTAs and 132 of those, 33.9 us with
+    // 108; 8 sequences, 2k: 14.4 us with 64, 16.4 us with 128); a larger one comes after it
+    // (128 sequences, 32k: 122 us with 144 CTAs, 134 us with 112).
     const int64_t hpc = group < 16 ? group : 16;
     const int64_t own_ctas = static_cast<int64_t>(d->batch) * d->kv_heads *
                              ((group + hpc - 1) / hpc) * plan->own_splits;

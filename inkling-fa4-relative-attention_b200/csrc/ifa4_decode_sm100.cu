@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = g + 8 * r;
+      if (row >= nh) break;
       if (qd == 0) {
         mm[warp * 16 + row] = m_r[r];
         ml[warp * 16 + row] = l_r[r];
