@@ -40,6 +40,7 @@ namespace decode {
 
 constexpr int kTileKeys = 64;
 constexpr int kStages = 3;
+constexpr int kPxDepth = 16;  // partials of a shared prefix that a warp fetches at a time
 constexpr int kConsumerWarps = 4;
 constexpr int kThreads = (kConsumerWarps + 1) * 32;
 constexpr uint32_t kHalf = kTileKeys * 128;             // 64 rows x 128 B
@@ -431,35 +432,46 @@ __global__ void __launch_bounds__(kThreads, 2)
           acc.w += o4.w * f;
         }
       }
+      // The prefix's partials, kPxDepth at a time: their sums and outputs are fetched together (an
+      // output without weight may never have been written: it is not used), then the running
+      // maximum and the sums take them in.
       auto larger = [](float x, float y) { return y > x || y != y ? y : x; };  // a NaN wins
       float m = M;
-      for (int i = lane; i < a.px_parts; i += 32) m = larger(m, a.px_lse[i * rows + at]);
+      const float* lse = a.px_lse + at;
+      const float4* po = reinterpret_cast<const float4*>(a.px_o + at * 128) + lane;
+#pragma unroll 1
+      for (int i0 = 0; i0 < a.px_parts; i0 += kPxDepth) {
+        float l[kPxDepth];
+        float4 o4[kPxDepth];
 #pragma unroll
-      for (int k = 16; k > 0; k >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, k));
-      if (m != -INFINITY) {
-        const float own = M == -INFINITY ? 0.f : fast_exp2(M - m);
-        L *= own;
-        acc.x *= own;
-        acc.y *= own;
-        acc.z *= own;
-        acc.w *= own;
-        for (int i0 = 0; i0 < a.px_parts; i0 += 8) {
-          float wt[8];
-          float4 o4[8];
+        for (int k = 0; k < kPxDepth; ++k) {
+          const int i = min(i0 + k, a.px_parts - 1);
+          l[k] = lse[i * rows];
+          o4[k] = po[i * rows * 32];
+        }
+        float mn = m;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            wt[k] = i0 + k < a.px_parts ? fast_exp2(a.px_lse[(i0 + k) * rows + at] - m) : 0.f;
-            o4[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (wt[k] != 0.f)  // no weight: its output may never have been written
-              o4[k] = reinterpret_cast<const float4*>(a.px_o + ((i0 + k) * rows + at) * 128)[lane];
-          }
+        for (int k = 0; k < kPxDepth; ++k) {
+          if (i0 + k >= a.px_parts) l[k] = -INFINITY;
+          mn = larger(mn, l[k]);
+        }
+        if (mn == -INFINITY) continue;
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+        m = mn;
+        L *= f;
+        acc.x *= f;
+        acc.y *= f;
+        acc.z *= f;
+        acc.w *= f;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            L += wt[k];
-            acc.x += wt[k] * o4[k].x;
-            acc.y += wt[k] * o4[k].y;
-            acc.z += wt[k] * o4[k].z;
-            acc.w += wt[k] * o4[k].w;
+        for (int k = 0; k < kPxDepth; ++k) {
+          const float wt = fast_exp2(l[k] - m);
+          L += wt;
+          if (wt != 0.f) {
+            acc.x += wt * o4[k].x;
+            acc.y += wt * o4[k].y;
+            acc.z += wt * o4[k].z;
+            acc.w += wt * o4[k].w;
           }
         }
       }
