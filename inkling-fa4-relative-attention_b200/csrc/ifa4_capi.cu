@@ -2,6 +2,7 @@
 // launch planning, error reporting.  Declared in include/inkling_fa4.h.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -900,6 +901,48 @@ struct SharedPrefixPlan {
   size_t bytes;           // workspace
 };
 
+// Estimated times (tenths of a microsecond) that choose the splits, fitted to sweeps over 2 to 256
+// sequences, 512 to 32k prefix keys and 100 to 2000 own ones.  A CTA of the prefix kernel: a start and
+// an end of 5 us; its first tiles arrive together (up to the three stages of its ring), the others
+// take 1.3 us each.  A CTA of the own keys' kernel: 4 us and 0.95 us for 64 keys.
+struct SharedPrefixShape {
+  int sms, ctas;       // CTAs of the prefix kernel for one split
+  int key_tiles;       // prefix tiles of 128 keys
+  int own_ctas;        // CTAs of the own keys' kernel for one split
+  int own_tiles;       // tiles of 64 keys of the longest own part
+};
+int prefix_cta_time(int tiles) {
+  return 50 + (tiles == 1 ? 13 : tiles <= 3 ? 32 : 13 * tiles + 13);
+}
+// The prefix splits with the least estimate for own keys in `own_splits` parts, and that estimate.
+// The own keys' kernel runs beside the prefix kernel on the SMs it leaves: when its CTAs (two per SM)
+// fit half of the GPU, that many SMs are left (33 sequences, 10k prefix: 20.4 us with 80 of these
+// CTAs, 26 us with 108); a larger one comes after it (128 sequences, 32k: 119 us with 144 CTAs,
+// 130 us with 112).  Every split adds 0.3 us to the merge in the own keys' kernel (3 sequences with
+// one KV head, 32k: 32.5 us with 64 splits, 28.8 us with 37), little to that of a kernel of its own
+// (21.3 us with 64, 23.0 us with 43).
+int best_prefix_splits(const SharedPrefixShape& x, int own_splits, int* estimate) {
+  const int own = x.own_ctas * own_splits;
+  const int room = own <= x.sms ? x.sms - (own + 1) / 2 : x.sms;
+  const int own_time = (95 * ((x.own_tiles + own_splits - 1) / own_splits) + 400) / 10;
+  int splits = 1, best = INT_MAX;
+  for (int s = x.key_tiles < 64 ? x.key_tiles : 64; s >= 1; --s) {
+    const int per = (x.key_tiles + s - 1) / s;
+    s = (x.key_tiles + per - 1) / per;  // the fewest splits of this length
+    const int total = x.ctas * s;
+    const int time = (total + room - 1) / room * prefix_cta_time(per) +
+                     (own_splits == 1 ? 3 * s : s / 2);
+    if (time >= best) continue;
+    best = time;
+    splits = s;
+    const int beside = total < x.sms ? 2 * (x.sms - total) : 0;
+    const int later = own > beside ? (own - beside + 2 * x.sms - 1) / (2 * x.sms) : 0;
+    *estimate = later > 0 ? time + later * own_time * 13 / 10  // two CTAs on every SM
+                          : (time > own_time ? time : own_time);
+  }
+  return splits;
+}
+
 int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) {
   const char* what = "decode_shared_prefix";
   if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
@@ -929,12 +972,37 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
   if (p->shared_prefix_len > 0 && d->max_seqlen_k > 0)
     plan->own.max_seqlen_k = d->max_seqlen_k > p->shared_prefix_len
                                  ? d->max_seqlen_k - p->shared_prefix_len : 1;
-  // Few own keys: one split, whose CTA merges the prefix's partials itself (8 sequences with up to
-  // 128 own keys behind 2k: 14.2 us, 16.4 us with two splits and a merge kernel).
+  SharedPrefixShape x{};
+  if (p->shared_prefix_len > 0) {
+    plan->seqs_per_tile = 128 / group;
+    const int tiles = (d->batch + plan->seqs_per_tile - 1) / plan->seqs_per_tile;
+    plan->key_pair = tiles == 1;
+    x.ctas = d->kv_heads * ((tiles + 1) / 2);
+    int64_t span = p->shared_prefix_len;
+    if (d->window_left >= 0 && d->window_left + 128LL < span) span = d->window_left + 128LL;
+    x.key_tiles = static_cast<int>((span + 127) / 128);
+    const int hpc = group < 16 ? group : 16;
+    x.own_ctas = d->batch * d->kv_heads * ((group + hpc - 1) / hpc);
+  }
+  // Up to 2048 own keys: one split, whose CTA merges the prefix's partials itself, or several and a
+  // kernel that merges (4 us), whichever is estimated faster (8 sequences, 32k prefix, 1000 own keys:
+  // 47 us with one, 61 us with two; 3 with one KV head: 29 us and 21 us).
+  int estimate = 0;
   if (p->shared_prefix_len > 0 && d->num_splits == 0 && d->chunk_len == 0 && d->max_seqlen_k > 0 &&
-      plan->own.max_seqlen_k <= 512) {
-    plan->own.num_splits = 1;
-    plan->own.chunk_len = (plan->own.max_seqlen_k + 63) / 64 * 64;
+      plan->own.max_seqlen_k <= 2048) {
+    if ((rc = sm_count(&x.sms))) return rc;
+    x.own_tiles = (plan->own.max_seqlen_k + 63) / 64;
+    int best = INT_MAX;
+    for (int n : {1, 2, 3, 4, 6, 8}) {
+      if (n > 1 && (n * 2 > x.own_tiles || static_cast<int64_t>(n) * x.own_ctas > 2 * x.sms)) break;
+      best_prefix_splits(x, n, &estimate);
+      if (n > 1) estimate += 40;
+      if (estimate < best) {
+        best = estimate;
+        plan->own.num_splits = n;
+      }
+    }
+    plan->own.chunk_len = (x.own_tiles + plan->own.num_splits - 1) / plan->own.num_splits * 64;
   }
   size_t own_bytes = 0;
   if ((rc = decode_plan(&plan->own, &plan->own_splits, &plan->chunk, &own_bytes))) return rc;
@@ -942,37 +1010,10 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
     plan->bytes = own_bytes;
     return IFA4_OK;
   }
-  plan->seqs_per_tile = 128 / group;
-  const int tiles = (d->batch + plan->seqs_per_tile - 1) / plan->seqs_per_tile;
-  plan->key_pair = tiles == 1;
-  int sms = 148;
-  if ((rc = sm_count(&sms))) return rc;
-  const int64_t ctas = static_cast<int64_t>(d->kv_heads) * ((tiles + 1) / 2);
-  int64_t span = p->shared_prefix_len;
-  if (d->window_left >= 0 && d->window_left + 128LL < span) span = d->window_left + 128LL;
-  const int64_t key_tiles = (span + 127) / 128;
   int splits = p->prefix_splits;
   if (splits == 0) {
-    // The split count with the least work on the busiest SM: waves of CTAs x (key tiles of a CTA
-    // + about three tiles' worth of start and epilogue).  The own keys' kernel runs beside this
-    // one on the SMs it leaves: when its CTAs (two per SM) fit half of the GPU, that many SMs are
-    // left (33 sequences, 10k prefix: 26.6 us with 80 of these CTAs and 132 of those, 33.9 us with
-    // 108; 8 sequences, 2k: 14.4 us with 64, 16.4 us with 128); a larger one comes after it
-    // (128 sequences, 32k: 122 us with 144 CTAs, 134 us with 112).
-    const int64_t hpc = group < 16 ? group : 16;
-    const int64_t own_ctas = static_cast<int64_t>(d->batch) * d->kv_heads *
-                             ((group + hpc - 1) / hpc) * plan->own_splits;
-    const int64_t room = own_ctas <= sms ? sms - (own_ctas + 1) / 2 : sms;
-    int64_t best = INT64_MAX;
-    const int64_t most = key_tiles < 64 ? key_tiles : 64;
-    for (int64_t s = 1; s <= most; ++s) {
-      const int64_t waves = (ctas * s + room - 1) / room;
-      const int64_t cost = waves * ((key_tiles + s - 1) / s + 3);
-      if (cost < best) {
-        best = cost;
-        splits = static_cast<int>(s);
-      }
-    }
+    if ((rc = sm_count(&x.sms))) return rc;
+    splits = best_prefix_splits(x, plan->own_splits, &estimate);
   }
   plan->splits = splits;
   plan->parts = plan->key_pair ? 2 * splits : splits;
