@@ -916,11 +916,10 @@ int prefix_cta_time(int tiles) {
 }
 // The prefix splits with the least estimate for own keys in `own_splits` parts, and that estimate.
 // The own keys' kernel runs beside the prefix kernel on the SMs it leaves: when its CTAs (two per SM)
-// fit half of the GPU, that many SMs are left (33 sequences, 10k prefix: 20.4 us with 80 of these
-// CTAs, 26 us with 108); a larger one comes after it (128 sequences, 32k: 119 us with 144 CTAs,
-// 130 us with 112).  Every split adds 0.3 us to the merge in the own keys' kernel (3 sequences with
-// one KV head, 32k: 32.5 us with 64 splits, 28.8 us with 37), little to that of a kernel of its own
-// (21.3 us with 64, 23.0 us with 43).
+// fit half of the GPU, that many SMs are left (33 sequences, 10k prefix: 23.7 us with 80 of these
+// CTAs, 30.7 us with 108); a larger one comes after it (128 sequences, 32k: 120 us with 144 CTAs,
+// 132 us with 112).  Every split adds 0.3 us to the merge in the own keys' kernel (3 sequences with
+// one KV head, 32k: 32.5 us with 64 splits, 28.8 us with 37), little to that of a kernel of its own.
 int best_prefix_splits(const SharedPrefixShape& x, int own_splits, int* estimate) {
   const int own = x.own_ctas * own_splits;
   const int room = own <= x.sms ? x.sms - (own + 1) / 2 : x.sms;
@@ -985,8 +984,8 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
     x.own_ctas = d->batch * d->kv_heads * ((group + hpc - 1) / hpc);
   }
   // Up to 2048 own keys: one split, whose CTA merges the prefix's partials itself, or several and a
-  // kernel that merges (4 us), whichever is estimated faster (8 sequences, 32k prefix, 1000 own keys:
-  // 47 us with one, 61 us with two; 3 with one KV head: 29 us and 21 us).
+  // kernel that merges (4 us), whichever is estimated faster (3 sequences with one KV head, 32k
+  // prefix, 1000 own keys: 29 us with one, 20 us with two; 64, GQA 8/2, 4k and 1500: 27.3 and 28.2).
   int estimate = 0;
   if (p->shared_prefix_len > 0 && d->num_splits == 0 && d->chunk_len == 0 && d->max_seqlen_k > 0 &&
       plan->own.max_seqlen_k <= 2048) {

@@ -593,16 +593,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merge of a row's partials (a.parts of the prefix, a.own_parts of its own keys): weights
-// 2^(lse_i - max lse).  kWarps warps share a row's partials, four in flight each; lanes own 4 of the
-// 128 dims, and the warps' sums meet in shared memory.  One warp walking all partials of a row
-// took 20 us for 75 of them (33 sequences x 12 heads), four 5.8 us; with 10 of them (128 x 32
-// rows) one warp takes 6.4 us and four 8.2 us.
+// 2^(lse_i - max lse).  kWarps warps share a row's partials, eight in flight each; lanes own 4 of the
+// 128 dims, and the warps' sums meet in shared memory.  With four in flight, weights first, one warp
+// walking all partials of a row took 20 us for 75 of them (33 sequences x 12 heads) and four 5.8 us;
+// with 10 of them (128 x 32 rows) one warp took 6.4 us and four 8.2 us; eight in one pass save 1 to
+// 2 us of the whole call (3 sequences behind 32k: 21.4 -> 19.9 us).
 constexpr int kCombineThreads = 128;
 template <int kWarps>
 __global__ void __launch_bounds__(kCombineThreads)
     shared_prefix_combine_kernel(const __grid_constant__ SharedPrefixKernelArgs a) {
   __shared__ __align__(16) float4 sums[kCombineThreads / 32][32];
-  __shared__ float weights[kCombineThreads / 32];
+  __shared__ float weights[kCombineThreads / 32], maxima[kCombineThreads / 32];
   const int warp = (threadIdx.x >> 5) % kWarps, lane = threadIdx.x & 31;
   const long long row = static_cast<long long>(blockIdx.x) * (kCombineThreads / 32 / kWarps) +
                         (threadIdx.x >> 5) / kWarps;
@@ -612,55 +613,78 @@ __global__ void __launch_bounds__(kCombineThreads)
   const int h = static_cast<int>(row - static_cast<long long>(b) * a.n_heads);
   const int n = a.parts + a.own_parts;
   wait_previous_kernel();  // both kernels' partials (the own keys' ends after the prefix's)
-  // partial i: the prefix's first, then the own keys'
-  auto lse_of = [&](int i) {
-    return i < a.parts ? a.ws_lse[i * rows + row] : a.own_lse[row * a.own_parts + (i - a.parts)];
-  };
+  // Partial i: the prefix's first, then the own keys'.  A warp takes kDepth at a time: sums and
+  // outputs are fetched together (an output without weight may never have been written: it is not
+  // used), then the running maximum and the sums take them in.
+  constexpr int kDepth = 8;
   auto larger = [](float x, float y) { return y > x || y != y ? y : x; };  // a NaN wins
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 32) m = larger(m, lse_of(i));
-#pragma unroll
-  for (int k = 16; k > 0; k >>= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, k));
-  float wsum = 0.f;
+  float m = -INFINITY, wsum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (m != -INFINITY) {
-    for (int i0 = warp; i0 < n; i0 += 4 * kWarps) {
-      float wt[4];
-      float4 o[4];
+  auto rescale = [&](float to) {  // to: the new maximum, not -inf
+    const float f = m == -INFINITY ? 0.f : fast_exp2(m - to);
+    m = to;
+    wsum *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+  };
+#pragma unroll 1
+  for (int i0 = warp * kDepth; i0 < n; i0 += kWarps * kDepth) {
+    float l[kDepth];
+    float4 o[kDepth];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int p = i0 + k * kWarps;
-        wt[k] = p < n ? fast_exp2(lse_of(p) - m) : 0.f;
-        o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (wt[k] != 0.f) {  // no weight: its output may never have been written
-          const float* src = p < a.parts ? a.ws_o + (p * rows + row) * 128
-                                         : a.own_o + (row * a.own_parts + (p - a.parts)) * 128;
-          o[k] = reinterpret_cast<const float4*>(src)[lane];
-        }
-      }
+    for (int k = 0; k < kDepth; ++k) {
+      const int i = min(i0 + k, n - 1);
+      const bool of_prefix = i < a.parts;
+      const long long own = row * a.own_parts + (i - a.parts);
+      l[k] = of_prefix ? a.ws_lse[i * rows + row] : a.own_lse[own];
+      o[k] = reinterpret_cast<const float4*>(of_prefix ? a.ws_o + (i * rows + row) * 128
+                                                       : a.own_o + own * 128)[lane];
+    }
+    float mn = m;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        wsum += wt[k];
-        acc.x += wt[k] * o[k].x;
-        acc.y += wt[k] * o[k].y;
-        acc.z += wt[k] * o[k].z;
-        acc.w += wt[k] * o[k].w;
+    for (int k = 0; k < kDepth; ++k) {
+      if (i0 + k >= n) l[k] = -INFINITY;
+      mn = larger(mn, l[k]);
+    }
+    if (mn == -INFINITY) continue;
+    rescale(mn);
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      const float wt = fast_exp2(l[k] - m);
+      wsum += wt;
+      if (wt != 0.f) {
+        acc.x += wt * o[k].x;
+        acc.y += wt * o[k].y;
+        acc.z += wt * o[k].z;
+        acc.w += wt * o[k].w;
       }
     }
   }
   if (kWarps > 1) {
     sums[warp][lane] = acc;
-    if (lane == 0) weights[warp] = wsum;
+    if (lane == 0) {
+      weights[warp] = wsum;
+      maxima[warp] = m;
+    }
     __syncthreads();
     if (warp != 0) return;
+    float mn = m;
 #pragma unroll
-    for (int k = 1; k < kWarps; ++k) {
-      const float4 o = sums[k][lane];
-      acc.x += o.x;
-      acc.y += o.y;
-      acc.z += o.z;
-      acc.w += o.w;
-      wsum += weights[k];
+    for (int k = 1; k < kWarps; ++k) mn = larger(mn, maxima[k]);
+    if (mn != -INFINITY) {
+      rescale(mn);
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) {
+        const float f = maxima[k] == -INFINITY ? 0.f : fast_exp2(maxima[k] - m);
+        const float4 o = sums[k][lane];
+        acc.x += f * o.x;
+        acc.y += f * o.y;
+        acc.z += f * o.z;
+        acc.w += f * o.w;
+        wsum += f * weights[k];
+      }
     }
   }
   const float inv = wsum > 0.f ? 1.f / wsum : (wsum == 0.f ? 0.f : wsum);  // NaN stays
