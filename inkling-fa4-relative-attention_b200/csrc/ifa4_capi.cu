@@ -2,7 +2,6 @@
 // launch planning, error reporting.  Declared in include/inkling_fa4.h.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <limits.h>
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
@@ -906,12 +905,13 @@ struct SharedPrefixPlan {
 // an end of 5 us; its first tiles arrive together (up to the three stages of its ring), the others
 // take 1.3 us each.  A CTA of the own keys' kernel: 4 us and 0.95 us for 64 keys.
 struct SharedPrefixShape {
-  int sms, ctas;       // CTAs of the prefix kernel for one split
-  int key_tiles;       // prefix tiles of 128 keys
-  int own_ctas;        // CTAs of the own keys' kernel for one split
-  int own_tiles;       // tiles of 64 keys of the longest own part
+  int sms;
+  int key_tiles;     // prefix tiles of 128 keys
+  int own_tiles;     // tiles of 64 keys of the longest own part
+  int64_t ctas;      // CTAs of the prefix kernel for one split
+  int64_t own_ctas;  // CTAs of the own keys' kernel for one split
 };
-int prefix_cta_time(int tiles) {
+int64_t prefix_cta_time(int64_t tiles) {
   return 50 + (tiles == 1 ? 13 : tiles <= 3 ? 32 : 13 * tiles + 13);
 }
 // The prefix splits with the least estimate for own keys in `own_splits` parts, and that estimate.
@@ -920,22 +920,23 @@ int prefix_cta_time(int tiles) {
 // CTAs, 30.7 us with 108); a larger one comes after it (128 sequences, 32k: 120 us with 144 CTAs,
 // 132 us with 112).  Every split adds 0.3 us to the merge in the own keys' kernel (3 sequences with
 // one KV head, 32k: 32.5 us with 64 splits, 28.8 us with 37), little to that of a kernel of its own.
-int best_prefix_splits(const SharedPrefixShape& x, int own_splits, int* estimate) {
-  const int own = x.own_ctas * own_splits;
-  const int room = own <= x.sms ? x.sms - (own + 1) / 2 : x.sms;
-  const int own_time = (95 * ((x.own_tiles + own_splits - 1) / own_splits) + 400) / 10;
-  int splits = 1, best = INT_MAX;
+int best_prefix_splits(const SharedPrefixShape& x, int own_splits, int64_t* estimate) {
+  const int64_t own = x.own_ctas * own_splits;
+  const int64_t room = own <= x.sms ? x.sms - (own + 1) / 2 : x.sms;
+  const int64_t own_time = (95LL * ((x.own_tiles + own_splits - 1) / own_splits) + 400) / 10;
+  int splits = 1;
+  int64_t best = INT64_MAX;
   for (int s = x.key_tiles < 64 ? x.key_tiles : 64; s >= 1; --s) {
     const int per = (x.key_tiles + s - 1) / s;
     s = (x.key_tiles + per - 1) / per;  // the fewest splits of this length
-    const int total = x.ctas * s;
-    const int time = (total + room - 1) / room * prefix_cta_time(per) +
-                     (own_splits == 1 ? 3 * s : s / 2);
+    const int64_t total = x.ctas * s;
+    const int64_t time = (total + room - 1) / room * prefix_cta_time(per) +
+                         (own_splits == 1 ? 3 * s : s / 2);
     if (time >= best) continue;
     best = time;
     splits = s;
-    const int beside = total < x.sms ? 2 * (x.sms - total) : 0;
-    const int later = own > beside ? (own - beside + 2 * x.sms - 1) / (2 * x.sms) : 0;
+    const int64_t beside = total < x.sms ? 2 * (x.sms - total) : 0;
+    const int64_t later = own > beside ? (own - beside + 2 * x.sms - 1) / (2 * x.sms) : 0;
     *estimate = later > 0 ? time + later * own_time * 13 / 10  // two CTAs on every SM
                           : (time > own_time ? time : own_time);
   }
@@ -976,24 +977,24 @@ int shared_prefix_plan(const IFA4SharedPrefixParams* p, SharedPrefixPlan* plan) 
     plan->seqs_per_tile = 128 / group;
     const int tiles = (d->batch + plan->seqs_per_tile - 1) / plan->seqs_per_tile;
     plan->key_pair = tiles == 1;
-    x.ctas = d->kv_heads * ((tiles + 1) / 2);
+    x.ctas = static_cast<int64_t>(d->kv_heads) * ((tiles + 1) / 2);
     int64_t span = p->shared_prefix_len;
     if (d->window_left >= 0 && d->window_left + 128LL < span) span = d->window_left + 128LL;
     x.key_tiles = static_cast<int>((span + 127) / 128);
     const int hpc = group < 16 ? group : 16;
-    x.own_ctas = d->batch * d->kv_heads * ((group + hpc - 1) / hpc);
+    x.own_ctas = static_cast<int64_t>(d->batch) * d->kv_heads * ((group + hpc - 1) / hpc);
   }
   // Up to 2048 own keys: one split, whose CTA merges the prefix's partials itself, or several and a
   // kernel that merges (4 us), whichever is estimated faster (3 sequences with one KV head, 32k
   // prefix, 1000 own keys: 29 us with one, 20 us with two; 64, GQA 8/2, 4k and 1500: 27.3 and 28.2).
-  int estimate = 0;
+  int64_t estimate = 0;
   if (p->shared_prefix_len > 0 && d->num_splits == 0 && d->chunk_len == 0 && d->max_seqlen_k > 0 &&
       plan->own.max_seqlen_k <= 2048) {
     if ((rc = sm_count(&x.sms))) return rc;
     x.own_tiles = (plan->own.max_seqlen_k + 63) / 64;
-    int best = INT_MAX;
+    int64_t best = INT64_MAX;
     for (int n : {1, 2, 3, 4, 6, 8}) {
-      if (n > 1 && (n * 2 > x.own_tiles || static_cast<int64_t>(n) * x.own_ctas > 2 * x.sms)) break;
+      if (n > 1 && (n * 2 > x.own_tiles || n * x.own_ctas > 2 * x.sms)) break;
       best_prefix_splits(x, n, &estimate);
       if (n > 1) estimate += 40;
       if (estimate < best) {
