@@ -116,6 +116,9 @@ CASES = [  # prefix, own, heads, kv, rel_extent, page, window
     (1500, [600, 700], 8, 2, 64, 32, 500),                     # window: no row sees the prefix
     (200, [2, 2, 2], 48, 1, 64, 16, -1),                       # group of 48: two sequences a tile
     (200, [2, 30, 2], 128, 1, 64, 16, -1),                     # group of 128
+    (260, [2000, 1, 700], 8, 2, 128, 16, -1),                  # long own keys: split, then merged
+    (4000, [0, 1100], 4, 1, 64, 64, -1),                       # more than 32 partials a row
+    (3000, [5, 40] * 8, 8, 1, 64, 16, -1),                     # the same, merged in the decode
 ]
 
 
