@@ -335,7 +335,8 @@ int ifa4_rel_logits_launch(const IFA4RelLogitsParams* params, void* stream);
  * worked on together); shorter ones are attended whole through their own table rows.  A value that
  * is no number reaches every sequence that is worked on with one that sees it.
  * decode.num_splits / chunk_len plan the keys behind the prefix; decode.max_seqlen_k is the
- * longest whole sequence, prefix included.  Deterministic: no atomics on results. */
+ * longest whole sequence, prefix included.  The workspace must be 16-byte aligned (32-byte aligned
+ * ones are written in whole sectors).  Deterministic: no atomics on results. */
 typedef struct IFA4SharedPrefixParams {
   IFA4DecodeParams decode;
   int32_t shared_prefix_len;  /* 0 to 2^30; 0 is a plain decode                            */

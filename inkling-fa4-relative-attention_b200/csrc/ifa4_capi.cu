@@ -1082,6 +1082,7 @@ int ifa4_decode_shared_prefix_launch(const IFA4SharedPrefixParams* p, void* work
   a.v_sp = d->v_stride_page;
   float* ws = static_cast<float*>(workspace);
   a.ws_o = ws;
+  a.ws_sectors = reinterpret_cast<uintptr_t>(workspace) % 32 == 0;
   const int own_parts = plan.own_splits > 1 ? plan.own_splits : 0;
   float* own_o = ws + rows * plan.parts * 128;
   a.ws_lse = own_o + rows * own_parts * 128;

@@ -189,7 +189,8 @@ struct SharedPrefixKernelArgs {
   int page_shift, box_shift, num_pages;
   const uint16_t* v;         // V cache base (the unit in which the prefix ends)
   long long v_st, v_sh, v_sp;
-  float* ws_o;               // [parts, batch, n_heads, 128]
+  float* ws_o;               // [parts, batch, n_heads, 128], 16-byte aligned
+  int ws_sectors;            // ws_o is 32-byte aligned
   float* ws_lse;             // [parts, batch, n_heads], log2 units, -inf: no visible key
   const float* own_o;        // [batch, n_heads, own_parts, 128]
   const float* own_lse;      // [batch, n_heads, own_parts]

@@ -112,6 +112,20 @@ __device__ __forceinline__ void issue_pv(uint32_t tmem_o, uint32_t tmem_p, uint3
             (kk > 0 || accumulate) ? 1u : 0u);
 }
 
+// Eight fp32 values of a row of partials, whose offsets in the workspace are multiples of 32 bytes:
+// one 32-byte store where the workspace itself starts on such a boundary (`sectors`), two 16-byte
+// ones where it is only 16-byte aligned, as the C ABI allows.
+__device__ __forceinline__ void store_sector(float* dst, const float (&f)[8], bool sectors) {
+  if (sectors) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "f"(f[0]), "f"(f[1]),
+                 "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  }
+}
+
 // Row r of row tile `tile`: its sequence and head, and whether it takes part.
 struct Row {
   int b, h, len;
@@ -572,10 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float f[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[8 * v + i]) * inv_l;
-              asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c * 32 + 8 * v),
-                           "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]),
-                           "f"(f[6]), "f"(f[7])
-                           : "memory");
+              store_sector(dst + c * 32 + 8 * v, f, a.ws_sectors);
             }
           }
           __syncwarp();
