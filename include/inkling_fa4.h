@@ -333,7 +333,9 @@ int ifa4_rel_logits_launch(const IFA4RelLogitsParams* params, void* stream);
  * keys and values there, as far as their windows reach (normally the same pages; the pages are
  * taken from the table row of the one whose window reaches furthest back among those that are
  * worked on together); shorter ones are attended whole through their own table rows.  A value that
- * is no number reaches every sequence that is worked on with one that sees it.
+ * is no number reaches every sequence that is worked on with one that sees it.  A logit that is no
+ * number, or +inf, makes its row NaN (ifa4_decode_launch, and a prefix of 0, leave the keys that it
+ * was added up with out of the row).
  * decode.num_splits / chunk_len plan the keys behind the prefix; decode.max_seqlen_k is the
  * longest whole sequence, prefix included.  The workspace must be 16-byte aligned (32-byte aligned
  * ones are written in whole sectors).  Deterministic: no atomics on results. */

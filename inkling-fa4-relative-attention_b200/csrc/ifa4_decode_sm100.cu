@@ -433,6 +433,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           acc.z += o4.z * f;
           acc.w += o4.w * f;
         }
+      } else {  // no score above -inf: every sum is 0, or NaN where a score was one
+#pragma unroll
+        for (int w = 0; w < kConsumerWarps; ++w) L += ml[w * 16 + row];
       }
       // The prefix's partials, kPxDepth at a time: their sums and outputs are fetched together (an
       // output without weight may never have been written: it is not used), then the running
@@ -506,9 +509,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           L += ml[w * 16 + row] * f;
           acc += mo[(w * 16 + row) * 128 + d] * f;
         }
+      } else if (a.prefix_len > 0) {  // as above: 0 or NaN
+#pragma unroll
+        for (int w = 0; w < kConsumerWarps; ++w) L += ml[w * 16 + row];
       }
       const int h = h0 + row;
-      const float val = L > 0.f ? acc / L : 0.f;
+      // Behind a shared prefix a NaN sum stays one and reaches the merge; without one such a row is
+      // stored as a row without keys (0 and -inf).
+      const bool none = a.prefix_len > 0 ? L == 0.f : !(L > 0.f);
+      const float val = none ? 0.f : acc / L;
       if (!IFA4_DBG_CHECK(a.status, si.q_row >= 0 && si.q_row < a.batch && h < a.n_heads)) {
         // a bad query row or head: nothing is stored
       } else if (a.ws_o == nullptr) {
@@ -518,11 +527,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         *dst = *reinterpret_cast<uint16_t*>(&bv);
         if (d == 0 && a.lse != nullptr)
           a.lse[static_cast<long long>(h) * a.lse_sh + static_cast<long long>(si.q_row) * a.lse_st] =
-              L > 0.f ? (M + __log2f(L)) * 0.6931471805599453f : -INFINITY;
+              none ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
       } else {
         const long long idx = (static_cast<long long>(b) * a.n_heads + h) * gridDim.x + split;
         a.ws_o[idx * 128 + d] = val;
-        if (d == 0) a.ws_lse[idx] = L > 0.f ? M + __log2f(L) : -INFINITY;
+        if (d == 0) a.ws_lse[idx] = none ? -INFINITY : M + __log2f(L);
       }
     }
   }
