@@ -201,6 +201,12 @@ def _prepare(name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, causal, window_s
     return q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale
 
 
+def _offsets(cu):
+    """Sequence offsets as the kernels read them: one int32 behind the other (a column of a wider
+    tensor is copied; anything that is no tensor is left to the checks)."""
+    return cu.contiguous() if isinstance(cu, torch.Tensor) else cu
+
+
 def _table(block_table):
     """Unit last stride, and never a NULL pointer (NULL means "not paged" in the C ABI): an empty
     table becomes one column of -1 entries, which read as zero keys."""
@@ -225,6 +231,7 @@ def prefill(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_s
     the launch is too small to fill the GPU (the partials go to ``workspace``, allocated here if
     not given or too small); 1 never splits; > 1 forces that many splits."""
     block_table = _table(block_table)
+    cu_seqlens_q, cu_seqlens_k = _offsets(cu_seqlens_q), _offsets(cu_seqlens_k)
     q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale = _prepare(
         "prefill", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, rel_extent, causal,
         window_size, n_heads, kv_heads, head_dim, softmax_scale, causal_align, out, block_table)
@@ -303,6 +310,7 @@ def decode(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_se
            num_splits=0, chunk_len=0, workspace=None, return_lse=False, lse=None,
            block_table=None):
     block_table = _table(block_table)
+    cu_seqlens_q, cu_seqlens_k = _offsets(cu_seqlens_q), _offsets(cu_seqlens_k)
     q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale = _prepare(
         "decode", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, rel_extent, causal,
         window_size, n_heads, kv_heads, head_dim, softmax_scale, causal_align, out, block_table)

@@ -22,6 +22,7 @@ def inkling_fa4_rel_attention_backward(dout, q, k, v, rel_logits, out, lse, cu_s
     ``lse`` ([n_heads, total_q] fp32, from ``return_lse=True``).  dq / dk / dv are bf16 like
     q / k / v; drel has rel_logits' shape (bf16), zero outside the band of distances
     [0, rel_extent) that reach a visible key."""
+    cu_seqlens_q, cu_seqlens_k = _ops._offsets(cu_seqlens_q), _ops._offsets(cu_seqlens_k)
     q, k, v, rel, out_, n_heads, kv_heads, rel_extent, window_left, scale = _ops._prepare(
         "backward", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, rel_extent, causal,
         window_size, n_heads, kv_heads, head_dim, softmax_scale, causal_align, out)

@@ -61,6 +61,7 @@ def _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_
     if block_table is None:
         raise ValueError(f"{name}: needs a paged cache (block_table)")
     block_table = _ops._table(block_table)
+    cu_seqlens_q, cu_seqlens_k = _ops._offsets(cu_seqlens_q), _ops._offsets(cu_seqlens_k)
     q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale = _ops._prepare(
         name, q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, rel_extent, True, window_size,
         n_heads, kv_heads, head_dim, softmax_scale, "bottom_right", out, block_table)
