@@ -7,6 +7,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -199,6 +200,19 @@ def _prepare(name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, causal, window_s
     if not scale > 0:
         raise ValueError(f"{name}: softmax_scale must be > 0")
     return q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale
+
+
+def differentiates(*tensors):
+    """Whether a call with these inputs has to go through its autograd function: one of them needs a
+    gradient, or forward-mode differentiation is on (a dual tensor needs none; the function refuses
+    it, where a plain call would return an output without the tangent)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and getattr(t, "requires_grad", False):
+                return True
+    return False
 
 
 def _offsets(cu):

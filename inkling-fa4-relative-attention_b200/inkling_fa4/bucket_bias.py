@@ -163,10 +163,10 @@ def inkling_bucket_bias(table, starts, total_q, rel_extent, cu_seqlens_q=None):
     """``rel_logits [total_q, n_heads, rel_extent]`` (bf16, token stride 0) of a learned ``table
     [num_buckets, n_heads]`` (bf16 or fp32) whose buckets begin at the distances ``starts
     [num_buckets]`` (int32 on the device, ascending; ``relative_bucket_starts`` makes the usual
-    ones).  Differentiable in ``table``; the gradient counts the tokens before
-    ``cu_seqlens_q[-1]`` (None: all).  The result is a view for reading: its tokens are the same
-    memory."""
-    if torch.is_grad_enabled() and isinstance(table, torch.Tensor) and table.requires_grad:
+    ones).  Differentiable in ``table`` (once, and not in forward mode, which is refused); the
+    gradient counts the tokens before ``cu_seqlens_q[-1]`` (None: all).  The result is a view for
+    reading: its tokens are the same memory."""
+    if _ops.differentiates(table):
         return BucketBiasFunction.apply(table, starts, total_q, rel_extent, cu_seqlens_q)
     return _forward(table, starts, total_q, rel_extent)
 

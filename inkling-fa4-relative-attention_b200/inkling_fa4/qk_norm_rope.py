@@ -221,10 +221,6 @@ def _checked_backward(name, dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k
     return dq, dk, dqw, dkw
 
 
-def _wants_grad(t):
-    return t is not None and getattr(t, "requires_grad", False)
-
-
 class QkNormRopeFunction(torch.autograd.Function):
     """Saves the inputs only; the backward recomputes the norms."""
 
@@ -248,7 +244,7 @@ def inkling_qk_norm_rope(q, k, q_weight=None, k_weight=None, cu_seqlens_q=None, 
                          *, eps=1e-6, inv_freq=None, interleaved=False):
     """Normalised and rotated ``(q_out, k_out)`` of ``q [total_q, n_heads, 128]`` and
     ``k [total_q, kv_heads, 128]`` (bf16; slices of a merged projection are read in place),
-    differentiable in q, k and the weights.
+    differentiable in q, k and the weights (once, and not in forward mode, which is refused).
 
     ``q_weight`` / ``k_weight``: ``[128]`` bf16 or fp32 (None: ones).  ``eps=None``: no norm.
     ``inv_freq``: ``[rotary_dim / 2]`` fp64 or fp32 tensor of angles per position, 8, 16, .., 64
@@ -256,8 +252,7 @@ def inkling_qk_norm_rope(q, k, q_weight=None, k_weight=None, cu_seqlens_q=None, 
     neighbouring dims instead of the two halves.  Rows behind the last sequence
     (``cu_seqlens_q[batch]``) come out as zeros, and so do their gradients, which count in no
     weight gradient."""
-    if torch.is_grad_enabled() and (_wants_grad(q) or _wants_grad(k) or _wants_grad(q_weight)
-                                    or _wants_grad(k_weight)):
+    if _ops.differentiates(q, k, q_weight, k_weight):
         return QkNormRopeFunction.apply(q, k, q_weight, k_weight, cu_seqlens_q, cu_seqlens_k, eps,
                                         inv_freq, interleaved)
     return _forward(q, k, q_weight, k_weight, cu_seqlens_q, cu_seqlens_k, eps, inv_freq,
