@@ -221,6 +221,12 @@ at::Tensor rows_like(const at::Tensor& t) {  // contiguous, same sizes
   return new_tensor(t.sizes(), at::kBFloat16, t);
 }
 
+// A caller's tensor was written: autograd refuses a backward that saved its old values.  (Tensors of
+// inference mode have no version.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // [tokens, heads, 128] bf16 rows the kernels read in place.
 bool plain_rows(const at::Tensor& t, const at::Tensor& like) {
   return t.is_cuda() && t.dim() == 3 && t.size(2) == 128 && t.scalar_type() == at::kBFloat16 &&
@@ -420,6 +426,8 @@ Tensors kv_append_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   p.num_pages = static_cast<int32_t>(k_cache.size(0));
   p.table_width = static_cast<int32_t>(block_table.size(1));
   if (ifa4_kv_append_launch(&p, stream_of(k))) return {};
+  written(k_cache);
+  written(v_cache);
   return {q_out};
 }
 

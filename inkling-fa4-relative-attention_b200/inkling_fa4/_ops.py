@@ -215,6 +215,13 @@ def differentiates(*tensors):
     return False
 
 
+def written(*tensors):
+    """The caller's tensors (None: none) were written by a kernel: autograd refuses a backward that
+    saved their old values.  (Tensors of inference mode have no version.)"""
+    torch.autograd.graph.increment_version([t for t in tensors
+                                            if t is not None and not t.is_inference()])
+
+
 def _offsets(cu):
     """Sequence offsets as the kernels read them: one int32 behind the other (a column of a wider
     tensor is copied; anything that is no tensor is left to the checks)."""

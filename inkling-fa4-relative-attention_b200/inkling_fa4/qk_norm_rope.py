@@ -286,6 +286,9 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
     below 0 or past the table, a row behind the last sequence) writes nothing to the caches.
     No two tokens of a call may have the same place.
 
+    Not differentiable: the queries that come back are cut off from ``q``'s graph, and a backward
+    that saved a cache (or ``q``, where ``q_out`` is ``q``) from before the call raises.
+
     Returns the queries (``q_out`` if given, which may be ``q`` itself: rows behind the last
     sequence are then left as they were; a new tensor has zeros there), or None without ``q``."""
     if q is not None and q_out is None and _ops.USE_TORCH_OPS:
@@ -366,6 +369,7 @@ def _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlen
     p.table_width = block_table.shape[1]
     with torch.cuda.device(device):
         _lib.check(_lib.lib().ifa4_kv_append_launch(ctypes.byref(p), _stream(device)))
+    _ops.written(k_cache, v_cache, None if zero_padding else q_out)
     return q_out
 
 

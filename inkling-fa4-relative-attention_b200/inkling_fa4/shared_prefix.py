@@ -57,6 +57,7 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k, v, rel_logits, cu_seqle
 def _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_extent,
              shared_prefix_len, window_size, n_heads, kv_heads, head_dim, block_table,
              softmax_scale, out, prefix_splits, num_splits, chunk_len, workspace, return_lse, lse):
+    given = (out, lse)
     name = "decode_shared_prefix"
     if block_table is None:
         raise ValueError(f"{name}: needs a paged cache (block_table)")
@@ -96,6 +97,7 @@ def _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_
         stream = torch.cuda.current_stream(q.device).cuda_stream
         _lib.check(L.ifa4_decode_shared_prefix_launch(ctypes.byref(p), ctypes.c_void_p(ptr), need,
                                                       ctypes.c_void_p(stream)))
+    _ops.written(*given)
     return (out, lse) if lse is not None else out
 
 
