@@ -68,6 +68,30 @@ def _check_written(name, nm, t):
                          "alignment")
 
 
+def _apart(a, b):
+    """Whether the rows ``a`` and ``b`` [tokens, heads, 128] are known to have no element in common:
+    they lie in different memory, one behind the other, or as columns of the same rows (slices of a
+    merged projection) or heads in turn."""
+    if (not a.numel() or not b.numel()
+            or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr()):
+        return True
+
+    def end(t):  # elements from the first to behind the last
+        return sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+
+    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if at >= end(a) or -at >= end(b):
+        return True
+
+    def within(step, a_width, b_width):  # modulo step, [0, a_width) and [at, at + b_width) are apart
+        return step > 0 and a_width <= at % step <= step - b_width
+
+    (at_, ah, _), (bt, bh, _) = a.stride(), b.stride()
+    return (at_ == bt and within(bt, end(a[0]), end(b[0]))
+            or ah == bh and ah > 0 and at_ % ah == 0 and bt % ah == 0
+            and within(ah, HEAD_DIM, HEAD_DIM))
+
+
 def _check_cu(name, device, cu_q, cu_k):
     for nm, cu in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
         if cu is not None and (not isinstance(cu, torch.Tensor) or cu.dtype is not torch.int32
@@ -289,8 +313,9 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
     Not differentiable: the queries that come back are cut off from ``q``'s graph, and a backward
     that saved a cache (or ``q``, where ``q_out`` is ``q``) from before the call raises.
 
-    Returns the queries (``q_out`` if given, which may be ``q`` itself: rows behind the last
-    sequence are then left as they were; a new tensor has zeros there), or None without ``q``."""
+    Returns the queries (``q_out`` if given, which may be ``q`` itself, where ``k`` and ``v`` have no
+    element in common with it: rows behind the last sequence are then left as they were; a new
+    tensor has zeros there), or None without ``q``."""
     if q is not None and q_out is None and _ops.USE_TORCH_OPS:
         outs = _lib.plain_call("kv_append", q, k, v, k_cache, v_cache, q_weight, k_weight,
                                inv_freq, cu_seqlens_q, cu_seqlens_k, block_table, interleaved,
@@ -353,6 +378,8 @@ def _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlen
             store = q_out.untyped_storage().data_ptr()
             if not same and any(t.untyped_storage().data_ptr() == store for t in (q, k, v)):
                 raise ValueError(f"{name}: q_out must be q itself or share no storage with q, k, v")
+            if not (_apart(q_out, k) and _apart(q_out, v)):
+                raise ValueError(f"{name}: k and v must have no element in common with q_out")
             q = _rows_ready(q)
     p = _lib.KvAppendParams()
     _fill_rows(p, k=k, v=v)
