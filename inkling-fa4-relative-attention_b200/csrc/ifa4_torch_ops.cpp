@@ -12,8 +12,10 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/record_function.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -615,6 +617,9 @@ struct WithoutGil {
 template <class Read>
 PyObject* call(const char* name, PyObject* const* objects, Py_ssize_t count, Read read) {
   Tensors out;
+  // A dispatch mode or a tracer does not see what these functions do; the checks refuse a tracer.
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set() || at::tracer::impl::is_dispatch_enabled())
+    Py_RETURN_NONE;
   try {
     RECORD_FUNCTION(name, c10::ArrayRef<const c10::IValue>{});
     Arguments a{objects, count};

@@ -8,6 +8,7 @@ import ctypes
 
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
 from . import _lib
 
@@ -213,6 +214,14 @@ def differentiates(*tensors):
             if t is not None and getattr(t, "requires_grad", False):
                 return True
     return False
+
+
+def refuse_tracing(name):
+    """The operators next to the attention are no dispatcher operators: in a graph that ``make_fx`` or
+    ``torch.jit.trace`` records, their outputs would be constants and their writes would be lost."""
+    if get_proxy_mode() is not None or torch.jit.is_tracing():
+        raise RuntimeError(f"{name}: cannot be traced (the call would become a constant); trace what "
+                           "is around it")
 
 
 def written(*tensors):

@@ -6,7 +6,10 @@ A table holds one value per bucket and head; ``rel_logits[t, h, d] = table[bucke
 distances ``0 <= d < rel_extent``, where ``bucket(d)`` is the last bucket whose start is <= d.  It
 is the same for every token, so the result is one ``[n_heads, rel_extent]`` table seen through
 token stride 0, which the attention entry points read as it is.  The gradient adds the
-attention's d rel_logits over tokens and over each bucket's distances."""
+attention's d rel_logits over tokens and over each bucket's distances.
+
+The calls are no dispatcher operators: dispatch modes do not see them, and under ``make_fx`` or
+``torch.jit.trace`` they are refused."""
 from __future__ import annotations
 
 import ctypes
@@ -66,6 +69,7 @@ def _forward(table, starts, total_q, rel_extent):
         outs = _lib.plain_call("bucket_bias", table, starts, total_q, rel_extent)
         if outs is not None:
             return outs[0]
+    _ops.refuse_tracing(name)
     if not isinstance(table, torch.Tensor):
         raise TypeError(f"{name}: table must be a torch.Tensor")
     if not table.is_cuda:
@@ -103,6 +107,7 @@ def _backward(drel, starts, dtype, cu_seqlens_q):
 @torch.no_grad()
 def _checked_backward(drel, starts, dtype, cu_seqlens_q):
     name = "bucket_bias_backward"
+    _ops.refuse_tracing(name)
     if not isinstance(drel, torch.Tensor):
         raise TypeError(f"{name}: drel must be a torch.Tensor")
     if not drel.is_cuda:

@@ -12,6 +12,9 @@ The reference repository has these steps only in its diagram (outputs/architectu
 in fp32 with one rounding to bf16; the pairs are ``(i, i + len(inv_freq))`` or, ``interleaved``,
 ``(2i, 2i + 1)``.  ``pos`` is the token's position in its sequence as the other entry points
 count it: ``t - cu_seqlens_q[b]``, plus ``len_k - len_q`` when ``cu_seqlens_k`` is given.
+
+The calls are no dispatcher operators: dispatch modes do not see them, and under ``make_fx`` or
+``torch.jit.trace`` they are refused.
 """
 from __future__ import annotations
 
@@ -181,6 +184,7 @@ def _forward(q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq, interleaved):
                                interleaved, _eps(eps))
         if outs is not None:
             return outs[0], outs[1]
+    _ops.refuse_tracing(name)
     _check_rows(name, "q", q, None)
     _check_rows(name, "k", k, q)
     cu_q, cu_k = _check_cu(name, q.device, cu_q, cu_k)
@@ -217,6 +221,7 @@ def _backward(dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_fre
 @torch.no_grad()
 def _checked_backward(name, dq_out, dk_out, q, k, q_weight, k_weight, cu_q, cu_k, eps, inv_freq,
                       interleaved, weight_grads):
+    _ops.refuse_tracing(name)
     _check_rows(name, "q", q, None)
     _check_rows(name, "k", k, q)
     _check_rows(name, "dq_out", dq_out, q, q.shape[1])
@@ -330,6 +335,7 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
 def _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlens_k, q, q_weight,
                     k_weight, eps, inv_freq, interleaved, q_out):
     name = "kv_append"
+    _ops.refuse_tracing(name)
     _check_rows(name, "k", k, None)
     _check_rows(name, "v", v, k, k.shape[1])
     device = k.device

@@ -1,5 +1,7 @@
 """Decode for a batch whose sequences begin with the same keys (a system prompt, a document that
-several questions are asked about), which the plain decode would read once per sequence."""
+several questions are asked about), which the plain decode would read once per sequence.  The call is
+no dispatcher operator: dispatch modes do not see it, and under ``make_fx`` or ``torch.jit.trace`` it is
+refused."""
 from __future__ import annotations
 
 import ctypes
@@ -59,6 +61,7 @@ def _checked(q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, max_seqlen_k, rel_
              softmax_scale, out, prefix_splits, num_splits, chunk_len, workspace, return_lse, lse):
     given = (out, lse)
     name = "decode_shared_prefix"
+    _ops.refuse_tracing(name)
     if block_table is None:
         raise ValueError(f"{name}: needs a paged cache (block_table)")
     block_table = _ops._table(block_table)
