@@ -336,6 +336,7 @@ int ifa4_rel_logits_launch(const IFA4RelLogitsParams* params, void* stream);
  * is no number reaches every sequence that is worked on with one that sees it.  A logit that is no
  * number, or +inf, makes its row NaN (ifa4_decode_launch, and a prefix of 0, leave the keys that it
  * was added up with out of the row).
+ * A shorter sequence of many keys is read by one CTA per KV head unless num_splits says otherwise.
  * decode.num_splits / chunk_len plan the keys behind the prefix; decode.max_seqlen_k is the
  * longest whole sequence, prefix included.  The workspace must be 16-byte aligned (32-byte aligned
  * ones are written in whole sectors).  Deterministic: no atomics on results. */
@@ -359,7 +360,7 @@ enum { IFA4_WEIGHT_BF16 = 0, IFA4_WEIGHT_F32 = 1 };
  * in fp32 with one rounding to bf16.  The pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with
  * interleaved.  pos is the token's position in its sequence as in IFA4RelLogitsParams (queries
  * and keys are the last len_q of len_k positions; cu_seqlens_q NULL: one sequence from 0); the
- * angle is exact for any position.
+ * angle is as good as pos * inv_freq_i in 64 bits (1e-6 rad at position 2^31).
  * q, k [total_q, heads, 128] (slices of a merged projection qualify), q_out, k_out alike; in
  * place (the same address and strides) is allowed.  Rows behind the last sequence are zeroed
  * with zero_padding, else left as they were.  All rows 16-byte aligned with strides that are

@@ -900,10 +900,14 @@ struct SharedPrefixPlan {
   size_t bytes;           // workspace
 };
 
-// Estimated times (tenths of a microsecond) that choose the splits, fitted to sweeps over 2 to 256
-// sequences, 512 to 32k prefix keys and 100 to 2000 own ones.  A CTA of the prefix kernel: a start and
-// an end of 5 us; its first tiles arrive together (up to the three stages of its ring), the others
-// take 1.3 us each.  A CTA of the own keys' kernel: 4 us and 0.95 us for 64 keys.
+// Estimated times (tenths of a microsecond) that choose the splits.  They rank plans and are no model
+// of one launch: their constants were fitted to the fastest plans of sweeps over 2 to 256 sequences,
+// 512 to 32k prefix keys and 100 to 2000 own ones.  A CTA of the prefix kernel counts 6.3 us for one
+// tile, 8.2 for two or three, 11.5 for four and 1.3 for every further one; the step behind three tiles,
+// what the ring of the single row tile takes in at once, favours CTAs of no more.  One set of constants
+// serves both modes.  Measured, a further tile takes 1.0 us (8 CTAs) to 1.7 us (144) with a single row
+// tile and 2.0 to 2.1 us with pairs, whose ring has two stages.  A CTA of the own keys' kernel: 4 us
+// and 0.95 us for 64 keys.
 struct SharedPrefixShape {
   int sms;
   int key_tiles;     // prefix tiles of 128 keys

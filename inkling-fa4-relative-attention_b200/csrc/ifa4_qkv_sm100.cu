@@ -6,9 +6,11 @@
 // token's position in its sequence (see IFA4QkNormRopeParams).
 //
 // Angles: the frequency is kept as a 64-bit fraction of a turn per position, F = frac(inv_freq /
-// 2 pi) 2^64, so pos * F modulo 2^64 is the exact fraction of a turn (the integer product wraps
-// where the angle does) and no position, however far, loses accuracy to range reduction; its top
-// 32 bits go to sincospif (error below 2e-7 rad).
+// 2 pi) 2^64, so pos * F modulo 2^64 is the fraction of a turn (the integer product wraps where the
+// angle does) and a far position loses nothing to range reduction.  What F itself is off by, the
+// rounding of inv_freq / 2 pi in 64 bits, grows with the position as it does in pos * inv_freq: below
+// 4e-7 rad at position 2^31 and one radian per position.  The top 32 bits go to sincospif (error below
+// 2e-7 rad).
 //
 // Work split: a unit is one token and a part of its heads; one warp per unit, eight lanes per head
 // row (16 dims each, so four rows run at once and a row's sum takes three shuffles), loaded and

@@ -277,8 +277,8 @@ def inkling_qk_norm_rope(q, k, q_weight=None, k_weight=None, cu_seqlens_q=None, 
 
     ``q_weight`` / ``k_weight``: ``[128]`` bf16 or fp32 (None: ones).  ``eps=None``: no norm.
     ``inv_freq``: ``[rotary_dim / 2]`` fp64 or fp32 tensor of angles per position, 8, 16, .., 64
-    entries (None: no rotation); angles are exact for any position.  ``interleaved`` pairs
-    neighbouring dims instead of the two halves.  Rows behind the last sequence
+    entries (None: no rotation); angles are good to 64-bit arithmetic, 1e-6 rad at position 2^31.
+    ``interleaved`` pairs neighbouring dims instead of the two halves.  Rows behind the last sequence
     (``cu_seqlens_q[batch]``) come out as zeros, and so do their gradients, which count in no
     weight gradient."""
     if _ops.differentiates(q, k, q_weight, k_weight):
