@@ -375,6 +375,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             mma_bf16(o[dt + 1], pa, b2, b3);
           }
         }
+        // The stage is refilled by TMA (the async proxy): the fragment loads above have to be done, not
+        // only issued, before it is given back.  Without the fence the release overtook the last
+        // ldmatrix of a tile now and then, which read the V rows of the tile three further on (dims
+        // 112 to 127 of a warp's keys; seen beside a running prefix kernel, in every call of 109
+        // sequences with 800 of its CTAs).  It costs 0.1 us of 16 (128 sequences of 2048 keys) or of 120
+        // (shared prefix, 128 behind 32k).
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->empty[st]);
       }
