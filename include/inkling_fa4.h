@@ -447,7 +447,8 @@ int ifa4_qk_norm_rope_backward_launch(const IFA4QkNormRopeBackwardParams* params
  * slot p % page_size.  k rows are normalised and rotated as in IFA4QkNormRopeParams, v rows are
  * copied, and q rows (optional, n_heads = 0 without) are normalised and rotated into q_out in
  * the same launch.  A position below 0 or past the table, and a table entry outside
- * [0, num_pages), writes nothing.  Nothing else in the caches is touched. */
+ * [0, num_pages), writes nothing.  Nothing else in the caches is touched.  q_out may be q (the same
+ * address and strides); apart from that no element that a call reads may be one that it writes. */
 typedef struct IFA4KvAppendParams {
   const void* q;
   const void* k;

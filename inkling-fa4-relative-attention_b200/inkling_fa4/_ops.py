@@ -234,7 +234,9 @@ def written(*tensors):
 def _offsets(cu):
     """Sequence offsets as the kernels read them: one int32 behind the other (a column of a wider
     tensor is copied; anything that is no tensor is left to the checks)."""
-    return cu.contiguous() if isinstance(cu, torch.Tensor) else cu
+    if not isinstance(cu, torch.Tensor) or cu.is_contiguous():
+        return cu
+    return cu.contiguous()
 
 
 def _table(block_table):

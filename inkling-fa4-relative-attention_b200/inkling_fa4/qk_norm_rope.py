@@ -313,7 +313,8 @@ def inkling_kv_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seql
     ``k`` and ``q`` take the step of ``inkling_qk_norm_rope`` (``eps=None`` and no ``inv_freq``:
     copied too).  A token without a place (a table entry outside ``[0, num_pages)``, a position
     below 0 or past the table, a row behind the last sequence) writes nothing to the caches.
-    No two tokens of a call may have the same place.
+    No two tokens of a call may have the same place, and ``k``, ``v`` and ``q`` must not lie in places
+    that the call writes.
 
     Not differentiable: the queries that come back are cut off from ``q``'s graph, and a backward
     that saved a cache (or ``q``, where ``q_out`` is ``q``) from before the call raises.

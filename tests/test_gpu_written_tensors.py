@@ -58,7 +58,8 @@ def test_inference_tensors(path):
         q = _randn(4, 2, 128)
         got, caches = _append(q, q_out=q)
         assert got is q and caches[0].is_inference()
-    _append(None, None, caches)                # tensors of inference mode outside of it
+    for q in (None, _randn(4, 2, 128)):        # tensors of inference mode outside of it
+        _append(q, None, caches)
 
 
 def test_shared_prefix_outputs(path):
