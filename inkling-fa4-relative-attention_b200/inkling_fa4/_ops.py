@@ -19,17 +19,27 @@ ALIGN = {"reference": _lib.IFA4_ALIGN_REFERENCE, "bottom_right": _lib.IFA4_ALIGN
 USE_TORCH_OPS = True
 
 
-def _tma_ready(t: torch.Tensor) -> torch.Tensor:
-    """q/k/v go through TMA: last stride 1, other strides multiples of 8 elements (16 bytes),
-    16-byte aligned base.  Anything else is copied to a contiguous tensor."""
+def copy_rows(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous copy at an aligned address (``contiguous()`` returns a contiguous tensor as it is,
+    wherever it starts)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def tma_layout(t: torch.Tensor) -> bool:
+    """q/k/v and the paged caches go through TMA: last stride 1, other strides multiples of 8
+    elements (16 bytes), 16-byte aligned base."""
     *outer, last = t.stride()
-    if last == 1 and t.data_ptr() % 16 == 0:
-        for s in outer:
-            if s <= 0 or s % 8:
-                break
-        else:
-            return t
-    return t.contiguous()
+    if last != 1 or t.data_ptr() % 16:
+        return False
+    for s in outer:
+        if s <= 0 or s % 8:
+            return False
+    return True
+
+
+def _tma_ready(t: torch.Tensor) -> torch.Tensor:
+    """Anything not laid out for TMA is copied to a contiguous tensor."""
+    return t if tma_layout(t) else copy_rows(t)
 
 
 def _inputs_ok(q, k, v, rel_logits, cu_q, cu_k, rel_extent, n_heads, kv_heads, head_dim,
@@ -183,7 +193,7 @@ def _prepare(name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, causal, window_s
     if block_table is not None:
         # a paged cache is never copied: it must already suit TMA
         for nm, t in (("k", k), ("v", v)):
-            if _tma_ready(t) is not t:
+            if not tma_layout(t):
                 raise ValueError(f"{name}: paged {nm} cache needs unit last stride, strides "
                                  "that are positive multiples of 8 elements, 16-byte alignment")
         q = _tma_ready(q)

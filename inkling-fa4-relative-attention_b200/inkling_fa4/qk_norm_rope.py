@@ -34,7 +34,7 @@ def _rows_ready(t: torch.Tensor) -> torch.Tensor:
     st, sh, sd = t.stride()
     if sd == 1 and st % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous()
+    return _ops.copy_rows(t)
 
 
 def _eps(eps):
@@ -353,7 +353,7 @@ def _checked_append(k, v, k_cache, v_cache, block_table, cu_seqlens_q, cu_seqlen
         if t.device != device or t.dim() != 4 or t.shape[2] != k.shape[1] or t.shape[3] != HEAD_DIM:
             raise ValueError(f"{name}: {nm} must be [num_pages, page_size, kv_heads, {HEAD_DIM}] "
                              "on k's device")
-        if _ops._tma_ready(t) is not t:
+        if not _ops.tma_layout(t):
             raise ValueError(f"{name}: {nm} needs unit last stride, strides that are positive "
                              "multiples of 8 elements, 16-byte alignment")
     if k_cache.shape != v_cache.shape:

@@ -19,7 +19,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, _ops
 
 D_REL = 16
 
@@ -59,14 +59,14 @@ def inkling_rel_logits(r, weight, cu_seqlens_q=None, cu_seqlens_k=None, *, alpha
     rel_extent = weight.shape[-1]
     if (weight.stride(-1) != 1 or weight.data_ptr() % 16 or w_sh % 8 or w_sj % 8
             or w_sj <= 0):
-        weight = weight.contiguous()
+        weight = _ops.copy_rows(weight)
         w_sh, w_sj = (0, weight.stride(0)) if weight.dim() == 2 else weight.stride()[:2]
     if rel_extent % 8:
         raise ValueError(f"rel_logits: rel_extent {rel_extent} must be a multiple of 8")
     if not (math.isfinite(nf) and nf > 0) or not math.isfinite(alpha):
         raise ValueError("rel_logits: nf must be finite and > 0, alpha finite")
     if r.stride(-1) != 1 or any(s % 8 for s in r.stride()[:2]) or r.data_ptr() % 16:
-        r = r.contiguous()
+        r = _ops.copy_rows(r)
     batch = 1
     for nm, cu in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k)):
         if cu is None:
