@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define IFA4_ABI_VERSION 8
+#define IFA4_ABI_VERSION 9
 
 enum {
   IFA4_OK = 0,
@@ -530,6 +530,177 @@ int ifa4_bucket_bias_backward_workspace_size(const IFA4BucketBiasBackwardParams*
                                              size_t* bytes_out);
 int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* params, void* workspace,
                                      size_t workspace_bytes, void* stream);
+
+/* Operators of long contexts over the paged cache (ABI version 9; not in the reference, whose calls
+ * read every visible key).  Queries are the last of their sequence's keys, as with
+ * IFA4_ALIGN_BOTTOM_RIGHT: row i of a sequence's len_q rows has position p = len_k - len_q + i and
+ * sees the keys j with 0 <= p - j (and p - j <= window_left where that is >= 0).  Key j of sequence b
+ * sits in page block_table[b * block_table_stride + j / page_size], slot j % page_size; an entry
+ * outside [0, num_pages), or past table_width, is no page (its keys read as zeros, nothing is written
+ * there).  Rows from cu_seqlens_q[batch] on belong to no sequence. */
+typedef struct IFA4PagedSeqs {
+  const int32_t* cu_seqlens_q;  /* int32 [batch + 1] on the device                         */
+  const int32_t* cu_seqlens_k;  /* int32 [batch + 1] on the device                         */
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t batch;
+  int32_t page_size;            /* a power of two in [16, 2^20]                            */
+  int32_t num_pages;
+  int32_t table_width;          /* entries of a table row                                  */
+} IFA4PagedSeqs;
+
+/* Bounds of pages: bounds[page, kv_head, 0] and [.., 1] become the elementwise minimum and maximum of
+ * the page's keys (bf16; NaN where one is), over the keys a sequence has in it, for the pages that
+ * hold any of the last len_q keys of a sequence (len_q = len_k: all its pages).  A page that several
+ * sequences hold must be full in each of them. */
+typedef struct IFA4PageBoundsParams {
+  IFA4PagedSeqs seqs;
+  const void* k_cache;          /* [num_pages, page_size, kv_heads, 128] bf16              */
+  void* bounds;                 /* [num_pages, kv_heads, 2, 128] bf16, written in place    */
+  int64_t k_stride_page, k_stride_t, k_stride_h;
+  int64_t bounds_stride_page, bounds_stride_h;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t max_seqlen_q;         /* grid-size hint; <= 0: the table's width                 */
+} IFA4PageBoundsParams;
+
+int ifa4_page_bounds_launch(const IFA4PageBoundsParams* params, void* stream);
+
+/* Scores of pages: scores[t, g, c] = max over the heads h of group g of
+ *   softmax_scale * sum_i (max(q_i, 0) max_i + min(q_i, 0) min_i) + max_j bias(t, h, p - j)
+ * with the bounds of page c and its visible keys j, bias(t, h, d) = rel[t, h, d] for
+ * 0 <= d < rel_extent and 0 beyond: no logit of the page is larger.  A page without a visible key
+ * gets -inf, the first first_pages and the last last_pages of a row's visible pages +inf.  NaN and
+ * infinite bounds give what the formula gives.  Rows of no sequence get -inf where
+ * zero_padding is set and stay as they are otherwise. */
+typedef struct IFA4PageScoresParams {
+  IFA4PagedSeqs seqs;
+  const void* q;
+  const void* bounds;
+  const void* rel;
+  float* scores;                /* [total_q, kv_heads, table_width], unit last stride      */
+  int64_t q_stride_t, q_stride_h;
+  int64_t bounds_stride_page, bounds_stride_h;
+  int64_t rel_stride_t, rel_stride_h;
+  int64_t scores_stride_t, scores_stride_h;
+  int64_t total_q;
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rel_extent;
+  int32_t window_left;
+  int32_t max_seqlen_q;         /* grid-size hint; <= 0: total_q                           */
+  int32_t first_pages;
+  int32_t last_pages;
+  int32_t zero_padding;
+  int32_t dtype;
+  float softmax_scale;
+} IFA4PageScoresParams;
+
+int ifa4_page_scores_launch(const IFA4PageScoresParams* params, void* stream);
+
+/* The num_selected largest of each row's scores, as ascending indices: ties take the lowest index,
+ * NaN ranks above everything, -inf is never taken; what is not filled is -1. */
+typedef struct IFA4SelectPagesParams {
+  const float* scores;          /* [rows, kv_heads, width], unit last stride               */
+  int32_t* pages;               /* [rows, kv_heads, num_selected], unit last stride        */
+  int64_t scores_stride_t, scores_stride_h;
+  int64_t pages_stride_t, pages_stride_h;
+  int64_t rows;
+  int32_t kv_heads;
+  int32_t width;
+  int32_t num_selected;
+} IFA4SelectPagesParams;
+
+int ifa4_select_pages_launch(const IFA4SelectPagesParams* params, void* stream);
+
+/* Attention over chosen pages: row t attends, for KV head g, to the visible keys of the pages
+ * pages[t, g, :] of its sequence (indices into its table row, in any order; an entry that is no index
+ * of a page with a visible key adds nothing, one that is listed twice counts twice).  Any number of
+ * rows a sequence.  A row without keys is 0 with the lse -inf; a logit that is NaN or +inf makes its
+ * row NaN.  decode.block_table and the seqs fields that repeat there have to agree (batch,
+ * cu_seqlens, page_size, num_pages come from decode); chunk_len is not used.  Rows of no sequence
+ * get 0 (lse -inf) where zero_padding is set and stay as they are otherwise. */
+typedef struct IFA4DecodePagesParams {
+  IFA4DecodeParams decode;
+  const int32_t* pages;         /* [total_q, kv_heads, num_selected], unit last stride     */
+  int64_t pages_stride_t, pages_stride_h;
+  int32_t num_selected;
+  int32_t table_width;
+  int32_t zero_padding;
+} IFA4DecodePagesParams;
+
+int ifa4_decode_pages_workspace_size(const IFA4DecodePagesParams* params, size_t* bytes_out);
+int ifa4_decode_pages_launch(const IFA4DecodePagesParams* params, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Attention weight that keys gather: mass[b, g, j] (+)= sum over the rows t of sequence b that see
+ * key j and the heads h of group g of exp(softmax_scale q_th . k_gj + bias(t, h, p - j) - lse[h, t]),
+ * in fp32 and in a fixed order.  lse is that of the attention over the same keys (a row whose lse is
+ * -inf adds nothing).  accumulate: places past a sequence's keys stay as they are; otherwise every
+ * place is written, those with 0.  n_heads / kv_heads <= 128. */
+typedef struct IFA4AttentionMassParams {
+  IFA4PagedSeqs seqs;
+  const void* q;
+  const void* k_cache;
+  const void* rel;
+  const float* lse;             /* [h * lse_stride_h + t * lse_stride_t]                   */
+  float* mass;                  /* [batch, kv_heads, mass_width], unit last stride         */
+  int64_t q_stride_t, q_stride_h;
+  int64_t k_stride_page, k_stride_t, k_stride_h;
+  int64_t rel_stride_t, rel_stride_h;
+  int64_t lse_stride_h, lse_stride_t;
+  int64_t mass_stride_b, mass_stride_h;
+  int64_t total_q;
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rel_extent;
+  int32_t window_left;
+  int32_t max_seqlen_q;         /* grid-size hints; <= 0: total_q, the mass's width        */
+  int32_t max_seqlen_k;
+  int32_t mass_width;           /* keys from here on have no place                         */
+  int32_t accumulate;
+  int32_t dtype;
+  float softmax_scale;
+} IFA4AttentionMassParams;
+
+int ifa4_attention_mass_launch(const IFA4AttentionMassParams* params, void* stream);
+
+/* Eviction: every sequence of more than budget keys keeps, for each KV head, its first `first` and
+ * its last `recent` keys and those of the largest mass (ties: the lowest place; NaN ranks above
+ * everything) up to budget, in their order; their K and V rows move to the places 0 .. budget - 1 of
+ * the sequence, in place.  kept gets the places they had (-1 behind the last), mass_out the masses of
+ * what is kept with zeros behind, cu_out the offsets of the new lengths.  Shorter sequences keep
+ * everything.  A kept key without a page is zeros at its new place.  No page may be held by two
+ * sequences, or twice by one.  seqs.cu_seqlens_q is not used; the workspace
+ * (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by calls that may run at
+ * the same time. */
+typedef struct IFA4KvEvictParams {
+  IFA4PagedSeqs seqs;
+  void* k_cache;
+  void* v_cache;
+  const float* mass;            /* [batch, kv_heads, mass_width], unit last stride         */
+  float* mass_out;              /* the same shape, other memory                            */
+  int32_t* kept;                /* [batch, kv_heads, budget], contiguous                   */
+  int32_t* cu_out;              /* [batch + 1]                                             */
+  int64_t k_stride_page, k_stride_t, k_stride_h;
+  int64_t v_stride_page, v_stride_t, v_stride_h;
+  int64_t mass_stride_b, mass_stride_h;
+  int64_t mass_out_stride_b, mass_out_stride_h;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t mass_width;           /* keys from here on count as of no mass                   */
+  int32_t budget;               /* >= 1, >= first + recent                                 */
+  int32_t first;
+  int32_t recent;
+  int32_t dtype;
+} IFA4KvEvictParams;
+
+int ifa4_kv_evict_workspace_size(const IFA4KvEvictParams* params, size_t* bytes_out);
+int ifa4_kv_evict_launch(const IFA4KvEvictParams* params, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* Self-test of the failure detection (test hook; the reference has no counterpart): launches
  * on `stream` a kernel whose barrier wait can never complete, so the kernels' bounded-wait path

@@ -1589,6 +1589,493 @@ int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* p, void
 }  // extern "C"
 
 // ---------------------------------------------------------------------------------------
+// Long contexts over the paged cache
+// ---------------------------------------------------------------------------------------
+namespace {
+
+int check_seqs(const char* what, const IFA4PagedSeqs* s, bool queries) {
+  if (s->batch < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative batch", what);
+  if (s->batch > 65534) return fail(IFA4_ERR_UNSUPPORTED, "%s: batch > 65534", what);
+  if (s->page_size < 16 || s->page_size > (1 << 20) || (s->page_size & (s->page_size - 1)) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: page_size %d must be a power of two in [16, 2^20]",
+                what, s->page_size);
+  if (s->num_pages < 0 || s->table_width < 0 || s->block_table_stride < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative num_pages, table_width or table stride",
+                what);
+  if (s->table_width > (1 << 26))
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: table_width > 2^26", what);
+  if (s->batch > 0 && ((queries && s->cu_seqlens_q == nullptr) || s->cu_seqlens_k == nullptr ||
+                       (s->block_table == nullptr && s->table_width > 0)))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null cu_seqlens or block_table", what);
+  return IFA4_OK;
+}
+
+ifa4::PagedSeqs paged_seqs(const IFA4PagedSeqs* s) {
+  ifa4::PagedSeqs k{};
+  k.cu_q = s->cu_seqlens_q;
+  k.cu_k = s->cu_seqlens_k;
+  k.block_table = s->block_table;
+  k.bt_stride = s->block_table_stride;
+  k.batch = s->batch;
+  k.page_shift = log2_exact(s->page_size);
+  k.num_pages = s->num_pages;
+  k.table_width = s->table_width;
+  return k;
+}
+
+// A cache or bounds tensor [pages, ..]: 16-byte aligned, strides positive multiples of 8.
+int check_pages(const char* what, const char* name, const void* p, int64_t sp, int64_t st,
+                int64_t sh, int num_pages) {
+  if (num_pages > 0 && p == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: %s is NULL", what, name);
+  if (!aligned16(p) || sp <= 0 || sp % 8 != 0 || st <= 0 || st % 8 != 0 || sh <= 0 || sh % 8 != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: %s needs 16-byte alignment and strides that are positive multiples of 8 elements",
+                what, name);
+  return IFA4_OK;
+}
+
+template <class P>
+int check_heads(const char* what, const P* p, int n_heads) {
+  if (p->dtype != IFA4_DTYPE_BF16)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: dtype %d unsupported (bf16 only)", what, p->dtype);
+  if (p->head_dim != ifa4::kHeadDim)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (128 only)", what, p->head_dim);
+  if (p->kv_heads <= 0 || n_heads <= 0 || n_heads % p->kv_heads != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: n_heads %d must be a positive multiple of kv_heads %d", what, n_heads,
+                p->kv_heads);
+  if (n_heads > 65535) return fail(IFA4_ERR_UNSUPPORTED, "%s: n_heads > 65535", what);
+  return IFA4_OK;
+}
+
+// Queries with their bias.
+template <class P>
+int check_queries(const char* what, const P* p) {
+  if (p->total_q < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative total_q", what);
+  if (p->rel_extent <= 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: rel_extent must be > 0", what);
+  if (!(p->softmax_scale > 0.f))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0", what);
+  if (p->rel_stride_t < 0 || p->rel_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative rel strides", what);
+  if (p->total_q == 0) return IFA4_OK;
+  if (!p->q || !p->rel) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if (!aligned16(p->q) || p->q_stride_t <= 0 || p->q_stride_t % 8 != 0 || p->q_stride_h <= 0 ||
+      p->q_stride_h % 8 != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: q needs 16-byte alignment and strides that are positive multiples of 8 elements",
+                what);
+  return IFA4_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Splits of the rows of an attention over chosen pages, and its workspace.
+int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes) {
+  const char* what = "decode_pages";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  const IFA4DecodeParams* d = &p->decode;
+  int rc = validate_common(d, what);
+  if (rc) return rc;
+  if (d->batch > 65534) return fail(IFA4_ERR_UNSUPPORTED, "%s: batch > 65534", what);
+  if (d->block_table == nullptr && d->batch > 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: needs a paged cache (block_table)", what);
+  if (d->causal_align != IFA4_ALIGN_BOTTOM_RIGHT || !d->causal)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: needs causal and IFA4_ALIGN_BOTTOM_RIGHT", what);
+  if (p->num_selected < 0 || p->num_selected > (1 << 26) || p->table_width < 0 ||
+      p->table_width > (1 << 26))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_selected and table_width must be in [0, 2^26]",
+                what);
+  if (d->num_splits < 0 || d->num_splits > 1024)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_splits must be in [0, 1024]", what);
+  *splits = 1;
+  *bytes = 0;
+  if (d->batch == 0 || d->total_q == 0) return IFA4_OK;
+  if (p->num_selected > 0 && p->pages == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: pages is NULL", what);
+  const int group = d->n_heads / d->kv_heads;
+  const int64_t rows = d->total_q * d->kv_heads * ceil_div(group, 16);
+  const int64_t tiles = ceil_div(static_cast<int64_t>(p->num_selected) * d->page_size, 64);
+  if (d->num_splits > 0) {
+    *splits = d->num_splits;
+  } else {
+    int sms = 148;
+    if ((rc = sm_count(&sms))) return rc;
+    // two CTAs an SM; a split of fewer than four tiles spends its time on starting and merging
+    int64_t s = 2 * sms / rows;
+    if (s > tiles / 4) s = tiles / 4;
+    if (s > 64) s = 64;
+    *splits = static_cast<int>(s < 1 ? 1 : s);
+  }
+  if (d->total_q * *splits > 0x7fffffff || ceil_div(d->total_q * d->n_heads, 4) > 0x7fffffff)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: too many rows", what);
+  if (*splits > 1) {
+    const size_t parts = static_cast<size_t>(d->total_q) * d->n_heads * *splits;
+    *bytes = parts * 130 * sizeof(float);
+  }
+  return IFA4_OK;
+}
+
+int validate_evict(const IFA4KvEvictParams* p) {
+  const char* what = "kv_evict";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  int rc = check_seqs(what, &p->seqs, false);
+  if (rc) return rc;
+  if ((rc = check_heads(what, p, p->kv_heads))) return rc;
+  if (p->budget < 1 || p->budget > (1 << 30) || p->first < 0 || p->recent < 0 ||
+      p->first > p->budget || p->recent > p->budget - p->first)
+    return fail(IFA4_ERR_INVALID_ARGUMENT,
+                "%s: budget must be in [1, 2^30] and hold the first and the recent keys", what);
+  if (p->mass_width < 0 || p->mass_width > (1 << 30))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_width must be in [0, 2^30]", what);
+  if (p->cu_out == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: cu_out is NULL", what);
+  if (p->seqs.batch == 0) return IFA4_OK;
+  if (p->kept == nullptr || (p->mass_width > 0 && (p->mass == nullptr || p->mass_out == nullptr)))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if (p->mass_width > 0 && p->mass == p->mass_out)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_out must be other memory than mass", what);
+  if ((rc = check_pages(what, "k_cache", p->k_cache, p->k_stride_page, p->k_stride_t, p->k_stride_h,
+                        p->seqs.num_pages)) ||
+      (rc = check_pages(what, "v_cache", p->v_cache, p->v_stride_page, p->v_stride_t, p->v_stride_h,
+                        p->seqs.num_pages)))
+    return rc;
+  return IFA4_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ifa4_page_bounds_launch(const IFA4PageBoundsParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "page_bounds";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  int rc;
+  if ((rc = check_seqs(what, &p->seqs, true)) || (rc = check_heads(what, p, p->kv_heads)) ||
+      (rc = check_pages(what, "k_cache", p->k_cache, p->k_stride_page, p->k_stride_t, p->k_stride_h,
+                        p->seqs.num_pages)) ||
+      (rc = check_pages(what, "bounds", p->bounds, p->bounds_stride_page, p->bounds_stride_h, 8,
+                        p->seqs.num_pages)))
+    return rc;
+  if (p->seqs.batch == 0 || p->seqs.num_pages == 0 || p->seqs.table_width == 0) return IFA4_OK;
+  ifa4::PageBoundsKernelArgs a{};
+  a.s = paged_seqs(&p->seqs);
+  a.k_cache = static_cast<const uint16_t*>(p->k_cache);
+  a.bounds = static_cast<uint16_t*>(p->bounds);
+  a.k_sp = p->k_stride_page;
+  a.k_st = p->k_stride_t;
+  a.k_sh = p->k_stride_h;
+  a.b_sp = p->bounds_stride_page;
+  a.b_sh = p->bounds_stride_h;
+  a.kv_heads = p->kv_heads;
+  // pages that the new tokens of a sequence can touch
+  int64_t pages = p->seqs.table_width;
+  if (p->max_seqlen_q > 0) {
+    const int64_t touched = (static_cast<int64_t>(p->max_seqlen_q) + p->seqs.page_size - 2) /
+                                p->seqs.page_size + 1;
+    if (touched < pages) pages = touched;
+  }
+  int64_t blocks = ceil_div(pages * p->kv_heads, ifa4::kPageBoundsWarps);
+  if (blocks > (1 << 20)) blocks = 1 << 20;
+  cudaError_t e = ifa4::launch_page_bounds_sm100(a, static_cast<int>(blocks),
+                                                 static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "page_bounds launch");
+  return IFA4_OK;
+}
+
+int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "page_scores";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  int rc;
+  if ((rc = check_seqs(what, &p->seqs, true)) || (rc = check_heads(what, p, p->n_heads)) ||
+      (rc = check_queries(what, p)) ||
+      (rc = check_pages(what, "bounds", p->bounds, p->bounds_stride_page, p->bounds_stride_h, 8,
+                        p->seqs.num_pages)))
+    return rc;
+  if (p->first_pages < 0 || p->last_pages < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative first_pages or last_pages", what);
+  if (p->kv_heads > 16383) return fail(IFA4_ERR_UNSUPPORTED, "%s: kv_heads > 16383", what);
+  if (p->seqs.batch == 0 || p->total_q == 0 || p->seqs.table_width == 0) return IFA4_OK;
+  if (p->scores == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores is NULL", what);
+  if (p->scores_stride_t < 0 || p->scores_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative scores strides", what);
+  ifa4::PageScoresKernelArgs a{};
+  a.s = paged_seqs(&p->seqs);
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.bounds = static_cast<const uint16_t*>(p->bounds);
+  a.rel = static_cast<const uint16_t*>(p->rel);
+  a.scores = p->scores;
+  a.q_st = p->q_stride_t;
+  a.q_sh = p->q_stride_h;
+  a.b_sp = p->bounds_stride_page;
+  a.b_sh = p->bounds_stride_h;
+  a.rel_st = p->rel_stride_t;
+  a.rel_sh = p->rel_stride_h;
+  a.sc_st = p->scores_stride_t;
+  a.sc_sh = p->scores_stride_h;
+  a.total_q = p->total_q;
+  a.n_heads = p->n_heads;
+  a.kv_heads = p->kv_heads;
+  a.group = p->n_heads / p->kv_heads;
+  a.rel_extent = p->rel_extent;
+  a.window_left = p->window_left < 0 ? -1 : p->window_left;
+  a.first_pages = p->first_pages;
+  a.last_pages = p->last_pages;
+  a.zero_padding = p->zero_padding != 0;
+  a.scale = p->softmax_scale;
+  const int tokens = a.group < 16 ? 16 / a.group : 1;
+  int64_t most = p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q;
+  int64_t blocks = ceil_div(most, tokens);
+  if (blocks > 65535 / p->kv_heads) blocks = 65535 / p->kv_heads;
+  a.row_blocks = static_cast<int>(blocks);
+  cudaError_t e = ifa4::launch_page_scores_sm100(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "page_scores launch");
+  return IFA4_OK;
+}
+
+int ifa4_select_pages_launch(const IFA4SelectPagesParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "select_pages";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  if (p->rows < 0 || p->kv_heads < 0 || p->kv_heads > 65535 || p->width < 0 || p->width > (1 << 26))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: rows, kv_heads or width out of range", what);
+  if (p->num_selected < 1 || p->num_selected > (1 << 26))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_selected must be in [1, 2^26]", what);
+  if (p->rows == 0 || p->kv_heads == 0) return IFA4_OK;
+  if ((p->scores == nullptr && p->width > 0) || p->pages == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if (p->scores_stride_t < 0 || p->scores_stride_h < 0 || p->pages_stride_t < 0 ||
+      p->pages_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative strides", what);
+  ifa4::SelectPagesKernelArgs a{};
+  a.scores = p->scores;
+  a.pages = p->pages;
+  a.sc_st = p->scores_stride_t;
+  a.sc_sh = p->scores_stride_h;
+  a.pg_st = p->pages_stride_t;
+  a.pg_sh = p->pages_stride_h;
+  a.rows = p->rows;
+  a.kv_heads = p->kv_heads;
+  a.width = p->width;
+  a.count = p->num_selected;
+  cudaError_t e = ifa4::launch_select_pages_sm100(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "select_pages launch");
+  return IFA4_OK;
+}
+
+int ifa4_decode_pages_workspace_size(const IFA4DecodePagesParams* p, size_t* bytes_out) {
+  g_last_error[0] = '\0';
+  int splits;
+  size_t bytes;
+  int rc = decode_pages_plan(p, &splits, &bytes);
+  if (rc) return rc;
+  if (bytes_out == nullptr)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "decode_pages: bytes_out is NULL");
+  *bytes_out = bytes;
+  return IFA4_OK;
+}
+
+int ifa4_decode_pages_launch(const IFA4DecodePagesParams* p, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  g_last_error[0] = '\0';
+  int splits;
+  size_t bytes;
+  int rc = decode_pages_plan(p, &splits, &bytes);
+  if (rc) return rc;
+  const IFA4DecodeParams* d = &p->decode;
+  if (d->batch == 0 || d->total_q == 0) return IFA4_OK;
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(IFA4_ERR_WORKSPACE, "decode_pages: workspace of %zu bytes required, got %zu", bytes,
+                workspace_bytes);
+  if (bytes > 0 && !aligned16(workspace))
+    return fail(IFA4_ERR_WORKSPACE, "decode_pages: workspace must be 16-byte aligned");
+  if (p->pages_stride_t < 0 || p->pages_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "decode_pages: negative pages strides");
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
+  ifa4::DecodePagesKernelArgs a{};
+  a.s.cu_q = d->cu_seqlens_q;
+  a.s.cu_k = d->cu_seqlens_k;
+  a.s.block_table = d->block_table;
+  a.s.bt_stride = d->block_table_stride;
+  a.s.batch = d->batch;
+  a.s.page_shift = log2_exact(d->page_size);
+  a.s.num_pages = d->num_pages;
+  a.s.table_width = p->table_width;
+  a.box_shift = a.s.page_shift < 6 ? a.s.page_shift : 6;
+  a.q = static_cast<const uint16_t*>(d->q);
+  a.rel = static_cast<const uint16_t*>(d->rel);
+  a.pages = p->pages;
+  a.out = static_cast<uint16_t*>(d->out);
+  a.q_st = d->q_stride_t;
+  a.q_sh = d->q_stride_h;
+  a.rel_st = d->rel_stride_t;
+  a.rel_sh = d->rel_stride_h;
+  a.out_st = d->out_stride_t;
+  a.out_sh = d->out_stride_h;
+  a.pg_st = p->pages_stride_t;
+  a.pg_sh = p->pages_stride_h;
+  a.total_q = d->total_q;
+  a.n_heads = d->n_heads;
+  a.kv_heads = d->kv_heads;
+  a.rel_extent = d->rel_extent;
+  a.window_left = d->window_left < 0 ? -1 : d->window_left;
+  a.group = d->n_heads / d->kv_heads;
+  a.heads_per_cta = a.group < 16 ? a.group : 16;
+  a.num_selected = p->num_selected;
+  a.num_splits = splits;
+  a.zero_padding = p->zero_padding != 0;
+  a.scale_log2 = d->softmax_scale * 1.4426950408889634f;
+  if (splits > 1) {
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = a.ws_o + static_cast<size_t>(d->total_q) * d->n_heads * splits * 128;
+  }
+  a.lse = d->lse;
+  a.lse_sh = d->lse_stride_h;
+  a.lse_st = d->lse_stride_t;
+  a.status = status;
+  CUtensorMap tk, tv;
+  if ((rc = encode_kv(d, 64, &tk, &tv))) return rc;
+  cudaError_t e = ifa4::launch_decode_pages_sm100(a, tk, tv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "decode_pages launch");
+  return IFA4_OK;
+}
+
+int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
+  g_last_error[0] = '\0';
+  const char* what = "attention_mass";
+  if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
+  int rc;
+  if ((rc = check_seqs(what, &p->seqs, true)) || (rc = check_heads(what, p, p->n_heads)) ||
+      (rc = check_queries(what, p)) ||
+      (rc = check_pages(what, "k_cache", p->k_cache, p->k_stride_page, p->k_stride_t, p->k_stride_h,
+                        p->seqs.num_pages)))
+    return rc;
+  const int group = p->n_heads / p->kv_heads;
+  if (group > 128)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: more than 128 query heads per KV head", what);
+  if (p->mass_width < 0 || p->mass_width > (1 << 30))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_width must be in [0, 2^30]", what);
+  if (p->mass_stride_b < 0 || p->mass_stride_h < 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative mass strides", what);
+  if (p->seqs.batch == 0 || p->mass_width == 0) return IFA4_OK;
+  if (p->mass == nullptr || (p->total_q > 0 && p->lse == nullptr))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if (p->total_q == 0 && p->accumulate) return IFA4_OK;
+  if (p->seqs.num_pages == 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_pages must be > 0", what);
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
+  int sms = 148;
+  if ((rc = sm_count(&sms))) return rc;
+  int64_t most_q = p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q;
+  const int rows = ifa4::attention_mass_tile_rows(most_q * group, group);
+  ifa4::AttentionMassKernelArgs a{};
+  a.s = paged_seqs(&p->seqs);
+  a.rel = static_cast<const uint16_t*>(p->rel);
+  a.lse = p->lse;
+  a.mass = p->mass;
+  a.rel_st = p->rel_stride_t;
+  a.rel_sh = p->rel_stride_h;
+  a.lse_sh = p->lse_stride_h;
+  a.lse_st = p->lse_stride_t;
+  a.mass_sb = p->mass_stride_b;
+  a.mass_sh = p->mass_stride_h;
+  a.total_q = p->total_q;
+  a.n_heads = p->n_heads;
+  a.kv_heads = p->kv_heads;
+  a.group = group;
+  a.rel_extent = p->rel_extent;
+  a.window_left = p->window_left < 0 ? -1 : p->window_left;
+  a.mass_width = p->mass_width;
+  a.accumulate = p->accumulate != 0;
+  a.box_shift = a.s.page_shift < 7 ? a.s.page_shift : 7;
+  a.tokens_per_tile = rows / group;
+  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  a.status = status;
+  CUtensorMap tq, tk;
+  // without rows nothing is loaded, but the map has to be one
+  if ((rc = encode_rows_heads_dims(&tq, p->total_q > 0 ? p->q : p->k_cache,
+                                   p->total_q > 0 ? p->total_q : 1, p->n_heads,
+                                   p->total_q > 0 ? p->q_stride_t : 128 * int64_t{p->n_heads},
+                                   p->total_q > 0 ? p->q_stride_h : 128,
+                                   static_cast<uint32_t>(a.tokens_per_tile), "q",
+                                   static_cast<uint32_t>(group))))
+    return rc;
+  if ((rc = encode_paged(&tk, p->k_cache, p->seqs.num_pages, p->seqs.page_size, p->kv_heads,
+                         p->k_stride_page, p->k_stride_t, p->k_stride_h, 1u << a.box_shift, "k")))
+    return rc;
+  // pairs of key tiles of the longest sequence; where all rows are one tile, a CTA takes several
+  int64_t most_k = p->mass_width;
+  if (a.accumulate && p->max_seqlen_k > 0 && p->max_seqlen_k < most_k) most_k = p->max_seqlen_k;
+  int64_t blocks = ceil_div(most_k, 256);
+  if (most_q * group <= rows) {
+    const int64_t want = ceil_div(4 * sms, int64_t{p->kv_heads} * p->seqs.batch);
+    if (blocks > want) blocks = want;
+  }
+  cudaError_t e = ifa4::launch_attention_mass_sm100(a, rows, tq, tk, static_cast<int>(blocks),
+                                                    static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "attention_mass launch");
+  return IFA4_OK;
+}
+
+int ifa4_kv_evict_workspace_size(const IFA4KvEvictParams* p, size_t* bytes_out) {
+  g_last_error[0] = '\0';
+  int rc = validate_evict(p);
+  if (rc) return rc;
+  if (bytes_out == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "kv_evict: bytes_out is NULL");
+  *bytes_out = 0;
+  return IFA4_OK;
+}
+
+int ifa4_kv_evict_launch(const IFA4KvEvictParams* p, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  g_last_error[0] = '\0';
+  int rc = validate_evict(p);
+  if (rc) return rc;
+  (void)workspace;
+  (void)workspace_bytes;
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
+  if (p->seqs.batch == 0) {
+    cudaError_t e = cudaMemsetAsync(p->cu_out, 0, sizeof(int32_t),
+                                    static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? IFA4_OK : cuda_fail(e, "kv_evict");
+  }
+  ifa4::KvEvictKernelArgs a{};
+  a.s = paged_seqs(&p->seqs);
+  a.k_cache = static_cast<uint16_t*>(p->k_cache);
+  a.v_cache = static_cast<uint16_t*>(p->v_cache);
+  a.mass = p->mass;
+  a.mass_out = p->mass_out;
+  a.kept = p->kept;
+  a.cu_out = p->cu_out;
+  a.k_sp = p->k_stride_page;
+  a.k_st = p->k_stride_t;
+  a.k_sh = p->k_stride_h;
+  a.v_sp = p->v_stride_page;
+  a.v_st = p->v_stride_t;
+  a.v_sh = p->v_stride_h;
+  a.mass_sb = p->mass_stride_b;
+  a.mass_sh = p->mass_stride_h;
+  a.mo_sb = p->mass_out_stride_b;
+  a.mo_sh = p->mass_out_stride_h;
+  a.kv_heads = p->kv_heads;
+  a.mass_width = p->mass_width;
+  a.budget = p->budget;
+  a.first = p->first;
+  a.recent = p->recent;
+  a.status = status;
+  cudaError_t e = ifa4::launch_kv_evict_sm100(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "kv_evict launch");
+  return IFA4_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------
 // rel_logits producer
 // ---------------------------------------------------------------------------------------
 namespace {

@@ -292,6 +292,105 @@ int plan_bucket_grad(BucketGradKernelArgs* a, int sms);
 cudaError_t launch_bucket_grad_sm100(const BucketGradKernelArgs& args, int vec,
                                      cudaStream_t stream);
 
+// Long contexts over the paged cache.
+struct PagedSeqs {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  const int32_t* block_table;
+  long long bt_stride;
+  int batch, page_shift, num_pages, table_width;
+};
+
+struct PageBoundsKernelArgs {
+  PagedSeqs s;
+  const uint16_t* k_cache;
+  uint16_t* bounds;          // [pages, kv_heads, 2, 128]
+  long long k_sp, k_st, k_sh, b_sp, b_sh;
+  int kv_heads;
+};
+// grid.y: sequences; the blocks of grid.x stride over a sequence's (page, head) units.
+constexpr int kPageBoundsWarps = 8;
+cudaError_t launch_page_bounds_sm100(const PageBoundsKernelArgs& args, int blocks_per_seq,
+                                     cudaStream_t stream);
+
+struct PageScoresKernelArgs {
+  PagedSeqs s;
+  const uint16_t* q;
+  const uint16_t* bounds;
+  const uint16_t* rel;
+  float* scores;
+  long long q_st, q_sh, b_sp, b_sh, rel_st, rel_sh, sc_st, sc_sh;
+  long long total_q;
+  int n_heads, kv_heads, group, rel_extent, window_left;
+  int first_pages, last_pages, zero_padding;
+  int row_blocks;            // blocks of rows of a sequence in the grid (strided over)
+  float scale;
+};
+cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream);
+
+struct SelectPagesKernelArgs {
+  const float* scores;
+  int32_t* pages;
+  long long sc_st, sc_sh, pg_st, pg_sh;
+  long long rows;
+  int kv_heads, width, count;
+};
+cudaError_t launch_select_pages_sm100(const SelectPagesKernelArgs& args, cudaStream_t stream);
+
+struct DecodePagesKernelArgs {
+  PagedSeqs s;
+  const uint16_t* q;
+  const uint16_t* rel;
+  const int32_t* pages;
+  uint16_t* out;
+  long long q_st, q_sh, rel_st, rel_sh, out_st, out_sh, pg_st, pg_sh;
+  long long total_q;
+  int n_heads, kv_heads, rel_extent, window_left;
+  int group, heads_per_cta;  // as in DecodeKernelArgs
+  int num_selected, num_splits, box_shift, zero_padding;
+  float scale_log2;
+  float* ws_o;               // [total_q, n_heads, num_splits, 128] (num_splits > 1)
+  float* ws_ml;              // [total_q, n_heads, num_splits, 2]: largest score (log2 units), sum
+  float* lse;                // optional natural-log LSE
+  long long lse_sh, lse_st;
+  int* status;
+};
+cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const CUtensorMap& tm_k,
+                                      const CUtensorMap& tm_v, cudaStream_t stream);
+
+struct AttentionMassKernelArgs {
+  PagedSeqs s;
+  const uint16_t* rel;
+  const float* lse;
+  float* mass;
+  long long rel_st, rel_sh, lse_sh, lse_st, mass_sb, mass_sh;
+  long long total_q;
+  int n_heads, kv_heads, group, rel_extent, window_left;
+  int mass_width, accumulate, box_shift;
+  int tokens_per_tile;       // query tokens of a tile of rows
+  float scale_log2;
+  int* status;
+};
+// Query rows of a tile for these many rows of a sequence: 16, 32, 64 or 128.
+int attention_mass_tile_rows(long long rows, int group);
+cudaError_t launch_attention_mass_sm100(const AttentionMassKernelArgs& args, int tile_rows,
+                                        const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                        int key_blocks, cudaStream_t stream);
+
+struct KvEvictKernelArgs {
+  PagedSeqs s;
+  uint16_t* k_cache;
+  uint16_t* v_cache;
+  const float* mass;
+  float* mass_out;
+  int32_t* kept;             // [batch, kv_heads, budget]
+  int32_t* cu_out;
+  long long k_sp, k_st, k_sh, v_sp, v_st, v_sh, mass_sb, mass_sh, mo_sb, mo_sh;
+  int kv_heads, mass_width, budget, first, recent;
+  int* status;
+};
+cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, cudaStream_t stream);
+
 struct BackwardKernelArgs {
   const uint16_t* rel;       // bf16 bits
   const uint16_t* out;       // forward output O

@@ -1,0 +1,499 @@
+// The attention weight that keys gather, and the eviction of the keys with the least from a paged
+// cache, for sm_100a.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ifa4_internal.h"
+#include "ifa4_paged.cuh"
+#include "ifa4_ptx.cuh"
+
+namespace ifa4 {
+namespace mass {
+
+// mass[b, g, j] (+)= sum over rows (t, h) of exp(scale q.k + bias - lse).
+//
+// S^T = K Q^T on tcgen05: a tile has 128 keys in the TMEM lanes and kN rows (query tokens x heads of
+// the group) in the columns, so a key's sum over the rows is a sum over one thread's own registers:
+// no shuffles, no atomics, a fixed order.  A CTA works on 256 keys at a time, 128 for each of two
+// warpgroups, which read the same tile of rows:
+//   warp 0      TMA producer: the K tiles of the pair (paged, 128-byte swizzle) and the ring of Q tiles
+//   warp 1      issues the products; scores are double-buffered in TMEM for each warpgroup
+//   warp 2      -lse, position and place of the bias of every row of a Q tile, beside it in the ring
+//   warps 4-11  exponentials and sums; the lane's key stays, the rows stream by
+// A sequence whose rows fit one tile keeps it in shared memory while the keys stream by (single tokens:
+// bound by HBM, 256 bytes a key); otherwise the keys stay and the rows stream by (prompts: bound by
+// the exponentials).
+constexpr int kKeys = 128;
+constexpr uint32_t kKHalf = kKeys * 128;       // 64 dims of a K tile
+constexpr uint32_t kKTile = 2 * kKHalf;        // 128 keys x 256 B
+constexpr int kThreads = 384;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int kN>
+struct Layout {
+  static constexpr int kKStages = kN >= 128 ? 1 : 2;
+  static constexpr int kQStages = kN >= 128 ? 4 : 2;
+  static constexpr uint32_t kQHalf = kN * 128;
+  static constexpr uint32_t kQTile = 2 * kQHalf;
+  static constexpr uint32_t kQ = kKStages * 2 * kKTile;
+  static constexpr uint32_t kMeta = kQ + kQStages * kQTile;
+  static constexpr uint32_t kBar = kMeta + kQStages * kN * 20;
+  static constexpr uint32_t kAlloc = kBar + 256 + 1024;
+  static constexpr uint32_t kTmemCols = 4 * kN;  // two tiles, two buffers
+  static constexpr int kChunk = kN < 32 ? 16 : 32;
+};
+
+template <int kN>
+struct Meta {  // of a Q tile's rows
+  long long rel[kN];   // element offset of the row's bias
+  float nlse[kN];      // -lse * log2(e); -inf: the row adds nothing
+  float lse[kN];
+  int pos[kN];
+};
+
+struct Bars {
+  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_empty[2][2], drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(Bars) <= 256, "barrier block");
+
+// Tiles of rows that see any of the keys [key0, key0 + 256) of a sequence.
+struct Rows {
+  int lo, hi;
+};
+__device__ __forceinline__ Rows rows_of(int key0, int n_q, int n_k, int window, int tokens) {
+  const int shift = n_k - n_q;  // position of token 0
+  int a = max(0, key0 - shift), z = n_q;
+  if (window >= 0) {
+    const long long last = static_cast<long long>(key0) + 2 * kKeys - 1 + window - shift;
+    if (last + 1 < z) z = static_cast<int>(last + 1 > 0 ? last + 1 : 0);
+  }
+  if (key0 >= n_k || a >= z) return {0, 0};
+  return {a / tokens, (z + tokens - 1) / tokens};
+}
+
+template <int kN>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_mass_kernel(const __grid_constant__ AttentionMassKernelArgs a,
+                          const __grid_constant__ CUtensorMap tm_q,
+                          const __grid_constant__ CUtensorMap tm_k) {
+  using L = Layout<kN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + L::kBar);
+  Meta<kN>* meta = reinterpret_cast<Meta<kN>*>(smem + L::kMeta);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y;
+  const int b = blockIdx.z;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kKStages; ++i) {
+      mbar_init(&bars->k_full[i], 1);
+      mbar_init(&bars->k_empty[i], 1);
+    }
+    for (int i = 0; i < L::kQStages; ++i) {
+      mbar_init(&bars->q_full[i], 2);   // TMA and warp 2
+      mbar_init(&bars->q_empty[i], 9);  // the products and the eight warps
+    }
+    for (int w = 0; w < 2; ++w)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bars->s_full[w][i], 1);
+        mbar_init(&bars->s_empty[w][i], 4);
+      }
+    mbar_init(&bars->drain, 1);
+    bars->abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+  }
+  if (warp == 3) {
+    tmem_alloc(&bars->tmem_base, L::kTmemCols);
+    tmem_relinquish();
+  }
+  const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
+  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  const int n_out = min(n_k, a.mass_width);  // keys with a place
+  const int n_pairs = ((a.accumulate ? n_out : a.mass_width) + 2 * kKeys - 1) / (2 * kKeys);
+  const int tokens = a.tokens_per_tile;
+  const bool resident = n_q <= tokens;  // one tile of rows: loaded once
+  const int shift = n_k - n_q;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  const AbortCtx ab{&bars->abort_flag, a.status, kStatusDecodeTimeout};
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    const uint64_t pol_k = resident ? l2_policy_evict_first() : l2_policy_evict_last();
+    const uint64_t pol_q = l2_policy_evict_last();
+    const int box = 1 << a.box_shift;
+    const int units = 2 * kKeys >> a.box_shift;  // of the pair, at most 16
+    const int page_mask = (1 << a.s.page_shift) - 1;
+    const int32_t* table = table_row(a.s, b);
+    const uint32_t q_bytes = 2u * static_cast<uint32_t>(tokens * a.group) * 128u;
+    uint32_t nk = 0, nq = 0;
+    bool ok = true;
+    for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+      const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
+      if (rows.lo >= rows.hi) continue;
+      const int key = kp * 2 * kKeys + lane * box;
+      int page = a.s.num_pages;  // out of range: zeros
+      if (lane < units && key < n_k) {
+        const int p = page_at(a.s, table, key >> a.s.page_shift);
+        if (p >= 0) page = p;
+      }
+      const uint32_t ks = nk % L::kKStages;
+      if (!(ok = mbar_wait_warp(&bars->k_empty[ks], ((nk / L::kKStages) & 1) ^ 1, ab))) break;
+      if (lane == 0) mbar_arrive_expect_tx(&bars->k_full[ks], 2 * kKTile);
+      __syncwarp();
+      if (lane < units) {
+        const int row = lane * box;  // of the pair
+        uint8_t* dst = smem + ks * 2 * kKTile + (row / kKeys) * kKTile + (row % kKeys) * 128;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          tma_load_4d_hint(dst + hf * kKHalf, &tm_k, &bars->k_full[ks], hf * 64, kvh,
+                           key & page_mask, page, pol_k);
+      }
+      ++nk;
+      for (int qt = rows.lo; qt < rows.hi && !(resident && nq > 0); ++qt, ++nq) {
+        const uint32_t qs = nq % L::kQStages;
+        if (!(ok = mbar_wait_warp(&bars->q_empty[qs], ((nq / L::kQStages) & 1) ^ 1, ab))) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->q_full[qs], q_bytes);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_3d_hint(smem + L::kQ + qs * L::kQTile + hf * L::kQHalf, &tm_q,
+                             &bars->q_full[qs], hf * 64, kvh * a.group, q0 + qt * tokens, pol_q);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) {  // every issued load has landed before the CTA may exit
+      for (uint32_t i = 0; i < L::kKStages && i < nk; ++i) {
+        const uint32_t at = nk - 1 - i;
+        mbar_wait(&bars->k_full[at % L::kKStages], (at / L::kKStages) & 1, ab);
+      }
+      for (uint32_t i = 0; i < L::kQStages && i < nq; ++i) {
+        const uint32_t at = nq - 1 - i;
+        mbar_wait(&bars->q_full[at % L::kQStages], (at / L::kQStages) & 1, ab);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_bf16_f32(kKeys, kN, false);
+      uint32_t nk = 0, nq = 0, step = 0;
+      bool ok = true;
+      for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+        const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
+        if (rows.lo >= rows.hi) continue;
+        const uint32_t ks = nk % L::kKStages;
+        if (!(ok = mbar_wait(&bars->k_full[ks], (nk / L::kKStages) & 1, ab))) break;
+        for (int qt = rows.lo; qt < rows.hi; ++qt, ++step) {
+          const uint32_t qs = resident ? 0u : nq % L::kQStages;
+          if (!(resident && nq > 0)) {
+            if (!(ok = mbar_wait(&bars->q_full[qs], (nq / L::kQStages) & 1, ab))) break;
+            ++nq;
+          }
+          const uint32_t buf = step & 1;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (!(ok = ok && mbar_wait(&bars->s_empty[w][buf], ((step >> 1) & 1) ^ 1, ab))) break;
+            tc_fence_after();
+            const uint64_t kd = sdesc_sw128(smem_u32(smem + (ks * 2 + w) * kKTile), 16, 1024);
+            const uint64_t qd = sdesc_sw128(smem_u32(smem + L::kQ + qs * L::kQTile), 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              umma_ss(tbase + (w * 2 + buf) * kN,
+                      sdesc_advance(kd, (kk >> 2) * kKHalf + (kk & 3) * 32),
+                      sdesc_advance(qd, (kk >> 2) * L::kQHalf + (kk & 3) * 32), idesc,
+                      kk > 0 ? 1u : 0u);
+            umma_commit(&bars->s_full[w][buf]);
+          }
+          if (!ok) break;
+          if (!resident) umma_commit(&bars->q_empty[qs]);
+        }
+        if (ok) umma_commit(&bars->k_empty[ks]);
+        ++nk;
+      }
+      umma_commit(&bars->drain);  // every issued product completes before TMEM is released
+      mbar_wait(&bars->drain, 0, ab);
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- the rows of each Q tile
+    uint32_t nq = 0;
+    bool ok = true;
+    for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+      const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
+      for (int qt = rows.lo; qt < rows.hi && !(resident && nq > 0); ++qt, ++nq) {
+        const uint32_t qs = nq % L::kQStages;
+        if (!(ok = mbar_wait_warp(&bars->q_empty[qs], ((nq / L::kQStages) & 1) ^ 1, ab))) break;
+        for (int r = lane; r < kN; r += 32) {
+          const int tok = r / a.group, i = qt * tokens + tok;
+          const int h = kvh * a.group + r - tok * a.group;
+          const bool on = tok < tokens && i < n_q;
+          const long long t = q0 + i;
+          float l = INFINITY;
+          if (on) l = __ldg(a.lse + h * a.lse_sh + t * a.lse_st);
+          meta[qs].nlse[r] = l == -INFINITY ? -INFINITY : -l * kLog2e;  // -inf for +inf, too
+          meta[qs].lse[r] = l;
+          meta[qs].pos[r] = shift + i;
+          meta[qs].rel[r] = on ? t * a.rel_st + h * a.rel_sh : 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->q_full[qs]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------------- exponentials and sums
+    const int w = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16) + w * 2 * kN;
+    const uint64_t mul2 = f2_pack(a.scale_log2, a.scale_log2);
+    constexpr int kC = L::kChunk;
+    uint32_t nq = 0, step = 0;
+    bool ok = true;
+    for (int kp = blockIdx.x; kp < n_pairs; kp += gridDim.x) {
+      const int tile0 = kp * 2 * kKeys + w * kKeys;
+      const int key = tile0 + row;
+      const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
+      uint64_t acc[4] = {0, 0, 0, 0};
+      float edge = 0.f;
+      for (int qt = rows.lo; qt < rows.hi && ok; ++qt, ++step) {
+        const uint32_t qs = resident ? 0u : nq % L::kQStages;
+        const uint32_t buf = step & 1;
+        // the wait on the Q tile makes what warp 2 wrote visible
+        if (!(ok = mbar_wait_warp(&bars->q_full[qs], resident ? 0u : (nq / L::kQStages) & 1, ab)))
+          break;
+        if (!resident) ++nq;
+        if (!(ok = mbar_wait_warp(&bars->s_full[w][buf], (step >> 1) & 1, ab))) break;
+        tc_fence_after();
+        const Meta<kN>& m = meta[qs];
+        const int cols = min(tokens, n_q - qt * tokens) * a.group;
+        const uint32_t t_s = t_lane + buf * kN;
+#pragma unroll 1
+        for (int c0 = 0; c0 < cols; c0 += kC) {
+          // positions of the chunk's first and last row
+          const int p_lo = m.pos[c0], p_hi = m.pos[min(c0 + kC, cols) - 1];
+          if (p_hi < tile0) continue;  // before every key of the tile
+          if (a.window_left >= 0 && p_lo - (tile0 + kKeys - 1) > a.window_left) continue;
+          uint32_t r[kC];
+          if constexpr (kC == 32) tmem_ld32(t_s + c0, r);
+          else tmem_ld16(t_s + c0, r);
+          tmem_wait_ld();
+          const bool inside = c0 + kC <= cols && p_lo - (tile0 + kKeys - 1) >= a.rel_extent &&
+                              (a.window_left < 0 || p_hi - tile0 <= a.window_left);
+          if (inside) {  // every row sees every key, and none through the bias
+#pragma unroll
+            for (int i = 0; i < kC; i += 4) {
+              const float4 nl = *reinterpret_cast<const float4*>(&m.nlse[c0 + i]);
+              float x0, x1, x2, x3;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), mul2,
+                               f2_pack(nl.x, nl.y)), x0, x1);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), mul2,
+                               f2_pack(nl.z, nl.w)), x2, x3);
+              acc[(i >> 1) & 3] = f2_add(acc[(i >> 1) & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
+              acc[((i >> 1) + 1) & 3] =
+                  f2_add(acc[((i >> 1) + 1) & 3], f2_pack(fast_exp2(x2), fast_exp2(x3)));
+            }
+          } else {
+            float bias[kC];
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              bias[i] = 0.f;
+              if (c0 + i < cols) {
+                const int d = m.pos[c0 + i] - key;
+                if (d >= 0 && d < a.rel_extent)
+                  bias[i] = bf16_bits_to_float(__ldg(a.rel + m.rel[c0 + i] + d));
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              if (c0 + i < cols) {
+                const int d = m.pos[c0 + i] - key;
+                // bias - lse first: either may be at the end of the range
+                const float x = __fmaf_rn(bias[i] - m.lse[c0 + i], kLog2e,
+                                          __uint_as_float(r[i]) * a.scale_log2);
+                if (d >= 0 && (a.window_left < 0 || d <= a.window_left) &&
+                    m.nlse[c0 + i] != -INFINITY)
+                  edge += fast_exp2(x);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->s_empty[w][buf]);
+          if (!resident) mbar_arrive(&bars->q_empty[qs]);
+        }
+      }
+      float s0, s1;
+      f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
+      const float sum = s0 + s1 + edge;
+      if (ok && key < a.mass_width && IFA4_DBG_CHECK(a.status, b < a.s.batch)) {
+        float* dst = a.mass + static_cast<long long>(b) * a.mass_sb +
+                     static_cast<long long>(kvh) * a.mass_sh + key;
+        if (!a.accumulate) *dst = key < n_out ? sum : 0.f;
+        else if (key < n_out && rows.lo < rows.hi) *dst += sum;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 3) tmem_dealloc(tbase, L::kTmemCols);
+}
+
+template <int kN>
+cudaError_t launch(const AttentionMassKernelArgs& args, const CUtensorMap& tm_q,
+                   const CUtensorMap& tm_k, int key_blocks, cudaStream_t stream) {
+  static std::atomic<bool> attr[64];
+  cudaError_t e = set_smem_limit_once(attention_mass_kernel<kN>, Layout<kN>::kAlloc, attr);
+  if (e != cudaSuccess) return e;
+  attention_mass_kernel<kN><<<dim3(key_blocks, args.kv_heads, args.s.batch), kThreads,
+                              Layout<kN>::kAlloc, stream>>>(args, tm_q, tm_k);
+  return cudaGetLastError();
+}
+
+}  // namespace mass
+
+namespace evict {
+
+// ---------------------------------------------------------------------------------------
+// What stays
+// ---------------------------------------------------------------------------------------
+// A block per sequence and KV head: the border of the masses (see select_largest), then the places
+// that stay, in order, with their masses.
+constexpr int kSelectThreads = 1024;
+
+__global__ void __launch_bounds__(kSelectThreads)
+    kv_evict_select_kernel(const __grid_constant__ KvEvictKernelArgs a) {
+  __shared__ SelectSmem<kSelectThreads> sm;
+  const int g = blockIdx.x, b = blockIdx.y;
+  if (g == 0 && b == 0 && threadIdx.x == 0) {
+    int sum = 0, at = __ldg(a.s.cu_k);
+    a.cu_out[0] = 0;
+    for (int i = 0; i < a.s.batch; ++i) {
+      const int end = __ldg(a.s.cu_k + i + 1);
+      sum += max(0, min(end - at, a.budget));
+      at = end;
+      a.cu_out[i + 1] = sum;
+    }
+  }
+  const int n = max(0, __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b));
+  const float* mass = a.mass + static_cast<long long>(b) * a.mass_sb +
+                      static_cast<long long>(g) * a.mass_sh;
+  float* mass_out = a.mass_out + static_cast<long long>(b) * a.mo_sb +
+                    static_cast<long long>(g) * a.mo_sh;
+  int32_t* kept = a.kept + (static_cast<long long>(b) * a.kv_heads + g) * a.budget;
+  const auto mass_of = [&](int i) { return i < a.mass_width ? mass[i] : 0.f; };
+  const auto keep = [&](int place, int i) {
+    kept[place] = i;
+    if (place < a.mass_width) mass_out[place] = mass_of(i);
+  };
+  int stay = n;
+  if (n <= a.budget) {
+    for (int i = threadIdx.x; i < n; i += kSelectThreads) keep(i, i);
+  } else {
+    // -inf ranks below every other mass here, but can be kept
+    stay = select_largest<kSelectThreads>(
+        sm, n, a.budget,
+        [&](int i) {
+          if (i < a.first || i >= n - a.recent) return kAlways;
+          return max(rank_of(mass_of(i)), 1u);
+        },
+        keep);
+  }
+  for (int i = stay + threadIdx.x; i < a.budget; i += kSelectThreads) kept[i] = -1;
+  for (int i = stay + threadIdx.x; i < a.mass_width; i += kSelectThreads) mass_out[i] = 0.f;
+}
+
+// ---------------------------------------------------------------------------------------
+// Its move to the front
+// ---------------------------------------------------------------------------------------
+// A block per sequence and KV head goes through the kept keys in order.  Key `place` comes from
+// kept[place] >= place, so what a stretch writes has been read: by this stretch, before the barrier,
+// or by an earlier one.
+constexpr int kMoveThreads = 512;
+constexpr int kMoveRows = 64;  // K and V rows of a stretch
+
+__global__ void __launch_bounds__(kMoveThreads)
+    kv_evict_move_kernel(const __grid_constant__ KvEvictKernelArgs a) {
+  const int g = blockIdx.x, b = blockIdx.y;
+  const int n = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  if (n <= a.budget) return;
+  const int32_t* kept = a.kept + (static_cast<long long>(b) * a.kv_heads + g) * a.budget;
+  const int32_t* table = table_row(a.s, b);
+  const int mask = (1 << a.s.page_shift) - 1;
+  const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;  // 32 rows at a time
+  constexpr int kTurns = kMoveRows / (kMoveThreads / 16);
+  for (int base = 0; base < a.budget; base += kMoveRows) {
+    uint4 k[kTurns], v[kTurns];
+    int to[kTurns];  // page of the destination, -1: nothing to write
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int place = base + sub + i * (kMoveThreads / 16);
+      const int from = place < a.budget ? kept[place] : place;
+      to[i] = from != place ? page_at(a.s, table, place >> a.s.page_shift) : -1;
+      k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (to[i] >= 0) {
+        const int page = page_at(a.s, table, from >> a.s.page_shift);
+        if (page >= 0) {
+          const long long slot = from & mask;
+          k[i] = *reinterpret_cast<const uint4*>(a.k_cache + page * a.k_sp + slot * a.k_st +
+                                                 g * a.k_sh + part * 8);
+          v[i] = *reinterpret_cast<const uint4*>(a.v_cache + page * a.v_sp + slot * a.v_st +
+                                                 g * a.v_sh + part * 8);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      if (to[i] >= 0) {
+        const long long slot = (base + sub + i * (kMoveThreads / 16)) & mask;
+        *reinterpret_cast<uint4*>(a.k_cache + to[i] * a.k_sp + slot * a.k_st + g * a.k_sh +
+                                  part * 8) = k[i];
+        *reinterpret_cast<uint4*>(a.v_cache + to[i] * a.v_sp + slot * a.v_st + g * a.v_sh +
+                                  part * 8) = v[i];
+      }
+    }
+  }
+}
+
+}  // namespace evict
+
+int attention_mass_tile_rows(long long rows, int group) {
+  int n = 16;
+  while (n < 128 && (n < rows || n < group)) n *= 2;
+  return n;
+}
+
+cudaError_t launch_attention_mass_sm100(const AttentionMassKernelArgs& args, int tile_rows,
+                                        const CUtensorMap& tm_q, const CUtensorMap& tm_k,
+                                        int key_blocks, cudaStream_t stream) {
+  switch (tile_rows) {
+    case 16: return mass::launch<16>(args, tm_q, tm_k, key_blocks, stream);
+    case 32: return mass::launch<32>(args, tm_q, tm_k, key_blocks, stream);
+    case 64: return mass::launch<64>(args, tm_q, tm_k, key_blocks, stream);
+    default: return mass::launch<128>(args, tm_q, tm_k, key_blocks, stream);
+  }
+}
+
+cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, cudaStream_t stream) {
+  const dim3 grid(args.kv_heads, args.s.batch);
+  evict::kv_evict_select_kernel<<<grid, evict::kSelectThreads, 0, stream>>>(args);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  evict::kv_evict_move_kernel<<<grid, evict::kMoveThreads, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+}  // namespace ifa4

@@ -1,0 +1,713 @@
+// Sparse attention over the pages of a paged cache, for sm_100a: bounds of a page's keys, scores of
+// pages for a query, the choice of pages, and attention over the chosen ones.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "ifa4_internal.h"
+#include "ifa4_paged.cuh"
+#include "ifa4_ptx.cuh"
+
+namespace ifa4 {
+namespace sparse {
+
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) {
+  return *reinterpret_cast<__nv_bfloat162*>(&x);
+}
+__device__ __forceinline__ uint32_t min_bf162(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hmin2_nan(as_bf162(a), as_bf162(b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max_bf162(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hmax2_nan(as_bf162(a), as_bf162(b));
+  return *reinterpret_cast<uint32_t*>(&r);
+}
+__device__ __forceinline__ uint4 min_v4(uint4 a, uint4 b) {
+  return make_uint4(min_bf162(a.x, b.x), min_bf162(a.y, b.y), min_bf162(a.z, b.z),
+                    min_bf162(a.w, b.w));
+}
+__device__ __forceinline__ uint4 max_v4(uint4 a, uint4 b) {
+  return make_uint4(max_bf162(a.x, b.x), max_bf162(a.y, b.y), max_bf162(a.z, b.z),
+                    max_bf162(a.w, b.w));
+}
+__device__ __forceinline__ uint4 shfl_xor_v4(uint4 v, int m) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, m), __shfl_xor_sync(0xffffffffu, v.y, m),
+                    __shfl_xor_sync(0xffffffffu, v.z, m), __shfl_xor_sync(0xffffffffu, v.w, m));
+}
+
+// ---------------------------------------------------------------------------------------
+// Bounds of pages
+// ---------------------------------------------------------------------------------------
+// A warp per page and KV head: half a warp reads a key (16 bytes a lane), eight keys of each half in
+// flight; the halves are joined at the end, one writes the minima, the other the maxima (512
+// contiguous bytes).  Bound by HBM: 256 bytes a key and head read, 512 a page and head written.
+__global__ void __launch_bounds__(kPageBoundsWarps * 32)
+    page_bounds_kernel(const __grid_constant__ PageBoundsKernelArgs a) {
+  const int lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
+  const int b = blockIdx.y;
+  const int n_q = __ldg(a.s.cu_q + b + 1) - __ldg(a.s.cu_q + b);
+  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  if (n_q <= 0 || n_k <= 0) return;
+  const int ps = 1 << a.s.page_shift;
+  const int c0 = max(0, n_k - n_q) >> a.s.page_shift;
+  const int pages = ((n_k - 1) >> a.s.page_shift) - c0 + 1;
+  const int32_t* row = table_row(a.s, b);
+  const long long units = static_cast<long long>(pages) * a.kv_heads;
+  const long long stride = static_cast<long long>(gridDim.x) * kPageBoundsWarps;
+  for (long long u = static_cast<long long>(blockIdx.x) * kPageBoundsWarps + (threadIdx.x >> 5);
+       u < units; u += stride) {
+    const int c = c0 + static_cast<int>(u / a.kv_heads), h = static_cast<int>(u % a.kv_heads);
+    const int page = page_at(a.s, row, c);
+    if (page < 0) continue;
+    const int keys = min(ps, n_k - (c << a.s.page_shift));
+    const uint16_t* src = a.k_cache + static_cast<long long>(page) * a.k_sp +
+                          static_cast<long long>(h) * a.k_sh + part * 8;
+    uint4 lo, hi;
+    lo = hi = *reinterpret_cast<const uint4*>(src);  // key 0 is always there
+    for (int r0 = half; r0 < keys; r0 += 16) {
+      uint4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // past the last key: that key once more
+        const int r = min(r0 + 2 * i, keys - 1);
+        x[i] = *reinterpret_cast<const uint4*>(src + static_cast<long long>(r) * a.k_st);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        lo = min_v4(lo, x[i]);
+        hi = max_v4(hi, x[i]);
+      }
+    }
+    lo = min_v4(lo, shfl_xor_v4(lo, 16));
+    hi = max_v4(hi, shfl_xor_v4(hi, 16));
+    uint16_t* dst = a.bounds + static_cast<long long>(page) * a.b_sp +
+                    static_cast<long long>(h) * a.b_sh + half * 128 + part * 8;
+    *reinterpret_cast<uint4*>(dst) = half ? hi : lo;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Scores of pages
+// ---------------------------------------------------------------------------------------
+// sum_i (max(q_i, 0) max_i + min(q_i, 0) min_i) is a matrix product of depth 256 with the bounds as
+// they lie in memory, and runs on warp-level MMAs (16 rows: the heads of a group, of 16 / group
+// tokens; 8 pages a warp).  The order of the 128 dims is free as long as both operands have the same:
+// lane qd of a quad takes 16 contiguous bytes of every 64, so the bounds go from global memory to the
+// fragments without shared memory, eight 16-byte loads a lane in flight.  Bound by HBM: 512 bytes a
+// page and head for 16 rows.
+constexpr int kScoreWarps = 4;
+constexpr int kScorePages = 128;  // pages of a block: 4 groups of 8 a warp
+
+__device__ __forceinline__ float max_nan(float x, float y) { return y > x || y != y ? y : x; }
+
+__global__ void __launch_bounds__(kScoreWarps * 32)
+    page_scores_kernel(const __grid_constant__ PageScoresKernelArgs a) {
+  __shared__ float tile[kScoreWarps][16][9];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
+  const int page0 = blockIdx.x * kScorePages;
+  const int kvh = blockIdx.y % a.kv_heads;
+  const int rb0 = blockIdx.y / a.kv_heads;
+  const int b = blockIdx.z;
+  const int width = a.s.table_width;
+  const int page1 = min(width, page0 + kScorePages);
+  if (b == a.s.batch) {  // rows of no sequence
+    const long long t0 = max(0, __ldg(a.s.cu_q + a.s.batch));
+    for (long long t = t0 + rb0; t < a.total_q; t += a.row_blocks)
+      for (int c = page0 + threadIdx.x; c < page1; c += kScoreWarps * 32)
+        a.scores[t * a.sc_st + kvh * a.sc_sh + c] = -INFINITY;
+    return;
+  }
+  const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
+  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  const int hb = min(a.group, 16);          // heads of a row block
+  const int tokens = 16 / hb;               // and tokens
+  const int32_t* table = table_row(a.s, b);
+  const int ps = 1 << a.s.page_shift;
+  for (int rb = rb0; rb * tokens < n_q; rb += a.row_blocks) {
+    const int tok0 = rb * tokens;
+    const int n_tok = min(tokens, n_q - tok0);
+    const int p0 = n_k - n_q + tok0;  // position of the block's first token
+    for (int c0 = page0 + warp * 8; c0 < page1; c0 += kScoreWarps * 8) {
+      // visible pages of any token of the block
+      const int first_key = a.window_left < 0 ? 0 : max(0, p0 - a.window_left);
+      const int last_key = p0 + n_tok - 1;
+      const bool any = last_key >= 0 && c0 <= last_key >> a.s.page_shift &&
+                       c0 + 7 >= first_key >> a.s.page_shift;
+      float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // outputs lane, lane + 32, ..
+      if (any) {
+        uint4 bound[8];  // maxima of 4 x 32 dims, then minima
+        const int page = page_at(a.s, table, c0 + g);
+        const uint16_t* src = a.bounds + static_cast<long long>(max(page, 0)) * a.b_sp +
+                              static_cast<long long>(kvh) * a.b_sh + qd * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          bound[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (page >= 0) bound[i] = ldg_nc_v4(src + (i < 4 ? 128 : 0) + (i & 3) * 32);
+        }
+        for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
+          const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint16_t* qrow[2];
+          const uint16_t* relrow[2];
+          int pos[2];
+          bool on[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
+            on[r] = row < n_rows;
+            const int tok = a.group <= 16 ? row / hb : 0;
+            const int head = kvh * a.group + (a.group <= 16 ? row - tok * hb : h0 + row);
+            const long long t = q0 + tok0 + (on[r] ? tok : 0);
+            pos[r] = p0 + tok;
+            qrow[r] = a.q + t * a.q_st + static_cast<long long>(on[r] ? head : 0) * a.q_sh + qd * 8;
+            relrow[r] = a.rel + t * a.rel_st + static_cast<long long>(on[r] ? head : 0) * a.rel_sh;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint4 x[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              x[r] = make_uint4(0u, 0u, 0u, 0u);
+              if (on[r]) x[r] = ldg_nc_v4(qrow[r] + i * 32);
+            }
+            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+            const uint4 p[2] = {max_v4(x[0], z), max_v4(x[1], z)};
+            const uint4 m[2] = {min_v4(x[0], z), min_v4(x[1], z)};
+            const uint32_t pa[4] = {p[0].x, p[1].x, p[0].y, p[1].y};
+            const uint32_t pb[4] = {p[0].z, p[1].z, p[0].w, p[1].w};
+            const uint32_t ma[4] = {m[0].x, m[1].x, m[0].y, m[1].y};
+            const uint32_t mb[4] = {m[0].z, m[1].z, m[0].w, m[1].w};
+            mma_bf16(acc, pa, bound[i].x, bound[i].y);
+            mma_bf16(acc, pb, bound[i].z, bound[i].w);
+            mma_bf16(acc, ma, bound[4 + i].x, bound[4 + i].y);
+            mma_bf16(acc, mb, bound[4 + i].z, bound[4 + i].w);
+          }
+          // bias bound and mask of (row, page): acc[2 r + e] is row g + 8 r, page 2 qd + e
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = c0 + 2 * qd + e;
+              float x = -INFINITY;
+              if (on[r] && pos[r] >= 0 && c <= pos[r] >> a.s.page_shift) {
+                const int key0 = c << a.s.page_shift;
+                const int d0 = max(0, pos[r] - (key0 + ps - 1));  // nearest key of the page
+                int d1 = pos[r] - key0;                           // and the furthest
+                if (a.window_left >= 0) d1 = min(d1, a.window_left);
+                if (d0 <= d1) {
+                  float bias = d1 >= a.rel_extent ? 0.f : -INFINITY;
+                  for (int d = d0; d <= min(d1, a.rel_extent - 1); ++d)
+                    bias = max_nan(bias, bf16_bits_to_float(__ldg(relrow[r] + d)));
+                  x = acc[2 * r + e] * a.scale + bias;
+                }
+              }
+              tile[warp][g + 8 * r][2 * qd + e] = x;
+            }
+          __syncwarp();
+          // largest over the heads of a token: output o is token o / 8, page o % 8
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int tok = (lane + 32 * k) >> 3, pg = lane & 7;
+            const int heads = a.group <= 16 ? hb : n_rows;
+            if (tok < n_tok)
+              for (int r = 0; r < heads; ++r) best[k] = max_nan(best[k], tile[warp][tok * heads + r][pg]);
+          }
+          __syncwarp();
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int tok = (lane + 32 * k) >> 3, c = c0 + (lane & 7);
+        if (tok < n_tok && c < width) {
+          const int p = p0 + tok;
+          float x = best[k];
+          if (p >= 0) {
+            const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> a.s.page_shift;
+            const int hi = p >> a.s.page_shift;
+            if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages)) x = INFINITY;
+          }
+          a.scores[(q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c] = x;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Choice of pages
+// ---------------------------------------------------------------------------------------
+// A block per row and KV head (see select_largest).
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
+    select_pages_kernel(const __grid_constant__ SelectPagesKernelArgs a) {
+  __shared__ SelectSmem<kThreads> sm;
+  const int g = blockIdx.y;
+  for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) {
+    const float* src = a.scores + t * a.sc_st + g * a.sc_sh;
+    int32_t* dst = a.pages + t * a.pg_st + g * a.pg_sh;
+    const int n = select_largest<kThreads>(
+        sm, a.width, a.count, [&](int i) { return rank_of(src[i]); },
+        [&](int place, int i) { dst[place] = i; });
+    for (int i = n + threadIdx.x; i < a.count; i += kThreads) dst[i] = -1;
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Attention over chosen pages
+// ---------------------------------------------------------------------------------------
+// The streaming decode with the keys of a list: a CTA takes tiles of 64 keys of one row's list for up
+// to 16 query heads of one KV head.  Warp 4 follows the list and the block table and loads the tiles'
+// units (min(page_size, 64) rows) by TMA into a ring; warps 0 to 3 take 16 keys of every tile, which
+// always lie in one page (page_size >= 16), so a warp reads one list entry per tile.  Units and slices
+// without a visible key are neither loaded nor computed.  Bound by HBM: 512 bytes a key and KV head.
+constexpr int kTileKeys = 64;
+constexpr int kStages = 3;
+constexpr int kConsumerWarps = 4;
+constexpr int kThreads = (kConsumerWarps + 1) * 32;
+constexpr uint32_t kHalf = kTileKeys * 128;   // 64 rows x 128 B
+constexpr uint32_t kKVTile = 2 * kHalf;       // 64 keys x 256 B
+constexpr uint32_t kStageBytes = 2 * kKVTile;
+constexpr uint32_t kSmemBar = kStages * kStageBytes;
+constexpr uint32_t kSmemAlloc = kSmemBar + 128 + 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct Bars {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  int abort_flag;
+  int last;  // last entry of the list with a visible key
+};
+static_assert(sizeof(Bars) <= 128, "barrier block");
+
+__device__ __forceinline__ uint32_t sw128_addr(uint32_t base, int row, int chunk) {
+  return base + (chunk >> 3) * kHalf + row * 128 + ((((chunk & 7) ^ (row & 7))) << 4);
+}
+
+// x + bias in log2 units.  A bias at the end of bf16's range passes fp32's there: the sum stays finite,
+// so that a row whose keys all have the lowest one is their mean, as the formula says.
+__device__ __forceinline__ float add_bias(float x, float bias) {
+  const float y = __fmaf_rn(bias, kLog2e, x);
+  return isinf(y) && isfinite(bias) && isfinite(x) ? copysignf(3.402823466e38f, y) : y;
+}
+
+__global__ void __launch_bounds__(kThreads, 2)
+    decode_pages_kernel(const __grid_constant__ DecodePagesKernelArgs a,
+                        const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Bars* bars = reinterpret_cast<Bars*>(smem + kSmemBar);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const long long t = blockIdx.x / a.num_splits;
+  const int split = static_cast<int>(blockIdx.x - t * a.num_splits);
+  const int head_blocks = (a.group + a.heads_per_cta - 1) / a.heads_per_cta;
+  const int kvh = blockIdx.y / head_blocks;
+  const int hblk = blockIdx.y % head_blocks;
+  const int h0 = kvh * a.group + hblk * a.heads_per_cta;
+  const int nh = min(a.heads_per_cta, a.group - hblk * a.heads_per_cta);
+  if (a.num_splits > 1) launch_dependents();
+  const int b = find_sequence(a.s.cu_q, a.s.batch, t);
+  if (b < 0) {
+    if (a.num_splits > 1) return;  // the merge writes such rows
+    if (!a.zero_padding) return;
+    for (int i = threadIdx.x; i < nh * 128; i += kThreads)
+      a.out[t * a.out_st + static_cast<long long>(h0 + (i >> 7)) * a.out_sh + (i & 127)] = 0;
+    if (a.lse != nullptr && threadIdx.x < nh)
+      a.lse[static_cast<long long>(h0 + threadIdx.x) * a.lse_sh + t * a.lse_st] = -INFINITY;
+    return;
+  }
+  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  const int pos = n_k - __ldg(a.s.cu_q + b + 1) + static_cast<int>(t);
+  const int hi = pos + 1;  // visible keys [lo, hi); none where hi <= 0
+  const int lo = a.window_left >= 0 ? max(0, pos - a.window_left) : 0;
+  const int c_lo = lo >> a.s.page_shift, c_hi = hi > 0 ? pos >> a.s.page_shift : -1;
+  const int32_t* list = a.pages + t * a.pg_st + kvh * a.pg_sh;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], kConsumerWarps);
+    }
+    bars->abort_flag = 0;
+    bars->last = -1;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  {
+    int last = -1;
+    for (int e = threadIdx.x; e < a.num_selected; e += kThreads) {
+      const int c = __ldg(list + e);
+      if (c >= c_lo && c <= c_hi) last = e;
+    }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0 && last >= 0) atomicMax(&bars->last, last);
+  }
+  __syncthreads();
+  const int last = bars->last;
+  const AbortCtx ab{&bars->abort_flag, a.status, kStatusDecodeTimeout};
+  const int ps = 1 << a.s.page_shift, page_mask = ps - 1;
+  const long long keys = static_cast<long long>(last + 1) << a.s.page_shift;
+  const int tiles = static_cast<int>((keys + kTileKeys - 1) / kTileKeys);
+  const int per = (tiles + a.num_splits - 1) / a.num_splits;
+  const int t_lo = split * per, t_hi = min(tiles, t_lo + per);
+
+  float m_r[2] = {-INFINITY, -INFINITY};
+  float l_r[2] = {0.f, 0.f};
+  float o[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+  if (warp == kConsumerWarps) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+    const uint64_t pol = l2_policy_evict_first();
+    const int box = 1 << a.box_shift;
+    const int units = kTileKeys >> a.box_shift;
+    const int32_t* table = table_row(a.s, b);
+    // page of unit `lane` of a tile: -2 nothing to load, num_pages reads zeros
+    auto unit_page = [&](int tile) {
+      const long long vk = static_cast<long long>(tile) * kTileKeys + lane * box;
+      const int e = static_cast<int>(vk >> a.s.page_shift);
+      int page = -2;
+      if (lane < units && e <= last) {
+        const int c = __ldg(list + e);
+        if (c >= c_lo && c <= c_hi) {
+          const int key0 = (c << a.s.page_shift) + (static_cast<int>(vk) & page_mask);
+          if (key0 < hi && key0 + box > lo) {
+            page = page_at(a.s, table, c);
+            if (page < 0) page = a.s.num_pages;
+          }
+        }
+      }
+      return page;
+    };
+    uint32_t n = 0;
+    int page = t_lo < t_hi ? unit_page(t_lo) : -2;
+    for (int tile = t_lo; tile < t_hi; ++tile, ++n) {
+      const int next = tile + 1 < t_hi ? unit_page(tile + 1) : -2;  // in flight across the wait
+      const uint32_t st = n % kStages;
+      if (!mbar_wait_warp(&bars->empty[st], ((n / kStages) & 1) ^ 1, ab)) break;
+      const uint32_t loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&bars->full[st], loads * box * 512u);
+      __syncwarp();
+      if (page >= 0) {
+        uint8_t* base = smem + st * kStageBytes + lane * box * 128;
+        const int in_page = static_cast<int>(static_cast<long long>(tile) * kTileKeys + lane * box) &
+                            page_mask;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          tma_load_4d_hint(base + hf * kHalf, &tm_k, &bars->full[st], hf * 64, kvh, in_page, page,
+                           pol);
+          tma_load_4d_hint(base + kKVTile + hf * kHalf, &tm_v, &bars->full[st], hf * 64, kvh,
+                           in_page, page, pol);
+        }
+      }
+      page = next;
+    }
+    if (lane == 0) {  // every issued load has landed before the CTA may exit
+      for (uint32_t i = 0; i < kStages && i < n; ++i) {
+        const uint32_t at = n - 1 - i;
+        mbar_wait(&bars->full[at % kStages], (at / kStages) & 1, ab);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- consumers
+    const int g = lane >> 2;
+    const int qd = lane & 3;
+    uint32_t qa[8][4];
+    const uint32_t* qrow0 = reinterpret_cast<const uint32_t*>(
+        a.q + t * a.q_st + static_cast<long long>(h0 + g) * a.q_sh);
+    const uint32_t* qrow1 = reinterpret_cast<const uint32_t*>(
+        a.q + t * a.q_st + static_cast<long long>(h0 + g + 8) * a.q_sh);
+    const bool r0v = g < nh, r1v = g + 8 < nh;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      qa[kk][0] = r0v ? __ldg(qrow0 + kk * 8 + qd) : 0u;
+      qa[kk][1] = r1v ? __ldg(qrow1 + kk * 8 + qd) : 0u;
+      qa[kk][2] = r0v ? __ldg(qrow0 + kk * 8 + 4 + qd) : 0u;
+      qa[kk][3] = r1v ? __ldg(qrow1 + kk * 8 + 4 + qd) : 0u;
+    }
+    const uint16_t* relr[2];
+    relr[0] = a.rel + t * a.rel_st + static_cast<long long>(h0 + g) * a.rel_sh;
+    relr[1] = a.rel + t * a.rel_st + static_cast<long long>(h0 + g + 8) * a.rel_sh;
+    const int wrow = warp * 16;  // this warp's 16 keys within the tile
+    // list entry of this warp's slice
+    auto entry = [&](int tile) {
+      const long long vk = static_cast<long long>(tile) * kTileKeys + wrow;
+      const int e = static_cast<int>(vk >> a.s.page_shift);
+      return e <= last ? __ldg(list + e) : -1;
+    };
+    uint32_t n = 0;
+    int c = t_lo < t_hi ? entry(t_lo) : -1;
+    for (int tile = t_lo; tile < t_hi; ++tile, ++n) {
+      const int next = tile + 1 < t_hi ? entry(tile + 1) : -1;
+      const uint32_t st = n % kStages;
+      if (!mbar_wait_warp(&bars->full[st], (n / kStages) & 1, ab)) break;
+      int kt = hi;  // position of the slice's first key
+      if (c >= c_lo && c <= c_hi)
+        kt = (c << a.s.page_shift) +
+             (static_cast<int>(static_cast<long long>(tile) * kTileKeys + wrow) & page_mask);
+      c = next;
+      if (kt < hi && kt + 16 > lo) {
+        const uint32_t kbase = smem_u32(smem + st * kStageBytes);
+        const uint32_t vbase = kbase + kKVTile;
+        // ---- S = Q K^T for 16 keys (two n8 tiles)
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        {
+          const int mi = lane >> 3;
+          const int krow = wrow + (mi >> 1) * 8 + (lane & 7);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4(sw128_addr(kbase, krow, 2 * kk + (mi & 1)), b0, b1, b2, b3);
+            mma_bf16(s[0], qa[kk], b0, b1);
+            mma_bf16(s[1], qa[kk], b2, b3);
+          }
+        }
+        // ---- scale, bias, mask
+        float x[2][2][2];  // [row r][ntile][e]
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[0][nt][e] = s[nt][e] * a.scale_log2;
+            x[1][nt][e] = s[nt][2 + e] * a.scale_log2;
+          }
+        if (pos - (kt + 15) < a.rel_extent) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (!(r == 0 ? r0v : r1v)) continue;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int d = pos - (kt + nt * 8 + 2 * qd + e);
+                if (d >= 0 && d < a.rel_extent)
+                  x[r][nt][e] = add_bias(x[r][nt][e], bf16_bits_to_float(__ldg(relr[r] + d)));
+              }
+          }
+        }
+        // masked keys may hold anything: their scores are replaced and their values zeroed (0 * NaN
+        // would reach the sum); this lane's V fragments hold keys 2 qd (+1) and 8 + 2 qd (+1)
+        uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
+        if (kt < lo || kt + 16 > hi) {
+          vm0 = vm1 = 0u;
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = kt + nt * 8 + 2 * qd + e;
+              if (key < lo || key >= hi) x[0][nt][e] = x[1][nt][e] = -INFINITY;
+              else (nt == 0 ? vm0 : vm1) |= e == 0 ? 0x0000ffffu : 0xffff0000u;
+            }
+        }
+        // ---- online softmax per row
+        uint32_t pa[4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float mt = fmaxf(fmaxf(x[r][0][0], x[r][0][1]), fmaxf(x[r][1][0], x[r][1][1]));
+          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+          mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+          const float m_new = fmaxf(m_r[r], mt);
+          const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_r[r] - m_new);
+          const float m_use = m_new == -INFINITY ? 0.f : m_new;
+          m_r[r] = m_new;
+          const float p00 = fast_exp2(x[r][0][0] - m_use), p01 = fast_exp2(x[r][0][1] - m_use);
+          const float p10 = fast_exp2(x[r][1][0] - m_use), p11 = fast_exp2(x[r][1][1] - m_use);
+          l_r[r] = l_r[r] * alpha + (p00 + p01 + p10 + p11);
+#pragma unroll
+          for (int dt = 0; dt < 16; ++dt) {
+            o[dt][2 * r] *= alpha;
+            o[dt][2 * r + 1] *= alpha;
+          }
+          // P is rounded to bf16 for the product with V, as in the other attention kernels; the sum
+          // has the unrounded values
+          pa[r] = pack_bf16x2(p00, p01);
+          pa[2 + r] = pack_bf16x2(p10, p11);
+        }
+        __syncwarp();
+        {
+          const int mi = lane >> 3;
+          const int vrow = wrow + (mi & 1) * 8 + (lane & 7);
+#pragma unroll
+          for (int dt = 0; dt < 16; dt += 2) {
+            uint32_t b0, b1, b2, b3;
+            ldsm_x4_t(sw128_addr(vbase, vrow, dt + (mi >> 1)), b0, b1, b2, b3);
+            b0 &= vm0;
+            b1 &= vm1;
+            b2 &= vm0;
+            b3 &= vm1;
+            mma_bf16(o[dt], pa, b0, b1);
+            mma_bf16(o[dt + 1], pa, b2, b3);
+          }
+        }
+      }
+      // the fragment loads have to be done, not only issued, before TMA refills the stage
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->empty[st]);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l_r[r] += __shfl_xor_sync(0xffffffffu, l_r[r], 1);
+      l_r[r] += __shfl_xor_sync(0xffffffffu, l_r[r], 2);
+    }
+  }
+
+  // ------------------------------------------------------------------ merge the 4 warps
+  __syncthreads();  // all TMA traffic has landed and all stages are consumed
+  float* mo = reinterpret_cast<float*>(smem);      // [4][16][128]
+  float* mm = mo + kConsumerWarps * 16 * 128;      // [4][16]
+  float* ml = mm + kConsumerWarps * 16;            // [4][16]
+  if (warp < kConsumerWarps) {
+    const int g = lane >> 2, qd = lane & 3;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + 8 * r;
+      if (row >= nh) break;
+      if (qd == 0) {
+        mm[warp * 16 + row] = m_r[r];
+        ml[warp * 16 + row] = l_r[r];
+      }
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt) {
+        mo[(warp * 16 + row) * 128 + dt * 8 + 2 * qd] = o[dt][2 * r];
+        mo[(warp * 16 + row) * 128 + dt * 8 + 2 * qd + 1] = o[dt][2 * r + 1];
+      }
+    }
+  }
+  __syncthreads();
+  // one warp per row, lanes own 4 of the 128 dims
+  for (int row = warp; row < nh; row += kConsumerWarps + 1) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kConsumerWarps; ++w) M = fmaxf(M, mm[w * 16 + row]);
+    const float base = M == -INFINITY ? 0.f : M;  // no score above -inf: sums are 0, or NaN
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kConsumerWarps; ++w) {
+      const float m = mm[w * 16 + row];
+      const float f = m == -INFINITY ? (ml[w * 16 + row] == 0.f ? 0.f : 1.f) : fast_exp2(m - base);
+      const float4 o4 = reinterpret_cast<const float4*>(mo + (w * 16 + row) * 128)[lane];
+      L += ml[w * 16 + row] * f;
+      acc.x += o4.x * f;
+      acc.y += o4.y * f;
+      acc.z += o4.z * f;
+      acc.w += o4.w * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // NaN stays
+    const float lse2 = L == 0.f ? -INFINITY : base + __log2f(L);
+    const int h = h0 + row;
+    acc.x *= inv;
+    acc.y *= inv;
+    acc.z *= inv;
+    acc.w *= inv;
+    if (!IFA4_DBG_CHECK(a.status, t < a.total_q && h < a.n_heads)) {
+      // a bad row or head: nothing is stored
+    } else if (a.num_splits == 1) {
+      *reinterpret_cast<uint2*>(a.out + t * a.out_st + static_cast<long long>(h) * a.out_sh +
+                                lane * 4) =
+          make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+      if (lane == 0 && a.lse != nullptr)
+        a.lse[static_cast<long long>(h) * a.lse_sh + t * a.lse_st] = lse2 * kLn2;
+    } else {
+      const long long at = (t * a.n_heads + h) * a.num_splits + split;
+      reinterpret_cast<float4*>(a.ws_o + at * 128)[lane] = acc;
+      if (lane == 0) reinterpret_cast<float2*>(a.ws_ml)[at] = make_float2(L == 0.f ? -INFINITY : base, L);
+    }
+  }
+}
+
+// Merge of num_splits normalised partials: a warp per row and head, weights L_s 2^(m_s - max m).
+constexpr int kMergeWarps = 4;
+__global__ void __launch_bounds__(kMergeWarps * 32)
+    decode_pages_merge_kernel(const __grid_constant__ DecodePagesKernelArgs a) {
+  const int lane = threadIdx.x & 31;
+  const long long at = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
+  if (at >= a.total_q * a.n_heads) return;
+  const long long t = at / a.n_heads;
+  const int h = static_cast<int>(at - t * a.n_heads);
+  const bool none = find_sequence(a.s.cu_q, a.s.batch, t) < 0;
+  if (none && !a.zero_padding) return;
+  wait_previous_kernel();
+  float M = -INFINITY, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (!none) {
+    const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + at * a.num_splits;
+    for (int s = 0; s < a.num_splits; ++s) M = fmaxf(M, ml[s].x);
+    if (M != -INFINITY) {
+      for (int s = 0; s < a.num_splits; ++s) {
+        const float2 p = ml[s];
+        const float w = p.x == -INFINITY ? 0.f : p.y * fast_exp2(p.x - M);  // NaN stays
+        const float4 o4 = reinterpret_cast<const float4*>(a.ws_o + (at * a.num_splits + s) * 128)[lane];
+        L += w;
+        acc.x += w * o4.x;
+        acc.y += w * o4.y;
+        acc.z += w * o4.z;
+        acc.w += w * o4.w;
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2*>(a.out + t * a.out_st + static_cast<long long>(h) * a.out_sh + lane * 4) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[static_cast<long long>(h) * a.lse_sh + t * a.lse_st] =
+        L == 0.f ? -INFINITY : (M + __log2f(L)) * kLn2;
+}
+
+}  // namespace sparse
+
+cudaError_t launch_page_bounds_sm100(const PageBoundsKernelArgs& args, int blocks_per_seq,
+                                     cudaStream_t stream) {
+  sparse::page_bounds_kernel<<<dim3(blocks_per_seq, args.s.batch), kPageBoundsWarps * 32, 0,
+                               stream>>>(args);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream) {
+  const dim3 grid((args.s.table_width + sparse::kScorePages - 1) / sparse::kScorePages,
+                  args.kv_heads * args.row_blocks, args.s.batch + (args.zero_padding ? 1 : 0));
+  sparse::page_scores_kernel<<<grid, sparse::kScoreWarps * 32, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_select_pages_sm100(const SelectPagesKernelArgs& args, cudaStream_t stream) {
+  const long long most = 1 << 20;
+  const dim3 grid(static_cast<unsigned>(args.rows < most ? args.rows : most), args.kv_heads);
+  if (args.width > 4096)
+    sparse::select_pages_kernel<1024><<<grid, 1024, 0, stream>>>(args);
+  else
+    sparse::select_pages_kernel<256><<<grid, 256, 0, stream>>>(args);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const CUtensorMap& tm_k,
+                                      const CUtensorMap& tm_v, cudaStream_t stream) {
+  static std::atomic<bool> attr[64];
+  cudaError_t e = set_smem_limit_once(sparse::decode_pages_kernel, sparse::kSmemAlloc, attr);
+  if (e != cudaSuccess) return e;
+  const int head_blocks = (args.group + args.heads_per_cta - 1) / args.heads_per_cta;
+  const dim3 grid(static_cast<unsigned>(args.total_q * args.num_splits),
+                  args.kv_heads * head_blocks);
+  sparse::decode_pages_kernel<<<grid, sparse::kThreads, sparse::kSmemAlloc, stream>>>(args, tm_k,
+                                                                                      tm_v);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || args.num_splits == 1) return e;
+  const long long warps = args.total_q * args.n_heads;
+  return launch_early(sparse::decode_pages_merge_kernel,
+                      dim3(static_cast<unsigned>((warps + sparse::kMergeWarps - 1) /
+                                                 sparse::kMergeWarps)),
+                      sparse::kMergeWarps * 32, 0, stream, args);
+}
+
+}  // namespace ifa4

@@ -558,6 +558,303 @@ Tensors bucket_bias_backward_op(const at::Tensor& drel, const at::Tensor& starts
   return {dtable};
 }
 
+// A paged cache or the bounds of its pages: [pages, .., 128] bf16, 16-byte aligned, unit last stride,
+// other strides positive multiples of 8.
+bool plain_pages(const at::Tensor& t, const at::Tensor& like) {
+  if (!t.is_cuda() || t.dim() != 4 || t.size(3) != 128 || t.stride(3) != 1 || t.size(0) < 1 ||
+      t.size(2) < 1 || t.scalar_type() != at::kBFloat16 || t.device() != like.device() ||
+      !aligned16(t))
+    return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.stride(i) <= 0 || t.stride(i) % 8 != 0) return false;
+  return true;
+}
+bool plain_page_size(int64_t n) { return n >= 16 && n <= (1 << 20) && (n & (n - 1)) == 0; }
+// Offsets and block table of a batch.
+bool plain_seqs(const at::Tensor& like, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                const at::Tensor& block_table, int64_t page_size) {
+  return plain_cu(cu_q, like) && plain_cu(cu_k, like) && cu_q.numel() == cu_k.numel() &&
+         cu_q.numel() <= 65535 && plain_page_size(page_size) && block_table.dim() == 2 &&
+         block_table.scalar_type() == at::kInt && block_table.device() == like.device() &&
+         block_table.size(0) == cu_q.numel() - 1 && block_table.size(1) >= 1 &&
+         block_table.size(1) <= (1 << 26) && block_table.stride(1) == 1 &&
+         block_table.stride(0) >= 0;
+}
+IFA4PagedSeqs seqs_of(const at::Tensor& cu_q, const at::Tensor& cu_k, const at::Tensor& block_table,
+                      int64_t page_size, int64_t num_pages) {
+  IFA4PagedSeqs s{};
+  s.cu_seqlens_q = static_cast<const int32_t*>(cu_q.data_ptr());
+  s.cu_seqlens_k = static_cast<const int32_t*>(cu_k.data_ptr());
+  s.block_table = static_cast<const int32_t*>(block_table.data_ptr());
+  s.block_table_stride = block_table.stride(0);
+  s.batch = static_cast<int32_t>(cu_q.numel() - 1);
+  s.page_size = static_cast<int32_t>(page_size);
+  s.num_pages = static_cast<int32_t>(num_pages);
+  s.table_width = static_cast<int32_t>(block_table.size(1));
+  return s;
+}
+// Queries with their bias, for the groups of kv_heads.
+bool plain_queries(const at::Tensor& q, const at::Tensor& rel, int64_t kv_heads, int64_t rel_extent,
+                   double softmax_scale) {
+  return plain_rows(q, q) && q.stride(0) > 0 && q.stride(1) > 0 && q.size(1) % kv_heads == 0 &&
+         q.size(1) >= 1 && q.size(1) <= 65535 && rel.dim() == 3 &&
+         rel.scalar_type() == at::kBFloat16 && rel.device() == q.device() &&
+         rel.size(0) == q.size(0) && rel.size(1) == q.size(1) && rel.stride(2) == 1 &&
+         rel.stride(0) >= 0 && rel.stride(1) >= 0 && rel_extent >= 1 &&
+         rel_extent <= rel.size(2) && softmax_scale > 0;
+}
+bool plain_int(int64_t x) { return x >= -1 && x <= 0x7fffffff; }
+
+// Returns bounds.
+Tensors page_bounds_op(const at::Tensor& k_cache, const at::Tensor& bounds,
+                       const at::Tensor& block_table, const at::Tensor& cu_q,
+                       const at::Tensor& cu_k, int64_t max_seqlen_q) {
+  if (!plain_pages(k_cache, k_cache) || !plain_pages(bounds, k_cache) ||
+      bounds.size(0) != k_cache.size(0) || bounds.size(1) != k_cache.size(2) ||
+      bounds.size(2) != 2 || bounds.stride(2) != 128 || !plain_int(max_seqlen_q) ||
+      !plain_seqs(k_cache, cu_q, cu_k, block_table, k_cache.size(1)))
+    return {};
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  IFA4PageBoundsParams p{};
+  p.seqs = seqs_of(cu_q, cu_k, block_table, k_cache.size(1), k_cache.size(0));
+  p.k_cache = k_cache.data_ptr();
+  p.bounds = bounds.data_ptr();
+  p.k_stride_page = k_cache.stride(0);
+  p.k_stride_t = k_cache.stride(1);
+  p.k_stride_h = k_cache.stride(2);
+  p.bounds_stride_page = bounds.stride(0);
+  p.bounds_stride_h = bounds.stride(1);
+  p.kv_heads = static_cast<int32_t>(k_cache.size(2));
+  p.head_dim = 128;
+  p.dtype = IFA4_DTYPE_BF16;
+  p.max_seqlen_q = static_cast<int32_t>(max_seqlen_q);
+  if (ifa4_page_bounds_launch(&p, stream_of(k_cache))) return {};
+  written(bounds);
+  return {bounds};
+}
+
+// Returns the scores.
+Tensors page_scores_op(const at::Tensor& q, const at::Tensor& bounds, const at::Tensor& rel,
+                       const at::Tensor& cu_q, const at::Tensor& cu_k,
+                       const at::Tensor& block_table, int64_t max_seqlen_q, int64_t rel_extent,
+                       int64_t page_size, int64_t window_left, double softmax_scale,
+                       int64_t first_pages, int64_t last_pages) {
+  if (!q.is_cuda() || !plain_pages(bounds, q) || bounds.size(2) != 2 || bounds.stride(2) != 128 ||
+      !plain_queries(q, rel, bounds.size(1), rel_extent, softmax_scale) ||
+      !plain_seqs(q, cu_q, cu_k, block_table, page_size) || !plain_int(max_seqlen_q) ||
+      !plain_int(window_left) || first_pages < 0 || first_pages > 0x7fffffff || last_pages < 0 ||
+      last_pages > 0x7fffffff)
+    return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor scores =
+      new_tensor({q.size(0), bounds.size(1), block_table.size(1)}, at::kFloat, q);
+  IFA4PageScoresParams p{};
+  p.seqs = seqs_of(cu_q, cu_k, block_table, page_size, bounds.size(0));
+  p.q = q.data_ptr();
+  p.bounds = bounds.data_ptr();
+  p.rel = rel.data_ptr();
+  p.scores = static_cast<float*>(scores.data_ptr());
+  p.q_stride_t = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.bounds_stride_page = bounds.stride(0);
+  p.bounds_stride_h = bounds.stride(1);
+  p.rel_stride_t = rel.stride(0);
+  p.rel_stride_h = rel.stride(1);
+  p.scores_stride_t = scores.stride(0);
+  p.scores_stride_h = scores.stride(1);
+  p.total_q = q.size(0);
+  p.n_heads = static_cast<int32_t>(q.size(1));
+  p.kv_heads = static_cast<int32_t>(bounds.size(1));
+  p.head_dim = 128;
+  p.rel_extent = static_cast<int32_t>(rel_extent);
+  p.window_left = static_cast<int32_t>(window_left);
+  p.max_seqlen_q = static_cast<int32_t>(max_seqlen_q);
+  p.first_pages = static_cast<int32_t>(first_pages);
+  p.last_pages = static_cast<int32_t>(last_pages);
+  p.zero_padding = 1;
+  p.dtype = IFA4_DTYPE_BF16;
+  p.softmax_scale = static_cast<float>(softmax_scale);
+  if (ifa4_page_scores_launch(&p, stream_of(q))) return {};
+  return {scores};
+}
+
+// Returns the pages.
+Tensors select_pages_op(const at::Tensor& scores, int64_t num_selected) {
+  if (!scores.is_cuda() || scores.dim() != 3 || scores.scalar_type() != at::kFloat ||
+      (scores.size(2) > 1 && scores.stride(2) != 1) || scores.stride(0) < 0 ||
+      scores.stride(1) < 0 || scores.size(1) > 65535 || scores.size(2) > (1 << 26) ||
+      num_selected < 1 || num_selected > (1 << 26))
+    return {};
+  const c10::cuda::CUDAGuard guard(scores.device());
+  const at::Tensor pages =
+      new_tensor({scores.size(0), scores.size(1), num_selected}, at::kInt, scores);
+  IFA4SelectPagesParams p{};
+  p.scores = static_cast<const float*>(scores.data_ptr());
+  p.pages = static_cast<int32_t*>(pages.data_ptr());
+  p.scores_stride_t = scores.stride(0);
+  p.scores_stride_h = scores.stride(1);
+  p.pages_stride_t = pages.stride(0);
+  p.pages_stride_h = pages.stride(1);
+  p.rows = scores.size(0);
+  p.kv_heads = static_cast<int32_t>(scores.size(1));
+  p.width = static_cast<int32_t>(scores.size(2));
+  p.num_selected = static_cast<int32_t>(num_selected);
+  if (ifa4_select_pages_launch(&p, stream_of(scores))) return {};
+  return {pages};
+}
+
+// Returns out.
+Tensors decode_pages_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                        const at::Tensor& rel, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                        const at::Tensor& pages, const at::Tensor& block_table,
+                        const MaybeTensor& workspace, int64_t rel_extent, int64_t window_left,
+                        int64_t max_seqlen_k, double softmax_scale, int64_t num_splits) {
+  if (!q.is_cuda() || !plain_pages(k, q) || !plain_pages(v, q) || v.sizes() != k.sizes() ||
+      !plain_queries(q, rel, k.size(2), rel_extent, softmax_scale) ||
+      !plain_seqs(q, cu_q, cu_k, block_table, k.size(1)) || !plain_int(window_left) ||
+      !plain_int(max_seqlen_k) || !plain_int(num_splits) || pages.dim() != 3 ||
+      pages.scalar_type() != at::kInt || pages.device() != q.device() ||
+      pages.size(0) != q.size(0) || pages.size(1) != k.size(2) || pages.size(2) > (1 << 26) ||
+      (pages.size(2) > 1 && pages.stride(2) != 1) || pages.stride(0) < 0 || pages.stride(1) < 0 ||
+      (workspace.has_value() &&
+       (workspace->device() != q.device() || !workspace->is_contiguous() || !aligned16(*workspace))))
+    return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor out = rows_like(q);
+  IFA4DecodePagesParams p{};
+  p.decode = decode_params(q, k, v, rel, out, cu_q, cu_k, c10::nullopt, block_table, rel_extent,
+                           true, window_left, IFA4_ALIGN_BOTTOM_RIGHT, max_seqlen_k, softmax_scale,
+                           num_splits, 0);
+  p.pages = static_cast<const int32_t*>(pages.data_ptr());
+  p.pages_stride_t = pages.stride(0);
+  p.pages_stride_h = pages.stride(1);
+  p.num_selected = static_cast<int32_t>(pages.size(2));
+  p.table_width = static_cast<int32_t>(block_table.size(1));
+  p.zero_padding = 1;
+  size_t need = 0;
+  if (ifa4_decode_pages_workspace_size(&p, &need)) return {};
+  at::Tensor ws;
+  if (need > 0)
+    ws = workspace.has_value() && static_cast<size_t>(workspace->nbytes()) >= need
+             ? *workspace : bytes_like(q, need);
+  if (ifa4_decode_pages_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(q)))
+    return {};
+  return {out};
+}
+
+// Returns the masses (`mass`, or a new tensor as wide as the table).
+Tensors attention_mass_op(const at::Tensor& q, const at::Tensor& k, const at::Tensor& rel,
+                          const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                          const at::Tensor& block_table, const MaybeTensor& mass,
+                          int64_t rel_extent, int64_t window_left, int64_t max_seqlen_q,
+                          int64_t max_seqlen_k, double softmax_scale) {
+  if (!q.is_cuda() || !plain_pages(k, q) ||
+      !plain_queries(q, rel, k.size(2), rel_extent, softmax_scale) || q.size(1) / k.size(2) > 128 ||
+      !plain_seqs(q, cu_q, cu_k, block_table, k.size(1)) || !plain_int(window_left) ||
+      !plain_int(max_seqlen_q) || !plain_int(max_seqlen_k) || lse.dim() != 2 ||
+      lse.scalar_type() != at::kFloat || lse.device() != q.device() || lse.size(0) != q.size(1) ||
+      lse.size(1) != q.size(0) || block_table.size(1) * k.size(1) > (1 << 30))
+    return {};
+  const int64_t batch = cu_q.numel() - 1, kv_heads = k.size(2);
+  if (mass.has_value() &&
+      (mass->dim() != 3 || mass->scalar_type() != at::kFloat || mass->device() != q.device() ||
+       mass->size(0) != batch || mass->size(1) != kv_heads || mass->size(2) > (1 << 30) ||
+       (mass->size(2) > 1 && mass->stride(2) != 1) || mass->stride(0) < mass->size(2) ||
+       mass->stride(1) < mass->size(2) || !mass->is_non_overlapping_and_dense()))
+    return {};
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor out =
+      mass.has_value() ? *mass
+                       : new_tensor({batch, kv_heads, block_table.size(1) * k.size(1)}, at::kFloat, q);
+  IFA4AttentionMassParams p{};
+  p.seqs = seqs_of(cu_q, cu_k, block_table, k.size(1), k.size(0));
+  p.q = q.data_ptr();
+  p.k_cache = k.data_ptr();
+  p.rel = rel.data_ptr();
+  p.lse = static_cast<const float*>(lse.data_ptr());
+  p.mass = static_cast<float*>(out.data_ptr());
+  p.q_stride_t = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.k_stride_page = k.stride(0);
+  p.k_stride_t = k.stride(1);
+  p.k_stride_h = k.stride(2);
+  p.rel_stride_t = rel.stride(0);
+  p.rel_stride_h = rel.stride(1);
+  p.lse_stride_h = lse.stride(0);
+  p.lse_stride_t = lse.stride(1);
+  p.mass_stride_b = out.stride(0);
+  p.mass_stride_h = out.stride(1);
+  p.total_q = q.size(0);
+  p.n_heads = static_cast<int32_t>(q.size(1));
+  p.kv_heads = static_cast<int32_t>(kv_heads);
+  p.head_dim = 128;
+  p.rel_extent = static_cast<int32_t>(rel_extent);
+  p.window_left = static_cast<int32_t>(window_left);
+  p.max_seqlen_q = static_cast<int32_t>(max_seqlen_q);
+  p.max_seqlen_k = static_cast<int32_t>(max_seqlen_k);
+  p.mass_width = static_cast<int32_t>(out.size(2));
+  p.accumulate = mass.has_value();
+  p.dtype = IFA4_DTYPE_BF16;
+  p.softmax_scale = static_cast<float>(softmax_scale);
+  if (ifa4_attention_mass_launch(&p, stream_of(q))) return {};
+  if (mass.has_value()) written(out);
+  return {out};
+}
+
+// Returns kept, the masses of what is kept and the new offsets.
+Tensors kv_evict_op(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& mass,
+                    const at::Tensor& block_table, const at::Tensor& cu_k, int64_t budget,
+                    int64_t first, int64_t recent) {
+  if (!plain_pages(k_cache, k_cache) || !plain_pages(v_cache, k_cache) ||
+      v_cache.sizes() != k_cache.sizes() || v_cache.data_ptr() == k_cache.data_ptr() ||
+      !plain_seqs(k_cache, cu_k, cu_k, block_table, k_cache.size(1)) || mass.dim() != 3 ||
+      mass.scalar_type() != at::kFloat || mass.device() != k_cache.device() ||
+      mass.size(0) != cu_k.numel() - 1 || mass.size(1) != k_cache.size(2) || mass.size(2) < 1 ||
+      mass.size(2) > (1 << 30) || mass.stride(2) != 1 || mass.stride(0) < 0 || mass.stride(1) < 0 ||
+      budget < 1 || budget > (1 << 30) || first < 0 || recent < 0 || first > budget ||
+      recent > budget - first)
+    return {};
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const int64_t batch = cu_k.numel() - 1, kv_heads = k_cache.size(2);
+  const at::Tensor kept = new_tensor({batch, kv_heads, budget}, at::kInt, k_cache);
+  const at::Tensor left = new_tensor(mass.sizes(), at::kFloat, k_cache);
+  const at::Tensor cu_out = new_tensor({batch + 1}, at::kInt, k_cache);
+  IFA4KvEvictParams p{};
+  p.seqs = seqs_of(cu_k, cu_k, block_table, k_cache.size(1), k_cache.size(0));
+  p.k_cache = k_cache.data_ptr();
+  p.v_cache = v_cache.data_ptr();
+  p.mass = static_cast<const float*>(mass.data_ptr());
+  p.mass_out = static_cast<float*>(left.data_ptr());
+  p.kept = static_cast<int32_t*>(kept.data_ptr());
+  p.cu_out = static_cast<int32_t*>(cu_out.data_ptr());
+  p.k_stride_page = k_cache.stride(0);
+  p.k_stride_t = k_cache.stride(1);
+  p.k_stride_h = k_cache.stride(2);
+  p.v_stride_page = v_cache.stride(0);
+  p.v_stride_t = v_cache.stride(1);
+  p.v_stride_h = v_cache.stride(2);
+  p.mass_stride_b = mass.stride(0);
+  p.mass_stride_h = mass.stride(1);
+  p.mass_out_stride_b = left.stride(0);
+  p.mass_out_stride_h = left.stride(1);
+  p.kv_heads = static_cast<int32_t>(kv_heads);
+  p.head_dim = 128;
+  p.mass_width = static_cast<int32_t>(mass.size(2));
+  p.budget = static_cast<int32_t>(budget);
+  p.first = static_cast<int32_t>(first);
+  p.recent = static_cast<int32_t>(recent);
+  p.dtype = IFA4_DTYPE_BF16;
+  size_t need = 0;
+  if (ifa4_kv_evict_workspace_size(&p, &need)) return {};
+  at::Tensor ws;
+  if (need > 0) ws = bytes_like(k_cache, need);
+  if (ifa4_kv_evict_launch(&p, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(k_cache)))
+    return {};
+  written(k_cache);
+  written(v_cache);
+  return {kept, left, cu_out};
+}
+
 // ---------------------------------------------------------------------------------------------
 // The same as Python functions: positional arguments; a tuple of tensors, or None.
 // ---------------------------------------------------------------------------------------------
@@ -718,6 +1015,79 @@ PyObject* py_bucket_bias_backward(PyObject*, PyObject* const* objects, Py_ssize_
   });
 }
 
+PyObject* py_page_bounds(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::page_bounds", objects, count, [](Arguments& a) {
+    auto k_cache = a.tensor(), bounds = a.tensor(), block_table = a.tensor();
+    auto cu_q = a.tensor(), cu_k = a.tensor();
+    const int64_t max_seqlen_q = a.integer();
+    return [=] { return page_bounds_op(k_cache, bounds, block_table, cu_q, cu_k, max_seqlen_q); };
+  });
+}
+
+PyObject* py_page_scores(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::page_scores", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), bounds = a.tensor(), rel = a.tensor();
+    auto cu_q = a.tensor(), cu_k = a.tensor(), block_table = a.tensor();
+    const int64_t max_seqlen_q = a.integer(), rel_extent = a.integer(), page_size = a.integer();
+    const int64_t window_left = a.integer();
+    const double softmax_scale = a.real();
+    const int64_t first_pages = a.integer(), last_pages = a.integer();
+    return [=] {
+      return page_scores_op(q, bounds, rel, cu_q, cu_k, block_table, max_seqlen_q, rel_extent,
+                            page_size, window_left, softmax_scale, first_pages, last_pages);
+    };
+  });
+}
+
+PyObject* py_select_pages(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::select_pages", objects, count, [](Arguments& a) {
+    auto scores = a.tensor();
+    const int64_t num_selected = a.integer();
+    return [=] { return select_pages_op(scores, num_selected); };
+  });
+}
+
+PyObject* py_decode_pages(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::decode_pages", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), k = a.tensor(), v = a.tensor(), rel = a.tensor();
+    auto cu_q = a.tensor(), cu_k = a.tensor(), pages = a.tensor(), block_table = a.tensor();
+    auto workspace = a.maybe();
+    const int64_t rel_extent = a.integer(), window_left = a.integer(), max_seqlen_k = a.integer();
+    const double softmax_scale = a.real();
+    const int64_t num_splits = a.integer();
+    return [=] {
+      return decode_pages_op(q, k, v, rel, cu_q, cu_k, pages, block_table, workspace, rel_extent,
+                             window_left, max_seqlen_k, softmax_scale, num_splits);
+    };
+  });
+}
+
+PyObject* py_attention_mass(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::attention_mass", objects, count, [](Arguments& a) {
+    auto q = a.tensor(), k = a.tensor(), rel = a.tensor(), lse = a.tensor();
+    auto cu_q = a.tensor(), cu_k = a.tensor(), block_table = a.tensor();
+    auto mass = a.maybe();
+    const int64_t rel_extent = a.integer(), window_left = a.integer();
+    const int64_t max_seqlen_q = a.integer(), max_seqlen_k = a.integer();
+    const double softmax_scale = a.real();
+    return [=] {
+      return attention_mass_op(q, k, rel, lse, cu_q, cu_k, block_table, mass, rel_extent,
+                               window_left, max_seqlen_q, max_seqlen_k, softmax_scale);
+    };
+  });
+}
+
+PyObject* py_kv_evict(PyObject*, PyObject* const* objects, Py_ssize_t count) {
+  return call("inkling_fa4::kv_evict", objects, count, [](Arguments& a) {
+    auto k_cache = a.tensor(), v_cache = a.tensor(), mass = a.tensor();
+    auto block_table = a.tensor(), cu_k = a.tensor();
+    const int64_t budget = a.integer(), first = a.integer(), recent = a.integer();
+    return [=] {
+      return kv_evict_op(k_cache, v_cache, mass, block_table, cu_k, budget, first, recent);
+    };
+  });
+}
+
 template <class F>
 PyMethodDef method(const char* name, F* f) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL,
@@ -730,6 +1100,12 @@ PyMethodDef kMethods[] = {
     method("decode_shared_prefix", py_decode_shared_prefix),
     method("bucket_bias", py_bucket_bias),
     method("bucket_bias_backward", py_bucket_bias_backward),
+    method("page_bounds", py_page_bounds),
+    method("page_scores", py_page_scores),
+    method("select_pages", py_select_pages),
+    method("decode_pages", py_decode_pages),
+    method("attention_mass", py_attention_mass),
+    method("kv_evict", py_kv_evict),
 };
 }  // namespace
 

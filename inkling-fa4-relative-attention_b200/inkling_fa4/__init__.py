@@ -8,7 +8,10 @@ statement for tests) and ``autotune_configs``; beyond the reference, the backwar
 fused ``rel_logits`` producer (``inkling_rel_logits``) and the learned bias by distance buckets
 (``inkling_bucket_bias``), the norm and rotation of queries and keys (``inkling_qk_norm_rope``), the
 append to the paged cache (``inkling_kv_append``) and decode for a batch that shares a prefix
-(``inkling_fa4_rel_attention_decode_shared_prefix``).  The kernels are hand-written CUDA for sm_100a
+(``inkling_fa4_rel_attention_decode_shared_prefix``); for long contexts, sparse attention over chosen
+pages (``inkling_kv_page_bounds``, ``inkling_kv_page_scores``, ``inkling_kv_select_pages``,
+``inkling_fa4_rel_attention_decode_pages``) and eviction by attention weight
+(``inkling_kv_attention_mass``, ``inkling_kv_evict``).  The kernels are hand-written CUDA for sm_100a
 behind the C ABI of include/inkling_fa4.h; there is no Triton and no CPU fallback.
 """
 from .triton_kernel import inkling_fa4_rel_attention_triton
@@ -21,6 +24,9 @@ from .qk_norm_rope import (inkling_kv_append, inkling_qk_norm_rope, inkling_qk_n
 from .shared_prefix import inkling_fa4_rel_attention_decode_shared_prefix
 from .bucket_bias import (inkling_bucket_bias, inkling_bucket_bias_backward,
                           relative_bucket_starts)
+from .page_sparse import (inkling_fa4_rel_attention_decode_pages, inkling_kv_page_bounds,
+                          inkling_kv_page_scores, inkling_kv_select_pages)
+from .kv_evict import inkling_kv_attention_mass, inkling_kv_evict
 
 __all__ = [
     "inkling_fa4_rel_attention_triton",
@@ -37,4 +43,10 @@ __all__ = [
     "inkling_bucket_bias",
     "inkling_bucket_bias_backward",
     "relative_bucket_starts",
+    "inkling_kv_page_bounds",
+    "inkling_kv_page_scores",
+    "inkling_kv_select_pages",
+    "inkling_fa4_rel_attention_decode_pages",
+    "inkling_kv_attention_mass",
+    "inkling_kv_evict",
 ]

@@ -26,7 +26,7 @@ IFA4_DTYPE_BF16 = 0
 IFA4_WEIGHT_BF16 = 0
 IFA4_WEIGHT_F32 = 1
 MAX_BUCKETS = 1024
-ABI_VERSION = 8
+ABI_VERSION = 9
 MAX_OUT_PEERS = 7
 MAX_KV_SPLITS = 16
 NOALLOC_DECODE_SCRATCH_BYTES = 16 * 1024 * 1024
@@ -50,6 +50,14 @@ EXPORTED_SYMBOLS = (
     "ifa4_bucket_bias_launch",
     "ifa4_bucket_bias_backward_launch",
     "ifa4_bucket_bias_backward_workspace_size",
+    "ifa4_page_bounds_launch",
+    "ifa4_page_scores_launch",
+    "ifa4_select_pages_launch",
+    "ifa4_decode_pages_launch",
+    "ifa4_decode_pages_workspace_size",
+    "ifa4_attention_mass_launch",
+    "ifa4_kv_evict_launch",
+    "ifa4_kv_evict_workspace_size",
     "ifa4_read_device_status",
     "ifa4_selftest_bounded_wait",
     "ifa4_measure_read_stream",
@@ -190,6 +198,70 @@ class BucketBiasBackwardParams(ctypes.Structure):
                                        "weight_dtype")]
 
 
+def _fields(pointers=(), int64=(), int32=(), float32=()):
+    return [(n, t) for names, t in ((pointers, ctypes.c_void_p), (int64, ctypes.c_int64),
+                                    (int32, ctypes.c_int32), (float32, ctypes.c_float))
+            for n in names]
+
+
+class PagedSeqs(ctypes.Structure):
+    """Mirror of ``IFA4PagedSeqs``."""
+    _fields_ = _fields(("cu_seqlens_q", "cu_seqlens_k", "block_table"), ("block_table_stride",),
+                       ("batch", "page_size", "num_pages", "table_width"))
+
+
+class PageBoundsParams(ctypes.Structure):
+    """Mirror of ``IFA4PageBoundsParams``."""
+    _fields_ = [("seqs", PagedSeqs)] + _fields(
+        ("k_cache", "bounds"),
+        ("k_stride_page", "k_stride_t", "k_stride_h", "bounds_stride_page", "bounds_stride_h"),
+        ("kv_heads", "head_dim", "dtype", "max_seqlen_q"))
+
+
+class PageScoresParams(ctypes.Structure):
+    """Mirror of ``IFA4PageScoresParams``."""
+    _fields_ = [("seqs", PagedSeqs)] + _fields(
+        ("q", "bounds", "rel", "scores"),
+        ("q_stride_t", "q_stride_h", "bounds_stride_page", "bounds_stride_h", "rel_stride_t",
+         "rel_stride_h", "scores_stride_t", "scores_stride_h", "total_q"),
+        ("n_heads", "kv_heads", "head_dim", "rel_extent", "window_left", "max_seqlen_q",
+         "first_pages", "last_pages", "zero_padding", "dtype"), ("softmax_scale",))
+
+
+class SelectPagesParams(ctypes.Structure):
+    """Mirror of ``IFA4SelectPagesParams``."""
+    _fields_ = _fields(("scores", "pages"),
+                       ("scores_stride_t", "scores_stride_h", "pages_stride_t", "pages_stride_h",
+                        "rows"), ("kv_heads", "width", "num_selected"))
+
+
+class DecodePagesParams(ctypes.Structure):
+    """Mirror of ``IFA4DecodePagesParams``."""
+    _fields_ = [("decode", DecodeParams)] + _fields(
+        ("pages",), ("pages_stride_t", "pages_stride_h"),
+        ("num_selected", "table_width", "zero_padding"))
+
+
+class AttentionMassParams(ctypes.Structure):
+    """Mirror of ``IFA4AttentionMassParams``."""
+    _fields_ = [("seqs", PagedSeqs)] + _fields(
+        ("q", "k_cache", "rel", "lse", "mass"),
+        ("q_stride_t", "q_stride_h", "k_stride_page", "k_stride_t", "k_stride_h", "rel_stride_t",
+         "rel_stride_h", "lse_stride_h", "lse_stride_t", "mass_stride_b", "mass_stride_h",
+         "total_q"),
+        ("n_heads", "kv_heads", "head_dim", "rel_extent", "window_left", "max_seqlen_q",
+         "max_seqlen_k", "mass_width", "accumulate", "dtype"), ("softmax_scale",))
+
+
+class KvEvictParams(ctypes.Structure):
+    """Mirror of ``IFA4KvEvictParams``."""
+    _fields_ = [("seqs", PagedSeqs)] + _fields(
+        ("k_cache", "v_cache", "mass", "mass_out", "kept", "cu_out"),
+        ("k_stride_page", "k_stride_t", "k_stride_h", "v_stride_page", "v_stride_t", "v_stride_h",
+         "mass_stride_b", "mass_stride_h", "mass_out_stride_b", "mass_out_stride_h"),
+        ("kv_heads", "head_dim", "mass_width", "budget", "first", "recent", "dtype"))
+
+
 class Ifa4Error(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"inkling_fa4 error {code}: {message}")
@@ -269,12 +341,15 @@ def lib() -> ctypes.CDLL:
     L.ifa4_rel_logits_launch.restype = ctypes.c_int
     for name, params in (("decode_shared_prefix", SharedPrefixParams),
                          ("qk_norm_rope_backward", QkNormRopeBackwardParams),
-                         ("bucket_bias_backward", BucketBiasBackwardParams)):
+                         ("bucket_bias_backward", BucketBiasBackwardParams),
+                         ("decode_pages", DecodePagesParams), ("kv_evict", KvEvictParams)):
         launch, size = getattr(L, f"ifa4_{name}_launch"), getattr(L, f"ifa4_{name}_workspace_size")
         launch.argtypes, launch.restype = [ctypes.POINTER(params), vp, sz, vp], ctypes.c_int
         size.argtypes, size.restype = [ctypes.POINTER(params), ctypes.POINTER(sz)], ctypes.c_int
     for name, params in (("qk_norm_rope", QkNormRopeParams), ("kv_append", KvAppendParams),
-                         ("bucket_bias", BucketBiasParams)):
+                         ("bucket_bias", BucketBiasParams), ("page_bounds", PageBoundsParams),
+                         ("page_scores", PageScoresParams), ("select_pages", SelectPagesParams),
+                         ("attention_mass", AttentionMassParams)):
         launch = getattr(L, f"ifa4_{name}_launch")
         launch.argtypes, launch.restype = [ctypes.POINTER(params), vp], ctypes.c_int
     L.ifa4_selftest_bounded_wait.argtypes = [ctypes.c_int64, vp]

@@ -30,7 +30,7 @@ OUT_DEBUG = os.path.join(PKG_DIR, "_lib", "libinkling_fa4_debug.so")
 OUT_TORCH_OPS = os.path.join(PKG_DIR, "_lib", "libifa4_torch_ops.so")
 SOURCES = ["ifa4_capi.cu", "ifa4_prefill_sm100.cu", "ifa4_decode_sm100.cu", "ifa4_backward_sm100.cu",
            "ifa4_rel_logits_sm100.cu", "ifa4_qkv_sm100.cu", "ifa4_shared_prefix_sm100.cu",
-           "ifa4_bucket_bias_sm100.cu"]
+           "ifa4_bucket_bias_sm100.cu", "ifa4_page_sparse_sm100.cu", "ifa4_kv_evict_sm100.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
