@@ -2015,6 +2015,7 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
     const int64_t want = ceil_div(4 * sms, int64_t{p->kv_heads} * p->seqs.batch);
     if (blocks > want) blocks = want;
   }
+  if (blocks > 65535) blocks = 65535;
   cudaError_t e = ifa4::launch_attention_mass_sm100(a, rows, tq, tk, static_cast<int>(blocks),
                                                     static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "attention_mass launch");

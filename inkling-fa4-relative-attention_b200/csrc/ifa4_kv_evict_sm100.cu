@@ -29,8 +29,9 @@ namespace mass {
 constexpr int kKeys = 128;
 constexpr uint32_t kKHalf = kKeys * 128;       // 64 dims of a K tile
 constexpr uint32_t kKTile = 2 * kKHalf;        // 128 keys x 256 B
-constexpr int kThreads = 384;
 constexpr float kLog2e = 1.4426950408889634f;
+
+constexpr uint32_t kBarBytes = 2560;
 
 template <int kN>
 struct Layout {
@@ -42,9 +43,12 @@ struct Layout {
   static constexpr uint32_t kCols = kQ + kQStages * kQTile;
   static constexpr uint32_t kSums = kCols + kN * 12;
   static constexpr uint32_t kBar = kSums + kQStages * kN * 8;
-  static constexpr uint32_t kAlloc = kBar + 256 + 1024;
+  static constexpr uint32_t kAlloc = kBar + kBarBytes + 1024;
   static constexpr uint32_t kTmemCols = 4 * kN;  // two tiles, two buffers
-  static constexpr int kChunk = kN < 32 ? 16 : 32;
+  // Warpgroups that share a tile's columns: two where the exponentials bound the kernel
+  static constexpr int kSplit = kN >= 128 ? 2 : 1;
+  static constexpr int kThreads = 128 + kSplit * 256;
+  static constexpr int kChunk = kN < 32 || kSplit > 1 ? 16 : 32;
 };
 
 // Rows of a Q tile: what they all have in common with the rows of every other tile, and their lse.
@@ -63,8 +67,10 @@ struct Bars {
   uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_empty[2][2], drain;
   uint32_t tmem_base;
   int abort_flag;
+  float half[2][2][kKeys];  // sums of the second half of the columns: pair parity, tile, key
 };
-static_assert(sizeof(Bars) <= 256, "barrier block");
+
+static_assert(sizeof(Bars) <= kBarBytes, "barrier block");
 
 // Tiles of rows that see any of the keys [key0, key0 + 256) of a sequence.
 struct Rows {
@@ -96,10 +102,12 @@ __device__ __forceinline__ void load_if(uint16_t& x, const uint16_t* p, bool on)
       : "l"(p), "r"(static_cast<int>(on)));
 }
 
-// acc += 2^(scale s + nlse) over a chunk of columns.
+// acc += 2^(scale s + nlse) over a chunk of columns.  All exponentials on the SFU: a share of 1, 2 or 3
+// in 8 on the FMA pipe (degree 5, 7.5e-8) took 5.18, 5.65 and 5.97 ms where this took 5.19 (32k prompt,
+// rel_extent 64), with the same results.
 template <int kC>
 __device__ __forceinline__ void add_chunk(const uint32_t (&r)[kC], const float* nlse, uint64_t mul2,
-                                          uint64_t (&acc)[4]) {
+                                          uint64_t (&acc)[2]) {
 #pragma unroll
   for (int i = 0; i < kC; i += 4) {
     const float4 nl = *reinterpret_cast<const float4*>(nlse + i);
@@ -108,14 +116,13 @@ __device__ __forceinline__ void add_chunk(const uint32_t (&r)[kC], const float* 
                      f2_pack(nl.x, nl.y)), x0, x1);
     f2_unpack(f2_fma(f2_pack(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), mul2,
                      f2_pack(nl.z, nl.w)), x2, x3);
-    acc[(i >> 1) & 3] = f2_add(acc[(i >> 1) & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
-    acc[((i >> 1) + 1) & 3] =
-        f2_add(acc[((i >> 1) + 1) & 3], f2_pack(fast_exp2(x2), fast_exp2(x3)));
+    acc[0] = f2_add(acc[0], f2_pack(fast_exp2(x0), fast_exp2(x1)));
+    acc[1] = f2_add(acc[1], f2_pack(fast_exp2(x2), fast_exp2(x3)));
   }
 }
 
 template <int kN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
     attention_mass_kernel(const __grid_constant__ AttentionMassKernelArgs a,
                           const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k) {
@@ -128,8 +135,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   Sums<kN>* sums = reinterpret_cast<Sums<kN>*>(smem + L::kSums);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y;
-  const int b = blockIdx.z;
+  // the pair of key tiles is the slowest index: with a prompt the first keys have the most rows, and
+  // the CTAs of all heads with the most rows start first
+  const int kvh = blockIdx.x;
+  const int b = blockIdx.y;
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kKStages; ++i) {
       mbar_init(&bars->k_full[i], 1);
@@ -137,12 +146,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < L::kQStages; ++i) {
       mbar_init(&bars->q_full[i], 2);   // TMA and warp 2
-      mbar_init(&bars->q_empty[i], 9);  // the products and the eight warps
+      mbar_init(&bars->q_empty[i], 1 + 8 * L::kSplit);  // the products and the summing warps
     }
     for (int w = 0; w < 2; ++w)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->s_full[w][i], 1);
-        mbar_init(&bars->s_empty[w][i], 4);
+        mbar_init(&bars->s_empty[w][i], 4 * L::kSplit);
       }
     mbar_init(&bars->drain, 1);
     bars->abort_flag = 0;
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tokens = a.tokens_per_tile;
   const bool resident = n_q <= tokens;  // one tile of rows: loaded once
   const int shift = n_k - n_q;
-  for (int r = threadIdx.x; r < kN; r += kThreads) {
+  for (int r = threadIdx.x; r < kN; r += L::kThreads) {
     const int tok = r / a.group;
     cols.token[r] = tok;
     cols.rel[r] = static_cast<long long>(tok) * (a.rel_st + 1) +
@@ -173,6 +182,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tbase = bars->tmem_base;
   const AbortCtx ab{&bars->abort_flag, a.status, kStatusDecodeTimeout};
 
+  // of the 96 registers that each of 640 threads starts with, the summing warps take 104 and the
+  // others keep 64: together the 61440 of the launch (fewer spills: 7.08 -> 6.82 ms)
+  if (L::kSplit > 1 && warp < 4) setmaxnreg_dec<64>();
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     const uint64_t pol_k = resident ? l2_policy_evict_first() : l2_policy_evict_last();
@@ -184,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t q_bytes = 2u * static_cast<uint32_t>(tokens * a.group) * 128u;
     uint32_t nk = 0, nq = 0;
     bool ok = true;
-    for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+    for (int kp = blockIdx.z; kp < n_pairs && ok; kp += gridDim.z) {
       const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
       if (rows.lo >= rows.hi) continue;
       const int key = kp * 2 * kKeys + lane * box;
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc = idesc_bf16_f32(kKeys, kN, false);
       uint32_t nk = 0, nq = 0, step = 0;
       bool ok = true;
-      for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+      for (int kp = blockIdx.z; kp < n_pairs && ok; kp += gridDim.z) {
         const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
         if (rows.lo >= rows.hi) continue;
         const uint32_t ks = nk % L::kKStages;
@@ -290,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     uint32_t nq = 0;
     bool ok = true;
-    for (int kp = blockIdx.x; kp < n_pairs && ok; kp += gridDim.x) {
+    for (int kp = blockIdx.z; kp < n_pairs && ok; kp += gridDim.z) {
       const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
       if (rows.lo >= rows.hi || (resident && nq > 0)) continue;
       fetch(rows.lo);
@@ -312,23 +324,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- exponentials and sums
-    const int w = (warp - 4) >> 2;
+    const int w = ((warp - 4) >> 2) & 1;
+    const int c_begin = ((warp - 4) >> 3) * (kN / L::kSplit);  // first column of this warpgroup
     const int row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16) + w * 2 * kN;
     const uint64_t mul2 = f2_pack(a.scale_log2, a.scale_log2);
-    constexpr int kC = L::kChunk;
+    constexpr int kC = L::kChunk, kW = kN / L::kSplit;
+    if (L::kSplit > 1) setmaxnreg_inc<104>();
     const int window = a.window_left < 0 ? 0x7fffffff : a.window_left;
-    uint32_t nq = 0, step = 0;
+    uint32_t nq = 0, step = 0, pairs = 0;
     bool ok = true;
-    for (int kp = blockIdx.x; kp < n_pairs; kp += gridDim.x) {
+    for (int kp = blockIdx.z; kp < n_pairs; kp += gridDim.z) {
       const int tile0 = kp * 2 * kKeys + w * kKeys;
       const int key = tile0 + row;
       const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
-      uint64_t acc[4] = {0, 0, 0, 0};
+      uint64_t acc[2] = {0, 0};
       float edge = 0.f;
       for (int qt = rows.lo; qt < rows.hi && ok; ++qt, ++step) {
         const uint32_t qs = resident ? 0u : nq % L::kQStages;
         const uint32_t buf = step & 1;
+        const int p0 = shift + qt * tokens;  // position of the tile's first token
+        const int n_tok = min(tokens, n_q - qt * tokens), n_cols = n_tok * a.group;
+        const int c_end = min(n_cols, c_begin + kW);
+        // distance of token 0, and its bias at that distance
+        const int dk = p0 - key;
+        const uint16_t* rel_key = a.rel + static_cast<long long>(q0 + qt * tokens) * a.rel_st + dk;
+        // the biases of a chunk, their loads in flight together; 0 where a row has none
+        const auto fetch = [&](int c0, uint16_t (&x)[kC]) {
+#pragma unroll
+          for (int i = 0; i < kC; ++i) x[i] = 0;
+          if (c0 >= c_end || p0 + cols.token[c0] - (tile0 + kKeys - 1) >= a.rel_extent) return;
+#pragma unroll
+          for (int i = 0; i < kC; ++i) {
+            const int tok = cols.token[c0 + i];
+            load_if(x[i], rel_key + cols.rel[c0 + i],
+                    tok < n_tok &&
+                        static_cast<unsigned>(dk + tok) < static_cast<unsigned>(a.rel_extent));
+          }
+        };
+        // whether every row sees every key of this tile, and none through the bias
+        const bool inside = p0 - (tile0 + kKeys - 1) >= a.rel_extent &&
+                            (a.window_left < 0 || p0 + n_tok - 1 - tile0 <= a.window_left);
+        uint16_t ahead[kC];
+        if (!inside) fetch(c_begin, ahead);
         // the wait on the Q tile makes what warp 2 wrote visible
         if (!(ok = mbar_wait_warp(&bars->q_full[qs], resident ? 0u : (nq / L::kQStages) & 1, ab)))
           break;
@@ -336,64 +374,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!(ok = mbar_wait_warp(&bars->s_full[w][buf], (step >> 1) & 1, ab))) break;
         tc_fence_after();
         const Sums<kN>& m = sums[qs];
-        const int p0 = shift + qt * tokens;  // position of the tile's first token
-        const int n_tok = min(tokens, n_q - qt * tokens), n_cols = n_tok * a.group;
-        const int p_last = p0 + n_tok - 1;
         const uint32_t t_s = t_lane + buf * kN;
-        int c_next = 0;
-        // every row sees every key of this tile, and none through the bias: the chunks that are full
-        if (p0 - (tile0 + kKeys - 1) >= a.rel_extent &&
-            (a.window_left < 0 || p_last - tile0 <= a.window_left)) {
+        int c_next = c_begin;
+        if (inside) {  // the chunks that are full
           uint32_t r[2][kC];
-          tmem_load(t_s, r[0]);
+          tmem_load(t_s + c_begin, r[0]);
           tmem_wait_ld();
 #pragma unroll
-          for (int c0 = 0; c0 < kN; c0 += kC) {
-            if (c0 + kC > n_cols) break;
-            if (c0 + kC < kN) tmem_load(t_s + c0 + kC, r[(c0 / kC + 1) & 1]);
-            add_chunk<kC>(r[(c0 / kC) & 1], &m.nlse[c0], mul2, acc);
-            if (c0 + kC < kN) tmem_wait_ld();
+          for (int c0 = 0; c0 < kW; c0 += kC) {
+            if (c_begin + c0 + kC > c_end) break;
+            if (c0 + kC < kW) tmem_load(t_s + c_begin + c0 + kC, r[(c0 / kC + 1) & 1]);
+            add_chunk<kC>(r[(c0 / kC) & 1], &m.nlse[c_begin + c0], mul2, acc);
+            if (c0 + kC < kW) tmem_wait_ld();
+            c_next += kC;
           }
-          c_next = n_cols & ~(kC - 1);
+          fetch(c_next, ahead);
         }
-        if (c_next < n_cols) {
-          // distance of token 0, and its bias at that distance
-          const int dk = p0 - key;
-          const uint16_t* rel_key = a.rel + static_cast<long long>(q0 + qt * tokens) * a.rel_st + dk;
 #pragma unroll 1
-          for (int c0 = c_next; c0 < n_cols; c0 += kC) {
-            // positions of the chunk's first and last row
-            const int p_lo = p0 + cols.token[c0], p_hi = p0 + cols.token[min(c0 + kC, n_cols) - 1];
-            if (p_hi < tile0) continue;  // before every key of the tile
-            if (a.window_left >= 0 && p_lo - (tile0 + kKeys - 1) > a.window_left) continue;
-            uint32_t r[kC];
-            tmem_load(t_s + c0, r);
-            // all loads of a chunk are in flight together
-            uint16_t bias[kC];
+        for (int c0 = c_next; c0 < c_end; c0 += kC) {
+          uint16_t bias[kC];
 #pragma unroll
-            for (int i = 0; i < kC; ++i) bias[i] = 0;
-            if (p_lo - (tile0 + kKeys - 1) < a.rel_extent) {
+          for (int i = 0; i < kC; ++i) bias[i] = ahead[i];
+          // positions of the chunk's first and last row
+          const int p_lo = p0 + cols.token[c0], p_hi = p0 + cols.token[min(c0 + kC, c_end) - 1];
+          uint32_t r[kC];
+          tmem_load(t_s + c0, r);
+          fetch(c0 + kC, ahead);
+          tmem_wait_ld();
+          if (p_hi < tile0) continue;  // before every key of the tile
+          if (a.window_left >= 0 && p_lo - (tile0 + kKeys - 1) > a.window_left) continue;
 #pragma unroll
-              for (int i = 0; i < kC; ++i) {
-                const int tok = cols.token[c0 + i];
-                const bool near = tok < n_tok && static_cast<unsigned>(dk + tok) <
-                                                     static_cast<unsigned>(a.rel_extent);
-                load_if(bias[i], rel_key + cols.rel[c0 + i], near);
-              }
-            }
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < kC; ++i) {
-              const int tok = cols.token[c0 + i];
-              // bias - lse first: either may be at the end of the range
-              const float x = __fmaf_rn(bf16_bits_to_float(bias[i]) - m.lse[c0 + i], kLog2e,
-                                        __uint_as_float(r[i]) * a.scale_log2);
-              const bool seen = tok < n_tok && static_cast<unsigned>(dk + tok) <=
-                                                   static_cast<unsigned>(window) &&
-                                m.nlse[c0 + i] != -INFINITY;
-              const float y = fast_exp2(x);
-              edge += seen ? y : 0.f;
-            }
+          for (int i = 0; i < kC; ++i) {
+            const int tok = cols.token[c0 + i];
+            // bias - lse first: either may be at the end of the range
+            const float x = __fmaf_rn(bf16_bits_to_float(bias[i]) - m.lse[c0 + i], kLog2e,
+                                      __uint_as_float(r[i]) * a.scale_log2);
+            const bool seen = tok < n_tok && static_cast<unsigned>(dk + tok) <=
+                                                 static_cast<unsigned>(window) &&
+                              m.nlse[c0 + i] != -INFINITY;
+            const float y = fast_exp2(x);
+            edge += seen ? y : 0.f;
           }
         }
         tc_fence_before();
@@ -404,9 +424,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       float s0, s1;
-      f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), s0, s1);
-      const float sum = s0 + s1 + edge;
-      if (ok && key < a.mass_width && IFA4_DBG_CHECK(a.status, b < a.s.batch)) {
+      f2_unpack(f2_add(acc[0], acc[1]), s0, s1);
+      float sum = s0 + s1 + edge;
+      if (L::kSplit > 1) {  // the other half of the columns
+        float* other = &bars->half[pairs & 1][w][row];
+        if (c_begin > 0) *other = sum;
+        asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory");
+        if (c_begin == 0) sum += *other;
+        ++pairs;
+      }
+      if (ok && c_begin == 0 && key < a.mass_width && IFA4_DBG_CHECK(a.status, b < a.s.batch)) {
         float* dst = a.mass + static_cast<long long>(b) * a.mass_sb +
                      static_cast<long long>(kvh) * a.mass_sh + key;
         if (!a.accumulate) *dst = key < n_out ? sum : 0.f;
@@ -426,7 +453,7 @@ cudaError_t launch(const AttentionMassKernelArgs& args, const CUtensorMap& tm_q,
   static std::atomic<bool> attr[64];
   cudaError_t e = set_smem_limit_once(attention_mass_kernel<kN>, Layout<kN>::kAlloc, attr);
   if (e != cudaSuccess) return e;
-  attention_mass_kernel<kN><<<dim3(key_blocks, args.kv_heads, args.s.batch), kThreads,
+  attention_mass_kernel<kN><<<dim3(args.kv_heads, args.s.batch, key_blocks), Layout<kN>::kThreads,
                               Layout<kN>::kAlloc, stream>>>(args, tm_q, tm_k);
   return cudaGetLastError();
 }
