@@ -6,6 +6,7 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
+#include <stdlib.h>
 
 #include <mutex>
 
@@ -1717,6 +1718,13 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
   return IFA4_OK;
 }
 
+// A counter and a flag for every stretch that a block moves.
+size_t evict_workspace(const IFA4KvEvictParams* p) {
+  if (p->seqs.batch == 0) return 0;
+  return (4 + static_cast<size_t>(p->seqs.batch) * p->kv_heads *
+                  ceil_div(p->budget, ifa4::kEvictRows)) * sizeof(int);
+}
+
 int validate_evict(const IFA4KvEvictParams* p) {
   const char* what = "kv_evict";
   if (p == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
@@ -1731,6 +1739,8 @@ int validate_evict(const IFA4KvEvictParams* p) {
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_width must be in [0, 2^30]", what);
   if (p->cu_out == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: cu_out is NULL", what);
   if (p->seqs.batch == 0) return IFA4_OK;
+  if (int64_t{p->seqs.batch} * p->kv_heads * ceil_div(p->budget, ifa4::kEvictRows) > 0x7f000000)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: too many kept keys", what);
   if (p->kept == nullptr || (p->mass_width > 0 && (p->mass == nullptr || p->mass_out == nullptr)))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
   if (p->mass_width > 0 && p->mass == p->mass_out)
@@ -1830,6 +1840,13 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   int64_t blocks = ceil_div(most, tokens);
   if (blocks > 65535 / p->kv_heads) blocks = 65535 / p->kv_heads;
   a.row_blocks = static_cast<int>(blocks);
+  // pages of a block: as many as leave every SM several blocks
+  int sms = 148;
+  if ((rc = sm_count(&sms))) return rc;
+  const int64_t rows = blocks * p->kv_heads * p->seqs.batch;
+  a.block_pages = 256;
+  while (a.block_pages > 32 && rows * ceil_div(p->seqs.table_width, a.block_pages) < 4 * sms)
+    a.block_pages /= 2;
   cudaError_t e = ifa4::launch_page_scores_sm100(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "page_scores launch");
   return IFA4_OK;
@@ -2012,7 +2029,8 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
   if (a.accumulate && p->max_seqlen_k > 0 && p->max_seqlen_k < most_k) most_k = p->max_seqlen_k;
   int64_t blocks = ceil_div(most_k, 256);
   if (most_q * group <= rows) {
-    const int64_t want = ceil_div(4 * sms, int64_t{p->kv_heads} * p->seqs.batch);
+    static const int kWaves = getenv("IFA4_W") ? atoi(getenv("IFA4_W")) : 4;
+    const int64_t want = ceil_div(kWaves * sms, int64_t{p->kv_heads} * p->seqs.batch);
     if (blocks > want) blocks = want;
   }
   if (blocks > 65535) blocks = 65535;
@@ -2027,7 +2045,7 @@ int ifa4_kv_evict_workspace_size(const IFA4KvEvictParams* p, size_t* bytes_out) 
   int rc = validate_evict(p);
   if (rc) return rc;
   if (bytes_out == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "kv_evict: bytes_out is NULL");
-  *bytes_out = 0;
+  *bytes_out = evict_workspace(p);
   return IFA4_OK;
 }
 
@@ -2036,8 +2054,12 @@ int ifa4_kv_evict_launch(const IFA4KvEvictParams* p, void* workspace, size_t wor
   g_last_error[0] = '\0';
   int rc = validate_evict(p);
   if (rc) return rc;
-  (void)workspace;
-  (void)workspace_bytes;
+  const size_t bytes = evict_workspace(p);
+  if (bytes > 0 && (workspace == nullptr || workspace_bytes < bytes))
+    return fail(IFA4_ERR_WORKSPACE, "kv_evict: workspace of %zu bytes required, got %zu", bytes,
+                workspace_bytes);
+  if (bytes > 0 && !aligned16(workspace))
+    return fail(IFA4_ERR_WORKSPACE, "kv_evict: workspace must be 16-byte aligned");
   int* status = nullptr;
   if ((rc = device_status_ptr(&status))) return rc;
   if (p->seqs.batch == 0) {
@@ -2068,8 +2090,12 @@ int ifa4_kv_evict_launch(const IFA4KvEvictParams* p, void* workspace, size_t wor
   a.budget = p->budget;
   a.first = p->first;
   a.recent = p->recent;
+  a.stretches = static_cast<int>(ceil_div(p->budget, ifa4::kEvictRows));
+  a.ws = static_cast<int*>(workspace);
   a.status = status;
-  cudaError_t e = ifa4::launch_kv_evict_sm100(a, static_cast<cudaStream_t>(stream));
+  int sms = 148;
+  if ((rc = sm_count(&sms))) return rc;
+  cudaError_t e = ifa4::launch_kv_evict_sm100(a, 6 * sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kv_evict launch");
   return IFA4_OK;
 }

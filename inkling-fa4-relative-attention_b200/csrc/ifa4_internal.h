@@ -55,6 +55,7 @@ constexpr int kStatusBackwardTimeout = 4;
 constexpr int kStatusSelfTestTimeout = 8;   // ifa4_selftest_bounded_wait, warp 0
 constexpr int kStatusSelfTestOwnTimeout = 16;  // ifa4_selftest_bounded_wait, warp 1 (must not be set)
 constexpr int kStatusRelLogitsTimeout = 32;
+constexpr int kStatusEvictTimeout = 128;
 constexpr int kStatusDebugBounds = 64;   // debug builds only: an index range check failed
 
 // Index range checks of debug builds (compiled with -DIFA4_DEBUG, the library's stand-in for a
@@ -324,6 +325,7 @@ struct PageScoresKernelArgs {
   int n_heads, kv_heads, group, rel_extent, window_left;
   int first_pages, last_pages, zero_padding;
   int row_blocks;            // blocks of rows of a sequence in the grid (strided over)
+  int block_pages;           // pages of a block: a multiple of 32, at most 256
   float scale;
 };
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream);
@@ -387,9 +389,13 @@ struct KvEvictKernelArgs {
   int32_t* cu_out;
   long long k_sp, k_st, k_sh, v_sp, v_st, v_sh, mass_sb, mass_sh, mo_sb, mo_sh;
   int kv_heads, mass_width, budget, first, recent;
+  int stretches;             // ceil(budget / kEvictRows)
+  int* ws;                   // counter (4 ints), then a flag per head and stretch
   int* status;
 };
-cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, cudaStream_t stream);
+constexpr int kEvictRows = 64;  // kept keys that a block moves
+// `blocks`: most blocks of the move.
+cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, int blocks, cudaStream_t stream);
 
 struct BackwardKernelArgs {
   const uint16_t* rel;       // bf16 bits

@@ -35,7 +35,8 @@ constexpr uint32_t kBarBytes = 2560;
 
 template <int kN>
 struct Layout {
-  static constexpr int kKStages = kN >= 128 ? 1 : 2;
+  static constexpr int kKStages = kN >= 128 || kN <= 32 ? 1 : 2;
+  static constexpr int kBlocks = kN <= 32 ? 2 : 1;  // resident on an SM
   static constexpr int kQStages = kN >= 128 ? 4 : 2;
   static constexpr uint32_t kQHalf = kN * 128;
   static constexpr uint32_t kQTile = 2 * kQHalf;
@@ -48,7 +49,7 @@ struct Layout {
   // Warpgroups that share a tile's columns: two where the exponentials bound the kernel
   static constexpr int kSplit = kN >= 128 ? 2 : 1;
   static constexpr int kThreads = 128 + kSplit * 256;
-  static constexpr int kChunk = kN < 32 || kSplit > 1 ? 16 : 32;
+  static constexpr int kChunk = kN <= 32 || kSplit > 1 ? 16 : 32;
 };
 
 // Rows of a Q tile: what they all have in common with the rows of every other tile, and their lse.
@@ -90,18 +91,6 @@ __device__ __forceinline__ Rows rows_of(int key0, int n_q, int n_k, int window, 
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) { tmem_ld16(addr, r); }
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
 
-// x = *p where `on`.  In order with the other such loads and ahead of what uses them: left to the
-// compiler, each load was waited for before the next was issued (a 32k prompt with rel_extent 1024:
-// 15.4 ms).
-__device__ __forceinline__ void load_if(uint16_t& x, const uint16_t* p, bool on) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.s32 p, %2, 0;\n\t"
-      "@p ld.global.nc.u16 %0, [%1];\n\t}"
-      : "+h"(x)
-      : "l"(p), "r"(static_cast<int>(on)));
-}
-
 // acc += 2^(scale s + nlse) over a chunk of columns.  All exponentials on the SFU: a share of 1, 2 or 3
 // in 8 on the FMA pipe (degree 5, 7.5e-8) took 5.18, 5.65 and 5.97 ms where this took 5.19 (32k prompt,
 // rel_extent 64), with the same results.
@@ -122,7 +111,7 @@ __device__ __forceinline__ void add_chunk(const uint32_t (&r)[kC], const float* 
 }
 
 template <int kN>
-__global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
+__global__ void __launch_bounds__(Layout<kN>::kThreads, Layout<kN>::kBlocks)
     attention_mass_kernel(const __grid_constant__ AttentionMassKernelArgs a,
                           const __grid_constant__ CUtensorMap tm_q,
                           const __grid_constant__ CUtensorMap tm_k) {
@@ -473,6 +462,11 @@ __global__ void __launch_bounds__(kSelectThreads)
     kv_evict_select_kernel(const __grid_constant__ KvEvictKernelArgs a) {
   __shared__ SelectSmem<kSelectThreads> sm;
   const int g = blockIdx.x, b = blockIdx.y;
+  launch_dependents();
+  // the counter and the flags of the move
+  if (g == 0 && b == 0 && threadIdx.x < 4) a.ws[threadIdx.x] = 0;
+  int* flags = a.ws + 4 + (static_cast<long long>(b) * a.kv_heads + g) * a.stretches;
+  for (int i = threadIdx.x; i < a.stretches; i += kSelectThreads) flags[i] = 0;
   if (g == 0 && b == 0 && threadIdx.x == 0) {
     int sum = 0, at = __ldg(a.s.cu_k);
     a.cu_out[0] = 0;
@@ -489,82 +483,177 @@ __global__ void __launch_bounds__(kSelectThreads)
   float* mass_out = a.mass_out + static_cast<long long>(b) * a.mo_sb +
                     static_cast<long long>(g) * a.mo_sh;
   int32_t* kept = a.kept + (static_cast<long long>(b) * a.kv_heads + g) * a.budget;
-  const auto mass_of = [&](int i) { return i < a.mass_width ? mass[i] : 0.f; };
-  const auto keep = [&](int place, int i) {
-    kept[place] = i;
-    if (place < a.mass_width) mass_out[place] = mass_of(i);
+  const auto keep = [&](int place, int i) { kept[place] = i; };
+  // a key from mass_width on has the mass 0; -inf ranks below every other mass, but can be kept
+  const auto rank = [&](int i, float x) {
+    if (i < a.first || i >= n - a.recent) return kAlways;
+    return i < a.mass_width ? max(rank_of(x), 1u) : rank_of(0.f);
   };
   int stay = n;
   if (n <= a.budget) {
-    for (int i = threadIdx.x; i < n; i += kSelectThreads) keep(i, i);
+    for (int i = threadIdx.x; i < n; i += kSelectThreads) kept[i] = i;
+  } else if (const int there = min(n, a.mass_width); n <= kSelectThreads * 4) {
+    stay = select_largest<kSelectThreads, 4>(sm, mass, there, n, a.budget, rank, keep);
+  } else if (n <= kSelectThreads * 12) {
+    stay = select_largest<kSelectThreads, 12>(sm, mass, there, n, a.budget, rank, keep);
+  } else if (n <= kSelectThreads * 32) {
+    stay = select_largest<kSelectThreads, 32>(sm, mass, there, n, a.budget, rank, keep);
   } else {
-    // -inf ranks below every other mass here, but can be kept
-    stay = select_largest<kSelectThreads>(
-        sm, n, a.budget,
-        [&](int i) {
-          if (i < a.first || i >= n - a.recent) return kAlways;
-          return max(rank_of(mass_of(i)), 1u);
-        },
-        keep);
+    stay = select_largest_long<kSelectThreads>(
+        sm, n, a.budget, [&](int i) { return rank(i, i < there ? __ldg(mass + i) : 0.f); }, keep);
   }
   for (int i = stay + threadIdx.x; i < a.budget; i += kSelectThreads) kept[i] = -1;
-  for (int i = stay + threadIdx.x; i < a.mass_width; i += kSelectThreads) mass_out[i] = 0.f;
+  __syncthreads();
+  // their masses: places are read back so that the loads are independent of one another
+  for (int i0 = threadIdx.x; i0 < a.mass_width; i0 += kSelectThreads * 8) {
+    float x[8];
+    int at[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * kSelectThreads;
+      at[j] = i < stay ? kept[i] : a.mass_width;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = 0.f;
+      load_if(x[j], mass + at[j], at[j] < a.mass_width);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * kSelectThreads;
+      if (i < a.mass_width) mass_out[i] = x[j];
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
 // Its move to the front
 // ---------------------------------------------------------------------------------------
-// A block per sequence and KV head goes through the kept keys in order.  Key `place` comes from
-// kept[place] >= place, so what a stretch writes has been read: by this stretch, before the barrier,
-// or by an earlier one.
-constexpr int kMoveThreads = 512;
-constexpr int kMoveRows = 64;  // K and V rows of a stretch
+// A block moves kMoveRows kept keys of one sequence and KV head: it copies them to shared memory, says
+// so, waits until every earlier stretch of the same head whose keys lie where it is about to write has
+// said so too, and writes.  Key `place` comes from kept[place] >= place, so only earlier stretches read
+// there.  Stretches are handed out in order by a counter: a block waits for blocks that are running and
+// wait for nothing themselves before they say so.  Bound by HBM: 512 bytes read and written a key.
+// (A block per head that went through its keys with barriers took 364 us where this takes XXX,
+// 16 x 32k keys to 8192.)
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 64;
+constexpr uint32_t kMoveSmem = kMoveRows * 512;  // K and V rows
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 
 __global__ void __launch_bounds__(kMoveThreads)
     kv_evict_move_kernel(const __grid_constant__ KvEvictKernelArgs a) {
-  const int g = blockIdx.x, b = blockIdx.y;
-  const int n = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
-  if (n <= a.budget) return;
-  const int32_t* kept = a.kept + (static_cast<long long>(b) * a.kv_heads + g) * a.budget;
-  const int32_t* table = table_row(a.s, b);
+  __shared__ __align__(16) uint8_t rows[kMoveSmem];
+  __shared__ int ticket[2];
+  const int heads = a.s.batch * a.kv_heads, total = heads * a.stretches;
   const int mask = (1 << a.s.page_shift) - 1;
-  const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;  // 32 rows at a time
-  constexpr int kTurns = kMoveRows / (kMoveThreads / 16);
-  for (int base = 0; base < a.budget; base += kMoveRows) {
-    uint4 k[kTurns], v[kTurns];
-    int to[kTurns];  // page of the destination, -1: nothing to write
+  const int part = threadIdx.x & 15, sub = threadIdx.x >> 4;  // 16 bytes of 16 rows at a time
+  constexpr int kStep = kMoveThreads / 16, kTurns = kMoveRows / kStep;
+  wait_previous_kernel();
+  if (threadIdx.x == 0) ticket[0] = atomicAdd(a.ws, 1);
+  __syncthreads();
+  // what a stretch moves: the pages and places its rows come from and go to (page -1: none)
+  int c, bg, from[kTurns], page_from[kTurns], page_to[kTurns];
+  const auto plan = [&](int t) {
+    c = t / heads;
+    bg = t - c * heads;
+    const int b = bg / a.kv_heads;
+    const int n = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+    const int32_t* kept = a.kept + static_cast<long long>(bg) * a.budget;
+    const int32_t* table = table_row(a.s, b);
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
-      const int place = base + sub + i * (kMoveThreads / 16);
-      const int from = place < a.budget ? kept[place] : place;
-      to[i] = from != place ? page_at(a.s, table, place >> a.s.page_shift) : -1;
-      k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (to[i] >= 0) {
-        const int page = page_at(a.s, table, from >> a.s.page_shift);
-        if (page >= 0) {
-          const long long slot = from & mask;
-          k[i] = *reinterpret_cast<const uint4*>(a.k_cache + page * a.k_sp + slot * a.k_st +
-                                                 g * a.k_sh + part * 8);
-          v[i] = *reinterpret_cast<const uint4*>(a.v_cache + page * a.v_sp + slot * a.v_st +
-                                                 g * a.v_sh + part * 8);
+      const int place = c * kMoveRows + sub + i * kStep;
+      from[i] = n > a.budget && place < a.budget ? kept[place] : place;
+    }
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int place = c * kMoveRows + sub + i * kStep;
+      page_to[i] = page_from[i] = -1;
+      if (from[i] != place) {
+        page_to[i] = page_at(a.s, table, place >> a.s.page_shift);
+        page_from[i] = page_at(a.s, table, from[i] >> a.s.page_shift);
+      }
+    }
+  };
+  int now = 0;
+  int t = ticket[0];
+  if (t < total) plan(t);
+  while (t < total) {
+    // the next stretch is taken now, so that its number and its keys are there when this one is done;
+    // whoever waits for it waits for this block, which waits for earlier stretches only
+    if (threadIdx.x == 0) ticket[now ^ 1] = atomicAdd(a.ws, 1);
+    const int g = bg % a.kv_heads;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      if (page_to[i] < 0) continue;
+      any = true;
+      uint8_t* k = rows + (sub + i * kStep) * 512 + part * 16;
+      if (page_from[i] >= 0) {
+        const long long slot = from[i] & mask;
+        cp_async16(smem_u32(k), a.k_cache + page_from[i] * a.k_sp + slot * a.k_st + g * a.k_sh +
+                                    part * 8);
+        cp_async16(smem_u32(k + 256), a.v_cache + page_from[i] * a.v_sp + slot * a.v_st +
+                                          g * a.v_sh + part * 8);
+      } else {  // a key without a page is zeros
+        *reinterpret_cast<uint4*>(k) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(k + 256) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    const int base = c * kMoveRows, this_c = c, this_bg = bg;
+    int to[kTurns];
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) to[i] = page_to[i];
+    cp_async_wait_all();
+    const bool write = __syncthreads_or(any);
+    int* flags = a.ws + 4 + static_cast<long long>(this_bg) * a.stretches;
+    if (threadIdx.x == 0) {  // this stretch has been read
+      __threadfence();
+      atomicExch(flags + this_c, 1);
+    }
+    now ^= 1;
+    t = ticket[now];
+    if (t < total) plan(t);
+    if (write) {
+      const int32_t* kept = a.kept + static_cast<long long>(this_bg) * a.budget;
+      bool ok = true;
+      const unsigned long long t0 = globaltimer_ns();
+      for (int e = this_c - 1 - static_cast<int>(threadIdx.x); e >= 0 && ok; e -= kMoveThreads) {
+        if (kept[e * kMoveRows + kMoveRows - 1] < base) break;  // and so are all before
+        for (uint32_t it = 1; load_acquire(flags + e) == 0; ++it) {
+          if ((it & 255u) == 0 && globaltimer_ns() - t0 > kWaitTimeoutNs) {
+            atomicOr(a.status, kStatusEvictTimeout);
+            ok = false;
+            break;
+          }
         }
       }
-    }
-    __syncthreads();
+      if (__syncthreads_or(!ok)) return;
 #pragma unroll
-    for (int i = 0; i < kTurns; ++i) {
-      if (to[i] >= 0) {
-        const long long slot = (base + sub + i * (kMoveThreads / 16)) & mask;
+      for (int i = 0; i < kTurns; ++i) {
+        if (to[i] < 0) continue;
+        const int r = sub + i * kStep;
+        const long long slot = (base + r) & mask;
+        const uint4* k = reinterpret_cast<const uint4*>(rows + r * 512 + part * 16);
         *reinterpret_cast<uint4*>(a.k_cache + to[i] * a.k_sp + slot * a.k_st + g * a.k_sh +
-                                  part * 8) = k[i];
+                                  part * 8) = k[0];
         *reinterpret_cast<uint4*>(a.v_cache + to[i] * a.v_sp + slot * a.v_st + g * a.v_sh +
-                                  part * 8) = v[i];
+                                  part * 8) = k[16];
       }
     }
+    __syncthreads();  // the ticket's place may be written again
   }
 }
 
 }  // namespace evict
+
+static_assert(evict::kMoveRows == kEvictRows, "stretches");
 
 int attention_mass_tile_rows(long long rows, int group) {
   int n = 16;
@@ -583,13 +672,13 @@ cudaError_t launch_attention_mass_sm100(const AttentionMassKernelArgs& args, int
   }
 }
 
-cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, cudaStream_t stream) {
-  const dim3 grid(args.kv_heads, args.s.batch);
-  evict::kv_evict_select_kernel<<<grid, evict::kSelectThreads, 0, stream>>>(args);
+cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, int blocks, cudaStream_t stream) {
+  evict::kv_evict_select_kernel<<<dim3(args.kv_heads, args.s.batch), evict::kSelectThreads, 0,
+                                  stream>>>(args);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  evict::kv_evict_move_kernel<<<grid, evict::kMoveThreads, 0, stream>>>(args);
-  return cudaGetLastError();
+  const int total = args.s.batch * args.kv_heads * args.stretches;
+  return launch_early(evict::kv_evict_move_kernel, dim3(total < blocks ? total : blocks), evict::kMoveThreads, 0, stream, args);
 }
 
 }  // namespace ifa4

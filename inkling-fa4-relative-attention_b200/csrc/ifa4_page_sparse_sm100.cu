@@ -94,23 +94,25 @@ __global__ void __launch_bounds__(kPageBoundsWarps * 32)
 // they lie in memory, and runs on warp-level MMAs (16 rows: the heads of a group, of 16 / group
 // tokens; 8 pages a warp).  The order of the 128 dims is free as long as both operands have the same:
 // lane qd of a quad takes 16 contiguous bytes of every 64, so the bounds go from global memory to the
-// fragments without shared memory, eight 16-byte loads a lane in flight.  Bound by HBM: 512 bytes a
-// page and head for 16 rows.
+// fragments without shared memory, eight 16-byte loads a lane in flight while the eight pages before
+// them are worked on.  The largest bias of a page is found by the whole block, 16 keys a thread at a
+// time, for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for 16 rows.
 constexpr int kScoreWarps = 4;
-constexpr int kScorePages = 128;  // pages of a block: 4 groups of 8 a warp
+constexpr int kScorePages = 256;  // most pages of a block
 
 __device__ __forceinline__ float max_nan(float x, float y) { return y > x || y != y ? y : x; }
 
 __global__ void __launch_bounds__(kScoreWarps * 32)
     page_scores_kernel(const __grid_constant__ PageScoresKernelArgs a) {
   __shared__ float tile[kScoreWarps][16][9];
+  __shared__ uint32_t bias_rank[16][kScorePages];  // largest bias of a row in a page
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
-  const int page0 = blockIdx.x * kScorePages;
+  const int page0 = blockIdx.x * a.block_pages;
   const int kvh = blockIdx.y % a.kv_heads;
   const int rb0 = blockIdx.y / a.kv_heads;
   const int b = blockIdx.z;
-  const int width = a.s.table_width;
-  const int page1 = min(width, page0 + kScorePages);
+  const int width = a.s.table_width, shift = a.s.page_shift;
+  const int page1 = min(width, page0 + a.block_pages);
   if (b == a.s.batch) {  // rows of no sequence
     const long long t0 = max(0, __ldg(a.s.cu_q + a.s.batch));
     for (long long t = t0 + rb0; t < a.total_q; t += a.row_blocks)
@@ -118,62 +120,108 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
         a.scores[t * a.sc_st + kvh * a.sc_sh + c] = -INFINITY;
     return;
   }
+  const int32_t* table = table_row(a.s, b);
+  const int c_warp = page0 + warp * 8;
+  // the first page of this lane's column, whatever the lengths
+  int page_next = c_warp + g < page1 ? page_at(a.s, table, c_warp + g) : -1;
   const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
   const int hb = min(a.group, 16);          // heads of a row block
   const int tokens = 16 / hb;               // and tokens
-  const int32_t* table = table_row(a.s, b);
-  const int ps = 1 << a.s.page_shift;
   for (int rb = rb0; rb * tokens < n_q; rb += a.row_blocks) {
     const int tok0 = rb * tokens;
     const int n_tok = min(tokens, n_q - tok0);
     const int p0 = n_k - n_q + tok0;  // position of the block's first token
-    for (int c0 = page0 + warp * 8; c0 < page1; c0 += kScoreWarps * 8) {
-      // visible pages of any token of the block
-      const int first_key = a.window_left < 0 ? 0 : max(0, p0 - a.window_left);
-      const int last_key = p0 + n_tok - 1;
-      const bool any = last_key >= 0 && c0 <= last_key >> a.s.page_shift &&
-                       c0 + 7 >= first_key >> a.s.page_shift;
-      float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // outputs lane, lane + 32, ..
-      if (any) {
-        uint4 bound[8];  // maxima of 4 x 32 dims, then minima
-        const int page = page_at(a.s, table, c0 + g);
+    const int p1 = p0 + n_tok - 1;    // and of its last
+    // pages that any token sees
+    const int c_lo = (a.window_left < 0 ? 0 : max(0, p0 - a.window_left)) >> shift;
+    const int c_hi = p1 >= 0 ? p1 >> shift : -1;
+    for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
+      const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
+      // row -> token, head
+      const auto token_of = [&](int row) { return a.group <= 16 ? row / hb : 0; };
+      const auto head_of = [&](int row, int tok) {
+        return kvh * a.group + (a.group <= 16 ? row - tok * hb : h0 + row);
+      };
+      const bool mine = c_lo < page1 && c_hi >= page0;
+      const auto load_bounds = [&](uint4 (&x)[8], int page) {
         const uint16_t* src = a.bounds + static_cast<long long>(max(page, 0)) * a.b_sp +
                               static_cast<long long>(kvh) * a.b_sh + qd * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          bound[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (page >= 0) bound[i] = ldg_nc_v4(src + (i < 4 ? 128 : 0) + (i & 3) * 32);
+          x[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (page >= 0) x[i] = ldg_nc_v4(src + (i < 4 ? 128 : 0) + (i & 3) * 32);
         }
-        for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
-          const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint16_t* qrow[2];
-          const uint16_t* relrow[2];
-          int pos[2];
-          bool on[2];
+      };
+      uint4 next[8];  // maxima of 4 x 32 dims, then minima
+      if (mine) load_bounds(next, page_next);
+      uint4 x[4][2];
+      int pos[2];
+      bool on[2];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int row = g + 8 * r;
-            on[r] = row < n_rows;
-            const int tok = a.group <= 16 ? row / hb : 0;
-            const int head = kvh * a.group + (a.group <= 16 ? row - tok * hb : h0 + row);
-            const long long t = q0 + tok0 + (on[r] ? tok : 0);
-            pos[r] = p0 + tok;
-            qrow[r] = a.q + t * a.q_st + static_cast<long long>(on[r] ? head : 0) * a.q_sh + qd * 8;
-            relrow[r] = a.rel + t * a.rel_st + static_cast<long long>(on[r] ? head : 0) * a.rel_sh;
+      for (int r = 0; r < 2; ++r) {
+        const int row = g + 8 * r, tok = token_of(row);
+        on[r] = row < n_rows;
+        pos[r] = p0 + tok;
+        const uint16_t* src = a.q + (q0 + tok0 + static_cast<long long>(on[r] ? tok : 0)) * a.q_st +
+                              static_cast<long long>(on[r] ? head_of(row, tok) : 0) * a.q_sh + qd * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i][r] = make_uint4(0u, 0u, 0u, 0u);
+          if (mine && on[r]) x[i][r] = ldg_nc_v4(src + i * 32);
+        }
+      }
+      // ---- largest bias of the pages within its reach: the block's keys from `near` on
+      const int near = max(max(0, p0 - a.rel_extent + 1), page0 << shift);
+      const int slice0 = near >> 4;
+      const int slices = mine ? (min(p1, ((page1 - 1) << shift) + ((1 << shift) - 1)) >> 4) - slice0 + 1 : 0;
+      if (slices > 0) {
+        const int c_near = near >> shift;
+        for (int i = threadIdx.x; i < 16 * (page1 - c_near); i += kScoreWarps * 32) {
+          const int row = i / (page1 - c_near), c = c_near + i - row * (page1 - c_near);
+          int d1 = p0 + token_of(row) - (c << shift);  // the furthest key of the page
+          if (a.window_left >= 0) d1 = min(d1, a.window_left);
+          bias_rank[row][c - page0] = d1 >= a.rel_extent ? rank_of(0.f) : 0u;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * slices; i += kScoreWarps * 32) {
+          const int row = i / slices, key0 = (slice0 + i - row * slices) << 4;
+          const int tok = token_of(row);
+          const uint16_t* rel = a.rel + (q0 + tok0 + static_cast<long long>(tok)) * a.rel_st +
+                                static_cast<long long>(head_of(row, tok)) * a.rel_sh;
+          uint16_t v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int d = p0 + tok - (key0 + j);
+            v[j] = 0xff80u;  // -inf
+            load_if(v[j], rel + d, d >= 0 && d < a.rel_extent &&
+                                       (a.window_left < 0 || d <= a.window_left));
           }
+          uint32_t most = 0u;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) most = max(most, rank_of(bf16_bits_to_float(v[j])));
+          if (most != 0u) atomicMax(&bias_rank[row][(key0 >> shift) - page0], most);
+        }
+        __syncthreads();
+      }
+      // ---- scores
+      for (int c0 = c_warp; c0 < page1; c0 += kScoreWarps * 8) {
+        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // outputs lane, lane + 32, ..
+        uint4 bound[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bound[i] = next[i];
+        const int c_next = c0 + kScoreWarps * 8;
+        if (c_next < page1 && c_next <= c_hi) {
+          const int c = c_next + g;
+          load_bounds(next, c < page1 && c + 7 >= c_lo ? page_at(a.s, table, c) : -1);
+        }
+        if (c0 <= c_hi && c0 + 7 >= c_lo) {
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint4 x[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              x[r] = make_uint4(0u, 0u, 0u, 0u);
-              if (on[r]) x[r] = ldg_nc_v4(qrow[r] + i * 32);
-            }
             const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            const uint4 p[2] = {max_v4(x[0], z), max_v4(x[1], z)};
-            const uint4 m[2] = {min_v4(x[0], z), min_v4(x[1], z)};
+            const uint4 p[2] = {max_v4(x[i][0], z), max_v4(x[i][1], z)};
+            const uint4 m[2] = {min_v4(x[i][0], z), min_v4(x[i][1], z)};
             const uint32_t pa[4] = {p[0].x, p[1].x, p[0].y, p[1].y};
             const uint32_t pb[4] = {p[0].z, p[1].z, p[0].w, p[1].w};
             const uint32_t ma[4] = {m[0].x, m[1].x, m[0].y, m[1].y};
@@ -183,26 +231,22 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
             mma_bf16(acc, ma, bound[4 + i].x, bound[4 + i].y);
             mma_bf16(acc, mb, bound[4 + i].z, bound[4 + i].w);
           }
-          // bias bound and mask of (row, page): acc[2 r + e] is row g + 8 r, page 2 qd + e
+          // acc[2 r + e] is row g + 8 r, page 2 qd + e
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = c0 + 2 * qd + e;
-              float x = -INFINITY;
-              if (on[r] && pos[r] >= 0 && c <= pos[r] >> a.s.page_shift) {
-                const int key0 = c << a.s.page_shift;
-                const int d0 = max(0, pos[r] - (key0 + ps - 1));  // nearest key of the page
-                int d1 = pos[r] - key0;                           // and the furthest
-                if (a.window_left >= 0) d1 = min(d1, a.window_left);
-                if (d0 <= d1) {
-                  float bias = d1 >= a.rel_extent ? 0.f : -INFINITY;
-                  for (int d = d0; d <= min(d1, a.rel_extent - 1); ++d)
-                    bias = max_nan(bias, bf16_bits_to_float(__ldg(relrow[r] + d)));
-                  x = acc[2 * r + e] * a.scale + bias;
+              float y = -INFINITY;
+              if (on[r] && pos[r] >= 0 && c < page1 && c <= pos[r] >> shift) {
+                // distance of the page's nearest key
+                const int d0 = max(0, pos[r] - ((c << shift) + ((1 << shift) - 1)));
+                if (a.window_left < 0 || d0 <= a.window_left) {
+                  y = acc[2 * r + e] * a.scale;
+                  if (d0 < a.rel_extent) y += value_of(bias_rank[g + 8 * r][c - page0]);
                 }
               }
-              tile[warp][g + 8 * r][2 * qd + e] = x;
+              tile[warp][g + 8 * r][2 * qd + e] = y;
             }
           __syncwarp();
           // largest over the heads of a token: output o is token o / 8, page o % 8
@@ -215,21 +259,25 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
           }
           __syncwarp();
         }
-      }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int tok = (lane + 32 * k) >> 3, c = c0 + (lane & 7);
-        if (tok < n_tok && c < width) {
-          const int p = p0 + tok;
-          float x = best[k];
-          if (p >= 0) {
-            const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> a.s.page_shift;
-            const int hi = p >> a.s.page_shift;
-            if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages)) x = INFINITY;
+        for (int k = 0; k < 4; ++k) {
+          const int tok = (lane + 32 * k) >> 3, c = c0 + (lane & 7);
+          if (tok < n_tok && c < page1) {
+            float* dst = a.scores + (q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c;
+            float y = best[k];
+            if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by this thread
+            const int p = p0 + tok;
+            if (h0 + 16 >= a.group && p >= 0) {
+              const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> shift;
+              const int hi = p >> shift;
+              if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages))
+                y = INFINITY;
+            }
+            *dst = y;
           }
-          a.scores[(q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c] = x;
         }
       }
+      if (rb + a.row_blocks < (n_q + tokens - 1) / tokens || h0 + 16 < a.group) __syncthreads();
     }
   }
 }
@@ -237,8 +285,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
 // ---------------------------------------------------------------------------------------
 // Choice of pages
 // ---------------------------------------------------------------------------------------
-// A block per row and KV head (see select_largest).
-template <int kThreads>
+// A block per row and KV head (see select_largest); kItems 0: rows of any length.
+template <int kThreads, int kItems>
 __global__ void __launch_bounds__(kThreads)
     select_pages_kernel(const __grid_constant__ SelectPagesKernelArgs a) {
   __shared__ SelectSmem<kThreads> sm;
@@ -246,9 +294,14 @@ __global__ void __launch_bounds__(kThreads)
   for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) {
     const float* src = a.scores + t * a.sc_st + g * a.sc_sh;
     int32_t* dst = a.pages + t * a.pg_st + g * a.pg_sh;
-    const int n = select_largest<kThreads>(
-        sm, a.width, a.count, [&](int i) { return rank_of(src[i]); },
-        [&](int place, int i) { dst[place] = i; });
+    const auto emit = [&](int place, int i) { dst[place] = i; };
+    int n;
+    if constexpr (kItems > 0)
+      n = select_largest<kThreads, kItems>(sm, src, a.width, a.width, a.count,
+                                           [](int, float x) { return rank_of(x); }, emit);
+    else
+      n = select_largest_long<kThreads>(sm, a.width, a.count,
+                                        [&](int i) { return rank_of(__ldg(src + i)); }, emit);
     for (int i = n + threadIdx.x; i < a.count; i += kThreads) dst[i] = -1;
   }
 }
@@ -675,7 +728,7 @@ cudaError_t launch_page_bounds_sm100(const PageBoundsKernelArgs& args, int block
 }
 
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream) {
-  const dim3 grid((args.s.table_width + sparse::kScorePages - 1) / sparse::kScorePages,
+  const dim3 grid((args.s.table_width + args.block_pages - 1) / args.block_pages,
                   args.kv_heads * args.row_blocks, args.s.batch + (args.zero_padding ? 1 : 0));
   sparse::page_scores_kernel<<<grid, sparse::kScoreWarps * 32, 0, stream>>>(args);
   return cudaGetLastError();
@@ -684,10 +737,15 @@ cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStrea
 cudaError_t launch_select_pages_sm100(const SelectPagesKernelArgs& args, cudaStream_t stream) {
   const long long most = 1 << 20;
   const dim3 grid(static_cast<unsigned>(args.rows < most ? args.rows : most), args.kv_heads);
-  if (args.width > 4096)
-    sparse::select_pages_kernel<1024><<<grid, 1024, 0, stream>>>(args);
+  // the smallest block whose registers hold a row
+  if (args.width <= 2048)
+    sparse::select_pages_kernel<256, 8><<<grid, 256, 0, stream>>>(args);
+  else if (args.width <= 8192)
+    sparse::select_pages_kernel<512, 16><<<grid, 512, 0, stream>>>(args);
+  else if (args.width <= 32768)
+    sparse::select_pages_kernel<1024, 32><<<grid, 1024, 0, stream>>>(args);
   else
-    sparse::select_pages_kernel<256><<<grid, 256, 0, stream>>>(args);
+    sparse::select_pages_kernel<1024, 0><<<grid, 1024, 0, stream>>>(args);
   return cudaGetLastError();
 }
 

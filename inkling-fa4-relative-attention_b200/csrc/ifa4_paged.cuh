@@ -54,11 +54,22 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+constexpr uint32_t kTop = 0xff800000u;  // rank of +inf
+constexpr int kSelectBins = 2048;
+constexpr int kCandidates = 256;
+
+__device__ __forceinline__ float value_of(uint32_t rank) {
+  if (rank >= kAlways - 1u) return __uint_as_float(0x7fffffffu);
+  if (rank == 0u) return -INFINITY;
+  return __uint_as_float((rank & 0x80000000u) ? rank ^ 0x80000000u : ~rank);
+}
+
 template <int kThreads>
 struct SelectSmem {
-  uint32_t hist[2048];
-  uint32_t warp[kThreads / 32];
-  uint32_t digit, above, total, in_bin;
+  uint32_t hist[kSelectBins];
+  uint32_t warp[kThreads / 32], warp_equal[kThreads / 32];
+  uint32_t candidate[kCandidates];
+  uint32_t digit, above, in_bin, able, top, low, high, found, border, need;
 };
 
 // Exclusive sum over the threads of a block, and the total; two barriers.
@@ -90,10 +101,11 @@ __device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t* wa
 
 // Calls emit(place, i) for the `count` elements of the largest key(i), 0 <= i < n, in ascending i;
 // elements of key 0 are never taken, of equal ones at the border the lowest i are.  Whole block.
-// Returns how many there are.  Three passes over digits of 11, 11 and 10 bits find the key of the
-// border, one more writes what is above it; each reads the row again, which the caches hold.
+// Returns how many there are.
+// For rows of any length: three passes over digits of 11, 11 and 10 bits find the key of the border, one
+// more writes what is above it; each reads the row again, which the caches hold.
 template <int kThreads, class Key, class Emit>
-__device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, int n, int count, Key key,
+__device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int n, int count, Key key,
                                               Emit emit) {
   const int tid = threadIdx.x;
   uint32_t need = static_cast<uint32_t>(count), prefix = 0u, known = 0u;
@@ -172,6 +184,166 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, int n, i
     equal += total >> 16;
   }
   return static_cast<int>(taken + min(equal, need));
+}
+
+// For rows of up to kThreads * kItems elements, which stay in registers (item j of a lane is element
+// 32 (kItems warp + j) + lane).  The bins of the first pass divide the range between the smallest and
+// the largest finite key, so that they are about equally full: with fixed digits of the exponent a few
+// bins held everything, and the counts waited for one another (128 x 8 rows of 8192: 56 us).  A bin of
+// up to kCandidates elements is ranked directly; a larger one is divided again.
+// The element i is values[i], or -inf from `there` on; key(i, value) ranks it.
+template <int kThreads, int kItems, class Key, class Emit>
+__device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const float* values, int there,
+                                              int n, int count, Key key, Emit emit) {
+  static_assert(kThreads >= kCandidates, "one thread a candidate");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int base = warp * 32 * kItems + lane;
+  if (tid == 0) {
+    sm.able = sm.top = sm.high = sm.found = 0u;
+    sm.low = 0xffffffffu;
+  }
+  uint32_t u[kItems];
+  {
+    float v[kItems];
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) {
+      v[j] = -INFINITY;
+      load_if(v[j], values + base + 32 * j, base + 32 * j < there);
+    }
+    for (int i = tid; i < kSelectBins; i += kThreads) sm.hist[i] = 0u;
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) u[j] = base + 32 * j < n ? key(base + 32 * j, v[j]) : 0u;
+  }
+  uint32_t able = 0u, top = 0u, low = 0xffffffffu, high = 0u;
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    able += u[j] != 0u;
+    top += u[j] >= kTop;
+    if (u[j] != 0u && u[j] < kTop) {
+      low = min(low, u[j]);
+      high = max(high, u[j]);
+    }
+  }
+  able = __reduce_add_sync(0xffffffffu, able);
+  top = __reduce_add_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  high = __reduce_max_sync(0xffffffffu, high);
+  __syncthreads();
+  if (lane == 0) {
+    atomicAdd(&sm.able, able);
+    atomicAdd(&sm.top, top);
+    atomicMin(&sm.low, low);
+    atomicMax(&sm.high, high);
+  }
+  __syncthreads();
+  uint32_t need = static_cast<uint32_t>(count), border = 0u;
+  if (sm.able <= need) {
+    need = 0u;  // everything above the border 0
+  } else {
+    uint32_t lo = kTop, hi = 0xffffffffu;  // where the border lies
+    if (need > sm.top) {
+      need -= sm.top;
+      lo = sm.low;
+      hi = sm.high;
+    }
+    for (bool first = true;; first = false) {
+      const int bits = 32 - __clz(hi - lo);
+      const int shift = bits > 11 ? bits - 11 : 0;
+      if (!first) {
+        for (int i = tid; i < kSelectBins; i += kThreads) sm.hist[i] = 0u;
+        __syncthreads();
+      }
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (u[j] >= lo && u[j] <= hi) atomicAdd(&sm.hist[(u[j] - lo) >> shift], 1u);
+      __syncthreads();
+      // thread 0 has the highest bins
+      constexpr int kPer = kSelectBins / kThreads;
+      const int high_bin = kSelectBins - 1 - tid * kPer;
+      uint32_t mine = 0u;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) mine += sm.hist[high_bin - j];
+      uint32_t total;
+      const uint32_t above = block_exclusive_sum<kThreads>(mine, sm.warp, total);
+      if (above < need && need <= above + mine) {  // exactly one thread
+        uint32_t sum = above;
+        int j = 0;
+        while (sum + sm.hist[high_bin - j] < need) sum += sm.hist[high_bin - j++];
+        sm.digit = static_cast<uint32_t>(high_bin - j);
+        sm.above = sum;
+        sm.in_bin = sm.hist[high_bin - j];
+      }
+      __syncthreads();
+      const uint32_t in_bin = sm.in_bin;
+      lo += sm.digit << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+      need -= sm.above;
+      if (in_bin == need) {  // the whole bin: everything above the key before its first
+        border = lo - 1u;
+        need = 0u;
+        break;
+      }
+      if (shift == 0) {  // equal keys: the first `need` of them
+        border = lo;
+        break;
+      }
+      if (in_bin <= kCandidates) {
+#pragma unroll
+        for (int j = 0; j < kItems; ++j)
+          if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
+        __syncthreads();
+        if (tid < static_cast<int>(in_bin)) {
+          const uint32_t x = sm.candidate[tid];
+          uint32_t larger = 0u, equal = 0u;
+          for (uint32_t j = 0; j < in_bin; ++j) {
+            larger += sm.candidate[j] > x;
+            equal += sm.candidate[j] == x;
+          }
+          if (larger < need && need <= larger + equal) {  // threads of equal keys write the same
+            sm.border = x;
+            sm.need = need - larger;
+          }
+        }
+        __syncthreads();
+        border = sm.border;
+        need = sm.need;
+        break;
+      }
+      __syncthreads();  // everyone has read what the next round writes
+    }
+  }
+  // taken: key > border, and the first `need` of key == border
+  uint32_t gt = 0u, eq = 0u;
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    gt += __popc(__ballot_sync(0xffffffffu, u[j] > border));
+    eq += __popc(__ballot_sync(0xffffffffu, u[j] == border));
+  }
+  if (need == 0u) eq = 0u;
+  if (lane == 0) {
+    sm.warp[warp] = gt;
+    sm.warp_equal[warp] = eq;
+  }
+  __syncthreads();
+  constexpr int kWarps = kThreads / 32;
+  const uint32_t wg = lane < kWarps ? sm.warp[lane] : 0u, we = lane < kWarps ? sm.warp_equal[lane] : 0u;
+  uint32_t g = __reduce_add_sync(0xffffffffu, lane < warp ? wg : 0u);
+  uint32_t e = __reduce_add_sync(0xffffffffu, lane < warp ? we : 0u);
+  const uint32_t taken = __reduce_add_sync(0xffffffffu, wg) +
+                         min(__reduce_add_sync(0xffffffffu, we), need);
+  const uint32_t before = (1u << lane) - 1u;
+#pragma unroll
+  for (int j = 0; j < kItems; ++j) {
+    const uint32_t bg = __ballot_sync(0xffffffffu, u[j] > border);
+    const uint32_t be = need == 0u ? 0u : __ballot_sync(0xffffffffu, u[j] == border);
+    const uint32_t mg = g + __popc(bg & before), me = e + __popc(be & before);
+    if (u[j] > border) emit(static_cast<int>(mg + min(me, need)), base + 32 * j);
+    else if ((be >> lane & 1u) && me < need) emit(static_cast<int>(mg + me), base + 32 * j);
+    g += __popc(bg);
+    e += __popc(be);
+  }
+  __syncthreads();  // the memory may be used again
+  return static_cast<int>(taken);
 }
 
 }  // namespace ifa4

@@ -207,6 +207,27 @@ __device__ __forceinline__ uint4 ldg_nc_v4(const void* p) {
   return r;
 }
 
+// x = *p where `on`.  In order with the other such loads and ahead of what uses them: left to the
+// compiler, each of a chunk's bias loads was waited for before the next was issued (gathered attention
+// weight of a 32k prompt with rel_extent 1024: 15.4 ms, 7.5 with the loads in flight together).
+__device__ __forceinline__ void load_if(uint16_t& x, const uint16_t* p, bool on) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "@p ld.global.nc.u16 %0, [%1];\n\t}"
+      : "+h"(x)
+      : "l"(p), "r"(static_cast<int>(on)));
+}
+
+__device__ __forceinline__ void load_if(float& x, const float* p, bool on) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "@p ld.global.nc.f32 %0, [%1];\n\t}"
+      : "+f"(x)
+      : "l"(p), "r"(static_cast<int>(on)));
+}
+
 __device__ __forceinline__ uint64_t l2_policy_evict_last() {
   uint64_t p;
   asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
