@@ -1835,6 +1835,7 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   a.last_pages = p->last_pages;
   a.zero_padding = p->zero_padding != 0;
   a.scale = p->softmax_scale;
+  if ((rc = device_status_ptr(&a.status))) return rc;
   const int tokens = a.group < 16 ? 16 / a.group : 1;
   int64_t most = p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q;
   int64_t blocks = ceil_div(most, tokens);
@@ -1845,7 +1846,7 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   if ((rc = sm_count(&sms))) return rc;
   const int64_t rows = blocks * p->kv_heads * p->seqs.batch;
   a.block_pages = 256;
-  while (a.block_pages > 32 && rows * ceil_div(p->seqs.table_width, a.block_pages) < 4 * sms)
+  while (a.block_pages > 32 && rows * ceil_div(p->seqs.table_width, a.block_pages) < 3 * sms)
     a.block_pages /= 2;
   cudaError_t e = ifa4::launch_page_scores_sm100(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "page_scores launch");
@@ -2012,6 +2013,30 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
   a.tokens_per_tile = rows / group;
   a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
   a.status = status;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.k_cache = static_cast<const uint16_t*>(p->k_cache);
+  a.q_st = p->q_stride_t;
+  a.q_sh = p->q_stride_h;
+  a.k_sp = p->k_stride_page;
+  a.k_st = p->k_stride_t;
+  a.k_sh = p->k_stride_h;
+  const int64_t heads = int64_t{p->kv_heads} * p->seqs.batch;
+  int64_t most_k = p->mass_width;
+  if (a.accumulate && p->max_seqlen_k > 0 && p->max_seqlen_k < most_k) most_k = p->max_seqlen_k;
+  if (most_q * group <= ifa4::kMassStreamRows) {
+    CUtensorMap tk16;
+    if ((rc = encode_paged(&tk16, p->k_cache, p->seqs.num_pages, p->seqs.page_size, p->kv_heads,
+                           p->k_stride_page, p->k_stride_t, p->k_stride_h, 16, "k")))
+      return rc;
+    int64_t blocks = ceil_div(most_k, 128);
+    static const int kWaves = getenv("IFA4_W") ? atoi(getenv("IFA4_W")) : 8;
+    const int64_t want = ceil_div(int64_t{kWaves} * sms, heads);
+    if (blocks > want) blocks = want;
+    cudaError_t e = ifa4::launch_attention_mass_stream_sm100(a, static_cast<int>(blocks), tk16,
+                                                             static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "attention_mass launch");
+    return IFA4_OK;
+  }
   CUtensorMap tq, tk;
   // without rows nothing is loaded, but the map has to be one
   if ((rc = encode_rows_heads_dims(&tq, p->total_q > 0 ? p->q : p->k_cache,
@@ -2025,12 +2050,9 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
                          p->k_stride_page, p->k_stride_t, p->k_stride_h, 1u << a.box_shift, "k")))
     return rc;
   // pairs of key tiles of the longest sequence; where all rows are one tile, a CTA takes several
-  int64_t most_k = p->mass_width;
-  if (a.accumulate && p->max_seqlen_k > 0 && p->max_seqlen_k < most_k) most_k = p->max_seqlen_k;
   int64_t blocks = ceil_div(most_k, 256);
   if (most_q * group <= rows) {
-    static const int kWaves = getenv("IFA4_W") ? atoi(getenv("IFA4_W")) : 4;
-    const int64_t want = ceil_div(kWaves * sms, int64_t{p->kv_heads} * p->seqs.batch);
+    const int64_t want = ceil_div(4 * sms, heads);
     if (blocks > want) blocks = want;
   }
   if (blocks > 65535) blocks = 65535;

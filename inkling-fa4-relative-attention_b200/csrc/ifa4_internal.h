@@ -325,8 +325,9 @@ struct PageScoresKernelArgs {
   int n_heads, kv_heads, group, rel_extent, window_left;
   int first_pages, last_pages, zero_padding;
   int row_blocks;            // blocks of rows of a sequence in the grid (strided over)
-  int block_pages;           // pages of a block: a multiple of 32, at most 256
+  int block_pages;           // pages of a block: 32, 64, 128 or 256
   float scale;
+  int* status;
 };
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream);
 
@@ -362,10 +363,12 @@ cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const C
 
 struct AttentionMassKernelArgs {
   PagedSeqs s;
+  const uint16_t* q;
+  const uint16_t* k_cache;
   const uint16_t* rel;
   const float* lse;
   float* mass;
-  long long rel_st, rel_sh, lse_sh, lse_st, mass_sb, mass_sh;
+  long long q_st, q_sh, k_sp, k_st, k_sh, rel_st, rel_sh, lse_sh, lse_st, mass_sb, mass_sh;
   long long total_q;
   int n_heads, kv_heads, group, rel_extent, window_left;
   int mass_width, accumulate, box_shift;
@@ -373,7 +376,12 @@ struct AttentionMassKernelArgs {
   float scale_log2;
   int* status;
 };
-// Query rows of a tile for these many rows of a sequence: 16, 32, 64 or 128.
+// For sequences of at most kMassStreamRows rows (query tokens x heads of a group).
+constexpr int kMassStreamRows = 16;
+// tm_k: boxes of 16 keys.
+cudaError_t launch_attention_mass_stream_sm100(const AttentionMassKernelArgs& args, int key_blocks,
+                                               const CUtensorMap& tm_k, cudaStream_t stream);
+// Query rows of a tile for these many rows of a sequence: 32, 64 or 128.
 int attention_mass_tile_rows(long long rows, int group);
 cudaError_t launch_attention_mass_sm100(const AttentionMassKernelArgs& args, int tile_rows,
                                         const CUtensorMap& tm_q, const CUtensorMap& tm_k,

@@ -93,20 +93,41 @@ __global__ void __launch_bounds__(kPageBoundsWarps * 32)
 // sum_i (max(q_i, 0) max_i + min(q_i, 0) min_i) is a matrix product of depth 256 with the bounds as
 // they lie in memory, and runs on warp-level MMAs (16 rows: the heads of a group, of 16 / group
 // tokens; 8 pages a warp).  The order of the 128 dims is free as long as both operands have the same:
-// lane qd of a quad takes 16 contiguous bytes of every 64, so the bounds go from global memory to the
-// fragments without shared memory, eight 16-byte loads a lane in flight while the eight pages before
-// them are worked on.  The largest bias of a page is found by the whole block, 16 keys a thread at a
-// time, for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for 16 rows.
+// lane qd of a quad takes 16 contiguous bytes of every 64 from the bounds as they were copied.  Every warp
+// has a ring of its own, eight pages a stage, refilled by bulk copies (512 contiguous bytes a page) as
+// soon as it has read a stage.  The largest bias of a page is found by the whole block, 16 keys a
+// thread at a time, for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for
+// 16 rows.  (64 sequences of up to 32k keys: 111 us with the bounds loaded straight to registers, 104
+// with the next eight pages loaded ahead.)
 constexpr int kScoreWarps = 4;
 constexpr int kScorePages = 256;  // most pages of a block
+constexpr int kScoreStages = 3;
+// Pages of a stage lie 576 bytes apart: a lane's 16 bytes and those of the seven it reads with are in
+// different banks.
+constexpr uint32_t kScorePitch = 576;
+constexpr uint32_t kScoreStage = 8 * kScorePitch;
+constexpr uint32_t kScoreRing = kScoreWarps * kScoreStages * kScoreStage;
+constexpr uint32_t kScoreBias = kScoreRing;
+constexpr uint32_t kScoreTile = kScoreBias + 16 * kScorePages * 4;
+constexpr uint32_t kScoreBar = kScoreTile + kScoreWarps * 16 * 9 * 4;
+constexpr uint32_t kScoreSmem = kScoreBar + kScoreWarps * kScoreStages * 12 + 16;
+static_assert(kScoreBar % 8 == 0, "barriers");
 
 __device__ __forceinline__ float max_nan(float x, float y) { return y > x || y != y ? y : x; }
 
-__global__ void __launch_bounds__(kScoreWarps * 32)
+__global__ void __launch_bounds__(kScoreWarps * 32, 3)
     page_scores_kernel(const __grid_constant__ PageScoresKernelArgs a) {
-  __shared__ float tile[kScoreWarps][16][9];
-  __shared__ uint32_t bias_rank[16][kScorePages];  // largest bias of a row in a page
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint32_t(&bias_rank)[16][kScorePages] =  // largest bias of a row in a page
+      *reinterpret_cast<uint32_t(*)[16][kScorePages]>(smem + kScoreBias);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
+  float(&tile)[16][9] = reinterpret_cast<float(*)[16][9]>(smem + kScoreTile)[warp];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kScoreBar) + warp * kScoreStages;
+  // pages of each stage that are none: their bounds are zeros
+  uint32_t* missing = reinterpret_cast<uint32_t*>(smem + kScoreBar + 8 * kScoreWarps * kScoreStages) +
+                      warp * kScoreStages;
+  int* abort_flag = reinterpret_cast<int*>(smem + kScoreBar + 12 * kScoreWarps * kScoreStages);
+  uint8_t* ring = smem + warp * kScoreStages * kScoreStage;
   const int page0 = blockIdx.x * a.block_pages;
   const int kvh = blockIdx.y % a.kv_heads;
   const int rb0 = blockIdx.y / a.kv_heads;
@@ -120,10 +141,19 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
         a.scores[t * a.sc_st + kvh * a.sc_sh + c] = -INFINITY;
     return;
   }
+  if (lane == 0) {
+    for (int i = 0; i < kScoreStages; ++i) mbar_init(&full[i], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const AbortCtx ab{abort_flag, a.status, kStatusDecodeTimeout};
+  const uint64_t pol = l2_policy_evict_first();
   const int32_t* table = table_row(a.s, b);
   const int c_warp = page0 + warp * 8;
-  // the first page of this lane's column, whatever the lengths
-  int page_next = c_warp + g < page1 ? page_at(a.s, table, c_warp + g) : -1;
+  constexpr int kStride = kScoreWarps * 8;
+  uint32_t done = 0;  // stages read so far: the ring goes on through all rounds
+  bool ok = true;
   const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
   const int hb = min(a.group, 16);          // heads of a row block
@@ -136,6 +166,25 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
     // pages that any token sees
     const int c_lo = (a.window_left < 0 ? 0 : max(0, p0 - a.window_left)) >> shift;
     const int c_hi = p1 >= 0 ? p1 >> shift : -1;
+    // eight pages of a warp's turn are read if any of them is seen
+    const auto seen = [&](int c0) { return c0 < page1 && c0 <= c_hi && c0 + 7 >= c_lo; };
+    const auto page_of = [&](int c0) {  // of lane's page, lanes 0 to 7
+      return lane < 8 && seen(c0) && c0 + lane < page1 ? page_at(a.s, table, c0 + lane) : -1;
+    };
+    const auto load = [&](int c0, int page, uint32_t st) {
+      if (!seen(c0)) return;
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) {
+        missing[st] = ~there;
+        mbar_arrive_expect_tx(&full[st], __popc(there) * 512u);
+      }
+      __syncwarp();
+      if (page >= 0)
+        bulk_load_hint(ring + st * kScoreStage + lane * kScorePitch,
+                       a.bounds + static_cast<long long>(page) * a.b_sp +
+                           static_cast<long long>(kvh) * a.b_sh,
+                       512, &full[st], pol);
+    };
     for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
       const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
       // row -> token, head
@@ -144,18 +193,20 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
         return kvh * a.group + (a.group <= 16 ? row - tok * hb : h0 + row);
       };
       const bool mine = c_lo < page1 && c_hi >= page0;
-      const auto load_bounds = [&](uint4 (&x)[8], int page) {
-        const uint16_t* src = a.bounds + static_cast<long long>(max(page, 0)) * a.b_sp +
-                              static_cast<long long>(kvh) * a.b_sh + qd * 8;
+      int c_first = c_warp;  // the first pages of this warp that are seen
+      if (mine && c_first + 7 < c_lo) c_first += (c_lo - c_first - 7 + kStride - 1) / kStride * kStride;
+      int page_next;
+      {
+        int pages[kScoreStages];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (page >= 0) x[i] = ldg_nc_v4(src + (i < 4 ? 128 : 0) + (i & 3) * 32);
-        }
-      };
-      uint4 next[8];  // maxima of 4 x 32 dims, then minima
-      if (mine) load_bounds(next, page_next);
-      uint4 x[4][2];
+        for (int i = 0; i < kScoreStages; ++i) pages[i] = page_of(c_first + i * kStride);
+        page_next = page_of(c_first + kScoreStages * kStride);
+#pragma unroll
+        for (int i = 0; i < kScoreStages; ++i)
+          load(c_first + i * kStride, pages[i], (done + i) % kScoreStages);
+      }
+      // max(q, 0) and min(q, 0) of rows g and g + 8
+      uint4 qp[4][2], qm[4][2];
       int pos[2];
       bool on[2];
 #pragma unroll
@@ -165,10 +216,13 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
         pos[r] = p0 + tok;
         const uint16_t* src = a.q + (q0 + tok0 + static_cast<long long>(on[r] ? tok : 0)) * a.q_st +
                               static_cast<long long>(on[r] ? head_of(row, tok) : 0) * a.q_sh + qd * 8;
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i][r] = make_uint4(0u, 0u, 0u, 0u);
-          if (mine && on[r]) x[i][r] = ldg_nc_v4(src + i * 32);
+          uint4 x = z;
+          if (mine && on[r]) x = ldg_nc_v4(src + i * 32);
+          qp[i][r] = max_v4(x, z);
+          qm[i][r] = min_v4(x, z);
         }
       }
       // ---- largest bias of the pages within its reach: the block's keys from `near` on
@@ -205,32 +259,35 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
         __syncthreads();
       }
       // ---- scores
-      for (int c0 = c_warp; c0 < page1; c0 += kScoreWarps * 8) {
+      for (int c0 = c_warp; c0 < page1; c0 += kStride) {
         float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // outputs lane, lane + 32, ..
-        uint4 bound[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) bound[i] = next[i];
-        const int c_next = c0 + kScoreWarps * 8;
-        if (c_next < page1 && c_next <= c_hi) {
-          const int c = c_next + g;
-          load_bounds(next, c < page1 && c + 7 >= c_lo ? page_at(a.s, table, c) : -1);
-        }
-        if (c0 <= c_hi && c0 + 7 >= c_lo) {
+        if (seen(c0) && ok) {
+          const uint32_t st = done % kScoreStages;
+          ok = mbar_wait_warp(&full[st], (done / kScoreStages) & 1, ab);
+          if (!ok) continue;
+          const bool none = missing[st] >> g & 1u;
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint8_t* src = ring + st * kScoreStage + g * kScorePitch + qd * 16;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            const uint4 p[2] = {max_v4(x[i][0], z), max_v4(x[i][1], z)};
-            const uint4 m[2] = {min_v4(x[i][0], z), min_v4(x[i][1], z)};
-            const uint32_t pa[4] = {p[0].x, p[1].x, p[0].y, p[1].y};
-            const uint32_t pb[4] = {p[0].z, p[1].z, p[0].w, p[1].w};
-            const uint32_t ma[4] = {m[0].x, m[1].x, m[0].y, m[1].y};
-            const uint32_t mb[4] = {m[0].z, m[1].z, m[0].w, m[1].w};
-            mma_bf16(acc, pa, bound[i].x, bound[i].y);
-            mma_bf16(acc, pb, bound[i].z, bound[i].w);
-            mma_bf16(acc, ma, bound[4 + i].x, bound[4 + i].y);
-            mma_bf16(acc, mb, bound[4 + i].z, bound[4 + i].w);
+            uint4 lo = *reinterpret_cast<const uint4*>(src + i * 64);
+            uint4 hi = *reinterpret_cast<const uint4*>(src + 256 + i * 64);
+            if (none) lo = hi = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t pa[4] = {qp[i][0].x, qp[i][1].x, qp[i][0].y, qp[i][1].y};
+            const uint32_t pb[4] = {qp[i][0].z, qp[i][1].z, qp[i][0].w, qp[i][1].w};
+            const uint32_t ma[4] = {qm[i][0].x, qm[i][1].x, qm[i][0].y, qm[i][1].y};
+            const uint32_t mb[4] = {qm[i][0].z, qm[i][1].z, qm[i][0].w, qm[i][1].w};
+            mma_bf16(acc, pa, hi.x, hi.y);
+            mma_bf16(acc, pb, hi.z, hi.w);
+            mma_bf16(acc, ma, lo.x, lo.y);
+            mma_bf16(acc, mb, lo.z, lo.w);
           }
+          // the stage has been read, not only asked for, before it is filled again
+          fence_proxy_async_smem();
+          __syncwarp();
+          ++done;
+          load(c0 + kScoreStages * kStride, page_next, st);
+          page_next = page_of(c0 + (kScoreStages + 1) * kStride);
           // acc[2 r + e] is row g + 8 r, page 2 qd + e
 #pragma unroll
           for (int r = 0; r < 2; ++r)
@@ -246,7 +303,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
                   if (d0 < a.rel_extent) y += value_of(bias_rank[g + 8 * r][c - page0]);
                 }
               }
-              tile[warp][g + 8 * r][2 * qd + e] = y;
+              tile[g + 8 * r][2 * qd + e] = y;
             }
           __syncwarp();
           // largest over the heads of a token: output o is token o / 8, page o % 8
@@ -255,7 +312,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
             const int tok = (lane + 32 * k) >> 3, pg = lane & 7;
             const int heads = a.group <= 16 ? hb : n_rows;
             if (tok < n_tok)
-              for (int r = 0; r < heads; ++r) best[k] = max_nan(best[k], tile[warp][tok * heads + r][pg]);
+              for (int r = 0; r < heads; ++r) best[k] = max_nan(best[k], tile[tok * heads + r][pg]);
           }
           __syncwarp();
         }
@@ -280,6 +337,10 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
       if (rb + a.row_blocks < (n_q + tokens - 1) / tokens || h0 + 16 < a.group) __syncthreads();
     }
   }
+  // after a wait that was given up: what is in flight has landed before the memory goes
+  if (!ok && lane == 0)
+    for (uint32_t i = 0; i < kScoreStages; ++i)
+      mbar_wait(&full[(done + i) % kScoreStages], ((done + i) / kScoreStages) & 1, ab);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -730,7 +791,10 @@ cudaError_t launch_page_bounds_sm100(const PageBoundsKernelArgs& args, int block
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream) {
   const dim3 grid((args.s.table_width + args.block_pages - 1) / args.block_pages,
                   args.kv_heads * args.row_blocks, args.s.batch + (args.zero_padding ? 1 : 0));
-  sparse::page_scores_kernel<<<grid, sparse::kScoreWarps * 32, 0, stream>>>(args);
+  static std::atomic<bool> attr[64];
+  cudaError_t e = set_smem_limit_once(sparse::page_scores_kernel, sparse::kScoreSmem, attr);
+  if (e != cudaSuccess) return e;
+  sparse::page_scores_kernel<<<grid, sparse::kScoreWarps * 32, sparse::kScoreSmem, stream>>>(args);
   return cudaGetLastError();
 }
 

@@ -43,33 +43,31 @@ __device__ __forceinline__ const int32_t* table_row(const PagedSeqs& s, int b) {
 // ---------------------------------------------------------------------------------------
 // The `count` largest of a row
 // ---------------------------------------------------------------------------------------
-// Order-preserving image of a float: -inf is 0 (never chosen), NaN is above +inf, the zeros are
-// equal; kAlways is above all of them.
+// Order-preserving image of a float: -inf is 0 (never chosen), the zeros are equal, and so are all
+// NaN, above +inf; kAlways is above all of them.  (x + 0 is +0 for -0 and the canonical NaN for NaN.)
 constexpr uint32_t kAlways = 0xffffffffu;
+constexpr uint32_t kLowest = 0x007fffffu;           // bits of -inf with their order
+constexpr uint32_t kTop = 0xff800000u - kLowest;    // rank of +inf
+constexpr uint32_t kRankNan = 0xffffffffu - kLowest;
+constexpr uint32_t kRankZero = 0x80000000u - kLowest;
 __device__ __forceinline__ uint32_t rank_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  if ((b & 0x7fffffffu) > 0x7f800000u) return kAlways - 1u;
-  if (b == 0xff800000u) return 0u;
-  if ((b & 0x7fffffffu) == 0u) return 0x80000000u;
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const uint32_t b = __float_as_uint(__fadd_rn(x, 0.f));
+  return (b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u)) - kLowest;
+}
+__device__ __forceinline__ float value_of(uint32_t rank) {
+  const uint32_t u = rank + kLowest;
+  return __uint_as_float(u ^ (static_cast<uint32_t>(static_cast<int32_t>(~u) >> 31) | 0x80000000u));
 }
 
-constexpr uint32_t kTop = 0xff800000u;  // rank of +inf
 constexpr int kSelectBins = 2048;
 constexpr int kCandidates = 256;
-
-__device__ __forceinline__ float value_of(uint32_t rank) {
-  if (rank >= kAlways - 1u) return __uint_as_float(0x7fffffffu);
-  if (rank == 0u) return -INFINITY;
-  return __uint_as_float((rank & 0x80000000u) ? rank ^ 0x80000000u : ~rank);
-}
 
 template <int kThreads>
 struct SelectSmem {
   uint32_t hist[kSelectBins];
   uint32_t warp[kThreads / 32], warp_equal[kThreads / 32];
   uint32_t candidate[kCandidates];
-  uint32_t digit, above, in_bin, able, top, low, high, found, border, need;
+  uint32_t digit, above, in_bin, low, high, found, border, need;
 };
 
 // Exclusive sum over the threads of a block, and the total; two barriers.
@@ -188,9 +186,11 @@ __device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int
 
 // For rows of up to kThreads * kItems elements, which stay in registers (item j of a lane is element
 // 32 (kItems warp + j) + lane).  The bins of the first pass divide the range between the smallest and
-// the largest finite key, so that they are about equally full: with fixed digits of the exponent a few
-// bins held everything, and the counts waited for one another (128 x 8 rows of 8192: 56 us).  A bin of
-// up to kCandidates elements is ranked directly; a larger one is divided again.
+// the largest finite element, so that they are about equally full: of the keys, which is logarithmic,
+// where all have one sign, and of the values where they have both (the keys of small values of either
+// sign would take up most of the bins).  With fixed digits of the exponent a few bins held everything,
+// and the counts waited for one another (128 x 8 rows of 8192: 56 us).  A bin of up to kCandidates
+// elements is ranked directly; a larger one is divided again.
 // The element i is values[i], or -inf from `there` on; key(i, value) ranks it.
 template <int kThreads, int kItems, class Key, class Emit>
 __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const float* values, int there,
@@ -199,7 +199,7 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int base = warp * 32 * kItems + lane;
   if (tid == 0) {
-    sm.able = sm.top = sm.high = sm.found = 0u;
+    sm.high = sm.found = 0u;
     sm.low = 0xffffffffu;
   }
   uint32_t u[kItems];
@@ -214,112 +214,146 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
 #pragma unroll
     for (int j = 0; j < kItems; ++j) u[j] = base + 32 * j < n ? key(base + 32 * j, v[j]) : 0u;
   }
-  uint32_t able = 0u, top = 0u, low = 0xffffffffu, high = 0u;
+  // smallest (less one, which leaves out the keys 0) and largest of the finite ones
+  uint32_t low = 0xffffffffu, high = 0u;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
-    able += u[j] != 0u;
-    top += u[j] >= kTop;
-    if (u[j] != 0u && u[j] < kTop) {
-      low = min(low, u[j]);
-      high = max(high, u[j]);
-    }
+    low = min(low, u[j] - 1u);
+    high = max(high, u[j] < kTop ? u[j] : 0u);
   }
-  able = __reduce_add_sync(0xffffffffu, able);
-  top = __reduce_add_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
   high = __reduce_max_sync(0xffffffffu, high);
   __syncthreads();
   if (lane == 0) {
-    atomicAdd(&sm.able, able);
-    atomicAdd(&sm.top, top);
     atomicMin(&sm.low, low);
     atomicMax(&sm.high, high);
   }
   __syncthreads();
-  uint32_t need = static_cast<uint32_t>(count), border = 0u;
-  if (sm.able <= need) {
-    need = 0u;  // everything above the border 0
-  } else {
-    uint32_t lo = kTop, hi = 0xffffffffu;  // where the border lies
-    if (need > sm.top) {
-      need -= sm.top;
-      lo = sm.low;
-      hi = sm.high;
+  // where the border lies; keys from kTop on are in the last bin of the first pass
+  uint32_t lo = sm.low + 1u, hi = sm.high, need = static_cast<uint32_t>(count), border = 0u;
+  float start = 0.f, scale = 0.f;  // the bins of values, where scale > 0
+  if (lo < kRankZero && hi > kRankZero) {
+    start = value_of(lo);
+    scale = (kSelectBins - 2) / (value_of(hi) - start);  // 0 where the range is not finite
+  }
+  // bins ascend with the keys (a difference and a product with a positive number do, rounded too)
+  const auto value_bin = [&](uint32_t key) {
+    return min(static_cast<uint32_t>((value_of(key) - start) * scale), kSelectBins - 2u);
+  };
+  for (bool first = true;; first = false) {
+    const int bits = hi > lo ? 32 - __clz(hi - lo) : 0;
+    const int shift = bits > 10 ? bits - 10 : 0;  // at most 1024 bins
+    if (!first) {
+      for (int i = tid; i < kSelectBins; i += kThreads) sm.hist[i] = 0u;
+      __syncthreads();
     }
-    for (bool first = true;; first = false) {
-      const int bits = 32 - __clz(hi - lo);
-      const int shift = bits > 11 ? bits - 11 : 0;
-      if (!first) {
-        for (int i = tid; i < kSelectBins; i += kThreads) sm.hist[i] = 0u;
-        __syncthreads();
-      }
+    const bool values_binned = first && scale > 0.f;
+    if (values_binned) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (u[j] != 0u) atomicAdd(&sm.hist[u[j] >= kTop ? kSelectBins - 1 : value_bin(u[j])], 1u);
+    } else if (first) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (u[j] != 0u) atomicAdd(&sm.hist[u[j] >= kTop ? kSelectBins - 1 : (u[j] - lo) >> shift], 1u);
+    } else {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
         if (u[j] >= lo && u[j] <= hi) atomicAdd(&sm.hist[(u[j] - lo) >> shift], 1u);
-      __syncthreads();
-      // thread 0 has the highest bins
-      constexpr int kPer = kSelectBins / kThreads;
-      const int high_bin = kSelectBins - 1 - tid * kPer;
-      uint32_t mine = 0u;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) mine += sm.hist[high_bin - j];
-      uint32_t total;
-      const uint32_t above = block_exclusive_sum<kThreads>(mine, sm.warp, total);
-      if (above < need && need <= above + mine) {  // exactly one thread
-        uint32_t sum = above;
-        int j = 0;
-        while (sum + sm.hist[high_bin - j] < need) sum += sm.hist[high_bin - j++];
-        sm.digit = static_cast<uint32_t>(high_bin - j);
-        sm.above = sum;
-        sm.in_bin = sm.hist[high_bin - j];
-      }
-      __syncthreads();
-      const uint32_t in_bin = sm.in_bin;
-      lo += sm.digit << shift;
-      hi = min(hi, lo + ((1u << shift) - 1u));
-      need -= sm.above;
-      if (in_bin == need) {  // the whole bin: everything above the key before its first
-        border = lo - 1u;
-        need = 0u;
-        break;
-      }
-      if (shift == 0) {  // equal keys: the first `need` of them
-        border = lo;
-        break;
-      }
-      if (in_bin <= kCandidates) {
-#pragma unroll
-        for (int j = 0; j < kItems; ++j)
-          if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
-        __syncthreads();
-        if (tid < static_cast<int>(in_bin)) {
-          const uint32_t x = sm.candidate[tid];
-          uint32_t larger = 0u, equal = 0u;
-          for (uint32_t j = 0; j < in_bin; ++j) {
-            larger += sm.candidate[j] > x;
-            equal += sm.candidate[j] == x;
-          }
-          if (larger < need && need <= larger + equal) {  // threads of equal keys write the same
-            sm.border = x;
-            sm.need = need - larger;
-          }
-        }
-        __syncthreads();
-        border = sm.border;
-        need = sm.need;
-        break;
-      }
-      __syncthreads();  // everyone has read what the next round writes
     }
+    __syncthreads();
+    // thread 0 has the highest bins
+    constexpr int kPer = kSelectBins / kThreads;
+    const int high_bin = kSelectBins - 1 - tid * kPer;
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) mine += sm.hist[high_bin - j];
+    uint32_t total;
+    const uint32_t above = block_exclusive_sum<kThreads>(mine, sm.warp, total);
+    if (first && total <= need) {  // everything that can be taken: above the border 0
+      need = 0u;
+      break;
+    }
+    if (above < need && need <= above + mine) {  // exactly one thread
+      uint32_t sum = above;
+      int j = 0;
+      while (sum + sm.hist[high_bin - j] < need) sum += sm.hist[high_bin - j++];
+      sm.digit = static_cast<uint32_t>(high_bin - j);
+      sm.above = sum;
+      sm.in_bin = sm.hist[high_bin - j];
+      sm.low = 0xffffffffu;
+      sm.high = 0u;
+    }
+    __syncthreads();
+    const uint32_t in_bin = sm.in_bin, digit = sm.digit;
+    need -= sm.above;
+    if (first && digit == kSelectBins - 1) {
+      lo = kTop;
+      hi = 0xffffffffu;
+    } else if (values_binned) {  // the smallest and the largest key of the bin
+      low = 0xffffffffu;
+      high = 0u;
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (u[j] != 0u && u[j] < kTop && value_bin(u[j]) == digit) {
+          low = min(low, u[j]);
+          high = max(high, u[j]);
+        }
+      low = __reduce_min_sync(0xffffffffu, low);
+      high = __reduce_max_sync(0xffffffffu, high);
+      if (lane == 0 && low <= high) {
+        atomicMin(&sm.low, low);
+        atomicMax(&sm.high, high);
+      }
+      __syncthreads();
+      lo = sm.low;
+      hi = sm.high;
+    } else {
+      lo += digit << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+    }
+    if (in_bin == need) {  // the whole bin: everything above the key before its first
+      border = lo - 1u;
+      need = 0u;
+      break;
+    }
+    if (lo == hi) {  // equal keys: the first `need` of them
+      border = lo;
+      break;
+    }
+    if (in_bin <= kCandidates) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
+      __syncthreads();
+      if (tid < static_cast<int>(in_bin)) {
+        const uint32_t x = sm.candidate[tid];
+        uint32_t larger = 0u, equal = 0u;
+        for (uint32_t j = 0; j < in_bin; ++j) {
+          larger += sm.candidate[j] > x;
+          equal += sm.candidate[j] == x;
+        }
+        if (larger < need && need <= larger + equal) {  // threads of equal keys write the same
+          const bool every = need == larger + equal;    // all equal ones: they are above x - 1
+          sm.border = every ? x - 1u : x;
+          sm.need = every ? 0u : need - larger;
+        }
+      }
+      __syncthreads();
+      border = sm.border;
+      need = sm.need;
+      break;
+    }
+    __syncthreads();  // everyone has read what the next round writes
   }
   // taken: key > border, and the first `need` of key == border
   uint32_t gt = 0u, eq = 0u;
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    gt += __popc(__ballot_sync(0xffffffffu, u[j] > border));
-    eq += __popc(__ballot_sync(0xffffffffu, u[j] == border));
+  for (int j = 0; j < kItems; ++j) gt += __popc(__ballot_sync(0xffffffffu, u[j] > border));
+  if (need != 0u) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) eq += __popc(__ballot_sync(0xffffffffu, u[j] == border));
   }
-  if (need == 0u) eq = 0u;
   if (lane == 0) {
     sm.warp[warp] = gt;
     sm.warp_equal[warp] = eq;
@@ -332,15 +366,29 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
   const uint32_t taken = __reduce_add_sync(0xffffffffu, wg) +
                          min(__reduce_add_sync(0xffffffffu, we), need);
   const uint32_t before = (1u << lane) - 1u;
+  if (need == 0u) {
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) {
-    const uint32_t bg = __ballot_sync(0xffffffffu, u[j] > border);
-    const uint32_t be = need == 0u ? 0u : __ballot_sync(0xffffffffu, u[j] == border);
-    const uint32_t mg = g + __popc(bg & before), me = e + __popc(be & before);
-    if (u[j] > border) emit(static_cast<int>(mg + min(me, need)), base + 32 * j);
-    else if ((be >> lane & 1u) && me < need) emit(static_cast<int>(mg + me), base + 32 * j);
-    g += __popc(bg);
-    e += __popc(be);
+    for (int j = 0; j < kItems; ++j) {
+      const uint32_t bg = __ballot_sync(0xffffffffu, u[j] > border);
+      if (bg != 0u) {
+        if (u[j] > border) emit(static_cast<int>(g + __popc(bg & before)), base + 32 * j);
+        g += __popc(bg);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < kItems; ++j) {
+      uint32_t x = 0u;  // u[j] without indexing registers
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) x = i == j ? u[i] : x;
+      const uint32_t bg = __ballot_sync(0xffffffffu, x > border);
+      const uint32_t be = __ballot_sync(0xffffffffu, x == border);
+      const uint32_t mg = g + __popc(bg & before), me = e + __popc(be & before);
+      if (x > border) emit(static_cast<int>(mg + min(me, need)), base + 32 * j);
+      else if (x == border && me < need) emit(static_cast<int>(mg + me), base + 32 * j);
+      g += __popc(bg);
+      e += __popc(be);
+    }
   }
   __syncthreads();  // the memory may be used again
   return static_cast<int>(taken);

@@ -171,6 +171,16 @@ __device__ __forceinline__ void tma_load_4d_hint(void* smem_dst, const CUtensorM
       : "memory");
 }
 
+// Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) without a tensor map.
+__device__ __forceinline__ void bulk_load_hint(void* smem_dst, const void* src, uint32_t bytes,
+                                               uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
 // Orders this thread's generic-proxy shared-memory writes before later async-proxy reads
 // (TMA / tcgen05.mma operands) of the same bytes.
 __device__ __forceinline__ void fence_proxy_async_smem() {
@@ -219,6 +229,16 @@ __device__ __forceinline__ void load_if(uint16_t& x, const uint16_t* p, bool on)
       : "l"(p), "r"(static_cast<int>(on)));
 }
 
+// The same for memory that this kernel writes.
+__device__ __forceinline__ void load_plain_if(float& x, const float* p, bool on) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "@p ld.global.f32 %0, [%1];\n\t}"
+      : "+f"(x)
+      : "l"(p), "r"(static_cast<int>(on))
+      : "memory");
+}
 __device__ __forceinline__ void load_if(float& x, const float* p, bool on) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
