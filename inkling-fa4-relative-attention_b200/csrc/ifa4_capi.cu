@@ -6,7 +6,6 @@
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
-#include <stdlib.h>
 
 #include <mutex>
 
@@ -1807,6 +1806,8 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   if (p->first_pages < 0 || p->last_pages < 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative first_pages or last_pages", what);
   if (p->kv_heads > 16383) return fail(IFA4_ERR_UNSUPPORTED, "%s: kv_heads > 16383", what);
+  if (p->bounds_stride_page > (int64_t{1} << 30))
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: bounds_stride_page > 2^30", what);
   if (p->seqs.batch == 0 || p->total_q == 0 || p->seqs.table_width == 0) return IFA4_OK;
   if (p->scores == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores is NULL", what);
   if (p->scores_stride_t < 0 || p->scores_stride_h < 0)
@@ -1831,11 +1832,11 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   a.group = p->n_heads / p->kv_heads;
   a.rel_extent = p->rel_extent;
   a.window_left = p->window_left < 0 ? -1 : p->window_left;
-  a.first_pages = p->first_pages;
-  a.last_pages = p->last_pages;
+  // no row has more pages than its table
+  a.first_pages = p->first_pages < p->seqs.table_width ? p->first_pages : p->seqs.table_width;
+  a.last_pages = p->last_pages < p->seqs.table_width ? p->last_pages : p->seqs.table_width;
   a.zero_padding = p->zero_padding != 0;
   a.scale = p->softmax_scale;
-  if ((rc = device_status_ptr(&a.status))) return rc;
   const int tokens = a.group < 16 ? 16 / a.group : 1;
   int64_t most = p->max_seqlen_q > 0 && p->max_seqlen_q < p->total_q ? p->max_seqlen_q : p->total_q;
   int64_t blocks = ceil_div(most, tokens);
@@ -1846,7 +1847,7 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
   if ((rc = sm_count(&sms))) return rc;
   const int64_t rows = blocks * p->kv_heads * p->seqs.batch;
   a.block_pages = 256;
-  while (a.block_pages > 32 && rows * ceil_div(p->seqs.table_width, a.block_pages) < 3 * sms)
+  while (a.block_pages > 32 && rows * ceil_div(p->seqs.table_width, a.block_pages) < 4 * sms)
     a.block_pages /= 2;
   cudaError_t e = ifa4::launch_page_scores_sm100(a, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "page_scores launch");
@@ -2029,8 +2030,7 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
                            p->k_stride_page, p->k_stride_t, p->k_stride_h, 16, "k")))
       return rc;
     int64_t blocks = ceil_div(most_k, 128);
-    static const int kWaves = getenv("IFA4_W") ? atoi(getenv("IFA4_W")) : 8;
-    const int64_t want = ceil_div(int64_t{kWaves} * sms, heads);
+    const int64_t want = ceil_div(8 * sms, heads);  // (measured: 52, 44 and 50 us with 4, 8 and 16)
     if (blocks > want) blocks = want;
     cudaError_t e = ifa4::launch_attention_mass_stream_sm100(a, static_cast<int>(blocks), tk16,
                                                              static_cast<cudaStream_t>(stream));

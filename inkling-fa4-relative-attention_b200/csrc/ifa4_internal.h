@@ -327,7 +327,6 @@ struct PageScoresKernelArgs {
   int row_blocks;            // blocks of rows of a sequence in the grid (strided over)
   int block_pages;           // pages of a block: 32, 64, 128 or 256
   float scale;
-  int* status;
 };
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream);
 

@@ -563,9 +563,11 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
         const uint32_t st = done % kStreamStages;
         if (!(ok = mbar_wait_warp(&full[st], (done / kStreamStages) & 1, ab))) break;
         const uint32_t base = smem_u32(ring + st * kStreamStage);
-        float acc[2][4];
+        float acc[2][4], half[2][4];  // two halves of the depth, which do not wait for one another
 #pragma unroll
-        for (int t = 0; t < 2; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = half[t][i] = 0.f;
         {
           const int mi = lane >> 3;  // which 8x8 matrix this lane addresses
           const int row = (mi >> 1) * 8 + (lane & 7);
@@ -575,10 +577,14 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
             uint32_t b0, b1, b2, b3;
             ldsm_x4(base + (chunk >> 3) * kStreamHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
                     b0, b1, b2, b3);
-            mma_bf16(acc[0], qa[kk], b0, b1);
-            mma_bf16(acc[1], qa[kk], b2, b3);
+            mma_bf16(kk & 1 ? half[0] : acc[0], qa[kk], b0, b1);
+            mma_bf16(kk & 1 ? half[1] : acc[1], qa[kk], b2, b3);
           }
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] += half[t][i];
         // the fragment loads have to be done, not only issued, before TMA refills the stage
         fence_proxy_async_smem();
         __syncwarp();

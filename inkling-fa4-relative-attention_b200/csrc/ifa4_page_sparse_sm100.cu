@@ -94,14 +94,14 @@ __global__ void __launch_bounds__(kPageBoundsWarps * 32)
 // they lie in memory, and runs on warp-level MMAs (16 rows: the heads of a group, of 16 / group
 // tokens; 8 pages a warp).  The order of the 128 dims is free as long as both operands have the same:
 // lane qd of a quad takes 16 contiguous bytes of every 64 from the bounds as they were copied.  Every warp
-// has a ring of its own, eight pages a stage, refilled by bulk copies (512 contiguous bytes a page) as
-// soon as it has read a stage.  The largest bias of a page is found by the whole block, 16 keys a
+// has a ring of its own, eight pages a stage, refilled by 16-byte asynchronous copies as soon as it has
+// read a stage (by bulk copies of 512 bytes: 99 us, the copy engine takes them one by one).  The largest bias of a page is found by the whole block, 16 keys a
 // thread at a time, for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for
 // 16 rows.  (64 sequences of up to 32k keys: 111 us with the bounds loaded straight to registers, 104
 // with the next eight pages loaded ahead.)
 constexpr int kScoreWarps = 4;
 constexpr int kScorePages = 256;  // most pages of a block
-constexpr int kScoreStages = 3;
+constexpr int kScoreStages = 2;
 // Pages of a stage lie 576 bytes apart: a lane's 16 bytes and those of the seven it reads with are in
 // different banks.
 constexpr uint32_t kScorePitch = 576;
@@ -109,24 +109,21 @@ constexpr uint32_t kScoreStage = 8 * kScorePitch;
 constexpr uint32_t kScoreRing = kScoreWarps * kScoreStages * kScoreStage;
 constexpr uint32_t kScoreBias = kScoreRing;
 constexpr uint32_t kScoreTile = kScoreBias + 16 * kScorePages * 4;
-constexpr uint32_t kScoreBar = kScoreTile + kScoreWarps * 16 * 9 * 4;
-constexpr uint32_t kScoreSmem = kScoreBar + kScoreWarps * kScoreStages * 12 + 16;
-static_assert(kScoreBar % 8 == 0, "barriers");
+constexpr uint32_t kScoreSmem = kScoreTile + kScoreWarps * 16 * 9 * 4;
 
-__device__ __forceinline__ float max_nan(float x, float y) { return y > x || y != y ? y : x; }
+__device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either is
+  float z;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(z) : "f"(x), "f"(y));
+  return z;
+}
 
-__global__ void __launch_bounds__(kScoreWarps * 32, 3)
+__global__ void __launch_bounds__(kScoreWarps * 32, 4)
     page_scores_kernel(const __grid_constant__ PageScoresKernelArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   uint32_t(&bias_rank)[16][kScorePages] =  // largest bias of a row in a page
       *reinterpret_cast<uint32_t(*)[16][kScorePages]>(smem + kScoreBias);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, qd = lane & 3;
   float(&tile)[16][9] = reinterpret_cast<float(*)[16][9]>(smem + kScoreTile)[warp];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kScoreBar) + warp * kScoreStages;
-  // pages of each stage that are none: their bounds are zeros
-  uint32_t* missing = reinterpret_cast<uint32_t*>(smem + kScoreBar + 8 * kScoreWarps * kScoreStages) +
-                      warp * kScoreStages;
-  int* abort_flag = reinterpret_cast<int*>(smem + kScoreBar + 12 * kScoreWarps * kScoreStages);
   uint8_t* ring = smem + warp * kScoreStages * kScoreStage;
   const int page0 = blockIdx.x * a.block_pages;
   const int kvh = blockIdx.y % a.kv_heads;
@@ -141,19 +138,22 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 3)
         a.scores[t * a.sc_st + kvh * a.sc_sh + c] = -INFINITY;
     return;
   }
-  if (lane == 0) {
-    for (int i = 0; i < kScoreStages; ++i) mbar_init(&full[i], 1);
-    if (warp == 0) *abort_flag = 0;
-    fence_mbar_init();
-  }
-  __syncthreads();
-  const AbortCtx ab{abort_flag, a.status, kStatusDecodeTimeout};
-  const uint64_t pol = l2_policy_evict_first();
   const int32_t* table = table_row(a.s, b);
   const int c_warp = page0 + warp * 8;
   constexpr int kStride = kScoreWarps * 8;
+  // what a lane copies: 16 bytes of every page (page strides are below 2^32 bytes)
+  const uint8_t* bounds_lane =
+      reinterpret_cast<const uint8_t*>(a.bounds + static_cast<long long>(kvh) * a.b_sh) + lane * 16;
+  const uint32_t page_bytes = static_cast<uint32_t>(a.b_sp * 2);
+  const uint32_t ring_lane = smem_u32(ring) + lane * 16;
   uint32_t done = 0;  // stages read so far: the ring goes on through all rounds
-  bool ok = true;
+  // the pages of the ring's first stages, whatever the lengths turn out to be
+  int first_pages[kScoreStages + 1];
+#pragma unroll
+  for (int i = 0; i <= kScoreStages; ++i) {
+    const int c = c_warp + i * kStride + lane;
+    first_pages[i] = lane < 8 && c < page1 ? page_at(a.s, table, c) : -1;
+  }
   const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
   const int hb = min(a.group, 16);          // heads of a row block
@@ -166,24 +166,28 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 3)
     // pages that any token sees
     const int c_lo = (a.window_left < 0 ? 0 : max(0, p0 - a.window_left)) >> shift;
     const int c_hi = p1 >= 0 ? p1 >> shift : -1;
+    // pages from here on are seen by every token's window and not among its first pages
+    const int c_first_seen =
+        ((a.window_left < 0 ? 0 : max(0, p1 - a.window_left)) >> shift) + max(1, a.first_pages);
     // eight pages of a warp's turn are read if any of them is seen
     const auto seen = [&](int c0) { return c0 < page1 && c0 <= c_hi && c0 + 7 >= c_lo; };
     const auto page_of = [&](int c0) {  // of lane's page, lanes 0 to 7
       return lane < 8 && seen(c0) && c0 + lane < page1 ? page_at(a.s, table, c0 + lane) : -1;
     };
+    // one group of copies a turn, empty past the last pages; no page: zeros
     const auto load = [&](int c0, int page, uint32_t st) {
-      if (!seen(c0)) return;
-      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0) {
-        missing[st] = ~there;
-        mbar_arrive_expect_tx(&full[st], __popc(there) * 512u);
+      if (seen(c0)) {
+        const uint32_t dst = ring_lane + st * kScoreStage;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int p = __shfl_sync(0xffffffffu, page, i);
+          cp_async16_or_zeros(dst + i * kScorePitch,
+                              bounds_lane + static_cast<uint64_t>(static_cast<uint32_t>(max(p, 0))) *
+                                                page_bytes,
+                              p >= 0);
+        }
       }
-      __syncwarp();
-      if (page >= 0)
-        bulk_load_hint(ring + st * kScoreStage + lane * kScorePitch,
-                       a.bounds + static_cast<long long>(page) * a.b_sp +
-                           static_cast<long long>(kvh) * a.b_sh,
-                       512, &full[st], pol);
+      cp_async_commit();
     };
     for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
       const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
@@ -197,10 +201,15 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 3)
       if (mine && c_first + 7 < c_lo) c_first += (c_lo - c_first - 7 + kStride - 1) / kStride * kStride;
       int page_next;
       {
-        int pages[kScoreStages];
+        int pages[kScoreStages + 1];
+        if (c_first == c_warp) {
 #pragma unroll
-        for (int i = 0; i < kScoreStages; ++i) pages[i] = page_of(c_first + i * kStride);
-        page_next = page_of(c_first + kScoreStages * kStride);
+          for (int i = 0; i <= kScoreStages; ++i) pages[i] = first_pages[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i <= kScoreStages; ++i) pages[i] = page_of(c_first + i * kStride);
+        }
+        page_next = pages[kScoreStages];
 #pragma unroll
         for (int i = 0; i < kScoreStages; ++i)
           load(c_first + i * kStride, pages[i], (done + i) % kScoreStages);
@@ -231,11 +240,14 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 3)
       const int slices = mine ? (min(p1, ((page1 - 1) << shift) + ((1 << shift) - 1)) >> 4) - slice0 + 1 : 0;
       if (slices > 0) {
         const int c_near = near >> shift;
-        for (int i = threadIdx.x; i < 16 * (page1 - c_near); i += kScoreWarps * 32) {
-          const int row = i / (page1 - c_near), c = c_near + i - row * (page1 - c_near);
-          int d1 = p0 + token_of(row) - (c << shift);  // the furthest key of the page
-          if (a.window_left >= 0) d1 = min(d1, a.window_left);
-          bias_rank[row][c - page0] = d1 >= a.rel_extent ? rank_of(0.f) : 0u;
+        const int c_end = min(page1 - 1, c_hi);
+        for (int row = 0; row < n_rows; ++row) {
+          const int p = p0 + token_of(row);
+          for (int c = c_near + static_cast<int>(threadIdx.x); c <= c_end; c += kScoreWarps * 32) {
+            int d1 = p - (c << shift);  // the furthest key of the page
+            if (a.window_left >= 0) d1 = min(d1, a.window_left);
+            bias_rank[row][c - page0] = d1 >= a.rel_extent ? kRankZero : 0u;
+          }
         }
         __syncthreads();
         for (int i = threadIdx.x; i < n_rows * slices; i += kScoreWarps * 32) {
@@ -259,88 +271,138 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 3)
         __syncthreads();
       }
       // ---- scores
-      for (int c0 = c_warp; c0 < page1; c0 += kStride) {
-        float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // outputs lane, lane + 32, ..
-        if (seen(c0) && ok) {
-          const uint32_t st = done % kScoreStages;
-          ok = mbar_wait_warp(&full[st], (done / kScoreStages) & 1, ab);
-          if (!ok) continue;
-          const bool none = missing[st] >> g & 1u;
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          const uint8_t* src = ring + st * kScoreStage + g * kScorePitch + qd * 16;
+      // a power of two of heads lie in lanes that shuffles reach; others go through shared memory
+      const bool by_shuffle = (hb & (hb - 1)) == 0 && (a.group <= 16 || n_rows == 16);
+      // stores the largest over the heads of a token, of all pages that the block has
+      const auto store = [&](int tok, int c, float y) {
+        float* dst = a.scores + (q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c;
+        if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by the same thread
+        if (h0 + 16 >= a.group && p0 + tok >= 0) {
+          const int p = p0 + tok, hi = p >> shift;
+          const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> shift;
+          if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages)) y = INFINITY;
+        }
+        *dst = y;
+      };
+      // where this lane stores the scores of pages 2 qd, 2 qd + 1: the tokens of rows g and g + 8
+      const int lanes = min(hb, 8);  // rows of a token among lanes
+      int tok_out[2];
+      float* out[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint4 lo = *reinterpret_cast<const uint4*>(src + i * 64);
-            uint4 hi = *reinterpret_cast<const uint4*>(src + 256 + i * 64);
-            if (none) lo = hi = make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t pa[4] = {qp[i][0].x, qp[i][1].x, qp[i][0].y, qp[i][1].y};
-            const uint32_t pb[4] = {qp[i][0].z, qp[i][1].z, qp[i][0].w, qp[i][1].w};
-            const uint32_t ma[4] = {qm[i][0].x, qm[i][1].x, qm[i][0].y, qm[i][1].y};
-            const uint32_t mb[4] = {qm[i][0].z, qm[i][1].z, qm[i][0].w, qm[i][1].w};
-            mma_bf16(acc, pa, hi.x, hi.y);
-            mma_bf16(acc, pb, hi.z, hi.w);
-            mma_bf16(acc, ma, lo.x, lo.y);
-            mma_bf16(acc, mb, lo.z, lo.w);
+      for (int r = 0; r < 2; ++r) {
+        const int tok = hb == 16 ? r : token_of(g + 8 * r);
+        tok_out[r] = (g & (lanes - 1)) == 0 && tok < n_tok ? tok : -1;
+        out[r] = a.scores + (q0 + tok0 + max(tok_out[r], 0)) * a.sc_st + kvh * a.sc_sh + 2 * qd;
+      }
+      for (int c0 = c_warp; c0 < page1; c0 += kStride) {
+        if (!seen(c0)) {
+          for (int i = lane; i < 8 * n_tok; i += 32)
+            if (c0 + (i & 7) < page1) store(i >> 3, c0 + (i & 7), -INFINITY);
+          continue;
+        }
+        const uint32_t st = done % kScoreStages;
+        cp_async_wait<kScoreStages - 1>();
+        __syncwarp();
+        float part[4][4];  // four products of depth 64, which do not wait for one another
+        const uint8_t* src = ring + st * kScoreStage + g * kScorePitch + qd * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 lo = *reinterpret_cast<const uint4*>(src + i * 64);
+          const uint4 hi = *reinterpret_cast<const uint4*>(src + 256 + i * 64);
+          const uint32_t pa[4] = {qp[i][0].x, qp[i][1].x, qp[i][0].y, qp[i][1].y};
+          const uint32_t pb[4] = {qp[i][0].z, qp[i][1].z, qp[i][0].w, qp[i][1].w};
+          const uint32_t ma[4] = {qm[i][0].x, qm[i][1].x, qm[i][0].y, qm[i][1].y};
+          const uint32_t mb[4] = {qm[i][0].z, qm[i][1].z, qm[i][0].w, qm[i][1].w};
+          if (i == 0) {
+            mma_bf16_first(part[0], pa, hi.x, hi.y);
+            mma_bf16_first(part[1], pb, hi.z, hi.w);
+            mma_bf16_first(part[2], ma, lo.x, lo.y);
+            mma_bf16_first(part[3], mb, lo.z, lo.w);
+          } else {
+            mma_bf16(part[0], pa, hi.x, hi.y);
+            mma_bf16(part[1], pb, hi.z, hi.w);
+            mma_bf16(part[2], ma, lo.x, lo.y);
+            mma_bf16(part[3], mb, lo.z, lo.w);
           }
-          // the stage has been read, not only asked for, before it is filled again
-          fence_proxy_async_smem();
-          __syncwarp();
-          ++done;
-          load(c0 + kScoreStages * kStride, page_next, st);
-          page_next = page_of(c0 + (kScoreStages + 1) * kStride);
-          // acc[2 r + e] is row g + 8 r, page 2 qd + e
+        }
+        __syncwarp();  // the stage has been read
+        ++done;
+        load(c0 + kScoreStages * kStride, page_next, st);
+        page_next = page_of(c0 + (kScoreStages + 1) * kStride);
+        float y[4];  // y[2 r + e] is row g + 8 r, page 2 qd + e
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          y[i] = ((part[0][i] + part[1][i]) + (part[2][i] + part[3][i])) * a.scale;
+        // whether every row sees all eight pages, without a bias, and none is taken always
+        const int c_near = (p0 - a.rel_extent + 1) >> shift;  // the first page within the bias's reach
+        const bool inside =
+            p0 >= a.rel_extent && c0 + 7 < c_near && c0 >= c_first_seen && h0 == 0 &&
+            a.group <= 16 && c0 + 7 < page1 && c0 + 7 <= (p0 >> shift) - a.last_pages;
+        if (!inside) {
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = c0 + 2 * qd + e;
-              float y = -INFINITY;
+              float x = -INFINITY;
               if (on[r] && pos[r] >= 0 && c < page1 && c <= pos[r] >> shift) {
                 // distance of the page's nearest key
                 const int d0 = max(0, pos[r] - ((c << shift) + ((1 << shift) - 1)));
                 if (a.window_left < 0 || d0 <= a.window_left) {
-                  y = acc[2 * r + e] * a.scale;
-                  if (d0 < a.rel_extent) y += value_of(bias_rank[g + 8 * r][c - page0]);
+                  x = y[2 * r + e];
+                  if (d0 < a.rel_extent) x += value_of(bias_rank[g + 8 * r][c - page0]);
                 }
               }
-              tile[g + 8 * r][2 * qd + e] = y;
+              y[2 * r + e] = x;
             }
-          __syncwarp();
-          // largest over the heads of a token: output o is token o / 8, page o % 8
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int tok = (lane + 32 * k) >> 3, pg = lane & 7;
-            const int heads = a.group <= 16 ? hb : n_rows;
-            if (tok < n_tok)
-              for (int r = 0; r < heads; ++r) best[k] = max_nan(best[k], tile[tok * heads + r][pg]);
-          }
-          __syncwarp();
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = (lane + 32 * k) >> 3, c = c0 + (lane & 7);
-          if (tok < n_tok && c < page1) {
-            float* dst = a.scores + (q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c;
-            float y = best[k];
-            if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by this thread
-            const int p = p0 + tok;
-            if (h0 + 16 >= a.group && p >= 0) {
-              const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> shift;
-              const int hi = p >> shift;
-              if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages))
-                y = INFINITY;
+        if (by_shuffle) {
+          const auto across = [&](int m) {  // rows 8 to 15 only where there are some
+            y[0] = max_nan(y[0], __shfl_xor_sync(0xffffffffu, y[0], m));
+            y[1] = max_nan(y[1], __shfl_xor_sync(0xffffffffu, y[1], m));
+            if (n_rows > 8) {
+              y[2] = max_nan(y[2], __shfl_xor_sync(0xffffffffu, y[2], m));
+              y[3] = max_nan(y[3], __shfl_xor_sync(0xffffffffu, y[3], m));
             }
-            *dst = y;
+          };
+          if (lanes >= 2) {
+            across(4);
+            if (lanes >= 4) across(8);
+            if (lanes == 8) across(16);
           }
+          if (hb == 16) {
+            y[0] = max_nan(y[0], y[2]);
+            y[1] = max_nan(y[1], y[3]);
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            if (tok_out[r] < 0) continue;
+            if (inside) {
+              out[r][c0] = y[2 * r];
+              out[r][c0 + 1] = y[2 * r + 1];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (c0 + 2 * qd + e < page1) store(tok_out[r], c0 + 2 * qd + e, y[2 * r + e]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tile[g + 8 * (i >> 1)][2 * qd + (i & 1)] = y[i];
+          __syncwarp();
+          const int heads = a.group <= 16 ? hb : n_rows;
+          for (int i = lane; i < 8 * n_tok; i += 32) {
+            const int tok = i >> 3, pg = i & 7;
+            float x = -INFINITY;
+            for (int r = 0; r < heads; ++r) x = max_nan(x, tile[tok * heads + r][pg]);
+            if (c0 + pg < page1) store(tok, c0 + pg, x);
+          }
+          __syncwarp();
         }
       }
       if (rb + a.row_blocks < (n_q + tokens - 1) / tokens || h0 + 16 < a.group) __syncthreads();
     }
   }
-  // after a wait that was given up: what is in flight has landed before the memory goes
-  if (!ok && lane == 0)
-    for (uint32_t i = 0; i < kScoreStages; ++i)
-      mbar_wait(&full[(done + i) % kScoreStages], ((done + i) / kScoreStages) & 1, ab);
 }
 
 // ---------------------------------------------------------------------------------------
