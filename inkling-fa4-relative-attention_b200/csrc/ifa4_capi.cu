@@ -1702,11 +1702,23 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
   } else {
     int sms = 148;
     if ((rc = sm_count(&sms))) return rc;
-    // two CTAs an SM; a split of fewer than four tiles spends its time on starting and merging
-    int64_t s = 2 * sms / rows;
-    if (s > tiles / 4) s = tiles / 4;
-    if (s > 64) s = 64;
-    *splits = static_cast<int>(s < 1 ? 1 : s);
+    // An estimate in ns, from measured times: two CTAs an SM share the HBM bandwidth (5 ns a tile of 64
+    // keys and CTA), a CTA alone takes 830 ns a tile; a round of CTAs costs 5 us besides, the merge
+    // 0.5 us and 0.15 us a split.  (64 rows x 8 heads of 256 pages of 16: 177 us whole, 189 in two; 48
+    // of 128 pages: 91 and 80; 16 of 64 pages: 22.4 and 18.7; one: 21.2 whole, 10.5 in eight, 11.2 in
+    // sixteen.)
+    const int64_t slots = 2 * sms;
+    int64_t best = 0;
+    for (int s = 1; s <= 64 && s <= (tiles > 0 ? tiles : 1); ++s) {
+      const int64_t per = ceil_div(tiles, s), ctas = rows * s;
+      const int64_t full = ctas / slots, rest = ctas % slots;
+      int64_t t = full * (5 * slots * per + 5000) + (s > 1 ? 500 + 150 * s : 0);
+      if (rest > 0) t += (5 * rest > 830 ? 5 * rest : 830) * per + 5000;
+      if (s == 1 || t < best) {
+        best = t;
+        *splits = s;
+      }
+    }
   }
   if (d->total_q * *splits > 0x7fffffff || ceil_div(d->total_q * d->n_heads, 4) > 0x7fffffff)
     return fail(IFA4_ERR_UNSUPPORTED, "%s: too many rows", what);

@@ -486,22 +486,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int h0 = kvh * a.group + hblk * a.heads_per_cta;
   const int nh = min(a.heads_per_cta, a.group - hblk * a.heads_per_cta);
   if (a.num_splits > 1) launch_dependents();
-  const int b = find_sequence(a.s.cu_q, a.s.batch, t);
-  if (b < 0) {
-    if (a.num_splits > 1) return;  // the merge writes such rows
-    if (!a.zero_padding) return;
-    for (int i = threadIdx.x; i < nh * 128; i += kThreads)
-      a.out[t * a.out_st + static_cast<long long>(h0 + (i >> 7)) * a.out_sh + (i & 127)] = 0;
-    if (a.lse != nullptr && threadIdx.x < nh)
-      a.lse[static_cast<long long>(h0 + threadIdx.x) * a.lse_sh + t * a.lse_st] = -INFINITY;
-    return;
-  }
-  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
-  const int pos = n_k - __ldg(a.s.cu_q + b + 1) + static_cast<int>(t);
-  const int hi = pos + 1;  // visible keys [lo, hi); none where hi <= 0
-  const int lo = a.window_left >= 0 ? max(0, pos - a.window_left) : 0;
-  const int c_lo = lo >> a.s.page_shift, c_hi = hi > 0 ? pos >> a.s.page_shift : -1;
+  // the list's first entries, on their way while the sequence is looked up
   const int32_t* list = a.pages + t * a.pg_st + kvh * a.pg_sh;
+  const int entry0 = threadIdx.x < a.num_selected ? __ldg(list + threadIdx.x) : -1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars->full[i], 1);
@@ -511,10 +498,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     bars->last = -1;
     fence_mbar_init();
   }
+  int n_k, pos;
+  const int b = find_sequence(a.s, t, n_k, pos);
+  if (b < 0) {
+    if (a.num_splits > 1) return;  // the merge writes such rows
+    if (!a.zero_padding) return;
+    for (int i = threadIdx.x; i < nh * 128; i += kThreads)
+      a.out[t * a.out_st + static_cast<long long>(h0 + (i >> 7)) * a.out_sh + (i & 127)] = 0;
+    if (a.lse != nullptr && threadIdx.x < nh)
+      a.lse[static_cast<long long>(h0 + threadIdx.x) * a.lse_sh + t * a.lse_st] = -INFINITY;
+    return;
+  }
+  const int hi = pos + 1;  // visible keys [lo, hi); none where hi <= 0
+  const int lo = a.window_left >= 0 ? max(0, pos - a.window_left) : 0;
+  const int c_lo = lo >> a.s.page_shift, c_hi = hi > 0 ? pos >> a.s.page_shift : -1;
   __syncthreads();
   {
-    int last = -1;
-    for (int e = threadIdx.x; e < a.num_selected; e += kThreads) {
+    int last = entry0 >= c_lo && entry0 <= c_hi ? static_cast<int>(threadIdx.x) : -1;
+    for (int e = threadIdx.x + kThreads; e < a.num_selected; e += kThreads) {
       const int c = __ldg(list + e);
       if (c >= c_lo && c <= c_hi) last = e;
     }
@@ -812,7 +813,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   if (at >= a.total_q * a.n_heads) return;
   const long long t = at / a.n_heads;
   const int h = static_cast<int>(at - t * a.n_heads);
-  const bool none = find_sequence(a.s.cu_q, a.s.batch, t) < 0;
+  int n_k, pos;
+  const bool none = find_sequence(a.s, t, n_k, pos) < 0;
   if (none && !a.zero_padding) return;
   wait_previous_kernel();
   float M = -INFINITY, L = 0.f;

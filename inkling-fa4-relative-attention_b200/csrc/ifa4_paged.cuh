@@ -9,24 +9,32 @@
 
 namespace ifa4 {
 
-// Sequence of row t: cu_q[b] <= t < cu_q[b + 1], -1 for a row of none.  Whole warp; 32 places are
-// looked at a time (one step for up to 33 sequences, two for 1057).
-__device__ __forceinline__ int find_sequence(const int32_t* cu_q, int batch, long long t) {
+// Sequence b of row t (cu_q[b] <= t < cu_q[b + 1]), its key count and the row's position; -1 for a row
+// of none.  Whole warp; one load for a decode batch (one row a sequence), otherwise 32 places are looked
+// at a time (one step for up to 33 sequences, two for 1057) and a load for the lengths follows.
+__device__ __forceinline__ int find_sequence(const PagedSeqs& s, long long t, int& n_k, int& pos) {
   const int lane = threadIdx.x & 31;
-  // one sequence a row is the usual decode batch
-  const int guess = t < batch ? static_cast<int>(t) : batch - 1;
-  const int32_t ends = __ldg(cu_q + (lane == 0 ? 0 : lane == 1 ? batch : guess + (lane & 1)));
+  const int guess = t < s.batch ? static_cast<int>(t) : s.batch - 1;
+  const int32_t ends = lane < 4 ? __ldg(s.cu_q + (lane == 0 ? 0 : lane == 1 ? s.batch : guess + lane - 2))
+                                : __ldg(s.cu_k + guess + (lane & 1));
   if (t < __shfl_sync(0xffffffffu, ends, 0) || t >= __shfl_sync(0xffffffffu, ends, 1)) return -1;
-  if (__shfl_sync(0xffffffffu, ends, 2) <= t && t < __shfl_sync(0xffffffffu, ends, 3)) return guess;
-  int lo = 0, hi = batch;  // cu_q[lo] <= t < cu_q[hi]
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int at = min(lo + (lane + 1) * step, hi);
-    const unsigned le = __ballot_sync(0xffffffffu, at < hi && __ldg(cu_q + at) <= t);
-    const int n = __popc(le);  // offsets ascend: the first n places
-    hi = min(lo + (n + 1) * step, hi);
-    lo += n * step;
+  int lo = guess, q_end = __shfl_sync(0xffffffffu, ends, 3);
+  n_k = __shfl_sync(0xffffffffu, ends, 5) - __shfl_sync(0xffffffffu, ends, 4);
+  if (t < __shfl_sync(0xffffffffu, ends, 2) || t >= q_end) {
+    lo = 0;
+    int hi = s.batch;  // cu_q[lo] <= t < cu_q[hi]
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32;
+      const int at = min(lo + (lane + 1) * step, hi);
+      const unsigned le = __ballot_sync(0xffffffffu, at < hi && __ldg(s.cu_q + at) <= t);
+      const int n = __popc(le);  // offsets ascend: the first n places
+      hi = min(lo + (n + 1) * step, hi);
+      lo += n * step;
+    }
+    q_end = __ldg(s.cu_q + lo + 1);
+    n_k = __ldg(s.cu_k + lo + 1) - __ldg(s.cu_k + lo);
   }
+  pos = n_k - q_end + static_cast<int>(t);
   return lo;
 }
 
