@@ -1704,15 +1704,16 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
     if ((rc = sm_count(&sms))) return rc;
     // An estimate in ns, from measured times: two CTAs an SM share the HBM bandwidth (5 ns a tile of 64
     // keys and CTA), a CTA alone takes 830 ns a tile; a round of CTAs costs 5 us besides, the merge
-    // 0.5 us and 0.15 us a split.  (64 rows x 8 heads of 256 pages of 16: 177 us whole, 189 in two; 48
-    // of 128 pages: 91 and 80; 16 of 64 pages: 22.4 and 18.7; one: 21.2 whole, 10.5 in eight, 11.2 in
-    // sixteen.)
+    // 0.5 us and 0.15 us a split, 2.5 us more through a workspace.  (64 rows x 8 heads of 256 pages of
+    // 16: 177 us whole, 196 in two; 48 of 128 pages: 92 and 82; 16 of 64 pages: 22.2 and 17.5; one:
+    // 21.2 whole, 7.7 in eight, 11.1 in sixteen.)
     const int64_t slots = 2 * sms;
     int64_t best = 0;
     for (int s = 1; s <= 64 && s <= (tiles > 0 ? tiles : 1); ++s) {
       const int64_t per = ceil_div(tiles, s), ctas = rows * s;
       const int64_t full = ctas / slots, rest = ctas % slots;
-      int64_t t = full * (5 * slots * per + 5000) + (s > 1 ? 500 + 150 * s : 0);
+      int64_t t = full * (5 * slots * per + 5000) + (s > 1 ? 500 + 150 * s : 0) +
+                  (s > ifa4::kDecodePagesCluster ? 2500 : 0);
       if (rest > 0) t += (5 * rest > 830 ? 5 * rest : 830) * per + 5000;
       if (s == 1 || t < best) {
         best = t;
@@ -1722,7 +1723,7 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
   }
   if (d->total_q * *splits > 0x7fffffff || ceil_div(d->total_q * d->n_heads, 4) > 0x7fffffff)
     return fail(IFA4_ERR_UNSUPPORTED, "%s: too many rows", what);
-  if (*splits > 1) {
+  if (*splits > ifa4::kDecodePagesCluster) {
     const size_t parts = static_cast<size_t>(d->total_q) * d->n_heads * *splits;
     *bytes = parts * 130 * sizeof(float);
   }
@@ -1959,7 +1960,7 @@ int ifa4_decode_pages_launch(const IFA4DecodePagesParams* p, void* workspace,
   a.num_splits = splits;
   a.zero_padding = p->zero_padding != 0;
   a.scale_log2 = d->softmax_scale * 1.4426950408889634f;
-  if (splits > 1) {
+  if (bytes > 0) {
     a.ws_o = static_cast<float*>(workspace);
     a.ws_ml = a.ws_o + static_cast<size_t>(d->total_q) * d->n_heads * splits * 128;
   }

@@ -351,12 +351,14 @@ struct DecodePagesKernelArgs {
   int group, heads_per_cta;  // as in DecodeKernelArgs
   int num_selected, num_splits, box_shift, zero_padding;
   float scale_log2;
-  float* ws_o;               // [total_q, n_heads, num_splits, 128] (num_splits > 1)
+  float* ws_o;               // [total_q, n_heads, num_splits, 128] (null: one split, or a cluster)
   float* ws_ml;              // [total_q, n_heads, num_splits, 2]: largest score (log2 units), sum
   float* lse;                // optional natural-log LSE
   long long lse_sh, lse_st;
   int* status;
 };
+// Splits of a row that merge in each other's shared memory; more go through a workspace.
+constexpr int kDecodePagesCluster = 8;
 cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const CUtensorMap& tm_k,
                                       const CUtensorMap& tm_v, cudaStream_t stream);
 

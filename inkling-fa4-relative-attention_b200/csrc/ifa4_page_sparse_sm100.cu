@@ -468,6 +468,8 @@ __device__ __forceinline__ float add_bias(float x, float bias) {
   return isinf(y) && isfinite(bias) && isfinite(x) ? copysignf(3.402823466e38f, y) : y;
 }
 
+// kCluster: the num_splits CTAs of a row are a cluster and merge in each other's shared memory.
+template <bool kCluster>
 __global__ void __launch_bounds__(kThreads, 2)
     decode_pages_kernel(const __grid_constant__ DecodePagesKernelArgs a,
                         const __grid_constant__ CUtensorMap tm_k,
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int hblk = blockIdx.y % head_blocks;
   const int h0 = kvh * a.group + hblk * a.heads_per_cta;
   const int nh = min(a.heads_per_cta, a.group - hblk * a.heads_per_cta);
-  if (a.num_splits > 1) launch_dependents();
+  if (!kCluster && a.num_splits > 1) launch_dependents();
   // the list's first entries, on their way while the sequence is looked up
   const int32_t* list = a.pages + t * a.pg_st + kvh * a.pg_sh;
   const int entry0 = threadIdx.x < a.num_selected ? __ldg(list + threadIdx.x) : -1;
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   int n_k, pos;
   const int b = find_sequence(a.s, t, n_k, pos);
   if (b < 0) {
-    if (a.num_splits > 1) return;  // the merge writes such rows
+    if (kCluster ? split > 0 : a.num_splits > 1) return;  // the merge kernel writes such rows
     if (!a.zero_padding) return;
     for (int i = threadIdx.x; i < nh * 128; i += kThreads)
       a.out[t * a.out_st + static_cast<long long>(h0 + (i >> 7)) * a.out_sh + (i & 127)] = 0;
@@ -762,6 +764,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   __syncthreads();
+  float* part_o = ml + kConsumerWarps * 16;                                  // [16][128]
+  float2* part_ml = reinterpret_cast<float2*>(part_o + 16 * 128);            // [16]
   // one warp per row, lanes own 4 of the 128 dims
   for (int row = warp; row < nh; row += kConsumerWarps + 1) {
     float M = -INFINITY;
@@ -788,7 +792,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     acc.y *= inv;
     acc.z *= inv;
     acc.w *= inv;
-    if (!IFA4_DBG_CHECK(a.status, t < a.total_q && h < a.n_heads)) {
+    if (kCluster) {  // for the merge below
+      reinterpret_cast<float4*>(part_o + row * 128)[lane] = acc;
+      if (lane == 0) part_ml[row] = make_float2(L == 0.f ? -INFINITY : base, L);
+    } else if (!IFA4_DBG_CHECK(a.status, t < a.total_q && h < a.n_heads)) {
       // a bad row or head: nothing is stored
     } else if (a.num_splits == 1) {
       *reinterpret_cast<uint2*>(a.out + t * a.out_st + static_cast<long long>(h) * a.out_sh +
@@ -802,9 +809,44 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) reinterpret_cast<float2*>(a.ws_ml)[at] = make_float2(L == 0.f ? -INFINITY : base, L);
     }
   }
+  if constexpr (kCluster) {
+    // The splits of a row are a cluster: each CTA merges some of the rows out of the others' memory
+    // (weights L_s 2^(m_s - max m)), with no second kernel and no workspace.
+    cluster_sync();
+    for (int row = split + warp * a.num_splits; row < nh;
+         row += (kConsumerWarps + 1) * a.num_splits) {
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = 0; s < a.num_splits; ++s)
+        M = fmaxf(M, load_cluster(&part_ml[row].x, s));
+      if (M != -INFINITY) {
+        for (int s = 0; s < a.num_splits; ++s) {
+          const float m = load_cluster(&part_ml[row].x, s), l = load_cluster(&part_ml[row].y, s);
+          const float w = m == -INFINITY ? 0.f : l * fast_exp2(m - M);  // NaN stays
+          const float4 o4 = load_cluster_v4(part_o + row * 128 + lane * 4, s);
+          L += w;
+          acc.x += w * o4.x;
+          acc.y += w * o4.y;
+          acc.z += w * o4.z;
+          acc.w += w * o4.w;
+        }
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const int h = h0 + row;
+      if (!IFA4_DBG_CHECK(a.status, t < a.total_q && h < a.n_heads)) continue;
+      *reinterpret_cast<uint2*>(a.out + t * a.out_st + static_cast<long long>(h) * a.out_sh +
+                                lane * 4) =
+          make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      if (lane == 0 && a.lse != nullptr)
+        a.lse[static_cast<long long>(h) * a.lse_sh + t * a.lse_st] =
+            L == 0.f ? -INFINITY : (M + __log2f(L)) * kLn2;
+    }
+    cluster_sync();  // nobody reads this CTA's memory any more
+  }
 }
 
-// Merge of num_splits normalised partials: a warp per row and head, weights L_s 2^(m_s - max m).
+// Merge of num_splits normalised partials through the workspace, for more splits than a cluster has: a
+// warp per row and head, weights L_s 2^(m_s - max m).
 constexpr int kMergeWarps = 4;
 __global__ void __launch_bounds__(kMergeWarps * 32)
     decode_pages_merge_kernel(const __grid_constant__ DecodePagesKernelArgs a) {
@@ -879,14 +921,30 @@ cudaError_t launch_select_pages_sm100(const SelectPagesKernelArgs& args, cudaStr
 
 cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const CUtensorMap& tm_k,
                                       const CUtensorMap& tm_v, cudaStream_t stream) {
-  static std::atomic<bool> attr[64];
-  cudaError_t e = set_smem_limit_once(sparse::decode_pages_kernel, sparse::kSmemAlloc, attr);
+  static std::atomic<bool> attr[64], attr_cluster[64];
+  const bool cluster = args.num_splits > 1 && args.ws_o == nullptr;
+  const auto kernel =
+      cluster ? sparse::decode_pages_kernel<true> : sparse::decode_pages_kernel<false>;
+  cudaError_t e = set_smem_limit_once(kernel, sparse::kSmemAlloc, cluster ? attr_cluster : attr);
   if (e != cudaSuccess) return e;
   const int head_blocks = (args.group + args.heads_per_cta - 1) / args.heads_per_cta;
   const dim3 grid(static_cast<unsigned>(args.total_q * args.num_splits),
                   args.kv_heads * head_blocks);
-  sparse::decode_pages_kernel<<<grid, sparse::kThreads, sparse::kSmemAlloc, stream>>>(args, tm_k,
-                                                                                      tm_v);
+  if (cluster) {
+    cudaLaunchAttribute dims;
+    dims.id = cudaLaunchAttributeClusterDimension;
+    dims.val.clusterDim.x = args.num_splits;
+    dims.val.clusterDim.y = dims.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(sparse::kThreads);
+    cfg.dynamicSmemBytes = sparse::kSmemAlloc;
+    cfg.stream = stream;
+    cfg.attrs = &dims;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args, tm_k, tm_v);
+  }
+  kernel<<<grid, sparse::kThreads, sparse::kSmemAlloc, stream>>>(args, tm_k, tm_v);
   e = cudaGetLastError();
   if (e != cudaSuccess || args.num_splits == 1) return e;
   const long long warps = args.total_q * args.n_heads;

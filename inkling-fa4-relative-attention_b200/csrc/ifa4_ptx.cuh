@@ -622,6 +622,31 @@ __device__ __forceinline__ void wait_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Thread-block clusters: a barrier of all their threads (what was written before it is visible after
+// it), and loads from the shared memory of another CTA, at the address that p has in this one.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float load_cluster(const float* p, uint32_t rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_address(p, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ float4 load_cluster_v4(const float* p, uint32_t rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(cluster_address(p, rank))
+               : "memory");
+  return x;
+}
+
 // Warpgroup-wide register re-split (every warp of the warpgroup executes it; the sum over the
 // CTA's warps must fit in the registers the CTA was launched with).
 template <uint32_t kRegs>

@@ -139,13 +139,13 @@ def test_decode_pages_refusals(kw, code, msg):
 def test_decode_pages_workspace():
     need = ctypes.c_size_t(0)
     L = _lib.lib()
-    for splits, want in ((1, 0), (2, 3 * 4 * 2 * 130 * 4), (64, 3 * 4 * 64 * 130 * 4)):
+    for splits, want in ((1, 0), (8, 0), (9, 3 * 4 * 9 * 130 * 4), (64, 3 * 4 * 64 * 130 * 4)):
         assert L.ifa4_decode_pages_workspace_size(ctypes.byref(_decode_pages(num_splits=splits)),
                                                   ctypes.byref(need)) == 0
         assert need.value == want
-    _refused("ifa4_decode_pages_launch", _decode_pages(), WORKSPACE, b"workspace", None,
-             ctypes.c_size_t(0), None)
-    _refused("ifa4_decode_pages_launch", _decode_pages(), WORKSPACE, b"aligned", ctypes.c_void_p(264),
+    many = _decode_pages(num_splits=9)
+    _refused("ifa4_decode_pages_launch", many, WORKSPACE, b"workspace", None, ctypes.c_size_t(0), None)
+    _refused("ifa4_decode_pages_launch", many, WORKSPACE, b"aligned", ctypes.c_void_p(264),
              ctypes.c_size_t(1 << 20), None)
 
 
