@@ -117,6 +117,9 @@ __device__ __forceinline__ float max_nan(float x, float y) {  // NaN if either i
   return z;
 }
 
+// kHeads: query heads of a KV head, where they are a power of two up to 16 (their largest score is found
+// by shuffles); 0: any number, 16 at a time, through shared memory.
+template <int kHeads>
 __global__ void __launch_bounds__(kScoreWarps * 32, 4)
     page_scores_kernel(const __grid_constant__ PageScoresKernelArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -156,7 +159,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
   }
   const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
-  const int hb = min(a.group, 16);          // heads of a row block
+  const int group = kHeads > 0 ? kHeads : a.group;
+  const int hb = min(group, 16);            // heads of a row block
   const int tokens = 16 / hb;               // and tokens
   for (int rb = rb0; rb * tokens < n_q; rb += a.row_blocks) {
     const int tok0 = rb * tokens;
@@ -166,14 +170,25 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
     // pages that any token sees
     const int c_lo = (a.window_left < 0 ? 0 : max(0, p0 - a.window_left)) >> shift;
     const int c_hi = p1 >= 0 ? p1 >> shift : -1;
-    // pages from here on are seen by every token's window and not among its first pages
-    const int c_first_seen =
-        ((a.window_left < 0 ? 0 : max(0, p1 - a.window_left)) >> shift) + max(1, a.first_pages);
     // eight pages of a warp's turn are read if any of them is seen
-    const auto seen = [&](int c0) { return c0 < page1 && c0 <= c_hi && c0 + 7 >= c_lo; };
-    const auto page_of = [&](int c0) {  // of lane's page, lanes 0 to 7
-      return lane < 8 && seen(c0) && c0 + lane < page1 ? page_at(a.s, table, c0 + lane) : -1;
+    const int c_last = min(c_hi, page1 - 1);
+    const auto seen = [&](int c0) { return c0 <= c_last && c0 + 7 >= c_lo; };
+    const int lane_page = lane < 8 ? lane : 1 << 28;
+    const auto page_of = [&](int c0) {  // of lane's page, lanes 0 to 7; pages that nobody sees are none
+      const int c = c0 + lane_page;
+      int p = -1;
+      if (c >= c_lo && c <= c_last) p = __ldg(table + c);
+      return static_cast<unsigned>(p) < static_cast<unsigned>(a.s.num_pages) ? p : -1;
     };
+    // Turns in which every row sees all eight pages, without a bias, and none is taken always: from
+    // the last token's first pages on (all but the first first_pages) up to those within the bias's
+    // reach of the first token
+    const int c_inside =
+        ((a.window_left < 0 ? 0 : max(0, p1 - a.window_left)) >> shift) + max(1, a.first_pages);
+    const int c_inside_end =
+        p0 < a.rel_extent || group > 16
+            ? -1
+            : min(min((p0 - a.rel_extent + 1) >> shift, page1), (p0 >> shift) - a.last_pages + 1) - 8;
     // one group of copies a turn, empty past the last pages; no page: zeros
     const auto load = [&](int c0, int page, uint32_t st) {
       if (seen(c0)) {
@@ -189,12 +204,12 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
       }
       cp_async_commit();
     };
-    for (int h0 = 0; h0 < a.group; h0 += 16) {  // one turn for groups of up to 16
-      const int n_rows = a.group <= 16 ? n_tok * hb : min(16, a.group - h0);
+    for (int h0 = 0; h0 < group; h0 += 16) {  // one turn for groups of up to 16
+      const int n_rows = group <= 16 ? n_tok * hb : min(16, group - h0);
       // row -> token, head
-      const auto token_of = [&](int row) { return a.group <= 16 ? row / hb : 0; };
+      const auto token_of = [&](int row) { return group <= 16 ? row / hb : 0; };
       const auto head_of = [&](int row, int tok) {
-        return kvh * a.group + (a.group <= 16 ? row - tok * hb : h0 + row);
+        return kvh * group + (group <= 16 ? row - tok * hb : h0 + row);
       };
       const bool mine = c_lo < page1 && c_hi >= page0;
       int c_first = c_warp;  // the first pages of this warp that are seen
@@ -271,13 +286,11 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
         __syncthreads();
       }
       // ---- scores
-      // a power of two of heads lie in lanes that shuffles reach; others go through shared memory
-      const bool by_shuffle = (hb & (hb - 1)) == 0 && (a.group <= 16 || n_rows == 16);
       // stores the largest over the heads of a token, of all pages that the block has
       const auto store = [&](int tok, int c, float y) {
         float* dst = a.scores + (q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c;
         if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by the same thread
-        if (h0 + 16 >= a.group && p0 + tok >= 0) {
+        if (h0 + 16 >= group && p0 + tok >= 0) {
           const int p = p0 + tok, hi = p >> shift;
           const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> shift;
           if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages)) y = INFINITY;
@@ -285,12 +298,12 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
         *dst = y;
       };
       // where this lane stores the scores of pages 2 qd, 2 qd + 1: the tokens of rows g and g + 8
-      const int lanes = min(hb, 8);  // rows of a token among lanes
+      constexpr int lanes = kHeads > 8 ? 8 : kHeads > 0 ? kHeads : 1;  // rows of a token among lanes
       int tok_out[2];
       float* out[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int tok = hb == 16 ? r : token_of(g + 8 * r);
+        const int tok = kHeads == 16 ? r : token_of(g + 8 * r);
         tok_out[r] = (g & (lanes - 1)) == 0 && tok < n_tok ? tok : -1;
         out[r] = a.scores + (q0 + tok0 + max(tok_out[r], 0)) * a.sc_st + kvh * a.sc_sh + 2 * qd;
       }
@@ -333,11 +346,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           y[i] = ((part[0][i] + part[1][i]) + (part[2][i] + part[3][i])) * a.scale;
-        // whether every row sees all eight pages, without a bias, and none is taken always
-        const int c_near = (p0 - a.rel_extent + 1) >> shift;  // the first page within the bias's reach
-        const bool inside =
-            p0 >= a.rel_extent && c0 + 7 < c_near && c0 >= c_first_seen && h0 == 0 &&
-            a.group <= 16 && c0 + 7 < page1 && c0 + 7 <= (p0 >> shift) - a.last_pages;
+        const bool inside = c0 >= c_inside && c0 <= c_inside_end;
         if (!inside) {
 #pragma unroll
           for (int r = 0; r < 2; ++r)
@@ -356,21 +365,17 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
               y[2 * r + e] = x;
             }
         }
-        if (by_shuffle) {
-          const auto across = [&](int m) {  // rows 8 to 15 only where there are some
+        if constexpr (kHeads > 0) {
+#pragma unroll
+          for (int m = 4; m < 4 * min(kHeads, 8); m *= 2) {
             y[0] = max_nan(y[0], __shfl_xor_sync(0xffffffffu, y[0], m));
             y[1] = max_nan(y[1], __shfl_xor_sync(0xffffffffu, y[1], m));
-            if (n_rows > 8) {
+            if (n_rows > 8) {  // rows 8 to 15 only where there are some
               y[2] = max_nan(y[2], __shfl_xor_sync(0xffffffffu, y[2], m));
               y[3] = max_nan(y[3], __shfl_xor_sync(0xffffffffu, y[3], m));
             }
-          };
-          if (lanes >= 2) {
-            across(4);
-            if (lanes >= 4) across(8);
-            if (lanes == 8) across(16);
           }
-          if (hb == 16) {
+          if (kHeads == 16) {
             y[0] = max_nan(y[0], y[2]);
             y[1] = max_nan(y[1], y[3]);
           }
@@ -390,7 +395,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
 #pragma unroll
           for (int i = 0; i < 4; ++i) tile[g + 8 * (i >> 1)][2 * qd + (i & 1)] = y[i];
           __syncwarp();
-          const int heads = a.group <= 16 ? hb : n_rows;
+          const int heads = group <= 16 ? hb : n_rows;
           for (int i = lane; i < 8 * n_tok; i += 32) {
             const int tok = i >> 3, pg = i & 7;
             float x = -INFINITY;
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
           __syncwarp();
         }
       }
-      if (rb + a.row_blocks < (n_q + tokens - 1) / tokens || h0 + 16 < a.group) __syncthreads();
+      if (rb + a.row_blocks < (n_q + tokens - 1) / tokens || h0 + 16 < group) __syncthreads();
     }
   }
 }
@@ -897,10 +902,16 @@ cudaError_t launch_page_bounds_sm100(const PageBoundsKernelArgs& args, int block
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream) {
   const dim3 grid((args.s.table_width + args.block_pages - 1) / args.block_pages,
                   args.kv_heads * args.row_blocks, args.s.batch + (args.zero_padding ? 1 : 0));
-  static std::atomic<bool> attr[64];
-  cudaError_t e = set_smem_limit_once(sparse::page_scores_kernel, sparse::kScoreSmem, attr);
+  static std::atomic<bool> attr[6][64];
+  static void (*const kernels[6])(PageScoresKernelArgs) = {
+      sparse::page_scores_kernel<0>, sparse::page_scores_kernel<1>, sparse::page_scores_kernel<2>,
+      sparse::page_scores_kernel<4>, sparse::page_scores_kernel<8>, sparse::page_scores_kernel<16>};
+  int i = 0;
+  for (int k = 1; k < 6; ++k)
+    if (args.group == 1 << (k - 1)) i = k;
+  cudaError_t e = set_smem_limit_once(kernels[i], sparse::kScoreSmem, attr[i]);
   if (e != cudaSuccess) return e;
-  sparse::page_scores_kernel<<<grid, sparse::kScoreWarps * 32, sparse::kScoreSmem, stream>>>(args);
+  kernels[i]<<<grid, sparse::kScoreWarps * 32, sparse::kScoreSmem, stream>>>(args);
   return cudaGetLastError();
 }
 
