@@ -328,9 +328,47 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
       const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
       uint64_t acc[2] = {0, 0};
       float edge = 0.f;
+      // Full tiles whose rows all see every key of this tile, and none through the bias: from in_lo on,
+      // in_n of them
+      int in_lo = 0, in_n = 0;
+      if (tokens * a.group == kN) {
+        const int past = a.rel_extent + tile0 + kKeys - 1 - shift;  // tokens from here on
+        in_lo = past > 0 ? (past + tokens - 1) / tokens : 0;
+        int in_end = n_q / tokens;
+        if (a.window_left >= 0) {
+          const long long last = static_cast<long long>(a.window_left) + tile0 - shift + 1;
+          in_end = last < tokens ? 0 : min(in_end, static_cast<int>(min(last / tokens, 1ll << 30)));
+        }
+        in_n = max(0, in_end - in_lo);
+      }
       for (int qt = rows.lo; qt < rows.hi && ok; ++qt, ++step) {
         const uint32_t qs = resident ? 0u : nq % L::kQStages;
         const uint32_t buf = step & 1;
+        if (static_cast<unsigned>(qt - in_lo) < static_cast<unsigned>(in_n)) {
+          if (!(ok = mbar_wait_warp(&bars->s_full[w][buf], (step >> 1) & 1, ab) &&
+                     mbar_wait_warp(&bars->q_full[qs], resident ? 0u : (nq / L::kQStages) & 1, ab)))
+            break;
+          if (!resident) ++nq;
+          tc_fence_after();
+          const float* nlse = &sums[qs].nlse[c_begin];
+          const uint32_t t_s = t_lane + buf * kN + c_begin;
+          uint32_t r[2][kC];
+          tmem_load(t_s, r[0]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c0 = 0; c0 < kW; c0 += kC) {
+            if (c0 + kC < kW) tmem_load(t_s + c0 + kC, r[(c0 / kC + 1) & 1]);
+            add_chunk<kC>(r[(c0 / kC) & 1], nlse + c0, mul2, acc);
+            if (c0 + kC < kW) tmem_wait_ld();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&bars->s_empty[w][buf]);
+            if (!resident) mbar_arrive(&bars->q_empty[qs]);
+          }
+          continue;
+        }
         const int p0 = shift + qt * tokens;  // position of the tile's first token
         const int n_tok = min(tokens, n_q - qt * tokens), n_cols = n_tok * a.group;
         const int c_end = min(n_cols, c_begin + kW);
