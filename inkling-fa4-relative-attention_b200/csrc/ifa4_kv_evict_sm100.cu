@@ -60,7 +60,7 @@ struct Columns {
 template <int kN>
 struct Sums {
   float nlse[kN];      // -lse * log2(e); -inf: the row adds nothing
-  float lse[kN];
+  float neg[kN];       // -lse, or -inf too
 };
 
 struct Bars {
@@ -301,8 +301,9 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
         for (int i = 0; i < kPer; ++i) {
           const int r = lane + 32 * i;
           if (r < kN) {
-            sums[qs].nlse[r] = l[i] == -INFINITY ? -INFINITY : -l[i] * kLog2e;  // -inf for +inf, too
-            sums[qs].lse[r] = l[i];
+            const float neg = l[i] == -INFINITY ? -INFINITY : -l[i];  // -inf for +inf, too
+            sums[qs].nlse[r] = neg * kLog2e;
+            sums[qs].neg[r] = neg;
           }
         }
         __syncwarp();
@@ -379,13 +380,20 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
         const auto fetch = [&](int c0, uint16_t (&x)[kC]) {
 #pragma unroll
           for (int i = 0; i < kC; ++i) x[i] = 0;
-          if (c0 >= c_end || p0 + cols.token[c0] - (tile0 + kKeys - 1) >= a.rel_extent) return;
+          if (c0 >= c_end) return;
+          const int p_lo = p0 + cols.token[c0], p_hi = p0 + cols.token[min(c0 + kC, c_end) - 1];
+          if (p_lo - (tile0 + kKeys - 1) >= a.rel_extent || p_hi < tile0) return;
+          if (c0 + kC <= c_end && p_hi - tile0 < a.rel_extent && p_lo >= tile0 + kKeys - 1) {
 #pragma unroll
-          for (int i = 0; i < kC; ++i) {
-            const int tok = cols.token[c0 + i];
-            load_if(x[i], rel_key + cols.rel[c0 + i],
-                    tok < n_tok &&
-                        static_cast<unsigned>(dk + tok) < static_cast<unsigned>(a.rel_extent));
+            for (int i = 0; i < kC; ++i) load_now(x[i], rel_key + cols.rel[c0 + i]);  // all have one
+          } else {
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              const int tok = cols.token[c0 + i];
+              load_if(x[i], rel_key + cols.rel[c0 + i],
+                      tok < n_tok &&
+                          static_cast<unsigned>(dk + tok) < static_cast<unsigned>(a.rel_extent));
+            }
           }
         };
         // whether every row sees every key of this tile, and none through the bias
@@ -429,17 +437,31 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
           tmem_wait_ld();
           if (p_hi < tile0) continue;  // before every key of the tile
           if (a.window_left >= 0 && p_lo - (tile0 + kKeys - 1) > a.window_left) continue;
+          // bias - lse first: either may be at the end of the range
+          if (c0 + kC <= c_end && p_lo >= tile0 + kKeys - 1 && p_hi - tile0 <= window) {
 #pragma unroll
-          for (int i = 0; i < kC; ++i) {
-            const int tok = cols.token[c0 + i];
-            // bias - lse first: either may be at the end of the range
-            const float x = __fmaf_rn(bf16_bits_to_float(bias[i]) - m.lse[c0 + i], kLog2e,
-                                      __uint_as_float(r[i]) * a.scale_log2);
-            const bool seen = tok < n_tok && static_cast<unsigned>(dk + tok) <=
-                                                 static_cast<unsigned>(window) &&
-                              m.nlse[c0 + i] != -INFINITY;
-            const float y = fast_exp2(x);
-            edge += seen ? y : 0.f;
+            for (int i = 0; i < kC; i += 4) {  // every row sees every key
+              const float4 neg = *reinterpret_cast<const float4*>(&m.neg[c0 + i]);
+              const float nl[4] = {neg.x, neg.y, neg.z, neg.w};
+              float y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                y[j] = fast_exp2(__fmaf_rn(__uint_as_float(r[i + j]), a.scale_log2,
+                                           (bf16_bits_to_float(bias[i + j]) + nl[j]) * kLog2e));
+              acc[0] = f2_add(acc[0], f2_pack(y[0], y[1]));
+              acc[1] = f2_add(acc[1], f2_pack(y[2], y[3]));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kC; ++i) {
+              const int tok = cols.token[c0 + i];
+              const float y = fast_exp2(__fmaf_rn(__uint_as_float(r[i]), a.scale_log2,
+                                                  (bf16_bits_to_float(bias[i]) + m.neg[c0 + i]) *
+                                                      kLog2e));
+              const bool seen = tok < n_tok && static_cast<unsigned>(dk + tok) <=
+                                                   static_cast<unsigned>(window);
+              edge += seen ? y : 0.f;
+            }
           }
         }
         tc_fence_before();

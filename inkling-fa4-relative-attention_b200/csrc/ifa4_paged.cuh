@@ -298,14 +298,19 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
     if (first && digit == kSelectBins - 1) {
       lo = kTop;
       hi = 0xffffffffu;
-    } else if (values_binned) {  // the smallest and the largest key of the bin
+    } else if (values_binned) {
+      // the keys of the bin lie among those of three bins (which is more than the rounding of a bin's
+      // number can be off): few need their own bin looked up
+      const uint32_t from = rank_of(start + (static_cast<float>(digit) - 1.f) / scale);
+      const uint32_t to = rank_of(start + (static_cast<float>(digit) + 2.f) / scale);
       low = 0xffffffffu;
       high = 0u;
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
-        if (u[j] != 0u && u[j] < kTop && value_bin(u[j]) == digit) {
+        if (u[j] - from <= to - from && u[j] != 0u && u[j] < kTop && value_bin(u[j]) == digit) {
           low = min(low, u[j]);
           high = max(high, u[j]);
+          if (in_bin <= kCandidates) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
         }
       low = __reduce_min_sync(0xffffffffu, low);
       high = __reduce_max_sync(0xffffffffu, high);
@@ -330,10 +335,12 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
       break;
     }
     if (in_bin <= kCandidates) {
+      if (!values_binned || digit == kSelectBins - 1) {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
-      __syncthreads();
+        for (int j = 0; j < kItems; ++j)
+          if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
+        __syncthreads();
+      }
       if (tid < static_cast<int>(in_bin)) {
         const uint32_t x = sm.candidate[tid];
         uint32_t larger = 0u, equal = 0u;

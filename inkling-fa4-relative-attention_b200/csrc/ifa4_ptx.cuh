@@ -219,6 +219,9 @@ __device__ __forceinline__ void load_if(uint16_t& x, const uint16_t* p, bool on)
       : "l"(p), "r"(static_cast<int>(on)));
 }
 
+__device__ __forceinline__ void load_now(uint16_t& x, const uint16_t* p) {
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(x) : "l"(p));
+}
 // The same for memory that this kernel writes.
 __device__ __forceinline__ void load_plain_if(float& x, const float* p, bool on) {
   asm volatile(
