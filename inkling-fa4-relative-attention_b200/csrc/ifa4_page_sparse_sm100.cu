@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
 // ---------------------------------------------------------------------------------------
 // A block per row and KV head (see select_largest); kItems 0: rows of any length.
 template <int kThreads, int kItems>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : kThreads == 256 ? 4 : 1)
     select_pages_kernel(const __grid_constant__ SelectPagesKernelArgs a) {
   __shared__ SelectSmem<kThreads> sm;
   const int g = blockIdx.y;

@@ -222,12 +222,13 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
 #pragma unroll
     for (int j = 0; j < kItems; ++j) u[j] = base + 32 * j < n ? key(base + 32 * j, v[j]) : 0u;
   }
-  // smallest (less one, which leaves out the keys 0) and largest of the finite ones
+  // smallest (less one, which leaves out the keys 0) and largest of the finite ones (less kTop, which
+  // puts those from kTop on below them)
   uint32_t low = 0xffffffffu, high = 0u;
 #pragma unroll
   for (int j = 0; j < kItems; ++j) {
     low = min(low, u[j] - 1u);
-    high = max(high, u[j] < kTop ? u[j] : 0u);
+    high = max(high, u[j] - kTop);
   }
   low = __reduce_min_sync(0xffffffffu, low);
   high = __reduce_max_sync(0xffffffffu, high);
@@ -238,15 +239,19 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
   }
   __syncthreads();
   // where the border lies; keys from kTop on are in the last bin of the first pass
-  uint32_t lo = sm.low + 1u, hi = sm.high, need = static_cast<uint32_t>(count), border = 0u;
+  uint32_t lo = sm.low + 1u, hi = sm.high + kTop, need = static_cast<uint32_t>(count), border = 0u;
   float start = 0.f, scale = 0.f;  // the bins of values, where scale > 0
-  if (lo < kRankZero && hi > kRankZero) {
+  if (lo < kRankZero && hi > kRankZero && hi < kTop) {
     start = value_of(lo);
     scale = (kSelectBins - 2) / (value_of(hi) - start);  // 0 where the range is not finite
+    if (!(scale < 1e30f)) scale = 0.f;                    // nor where it is next to nothing
   }
-  // bins ascend with the keys (a difference and a product with a positive number do, rounded too)
+  const float offset = -start * scale;
+  // Bins ascend with the keys (a product with a positive number and a sum do, rounded too).  Keys from
+  // kTop on, NaN among them, are in the last bin, and no finite one is.
   const auto value_bin = [&](uint32_t key) {
-    return min(static_cast<uint32_t>((value_of(key) - start) * scale), kSelectBins - 2u);
+    const float x = __fmaf_rn(value_of(key), scale, offset);
+    return static_cast<uint32_t>(fminf(x, key < kTop ? kSelectBins - 2.f : kSelectBins - 1.f));
   };
   for (bool first = true;; first = false) {
     const int bits = hi > lo ? 32 - __clz(hi - lo) : 0;
@@ -259,7 +264,7 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
     if (values_binned) {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
-        if (u[j] != 0u) atomicAdd(&sm.hist[u[j] >= kTop ? kSelectBins - 1 : value_bin(u[j])], 1u);
+        if (u[j] != 0u) atomicAdd(&sm.hist[value_bin(u[j])], 1u);
     } else if (first) {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
@@ -363,11 +368,18 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
   }
   // taken: key > border, and the first `need` of key == border
   uint32_t gt = 0u, eq = 0u;
+  if (need == 0u) {  // the keys are not needed any more: which lanes' are above
 #pragma unroll
-  for (int j = 0; j < kItems; ++j) gt += __popc(__ballot_sync(0xffffffffu, u[j] > border));
-  if (need != 0u) {
+    for (int j = 0; j < kItems; ++j) {
+      u[j] = __ballot_sync(0xffffffffu, u[j] > border);
+      gt += __popc(u[j]);
+    }
+  } else {
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) eq += __popc(__ballot_sync(0xffffffffu, u[j] == border));
+    for (int j = 0; j < kItems; ++j) {
+      gt += __popc(__ballot_sync(0xffffffffu, u[j] > border));
+      eq += __popc(__ballot_sync(0xffffffffu, u[j] == border));
+    }
   }
   if (lane == 0) {
     sm.warp[warp] = gt;
@@ -384,11 +396,8 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
   if (need == 0u) {
 #pragma unroll
     for (int j = 0; j < kItems; ++j) {
-      const uint32_t bg = __ballot_sync(0xffffffffu, u[j] > border);
-      if (bg != 0u) {
-        if (u[j] > border) emit(static_cast<int>(g + __popc(bg & before)), base + 32 * j);
-        g += __popc(bg);
-      }
+      if (u[j] >> lane & 1u) emit(static_cast<int>(g + __popc(u[j] & before)), base + 32 * j);
+      g += __popc(u[j]);
     }
   } else {
 #pragma unroll 1
