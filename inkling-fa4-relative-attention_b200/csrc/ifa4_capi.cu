@@ -1687,6 +1687,8 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
       p->table_width > (1 << 26))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_selected and table_width must be in [0, 2^26]",
                 what);
+  if (static_cast<int64_t>(p->num_selected) * d->page_size > int64_t{1} << 36)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: more than 2^36 listed keys", what);
   if (d->num_splits < 0 || d->num_splits > 1024)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: num_splits must be in [0, 1024]", what);
   *splits = 1;
@@ -2025,7 +2027,7 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
   a.accumulate = p->accumulate != 0;
   a.box_shift = a.s.page_shift < 7 ? a.s.page_shift : 7;
   a.tokens_per_tile = rows / group;
-  a.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  a.scale_log2 = static_cast<float>(p->softmax_scale * 1.4426950408889634);
   a.status = status;
   a.q = static_cast<const uint16_t*>(p->q);
   a.k_cache = static_cast<const uint16_t*>(p->k_cache);

@@ -33,6 +33,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 constexpr uint32_t kBarBytes = 2560;
 
+// x log2(e) rounded once: the error of a row's lse is one of all its weights, which no sum over the keys
+// averages out.
+__device__ __forceinline__ float scaled_lse(float x) {
+  return static_cast<float>(static_cast<double>(x) * 1.4426950408889634);
+}
+
 template <int kN>
 struct Layout {
   static constexpr int kKStages = kN >= 128 ? 1 : 2;
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
           const int r = lane + 32 * i;
           if (r < kN) {
             const float neg = l[i] == -INFINITY ? -INFINITY : -l[i];  // -inf for +inf, too
-            sums[qs].nlse[r] = neg * kLog2e;
+            sums[qs].nlse[r] = scaled_lse(neg);
             sums[qs].neg[r] = neg;
           }
         }
@@ -328,7 +334,6 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
       const int key = tile0 + row;
       const Rows rows = rows_of(kp * 2 * kKeys, n_q, n_k, a.window_left, tokens);
       uint64_t acc[2] = {0, 0};
-      float edge = 0.f;
       // Full tiles whose rows all see every key of this tile, and none through the bias: from in_lo on,
       // in_n of them
       int in_lo = 0, in_n = 0;
@@ -351,6 +356,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
             break;
           if (!resident) ++nq;
           tc_fence_after();
+          // a sum for each tile, then the sum of those: no long chain of additions to one number
+          uint64_t part[2] = {0, 0};
           const float* nlse = &sums[qs].nlse[c_begin];
           const uint32_t t_s = t_lane + buf * kN + c_begin;
           uint32_t r[2][kC];
@@ -359,9 +366,11 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
 #pragma unroll
           for (int c0 = 0; c0 < kW; c0 += kC) {
             if (c0 + kC < kW) tmem_load(t_s + c0 + kC, r[(c0 / kC + 1) & 1]);
-            add_chunk<kC>(r[(c0 / kC) & 1], nlse + c0, mul2, acc);
+            add_chunk<kC>(r[(c0 / kC) & 1], nlse + c0, mul2, part);
             if (c0 + kC < kW) tmem_wait_ld();
           }
+          acc[0] = f2_add(acc[0], part[0]);
+          acc[1] = f2_add(acc[1], part[1]);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -409,6 +418,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
         tc_fence_after();
         const Sums<kN>& m = sums[qs];
         const uint32_t t_s = t_lane + buf * kN;
+        uint64_t part[2] = {0, 0};
+        float edge = 0.f;
         int c_next = c_begin;
         if (inside) {  // the chunks that are full
           uint32_t r[2][kC];
@@ -418,7 +429,7 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
           for (int c0 = 0; c0 < kW; c0 += kC) {
             if (c_begin + c0 + kC > c_end) break;
             if (c0 + kC < kW) tmem_load(t_s + c_begin + c0 + kC, r[(c0 / kC + 1) & 1]);
-            add_chunk<kC>(r[(c0 / kC) & 1], &m.nlse[c_begin + c0], mul2, acc);
+            add_chunk<kC>(r[(c0 / kC) & 1], &m.nlse[c_begin + c0], mul2, part);
             if (c0 + kC < kW) tmem_wait_ld();
             c_next += kC;
           }
@@ -448,8 +459,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
               for (int j = 0; j < 4; ++j)
                 y[j] = fast_exp2(__fmaf_rn(__uint_as_float(r[i + j]), a.scale_log2,
                                            (bf16_bits_to_float(bias[i + j]) + nl[j]) * kLog2e));
-              acc[0] = f2_add(acc[0], f2_pack(y[0], y[1]));
-              acc[1] = f2_add(acc[1], f2_pack(y[2], y[3]));
+              part[0] = f2_add(part[0], f2_pack(y[0], y[1]));
+              part[1] = f2_add(part[1], f2_pack(y[2], y[3]));
             }
           } else {
 #pragma unroll
@@ -464,6 +475,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
             }
           }
         }
+        acc[0] = f2_add(acc[0], f2_add(part[0], f2_pack(edge, 0.f)));
+        acc[1] = f2_add(acc[1], part[1]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -473,7 +486,7 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
       }
       float s0, s1;
       f2_unpack(f2_add(acc[0], acc[1]), s0, s1);
-      float sum = s0 + s1 + edge;
+      float sum = s0 + s1;
       if (L::kSplit > 1) {  // the other half of the columns
         float* other = &bars->half[pairs & 1][w][row];
         if (c_begin > 0) *other = sum;
@@ -600,7 +613,7 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
         qa[kk][2 + r] = on ? __ldg(src + kk * 8 + 4 + qd) : 0u;
       }
       lse[r] = on ? __ldg(a.lse + h * a.lse_sh + t * a.lse_st) : -INFINITY;
-      nlse[r] = lse[r] == -INFINITY ? -INFINITY : -lse[r] * kLog2e;
+      nlse[r] = lse[r] == -INFINITY ? -INFINITY : scaled_lse(-lse[r]);
       pos[r] = lse[r] == -INFINITY ? -1 : shift + tok;  // a row that adds nothing sees nothing
       rel[r] = a.rel + t * a.rel_st + static_cast<long long>(h) * a.rel_sh;
     }

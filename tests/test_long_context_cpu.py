@@ -127,7 +127,9 @@ def _decode_pages(**kw):
     (dict(block_table=None), INVALID, b"block_table"), (dict(causal=0), INVALID, b"causal"),
     (dict(causal_align=0), INVALID, b"BOTTOM_RIGHT"), (dict(pages=None), INVALID, b"pages"),
     (dict(num_selected=-1), INVALID, b"num_selected"), (dict(num_splits=-1), INVALID, b"num_splits"),
-    (dict(num_splits=1025), INVALID, b"num_splits"), (dict(page_size=24), INVALID, b"page_size"),
+    (dict(num_splits=1025), INVALID, b"num_splits"),
+    (dict(num_selected=1 << 26, page_size=1 << 12), UNSUPPORTED, b"2^36"),
+    (dict(page_size=24), INVALID, b"page_size"),
     (dict(total_q=1 << 31), UNSUPPORTED, b"rows"), (dict(batch=65535), UNSUPPORTED, b"batch"),
     (dict(q=260), INVALID, b"aligned")])
 def test_decode_pages_refusals(kw, code, msg):
