@@ -621,7 +621,9 @@ int ifa4_select_pages_launch(const IFA4SelectPagesParams* params, void* stream);
  * rows a sequence.  A row without keys is 0 with the lse -inf; a logit that is NaN or +inf makes its
  * row NaN.  decode.block_table and the seqs fields that repeat there have to agree (batch,
  * cu_seqlens, page_size, num_pages come from decode); chunk_len is not used.  Rows of no sequence
- * get 0 (lse -inf) where zero_padding is set and stay as they are otherwise. */
+ * get 0 (lse -inf) where zero_padding is set and stay as they are otherwise.  A workspace is needed
+ * for more than eight splits of a row only (the size is 0 otherwise); it must be 16-byte aligned and
+ * not shared by calls that may run at the same time. */
 typedef struct IFA4DecodePagesParams {
   IFA4DecodeParams decode;
   const int32_t* pages;         /* [total_q, kv_heads, num_selected], unit last stride     */
@@ -723,8 +725,8 @@ int ifa4_measure_read_stream(const void* buf, size_t bytes, uint32_t* sink, void
  * calling thread until the stream has reached this point.  Nonzero means a kernel gave up on
  * a bounded wait (a bug, never expected): bit 0 prefill, bit 1 decode, bit 2 backward, bits 3-4
  * ifa4_selftest_bounded_wait, bit 5 rel_logits producer, bit 6 (debug builds compiled with
- * -DIFA4_DEBUG only) an index range check failed and the access was skipped, bit 7 eviction.  Test hook; the
- * reference has no counterpart. */
+ * -DIFA4_DEBUG only) an index range check failed and the access was skipped, bit 7 eviction.  Test
+ * hook; the reference has no counterpart. */
 int ifa4_read_device_status(void* stream, int32_t clear, int32_t* status_out);
 
 /* Name of the sm_100a prefill tile configuration `tile_config` resolves to (the counterpart

@@ -22,10 +22,15 @@ namespace mass {
 //   warp 0      TMA producer: the K tiles of the pair (paged, 128-byte swizzle) and the ring of Q tiles
 //   warp 1      issues the products; scores are double-buffered in TMEM for each warpgroup
 //   warp 2      -lse, position and place of the bias of every row of a Q tile, beside it in the ring
-//   warps 4-11  exponentials and sums; the lane's key stays, the rows stream by
-// A sequence whose rows fit one tile keeps it in shared memory while the keys stream by (single tokens:
+//   warps 4-..  exponentials and sums; the lane's key stays, the rows stream by (8 warps, 16 where
+//               kN is 128, each tile's columns in two halves)
+// A sequence whose rows fit one tile keeps it in shared memory while the keys stream by (a few tokens:
 // bound by HBM, 256 bytes a key); otherwise the keys stay and the rows stream by (prompts: bound by
-// the exponentials).
+// the exponentials and what issues them).  Tiles of rows that all see a key tile, and none of them
+// through the bias, take a path without checks; so do chunks of 16 rows that all have a bias.
+// 32k tokens causal, 32 heads on 8: 5.0 ms with rel_extent 64 (883 TFLOP/s; the exponentials alone 3.8 to
+// 4.1), 6.0 ms with 1024 (5.8 to 6.5 by the power cap).  Counters at 5.2 ms: SFU 68 % busy, tensor
+// cores 35 %, issue slots 55 %.
 constexpr int kKeys = 128;
 constexpr uint32_t kKHalf = kKeys * 128;       // 64 dims of a K tile
 constexpr uint32_t kKTile = 2 * kKHalf;        // 128 keys x 256 B
@@ -97,8 +102,9 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[16]) { tm
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&r)[32]) { tmem_ld32(addr, r); }
 
 // acc += 2^(scale s + nlse) over a chunk of columns.  All exponentials on the SFU: a share of 1, 2 or 3
-// in 8 on the FMA pipe (degree 5, 7.5e-8) took 5.18, 5.65 and 5.97 ms where this took 5.19 (32k prompt,
-// rel_extent 64), with the same results.
+// in 8 as polynomials on the FMA pipe (degree 5, 7.5e-8) took 5.18, 5.65 and 5.97 ms where this took 5.19
+// (32k prompt, rel_extent 64); a share of 1 or 2 in 16 later 4.83 and 4.92 where this took 4.97, and with
+// rel_extent 1024 5.84 and 5.91 where this took 5.88: not worth a second way to the same number.
 template <int kC>
 __device__ __forceinline__ void add_chunk(const uint32_t (&r)[kC], const float* nlse, uint64_t mul2,
                                           uint64_t (&acc)[2]) {
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
   const AbortCtx ab{&bars->abort_flag, a.status, kStatusDecodeTimeout};
 
   // of the 96 registers that each of 640 threads starts with, the summing warps take 104 and the
-  // others keep 64: together the 61440 of the launch (fewer spills: 7.08 -> 6.82 ms)
+  // others keep 64: together the 61440 of the launch (fewer spills: 7.08 -> 6.82 ms;
+  // 112 and 32 the same)
   if (L::kSplit > 1 && warp < 4) setmaxnreg_dec<64>();
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
@@ -278,7 +285,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
     }
   } else if (warp == 2) {
     // ---------------------------------------------------------------- the lse of each Q tile's rows
-    // fetched a tile ahead: a tile waited for its own loads before (25.5 ms of a 32k prompt, see below)
+    // fetched a tile ahead: a tile waited for its own loads before (25.5 ms of a 32k
+    // prompt, 7.5 with this and with the loads of the biases issued together)
     constexpr int kPer = (kN + 31) / 32;
     float l[kPer];
     const auto fetch = [&](int qt) {
@@ -513,7 +521,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
 // own, 16 keys a stage, which one of its lanes refills by TMA as soon as the warp has read a stage: no
 // barriers between warps, no start to speak of, and 192 KB in flight on an SM.  Bound by HBM, 256 bytes
 // a key.  (8 sequences of 4k to 32k keys, one token each: 62 us on the kernel above, whose CTAs start
-// slowly and end in a half-empty wave; 50 us with the keys in registers, 64 KB in flight.)
+// slowly and end in a half-empty wave; 50 us with the keys in registers, 64 KB in flight; 43 us, 45 a
+// call, so: 5.0 TB/s.  A contiguous stretch of keys for each warp: 55 us.)
 constexpr int kStreamWarps = 8;
 constexpr int kStreamStages = 3;
 constexpr uint32_t kStreamHalf = 16 * 128;            // 16 keys, 64 dims
@@ -824,8 +833,8 @@ __global__ void __launch_bounds__(kSelectThreads)
 // said so too, and writes.  Key `place` comes from kept[place] >= place, so only earlier stretches read
 // there.  Stretches are handed out in order by a counter: a block waits for blocks that are running and
 // wait for nothing themselves before they say so.  Bound by HBM: 512 bytes read and written a key.
-// (A block per head that went through its keys with barriers took 364 us where this takes XXX,
-// 16 x 32k keys to 8192.)
+// (16 sequences of 32k keys to 8192, 8 KV heads: 187 us, 5.5 TB/s, of a call of 217 with the choice's 35;
+// a block per head that went through its keys with barriers took the call to 364.)
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 64;
 constexpr uint32_t kMoveSmem = kMoveRows * 512;  // K and V rows

@@ -42,7 +42,8 @@ __device__ __forceinline__ uint4 shfl_xor_v4(uint4 v, int m) {
 // ---------------------------------------------------------------------------------------
 // A warp per page and KV head: half a warp reads a key (16 bytes a lane), eight keys of each half in
 // flight; the halves are joined at the end, one writes the minima, the other the maxima (512
-// contiguous bytes).  Bound by HBM: 256 bytes a key and head read, 512 a page and head written.
+// contiguous bytes).  Bound by HBM: 256 bytes a key and head read, 512 a page and head written (8 x 32k keys,
+// 8 KV heads: 86 us of 83.5 at the copy rate).
 __global__ void __launch_bounds__(kPageBoundsWarps * 32)
     page_bounds_kernel(const __grid_constant__ PageBoundsKernelArgs a) {
   const int lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
@@ -93,12 +94,13 @@ __global__ void __launch_bounds__(kPageBoundsWarps * 32)
 // sum_i (max(q_i, 0) max_i + min(q_i, 0) min_i) is a matrix product of depth 256 with the bounds as
 // they lie in memory, and runs on warp-level MMAs (16 rows: the heads of a group, of 16 / group
 // tokens; 8 pages a warp).  The order of the 128 dims is free as long as both operands have the same:
-// lane qd of a quad takes 16 contiguous bytes of every 64 from the bounds as they were copied.  Every warp
-// has a ring of its own, eight pages a stage, refilled by 16-byte asynchronous copies as soon as it has
-// read a stage (by bulk copies of 512 bytes: 99 us, the copy engine takes them one by one).  The largest bias of a page is found by the whole block, 16 keys a
-// thread at a time, for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for
-// 16 rows.  (64 sequences of up to 32k keys: 111 us with the bounds loaded straight to registers, 104
-// with the next eight pages loaded ahead.)
+// lane qd of a quad takes 16 contiguous bytes of every 64 from the bounds as they were copied.  Every
+// warp has a ring of its own, eight pages a stage, refilled by 16-byte asynchronous copies as soon as it
+// has read a stage.  The largest bias of a page is found by the whole block, 16 keys a thread at a time,
+// for the pages within its reach only.  Bound by HBM: 512 bytes a page and head for 16 rows.
+// (64 sequences of up to 32k keys: 72 us, 4.9 TB/s.  111 with the bounds loaded straight to registers,
+// 104 with the next eight pages loaded ahead, 99 with bulk copies of 512 bytes, which the copy engine
+// takes one by one, 105 with blocks that stay and fetch their next piece of work.)
 constexpr int kScoreWarps = 4;
 constexpr int kScorePages = 256;  // most pages of a block
 constexpr int kScoreStages = 2;
@@ -413,7 +415,10 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
 // ---------------------------------------------------------------------------------------
 // Choice of pages
 // ---------------------------------------------------------------------------------------
-// A block per row and KV head (see select_largest); kItems 0: rows of any length.
+// A block per row and KV head (see select_largest); kItems 0: rows of any length.  Bound by issue slots
+// (65 % busy) and the passes' barriers: every element is read once, and its key ranked, binned, counted
+// and emitted from registers.  (128 x 8 rows of 8192 pages: 26.7 us with three blocks an SM, 28.7 with
+// two, 30.6 with four, which spill; one row of 2048: 5.5, 5.9 and 5.9 a call.)
 template <int kThreads, int kItems>
 __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : kThreads == 256 ? 4 : 1)
     select_pages_kernel(const __grid_constant__ SelectPagesKernelArgs a) {
@@ -441,7 +446,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : kThreads == 25
 // to 16 query heads of one KV head.  Warp 4 follows the list and the block table and loads the tiles'
 // units (min(page_size, 64) rows) by TMA into a ring; warps 0 to 3 take 16 keys of every tile, which
 // always lie in one page (page_size >= 16), so a warp reads one list entry per tile.  Units and slices
-// without a visible key are neither loaded nor computed.  Bound by HBM: 512 bytes a key and KV head.
+// without a visible key are neither loaded nor computed.  Bound by HBM: 512 bytes a key and KV head
+// (64 rows of 256 pages of 16 keys, 8 KV heads: 180 us, 6.0 TB/s of the listed keys).
 constexpr int kTileKeys = 64;
 constexpr int kStages = 3;
 constexpr int kConsumerWarps = 4;
