@@ -675,8 +675,8 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* params, void* stre
  * everything) up to budget, in their order; their K and V rows move to the places 0 .. budget - 1 of
  * the sequence, in place.  kept gets the places they had (-1 behind the last), mass_out the masses of
  * what is kept with zeros behind, cu_out the offsets of the new lengths.  Shorter sequences keep
- * everything.  A kept key without a page is zeros at its new place.  No page may be held by two
- * sequences, or twice by one.  seqs.cu_seqlens_q is not used; the workspace
+ * everything.  A kept key without a page is zeros at its new place.  No page that keys
+ * move into or out of may be held by another sequence, or twice by its own.  seqs.cu_seqlens_q is not used; the workspace
  * (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by calls that may run at
  * the same time. */
 typedef struct IFA4KvEvictParams {

@@ -2,12 +2,16 @@
 // launch planning, error reporting.  Declared in include/inkling_fa4.h.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdarg.h>
 #include <stdint.h>
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
+#include <initializer_list>
 #include <mutex>
+#include <utility>
 
 #include "../../include/inkling_fa4.h"
 #include "ifa4_internal.h"
@@ -1593,6 +1597,22 @@ int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* p, void
 // ---------------------------------------------------------------------------------------
 namespace {
 
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// Whether no two rows of `row` elements share one; pairs of stride and count.
+bool rows_apart(int64_t row, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+  std::pair<int64_t, int64_t> d[3];
+  int n = 0;
+  for (const auto& x : dims)
+    if (x.second > 1) d[n++] = x;
+  std::sort(d, d + n);
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < row) return false;
+    row += d[i].first * (d[i].second - 1);
+  }
+  return true;
+}
+
 int check_seqs(const char* what, const IFA4PagedSeqs* s, bool queries) {
   if (s->batch < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative batch", what);
   if (s->batch > 65534) return fail(IFA4_ERR_UNSUPPORTED, "%s: batch > 65534", what);
@@ -1607,6 +1627,9 @@ int check_seqs(const char* what, const IFA4PagedSeqs* s, bool queries) {
   if (s->batch > 0 && ((queries && s->cu_seqlens_q == nullptr) || s->cu_seqlens_k == nullptr ||
                        (s->block_table == nullptr && s->table_width > 0)))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null cu_seqlens or block_table", what);
+  if ((queries && !aligned4(s->cu_seqlens_q)) || !aligned4(s->cu_seqlens_k) ||
+      !aligned4(s->block_table))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned cu_seqlens or block_table", what);
   return IFA4_OK;
 }
 
@@ -1655,12 +1678,14 @@ int check_queries(const char* what, const P* p) {
   if (p->total_q < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative total_q", what);
   if (p->rel_extent <= 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: rel_extent must be > 0", what);
-  if (!(p->softmax_scale > 0.f))
-    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0", what);
+  if (!(p->softmax_scale > 0.f && p->softmax_scale < INFINITY))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0 and finite", what);
   if (p->rel_stride_t < 0 || p->rel_stride_h < 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative rel strides", what);
   if (p->total_q == 0) return IFA4_OK;
   if (!p->q || !p->rel) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
+  if ((reinterpret_cast<uintptr_t>(p->rel) & 1u) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned rel", what);
   if (!aligned16(p->q) || p->q_stride_t <= 0 || p->q_stride_t % 8 != 0 || p->q_stride_h <= 0 ||
       p->q_stride_h % 8 != 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT,
@@ -1696,6 +1721,14 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
   if (d->batch == 0 || d->total_q == 0) return IFA4_OK;
   if (p->num_selected > 0 && p->pages == nullptr)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: pages is NULL", what);
+  if (!aligned4(p->pages) || !aligned4(d->cu_seqlens_q) || !aligned4(d->cu_seqlens_k) ||
+      !aligned4(d->block_table) || !aligned4(d->lse))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned pages, cu_seqlens, block_table or lse",
+                what);
+  if ((reinterpret_cast<uintptr_t>(d->rel) & 1u) != 0)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned rel", what);
+  if (!(d->softmax_scale < INFINITY))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be finite", what);
   const int group = d->n_heads / d->kv_heads;
   const int64_t rows = d->total_q * d->kv_heads * ceil_div(group, 16);
   const int64_t tiles = ceil_div(static_cast<int64_t>(p->num_selected) * d->page_size, 64);
@@ -1764,6 +1797,18 @@ int validate_evict(const IFA4KvEvictParams* p) {
       (rc = check_pages(what, "v_cache", p->v_cache, p->v_stride_page, p->v_stride_t, p->v_stride_h,
                         p->seqs.num_pages)))
     return rc;
+  if (!aligned4(p->kept) || !aligned4(p->mass) || !aligned4(p->mass_out) || !aligned4(p->cu_out))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned kept, mass or cu_out", what);
+  if (!rows_apart(p->head_dim, {{p->k_stride_page, p->seqs.num_pages},
+                                {p->k_stride_t, p->seqs.page_size}, {p->k_stride_h, p->kv_heads}}) ||
+      !rows_apart(p->head_dim, {{p->v_stride_page, p->seqs.num_pages},
+                                {p->v_stride_t, p->seqs.page_size}, {p->v_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: strides of k_cache or v_cache overlap", what);
+  if (p->mass_stride_b < 0 || p->mass_stride_h < 0 ||
+      !rows_apart(p->mass_width, {{p->mass_out_stride_b, p->seqs.batch},
+                                  {p->mass_out_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative mass strides, or strides of mass_out overlap",
+                what);
   return IFA4_OK;
 }
 
@@ -1783,6 +1828,9 @@ int ifa4_page_bounds_launch(const IFA4PageBoundsParams* p, void* stream) {
                         p->seqs.num_pages)))
     return rc;
   if (p->seqs.batch == 0 || p->seqs.num_pages == 0 || p->seqs.table_width == 0) return IFA4_OK;
+  if (!rows_apart(2 * p->head_dim, {{p->bounds_stride_page, p->seqs.num_pages},
+                                    {p->bounds_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: strides of bounds overlap", what);
   ifa4::PageBoundsKernelArgs a{};
   a.s = paged_seqs(&p->seqs);
   a.k_cache = static_cast<const uint16_t*>(p->k_cache);
@@ -1825,8 +1873,10 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
     return fail(IFA4_ERR_UNSUPPORTED, "%s: bounds_stride_page > 2^30", what);
   if (p->seqs.batch == 0 || p->total_q == 0 || p->seqs.table_width == 0) return IFA4_OK;
   if (p->scores == nullptr) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores is NULL", what);
-  if (p->scores_stride_t < 0 || p->scores_stride_h < 0)
-    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative scores strides", what);
+  if (!aligned4(p->scores) ||
+      !rows_apart(p->seqs.table_width, {{p->scores_stride_t, p->total_q},
+                                        {p->scores_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores are misaligned, or their strides overlap", what);
   ifa4::PageScoresKernelArgs a{};
   a.s = paged_seqs(&p->seqs);
   a.q = static_cast<const uint16_t*>(p->q);
@@ -1880,9 +1930,12 @@ int ifa4_select_pages_launch(const IFA4SelectPagesParams* p, void* stream) {
   if (p->rows == 0 || p->kv_heads == 0) return IFA4_OK;
   if ((p->scores == nullptr && p->width > 0) || p->pages == nullptr)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
-  if (p->scores_stride_t < 0 || p->scores_stride_h < 0 || p->pages_stride_t < 0 ||
-      p->pages_stride_h < 0)
+  if (p->scores_stride_t < 0 || p->scores_stride_h < 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative strides", what);
+  if (!aligned4(p->scores) || !aligned4(p->pages) ||
+      !rows_apart(p->num_selected, {{p->pages_stride_t, p->rows}, {p->pages_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores or pages are misaligned, or strides of pages overlap",
+                what);
   ifa4::SelectPagesKernelArgs a{};
   a.scores = p->scores;
   a.pages = p->pages;
@@ -1992,9 +2045,11 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
     return fail(IFA4_ERR_UNSUPPORTED, "%s: more than 128 query heads per KV head", what);
   if (p->mass_width < 0 || p->mass_width > (1 << 30))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_width must be in [0, 2^30]", what);
-  if (p->mass_stride_b < 0 || p->mass_stride_h < 0)
-    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative mass strides", what);
   if (p->seqs.batch == 0 || p->mass_width == 0) return IFA4_OK;
+  if (!aligned4(p->mass) || !aligned4(p->lse) ||
+      !rows_apart(p->mass_width, {{p->mass_stride_b, p->seqs.batch}, {p->mass_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass or lse is misaligned, or strides of mass overlap",
+                what);
   if (p->mass == nullptr || (p->total_q > 0 && p->lse == nullptr))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", what);
   if (p->total_q == 0 && p->accumulate) return IFA4_OK;

@@ -42,8 +42,8 @@ __device__ __forceinline__ uint4 shfl_xor_v4(uint4 v, int m) {
 // ---------------------------------------------------------------------------------------
 // A warp per page and KV head: half a warp reads a key (16 bytes a lane), eight keys of each half in
 // flight; the halves are joined at the end, one writes the minima, the other the maxima (512
-// contiguous bytes).  Bound by HBM: 256 bytes a key and head read, 512 a page and head written (8 x 32k keys,
-// 8 KV heads: 86 us of 83.5 at the copy rate).
+// contiguous bytes).  Bound by HBM: 256 bytes a key and head read, 512 a page and head written (8 x 32k
+// keys, 8 KV heads: 86 us, 83.5 at the copy rate).
 __global__ void __launch_bounds__(kPageBoundsWarps * 32)
     page_bounds_kernel(const __grid_constant__ PageBoundsKernelArgs a) {
   const int lane = threadIdx.x & 31, half = lane >> 4, part = lane & 15;
@@ -863,13 +863,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
     decode_pages_merge_kernel(const __grid_constant__ DecodePagesKernelArgs a) {
   const int lane = threadIdx.x & 31;
   const long long at = static_cast<long long>(blockIdx.x) * kMergeWarps + (threadIdx.x >> 5);
-  if (at >= a.total_q * a.n_heads) return;
   const long long t = at / a.n_heads;
   const int h = static_cast<int>(at - t * a.n_heads);
   int n_k, pos;
-  const bool none = find_sequence(a.s, t, n_k, pos) < 0;
-  if (none && !a.zero_padding) return;
+  const bool none = t >= a.total_q || find_sequence(a.s, t, n_k, pos) < 0;
+  // warps with nothing to write wait, too: this grid does not end before the one it was launched beside
   wait_previous_kernel();
+  if (t >= a.total_q || (none && !a.zero_padding)) return;
   float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (!none) {

@@ -16,6 +16,8 @@ not differentiable: what they return is cut off from the graph of their inputs; 
 ``torch.jit.trace`` they are refused."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib, _ops, _paged
@@ -233,6 +235,8 @@ def _checked_decode(q, k, v, rel_logits, cu_q, cu_k, max_seqlen_k, rel_extent, p
     if any(s <= 0 for s in out.stride()[:-1]) and out.numel():
         raise ValueError(f"{name}: out must not be an expanded tensor")
     lse = _ops._lse_buffer(q, n_heads, return_lse, lse)
+    if scale == math.inf:
+        raise ValueError(f"{name}: softmax_scale must be finite")
     _paged.tensor(name, "pages", pages, q.device, torch.int32, 3)
     if pages.shape[:2] != (q.shape[0], kv_heads) or pages.shape[2] > _paged.MOST:
         raise ValueError(f"{name}: pages must be [total_q, kv_heads, num_selected], got "

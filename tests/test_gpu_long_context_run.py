@@ -346,5 +346,29 @@ def test_python_refusals():
     bad(TypeError, "float32", E, c.k, c.v, mass.double(), c.table, c.cu_k, 10)
 
 
+def test_written_memory_that_overlaps_and_scales_that_are_not_finite_are_refused():
+    c = Case([1], [50], 4, 2, 16, 20, seed=14)
+    bounds = inkling_kv_page_bounds(c.k, c.table, c.cu_k, c.cu_k)
+    pages, lse, mass = choose(c, 2), _lse(c, -1), _mass(c)
+    kw = dict(block_table=c.table, softmax_scale=math.inf)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        inkling_kv_page_scores(c.q, bounds, c.rel, c.cu_q, c.cu_k, 1, 20, 16, **kw)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        inkling_kv_attention_mass(c.q, c.k, c.rel, lse, c.cu_q, c.cu_k, 1, 50, 20, **kw)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        inkling_fa4_rel_attention_decode_pages(c.q, c.k, c.v, c.rel, c.cu_q, c.cu_k, 1, 50, 20, pages,
+                                               **kw)
+    # a head's maxima in the place of the next one's minima; tokens of one page in the place of the next's
+    flat = torch.zeros(c.pages * 768, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(_lib.Ifa4Error, match="overlap"):
+        inkling_kv_page_bounds(c.k, c.table, c.cu_q, c.cu_k,
+                               bounds=flat.as_strided((c.pages, 2, 2, 128), (512, 128, 128, 1)))
+    before = c.k.clone()
+    k = c.k.as_strided((c.pages - 1, 16, 2, 128), (128, 256, 128, 1))
+    with pytest.raises(_lib.Ifa4Error, match="overlap"):
+        inkling_kv_evict(k, c.v[:-1], mass, c.table, c.cu_k, 10)
+    assert torch.equal(c.k.view(torch.int16), before.view(torch.int16))  # NaN in unused slots
+
+
 def test_no_wait_was_given_up():
     assert _lib.read_device_status(torch.cuda.current_stream().cuda_stream, clear=False) == 0

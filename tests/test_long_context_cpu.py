@@ -72,6 +72,8 @@ QUERIES = [(dict(q=None), INVALID, b"null"), (dict(q_stride_t=0), INVALID, b"q n
            (dict(q=260), INVALID, b"q needs"), (dict(rel_extent=0), INVALID, b"rel_extent"),
            (dict(softmax_scale=0.0), INVALID, b"softmax_scale"),
            (dict(softmax_scale=float("nan")), INVALID, b"softmax_scale"),
+           (dict(softmax_scale=float("inf")), INVALID, b"softmax_scale"),
+           (dict(rel=257), INVALID, b"misaligned rel"), (dict(cu_seqlens_q=258), INVALID, b"cu_seqlens"),
            (dict(rel_stride_t=-1), INVALID, b"rel"), (dict(total_q=-1), INVALID, b"total_q"),
            (dict(n_heads=5), INVALID, b"n_heads")]
 
@@ -84,6 +86,8 @@ def _refused(fn, p, code, msg, *rest):
 
 @pytest.mark.parametrize("kw,code,msg", COMMON + KEYS + [
     (dict(bounds=None), INVALID, b"bounds"), (dict(bounds_stride_page=0), INVALID, b"bounds"),
+    (dict(bounds_stride_h=128), INVALID, b"overlap"), (dict(bounds_stride_page=256), INVALID, b"overlap"),
+    (dict(block_table=257), INVALID, b"misaligned"), (dict(cu_seqlens_k=258), INVALID, b"misaligned"),
     (dict(cu_seqlens_q=None), INVALID, b"cu_seqlens")])
 def test_page_bounds_refusals(kw, code, msg):
     _refused("ifa4_page_bounds_launch", _set(_lib.PageBoundsParams(), **{**SEQS, **CACHE, **BOUNDS, **kw}),
@@ -92,7 +96,9 @@ def test_page_bounds_refusals(kw, code, msg):
 
 @pytest.mark.parametrize("kw,code,msg", [x for x in COMMON if x[2] != b"kv_heads"] + QUERIES + [
     (dict(bounds=None), INVALID, b"bounds"), (dict(first_pages=-1), INVALID, b"first_pages"),
-    (dict(scores=None), INVALID, b"scores"), (dict(scores_stride_t=-1), INVALID, b"strides")])
+    (dict(scores=None), INVALID, b"scores"), (dict(scores_stride_t=-1), INVALID, b"strides"),
+    (dict(scores=258), INVALID, b"misaligned"), (dict(scores_stride_h=3), INVALID, b"overlap"),
+    (dict(scores_stride_t=0), INVALID, b"overlap")])
 def test_page_scores_refusals(kw, code, msg):
     base = {**SEQS, **BOUNDS, **QUERY, "kv_heads": 2, "head_dim": 128, "scores": 256,
             "scores_stride_t": 8, "scores_stride_h": 4}
@@ -103,9 +109,11 @@ def test_page_scores_refusals(kw, code, msg):
     (dict(num_selected=0), INVALID, b"num_selected"), (dict(width=-1), INVALID, b"width"),
     (dict(rows=-1), INVALID, b"rows"), (dict(scores=None), INVALID, b"null"),
     (dict(pages=None), INVALID, b"null"), (dict(pages_stride_h=-1), INVALID, b"strides"),
-    (dict(kv_heads=65536), INVALID, b"kv_heads")])
+    (dict(scores=258), INVALID, b"misaligned"), (dict(pages=257), INVALID, b"misaligned"),
+    (dict(pages_stride_t=2), INVALID, b"overlap"), (dict(kv_heads=65536), INVALID, b"kv_heads")])
 def test_select_pages_refusals(kw, code, msg):
-    base = dict(scores=256, pages=256, rows=2, kv_heads=2, width=4, num_selected=2)
+    base = dict(scores=256, pages=256, rows=2, kv_heads=2, width=4, num_selected=2, pages_stride_t=4,
+                pages_stride_h=2)
     _refused("ifa4_select_pages_launch", _set(_lib.SelectPagesParams(), **{**base, **kw}), code, msg, None)
 
 
@@ -131,6 +139,9 @@ def _decode_pages(**kw):
     (dict(num_selected=1 << 26, page_size=1 << 12), UNSUPPORTED, b"2^36"),
     (dict(page_size=24), INVALID, b"page_size"),
     (dict(total_q=1 << 31), UNSUPPORTED, b"rows"), (dict(batch=65535), UNSUPPORTED, b"batch"),
+    (dict(pages=258), INVALID, b"misaligned"), (dict(rel=257), INVALID, b"misaligned"),
+    (dict(lse=258), INVALID, b"misaligned"), (dict(block_table=257), INVALID, b"misaligned"),
+    (dict(softmax_scale=float("inf")), INVALID, b"softmax_scale"),
     (dict(q=260), INVALID, b"aligned")])
 def test_decode_pages_refusals(kw, code, msg):
     need = ctypes.c_size_t(0)
@@ -154,7 +165,9 @@ def test_decode_pages_workspace():
 @pytest.mark.parametrize("kw,code,msg", COMMON[:-1] + KEYS + QUERIES + [
     (dict(n_heads=258), UNSUPPORTED, b"128"), (dict(mass_width=-1), INVALID, b"mass_width"),
     (dict(mass=None), INVALID, b"null"), (dict(lse=None), INVALID, b"null"),
-    (dict(mass_stride_b=-1), INVALID, b"mass"), (dict(num_pages=0), INVALID, b"num_pages")])
+    (dict(mass_stride_b=-1), INVALID, b"mass"), (dict(num_pages=0), INVALID, b"num_pages"),
+    (dict(mass=258), INVALID, b"misaligned"), (dict(lse=257), INVALID, b"misaligned"),
+    (dict(mass_stride_h=63), INVALID, b"overlap"), (dict(mass_stride_b=0), INVALID, b"overlap")])
 def test_attention_mass_refusals(kw, code, msg):
     base = {**SEQS, **CACHE, **QUERY, "lse": 256, "mass": 256, "mass_width": 64, "mass_stride_b": 128,
             "mass_stride_h": 64}
@@ -167,6 +180,9 @@ def test_attention_mass_refusals(kw, code, msg):
     (dict(first=3, recent=2), INVALID, b"budget"), (dict(first=-1), INVALID, b"budget"),
     (dict(mass=None), INVALID, b"null"), (dict(mass=512), INVALID, b"mass_out"),
     (dict(kept=None), INVALID, b"null"), (dict(cu_out=None), INVALID, b"cu_out"),
+    (dict(kept=258), INVALID, b"misaligned"), (dict(cu_out=257), INVALID, b"misaligned"),
+    (dict(k_stride_t=128), INVALID, b"overlap"), (dict(v_stride_page=2048), INVALID, b"overlap"),
+    (dict(mass_stride_b=-1), INVALID, b"mass"), (dict(mass_out_stride_h=0), INVALID, b"overlap"),
     (dict(mass_width=-1), INVALID, b"mass_width")])
 def test_kv_evict_refusals(kw, code, msg):
     base = {**SEQS, **CACHE, "v_cache": 512, "v_stride_page": 4096, "v_stride_t": 256,
