@@ -2099,9 +2099,10 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
     if ((rc = encode_paged(&tk16, p->k_cache, p->seqs.num_pages, p->seqs.page_size, p->kv_heads,
                            p->k_stride_page, p->k_stride_t, p->k_stride_h, 16, "k")))
       return rc;
-    int64_t blocks = ceil_div(most_k, 128);
-    const int64_t want = ceil_div(8 * sms, heads);  // (measured: 52, 44 and 50 us with 4, 8 and 16)
-    if (blocks > want) blocks = want;
+    // a wave of two CTAs an SM, as far as there are 128 keys for each
+    int64_t blocks = 2 * sms / p->kv_heads;
+    if (blocks > ceil_div(most_k, 128) * p->seqs.batch) blocks = ceil_div(most_k, 128) * p->seqs.batch;
+    if (blocks < 1) blocks = 1;
     cudaError_t e = ifa4::launch_attention_mass_stream_sm100(a, static_cast<int>(blocks), tk16,
                                                              static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_fail(e, "attention_mass launch");

@@ -380,7 +380,7 @@ struct AttentionMassKernelArgs {
 // For sequences of at most kMassStreamRows rows (query tokens x heads of a group).
 constexpr int kMassStreamRows = 16;
 // tm_k: boxes of 16 keys.
-cudaError_t launch_attention_mass_stream_sm100(const AttentionMassKernelArgs& args, int key_blocks,
+cudaError_t launch_attention_mass_stream_sm100(const AttentionMassKernelArgs& args, int blocks,
                                                const CUtensorMap& tm_k, cudaStream_t stream);
 // Query rows of a tile for these many rows of a sequence: 32, 64 or 128.
 int attention_mass_tile_rows(long long rows, int group);

@@ -521,16 +521,22 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
 // own, 16 keys a stage, which one of its lanes refills by TMA as soon as the warp has read a stage: no
 // barriers between warps, no start to speak of, and 192 KB in flight on an SM.  Bound by HBM, 256 bytes
 // a key.  (8 sequences of 4k to 32k keys, one token each: 62 us on the kernel above, whose CTAs start
-// slowly and end in a half-empty wave; 50 us with the keys in registers, 64 KB in flight; 43 us, 45 a
-// call, so: 5.0 TB/s.  A contiguous stretch of keys for each warp: 55 us.)
+// slowly and end in a half-empty wave; 50 us with the keys in registers, 64 KB in flight.)  One wave of
+// CTAs shares out what all sequences read, in units of 128 keys of one head, so that lengths do not
+// matter: 38 us, 40 a call, 5.7 TB/s; 43 with the same number of CTAs for each sequence, four waves of
+// them, and 72 with one.  (Two stages and three CTAs an SM: 44; four warps, three stages, four CTAs: 39;
+// six stages, two CTAs: 47.)
 constexpr int kStreamWarps = 8;
+constexpr int kStreamThreads = kStreamWarps * 32;
+constexpr int kUnit = kStreamWarps * 16;  // keys that the warps take together
 constexpr int kStreamStages = 3;
 constexpr uint32_t kStreamHalf = 16 * 128;            // 16 keys, 64 dims
 constexpr uint32_t kStreamStage = 2 * kStreamHalf;
 constexpr uint32_t kStreamBar = kStreamWarps * kStreamStages * kStreamStage;
 constexpr uint32_t kStreamSmem = kStreamBar + 256 + 1024;
+static_assert(kStreamWarps * kStreamStages * 8 + 4 <= 256, "barriers and the flag");
 
-__global__ void __launch_bounds__(kStreamWarps * 32, 2)
+__global__ void __launch_bounds__(kStreamThreads, 2)
     attention_mass_stream_kernel(const __grid_constant__ AttentionMassKernelArgs a,
                                  const __grid_constant__ CUtensorMap tm_k) {
   extern __shared__ uint8_t smem_raw[];
@@ -540,7 +546,8 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStreamBar) + warp * kStreamStages;
   int* abort_flag = reinterpret_cast<int*>(smem + kStreamBar + 8 * kStreamWarps * kStreamStages);
   uint8_t* ring = smem + warp * kStreamStages * kStreamStage;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  __shared__ uint32_t sums[kStreamWarps], pre[kStreamThreads + 1];
+  const int kvh = blockIdx.y;
   if (lane == 0) {
     for (int i = 0; i < kStreamStages; ++i) mbar_init(&full[i], 1);
     if (warp == 0) {
@@ -551,184 +558,237 @@ __global__ void __launch_bounds__(kStreamWarps * 32, 2)
   }
   __syncthreads();
   const AbortCtx ab{abort_flag, a.status, kStatusDecodeTimeout};
-  const int32_t* table = table_row(a.s, b);
   const int mask = (1 << a.s.page_shift) - 1;
-  const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
-  const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
-  const int n_out = min(n_k, a.mass_width);
-  const int n_all = a.accumulate ? n_out : a.mass_width;  // places that are written
-  float* mass = a.mass + static_cast<long long>(b) * a.mass_sb + static_cast<long long>(kvh) * a.mass_sh;
-  const int shift = n_k - n_q;
-  const int n_rows = n_q * a.group;
-  // the first key that any row sees
-  const int first = a.window_left < 0 ? 0 : max(0, shift - a.window_left);
-  const int stride = static_cast<int>(gridDim.x) * kStreamWarps * 16;
-  const int k_warp = (static_cast<int>(blockIdx.x) * kStreamWarps + warp) * 16;
   const uint64_t pol = l2_policy_evict_first();
-
-  const auto visible = [&](int k0) { return k0 < n_out && k0 + 15 >= first && n_rows > 0; };
-  // page of the 16 keys from k0 on (page_size is a multiple of 16); num_pages reads zeros
-  const auto page_of = [&](int k0) {
-    int page = a.s.num_pages;
-    if (visible(k0)) {
-      const int p = page_at(a.s, table, k0 >> a.s.page_shift);
-      if (p >= 0) page = p;
-    }
-    return page;
-  };
-  const auto load = [&](int k0, int page, uint32_t st) {
-    if (lane == 0 && visible(k0)) {
-      mbar_arrive_expect_tx(&full[st], kStreamStage);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-        tma_load_4d_hint(ring + st * kStreamStage + hf * kStreamHalf, &tm_k, &full[st], hf * 64, kvh,
-                         k0 & mask, page, pol);
-    }
-  };
-  uint32_t done = 0;  // stages read so far: the ring goes on through all rounds
+  uint32_t done = 0;  // stages read so far: the ring goes on through all sequences
   bool ok = true;
-  // more than 16 rows (the caller's hint was too small): the keys once more for the next 16
-  for (int r0 = 0; (r0 == 0 || r0 < n_rows) && ok; r0 += 16) {
-    // the first visible keys of this warp, and the ring's first stages
-    int k_first = k_warp;
-    if (n_rows > 0 && k_first + 15 < first)
-      k_first += (first - k_first - 15 + stride - 1) / stride * stride;
-    int page_next;
-    {
-      int pages[kStreamStages];
-#pragma unroll
-      for (int i = 0; i < kStreamStages; ++i) pages[i] = page_of(k_first + i * stride);
-      page_next = page_of(k_first + kStreamStages * stride);
-#pragma unroll
-      for (int i = 0; i < kStreamStages; ++i)
-        load(k_first + i * stride, pages[i], (done + i) % kStreamStages);
-    }
-    // the rows: g and g + 8
-    uint32_t qa[8][4];
-    float lse[2], nlse[2];
-    int pos[2];
-    const uint16_t* rel[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = r0 + g + 8 * r, tok = row / a.group;
-      const bool on = row < n_rows;
-      const long long t = q0 + (on ? tok : 0);
-      const int h = kvh * a.group + (on ? row - tok * a.group : 0);
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(
-          a.q + t * a.q_st + static_cast<long long>(h) * a.q_sh);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        qa[kk][r] = on ? __ldg(src + kk * 8 + qd) : 0u;
-        qa[kk][2 + r] = on ? __ldg(src + kk * 8 + 4 + qd) : 0u;
-      }
-      lse[r] = on ? __ldg(a.lse + h * a.lse_sh + t * a.lse_st) : -INFINITY;
-      nlse[r] = lse[r] == -INFINITY ? -INFINITY : scaled_lse(-lse[r]);
-      pos[r] = lse[r] == -INFINITY ? -1 : shift + tok;  // a row that adds nothing sees nothing
-      rel[r] = a.rel + t * a.rel_st + static_cast<long long>(h) * a.rel_sh;
-    }
-    const int window = a.window_left < 0 ? 0x7fffffff : a.window_left;
-    const int p_min = __reduce_min_sync(0xffffffffu, min(pos[0] < 0 ? 0x7fffffff : pos[0],
-                                                         pos[1] < 0 ? 0x7fffffff : pos[1]));
-    const int p_max = __reduce_max_sync(0xffffffffu, max(pos[0], pos[1]));
 
-    for (int k0 = k_warp; k0 < n_all && ok; k0 += stride) {
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};  // keys k0 + 8 t + 2 qd + e
+  // What is read of a sequence: from the first key that any row sees to the last that has a place
+  struct Sequence {
+    int n_k, q0, n_q, n_out, first;
+    __device__ __forceinline__ int units() const {
+      return n_q > 0 && first < n_out ? ((n_out + kUnit - 1) / kUnit) - first / kUnit : 0;
+    }
+  };
+  const auto sequence = [&](int b) {
+    Sequence x;
+    x.n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+    x.q0 = __ldg(a.s.cu_q + b);
+    x.n_q = __ldg(a.s.cu_q + b + 1) - x.q0;
+    x.n_out = min(x.n_k, a.mass_width);
+    x.first = first_key(x.n_k - x.n_q, a.window_left);
+    return x;
+  };
+
+  // The keys [key_lo, key_hi) of sequence b, as far as they are read; key_lo a multiple of kUnit.
+  const auto stretch = [&](int b, int key_lo, int key_hi) {
+    const int32_t* table = table_row(a.s, b);
+    const Sequence seq = sequence(b);
+    const int q0 = seq.q0, first = seq.first, end = min(key_hi, seq.n_out);
+    float* mass = a.mass + static_cast<long long>(b) * a.mass_sb +
+                  static_cast<long long>(kvh) * a.mass_sh;
+    const int shift = seq.n_k - seq.n_q;
+    const int n_rows = seq.n_q * a.group;
+    int k_first = key_lo + warp * 16;
+    if (k_first + 15 < first) k_first += kUnit * ((first - k_first - 15 + kUnit - 1) / kUnit);
+    const auto visible = [&](int k0) { return k0 < end; };
+    // page of the 16 keys from k0 on (page_size is a multiple of 16); num_pages reads zeros
+    const auto page_of = [&](int k0) {
+      int page = a.s.num_pages;
       if (visible(k0)) {
-        // what the place holds, on its way while the keys are waited for
-        float old[2] = {0.f, 0.f};
-        const int place = k0 + 8 * g + 2 * qd;
-        if (a.accumulate || r0 > 0) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            load_plain_if(old[e], mass + place + e, g < 2 && place + e < n_out);
-        }
-        const uint32_t st = done % kStreamStages;
-        if (!(ok = mbar_wait_warp(&full[st], (done / kStreamStages) & 1, ab))) break;
-        const uint32_t base = smem_u32(ring + st * kStreamStage);
-        float acc[2][4], half[2][4];  // two halves of the depth, which do not wait for one another
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = half[t][i] = 0.f;
-        {
-          const int mi = lane >> 3;  // which 8x8 matrix this lane addresses
-          const int row = (mi >> 1) * 8 + (lane & 7);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const int chunk = 2 * kk + (mi & 1);
-            uint32_t b0, b1, b2, b3;
-            ldsm_x4(base + (chunk >> 3) * kStreamHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
-                    b0, b1, b2, b3);
-            mma_bf16(kk & 1 ? half[0] : acc[0], qa[kk], b0, b1);
-            mma_bf16(kk & 1 ? half[1] : acc[1], qa[kk], b2, b3);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] += half[t][i];
-        // the fragment loads have to be done, not only issued, before TMA refills the stage
-        fence_proxy_async_smem();
-        __syncwarp();
-        ++done;
-        load(k0 + kStreamStages * stride, page_next, st);
-        page_next = page_of(k0 + (kStreamStages + 1) * stride);
-        const bool near = p_min - (k0 + 15) < a.rel_extent;
-        if (!near && k0 + 15 <= p_min && p_max - k0 <= window) {
-          // every row sees every key, and none through the bias
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const float y = fast_exp2(__fmaf_rn(acc[t][2 * r + e], a.scale_log2, nlse[r]));
-                sum[2 * t + e] += pos[r] >= 0 ? y : 0.f;
-              }
-        } else {
-          uint16_t bias[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // t, e, r
-            const int r = i & 1, d = pos[r] - (k0 + 8 * (i >> 2) + 2 * qd + (i >> 1 & 1));
-            bias[i] = 0;
-            load_if(bias[i], rel[r] + d, pos[r] >= 0 && d >= 0 && d < a.rel_extent);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i & 1, t = i >> 2, e = i >> 1 & 1;
-            const int d = pos[r] - (k0 + 8 * t + 2 * qd + e);
-            // bias - lse first: either may be at the end of the range
-            const float y = fast_exp2(__fmaf_rn(bf16_bits_to_float(bias[i]) - lse[r], kLog2e,
-                                                acc[t][2 * r + e] * a.scale_log2));
-            sum[2 * t + e] += pos[r] >= 0 && d >= 0 && d <= window ? y : 0.f;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 4);
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
-          sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (g == t) sum[2 * t + e] += old[e];
+        const int p = page_at(a.s, table, k0 >> a.s.page_shift);
+        if (p >= 0) page = p;
       }
-      // lane qd of the first quad has keys 2 qd, 2 qd + 1 of the first eight; the second of the others
-      if (g < 2) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = k0 + 8 * g + 2 * qd + e;
-          const float y = g == 0 ? sum[e] : sum[2 + e];
-          if (key < n_all && IFA4_DBG_CHECK(a.status, key < a.mass_width)) {
-            if (key < n_out && visible(k0)) mass[key] = y;
-            else if (!a.accumulate && r0 == 0) mass[key] = 0.f;
+      return page;
+    };
+    const auto load = [&](int k0, int page, uint32_t st) {
+      if (lane == 0 && visible(k0)) {
+        mbar_arrive_expect_tx(&full[st], kStreamStage);
+  #pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          tma_load_4d_hint(ring + st * kStreamStage + hf * kStreamHalf, &tm_k, &full[st], hf * 64, kvh,
+                           k0 & mask, page, pol);
+      }
+    };
+    // more than 16 rows (the caller's hint was too small): the keys once more for the next 16
+    for (int r0 = 0; (r0 == 0 || r0 < n_rows) && ok; r0 += 16) {
+      // the ring's first stages
+      int page_next;
+      {
+        int pages[kStreamStages];
+  #pragma unroll
+        for (int i = 0; i < kStreamStages; ++i) pages[i] = page_of(k_first + i * kUnit);
+        page_next = page_of(k_first + kStreamStages * kUnit);
+  #pragma unroll
+        for (int i = 0; i < kStreamStages; ++i)
+          load(k_first + i * kUnit, pages[i], (done + i) % kStreamStages);
+      }
+      // the rows: g and g + 8
+      uint32_t qa[8][4];
+      float lse[2], nlse[2];
+      int pos[2];
+      const uint16_t* rel[2];
+  #pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = r0 + g + 8 * r, tok = row / a.group;
+        const bool on = row < n_rows;
+        const long long t = q0 + (on ? tok : 0);
+        const int h = kvh * a.group + (on ? row - tok * a.group : 0);
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(
+            a.q + t * a.q_st + static_cast<long long>(h) * a.q_sh);
+  #pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qa[kk][r] = on ? __ldg(src + kk * 8 + qd) : 0u;
+          qa[kk][2 + r] = on ? __ldg(src + kk * 8 + 4 + qd) : 0u;
+        }
+        lse[r] = on ? __ldg(a.lse + h * a.lse_sh + t * a.lse_st) : -INFINITY;
+        nlse[r] = lse[r] == -INFINITY ? -INFINITY : scaled_lse(-lse[r]);
+        pos[r] = lse[r] == -INFINITY ? -1 : shift + tok;  // a row that adds nothing sees nothing
+        rel[r] = a.rel + t * a.rel_st + static_cast<long long>(h) * a.rel_sh;
+      }
+      const int window = a.window_left < 0 ? 0x7fffffff : a.window_left;
+      const int p_min = __reduce_min_sync(0xffffffffu, min(pos[0] < 0 ? 0x7fffffff : pos[0],
+                                                           pos[1] < 0 ? 0x7fffffff : pos[1]));
+      const int p_max = __reduce_max_sync(0xffffffffu, max(pos[0], pos[1]));
+
+      for (int k0 = k_first; k0 < end; k0 += kUnit) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};  // keys k0 + 8 t + 2 qd + e
+        {
+          // what the place holds, on its way while the keys are waited for
+          float old[2] = {0.f, 0.f};
+          const int place = k0 + 8 * g + 2 * qd;
+          if (a.accumulate || r0 > 0) {
+  #pragma unroll
+            for (int e = 0; e < 2; ++e)
+              load_plain_if(old[e], mass + place + e, g < 2 && place + e < end);
+          }
+          const uint32_t st = done % kStreamStages;
+          if (!(ok = mbar_wait_warp(&full[st], (done / kStreamStages) & 1, ab))) break;
+          const uint32_t base = smem_u32(ring + st * kStreamStage);
+          float acc[2][4], half[2][4];  // two halves of the depth, which do not wait for one another
+  #pragma unroll
+          for (int t = 0; t < 2; ++t)
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][i] = half[t][i] = 0.f;
+          {
+            const int mi = lane >> 3;  // which 8x8 matrix this lane addresses
+            const int row = (mi >> 1) * 8 + (lane & 7);
+  #pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const int chunk = 2 * kk + (mi & 1);
+              uint32_t b0, b1, b2, b3;
+              ldsm_x4(base + (chunk >> 3) * kStreamHalf + row * 128 + (((chunk & 7) ^ (row & 7)) << 4),
+                      b0, b1, b2, b3);
+              mma_bf16(kk & 1 ? half[0] : acc[0], qa[kk], b0, b1);
+              mma_bf16(kk & 1 ? half[1] : acc[1], qa[kk], b2, b3);
+            }
+          }
+  #pragma unroll
+          for (int t = 0; t < 2; ++t)
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][i] += half[t][i];
+          // the fragment loads have to be done, not only issued, before TMA refills the stage
+          fence_proxy_async_smem();
+          __syncwarp();
+          ++done;
+          load(k0 + kStreamStages * kUnit, page_next, st);
+          page_next = page_of(k0 + (kStreamStages + 1) * kUnit);
+          const bool near = p_min - (k0 + 15) < a.rel_extent;
+          if (!near && k0 + 15 <= p_min && p_max - k0 <= window) {
+            // every row sees every key, and none through the bias
+  #pragma unroll
+            for (int t = 0; t < 2; ++t)
+  #pragma unroll
+              for (int e = 0; e < 2; ++e)
+  #pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  const float y = fast_exp2(__fmaf_rn(acc[t][2 * r + e], a.scale_log2, nlse[r]));
+                  sum[2 * t + e] += pos[r] >= 0 ? y : 0.f;
+                }
+          } else {
+            uint16_t bias[8];
+  #pragma unroll
+            for (int i = 0; i < 8; ++i) {  // t, e, r
+              const int r = i & 1, d = pos[r] - (k0 + 8 * (i >> 2) + 2 * qd + (i >> 1 & 1));
+              bias[i] = 0;
+              load_if(bias[i], rel[r] + d, pos[r] >= 0 && d >= 0 && d < a.rel_extent);
+            }
+  #pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = i & 1, t = i >> 2, e = i >> 1 & 1;
+              const int d = pos[r] - (k0 + 8 * t + 2 * qd + e);
+              // bias - lse first: either may be at the end of the range
+              const float y = fast_exp2(__fmaf_rn(bf16_bits_to_float(bias[i]) - lse[r], kLog2e,
+                                                  acc[t][2 * r + e] * a.scale_log2));
+              sum[2 * t + e] += pos[r] >= 0 && d >= 0 && d <= window ? y : 0.f;
+            }
+          }
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 4);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 16);
+          }
+  #pragma unroll
+          for (int t = 0; t < 2; ++t)
+  #pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (g == t) sum[2 * t + e] += old[e];
+        }
+        // lane qd of the first quad has keys 2 qd, 2 qd + 1 of the first eight; the second of the others
+        if (g < 2) {
+  #pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = k0 + 8 * g + 2 * qd + e;
+            const float y = g == 0 ? sum[e] : sum[2 + e];
+            if (key < end && IFA4_DBG_CHECK(a.status, key < a.mass_width)) mass[key] = y;
           }
         }
       }
     }
+  };
+
+  // The units of all sequences in a row, an equal share of them for every CTA of a head
+  const auto units = [&](int b) {
+    return b < a.s.batch ? static_cast<uint32_t>(sequence(b).units()) : 0u;
+  };
+  const int tid = threadIdx.x;
+  uint32_t total = 0, sum, before = 0, mine = 0;
+  for (int b0 = 0; b0 < a.s.batch; b0 += kStreamThreads) {
+    mine = units(b0 + tid);
+    before = block_exclusive_sum<kStreamThreads>(mine, sums, sum);
+    total += sum;
   }
+  const uint32_t lo = static_cast<uint32_t>(static_cast<uint64_t>(total) * blockIdx.x / gridDim.x);
+  const uint32_t hi = static_cast<uint32_t>(static_cast<uint64_t>(total) * (blockIdx.x + 1) / gridDim.x);
+  uint32_t base = 0;
+  for (int b0 = 0; b0 < a.s.batch && base < hi; b0 += kStreamThreads) {
+    if (a.s.batch > kStreamThreads) {
+      mine = units(b0 + tid);
+      before = block_exclusive_sum<kStreamThreads>(mine, sums, sum);
+    }
+    pre[tid] = base + before;
+    if (tid == kStreamThreads - 1) pre[kStreamThreads] = base + sum;
+    base += sum;
+    // the first sequence that does not end before the share
+    const int i0 = __syncthreads_count(pre[tid] + mine <= lo);
+    for (int i = i0; i < kStreamThreads && pre[i] < hi && ok; ++i) {
+      if (pre[i + 1] == pre[i]) continue;
+      const int u0 = sequence(b0 + i).first / kUnit;
+      stretch(b0 + i, (static_cast<int>(max(lo, pre[i]) - pre[i]) + u0) * kUnit,
+              (static_cast<int>(min(hi, pre[i + 1]) - pre[i]) + u0) * kUnit);
+    }
+    __syncthreads();
+  }
+  if (!a.accumulate)  // places of keys that no row sees, and those behind the keys
+    for (int b = 0; b < a.s.batch; ++b) {
+      const Sequence seq = sequence(b);
+      float* mass = a.mass + static_cast<long long>(b) * a.mass_sb +
+                    static_cast<long long>(kvh) * a.mass_sh;
+      const int step = static_cast<int>(gridDim.x) * kStreamThreads;
+      for (int key = static_cast<int>(blockIdx.x) * kStreamThreads + tid; key < a.mass_width; key += step)
+        if (key >= seq.n_out || seq.n_q <= 0 || (key | 15) < seq.first) mass[key] = 0.f;
+    }
   // after a wait that was given up: what is in flight has landed before the memory goes
   if (!ok && lane == 0)
     for (uint32_t i = 0; i < kStreamStages; ++i)
@@ -960,14 +1020,13 @@ int attention_mass_tile_rows(long long rows, int group) {
   return n;
 }
 
-cudaError_t launch_attention_mass_stream_sm100(const AttentionMassKernelArgs& args, int key_blocks,
+cudaError_t launch_attention_mass_stream_sm100(const AttentionMassKernelArgs& args, int blocks,
                                                const CUtensorMap& tm_k, cudaStream_t stream) {
   static std::atomic<bool> attr[64];
   cudaError_t e = set_smem_limit_once(mass::attention_mass_stream_kernel, mass::kStreamSmem, attr);
   if (e != cudaSuccess) return e;
-  mass::attention_mass_stream_kernel<<<dim3(key_blocks, args.kv_heads, args.s.batch),
-                                       mass::kStreamWarps * 32, mass::kStreamSmem, stream>>>(args,
-                                                                                             tm_k);
+  mass::attention_mass_stream_kernel<<<dim3(blocks, args.kv_heads), mass::kStreamThreads,
+                                       mass::kStreamSmem, stream>>>(args, tm_k);
   return cudaGetLastError();
 }
 
@@ -987,7 +1046,8 @@ cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, int blocks, cud
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int total = args.s.batch * args.kv_heads * args.stretches;
-  return launch_early(evict::kv_evict_move_kernel, dim3(total < blocks ? total : blocks), evict::kMoveThreads, 0, stream, args);
+  return launch_early(evict::kv_evict_move_kernel, dim3(total < blocks ? total : blocks),
+                      evict::kMoveThreads, 0, stream, args);
 }
 
 }  // namespace ifa4

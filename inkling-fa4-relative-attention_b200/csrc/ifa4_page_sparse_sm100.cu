@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
     const int p0 = n_k - n_q + tok0;  // position of the block's first token
     const int p1 = p0 + n_tok - 1;    // and of its last
     // pages that any token sees
-    const int c_lo = (a.window_left < 0 ? 0 : max(0, p0 - a.window_left)) >> shift;
+    const int c_lo = first_key(p0, a.window_left) >> shift;
     const int c_hi = p1 >= 0 ? p1 >> shift : -1;
     // eight pages of a warp's turn are read if any of them is seen
     const int c_last = min(c_hi, page1 - 1);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
     // the last token's first pages on (all but the first first_pages) up to those within the bias's
     // reach of the first token
     const int c_inside =
-        ((a.window_left < 0 ? 0 : max(0, p1 - a.window_left)) >> shift) + max(1, a.first_pages);
+        (first_key(p1, a.window_left) >> shift) + max(1, a.first_pages);
     const int c_inside_end =
         p0 < a.rel_extent || group > 16
             ? -1
@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
       // ---- largest bias of the pages within its reach: the block's keys from `near` on
       const int near = max(max(0, p0 - a.rel_extent + 1), page0 << shift);
       const int slice0 = near >> 4;
-      const int slices = mine ? (min(p1, ((page1 - 1) << shift) + ((1 << shift) - 1)) >> 4) - slice0 + 1 : 0;
+      const int slices =
+          mine ? (min(p1, ((page1 - 1) << shift) + ((1 << shift) - 1)) >> 4) - slice0 + 1 : 0;
       if (slices > 0) {
         const int c_near = near >> shift;
         const int c_end = min(page1 - 1, c_hi);
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
         if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by the same thread
         if (h0 + 16 >= group && p0 + tok >= 0) {
           const int p = p0 + tok, hi = p >> shift;
-          const int lo = (a.window_left < 0 ? 0 : max(0, p - a.window_left)) >> shift;
+          const int lo = first_key(p, a.window_left) >> shift;
           if (c >= lo && c <= hi && (c - lo < a.first_pages || hi - c < a.last_pages)) y = INFINITY;
         }
         *dst = y;
@@ -523,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     return;
   }
   const int hi = pos + 1;  // visible keys [lo, hi); none where hi <= 0
-  const int lo = a.window_left >= 0 ? max(0, pos - a.window_left) : 0;
+  const int lo = first_key(pos, a.window_left);
   const int c_lo = lo >> a.s.page_shift, c_hi = hi > 0 ? pos >> a.s.page_shift : -1;
   __syncthreads();
   {

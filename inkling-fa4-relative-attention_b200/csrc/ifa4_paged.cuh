@@ -9,6 +9,11 @@
 
 namespace ifa4 {
 
+// The first key that position p sees (p may be negative, the window as long as it likes).
+__device__ __forceinline__ int first_key(int p, int window_left) {
+  return window_left >= 0 && p > window_left ? p - window_left : 0;
+}
+
 // Sequence b of row t (cu_q[b] <= t < cu_q[b + 1]), its key count and the row's position; -1 for a row
 // of none.  Whole warp; one load for a decode batch (one row a sequence), otherwise 32 places are looked
 // at a time (one step for up to 33 sequences, two for 1057) and a load for the lengths follows.

@@ -219,6 +219,19 @@ def test_mass_of_single_tokens_over_many_turns(window):
     _check_mass(c, _lse(c, window), window)
 
 
+@pytest.mark.parametrize("window", [-1, 37])
+@pytest.mark.parametrize("batch,most", [(40, 700), (600, 90)])  # 600: more than a block counts at once
+def test_mass_of_single_tokens_of_many_sequences(batch, most, window):
+    rng = np.random.default_rng(batch)
+    n_k = [int(n) for n in rng.integers(0, most, batch)]
+    n_q = [int(n) for n in rng.integers(0, 3, batch)]
+    n_k[7], n_k[-1], n_q[7], n_q[-1] = 4 * most, 3 * most, 1, 2
+    c = Case(n_q, n_k, 4, 2, 16, 50, seed=16)
+    lse = _lse(c, window)
+    _check_mass(c, lse, window)
+    _check_mass(c, lse, window, _mass(c))
+
+
 def test_chunks_of_scores_and_attention():
     """More tokens than a block of rows, windows that begin inside a block's pages."""
     c = Case([70, 33], [900, 40], 8, 2, 16, 60, seed=8)
@@ -368,6 +381,26 @@ def test_written_memory_that_overlaps_and_scales_that_are_not_finite_are_refused
     with pytest.raises(_lib.Ifa4Error, match="overlap"):
         inkling_kv_evict(k, c.v[:-1], mass, c.table, c.cu_k, 10)
     assert torch.equal(c.k.view(torch.int16), before.view(torch.int16))  # NaN in unused slots
+
+
+@pytest.mark.parametrize("heads", [4, 40])  # streamed keys, tiles of rows
+def test_a_window_as_long_as_it_can_be_is_none(heads):
+    c = Case([6, 2, 1], [3, 90, 0], heads, 2, 16, 20, seed=15)  # the first rows lie before every key
+    bounds = inkling_kv_page_bounds(c.k, c.table, c.cu_k, c.cu_k)
+    pages, lse = choose(c, 3), _lse(c, -1)
+
+    def run(window):
+        kw = dict(block_table=c.table)
+        return (inkling_kv_page_scores(c.q, bounds, c.rel, c.cu_q, c.cu_k, 6, 20, 16, window, **kw),
+                inkling_fa4_rel_attention_decode_pages(c.q, c.k, c.v, c.rel, c.cu_q, c.cu_k, 6, 90, 20,
+                                                       pages, window, **kw),
+                inkling_kv_attention_mass(c.q, c.k, c.rel, lse, c.cu_q, c.cu_k, 6, 90, 20, window, **kw))
+
+    want = run((-1, -1))
+    assert torch.isfinite(want[0]).any() and want[2].any()
+    for window in (2**31 - 1, 2**31 - 2, 2**40):
+        for x, y in zip(run((window, 0)), want):
+            assert torch.equal(x, y)
 
 
 def test_no_wait_was_given_up():
