@@ -197,6 +197,15 @@ def test_select_rows_that_no_block_holds(width):
     _select(x, width - 3)
 
 
+@pytest.mark.parametrize("width", [8193, 12345, 16384, 16385])
+def test_select_wide_rows(width):
+    g = torch.Generator().manual_seed(width)
+    x = torch.randn(2, 2, width, generator=g).cuda()
+    x[1] = x[1].round()
+    for count in (1, 700, width - 1):
+        _select(x, count)
+
+
 @pytest.mark.parametrize("n", [13000, 40000])
 def test_evict_long_sequences(n):
     c = Case([1], [n], 2, 1, 256, 8, seed=5)
