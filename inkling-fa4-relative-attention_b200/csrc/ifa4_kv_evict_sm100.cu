@@ -780,14 +780,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     }
     __syncthreads();
   }
-  if (!a.accumulate)  // places of keys that no row sees, and those behind the keys
+  if (!a.accumulate)  // places that no warp above wrote: of keys that no row sees, and behind the keys
     for (int b = 0; b < a.s.batch; ++b) {
       const Sequence seq = sequence(b);
       float* mass = a.mass + static_cast<long long>(b) * a.mass_sb +
                     static_cast<long long>(kvh) * a.mass_sh;
       const int step = static_cast<int>(gridDim.x) * kStreamThreads;
       for (int key = static_cast<int>(blockIdx.x) * kStreamThreads + tid; key < a.mass_width; key += step)
-        if (key >= seq.n_out || seq.n_q <= 0 || (key | 15) < seq.first) mass[key] = 0.f;
+        if (key >= seq.n_out || seq.units() == 0 || (key | 15) < seq.first) mass[key] = 0.f;
     }
   // after a wait that was given up: what is in flight has landed before the memory goes
   if (!ok && lane == 0)
