@@ -537,7 +537,7 @@ int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* params,
  * sees the keys j with 0 <= p - j (and p - j <= window_left where that is >= 0).  Key j of sequence b
  * sits in page block_table[b * block_table_stride + j / page_size], slot j % page_size; an entry
  * outside [0, num_pages), or past table_width, is no page (its keys read as zeros, nothing is written
- * there).  Rows from cu_seqlens_q[batch] on belong to no sequence. */
+ * there).  Rows in front of cu_seqlens_q[0] and from cu_seqlens_q[batch] on belong to no sequence. */
 typedef struct IFA4PagedSeqs {
   const int32_t* cu_seqlens_q;  /* int32 [batch + 1] on the device                         */
   const int32_t* cu_seqlens_k;  /* int32 [batch + 1] on the device                         */

@@ -136,11 +136,14 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
   const int b = blockIdx.z;
   const int width = a.s.table_width, shift = a.s.page_shift;
   const int page1 = min(width, page0 + a.block_pages);
-  if (b == a.s.batch) {  // rows of no sequence
-    const long long t0 = max(0, __ldg(a.s.cu_q + a.s.batch));
-    for (long long t = t0 + rb0; t < a.total_q; t += a.row_blocks)
+  if (b == a.s.batch) {  // rows of no sequence: in front of the first and behind the last
+    const long long first = max(0, __ldg(a.s.cu_q)), end = max(0, __ldg(a.s.cu_q + a.s.batch));
+    for (long long i = rb0;; i += a.row_blocks) {
+      const long long t = i < first ? i : end + (i - first);
+      if (t >= a.total_q) break;
       for (int c = page0 + threadIdx.x; c < page1; c += kScoreWarps * 32)
         a.scores[t * a.sc_st + kvh * a.sc_sh + c] = -INFINITY;
+    }
     return;
   }
   const int32_t* table = table_row(a.s, b);

@@ -81,8 +81,9 @@ def inkling_kv_page_scores(q, bounds, rel_logits, cu_seqlens_q, cu_seqlens_k, ma
     without a visible key scores -inf; the first ``first_pages`` and the last ``last_pages`` of a
     query's visible pages score +inf, so they are always chosen.  NaN or infinite bounds give what the
     formula gives (a choice ranks NaN above everything).  A table entry that is no page counts as a
-    page of zero keys, as the attention reads it.  Rows behind the last sequence are -inf in a new
-    tensor and stay as they are in ``out``."""
+    page of zero keys, as the attention reads it.  Rows of no sequence (behind the last, or in front
+    of the first where the offsets do not begin at 0) are -inf in a new tensor and stay as they are
+    in ``out``."""
     if out is None and _ops.USE_TORCH_OPS:
         outs = _lib.plain_call("page_scores", q, bounds, rel_logits, cu_seqlens_q, cu_seqlens_k,
                                block_table, max_seqlen_q or 0, rel_extent, page_size,
@@ -199,8 +200,8 @@ def inkling_fa4_rel_attention_decode_pages(q, k, v, rel_logits, cu_seqlens_q, cu
 
     Any number of queries a sequence (each reads its own pages: for long chunks that share their keys
     the prefill does less).  A query without keys gets 0 (lse -inf); one whose logits hold NaN or +inf
-    is NaN.  Rows behind the last sequence are zeros (lse -inf) in new tensors and stay as they are in
-    ``out`` / ``lse`` where ``out`` is given.  ``num_splits``: CTAs that share a query's pages (0:
+    is NaN.  Rows of no sequence are zeros (lse -inf) in new tensors and stay as they are in ``out`` /
+    ``lse`` where ``out`` is given.  ``num_splits``: CTAs that share a query's pages (0:
     automatic); ``workspace``: a reusable uint8 CUDA tensor (allocated per call when absent or too
     small); calls that may run at the same time need one each."""
     if (out is None and lse is None and not return_lse and n_heads is None and kv_heads is None
