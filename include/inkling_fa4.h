@@ -640,7 +640,7 @@ int ifa4_decode_pages_launch(const IFA4DecodePagesParams* params, void* workspac
 /* Attention weight that keys gather: mass[b, g, j] (+)= sum over the rows t of sequence b that see
  * key j and the heads h of group g of exp(softmax_scale q_th . k_gj + bias(t, h, p - j) - lse[h, t]),
  * in fp32 and in a fixed order.  lse is that of the attention over the same keys (a row whose lse is
- * -inf adds nothing).  accumulate: places past a sequence's keys stay as they are; otherwise every
+ * -inf adds nothing, whatever its query, its bias and the keys that only such rows see hold).  accumulate: places past a sequence's keys stay as they are; otherwise every
  * place is written, those with 0.  n_heads / kv_heads <= 128. */
 typedef struct IFA4AttentionMassParams {
   IFA4PagedSeqs seqs;

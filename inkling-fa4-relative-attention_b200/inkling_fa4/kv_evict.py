@@ -19,8 +19,9 @@ def inkling_kv_attention_mass(q, k, rel_logits, lse, cu_seqlens_q, cu_seqlens_k,
 
     over the queries that see it (``causal_align="bottom_right"``, the window, the relative bias as in
     the attention), in fp32 and in a fixed order.  ``lse [n_heads, total_q]`` fp32 is what the
-    attention call on the same arguments returns with ``return_lse=True``; a query without keys (lse
-    -inf) adds nothing.
+    attention call on the same arguments (with ``causal_align="bottom_right"``) returns with
+    ``return_lse=True``; a query whose lse is -inf (one without keys, or padding for which the caller
+    sets it) adds nothing, whatever it holds.
 
     ``k`` is the paged cache.  ``mass [batch, kv_heads, width]`` fp32 with unit last stride is added to
     in place, at the places of the sequences' keys only (a key from ``width`` on has none); without it
