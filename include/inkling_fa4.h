@@ -537,7 +537,9 @@ int ifa4_bucket_bias_backward_launch(const IFA4BucketBiasBackwardParams* params,
  * sees the keys j with 0 <= p - j (and p - j <= window_left where that is >= 0).  Key j of sequence b
  * sits in page block_table[b * block_table_stride + j / page_size], slot j % page_size; an entry
  * outside [0, num_pages), or past table_width, is no page (its keys read as zeros, nothing is written
- * there).  Rows in front of cu_seqlens_q[0] and from cu_seqlens_q[batch] on belong to no sequence. */
+ * there).  Rows in front of cu_seqlens_q[0] and from cu_seqlens_q[batch] on belong to no sequence.  No
+ * element that a call writes may be one that it reads, but for the caches of an eviction and masses
+ * that are added to, and no two outputs may share one. */
 typedef struct IFA4PagedSeqs {
   const int32_t* cu_seqlens_q;  /* int32 [batch + 1] on the device                         */
   const int32_t* cu_seqlens_k;  /* int32 [batch + 1] on the device                         */
@@ -640,8 +642,9 @@ int ifa4_decode_pages_launch(const IFA4DecodePagesParams* params, void* workspac
 /* Attention weight that keys gather: mass[b, g, j] (+)= sum over the rows t of sequence b that see
  * key j and the heads h of group g of exp(softmax_scale q_th . k_gj + bias(t, h, p - j) - lse[h, t]),
  * in fp32 and in a fixed order.  lse is that of the attention over the same keys (a row whose lse is
- * -inf adds nothing, whatever its query, its bias and the keys that only such rows see hold).  accumulate: places past a sequence's keys stay as they are; otherwise every
- * place is written, those with 0.  n_heads / kv_heads <= 128. */
+ * -inf adds nothing, whatever its query, its bias and the keys that only such rows see hold).
+ * accumulate: places past a sequence's keys stay as they are; otherwise every place is written, those
+ * with 0.  n_heads / kv_heads <= 128. */
 typedef struct IFA4AttentionMassParams {
   IFA4PagedSeqs seqs;
   const void* q;
@@ -675,10 +678,12 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* params, void* stre
  * everything) up to budget, in their order; their K and V rows move to the places 0 .. budget - 1 of
  * the sequence, in place.  kept gets the places they had (-1 behind the last), mass_out the masses of
  * what is kept with zeros behind, cu_out the offsets of the new lengths.  Shorter sequences keep
- * everything.  A kept key without a page is zeros at its new place.  No page that keys
- * move into or out of may be held by another sequence, or twice by its own.  seqs.cu_seqlens_q is not used; the workspace
- * (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by calls that may run at
- * the same time. */
+ * everything.  A kept key without a page is zeros at its new place.  No page that keys move into or
+ * out of may be held by another sequence, or twice by its own.  k_cache and v_cache have no element in
+ * common (two tensors, or slices of one with the same strides); mass_out, kept and cu_out are other
+ * memory than all the rest, so the lengths are not updated in place.  seqs.cu_seqlens_q is not used;
+ * the workspace (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by calls that
+ * may run at the same time. */
 typedef struct IFA4KvEvictParams {
   IFA4PagedSeqs seqs;
   void* k_cache;
@@ -686,7 +691,7 @@ typedef struct IFA4KvEvictParams {
   const float* mass;            /* [batch, kv_heads, mass_width], unit last stride         */
   float* mass_out;              /* the same shape, other memory                            */
   int32_t* kept;                /* [batch, kv_heads, budget], contiguous                   */
-  int32_t* cu_out;              /* [batch + 1]                                             */
+  int32_t* cu_out;              /* [batch + 1], other memory than seqs.cu_seqlens_k        */
   int64_t k_stride_page, k_stride_t, k_stride_h;
   int64_t v_stride_page, v_stride_t, v_stride_h;
   int64_t mass_stride_b, mass_stride_h;

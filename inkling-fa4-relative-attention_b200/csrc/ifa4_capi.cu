@@ -1613,6 +1613,63 @@ bool rows_apart(int64_t row, std::initializer_list<std::pair<int64_t, int64_t>> 
   return true;
 }
 
+// Memory from the first to behind the last byte of a tensor.
+struct Span {
+  const char* name;
+  uintptr_t lo, hi;
+};
+Span span_of(const char* name, const void* p, int64_t row_bytes,
+             std::initializer_list<std::pair<int64_t, int64_t>> dims = {}) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  Span s{name, lo, lo};
+  int64_t bytes = row_bytes;
+  for (const auto& d : dims) {
+    if (d.second <= 0) return s;  // nothing
+    bytes += d.first * (d.second - 1);
+  }
+  if (p != nullptr && bytes > 0) s.hi += static_cast<uintptr_t>(bytes);
+  return s;
+}
+bool spans_meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// Whether two tensors of the same shape have an element in common: rows of `row` bytes at a + sum i_d
+// stride_d and b + sum j_d stride_d (bytes).  Exact where both have the same strides, none of whose rows
+// share an element (see rows_apart); with other strides, whether their spans meet.
+struct RowDim {
+  int64_t stride_a, stride_b, count;
+};
+bool rows_meet(int64_t apart, int64_t row, const RowDim* d, int n) {  // strides descend
+  if (n == 0) return apart > -row && apart < row;
+  int64_t reach = row;  // bytes that the inner dimensions take up
+  for (int i = 1; i < n; ++i) reach += d[i].stride_a * (d[i].count - 1);
+  const int64_t s = d[0].stride_a;  // at least `reach`: two steps at most bring the rows near one another
+  for (int64_t step = apart / s - 1; step <= apart / s + 1; ++step) {
+    const int64_t left = apart - step * s;
+    if (step > -d[0].count && step < d[0].count && left > -reach && left < reach &&
+        rows_meet(left, row, d + 1, n - 1))
+      return true;
+  }
+  return false;
+}
+bool tensors_meet(const void* a, const void* b, int64_t row, std::initializer_list<RowDim> dims) {
+  RowDim d[3];
+  int n = 0;
+  int64_t end_a = row, end_b = row;
+  bool same = true;
+  for (const auto& x : dims) {
+    if (x.count <= 0) return false;
+    if (x.count == 1) continue;
+    end_a += x.stride_a * (x.count - 1);
+    end_b += x.stride_b * (x.count - 1);
+    same = same && x.stride_a == x.stride_b;
+    d[n++] = x;
+  }
+  const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+  if (row <= 0 || apart >= end_a || -apart >= end_b) return false;
+  std::sort(d, d + n, [](const RowDim& x, const RowDim& y) { return x.stride_a > y.stride_a; });
+  return !same || rows_meet(apart, row, d, n);
+}
+
 int check_seqs(const char* what, const IFA4PagedSeqs* s, bool queries) {
   if (s->batch < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative batch", what);
   if (s->batch > 65534) return fail(IFA4_ERR_UNSUPPORTED, "%s: batch > 65534", what);
@@ -1809,6 +1866,45 @@ int validate_evict(const IFA4KvEvictParams* p) {
                                   {p->mass_out_stride_h, p->kv_heads}}))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative mass strides, or strides of mass_out overlap",
                 what);
+  // Blocks read what others write: the lengths and masses while the new ones are written, the rows of
+  // both caches while rows move.
+  if (tensors_meet(p->k_cache, p->v_cache, 2 * p->head_dim,
+                   {{2 * p->k_stride_page, 2 * p->v_stride_page, p->seqs.num_pages},
+                    {2 * p->k_stride_t, 2 * p->v_stride_t, p->seqs.page_size},
+                    {2 * p->k_stride_h, 2 * p->v_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: k_cache and v_cache share memory", what);
+  if (tensors_meet(p->mass, p->mass_out, 4 * int64_t{p->mass_width},
+                   {{4 * p->mass_stride_b, 4 * p->mass_out_stride_b, p->seqs.batch},
+                    {4 * p->mass_stride_h, 4 * p->mass_out_stride_h, p->kv_heads}}))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: mass_out shares memory with mass", what);
+  const int64_t batch = p->seqs.batch, heads = p->kv_heads;
+  const Span written[] = {
+      span_of("kept", p->kept, 4 * batch * heads * p->budget),
+      span_of("cu_out", p->cu_out, 4 * (batch + 1)),
+      span_of("mass_out", p->mass_width > 0 ? p->mass_out : nullptr, 4 * int64_t{p->mass_width},
+              {{4 * p->mass_out_stride_b, batch}, {4 * p->mass_out_stride_h, heads}})};
+  const Span other[] = {
+      span_of("cu_seqlens_k", p->seqs.cu_seqlens_k, 4 * (batch + 1)),
+      span_of("block_table", p->seqs.block_table, 4 * int64_t{p->seqs.table_width},
+              {{4 * p->seqs.block_table_stride, batch}}),
+      span_of("mass", p->mass_width > 0 ? p->mass : nullptr, 4 * int64_t{p->mass_width},
+              {{4 * p->mass_stride_b, batch}, {4 * p->mass_stride_h, heads}}),
+      span_of("k_cache", p->k_cache, 2 * p->head_dim,
+              {{2 * p->k_stride_page, p->seqs.num_pages}, {2 * p->k_stride_t, p->seqs.page_size},
+               {2 * p->k_stride_h, heads}}),
+      span_of("v_cache", p->v_cache, 2 * p->head_dim,
+              {{2 * p->v_stride_page, p->seqs.num_pages}, {2 * p->v_stride_t, p->seqs.page_size},
+               {2 * p->v_stride_h, heads}})};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (spans_meet(written[i], written[j]))
+        return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: %s shares memory with %s", what, written[i].name,
+                    written[j].name);
+    for (int j = 0; j < 5; ++j)
+      if (!(i == 2 && j == 2) && spans_meet(written[i], other[j]))
+        return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: %s shares memory with %s", what, written[i].name,
+                    other[j].name);
+  }
   return IFA4_OK;
 }
 
