@@ -2032,6 +2032,12 @@ int ifa4_select_pages_launch(const IFA4SelectPagesParams* p, void* stream) {
       !rows_apart(p->num_selected, {{p->pages_stride_t, p->rows}, {p->pages_stride_h, p->kv_heads}}))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores or pages are misaligned, or strides of pages overlap",
                 what);
+  // a long row is read again while its choice is written
+  if (spans_meet(span_of("pages", p->pages, 4 * int64_t{p->num_selected},
+                         {{4 * p->pages_stride_t, p->rows}, {4 * p->pages_stride_h, p->kv_heads}}),
+                 span_of("scores", p->scores, 4 * int64_t{p->width},
+                         {{4 * p->scores_stride_t, p->rows}, {4 * p->scores_stride_h, p->kv_heads}})))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: pages share memory with scores", what);
   ifa4::SelectPagesKernelArgs a{};
   a.scores = p->scores;
   a.pages = p->pages;

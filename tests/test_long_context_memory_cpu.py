@@ -1,4 +1,4 @@
-"""Memory that the eviction refuses: outputs on top of inputs or of one another, caches that
+"""Memory that the eviction and the choice refuse: outputs on top of inputs or of one another, caches that
 share elements; against the sets of elements.  The C ABI refuses before any CUDA call; of what it
 accepts only the workspace's size is asked for, so the addresses are never used."""
 import ctypes
@@ -129,3 +129,12 @@ def test_outputs_next_to_something():
     wide = dict(mass_stride_b=256, mass_stride_h=128, mass_out_stride_b=256, mass_out_stride_h=128)
     assert _says(_evict(k, v, mass_out=(1 << 22) + 64 * 4, **wide)) is None
     assert "mass_out" in _says(_evict(k, v, mass_out=(1 << 22) + 63 * 4, **wide))
+
+
+def test_a_choice_on_top_of_its_scores():
+    p = _lib.SelectPagesParams()
+    p.scores, p.rows, p.kv_heads, p.width, p.num_selected = 1 << 20, 2, 2, 64, 8
+    p.scores_stride_t, p.scores_stride_h, p.pages_stride_t, p.pages_stride_h = 128, 64, 16, 8
+    for p.pages in (1 << 20, (1 << 20) + 1020, (1 << 20) - 92):
+        assert _lib.lib().ifa4_select_pages_launch(ctypes.byref(p), None) == INVALID
+        assert b"share memory" in _lib.lib().ifa4_last_error_string()
