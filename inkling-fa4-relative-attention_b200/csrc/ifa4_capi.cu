@@ -1786,6 +1786,10 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned rel", what);
   if (!(d->softmax_scale < INFINITY))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be finite", what);
+  if (!rows_apart(d->head_dim, {{d->out_stride_t, d->total_q}, {d->out_stride_h, d->n_heads}}) ||
+      (d->lse != nullptr &&
+       !rows_apart(1, {{d->lse_stride_t, d->total_q}, {d->lse_stride_h, d->n_heads}})))
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: strides of out or lse overlap", what);
   const int group = d->n_heads / d->kv_heads;
   const int64_t rows = d->total_q * d->kv_heads * ceil_div(group, 16);
   const int64_t tiles = ceil_div(static_cast<int64_t>(p->num_selected) * d->page_size, 64);
