@@ -590,7 +590,7 @@ typedef struct IFA4PageScoresParams {
   int32_t n_heads;
   int32_t kv_heads;
   int32_t head_dim;
-  int32_t rel_extent;
+  int32_t rel_extent;           /* 1 to 2^29                                               */
   int32_t window_left;
   int32_t max_seqlen_q;         /* grid-size hint; <= 0: total_q                           */
   int32_t first_pages;
@@ -661,7 +661,7 @@ typedef struct IFA4AttentionMassParams {
   int32_t n_heads;
   int32_t kv_heads;
   int32_t head_dim;
-  int32_t rel_extent;
+  int32_t rel_extent;           /* 1 to 2^29                                               */
   int32_t window_left;
   int32_t max_seqlen_q;         /* grid-size hints; <= 0: total_q, the mass's width        */
   int32_t max_seqlen_k;

@@ -1729,12 +1729,17 @@ int check_heads(const char* what, const P* p, int n_heads) {
   return IFA4_OK;
 }
 
+// The kernels add a distance to positions of up to 2^30 in 32 bits.
+constexpr int kMostDistances = 1 << 29;
+
 // Queries with their bias.
 template <class P>
 int check_queries(const char* what, const P* p) {
   if (p->total_q < 0) return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: negative total_q", what);
   if (p->rel_extent <= 0)
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: rel_extent must be > 0", what);
+  if (p->rel_extent > kMostDistances)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: rel_extent > 2^29", what);
   if (!(p->softmax_scale > 0.f && p->softmax_scale < INFINITY))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0 and finite", what);
   if (p->rel_stride_t < 0 || p->rel_stride_h < 0)
@@ -1786,6 +1791,8 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: misaligned rel", what);
   if (!(d->softmax_scale < INFINITY))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be finite", what);
+  if (d->rel_extent > kMostDistances)
+    return fail(IFA4_ERR_UNSUPPORTED, "%s: rel_extent > 2^29", what);
   if (!rows_apart(d->head_dim, {{d->out_stride_t, d->total_q}, {d->out_stride_h, d->n_heads}}) ||
       (d->lse != nullptr &&
        !rows_apart(1, {{d->lse_stride_t, d->total_q}, {d->lse_stride_h, d->n_heads}})))

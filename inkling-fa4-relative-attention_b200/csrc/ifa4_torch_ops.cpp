@@ -601,7 +601,8 @@ bool plain_queries(const at::Tensor& q, const at::Tensor& rel, int64_t kv_heads,
          rel.scalar_type() == at::kBFloat16 && rel.device() == q.device() &&
          rel.size(0) == q.size(0) && rel.size(1) == q.size(1) && rel.stride(2) == 1 &&
          rel.stride(0) >= 0 && rel.stride(1) >= 0 && rel_extent >= 1 &&
-         rel_extent <= rel.size(2) && softmax_scale > 0 && softmax_scale < 1e38;
+         rel_extent <= rel.size(2) && rel_extent <= (1 << 29) && softmax_scale > 0 &&
+         softmax_scale < 1e38;
 }
 bool plain_int(int64_t x) { return x >= -1 && x <= 0x7fffffff; }
 

@@ -11,6 +11,7 @@ from . import _lib, _ops
 
 HEAD_DIM = _ops.HEAD_DIM
 MOST = 1 << 26  # entries of a table row or of a choice
+MOST_DISTANCES = 1 << 29
 
 
 def tensor(name, nm, t, device, dtype, dims):
@@ -58,6 +59,11 @@ def page_bounds(name, t, kv_heads, num_pages, device):
         raise ValueError(f"{name}: minima and maxima of a page and head must be contiguous in bounds")
 
 
+def distances(name, rel_extent):
+    if rel_extent > MOST_DISTANCES:
+        raise ValueError(f"{name}: rel_extent {rel_extent} must be at most 2^29")
+
+
 def sequences(name, device, cu_q, cu_k, block_table):
     """Checked offsets and table as the kernels read them."""
     for nm, cu in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
@@ -85,6 +91,7 @@ def queries(name, q, rel_logits, kv_heads, rel_extent, softmax_scale, device):
     if rel_extent <= 0 or rel_logits.shape[2] < rel_extent:
         raise ValueError(f"{name}: rel_extent {rel_extent} out of range for rel_logits "
                          f"{tuple(rel_logits.shape)}")
+    distances(name, rel_extent)
     scale = 1.0 / HEAD_DIM if softmax_scale is None else float(softmax_scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"{name}: softmax_scale must be > 0")

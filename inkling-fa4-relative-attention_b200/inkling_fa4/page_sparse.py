@@ -230,6 +230,7 @@ def _checked_decode(q, k, v, rel_logits, cu_q, cu_k, max_seqlen_k, rel_extent, p
     _paged.cache(name, "v", v, k.device)
     cu_q, cu_k, block_table = _paged.sequences(name, k.device, cu_q, cu_k, block_table)
     given = (out, lse)
+    _paged.distances(name, int(rel_extent))
     q, k, v, rel, out, n_heads, kv_heads, rel_extent, window_left, scale = _ops._prepare(
         name, q, k, v, rel_logits, cu_q, cu_k, rel_extent, True, window_size, n_heads, kv_heads,
         head_dim, softmax_scale, "bottom_right", out, block_table)
