@@ -1938,7 +1938,10 @@ int ifa4_page_bounds_launch(const IFA4PageBoundsParams* p, void* stream) {
   if (!rows_apart(2 * p->head_dim, {{p->bounds_stride_page, p->seqs.num_pages},
                                     {p->bounds_stride_h, p->kv_heads}}))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: strides of bounds overlap", what);
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
   ifa4::PageBoundsKernelArgs a{};
+  a.status = status;
   a.s = paged_seqs(&p->seqs);
   a.k_cache = static_cast<const uint16_t*>(p->k_cache);
   a.bounds = static_cast<uint16_t*>(p->bounds);
@@ -1984,7 +1987,10 @@ int ifa4_page_scores_launch(const IFA4PageScoresParams* p, void* stream) {
       !rows_apart(p->seqs.table_width, {{p->scores_stride_t, p->total_q},
                                         {p->scores_stride_h, p->kv_heads}}))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: scores are misaligned, or their strides overlap", what);
+  int* status = nullptr;
+  if ((rc = device_status_ptr(&status))) return rc;
   ifa4::PageScoresKernelArgs a{};
+  a.status = status;
   a.s = paged_seqs(&p->seqs);
   a.q = static_cast<const uint16_t*>(p->q);
   a.bounds = static_cast<const uint16_t*>(p->bounds);
@@ -2049,7 +2055,11 @@ int ifa4_select_pages_launch(const IFA4SelectPagesParams* p, void* stream) {
                  span_of("scores", p->scores, 4 * int64_t{p->width},
                          {{4 * p->scores_stride_t, p->rows}, {4 * p->scores_stride_h, p->kv_heads}})))
     return fail(IFA4_ERR_INVALID_ARGUMENT, "%s: pages share memory with scores", what);
+  int* status = nullptr;
+  const int rc = device_status_ptr(&status);
+  if (rc) return rc;
   ifa4::SelectPagesKernelArgs a{};
+  a.status = status;
   a.scores = p->scores;
   a.pages = p->pages;
   a.sc_st = p->scores_stride_t;

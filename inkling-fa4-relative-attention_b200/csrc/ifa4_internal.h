@@ -308,6 +308,7 @@ struct PageBoundsKernelArgs {
   uint16_t* bounds;          // [pages, kv_heads, 2, 128]
   long long k_sp, k_st, k_sh, b_sp, b_sh;
   int kv_heads;
+  int* status;
 };
 // grid.y: sequences; the blocks of grid.x stride over a sequence's (page, head) units.
 constexpr int kPageBoundsWarps = 8;
@@ -327,6 +328,7 @@ struct PageScoresKernelArgs {
   int row_blocks;            // blocks of rows of a sequence in the grid (strided over)
   int block_pages;           // pages of a block: 32, 64, 128 or 256
   float scale;
+  int* status;
 };
 cudaError_t launch_page_scores_sm100(const PageScoresKernelArgs& args, cudaStream_t stream);
 
@@ -336,6 +338,7 @@ struct SelectPagesKernelArgs {
   long long sc_st, sc_sh, pg_st, pg_sh;
   long long rows;
   int kv_heads, width, count;
+  int* status;
 };
 cudaError_t launch_select_pages_sm100(const SelectPagesKernelArgs& args, cudaStream_t stream);
 

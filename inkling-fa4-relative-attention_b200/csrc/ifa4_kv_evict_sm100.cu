@@ -195,7 +195,9 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
     tmem_alloc(&bars->tmem_base, L::kTmemCols);
     tmem_relinquish();
   }
-  const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
+  const int q0 = __ldg(a.s.cu_q + b);
+  int n_q = __ldg(a.s.cu_q + b + 1) - q0;
+  if (!IFA4_DBG_CHECK(a.status, n_q <= 0 || (q0 >= 0 && n_q <= a.total_q - q0))) n_q = 0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
   const int n_out = min(n_k, a.mass_width);  // keys with a place
   const int n_pairs = ((a.accumulate ? n_out : a.mass_width) + 2 * kKeys - 1) / (2 * kKeys);
@@ -242,7 +244,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
       if (!(ok = mbar_wait_warp(&bars->k_empty[ks], ((nk / L::kKStages) & 1) ^ 1, ab))) break;
       if (lane == 0) mbar_arrive_expect_tx(&bars->k_full[ks], 2 * kKTile);
       __syncwarp();
-      if (lane < units) {
+      if (lane < units && IFA4_DBG_CHECK(a.status, page <= a.s.num_pages && (lane + 1) * box <= 2 * kKeys &&
+                                                       (key & page_mask) + box <= page_mask + 1)) {
         const int row = lane * box;  // of the pair
         uint8_t* dst = smem + ks * 2 * kKTile + (row / kKeys) * kKTile + (row % kKeys) * 128;
 #pragma unroll
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int r = lane + 32 * i;
-          if (r < kN) {
+          if (r < kN && IFA4_DBG_CHECK(a.status, qt * tokens < n_q)) {
             const float neg = l[i] == -INFINITY ? -INFINITY : -l[i];  // -inf for +inf, too
             sums[qs].nlse[r] = scaled_lse(neg);
             sums[qs].neg[r] = neg;
@@ -449,7 +452,10 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
           if (p_lo - (tile0 + kKeys - 1) >= a.rel_extent || p_hi < tile0) return;
           if (c0 + kC <= c_end && p_hi - tile0 < a.rel_extent && p_lo >= tile0 + kKeys - 1) {
 #pragma unroll
-            for (int i = 0; i < kC; ++i) load_now(x[i], rel_key + cols.rel[c0 + i]);  // all have one
+            for (int i = 0; i < kC; ++i)  // all have one
+              if (IFA4_DBG_CHECK(a.status, static_cast<unsigned>(dk + cols.token[c0 + i]) <
+                                               static_cast<unsigned>(a.rel_extent)))
+                load_now(x[i], rel_key + cols.rel[c0 + i]);
           } else {
 #pragma unroll
             for (int i = 0; i < kC; ++i) {
@@ -553,7 +559,8 @@ __global__ void __launch_bounds__(Layout<kN>::kThreads, 1)
         if (c_begin == 0) sum += *other;
         ++pairs;
       }
-      if (ok && c_begin == 0 && key < a.mass_width && IFA4_DBG_CHECK(a.status, b < a.s.batch)) {
+      if (ok && c_begin == 0 && key < a.mass_width &&
+          IFA4_DBG_CHECK(a.status, key >= 0 && (a.accumulate == 0 || n_pairs * 2 * kKeys > key))) {
         float* dst = a.mass + static_cast<long long>(b) * a.mass_sb +
                      static_cast<long long>(kvh) * a.mass_sh + key;
         if (!a.accumulate) *dst = key < n_out ? sum : 0.f;
@@ -626,6 +633,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     x.n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
     x.q0 = __ldg(a.s.cu_q + b);
     x.n_q = __ldg(a.s.cu_q + b + 1) - x.q0;
+    if (!IFA4_DBG_CHECK(a.status, x.n_q <= 0 || (x.q0 >= 0 && x.n_q <= a.total_q - x.q0))) x.n_q = 0;
     x.n_out = min(x.n_k, a.mass_width);
     x.first = first_key(x.n_k - x.n_q, a.window_left);
     return x;
@@ -653,7 +661,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
       return page;
     };
     const auto load = [&](int k0, int page, uint32_t st) {
-      if (lane == 0 && visible(k0)) {
+      if (lane == 0 && visible(k0) && IFA4_DBG_CHECK(a.status, page <= a.s.num_pages && (k0 & 15) == 0)) {
         mbar_arrive_expect_tx(&full[st], kStreamStage);
   #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
@@ -792,7 +800,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
           for (int e = 0; e < 2; ++e) {
             const int key = k0 + 8 * g + 2 * qd + e;
             const float y = g == 0 ? sum[e] : sum[2 + e];
-            if (key < end && IFA4_DBG_CHECK(a.status, key < a.mass_width)) mass[key] = y;
+            if (key < end && IFA4_DBG_CHECK(a.status, key >= key_lo && key < a.mass_width)) mass[key] = y;
           }
         }
       }
@@ -893,7 +901,9 @@ __global__ void __launch_bounds__(kSelectThreads)
   float* mass_out = a.mass_out + static_cast<long long>(b) * a.mo_sb +
                     static_cast<long long>(g) * a.mo_sh;
   int32_t* kept = a.kept + (static_cast<long long>(b) * a.kv_heads + g) * a.budget;
-  const auto keep = [&](int place, int i) { kept[place] = i; };
+  const auto keep = [&](int place, int i) {
+    if (IFA4_DBG_CHECK(a.status, place >= 0 && place <= i && place < a.budget && i < n)) kept[place] = i;
+  };
   // a key from mass_width on has the mass 0; -inf ranks below every other mass, but can be kept
   const auto rank = [&](int i, float x) {
     if (i < a.first || i >= n - a.recent) return kAlways;
@@ -903,15 +913,16 @@ __global__ void __launch_bounds__(kSelectThreads)
   if (n <= a.budget) {
     for (int i = threadIdx.x; i < n; i += kSelectThreads) kept[i] = i;
   } else if (const int there = min(n, a.mass_width); n <= kSelectThreads * 4) {
-    stay = select_largest<kSelectThreads, 4>(sm, mass, there, n, a.budget, rank, keep);
+    stay = select_largest<kSelectThreads, 4>(sm, a.status, mass, there, n, a.budget, rank, keep);
   } else if (n <= kSelectThreads * 12) {
-    stay = select_largest<kSelectThreads, 12>(sm, mass, there, n, a.budget, rank, keep);
+    stay = select_largest<kSelectThreads, 12>(sm, a.status, mass, there, n, a.budget, rank, keep);
   } else if (n <= kSelectThreads * 32) {
-    stay = select_largest<kSelectThreads, 32>(sm, mass, there, n, a.budget, rank, keep);
+    stay = select_largest<kSelectThreads, 32>(sm, a.status, mass, there, n, a.budget, rank, keep);
   } else {
     stay = select_largest_long<kSelectThreads>(
-        sm, n, a.budget, [&](int i) { return rank(i, i < there ? __ldg(mass + i) : 0.f); }, keep);
+        sm, a.status, n, a.budget, [&](int i) { return rank(i, i < there ? __ldg(mass + i) : 0.f); }, keep);
   }
+  if (!IFA4_DBG_CHECK(a.status, stay >= 0 && stay <= a.budget)) stay = 0;
   for (int i = stay + threadIdx.x; i < a.budget; i += kSelectThreads) kept[i] = -1;
   __syncthreads();
   // their masses: places are read back so that the loads are independent of one another
@@ -926,7 +937,7 @@ __global__ void __launch_bounds__(kSelectThreads)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       x[j] = 0.f;
-      load_if(x[j], mass + at[j], at[j] < a.mass_width);
+      load_if(x[j], mass + at[j], at[j] < a.mass_width && IFA4_DBG_CHECK(a.status, at[j] >= 0));
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -985,7 +996,8 @@ __global__ void __launch_bounds__(kMoveThreads)
     for (int i = 0; i < kTurns; ++i) {
       const int place = c * kMoveRows + sub + i * kStep;
       page_to[i] = page_from[i] = -1;
-      if (from[i] != place) {
+      if (from[i] != place && IFA4_DBG_CHECK(a.status, from[i] > place && from[i] < n && place < a.budget &&
+                                                           b < a.s.batch && c < a.stretches)) {
         page_to[i] = page_at(a.s, table, place >> a.s.page_shift);
         page_from[i] = page_at(a.s, table, from[i] >> a.s.page_shift);
       }
@@ -1003,6 +1015,10 @@ __global__ void __launch_bounds__(kMoveThreads)
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
       if (page_to[i] < 0) continue;
+      if (!IFA4_DBG_CHECK(a.status, page_to[i] < a.s.num_pages && page_from[i] < a.s.num_pages)) {
+        page_to[i] = -1;
+        continue;
+      }
       any = true;
       uint8_t* k = rows + (sub + i * kStep) * 512 + part * 16;
       if (page_from[i] >= 0) {

@@ -63,6 +63,8 @@ __global__ void __launch_bounds__(kPageBoundsWarps * 32)
     const int page = page_at(a.s, row, c);
     if (page < 0) continue;
     const int keys = min(ps, n_k - (c << a.s.page_shift));
+    if (!IFA4_DBG_CHECK(a.status, page < a.s.num_pages && h < a.kv_heads && keys >= 1 && keys <= ps))
+      continue;
     const uint16_t* src = a.k_cache + static_cast<long long>(page) * a.k_sp +
                           static_cast<long long>(h) * a.k_sh + part * 8;
     uint4 lo, hi;
@@ -164,6 +166,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
   }
   const int q0 = __ldg(a.s.cu_q + b), n_q = __ldg(a.s.cu_q + b + 1) - q0;
   const int n_k = __ldg(a.s.cu_k + b + 1) - __ldg(a.s.cu_k + b);
+  if (!IFA4_DBG_CHECK(a.status, n_q <= 0 || (q0 >= 0 && n_q <= a.total_q - q0))) return;
   const int group = kHeads > 0 ? kHeads : a.group;
   const int hb = min(group, 16);            // heads of a row block
   const int tokens = 16 / hb;               // and tokens
@@ -200,7 +203,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
         const uint32_t dst = ring_lane + st * kScoreStage;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int p = __shfl_sync(0xffffffffu, page, i);
+          int p = __shfl_sync(0xffffffffu, page, i);
+          if (!IFA4_DBG_CHECK(a.status, p < a.s.num_pages)) p = -1;
           cp_async16_or_zeros(dst + i * kScorePitch,
                               bounds_lane + static_cast<uint64_t>(static_cast<uint32_t>(max(p, 0))) *
                                                 page_bytes,
@@ -267,7 +271,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
           for (int c = c_near + static_cast<int>(threadIdx.x); c <= c_end; c += kScoreWarps * 32) {
             int d1 = p - (c << shift);  // the furthest key of the page
             if (a.window_left >= 0) d1 = min(d1, a.window_left);
-            bias_rank[row][c - page0] = d1 >= a.rel_extent ? kRankZero : 0u;
+            if (IFA4_DBG_CHECK(a.status, c >= page0 && c - page0 < kScorePages && row < 16))
+              bias_rank[row][c - page0] = d1 >= a.rel_extent ? kRankZero : 0u;
           }
         }
         __syncthreads();
@@ -287,13 +292,16 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
           uint32_t most = 0u;
 #pragma unroll
           for (int j = 0; j < 16; ++j) most = max(most, rank_of(bf16_bits_to_float(v[j])));
-          if (most != 0u) atomicMax(&bias_rank[row][(key0 >> shift) - page0], most);
+          if (most != 0u && IFA4_DBG_CHECK(a.status, static_cast<unsigned>((key0 >> shift) - page0) <
+                                                         static_cast<unsigned>(page1 - page0)))
+            atomicMax(&bias_rank[row][(key0 >> shift) - page0], most);
         }
         __syncthreads();
       }
       // ---- scores
       // stores the largest over the heads of a token, of all pages that the block has
       const auto store = [&](int tok, int c, float y) {
+        if (!IFA4_DBG_CHECK(a.status, q0 + tok0 + tok < a.total_q && c < width)) return;
         float* dst = a.scores + (q0 + tok0 + tok) * a.sc_st + kvh * a.sc_sh + c;
         if (h0 > 0) y = max_nan(*dst, y);  // of the heads before, by the same thread
         if (h0 + 16 >= group && p0 + tok >= 0) {
@@ -365,7 +373,9 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
                 const int d0 = max(0, pos[r] - ((c << shift) + ((1 << shift) - 1)));
                 if (a.window_left < 0 || d0 <= a.window_left) {
                   x = y[2 * r + e];
-                  if (d0 < a.rel_extent) x += value_of(bias_rank[g + 8 * r][c - page0]);
+                  if (d0 < a.rel_extent &&
+                      IFA4_DBG_CHECK(a.status, (c << shift) + ((1 << shift) - 1) >= near))
+                    x += value_of(bias_rank[g + 8 * r][c - page0]);
                 }
               }
               y[2 * r + e] = x;
@@ -388,7 +398,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 4)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             if (tok_out[r] < 0) continue;
-            if (inside) {
+            if (inside && IFA4_DBG_CHECK(a.status, q0 + tok0 + tok_out[r] < a.total_q &&
+                                                       c0 + 2 * qd + 1 < width)) {
               out[r][c0] = y[2 * r];
               out[r][c0 + 1] = y[2 * r + 1];
             } else {
@@ -431,13 +442,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : kThreads == 25
   for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) {
     const float* src = a.scores + t * a.sc_st + g * a.sc_sh;
     int32_t* dst = a.pages + t * a.pg_st + g * a.pg_sh;
-    const auto emit = [&](int place, int i) { dst[place] = i; };
+    const auto emit = [&](int place, int i) {
+      if (IFA4_DBG_CHECK(a.status, place >= 0 && place < a.count && i >= 0 && i < a.width)) dst[place] = i;
+    };
     int n;
     if constexpr (kItems > 0)
-      n = select_largest<kThreads, kItems>(sm, src, a.width, a.width, a.count,
+      n = select_largest<kThreads, kItems>(sm, a.status, src, a.width, a.width, a.count,
                                            [](int, float x) { return rank_of(x); }, emit);
     else
-      n = select_largest_long<kThreads>(sm, a.width, a.count,
+      n = select_largest_long<kThreads>(sm, a.status, a.width, a.count,
                                         [&](int i) { return rank_of(__ldg(src + i)); }, emit);
     for (int i = n + threadIdx.x; i < a.count; i += kThreads) dst[i] = -1;
   }
@@ -579,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const long long vk = static_cast<long long>(tile) * kTileKeys + lane * box;
       const int e = static_cast<int>(vk >> a.s.page_shift);
       int page = -2;
-      if (lane < units && e <= last) {
+      if (lane < units && e <= last && IFA4_DBG_CHECK(a.status, e >= 0 && e < a.num_selected)) {
         const int c = __ldg(list + e);
         if (c >= c_lo && c <= c_hi) {
           const int key0 = (c << a.s.page_shift) + (static_cast<int>(vk) & page_mask);
@@ -600,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
       if (lane == 0) mbar_arrive_expect_tx(&bars->full[st], loads * box * 512u);
       __syncwarp();
-      if (page >= 0) {
+      if (page >= 0 && IFA4_DBG_CHECK(a.status, page <= a.s.num_pages && (lane + 1) * box <= kTileKeys)) {
         uint8_t* base = smem + st * kStageBytes + lane * box * 128;
         const int in_page = static_cast<int>(static_cast<long long>(tile) * kTileKeys + lane * box) &
                             page_mask;
@@ -645,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     auto entry = [&](int tile) {
       const long long vk = static_cast<long long>(tile) * kTileKeys + wrow;
       const int e = static_cast<int>(vk >> a.s.page_shift);
-      return e <= last ? __ldg(list + e) : -1;
+      return e <= last && IFA4_DBG_CHECK(a.status, e >= 0 && e < a.num_selected) ? __ldg(list + e) : -1;
     };
     uint32_t n = 0;
     int c = t_lo < t_hi ? entry(t_lo) : -1;

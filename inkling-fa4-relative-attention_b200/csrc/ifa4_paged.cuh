@@ -116,8 +116,8 @@ __device__ __forceinline__ uint32_t block_exclusive_sum(uint32_t v, uint32_t* wa
 // For rows of any length: three passes over digits of 11, 11 and 10 bits find the key of the border, one
 // more writes what is above it; each reads the row again, which the caches hold.
 template <int kThreads, class Key, class Emit>
-__device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int n, int count, Key key,
-                                              Emit emit) {
+__device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int* status, int n, int count,
+                                                   Key key, Emit emit) {
   const int tid = threadIdx.x;
   uint32_t need = static_cast<uint32_t>(count), prefix = 0u, known = 0u;
   bool all = false, bin_whole = false;
@@ -147,7 +147,7 @@ __device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int
     if (above < need && need <= above + mine) {  // exactly one thread
       uint32_t sum = above;
       int j = 0;
-      while (sum + sm.hist[top - j] < need) sum += sm.hist[top - j++];
+      while (IFA4_DBG_CHECK(status, j < per) && sum + sm.hist[top - j] < need) sum += sm.hist[top - j++];
       sm.digit = static_cast<uint32_t>(top - j);
       sm.above = sum;
       sm.in_bin = sm.hist[top - j];
@@ -206,8 +206,8 @@ __device__ __forceinline__ int select_largest_long(SelectSmem<kThreads>& sm, int
 // elements is ranked directly; a larger one is divided again.
 // The element i is values[i], or -inf from `there` on; key(i, value) ranks it.
 template <int kThreads, int kItems, class Key, class Emit>
-__device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const float* values, int there,
-                                              int n, int count, Key key, Emit emit) {
+__device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, int* status, const float* values,
+                                              int there, int n, int count, Key key, Emit emit) {
   static_assert(kThreads >= kCandidates, "one thread a candidate");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int base = warp * 32 * kItems + lane;
@@ -266,18 +266,25 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
       __syncthreads();
     }
     const bool values_binned = first && scale > 0.f;
+    const auto add = [&](uint32_t bin) {
+      if (IFA4_DBG_CHECK(status, bin < kSelectBins)) atomicAdd(&sm.hist[bin], 1u);
+    };
+    const auto candidate = [&](uint32_t key) {
+      const uint32_t at = atomicAdd(&sm.found, 1u);
+      if (IFA4_DBG_CHECK(status, at < kCandidates)) sm.candidate[at] = key;
+    };
     if (values_binned) {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
-        if (u[j] != 0u) atomicAdd(&sm.hist[value_bin(u[j])], 1u);
+        if (u[j] != 0u) add(value_bin(u[j]));
     } else if (first) {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
-        if (u[j] != 0u) atomicAdd(&sm.hist[u[j] >= kTop ? kSelectBins - 1 : (u[j] - lo) >> shift], 1u);
+        if (u[j] != 0u) add(u[j] >= kTop ? kSelectBins - 1 : (u[j] - lo) >> shift);
     } else {
 #pragma unroll
       for (int j = 0; j < kItems; ++j)
-        if (u[j] >= lo && u[j] <= hi) atomicAdd(&sm.hist[(u[j] - lo) >> shift], 1u);
+        if (u[j] >= lo && u[j] <= hi) add((u[j] - lo) >> shift);
     }
     __syncthreads();
     // thread 0 has the highest bins
@@ -295,7 +302,8 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
     if (above < need && need <= above + mine) {  // exactly one thread
       uint32_t sum = above;
       int j = 0;
-      while (sum + sm.hist[high_bin - j] < need) sum += sm.hist[high_bin - j++];
+      while (IFA4_DBG_CHECK(status, j < kPer) && sum + sm.hist[high_bin - j] < need)
+        sum += sm.hist[high_bin - j++];
       sm.digit = static_cast<uint32_t>(high_bin - j);
       sm.above = sum;
       sm.in_bin = sm.hist[high_bin - j];
@@ -320,7 +328,7 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
         if (u[j] - from <= to - from && u[j] != 0u && u[j] < kTop && value_bin(u[j]) == digit) {
           low = min(low, u[j]);
           high = max(high, u[j]);
-          if (in_bin <= kCandidates) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
+          if (in_bin <= kCandidates) candidate(u[j]);
         }
       low = __reduce_min_sync(0xffffffffu, low);
       high = __reduce_max_sync(0xffffffffu, high);
@@ -348,7 +356,7 @@ __device__ __forceinline__ int select_largest(SelectSmem<kThreads>& sm, const fl
       if (!values_binned || digit == kSelectBins - 1) {
 #pragma unroll
         for (int j = 0; j < kItems; ++j)
-          if (u[j] >= lo && u[j] <= hi) sm.candidate[atomicAdd(&sm.found, 1u)] = u[j];
+          if (u[j] >= lo && u[j] <= hi) candidate(u[j]);
         __syncthreads();
       }
       if (tid < static_cast<int>(in_bin)) {
