@@ -718,6 +718,10 @@ int ifa4_kv_evict_launch(const IFA4KvEvictParams* params, void* workspace, size_
  * abandon their waits too (that is how one failure stops the others). */
 int ifa4_selftest_bounded_wait(int64_t timeout_ns, void* stream);
 
+/* The same for the wait of an eviction's blocks on one another: a flag that nothing sets, 32 threads.
+ * Afterwards the status word holds exactly bit 7 (value 128). */
+int ifa4_selftest_evict_wait(int64_t timeout_ns, void* stream);
+
 /* Measurement hook (no counterpart in the reference): launches on `stream` one read-only pass
  * over `bytes` bytes at `buf` (16-byte aligned, bytes a multiple of 16) with 16-byte
  * non-coherent loads, four in flight per thread, 4 CTAs of 512 threads per SM.  Timing it gives
@@ -730,8 +734,9 @@ int ifa4_measure_read_stream(const void* buf, size_t bytes, uint32_t* sink, void
  * calling thread until the stream has reached this point.  Nonzero means a kernel gave up on
  * a bounded wait (a bug, never expected): bit 0 prefill, bit 1 decode, bit 2 backward, bits 3-4
  * ifa4_selftest_bounded_wait, bit 5 rel_logits producer, bit 6 (debug builds compiled with
- * -DIFA4_DEBUG only) an index range check failed and the access was skipped, bit 7 eviction.  Test
- * hook; the reference has no counterpart. */
+ * -DIFA4_DEBUG only) an index range check failed and the access was skipped, bit 7 eviction.  What a
+ * call wrote that set a bit is not valid; an eviction that set bit 7 has moved some of its keys and not
+ * others, so its caches and outputs are to be given up.  Test hook; the reference has no counterpart. */
 int ifa4_read_device_status(void* stream, int32_t clear, int32_t* status_out);
 
 /* Name of the sm_100a prefill tile configuration `tile_config` resolves to (the counterpart

@@ -2436,6 +2436,19 @@ int ifa4_selftest_bounded_wait(int64_t timeout_ns, void* stream) {
   return IFA4_OK;
 }
 
+int ifa4_selftest_evict_wait(int64_t timeout_ns, void* stream) {
+  g_last_error[0] = '\0';
+  if (timeout_ns <= 0 || timeout_ns > 1000000000LL)
+    return fail(IFA4_ERR_INVALID_ARGUMENT, "selftest: timeout_ns must be in (0, 1e9]");
+  int* status = nullptr;
+  int rc = device_status_ptr(&status);
+  if (rc) return rc;
+  cudaError_t e = ifa4::launch_evict_wait_selftest_sm100(
+      status, static_cast<unsigned long long>(timeout_ns), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "selftest launch");
+  return IFA4_OK;
+}
+
 int ifa4_measure_read_stream(const void* buf, size_t bytes, uint32_t* sink, void* stream) {
   g_last_error[0] = '\0';
   if (buf == nullptr || sink == nullptr || bytes == 0)

@@ -408,6 +408,9 @@ struct KvEvictKernelArgs {
 constexpr int kEvictRows = 64;  // kept keys that a block moves
 // `blocks`: most blocks of the move.
 cudaError_t launch_kv_evict_sm100(const KvEvictKernelArgs& args, int blocks, cudaStream_t stream);
+// The move's wait on a flag that nothing sets.
+cudaError_t launch_evict_wait_selftest_sm100(int* status, unsigned long long timeout_ns,
+                                             cudaStream_t stream);
 
 struct BackwardKernelArgs {
   const uint16_t* rel;       // bf16 bits

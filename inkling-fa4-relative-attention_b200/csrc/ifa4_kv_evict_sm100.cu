@@ -967,6 +967,24 @@ __device__ __forceinline__ int load_acquire(const int* p) {
   return v;
 }
 
+// Waits until *flag is set, up to timeout_ns after t0; then the status bit is set and it returns false.
+__device__ __forceinline__ bool wait_flag(const int* flag, int* status, unsigned long long t0,
+                                          unsigned long long timeout_ns = kWaitTimeoutNs) {
+  for (uint32_t it = 1; load_acquire(flag) == 0; ++it) {
+    if ((it & 255u) == 0 && globaltimer_ns() - t0 > timeout_ns) {
+      atomicOr(status, kStatusEvictTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+// The wait on a flag that nothing sets.
+__device__ int g_never_set = 0;
+__global__ void __launch_bounds__(32) wait_selftest_kernel(int* status, unsigned long long timeout_ns) {
+  wait_flag(&g_never_set, status, globaltimer_ns(), timeout_ns);
+}
+
 __global__ void __launch_bounds__(kMoveThreads)
     kv_evict_move_kernel(const __grid_constant__ KvEvictKernelArgs a) {
   __shared__ __align__(16) uint8_t rows[kMoveSmem];
@@ -1052,13 +1070,7 @@ __global__ void __launch_bounds__(kMoveThreads)
       const unsigned long long t0 = globaltimer_ns();
       for (int e = this_c - 1 - static_cast<int>(threadIdx.x); e >= 0 && ok; e -= kMoveThreads) {
         if (kept[e * kMoveRows + kMoveRows - 1] < base) break;  // and so are all before
-        for (uint32_t it = 1; load_acquire(flags + e) == 0; ++it) {
-          if ((it & 255u) == 0 && globaltimer_ns() - t0 > kWaitTimeoutNs) {
-            atomicOr(a.status, kStatusEvictTimeout);
-            ok = false;
-            break;
-          }
-        }
+        ok = wait_flag(flags + e, a.status, t0);
       }
       if (__syncthreads_or(!ok)) return;
 #pragma unroll
@@ -1080,6 +1092,12 @@ __global__ void __launch_bounds__(kMoveThreads)
 }  // namespace evict
 
 static_assert(evict::kMoveRows == kEvictRows, "stretches");
+
+cudaError_t launch_evict_wait_selftest_sm100(int* status, unsigned long long timeout_ns,
+                                             cudaStream_t stream) {
+  evict::wait_selftest_kernel<<<1, 32, 0, stream>>>(status, timeout_ns);
+  return cudaGetLastError();
+}
 
 int attention_mass_tile_rows(long long rows, int group) {
   int n = 32;

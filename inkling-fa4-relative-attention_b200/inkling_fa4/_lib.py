@@ -60,6 +60,7 @@ EXPORTED_SYMBOLS = (
     "ifa4_kv_evict_workspace_size",
     "ifa4_read_device_status",
     "ifa4_selftest_bounded_wait",
+    "ifa4_selftest_evict_wait",
     "ifa4_measure_read_stream",
     "ifa4_prefill_tile_config_name",
     "ifa4_last_error_string",
@@ -352,8 +353,9 @@ def lib() -> ctypes.CDLL:
                          ("attention_mass", AttentionMassParams)):
         launch = getattr(L, f"ifa4_{name}_launch")
         launch.argtypes, launch.restype = [ctypes.POINTER(params), vp], ctypes.c_int
-    L.ifa4_selftest_bounded_wait.argtypes = [ctypes.c_int64, vp]
-    L.ifa4_selftest_bounded_wait.restype = ctypes.c_int
+    for name in ("bounded_wait", "evict_wait"):
+        test = getattr(L, f"ifa4_selftest_{name}")
+        test.argtypes, test.restype = [ctypes.c_int64, vp], ctypes.c_int
     L.ifa4_measure_read_stream.argtypes = [vp, sz, vp, vp]
     L.ifa4_measure_read_stream.restype = ctypes.c_int
     L.ifa4_read_device_status.argtypes = [vp, i32, ctypes.POINTER(i32)]
