@@ -621,8 +621,8 @@ int ifa4_select_pages_launch(const IFA4SelectPagesParams* params, void* stream);
  * pages[t, g, :] of its sequence (indices into its table row, in any order; an entry that is no index
  * of a page with a visible key adds nothing, one that is listed twice counts twice).  Any number of
  * rows a sequence.  A row without keys is 0 with the lse -inf; a logit that is NaN or +inf makes its
- * row NaN.  decode.block_table and the seqs fields that repeat there have to agree (batch,
- * cu_seqlens, page_size, num_pages come from decode); chunk_len is not used.  Rows of no sequence
+ * row NaN.  The sequences and the cache are those of decode (cu_seqlens, batch, block_table, page_size,
+ * num_pages), to which table_width adds the entries of a table row; decode.chunk_len is not used.  Rows of no sequence
  * get 0 (lse -inf) where zero_padding is set and stay as they are otherwise.  A workspace is needed
  * for more than eight splits of a row only (the size is 0 otherwise); it must be 16-byte aligned and
  * not shared by calls that may run at the same time. */

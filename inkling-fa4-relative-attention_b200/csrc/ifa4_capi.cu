@@ -1808,8 +1808,8 @@ int decode_pages_plan(const IFA4DecodePagesParams* p, int* splits, size_t* bytes
     // An estimate in ns, from measured times: two CTAs an SM share the HBM bandwidth (5 ns a tile of 64
     // keys and CTA), a CTA alone takes 830 ns a tile; a round of CTAs costs 5 us besides, the merge
     // 0.5 us and 0.15 us a split, 2.5 us more through a workspace.  (64 rows x 8 heads of 256 pages of
-    // 16: 177 us whole, 196 in two; 48 of 128 pages: 92 and 82; 16 of 64 pages: 22.2 and 17.5; one:
-    // 21.2 whole, 7.7 in eight, 11.1 in sixteen.)
+    // 16, captured calls on changing inputs: 180 us whole, 200 in two; 48 of 128 pages: 95 and 85; 16 of
+    // 64 pages: 25.3 and 20.2; one: 23.3 whole, 12.0 in four, 10.0 in eight, 13.9 in sixteen.)
     const int64_t slots = 2 * sms;
     int64_t best = 0;
     for (int s = 1; s <= 64 && s <= (tiles > 0 ? tiles : 1); ++s) {
@@ -2196,7 +2196,6 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
   a.mass_sb = p->mass_stride_b;
   a.mass_sh = p->mass_stride_h;
   a.total_q = p->total_q;
-  a.n_heads = p->n_heads;
   a.kv_heads = p->kv_heads;
   a.group = group;
   a.rel_extent = p->rel_extent;
@@ -2208,12 +2207,8 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
   a.scale_log2 = static_cast<float>(p->softmax_scale * 1.4426950408889634);
   a.status = status;
   a.q = static_cast<const uint16_t*>(p->q);
-  a.k_cache = static_cast<const uint16_t*>(p->k_cache);
   a.q_st = p->q_stride_t;
   a.q_sh = p->q_stride_h;
-  a.k_sp = p->k_stride_page;
-  a.k_st = p->k_stride_t;
-  a.k_sh = p->k_stride_h;
   const int64_t heads = int64_t{p->kv_heads} * p->seqs.batch;
   int64_t most_k = p->mass_width;
   if (a.accumulate && p->max_seqlen_k > 0 && p->max_seqlen_k < most_k) most_k = p->max_seqlen_k;
@@ -2231,12 +2226,8 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* p, void* stream) {
     if (e != cudaSuccess) return cuda_fail(e, "attention_mass launch");
     return IFA4_OK;
   }
-  CUtensorMap tq, tk;
-  // without rows nothing is loaded, but the map has to be one
-  if ((rc = encode_rows_heads_dims(&tq, p->total_q > 0 ? p->q : p->k_cache,
-                                   p->total_q > 0 ? p->total_q : 1, p->n_heads,
-                                   p->total_q > 0 ? p->q_stride_t : 128 * int64_t{p->n_heads},
-                                   p->total_q > 0 ? p->q_stride_h : 128,
+  CUtensorMap tq, tk;  // there are rows: none are few
+  if ((rc = encode_rows_heads_dims(&tq, p->q, p->total_q, p->n_heads, p->q_stride_t, p->q_stride_h,
                                    static_cast<uint32_t>(a.tokens_per_tile), "q",
                                    static_cast<uint32_t>(group))))
     return rc;

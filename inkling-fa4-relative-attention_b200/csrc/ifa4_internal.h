@@ -368,13 +368,12 @@ cudaError_t launch_decode_pages_sm100(const DecodePagesKernelArgs& args, const C
 struct AttentionMassKernelArgs {
   PagedSeqs s;
   const uint16_t* q;
-  const uint16_t* k_cache;
   const uint16_t* rel;
   const float* lse;
   float* mass;
-  long long q_st, q_sh, k_sp, k_st, k_sh, rel_st, rel_sh, lse_sh, lse_st, mass_sb, mass_sh;
-  long long total_q;
-  int n_heads, kv_heads, group, rel_extent, window_left;
+  long long q_st, q_sh, rel_st, rel_sh, lse_sh, lse_st, mass_sb, mass_sh;
+  long long total_q;         // index checks only
+  int kv_heads, group, rel_extent, window_left;
   int mass_width, accumulate, box_shift;
   int tokens_per_tile;       // query tokens of a tile of rows
   float scale_log2;

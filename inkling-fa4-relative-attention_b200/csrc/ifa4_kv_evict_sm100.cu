@@ -873,7 +873,10 @@ namespace evict {
 // What stays
 // ---------------------------------------------------------------------------------------
 // A block per sequence and KV head: the border of the masses (see select_largest), then the places
-// that stay, in order, with their masses.
+// that stay, in order, with their masses.  Rows of up to 4, 12 and 32 masses a thread are held in
+// registers (16 x 8 heads, 64 stay, with the move: 4096 masses 13.0 us with 4 a thread, 15.6 with 12, 23.7
+// with 32; 6000 to 12288 15.9 to 17.0 with 12, 17.3 to 18.1 with 16, 23.8 to 24.4 with 32; 14000 to 16384
+// 18.3 to 18.9 with 16, 24.5 to 25.1 with 32, which the rows there take; 32768 27.8).
 constexpr int kSelectThreads = 1024;
 
 __global__ void __launch_bounds__(kSelectThreads)
@@ -955,7 +958,7 @@ __global__ void __launch_bounds__(kSelectThreads)
 // said so too, and writes.  Key `place` comes from kept[place] >= place, so only earlier stretches read
 // there.  Stretches are handed out in order by a counter: a block waits for blocks that are running and
 // wait for nothing themselves before they say so.  Bound by HBM: 512 bytes read and written a key.
-// (16 sequences of 32k keys to 8192, 8 KV heads: 187 us, 5.5 TB/s, of a call of 217 with the choice's 35;
+// (16 sequences of 32k keys to 8192, 8 KV heads: 187 us, 5.5 TB/s, of a call of 220 with the choice's 35;
 // a block per head that went through its keys with barriers took the call to 364.)
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 64;

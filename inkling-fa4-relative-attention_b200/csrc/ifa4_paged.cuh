@@ -16,7 +16,7 @@ __device__ __forceinline__ int first_key(int p, int window_left) {
 
 // Sequence b of row t (cu_q[b] <= t < cu_q[b + 1]), its key count and the row's position; -1 for a row
 // of none.  Whole warp; one load for a decode batch (one row a sequence), otherwise 32 places are looked
-// at a time (one step for up to 33 sequences, two for 1057) and a load for the lengths follows.
+// at a time (one step for up to 32 sequences, two for 1024) and a load for the lengths follows.
 __device__ __forceinline__ int find_sequence(const PagedSeqs& s, long long t, int& n_k, int& pos) {
   const int lane = threadIdx.x & 31;
   const int guess = t < s.batch ? static_cast<int>(t) : s.batch - 1;
