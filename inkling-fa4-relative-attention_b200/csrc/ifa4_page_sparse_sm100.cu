@@ -464,8 +464,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 512 ? 3 : kThreads == 25
 // units (min(page_size, 64) rows) by TMA into a ring; warps 0 to 3 take 16 keys of every tile, which
 // always lie in one page (page_size >= 16), so a warp reads one list entry per tile.  Units and slices
 // without a visible key are neither loaded nor computed.  Bound by HBM: 512 bytes a key and KV head
-// (64 rows of 256 pages of 16 keys, 8 KV heads: 184 us of the kernel back to back, 190 to 194 a call on
-// changing inputs, 5.6 TB/s of the listed keys).
+// (64 rows of 256 pages of 16 keys, 8 KV heads: 180 to 184 us captured, 188 to 194 a call, 5.7 TB/s of the
+// listed keys).
 constexpr int kTileKeys = 64;
 constexpr int kStages = 3;
 constexpr int kConsumerWarps = 4;

@@ -145,7 +145,7 @@ def inkling_kv_select_pages(scores, num_selected, *, out=None):
     """``[total_q, kv_heads, num_selected]`` int32: the places of the ``num_selected`` largest of every
     row of ``scores [total_q, kv_heads, max_pages]`` fp32, ascending.  Of equal scores at the border
     the lowest places are taken, NaN ranks above everything, -inf is never taken; a row with fewer
-    choices ends in -1."""
+    choices ends in -1.  ``out`` is other memory than ``scores``."""
     if out is None and _ops.USE_TORCH_OPS:
         outs = _lib.plain_call("select_pages", scores, num_selected)
         if outs is not None:
@@ -203,7 +203,8 @@ def inkling_fa4_rel_attention_decode_pages(q, k, v, rel_logits, cu_seqlens_q, cu
     is NaN.  Rows of no sequence are zeros (lse -inf) in new tensors and stay as they are in ``out`` /
     ``lse`` where ``out`` is given.  ``num_splits``: CTAs that share a query's pages (0:
     automatic); ``workspace``: a reusable uint8 CUDA tensor (allocated per call when absent or too
-    small); calls that may run at the same time need one each."""
+    small); calls that may run at the same time need one each.  Logits, weights and sums are held in 32
+    bits, the weights to 16 in the product with ``v``; the output's is the only other rounding."""
     if (out is None and lse is None and not return_lse and n_heads is None and kv_heads is None
             and head_dim == _ops.HEAD_DIM and _ops.USE_TORCH_OPS):
         outs = _lib.plain_call("decode_pages", q, k, v, rel_logits, cu_seqlens_q, cu_seqlens_k, pages,
