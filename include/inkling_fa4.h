@@ -680,10 +680,10 @@ int ifa4_attention_mass_launch(const IFA4AttentionMassParams* params, void* stre
  * what is kept with zeros behind, cu_out the offsets of the new lengths.  Shorter sequences keep
  * everything.  A kept key without a page is zeros at its new place.  No page that keys move into or
  * out of may be held by another sequence, or twice by its own.  k_cache and v_cache have no element in
- * common (two tensors, or slices of one with the same strides); mass_out, kept and cu_out are other
- * memory than all the rest, so the lengths are not updated in place.  seqs.cu_seqlens_q is not used;
- * the workspace (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by calls that
- * may run at the same time. */
+ * common (two tensors, or slices of one: with the same strides, or in turn); mass_out, kept and cu_out
+ * are other memory than all the rest, so the lengths are not updated in place.  seqs.cu_seqlens_q is
+ * not used; the workspace (ifa4_kv_evict_workspace_size bytes, 16-byte aligned) must not be shared by
+ * calls that may run at the same time. */
 typedef struct IFA4KvEvictParams {
   IFA4PagedSeqs seqs;
   void* k_cache;

@@ -1621,20 +1621,20 @@ struct Span {
 Span span_of(const char* name, const void* p, int64_t row_bytes,
              std::initializer_list<std::pair<int64_t, int64_t>> dims = {}) {
   const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  Span s{name, lo, lo};
-  int64_t bytes = row_bytes;
+  int64_t bytes = p != nullptr && row_bytes > 0 ? row_bytes : 0;
   for (const auto& d : dims) {
-    if (d.second <= 0) return s;  // nothing
-    bytes += d.first * (d.second - 1);
+    if (d.second <= 0) bytes = 0;  // nothing: meets no span
+    if (bytes > 0) bytes += d.first * (d.second - 1);
   }
-  if (p != nullptr && bytes > 0) s.hi += static_cast<uintptr_t>(bytes);
-  return s;
+  if (bytes <= 0) return {name, 0, 0};
+  return {name, lo, lo + static_cast<uintptr_t>(bytes)};
 }
 bool spans_meet(const Span& a, const Span& b) { return a.lo < b.hi && b.lo < a.hi; }
 
 // Whether two tensors of the same shape have an element in common: rows of `row` bytes at a + sum i_d
 // stride_d and b + sum j_d stride_d (bytes).  Exact where both have the same strides, none of whose rows
-// share an element (see rows_apart); with other strides, whether their spans meet.
+// share an element (see rows_apart).  With other strides, no where their spans do not meet or one
+// dimension has the same stride in both and their pieces within it lie in turn; yes otherwise.
 struct RowDim {
   int64_t stride_a, stride_b, count;
 };
@@ -1666,8 +1666,19 @@ bool tensors_meet(const void* a, const void* b, int64_t row, std::initializer_li
   }
   const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
   if (row <= 0 || apart >= end_a || -apart >= end_b) return false;
+  if (!same) {
+    for (int i = 0; i < n; ++i) {
+      const int64_t s = d[i].stride_a;
+      const int64_t piece_a = end_a - s * (d[i].count - 1);
+      const int64_t piece_b = end_b - d[i].stride_b * (d[i].count - 1);
+      if (d[i].stride_b != s || piece_a > s || piece_b > s) continue;
+      const int64_t at = (apart % s + s) % s;  // of b's piece behind a's
+      if (at >= piece_a && at + piece_b <= s) return false;
+    }
+    return true;
+  }
   std::sort(d, d + n, [](const RowDim& x, const RowDim& y) { return x.stride_a > y.stride_a; });
-  return !same || rows_meet(apart, row, d, n);
+  return rows_meet(apart, row, d, n);
 }
 
 int check_seqs(const char* what, const IFA4PagedSeqs* s, bool queries) {

@@ -114,8 +114,8 @@ def inkling_kv_evict(k_cache, v_cache, mass, block_table, cu_seqlens_k, budget, 
     take it from ``inkling_qk_norm_rope`` with the offsets before the eviction and are appended
     without one.  Bounds of pages (``inkling_kv_page_bounds``) have to be made anew.
 
-    ``k_cache`` and ``v_cache`` are two tensors, or slices of one (with the same strides, without an
-    element in common; others are refused).  No page that keys move into or out of may be held by
+    ``k_cache`` and ``v_cache`` are two tensors, or slices of one without an element in common (with the
+    same strides, or in turn; others are refused).  No page that keys move into or out of may be held by
     another sequence, or twice by its own (the first ``first`` keys stay where they are, so pages full
     of them may be shared).  A kept key whose table entry is no page becomes zeros at its new place, and
     nothing is written to a place without a page."""

@@ -27,6 +27,8 @@ def _evict(k, v, kept=1 << 20, cu_out=1 << 21, mass=1 << 22, mass_out=1 << 23, c
     p.kept, p.cu_out, p.mass, p.mass_out = kept, cu_out, mass, mass_out
     p.mass_stride_b = p.mass_out_stride_b = 64 * k.shape[2]
     p.mass_stride_h = p.mass_out_stride_h = 64
+    if not k.shape[0]:
+        p.k_cache = p.v_cache = 1 << 20  # no pages: nothing lies there
     for n, x in strides.items():
         setattr(p, n, x)
     return p
@@ -107,6 +109,32 @@ def test_caches_of_other_strides():
     assert _says(_evict(k, pool.as_strided((2, 16, 2, 128), other, 8192))) is None
 
 
+def test_caches_of_other_strides_in_turn():
+    """Keys [token, head] and values [head, token] of a page, page after page."""
+    pool = torch.zeros(3, 2, 16 * 2 * 128, dtype=torch.bfloat16)
+    k = pool[:, 0].view(3, 16, 2, 128)
+    v = pool[:, 1].view(3, 2, 16, 128).transpose(1, 2)
+    assert _says(_evict(k, v)) is None and _says(_evict(v, k)) is None
+    shifted = v.as_strided(v.shape, v.stride(), v.storage_offset() - 8)
+    assert "v_cache" in _says(_evict(k, shifted)) and "v_cache" in _says(_evict(shifted, k))
+
+
+def test_never_accepts_other_strides_that_share_an_element():
+    rng = random.Random(4)
+    pool = torch.zeros(60000, dtype=torch.bfloat16)
+    seen = {True: 0, False: 0}
+    for _ in range(800):
+        shape = (rng.randint(1, 3), 16, rng.randint(1, 3), 128)
+        page, views = 2 * 16 * shape[2] * 128 + 8 * rng.choice([0, 16]), []
+        for _ in range(2):
+            inner = rng.choice([(shape[2] * 128, 128), (128, 16 * 128), (shape[2] * 128 + 8, 128)])
+            views.append(pool.as_strided(shape, (page, *inner, 1), 8 * rng.randint(0, 3000)))
+        refused = _says(_evict(*views)) is not None
+        seen[refused] += 1
+        assert refused or not _elements(views[0]) & _elements(views[1])
+    assert min(seen.values()) > 50
+
+
 @pytest.mark.parametrize("what,with_,kw", [
     ("cu_out", "cu_seqlens_k", dict(cu_out=1 << 24)), ("cu_out", "cu_seqlens_k", dict(cu_out=(1 << 24) + 8)),
     ("cu_out", "cu_seqlens_k", dict(cu_out=(1 << 24) - 8)), ("cu_out", "block_table", dict(cu_out=1 << 25)),
@@ -118,6 +146,11 @@ def test_caches_of_other_strides():
 def test_outputs_on_top_of_something(what, with_, kw):
     text = _says(_evict(*_caches("two tensors"), **kw))
     assert text is not None and what in text and with_ in text
+
+
+def test_caches_without_pages():
+    k = torch.empty(1, 16, 2, 128, dtype=torch.bfloat16)[:0]
+    assert _says(_evict(k, k)) is None
 
 
 def test_outputs_next_to_something():
